@@ -46,6 +46,13 @@ _SIGNATURES = {
     "ferris_gemm_skinny": [_VP, _I, _VP, _VP, _F, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
     "ferris_gemm_skinny_takes": [_I, _I, _I, _I, _I],
     "ferris_embed_gather": [_VP, _I, _VP, _VP, _I, _I, _I, _VP, _VP],
+    "ferris_packed_cache_write": [_VP, _VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP],
+    "ferris_packed_cache_read": [_VP, _VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP],
+    "ferris_packed_cache_evict": [_VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _I, _VP, _I, _VP, _VP, _VP, _LL, _I, _I,
+                                  _VP, _VP, _LL, _I, _I, _I, _I, _I, _VP],
+    "ferris_packed_attention_splits": [_I, _I, _I, _I, _I],
+    "ferris_packed_attention": [_VP, _I, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _VP,
+                                _VP, _I, _VP, _VP, _LL, _I, _I, _I, _VP],
 }
 _declared = False
 
@@ -2353,3 +2360,211 @@ def sample(logits: torch.Tensor, out_token: torch.Tensor, out_prob: Optional[tor
                              _ptr(slots), _ptr(rng_states), _ptr(out_token), _ptr(out_prob), _stream()),
         "sample",
     )
+
+
+# ------------------------------------------------------------------------------------------
+# the paged cache in 4 bits
+# ------------------------------------------------------------------------------------------
+PACKED_GROUP = 32  # neighbours of a head that share a scale
+
+
+class PackedPages:
+    """Keys and values of a paged cache in 4 bits: every ``PACKED_GROUP`` neighbours of a head stand as
+    scale * code + least, codes 0..15 (``csrc/packed_cache.cuh`` says in which order).
+
+    ``k_codes``, ``v_codes`` uint8 [pages, kv heads, page size, head size / 2]; ``k_scales``, ``v_scales`` bf16
+    [pages, kv heads, page size, head size / 32, 2], (scale, least) of each group.  A row takes 5 bits an element, scales
+    included, against 16 of a cache in bf16."""
+
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "pages", "kv_heads", "page_size", "head_dim", "_args")
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales):
+        for t, what, dtype in ((k_codes, "packed key codes", torch.uint8), (k_scales, "packed key scales", torch.bfloat16),
+                               (v_codes, "packed value codes", torch.uint8), (v_scales, "packed value scales", torch.bfloat16)):
+            _need(t, what, dtype)
+        if k_codes.dim() != 4:
+            raise KernelError(f"packed codes are [pages, kv heads, page size, head size / 2], found {tuple(k_codes.shape)}")
+        self.pages, self.kv_heads, self.page_size, half = k_codes.shape
+        self.head_dim = 2 * half
+        if self.head_dim % PACKED_GROUP or not 0 < self.head_dim <= 256 or 0 in k_codes.shape:
+            raise KernelError(f"packed heads have a multiple of {PACKED_GROUP} elements, at most 256: codes {tuple(k_codes.shape)}")
+        scales = (*k_codes.shape[:3], self.head_dim // PACKED_GROUP, 2)
+        if v_codes.shape != k_codes.shape or k_scales.shape != scales or v_scales.shape != scales:
+            raise KernelError(f"packed cache: codes {tuple(k_codes.shape)} and {tuple(v_codes.shape)}, scales "
+                              f"{tuple(k_scales.shape)} and {tuple(v_scales.shape)}; scales of {scales} are needed")
+        if any(t.device != k_codes.device for t in (k_scales, v_codes, v_scales)):
+            raise KernelError("packed cache: its four tensors must be on one device")
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self._args = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device) -> "PackedPages":
+        """A cache of zeroed rows."""
+        if head_dim % PACKED_GROUP:
+            raise KernelError(f"packed heads have a multiple of {PACKED_GROUP} elements, not {head_dim}")
+        codes, scales = (pages, kv_heads, page_size, head_dim // 2), (pages, kv_heads, page_size, head_dim // PACKED_GROUP, 2)
+        return cls(*(torch.zeros(shape, dtype=dtype, device=device)
+                     for shape, dtype in ((codes, torch.uint8), (scales, torch.bfloat16)) * 2))
+
+    @staticmethod
+    def bytes_per_token(kv_heads: int, head_dim: int) -> int:
+        """Bytes that a token's keys and values take, scales included."""
+        return 2 * kv_heads * (head_dim // 2 + 4 * (head_dim // PACKED_GROUP))
+
+
+def _packed_rows(k, v, slot_mapping, pages: PackedPages, what: str):
+    """Checks rows of keys and values that go with ``pages``; their strides."""
+    T, n, ldk = _rows(k, f"{what}: keys")
+    T2, n2, ldv = _rows(v, f"{what}: values")
+    _need(slot_mapping, f"{what}: slot mapping", torch.int32)
+    width = pages.kv_heads * pages.head_dim
+    if T != T2 or n != width or n2 != width or k.dtype != v.dtype or slot_mapping.numel() != T:
+        raise KernelError(f"{what}: keys {tuple(k.shape)} {k.dtype}, values {tuple(v.shape)} {v.dtype}, {slot_mapping.numel()} slots for "
+                          f"{pages.kv_heads} heads of {pages.head_dim}")
+    if any(t.device != pages.k_codes.device for t in (k, v, slot_mapping)):
+        raise KernelError(f"{what}: keys, values, slots and cache must be on one device")
+    return T, ldk, ldv
+
+
+def packed_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, pages: PackedPages):
+    """Keys and values [T, kv heads x head size] (bf16 or fp32, rows contiguous: columns of a fused projection are fine) into
+    the rows ``slot_mapping`` (int32 [T], page * page_size + offset; below 0: the token is left out) of the packed cache.  Per
+    group of 32: least = its minimum rounded down to bf16, scale = bf16((maximum - least) / 15), code = (x - least) / scale
+    rounded to even; a group with NaN or infinity stands as NaN.  Two tokens with one slot leave one of them."""
+    T, ldk, ldv = _packed_rows(k, v, slot_mapping, pages, "packed cache write")
+    if T == 0:
+        return
+    _check(_lib().ferris_packed_cache_write(k.data_ptr(), v.data_ptr(), _dt(k, "keys"), ldk, ldv, slot_mapping.data_ptr(), *pages._args,
+                                            pages.pages, pages.kv_heads, pages.page_size, pages.head_dim, T, _stream()),
+           "packed cache write")
+
+
+def packed_cache_read(pages: PackedPages, slot_mapping: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+    """k[t], v[t] [kv heads x head size] = the values that row ``slot_mapping[t]`` of the packed cache stands for, rounded once
+    to their type (zeros where the slot is below 0)."""
+    T, ldk, ldv = _packed_rows(k, v, slot_mapping, pages, "packed cache read")
+    if T == 0:
+        return
+    _check(_lib().ferris_packed_cache_read(k.data_ptr(), v.data_ptr(), _dt(k, "keys"), ldk, ldv, slot_mapping.data_ptr(), *pages._args,
+                                           pages.pages, pages.kv_heads, pages.page_size, pages.head_dim, T, _stream()),
+           "packed cache read")
+
+
+def _weight_rows(weights, kv_heads: int, what: str) -> tuple:
+    """(slots, rows, slot stride, head stride) of weights fp32 [slots, kv heads, rows]."""
+    _need(weights, what, torch.float32, contiguous=False)
+    if weights.dim() != 3 or weights.shape[1] != kv_heads or (weights.shape[2] > 1 and weights.stride(2) != 1):
+        raise KernelError(f"{what} must be [slots, {kv_heads}, rows] with contiguous rows, found {tuple(weights.shape)}")
+    return weights.shape[0], weights.shape[2], weights.stride(0), weights.stride(1)
+
+
+def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, block_tables: torch.Tensor, seq_q_start: torch.Tensor,
+                     seq_start_row: torch.Tensor, max_q_len: int, max_kv_len: int, num_heads: int, scale: float, window: int = 0,
+                     weights: Optional[torch.Tensor] = None, seq_slot: Optional[torch.Tensor] = None, add_weights: bool = True,
+                     workspace=None):
+    """Attention of a step's queries over the packed cache, in which their own keys and values already are.
+
+    ``q`` [T, >= num_heads x head size] (bf16 or fp32; its first columns, so the rows of a fused projection will do), ``out``
+    [T, num_heads x head size] of the same type; request s brings the rows ``seq_q_start[s]`` .. ``seq_q_start[s + 1] - 1`` (int32
+    [S + 1]; they cover all of q) and held ``seq_start_row[s]`` rows (int32 [S]) of the cache before them; its query i sees rows
+    0 .. seq_start_row[s] + i, with ``window`` > 0 the last so many of them, as far as ``block_tables`` (int32 [S, blocks]) names
+    pages for them.  A query that sees nothing gives zeros.  ``max_q_len``, ``max_kv_len``: the most queries and rows (those of the
+    step included) of any request.
+
+    ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` for request s, row s without it): every cached row's weight
+    in the softmax, summed over the request's queries and the query heads of the kv head, is added to it; the rows that
+    came with this step (and with ``add_weights`` False all of them) are set instead."""
+    T, cols, ldq = _rows(q, "packed attention queries")
+    T2, width, ldo = _rows(out, "packed attention output")
+    _need(block_tables, "block tables", torch.int32)
+    _need(seq_q_start, "first query rows", torch.int32)
+    _need(seq_start_row, "rows held before the step", torch.int32)
+    S, D = seq_start_row.numel(), pages.head_dim
+    if num_heads <= 0 or num_heads % pages.kv_heads:
+        raise KernelError(f"packed attention: {num_heads} heads cannot share {pages.kv_heads} kv heads")
+    if T != T2 or cols < num_heads * D or width != num_heads * D or out.dtype != q.dtype:
+        raise KernelError(f"packed attention: q {tuple(q.shape)} {q.dtype}, out {tuple(out.shape)} {out.dtype} for {num_heads} heads of {D}")
+    if block_tables.dim() != 2 or block_tables.shape[0] != S or seq_q_start.numel() != S + 1:
+        raise KernelError(f"packed attention: tables {tuple(block_tables.shape)}, {seq_q_start.numel()} first rows for {S} requests")
+    if max_q_len < 0 or max_kv_len < 0 or window < 0:
+        raise KernelError(f"packed attention: at most {max_q_len} queries, {max_kv_len} rows, window {window}")
+    if any(t.device != pages.k_codes.device for t in (q, out, block_tables, seq_q_start, seq_start_row)):
+        raise KernelError("packed attention: all tensors must be on the cache's device")
+    dt = _dt(q, "packed attention queries")
+    w = (None, None, 0, 0, 0)
+    if weights is not None:
+        slots, rows, slot_stride, head_stride = _weight_rows(weights, pages.kv_heads, "packed attention weights")
+        if seq_slot is not None:
+            _need(seq_slot, "slots of the weights", torch.int32)
+        if (seq_slot.numel() != S if seq_slot is not None else slots < S) or rows < max_kv_len or weights.device != q.device:
+            raise KernelError(f"packed attention: weights {tuple(weights.shape)} for {S} requests of at most {max_kv_len} rows")
+        w = (weights.data_ptr(), None if seq_slot is None else seq_slot.data_ptr(), slot_stride, head_stride, rows)
+    if T == 0 or S == 0 or max_q_len == 0:
+        return
+    if block_tables.shape[1] == 0:
+        out.zero_()
+        return
+    lib = _lib()
+    splits = lib.ferris_packed_attention_splits(S, pages.kv_heads, num_heads // pages.kv_heads, max_q_len,
+                                                min(max_kv_len, window + max_q_len) if window else max_kv_len)
+    if workspace is None and (splits > 1 or weights is not None):
+        raise KernelError("packed attention: a workspace is needed")
+    parts = workspace.get("packed_attention_parts", (splits * T * num_heads * (D + 2),), torch.float32).data_ptr() if splits > 1 else None
+    lse = workspace.get("packed_attention_lse", (T * num_heads,), torch.float32).data_ptr() if weights is not None else None
+    _check(lib.ferris_packed_attention(q.data_ptr(), ldq, out.data_ptr(), ldo, dt, *pages._args, pages.pages, pages.kv_heads, pages.page_size, D,
+                                       block_tables.data_ptr(), block_tables.shape[1], seq_q_start.data_ptr(), seq_start_row.data_ptr(), S, T,
+                                       num_heads, max_q_len, max_kv_len, window, scale, lse, parts, splits, *w, 1 if add_weights else 0,
+                                       _stream()),
+           "packed attention", 1 + (splits > 1) + (weights is not None))
+
+
+def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows: torch.Tensor, weights: torch.Tensor,
+                       kept_pages: PackedPages, kept_tables: torch.Tensor, kept_rows: torch.Tensor, budget: int, keep_first: int = 0,
+                       keep_last: int = 0, seq_slot: Optional[torch.Tensor] = None, kept_weights: Optional[torch.Tensor] = None,
+                       workspace=None):
+    """Cut every request down to ``budget`` rows of the packed cache, each kv head to its own.
+
+    Of the ``seq_rows[s]`` rows (int32 [S]) of request s there stay its first ``keep_first``, its last ``keep_last`` and, of the
+    others, those of the greatest ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` or s; the lower row first among
+    equals, NaN before every number).  They move, in their order, into rows 0, 1, ... of the pages that ``kept_tables`` (int32
+    [S, blocks]) names in ``kept_pages`` (the same cache will do; none of the pages that are read).  The old pages keep what they
+    held, so other requests may share them.  Afterwards the request holds min(seq_rows[s], budget) rows.
+    ``kept_rows`` (int32 [S, kv heads, budget]) gets their numbers, -1 behind them; ``kept_weights`` (fp32 [slots, kv heads, >=
+    budget], not the memory of ``weights``) their weights.  ``workspace`` is for scratch that large requests need."""
+    for t, what in ((block_tables, "block tables"), (seq_rows, "rows of the requests"), (kept_tables, "block tables of the kept rows"),
+                    (kept_rows, "numbers of the kept rows")):
+        _need(t, what, torch.int32)
+    S, hkv = seq_rows.numel(), pages.kv_heads
+    if kept_pages.kv_heads != hkv or kept_pages.head_dim != pages.head_dim:
+        raise KernelError(f"eviction: from {hkv} heads of {pages.head_dim} into {kept_pages.kv_heads} of {kept_pages.head_dim}")
+    if budget <= 0 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
+        raise KernelError(f"eviction: {keep_first} first and {keep_last} last rows of a budget of {budget}")
+    if block_tables.dim() != 2 or kept_tables.dim() != 2 or block_tables.shape[0] != S or kept_tables.shape[0] != S:
+        raise KernelError(f"eviction: tables {tuple(block_tables.shape)} and {tuple(kept_tables.shape)} for {S} requests")
+    if tuple(kept_rows.shape) != (S, hkv, budget):
+        raise KernelError(f"eviction: numbers of kept rows are [{S}, {hkv}, {budget}], found {tuple(kept_rows.shape)}")
+    slots, rows, slot_stride, head_stride = _weight_rows(weights, hkv, "eviction: weights")
+    if seq_slot is not None:
+        _need(seq_slot, "slots of the weights", torch.int32)
+    if seq_slot.numel() != S if seq_slot is not None else slots < S:
+        raise KernelError(f"eviction: weights {tuple(weights.shape)} for {S} requests")
+    kept = (None, 0, 0)
+    if kept_weights is not None:
+        kslots, krows, kslot_stride, khead_stride = _weight_rows(kept_weights, hkv, "eviction: kept weights")
+        if krows < budget or kslots < (slots if seq_slot is not None else S):
+            raise KernelError(f"eviction: kept weights {tuple(kept_weights.shape)} for {budget} rows of {S} requests")
+        if kept_weights.data_ptr() == weights.data_ptr():
+            raise KernelError("eviction: kept weights need memory of their own")
+        kept = (kept_weights.data_ptr(), kslot_stride, khead_stride)
+    tensors = [block_tables, seq_rows, weights, kept_pages.k_codes, kept_tables, kept_rows, seq_slot, kept_weights]
+    if any(t is not None and t.device != pages.k_codes.device for t in tensors):
+        raise KernelError("eviction: all tensors must be on the cache's device")
+    if S == 0 or rows == 0 or block_tables.shape[1] == 0 or kept_tables.shape[1] == 0:
+        kept_rows.fill_(-1)
+        return
+    _check(_lib().ferris_packed_cache_evict(*pages._args, pages.pages, pages.page_size, *kept_pages._args, kept_pages.pages,
+                                            kept_pages.page_size, hkv, pages.head_dim, block_tables.data_ptr(), block_tables.shape[1],
+                                            kept_tables.data_ptr(), kept_tables.shape[1], seq_rows.data_ptr(),
+                                            None if seq_slot is None else seq_slot.data_ptr(), weights.data_ptr(), slot_stride, head_stride,
+                                            rows, kept_rows.data_ptr(), *kept, S, budget, keep_first, keep_last, _stream()),
+           "eviction", 2)

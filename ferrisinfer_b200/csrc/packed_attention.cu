@@ -1,19 +1,29 @@
 // Attention over the paged cache in 4 bits (its bytes: packed_cache.cuh), on mma.sync, for every geometry.
 //
 // A query row r of a request and kv head is (query i = r / G, head r % G of the G heads that share the kv head); it sees
-// the cached rows max(0, p - window + 1) .. p with p = start + i that have a page.  Eight rows are the columns of the
-// MMAs, sixteen cached rows their rows:
+// the cached rows max(0, p - window + 1) .. p with p = start + i that have a page.  Query rows are the columns of the
+// MMAs (eight to a tile), sixteen cached rows their rows:
 //   S^T = K Q^T   per group j of 32 elements:  s[key][q] += scale_j[key] (codes_j[key] . q_j) + least_j[key] sum(q_j)
-//   O^T = V^T P^T per group j:                 o[elem][q] += codes_j[elem][key] (p[key][q] scale_j[key]) + least_j[key] p[key][q]
-// Codes are whole numbers of four bits and least has eight bits, both exact as bf16, so the only roundings before the
-// 32-bit sums are those of the other operand: the queries (exact for bf16 rows, three bf16 parts for 32-bit rows) and
-// the weights p and p scale (one bf16 part for bf16 rows, three for 32-bit ones).  Neither keys nor values are ever
-// formed in fewer than 32 bits.
+//   O^T = V^T P^T per group j:                 o[elem][q] += codes_j[elem][key] (p[key][q] scale_j[key]), and least_j[key] p[key][q] in 32 bits
+// so that keys and values are never formed.  A word of eight codes becomes four operands of fp16 pairs with an AND / OR (1024 + code
+// or, from the upper four bits of a byte, 1024 + 16 code) and a subtraction each; values subtract 8 more and add 8 scale to their
+// least, so that what the sums hold is of the size of the result (unsigned codes add up to something that least nearly cancels:
+// over 32,768 rows the accumulators' rounding alone came to 0.0015 of the output).  What meets the codes is scaled by powers of two into the
+// range of fp16: a query row by its greatest element (bf16 rows then lose nothing that 32 bits would keep; 32-bit rows go in
+// two parts, 22 bits), p scale by the greatest scale that the warp has met, in eleven bits for bf16 rows, twice eleven for
+// 32-bit ones.  (In bf16's eight bits the outputs were off by 0.0025 to 0.005 of their norm, 0.0016 of which is their own rounding;
+// codes as fp16 numbers below the normal range need no subtraction, but the tensor cores align their products as if they
+// were large: 3e-5 of a 32-bit output.)
+#include <cuda_fp16.h>
+#include <float.h>
+
 #include "packed_cache.cuh"
 
 namespace {
 
-constexpr int KEYS = 16;  // cached rows of a tile
+constexpr int KEYS = 16;   // cached rows of an MMA
+constexpr int STAGE = 32;  // cached rows that a warp fetches at once
+constexpr int WARPS = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct PackedAttention {
@@ -48,78 +58,198 @@ __device__ __forceinline__ int page_of(const PackedAttention& p, const int* tabl
     return page;
 }
 
-// x in NP bf16 parts whose sum is x to 8 NP bits.
-template <int NP>
-__device__ __forceinline__ void split_parts(float x, float (&part)[NP]) {
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// The exponential unit alone: results below the normal range become nought.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 16 (or 8, or 4) bytes global -> shared without registers; `live` false: zeros, and nothing is read.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
+    const int n = live ? BYTES : 0;
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// The four pairs of a word of codes, each an operand register: places i and i + 4 (keys), or the two halves' i (values); the odd
+// ones times 16, all of them less `OFF`.
+template <int OFF>
+__device__ __forceinline__ void code_pairs(uint32_t word, uint32_t (&pair)[4]) {
+    const uint32_t up = word >> 8;
+    pair[0] = (word & 0x000f000fu) | 0x64006400u;
+    pair[1] = (word & 0x00f000f0u) | 0x64006400u;
+    pair[2] = (up & 0x000f000fu) | 0x64006400u;
+    pair[3] = (up & 0x00f000f0u) | 0x64006400u;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        part[i] = i + 1 < NP ? __bfloat162float(__float2bfloat16_rn(x)) : x;
-        x -= part[i];
+    for (int i = 0; i < 4; ++i) {
+        const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&pair[i]), __float2half2_rn(1024.0f + (i & 1 ? 16 * OFF : OFF)));
+        pair[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
 }
 
-// The eight codes of a key word as four pairs (elements i and i + 4), exact bf16 numbers: 128 + code, minus 128.
-__device__ __forceinline__ uint32_t code_pair(uint32_t word, int i) {
-    const uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(128.0f, 128.0f));
-    return *reinterpret_cast<const uint32_t*>(&r);
+// W words from shared memory, in the widest loads that their alignment allows.
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&r)[W], const unsigned char* p) {
+    if constexpr (W % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w;
+        }
+    } else if constexpr (W % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+            const uint2 v = reinterpret_cast<const uint2*>(p)[i];
+            r[2 * i] = v.x, r[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) r[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
 }
 
-// What a lane (g = lane / 4, c = lane % 4) holds of eight query rows as the B operand: row g of the tile.
+// What a warp fetches at once: STAGE cached rows.  Row strides keep the fragments' loads free of bank conflicts: of keys a
+// lane (g, c) takes 4 W bytes of row g at 4 W c, of values 2 W bytes of rows 2c, 2c + 1, 2c + 8, 2c + 9 at 2 W g.
+template <int W>
+struct Stage {
+    static constexpr int K_ROW = W == 8 ? 144 : 16 * W, V_ROW = 16 * W + 16, S_ROW = 4 * W;
+    static constexpr int V_AT = STAGE * K_ROW, KS_AT = V_AT + STAGE * V_ROW, VS_AT = KS_AT + STAGE * S_ROW, BYTES = VS_AT + STAGE * S_ROW;
+    static_assert(BYTES % 16 == 0 && KS_AT % 16 == 0, "copies of 16 bytes");
+
+    // Requests rows first .. first + 31 (those from `end` on, and those without a page, become zeros); which of them are there.
+    static __device__ __forceinline__ uint32_t request(const PackedAttention& p, const int* table, int head, int first, int end, unsigned char* to,
+                                                       int lane) {
+        const int row = first + lane;
+        if (first >= end) {  // (the whole warp) nothing to fetch, but a group to count
+            copy_commit();
+            return 0;
+        }
+        const int page = row < end ? page_of(p, table, row) : -1;
+        const size_t at = page >= 0 ? p.cache.row(page, head, row % p.cache.page_size) : 0;
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+        const uint32_t dst = smem_u32(to);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {  // W pieces of 16 bytes a row: neighbouring lanes take neighbouring pieces
+            const int piece = i * 32 + lane, r = piece / W, part = piece % W;
+            const size_t a = __shfl_sync(0xffffffffu, (unsigned long long)at, r);
+            const bool live = there >> r & 1;
+            copy_async<16>(dst + r * K_ROW + 16 * part, p.cache.k_codes + (a * W + part) * 16, live);
+            copy_async<16>(dst + V_AT + r * V_ROW + 16 * part, p.cache.v_codes + (a * W + part) * 16, live);
+        }
+        constexpr int N = W % 4 == 0 ? 16 : W % 2 == 0 ? 8 : 4;
+#pragma unroll
+        for (int i = 0; i < S_ROW / N; ++i) {
+            copy_async<N>(dst + KS_AT + lane * S_ROW + N * i, (const char*)(p.cache.k_scales + at * W) + N * i, page >= 0);
+            copy_async<N>(dst + VS_AT + lane * S_ROW + N * i, (const char*)(p.cache.v_scales + at * W) + N * i, page >= 0);
+        }
+        copy_commit();
+        return there;
+    }
+};
+
+// What a lane (g = lane / 4, c = lane % 4) holds of eight query rows as the B operand: row g of the tile, times `factor`, a
+// power of two that brings its greatest element to 2^13.
 template <typename T, int W, int NP>
 struct Queries {
-    uint32_t b[W][2][2][NP];   // group, half of the group's word, register
-    uint32_t sum[(W + 3) / 4][2];  // the group's sum in three parts (group 4 i + c)
+    uint32_t b[W][2][2][NP];       // group, half of the group's word, register
+    uint32_t sum[(W + 3) / 4][2];  // the sum of group 4 i + c in three bf16 parts
+    float factor;
 
     __device__ __forceinline__ void load(const T* row, int c, bool valid) {
+        float x[W][8], top = 0.0f;
 #pragma unroll
         for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[j][i] = valid ? to_float(row[32 * j + 8 * c + i]) : 0.0f;
+                top = fmaxf(top, fabsf(x[j][i]));
+            }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^(13 - e) for 2^e <= top < 2^(e + 1), at most 2^126
+        const int e = (int)(__float_as_uint(top) >> 23);
+        factor = top > 0.0f && e < 255 ? __uint_as_float((uint32_t)min(267 - e, 253) << 23) : 1.0f;
+        float mine[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            mine[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                mine[j] += x[j][i];
+                x[j][i] *= (i & 1) ? factor * 0.0625f : factor;  // odd places meet codes x 16
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int e = 32 * j + 8 * c + 2 * t + r;  // pairs (e, e + 4): the order of code_pair
-                    float lo[NP], hi[NP];
-                    split_parts<NP>(valid ? to_float(row[e]) : 0.0f, lo);
-                    split_parts<NP>(valid ? to_float(row[e + 4]) : 0.0f, hi);
+                    const int i = 2 * t + r;  // pairs (i, i + 4): the order of code_pairs
+                    float lo = x[j][i], hi = x[j][i + 4];
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) b[j][t][r][i] = pack_bf16(lo[i], hi[i]);
+                    for (int n = 0; n < NP; ++n) {
+                        const uint32_t v = pack_f16(lo, hi);
+                        b[j][t][r][n] = v;
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                        lo -= f.x, hi -= f.y;
+                    }
                 }
+        }
+        float own[(W + 3) / 4] = {};
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            mine[j] += __shfl_xor_sync(0xffffffffu, mine[j], 1);
+            mine[j] += __shfl_xor_sync(0xffffffffu, mine[j], 2);
+            if (j % 4 == c) own[j / 4] = mine[j];
+        }
 #pragma unroll
         for (int i = 0; i < (W + 3) / 4; ++i) {
-            float s = 0.0f, part[3];
-            if (valid && 4 * i + c < W)
-                for (int e = 0; e < 32; ++e) s += to_float(row[32 * (4 * i + c) + e]);
-            split_parts<3>(s, part);
-            sum[i][0] = pack_bf16(part[0], part[1]);
-            sum[i][1] = pack_bf16(part[2], 0.0f);
+            const float s = own[i] * factor;
+            const float s1 = __bfloat162float(__float2bfloat16_rn(s)), s2 = __bfloat162float(__float2bfloat16_rn(s - s1));
+            sum[i][0] = pack_bf16(s1, s2);
+            sum[i][1] = pack_bf16(s - s1 - s2, 0.0f);
         }
     }
 };
 
-// Codes and scales of the keys of a tile: this lane's rows g and g + 8.
+// Codes and scales of the keys of sixteen rows: this lane's rows g and g + 8.
 template <int W>
 struct Keys {
     uint32_t word[2][W], scale[2][W];
 
-    __device__ __forceinline__ void load(const PackedAttention& p, const int* table, int head, int first, int end, int g, int c) {
+    __device__ __forceinline__ void load(const unsigned char* stage, int first, int g, int c) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int row = first + g + 8 * u;
-            const int page = row < end ? page_of(p, table, row) : -1;
-            const size_t at = page >= 0 ? p.cache.row(page, head, row % p.cache.page_size) : 0;
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                word[u][j] = page >= 0 ? reinterpret_cast<const uint32_t*>(p.cache.k_codes)[at * (4 * W) + c * W + j] : 0u;
-                scale[u][j] = page >= 0 ? p.cache.k_scales[at * W + j] : 0u;
-            }
+            load_words<W>(word[u], stage + (first + g + 8 * u) * Stage<W>::K_ROW + 4 * W * c);
+            load_words<W>(scale[u], stage + Stage<W>::KS_AT + (first + g + 8 * u) * Stage<W>::S_ROW);
         }
     }
 
-    // s[0..3]: (key g, rows 2c and 2c + 1), (key g + 8, the same)
-    template <typename T, int NP>
-    __device__ __forceinline__ void scores(const Queries<T, W, NP>& q, int c, float (&s)[4]) const {
-        s[0] = s[1] = s[2] = s[3] = 0.0f;
+    // s[n][0..3]: (key g, rows 2c and 2c + 1 of tile n), (key g + 8, the same), times factor
+    template <typename T, int NP, int NT>
+    __device__ __forceinline__ void scores(const Queries<T, W, NP> (&q)[NT], int c, float (&s)[NT][4]) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
         for (int i = 0; i < (W + 3) / 4; ++i) {  // least times the sums of the queries' groups
             uint32_t l0 = 0, l1 = 0;
@@ -131,269 +261,358 @@ struct Keys {
                 }
             const uint32_t a0 = __byte_perm(l0, l0, 0x3232), a1 = __byte_perm(l1, l1, 0x3232);
             const uint32_t a[4] = {a0, a1, a0, a1};
-            mma_bf16_16816(s, a, q.sum[i][0], q.sum[i][1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16_16816(s[n], a, q[n].sum[i][0], q[n].sum[i][1]);
         }
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t a[4] = {code_pair(word[0][j], 2 * t), code_pair(word[1][j], 2 * t), code_pair(word[0][j], 2 * t + 1),
-                                       code_pair(word[1][j], 2 * t + 1)};
-#pragma unroll
-                for (int i = 0; i < NP; ++i) mma_bf16_16816(d, a, q.b[j][t][0][i], q.b[j][t][1][i]);
-            }
+            uint32_t a0[4], a1[4];
+            code_pairs<0>(word[0][j], a0);
+            code_pairs<0>(word[1][j], a1);
             const float s0 = packed_scale(scale[0][j]), s1 = packed_scale(scale[1][j]);
-            s[0] = fmaf(s0, d[0], s[0]);
-            s[1] = fmaf(s0, d[1], s[1]);
-            s[2] = fmaf(s1, d[2], s[2]);
-            s[3] = fmaf(s1, d[3], s[3]);
-        }
-    }
-};
-
-// What the eight rows of a tile see: for this lane's two columns 2c and 2c + 1 and for all of them.
-struct Rows {
-    int low[2], high[2];       // first row seen, one past the last
-    int least, most;           // over all rows of the tile: the range to go through
-    int all_low, all_high;     // rows that every row of the tile sees
-
-    __device__ __forceinline__ void set(const PackedAttention& p, int first, int count, int start, int limit, int lane) {
-        least = 0x7fffffff, most = 0, all_low = 0, all_high = 0x7fffffff;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            int lo = 0, hi = 0;
-            if (first + r < count) {
-                const int at = start + (first + r) / p.group;
-                hi = min(at + 1, limit);
-                lo = p.window > 0 ? max(0, at - p.window + 1) : 0;
-                if (hi > lo) {
-                    least = min(least, lo);
-                    most = max(most, hi);
+            for (int n = 0; n < NT; ++n) {
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t a[4] = {a0[2 * t], a1[2 * t], a0[2 * t + 1], a1[2 * t + 1]};
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) mma_f16_16816(d, a, q[n].b[j][t][0][i], q[n].b[j][t][1][i]);
                 }
-                all_low = max(all_low, lo);
-                all_high = min(all_high, hi);
+                s[n][0] = fmaf(s0, d[0], s[n][0]);
+                s[n][1] = fmaf(s0, d[1], s[n][1]);
+                s[n][2] = fmaf(s1, d[2], s[n][2]);
+                s[n][3] = fmaf(s1, d[3], s[n][3]);
             }
-            if (r == 2 * (lane & 3)) low[0] = lo, high[0] = hi;
-            if (r == 2 * (lane & 3) + 1) low[1] = lo, high[1] = hi;
         }
-        if (least > most) least = most;
     }
 };
 
-constexpr int WARPS = 8;
+// What the rows of NT tiles of eight see: for this lane's columns 2c and 2c + 1 of each and for all of them.
+template <int NT>
+struct Rows {
+    int low[NT][2], high[NT][2];  // first row seen, one past the last
+    int least, most;              // over all rows: the range to go through
+    int all_low, all_high;        // rows that every row of the tiles sees
 
-// Block (row tile, kv head, request x split): WARPS warps take the tiles of the block's range of cached rows in turn,
-// each with its own running maximum and sum, and are joined in shared memory in their order.
-template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32) packed_attention_rows_kernel(const PackedAttention p) {
-    constexpr int W = D / 32, NP = sizeof(T) == 4 ? 3 : 1;
-    extern __shared__ float joined[];  // [WARPS][8][D + 2]
+    static __device__ __forceinline__ void sees(const PackedAttention& p, int r, int start, int limit, int& lo, int& hi) {
+        const int at = start + r / p.group;
+        hi = min(at + 1, limit);
+        lo = p.window > 0 ? max(0, at - p.window + 1) : 0;
+    }
+
+    // (what rows see moves on with their number: the first and the last row of the tiles bound all of them)
+    __device__ __forceinline__ void set(const PackedAttention& p, int first, int count, int start, int limit, int c) {
+        const int last = min(first + 8 * NT, count) - 1;
+        int hi;
+        sees(p, first, start, limit, least, all_high);
+        sees(p, last, start, limit, all_low, most);
+        hi = max(most, 0);
+        most = hi;
+        least = min(least, most);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = first + 8 * n + 2 * c + u;
+                low[n][u] = 0, high[n][u] = 0;
+                if (r < count) sees(p, r, start, limit, low[n][u], high[n][u]);
+            }
+    }
+};
+
+template <int D, int NT>
+struct RowsPlan {
+    static constexpr int W = D / 32, STAGE_BYTES = Stage<W>::BYTES;
+    static constexpr int STAGES = D <= 64 ? 3 : 2;
+    static constexpr int RING = WARPS * STAGES * STAGE_BYTES, JOIN = WARPS * 8 * NT * (D + 2) * 4;
+    static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+};
+
+// Block (row tiles, kv head, request x split): the warps take the stages of the block's range of cached rows in turn, each
+// with rings of copies, a running maximum and a sum of its own, and are joined in shared memory in their order.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 2 : 1) packed_attention_rows_kernel(const PackedAttention p) {
+    using Plan = RowsPlan<D, NT>;
+    constexpr int W = D / 32, NP = sizeof(T) == 4 ? 2 : 1, STAGES = Plan::STAGES;
+    extern __shared__ __align__(16) unsigned char smem[];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const int head = blockIdx.y, seq = blockIdx.z / p.splits, split = blockIdx.z % p.splits;
-    const int t0 = max(p.q_start[seq], 0), count = (min(p.q_start[seq + 1], p.tokens) - t0) * p.group, first = blockIdx.x * 8;
+    const int t0 = max(p.q_start[seq], 0), count = (min(p.q_start[seq + 1], p.tokens) - t0) * p.group, first = blockIdx.x * 8 * NT;
     if (first >= count) return;
     const int* table = p.tables + (size_t)seq * p.width;
-    Rows rows;
-    rows.set(p, first, count, p.start_row[seq], p.width * p.cache.page_size, lane);
-    const int tiles = (rows.most - rows.least / KEYS * KEYS + KEYS - 1) / KEYS, per = (tiles + p.splits - 1) / p.splits;
-    const int base = rows.least / KEYS * KEYS + split * per * KEYS, end = min(rows.most, base + per * KEYS);
+    Rows<NT> rows;
+    rows.set(p, first, count, p.start_row[seq], p.width * p.cache.page_size, c);
+    const int floor = rows.least / STAGE * STAGE, stages = (rows.most - floor + STAGE - 1) / STAGE, per = (stages + p.splits - 1) / p.splits;
+    const int base = floor + split * per * STAGE, end = min(rows.most, base + per * STAGE);
 
-    Queries<T, W, NP> q;
-    {
-        const int r = first + g;
-        const T* row = (const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D;
-        q.load(row, c, r < count);
+    unsigned char* ring = smem + warp * STAGES * Plan::STAGE_BYTES;
+    uint32_t there[STAGES];
+    const int begin = base + warp * STAGE;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+        there[i] = Stage<W>::request(p, table, head, begin + i * WARPS * STAGE, end, ring + i * Plan::STAGE_BYTES, lane);
+
+    Queries<T, W, NP> q[NT];
+    float qs[NT][2];  // what makes a score of `scores` one to the base of 2
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = first + 8 * n + g;
+        q[n].load((const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D, c, r < count);
+        const float inv = p.scale / q[n].factor;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) qs[n][u] = __shfl_sync(0xffffffffu, inv, 4 * (2 * c + u));
     }
-    float o[W][2][4] = {}, low_o[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    uint32_t bad = 0;  // groups whose output is not finite: bit j of column 2c, bit j + 8 of column 2c + 1
+    float o[NT][W][2][4] = {}, low_o[NT][W][2] = {}, m[NT][2], l[NT][2] = {};
+    float v_top = 0.0f, v_fit = 1.0f;  // a power of two no scale of values met so far is above, and what brings such scales to 2^6
+    uint32_t bad[NT] = {};             // groups whose output is not finite: bit j of column 2c, bit j + 8 of column 2c + 1
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -FLT_MAX;  // (finite: differences of it are numbers)
 
-    for (int at = base + warp * KEYS; at < end; at += WARPS * KEYS) {
-        Keys<W> k;
-        k.load(p, table, head, at, end, g, c);
-        float s[4];
-        k.template scores<T, NP>(q, c, s);
-        const bool whole = at >= rows.all_low && at + KEYS <= rows.all_high;
-        bool seen[4];
+    int slot = 0;
+    for (int at = begin; at < end; at += WARPS * STAGE) {
+        {
+            const int ahead = slot == 0 ? STAGES - 1 : slot - 1;  // the place that the stage before this one has left
+            const uint32_t t = Stage<W>::request(p, table, head, at + (STAGES - 1) * WARPS * STAGE, end, ring + ahead * Plan::STAGE_BYTES, lane);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = at + g + 8 * (i >> 1);
-            seen[i] = whole || (row >= rows.low[i & 1] && row < rows.high[i & 1]);
-            s[i] *= p.scale;
+            for (int i = 0; i < STAGES; ++i)
+                if (i == ahead) there[i] = t;
         }
-        // rows without a page are seen by nobody
-        bool hole = false;
+        copy_wait<STAGES - 1>();
+        __syncwarp();
+        const unsigned char* stage = ring + slot * Plan::STAGE_BYTES;
+        uint32_t here = 0;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = at + g + 8 * u;
-            if (row < end && page_of(p, table, row) < 0) {
-                hole = true;
-                seen[2 * u] = seen[2 * u + 1] = false;
-            }
+        for (int i = 0; i < STAGES; ++i)
+            if (i == slot) here = there[i];
+
+        float s[2][NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Keys<W> k;
+            k.load(stage, KEYS * h, g, c);
+            k.scores(q, c, s[h]);
         }
-        const bool masked = __any_sync(0xffffffffu, hole) || !whole;
+        const bool whole = at >= rows.all_low && at + STAGE <= rows.all_high && here == 0xffffffffu;
+        uint32_t seen = 0xffffffffu;  // bit 4 n + 2 x + u of half h at 16 h
+        if (!whole) {
+            seen = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = seen[i] ? s[i] : -INFINITY;
-        float pr[4], rescale[2];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float top = fmaxf(s[u], s[u + 2]);
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float now = fmaxf(m[u], top), from = now == -INFINITY ? 0.0f : now;
-            rescale[u] = exp2f(m[u] - from);
-            m[u] = now;
-            pr[u] = seen[u] ? exp2f(s[u] - from) : 0.0f;
-            pr[u + 2] = seen[u + 2] ? exp2f(s[u + 2] - from) : 0.0f;
-            l[u] = fmaf(l[u], rescale[u], pr[u] + pr[u + 2]);
-        }
-        // values: this lane's rows (keys) 2c, 2c + 1, 2c + 8, 2c + 9 and, for the scales, g and g + 8
-        uint32_t vword[4][(W + 1) / 2], vleast[4], vs[2][W];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int row = at + 2 * c + (u & 1) + 8 * (u >> 1);
-            const int page = row < end ? page_of(p, table, row) : -1;
-            const size_t r = page >= 0 ? p.cache.row(page, head, row % p.cache.page_size) : 0;
-            const uint16_t* src = reinterpret_cast<const uint16_t*>(p.cache.v_codes) + r * (8 * W) + g * W;
-#pragma unroll
-            for (int j = 0; j < (W + 1) / 2; ++j) {
-                uint32_t w = 0;
-                if (page >= 0) {
-                    w = src[2 * j];
-                    if (2 * j + 1 < W) w |= (uint32_t)src[2 * j + 1] << 16;
-                }
-                vword[u][j] = w;
-            }
-            vleast[u] = page >= 0 && g < W ? p.cache.v_scales[r * W + g] : 0u;
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = at + g + 8 * u;
-            const int page = row < end ? page_of(p, table, row) : -1;
-            const size_t r = page >= 0 ? p.cache.row(page, head, row % p.cache.page_size) : 0;
-#pragma unroll
-            for (int j = 0; j < W; ++j) vs[u][j] = page >= 0 ? p.cache.v_scales[r * W + j] : 0u;
-        }
-        if (masked) {
-            // A weight of nought would still carry NaN from a row that the query does not see: groups that are not finite
-            // are taken out of the tile, and those outputs that do see them are marked.
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int j = 0; j < W; ++j)
-                    if (packed_not_finite(vs[u][j])) {
-                        vs[u][j] = 0;
-                        bad |= (seen[2 * u] ? 1u << j : 0u) | (seen[2 * u + 1] ? 1u << (j + 8) : 0u);
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = KEYS * h + g + 8 * (i >> 1);
+                        if ((here >> r & 1) && at + r >= rows.low[n][i & 1] && at + r < rows.high[n][i & 1]) seen |= 1u << (16 * h + 4 * n + i);
                     }
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (packed_not_finite(vleast[u])) vleast[u] = 0;
         }
+        // The maximum is left behind by up to 2^8: only a score above that makes the warp find a new one and scale what it has.
+        bool grew = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[h][n][i] *= qs[n][i & 1];
+                    if (!whole && !(seen >> (16 * h + 4 * n + i) & 1)) s[h][n][i] = -INFINITY;
+                    grew |= s[h][n][i] > m[n][i & 1] + 8.0f;
+                }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float top = fmaxf(fmaxf(s[0][n][u], s[0][n][u + 2]), fmaxf(s[1][n][u], s[1][n][u + 2]));
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const float now = fmaxf(m[n][u], top), f = exp2_fast(m[n][u] - now);
+                    m[n][u] = now;
+                    l[n][u] *= f;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        low_o[n][j][u] *= f;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            o[n][j][t][u] *= f;
+                            o[n][j][t][u + 2] *= f;
+                        }
+                    }
+                }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = exp2_fast(s[h][n][i] - m[n][i & 1]);
+                    s[h][n][i] = e;
+                    l[n][i & 1] += e;
+                }
+
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t vs[2][W];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) load_words<W>(vs[u], stage + Stage<W>::VS_AT + (KEYS * h + g + 8 * u) * Stage<W>::S_ROW);
+            if (!whole) {
+                // A weight of nought would still carry NaN from a row that the query does not see: groups that are not finite
+                // are taken out of the stage, and those outputs that do see them are marked.
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+                        if (packed_not_finite(vs[u][j])) {
+                            vs[u][j] = 0;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const uint32_t sees = seen >> (16 * h + 4 * n + 2 * u);
+                                bad[n] |= (sees & 1) << j | (sees >> 1 & 1) << (j + 8);
+                            }
+                        }
+            }
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) top = fmaxf(top, fmaxf(packed_scale(vs[0][j]), packed_scale(vs[1][j])));
+            if (__any_sync(0xffffffffu, top > v_top)) {
+                top = warp_max(top);  // the next power of two, between 2^-120 and 2^127
+                const uint32_t e = min(max((__float_as_uint(top) >> 23) + 1, 7u), 254u);
+                const float now = __uint_as_float(e << 23), f = v_top / now;
+                v_top = now;
+                v_fit = __uint_as_float((260u - e) << 23);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[n][j][t][i] *= f;
+            }
+            uint32_t word[4][(W + 1) / 2];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const unsigned char* src = stage + Stage<W>::V_AT + (KEYS * h + 2 * c + (u & 1) + 8 * (u >> 1)) * Stage<W>::V_ROW + 2 * W * g;
+                if constexpr (W % 2 == 0) {
+                    load_words<W / 2>(word[u], src);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        const uint32_t v = reinterpret_cast<const uint16_t*>(src)[j];
+                        word[u][j / 2] = j & 1 ? word[u][j / 2] | v << 16 : v;
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float s0 = packed_scale(vs[0][j]) * v_fit, s1 = packed_scale(vs[1][j]) * v_fit;
+                const float l0 = fmaf(8.0f, packed_scale(vs[0][j]), packed_least(vs[0][j])), l1 = fmaf(8.0f, packed_scale(vs[1][j]), packed_least(vs[1][j]));
+                const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
+                uint32_t a0[4], a1[4];
+                code_pairs<8>(__byte_perm(word[0][j / 2], word[1][j / 2], sel), a0);
+                code_pairs<8>(__byte_perm(word[2][j / 2], word[3][j / 2], sel), a1);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float(&pr)[4] = s[h][n];
+                    low_o[n][j][0] = fmaf(pr[0], l0, fmaf(pr[2], l1, low_o[n][j][0]));
+                    low_o[n][j][1] = fmaf(pr[1], l0, fmaf(pr[3], l1, low_o[n][j][1]));
+                    float w[4] = {pr[0] * s0, pr[1] * s0, pr[2] * s1, pr[3] * s1};
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        const uint32_t x0 = pack_f16(w[0], w[1]), x1 = pack_f16(w[2], w[3]);
+                        if (i + 1 < NP) {
+                            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&x0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&x1));
+                            w[0] -= f0.x, w[1] -= f0.y, w[2] -= f1.x, w[3] -= f1.y;
+                        }
+                        const uint32_t b0 = movmatrix_trans(x0), b1 = movmatrix_trans(x1);
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const uint32_t a[4] = {a0[2 * t], a0[2 * t + 1], a1[2 * t], a1[2 * t + 1]};
+                            mma_f16_16816(o[n][j][t], a, b0, b1);
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();  // the next request overwrites the stage that has just been read
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+    copy_wait<0>();
+    __syncthreads();  // the rings are read and written no more: the joined rows take their place
+
+    // over the eight lanes of a column: sums, groups that are not finite; then the warp's part in shared memory
+    float* joined = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+            bad[n] |= __shfl_xor_sync(0xffffffffu, bad[n], x);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                l[n][u] += __shfl_xor_sync(0xffffffffu, l[n][u], x);
+#pragma unroll
+                for (int j = 0; j < W; ++j) low_o[n][j][u] += __shfl_xor_sync(0xffffffffu, low_o[n][j][u], x);
+            }
+        }
+        float* mine = joined + (size_t)(warp * NT + n) * 8 * (D + 2);
 #pragma unroll
         for (int j = 0; j < W; ++j)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[j][t][i] *= rescale[i & 1];
-        low_o[0] *= rescale[0];
-        low_o[1] *= rescale[1];
-        {  // least times the weights: rows of the product are the groups
-            const uint32_t a[4] = {g < W ? __byte_perm(vleast[0], vleast[1], 0x7632) : 0u, 0u, g < W ? __byte_perm(vleast[2], vleast[3], 0x7632) : 0u, 0u};
-            float part[4][NP];
+                for (int i = 0; i < 4; ++i) {
+                    // rows g + 8 of the product met codes x 16; the weights were 2^6 / v_top times the true ones
+                    const float v = o[n][j][t][i] * (i >> 1 ? 0.0009765625f : 0.015625f) * v_top + low_o[n][j][i & 1];
+                    mine[(2 * c + (i & 1)) * (D + 2) + 32 * j + 4 * g + 2 * t + (i >> 1)] = bad[n] >> (j + 8 * (i & 1)) & 1 ? NAN : v;
+                }
+        if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) split_parts<NP>(pr[i], part[i]);
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-                mma_bf16_16816(low_o, a, movmatrix_trans(pack_bf16(part[0][i], part[1][i])), movmatrix_trans(pack_bf16(part[2][i], part[3][i])));
-        }
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const float s0 = packed_scale(vs[0][j]), s1 = packed_scale(vs[1][j]);
-            float part[4][NP];
-            split_parts<NP>(pr[0] * s0, part[0]);
-            split_parts<NP>(pr[1] * s0, part[1]);
-            split_parts<NP>(pr[2] * s1, part[2]);
-            split_parts<NP>(pr[3] * s1, part[3]);
-            const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
-            const uint32_t x0 = __byte_perm(vword[0][j / 2], vword[1][j / 2], sel), x1 = __byte_perm(vword[2][j / 2], vword[3][j / 2], sel);
-            uint32_t a[2][4];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                a[t][0] = code_pair(x0, 2 * t);
-                a[t][1] = code_pair(x0, 2 * t + 1);
-                a[t][2] = code_pair(x1, 2 * t);
-                a[t][3] = code_pair(x1, 2 * t + 1);
+            for (int u = 0; u < 2; ++u) {
+                mine[(2 * c + u) * (D + 2) + D] = m[n][u];
+                mine[(2 * c + u) * (D + 2) + D + 1] = l[n][u];
             }
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const uint32_t b0 = movmatrix_trans(pack_bf16(part[0][i], part[1][i])), b1 = movmatrix_trans(pack_bf16(part[2][i], part[3][i]));
-                mma_bf16_16816(o[j][0], a[0], b0, b1);
-                mma_bf16_16816(o[j][1], a[1], b0, b1);
-            }
-        }
-    }
-
-    // over the eight lanes of a column: the sum, the groups that are not finite; then the warp's part in shared memory
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-        l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
-        l[1] += __shfl_xor_sync(0xffffffffu, l[1], x);
-        bad |= __shfl_xor_sync(0xffffffffu, bad, x);
-    }
-    float* mine = joined + (size_t)warp * 8 * (D + 2);
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-        const float low0 = __shfl_sync(0xffffffffu, low_o[0], 4 * j + c), low1 = __shfl_sync(0xffffffffu, low_o[1], 4 * j + c);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool nan = bad >> (j + 8 * (i & 1)) & 1;
-                mine[(2 * c + (i & 1)) * (D + 2) + 32 * j + 4 * g + 2 * t + (i >> 1)] = nan ? NAN : o[j][t][i] + (i & 1 ? low1 : low0);
-            }
-    }
-    if (g == 0) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            mine[(2 * c + u) * (D + 2) + D] = m[u];
-            mine[(2 * c + u) * (D + 2) + D + 1] = l[u];
         }
     }
     __syncthreads();
-    const int r = first + warp;  // a warp joins one row
-    if (r >= count) return;
-    const int token = t0 + r / p.group, qh = head * p.group + r % p.group;
-    float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, joined[(w * 8 + warp) * (D + 2) + D]);
-    const float from = top == -INFINITY ? 0.0f : top;
-    float f[WARPS];
+    for (int n = 0; n < NT; ++n) {  // a warp joins one row of each tile
+        const int r = first + 8 * n + warp;
+        if (r >= count) break;
+        const int token = t0 + r / p.group, qh = head * p.group + r % p.group;
+        const float* row = joined + (size_t)(n * 8 + warp) * (D + 2);
+        constexpr int NEXT = NT * 8 * (D + 2);
+        float top = -FLT_MAX, sum = 0.0f, f[WARPS];
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        f[w] = exp2f(joined[(w * 8 + warp) * (D + 2) + D] - from);
-        sum += f[w] * joined[(w * 8 + warp) * (D + 2) + D + 1];
-    }
-    const bool partial = p.splits > 1;
-    float* part = partial ? p.parts + (((size_t)split * p.tokens + token) * p.heads + qh) * (D + 2) : nullptr;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, row[w * NEXT + D]);
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-        float acc = 0.0f;
+        for (int w = 0; w < WARPS; ++w) {
+            f[w] = exp2_fast(row[w * NEXT + D] - top);
+            sum += f[w] * row[w * NEXT + D + 1];
+        }
+        const bool partial = p.splits > 1;
+        float* part = partial ? p.parts + (((size_t)split * p.tokens + token) * p.heads + qh) * (D + 2) : nullptr;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) acc += f[w] * joined[(w * 8 + warp) * (D + 2) + 32 * j + lane];
-        if (partial)
-            part[32 * j + lane] = acc;
-        else
-            ((T*)p.out)[(size_t)token * p.ldo + (size_t)qh * D + 32 * j + lane] = from_float<T>(acc * inv);
-    }
-    if (lane == 0) {
-        if (partial) {
-            part[D] = top;
-            part[D + 1] = sum;
-        } else if (p.lse) {
-            p.lse[(size_t)token * p.heads + qh] = sum == 0.0f ? INFINITY : from + log2f(sum);
+        for (int j = 0; j < W; ++j) {
+            float acc = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) acc += f[w] * row[w * NEXT + 32 * j + lane];
+            if (partial)
+                part[32 * j + lane] = acc;
+            else
+                ((T*)p.out)[(size_t)token * p.ldo + (size_t)qh * D + 32 * j + lane] = from_float<T>(acc * inv);
+        }
+        if (lane == 0) {
+            if (partial) {
+                part[D] = top;
+                part[D + 1] = sum;
+            } else if (p.lse) {
+                p.lse[(size_t)token * p.heads + qh] = sum == 0.0f ? INFINITY : top + log2f(sum);
+            }
         }
     }
 }
@@ -409,13 +628,12 @@ __global__ void __launch_bounds__(256) packed_attention_join_kernel(const Packed
     if (i >= (long long)p.tokens * p.heads || i < (long long)p.q_start[0] * p.heads || i >= (long long)p.q_start[p.seqs] * p.heads) return;
     const float* part = p.parts + (size_t)i * (D + 2);
     const size_t stride = (size_t)p.tokens * p.heads * (D + 2);
-    float top = -INFINITY;
+    float top = -FLT_MAX;
     for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, part[s * stride + D]);
     top = warp_max(top);
-    const float from = top == -INFINITY ? 0.0f : top;
     float acc[W] = {}, sum = 0.0f;
     for (int s = 0; s < p.splits; ++s) {
-        const float f = exp2f(part[s * stride + D] - from);
+        const float f = exp2_fast(part[s * stride + D] - top);
         sum += f * part[s * stride + D + 1];
 #pragma unroll
         for (int j = 0; j < W; ++j) acc[j] += f * part[s * stride + 32 * j + lane];
@@ -425,78 +643,99 @@ __global__ void __launch_bounds__(256) packed_attention_join_kernel(const Packed
 #pragma unroll
     for (int j = 0; j < W; ++j)
         ((T*)p.out)[(size_t)token * p.ldo + (size_t)qh * D + 32 * j + lane] = from_float<T>(acc[j] * inv);
-    if (lane == 0 && p.lse) p.lse[i] = sum == 0.0f ? INFINITY : from + log2f(sum);
+    if (lane == 0 && p.lse) p.lse[i] = sum == 0.0f ? INFINITY : top + log2f(sum);
 }
 
 // Weights of the cached rows:  w[key] (+)= sum over the request's queries and the kv head's query heads of
-// exp2(s - lse), a warp sixteen rows of the cache, the query rows in their order.
+// exp2(s - lse), a warp 32 rows of the cache, the query rows in their order.
 template <typename T, int D>
 __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(const PackedAttention p) {
-    constexpr int W = D / 32, NP = sizeof(T) == 4 ? 3 : 1;
+    constexpr int W = D / 32, NP = sizeof(T) == 4 ? 2 : 1;
+    extern __shared__ __align__(16) unsigned char smem[];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-    const int head = blockIdx.y, seq = blockIdx.z, at = (blockIdx.x * WARPS + warp) * KEYS;
+    const int head = blockIdx.y, seq = blockIdx.z, at = (blockIdx.x * WARPS + warp) * STAGE;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
     const int limit = p.width * p.cache.page_size, end = min(min(start + n, limit), p.max_rows);
     if (at >= end) return;
     const int* table = p.tables + (size_t)seq * p.width;
-    Keys<W> k;
-    k.load(p, table, head, at, end, g, c);
-    bool page[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) page[u] = at + g + 8 * u < end && page_of(p, table, at + g + 8 * u) >= 0;
-    float total[2] = {0.0f, 0.0f};
-    // the first query row that sees the tile's first cached row
-    const int from_row = max(0, at - start) * p.group / 8 * 8;
-    for (int first = from_row; first < count; first += 8) {
-        Rows rows;
-        rows.set(p, first, count, start, limit, lane);
-        if (rows.least >= at + KEYS) break;  // with a window: this and all later rows have passed the tile
+    unsigned char* stage = smem + warp * Stage<W>::BYTES;
+    const uint32_t there = Stage<W>::request(p, table, head, at, end, stage, lane);
+    copy_wait<0>();
+    __syncwarp();
+    Keys<W> k[2];
+    k[0].load(stage, 0, g, c);
+    k[1].load(stage, KEYS, g, c);
+    float total[2][2] = {};
+    // from the first query row that sees the first of these cached rows
+    for (int first = (int)min((long long)max(0, at - start) * p.group, (long long)count) / 8 * 8; first < count; first += 8) {
+        Rows<1> rows;
+        rows.set(p, first, count, start, limit, c);
+        if (rows.least >= at + STAGE) break;  // with a window: this and all later rows have passed these
         if (rows.most <= at) continue;
-        Queries<T, W, NP> q;
+        Queries<T, W, NP> q[1];
         const int r = first + g;
-        q.load((const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D, c, r < count);
-        float s[4];
-        k.template scores<T, NP>(q, c, s);
+        q[0].load((const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D, c, r < count);
+        const float inv = p.scale / q[0].factor;
+        float qs[2], lse[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int col = first + 2 * c + u;
-            const float lse = col < count ? p.lse[(size_t)(t0 + col / p.group) * p.heads + head * p.group + col % p.group] : INFINITY;
+            qs[u] = __shfl_sync(0xffffffffu, inv, 4 * (2 * c + u));
+            lse[u] = col < count ? p.lse[(size_t)(t0 + col / p.group) * p.heads + head * p.group + col % p.group] : INFINITY;
+        }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int row = at + g + 8 * x;
-                if (page[x] && row >= rows.low[u] && row < rows.high[u]) total[x] += exp2f(s[u + 2 * x] * p.scale - lse);
+        for (int h = 0; h < 2; ++h) {
+            float s[1][4];
+            k[h].scores(q, c, s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int off = KEYS * h + g + 8 * (i >> 1), row = at + off;
+                if ((there >> off & 1) && row >= rows.low[0][i & 1] && row < rows.high[0][i & 1])
+                    total[h][i >> 1] += exp2_fast(s[0][i] * qs[i & 1] - lse[i & 1]);
             }
         }
     }
+    float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        total[x] += __shfl_xor_sync(0xffffffffu, total[x], 1);
-        total[x] += __shfl_xor_sync(0xffffffffu, total[x], 2);
-    }
-    if (c == 0) {
-        float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const int row = at + g + 8 * x;
-            if (row < end) w[row] = p.add && row < start ? w[row] + total[x] : total[x];
+            float t = total[h][x];
+            t += __shfl_xor_sync(0xffffffffu, t, 1);
+            t += __shfl_xor_sync(0xffffffffu, t, 2);
+            const int row = at + KEYS * h + g + 8 * x;
+            if (c == 0 && row < end) w[row] = p.add && row < start ? w[row] + t : t;
         }
-    }
 }
 
+template <typename T, int D, int NT>
+int attend_rows(const PackedAttention& p, int max_q, cudaStream_t st) {
+    const int row_tiles = (max_q * p.group + 8 * NT - 1) / (8 * NT);
+    auto kernel = packed_attention_rows_kernel<T, D, NT>;
+    constexpr size_t smem = RowsPlan<D, NT>::SMEM;
+    if (const int e = ferris_allow_dynamic_smem((const void*)kernel, smem)) return e;
+    return (int)ferris_launch(kernel, dim3(row_tiles, p.cache.kv_heads, p.seqs * p.splits), dim3(WARPS * 32), smem, st, p);
+}
+
+// Tiles of eight query rows that a block takes: two where there are more rows than eight and the registers hold them.
 template <typename T, int D>
 int attend(const PackedAttention& p, int max_q, int max_kv, cudaStream_t st) {
-    const int row_tiles = (max_q * p.group + 7) / 8;
-    const size_t smem = (size_t)WARPS * 8 * (D + 2) * sizeof(float);
-    if (const int e = ferris_allow_dynamic_smem((const void*)packed_attention_rows_kernel<T, D>, smem)) return e;
-    cudaError_t e = ferris_launch(packed_attention_rows_kernel<T, D>, dim3(row_tiles, p.cache.kv_heads, p.seqs * p.splits), dim3(WARPS * 32), smem,
-                                  st, p);
-    if (e == cudaSuccess && p.splits > 1)
-        e = ferris_launch(packed_attention_join_kernel<T, D>, dim3((unsigned)(((long long)p.tokens * p.heads + 7) / 8)), dim3(256), 0, st, p);
-    if (e == cudaSuccess && p.weights)
-        e = ferris_launch(packed_attention_weights_kernel<T, D>, dim3((max_kv + WARPS * KEYS - 1) / (WARPS * KEYS), p.cache.kv_heads, p.seqs),
-                          dim3(WARPS * 32), 0, st, p);
+    int e;
+    if (max_q * p.group > 8 && (sizeof(T) == 2 || D <= 128))
+        e = attend_rows<T, D, (sizeof(T) == 2 || D <= 128) ? 2 : 1>(p, max_q, st);
+    else
+        e = attend_rows<T, D, 1>(p, max_q, st);
+    if (e == 0 && p.splits > 1)
+        e = (int)ferris_launch(packed_attention_join_kernel<T, D>, dim3((unsigned)(((long long)p.tokens * p.heads + 7) / 8)), dim3(256), 0, st, p);
+    if (e == 0 && p.weights) {
+        auto kernel = packed_attention_weights_kernel<T, D>;
+        constexpr size_t smem = (size_t)WARPS * Stage<D / 32>::BYTES;
+        e = ferris_allow_dynamic_smem((const void*)kernel, smem);
+        if (e == 0)
+            e = (int)ferris_launch(kernel, dim3((max_kv + WARPS * STAGE - 1) / (WARPS * STAGE), p.cache.kv_heads, p.seqs), dim3(WARPS * 32), smem, st, p);
+    }
     FERRIS_LAUNCH_CHECK();
 }
 
@@ -517,11 +756,11 @@ int attend_dim(const PackedAttention& p, int max_q, int max_kv, cudaStream_t st)
 
 }  // namespace
 
-// Into how many ranges the cached rows of a step are cut: enough blocks for two to an SM, at least eight tiles of sixteen a warp.
+// Into how many ranges the cached rows of a step are cut: enough blocks for two to an SM, at least a stage a warp.
 FERRIS_API int ferris_packed_attention_splits(int seqs, int kv_heads, int group, int max_q, int max_kv) {
     const int sms = ferris_sm_count() > 0 ? ferris_sm_count() : 148;
     const long long blocks = (long long)seqs * kv_heads * ((max_q * group + 7) / 8);
-    long long want = blocks > 0 ? 2 * sms / blocks : 1, most = max_kv / (WARPS * KEYS * 2);
+    long long want = blocks > 0 ? 2 * sms / blocks : 1, most = max_kv / (WARPS * STAGE);
     if (want > most) want = most;
     if (want > 65535 / (seqs > 0 ? seqs : 1)) want = 65535 / (seqs > 0 ? seqs : 1);
     return want < 1 ? 1 : (int)want;
@@ -541,7 +780,7 @@ FERRIS_API int ferris_packed_attention(const void* q, int ldq, void* out, int ld
     if (weights && !lse) FERRIS_REFUSE("packed attention: weights without scratch");
     if (seqs <= 0 || tokens <= 0 || max_q <= 0) return FERRIS_OK;
     if ((long long)seqs * splits > 65535 || kv_heads > 65535) FERRIS_REFUSE("packed attention: %d requests, %d splits", seqs, splits);
-    if ((long long)width * page_size > 0x7fffffff - 2 * KEYS) FERRIS_REFUSE("packed attention: %d blocks of %d rows", width, page_size);
+    if ((long long)width * page_size > 0x7fffffff - 16 * WARPS * STAGE) FERRIS_REFUSE("packed attention: %d blocks of %d rows", width, page_size);
     p.q = q, p.out = out, p.ldq = ldq, p.ldo = ldo;
     p.tables = tables, p.width = width, p.q_start = q_start, p.start_row = start_row;
     p.seqs = seqs, p.heads = heads, p.group = heads / kv_heads, p.window = window, p.scale = scale * LOG2E;

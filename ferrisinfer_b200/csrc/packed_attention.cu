@@ -38,18 +38,30 @@ struct PackedAttention {
     int seqs, heads, group, window;
     float scale;  // of the scores, times log2(e)
     float* lse;   // log2 of the softmax's sum of every (token, head), or nullptr
-    float* parts;  // [split][token][head][D + 2]: unnormalised outputs, maximum, sum
+    float* parts;  // unnormalised outputs, maximum and sum (D + 2 floats) of every query row, by [split][token][head] or [part][row]
     int splits, tokens;
+    int even;       // the stages of all requests are dealt out evenly (steps whose rows fit one block)
+    int* counters;  // per (request, kv head): blocks that have left their part (even), or nullptr: a kernel joins
+    float* scores;  // [request][kv head][stage][32][8 NT], to the base of 2, or nullptr
+    int max_stages;
+    uint32_t page_mul;  // division by the page size
+    int page_shift;
     float* weights;
     const int* seq_slot;
     long long slot_stride;
     int head_stride, max_rows, add;
     int* status;
+
+    // row / page_size for rows below 2^31: page_mul = ceil(2^(32 + shift) / page_size) with 2^shift < page_size <= 2^(shift + 1)
+    __device__ __forceinline__ int block_of(int row) const { return page_mul ? (int)(__umulhi((uint32_t)row, page_mul) >> page_shift) : row; }
+    // Index of a row of the cache: below 2^32, which the C entry sees to.
+    __device__ __forceinline__ uint32_t row_of(int page, int head, int row, int block) const {
+        return (uint32_t)(page * cache.kv_heads + head) * cache.page_size + (uint32_t)(row - block * cache.page_size);
+    }
 };
 
 // The page of a request's row, -1 where it has none.
-__device__ __forceinline__ int page_of(const PackedAttention& p, const int* table, int row) {
-    const int block = row / p.cache.page_size;
+__device__ __forceinline__ int page_of(const PackedAttention& p, const int* table, int block) {
     const int page = block < p.width ? table[block] : -1;
     if (page >= p.cache.pages) {
         ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 83);
@@ -146,23 +158,24 @@ struct Stage {
             copy_commit();
             return 0;
         }
-        const int page = row < end ? page_of(p, table, row) : -1;
-        const size_t at = page >= 0 ? p.cache.row(page, head, row % p.cache.page_size) : 0;
+        const int block = p.block_of(row), page = row < end ? page_of(p, table, block) : -1;
+        const uint32_t at = page >= 0 ? p.row_of(page, head, row, block) : 0;
         const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
         const uint32_t dst = smem_u32(to);
 #pragma unroll
         for (int i = 0; i < W; ++i) {  // W pieces of 16 bytes a row: neighbouring lanes take neighbouring pieces
             const int piece = i * 32 + lane, r = piece / W, part = piece % W;
-            const size_t a = __shfl_sync(0xffffffffu, (unsigned long long)at, r);
+            const uint32_t a = __shfl_sync(0xffffffffu, at, r);
             const bool live = there >> r & 1;
-            copy_async<16>(dst + r * K_ROW + 16 * part, p.cache.k_codes + (a * W + part) * 16, live);
-            copy_async<16>(dst + V_AT + r * V_ROW + 16 * part, p.cache.v_codes + (a * W + part) * 16, live);
+            const size_t src = (size_t)a * (16 * W) + 16 * part;
+            copy_async<16>(dst + r * K_ROW + 16 * part, p.cache.k_codes + src, live);
+            copy_async<16>(dst + V_AT + r * V_ROW + 16 * part, p.cache.v_codes + src, live);
         }
         constexpr int N = W % 4 == 0 ? 16 : W % 2 == 0 ? 8 : 4;
 #pragma unroll
         for (int i = 0; i < S_ROW / N; ++i) {
-            copy_async<N>(dst + KS_AT + lane * S_ROW + N * i, (const char*)(p.cache.k_scales + at * W) + N * i, page >= 0);
-            copy_async<N>(dst + VS_AT + lane * S_ROW + N * i, (const char*)(p.cache.v_scales + at * W) + N * i, page >= 0);
+            copy_async<N>(dst + KS_AT + lane * S_ROW + N * i, (const char*)(p.cache.k_scales + (size_t)at * W) + N * i, page >= 0);
+            copy_async<N>(dst + VS_AT + lane * S_ROW + N * i, (const char*)(p.cache.v_scales + (size_t)at * W) + N * i, page >= 0);
         }
         copy_commit();
         return there;
@@ -235,11 +248,14 @@ struct Queries {
 // Codes and scales of the keys of sixteen rows: this lane's rows g and g + 8.
 template <int W>
 struct Keys {
-    uint32_t word[2][W], scale[2][W];
+    uint32_t word[2][W], scale[2][W], mine[2][(W + 3) / 4];  // mine: the scales' words of groups 4 i + c
 
     __device__ __forceinline__ void load(const unsigned char* stage, int first, int g, int c) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < (W + 3) / 4; ++i)
+                mine[u][i] = 4 * i + c < W ? reinterpret_cast<const uint32_t*>(stage + Stage<W>::KS_AT + (first + g + 8 * u) * Stage<W>::S_ROW)[4 * i + c] : 0u;
             load_words<W>(word[u], stage + (first + g + 8 * u) * Stage<W>::K_ROW + 4 * W * c);
             load_words<W>(scale[u], stage + Stage<W>::KS_AT + (first + g + 8 * u) * Stage<W>::S_ROW);
         }
@@ -252,14 +268,7 @@ struct Keys {
         for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
         for (int i = 0; i < (W + 3) / 4; ++i) {  // least times the sums of the queries' groups
-            uint32_t l0 = 0, l1 = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (4 * i + k < W && c == k) {
-                    l0 = scale[0][4 * i + k];
-                    l1 = scale[1][4 * i + k];
-                }
-            const uint32_t a0 = __byte_perm(l0, l0, 0x3232), a1 = __byte_perm(l1, l1, 0x3232);
+            const uint32_t a0 = __byte_perm(mine[0][i], 0u, 0x3232), a1 = __byte_perm(mine[1][i], 0u, 0x3232);
             const uint32_t a[4] = {a0, a1, a0, a1};
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma_bf16_16816(s[n], a, q[n].sum[i][0], q[n].sum[i][1]);
@@ -329,24 +338,27 @@ struct RowsPlan {
     static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 };
 
-// Block (row tiles, kv head, request x split): the warps take the stages of the block's range of cached rows in turn, each
-// with rings of copies, a running maximum and a sum of its own, and are joined in shared memory in their order.
+// A run of stages of one request, kv head and tiles of query rows.
+template <int NT>
+struct Segment {
+    int seq, head, t0, count, first;
+    int base, end;       // cached rows
+    float* part;         // where its rows leave their parts: row r at part + offset(r), or nullptr: the whole of it is here
+    size_t row_stride;   // between the rows of a part, 0: by token and head
+    Rows<NT> rows;
+};
+
+// The warps take the stages of the segment in turn, each with a ring of copies, a running maximum and a sum of its own, and
+// are joined in shared memory in their order.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 2 : 1) packed_attention_rows_kernel(const PackedAttention p) {
+__device__ __forceinline__ void attend_segment(const PackedAttention& p, const Segment<NT>& seg, unsigned char* smem) {
     using Plan = RowsPlan<D, NT>;
     constexpr int W = D / 32, NP = sizeof(T) == 4 ? 2 : 1, STAGES = Plan::STAGES;
-    extern __shared__ __align__(16) unsigned char smem[];
-    pdl_launch_dependents();
-    pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-    const int head = blockIdx.y, seq = blockIdx.z / p.splits, split = blockIdx.z % p.splits;
-    const int t0 = max(p.q_start[seq], 0), count = (min(p.q_start[seq + 1], p.tokens) - t0) * p.group, first = blockIdx.x * 8 * NT;
-    if (first >= count) return;
-    const int* table = p.tables + (size_t)seq * p.width;
-    Rows<NT> rows;
-    rows.set(p, first, count, p.start_row[seq], p.width * p.cache.page_size, c);
-    const int floor = rows.least / STAGE * STAGE, stages = (rows.most - floor + STAGE - 1) / STAGE, per = (stages + p.splits - 1) / p.splits;
-    const int base = floor + split * per * STAGE, end = min(rows.most, base + per * STAGE);
+    const int head = seg.head, t0 = seg.t0, count = seg.count, first = seg.first, base = seg.base, end = seg.end;
+    const int* table = p.tables + (size_t)seg.seq * p.width;
+    const Rows<NT>& rows = seg.rows;
+    float* scores = p.scores ? p.scores + ((size_t)seg.seq * p.cache.kv_heads + head) * p.max_stages * (STAGE * 8 * NT) : nullptr;
 
     unsigned char* ring = smem + warp * STAGES * Plan::STAGE_BYTES;
     uint32_t there[STAGES];
@@ -397,6 +409,12 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
         }
         const bool whole = at >= rows.all_low && at + STAGE <= rows.all_high && here == 0xffffffffu;
         uint32_t seen = 0xffffffffu;  // bit 4 n + 2 x + u of half h at 16 h
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[h][n][i] *= qs[n][i & 1];
         if (!whole) {
             seen = 0;
 #pragma unroll
@@ -406,27 +424,37 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int r = KEYS * h + g + 8 * (i >> 1);
-                        if ((here >> r & 1) && at + r >= rows.low[n][i & 1] && at + r < rows.high[n][i & 1]) seen |= 1u << (16 * h + 4 * n + i);
+                        if ((here >> r & 1) && at + r >= rows.low[n][i & 1] && at + r < rows.high[n][i & 1])
+                            seen |= 1u << (16 * h + 4 * n + i);
+                        else
+                            s[h][n][i] = -INFINITY;
                     }
         }
+        if (scores) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        *reinterpret_cast<float2*>(scores + ((size_t)at + KEYS * h + g + 8 * x) * (8 * NT) + 8 * n + 2 * c) = make_float2(s[h][n][2 * x], s[h][n][2 * x + 1]);
+        }
         // The maximum is left behind by up to 2^8: only a score above that makes the warp find a new one and scale what it has.
+        float high[NT][2];
         bool grew = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[h][n][i] *= qs[n][i & 1];
-                    if (!whole && !(seen >> (16 * h + 4 * n + i) & 1)) s[h][n][i] = -INFINITY;
-                    grew |= s[h][n][i] > m[n][i & 1] + 8.0f;
-                }
+            for (int u = 0; u < 2; ++u) {
+                high[n][u] = fmaxf(fmaxf(s[0][n][u], s[0][n][u + 2]), fmaxf(s[1][n][u], s[1][n][u + 2]));
+                grew |= high[n][u] - 8.0f > m[n][u];
+            }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    float top = fmaxf(fmaxf(s[0][n][u], s[0][n][u + 2]), fmaxf(s[1][n][u], s[1][n][u + 2]));
+                    float top = high[n][u];
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                     const float now = fmaxf(m[n][u], top), f = exp2_fast(m[n][u] - now);
@@ -593,8 +621,8 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
             f[w] = exp2_fast(row[w * NEXT + D] - top);
             sum += f[w] * row[w * NEXT + D + 1];
         }
-        const bool partial = p.splits > 1;
-        float* part = partial ? p.parts + (((size_t)split * p.tokens + token) * p.heads + qh) * (D + 2) : nullptr;
+        const bool partial = seg.part != nullptr;
+        float* part = seg.part + (seg.row_stride ? (size_t)(8 * n + warp) * seg.row_stride : ((size_t)token * p.heads + qh) * (D + 2));
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int j = 0; j < W; ++j) {
@@ -615,6 +643,225 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
             }
         }
     }
+}
+
+// Stages of 32 cached rows that a request's queries see together (at least one, so that every request has a block), from which on.
+__device__ __forceinline__ int stages_of(const PackedAttention& p, int seq, int& floor) {
+    const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, start = p.start_row[seq];
+    const int most = max(0, min(start + n, p.width * p.cache.page_size));
+    const int least = min(p.window > 0 ? max(0, start - p.window + 1) : 0, most);
+    floor = least / STAGE * STAGE;
+    return n > 0 ? max(1, (most - floor + STAGE - 1) / STAGE) : 0;
+}
+
+constexpr int EVEN_SEQS = 1024;  // most requests of a step whose stages are dealt out evenly
+constexpr int EVEN_STAGES = WARPS;  // fewest stages of a block, so that each warp has one
+
+// Which parts hold the stages a .. b - 1 of `units` that are dealt out to `blocks` blocks: block i gets stages i units / blocks up to
+// (i + 1) units / blocks.  A block leaves the part that another block began in place 2 i, the part that it begins itself in 2 i + 1.
+__device__ __forceinline__ int block_of_unit(int u, int units, int blocks) { return (int)((((long long)u + 1) * blocks - 1) / units); }
+
+__device__ __forceinline__ int even_blocks(int units, int most) { return min(most, max(1, units / EVEN_STAGES)); }
+
+// A warp joins the parts first .. last of one query row in their order.
+template <typename T, int D>
+__device__ __forceinline__ void join_row(const PackedAttention& p, int first, int last, int rows, int r, int token, int qh, int lane) {
+    constexpr int W = D / 32;
+    const auto at = [&](int i) { return p.parts + ((size_t)(2 * i + (i == first)) * rows + r) * (D + 2); };
+    float top = -FLT_MAX;
+    for (int i = first + lane; i <= last; i += 32) top = fmaxf(top, __ldcg(at(i) + D));
+    top = warp_max(top);
+    float acc[W] = {}, sum = 0.0f;
+#pragma unroll 4
+    for (int i = first; i <= last; ++i) {
+        const float* part = at(i);
+        const float f = exp2_fast(__ldcg(part + D) - top);
+        sum += f * __ldcg(part + D + 1);
+#pragma unroll
+        for (int j = 0; j < W; ++j) acc[j] += f * __ldcg(part + 32 * j + lane);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < W; ++j) ((T*)p.out)[(size_t)token * p.ldo + (size_t)qh * D + 32 * j + lane] = from_float<T>(acc[j] * inv);
+    if (lane == 0 && p.lse) p.lse[(size_t)token * p.heads + qh] = sum == 0.0f ? INFINITY : top + log2f(sum);
+}
+
+// Grid (row tiles, kv heads, requests x splits): a block a segment.  Or, where the rows of every request fit one block's tiles
+// (single tokens), a grid of as many blocks as the GPU holds: the stages of all requests and kv heads in a row, dealt out evenly
+// whatever the requests' lengths; a request that several blocks share is joined by the last of them to finish, or by a kernel.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 2 : 1) packed_attention_rows_kernel(const PackedAttention p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int before[EVEN_SEQS + 1];  // stages of the requests before each one
+    __shared__ int warp_total[WARPS], last_here;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int c = threadIdx.x & 3, limit = p.width * p.cache.page_size;
+    Segment<NT> seg;
+    if (p.even) {  // running sums: four requests a thread
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        int mine[EVEN_SEQS / (WARPS * 32)], sum = 0, floor;
+#pragma unroll
+        for (int i = 0; i < EVEN_SEQS / (WARPS * 32); ++i) {
+            const int s = threadIdx.x * (EVEN_SEQS / (WARPS * 32)) + i;
+            mine[i] = s < p.seqs ? stages_of(p, s, floor) * p.cache.kv_heads : 0;
+            sum += mine[i];
+        }
+        int upto = sum;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, x);
+            if (lane >= x) upto += v;
+        }
+        if (lane == 31) warp_total[warp] = upto;
+        __syncthreads();
+        upto -= sum;
+        for (int w = 0; w < warp; ++w) upto += warp_total[w];
+#pragma unroll
+        for (int i = 0; i < EVEN_SEQS / (WARPS * 32); ++i) {
+            before[threadIdx.x * (EVEN_SEQS / (WARPS * 32)) + i] = upto;
+            upto += mine[i];
+        }
+        if (threadIdx.x == WARPS * 32 - 1) before[EVEN_SEQS] = upto;
+        __syncthreads();
+    }
+    int units = 0, blocks = 0, u = 0, stop = 1, s = 0;
+    const int me = blockIdx.x;
+    if (p.even) {
+        units = before[EVEN_SEQS], blocks = even_blocks(units, gridDim.x);
+        if (me >= blocks) return;
+        u = (int)((long long)me * units / blocks), stop = (int)((long long)(me + 1) * units / blocks);
+    }
+    while (u < stop) {
+        int stages = 1, begin = 0, take = 1, from = 0, split = 0;
+        if (p.even) {
+            for (int step = EVEN_SEQS / 2; step; step >>= 1)  // the last request that begins at or before u (and has stages)
+                if (s + step < EVEN_SEQS && before[s + step] <= u) s += step;
+            int floor;
+            stages = stages_of(p, s, floor);
+            const int rel = u - before[s];
+            seg.head = rel / stages, from = rel - seg.head * stages;
+            begin = u - from, take = min(stages - from, stop - u);
+            seg.first = 0;
+        } else {
+            s = blockIdx.z / p.splits, split = blockIdx.z % p.splits, seg.head = blockIdx.y, seg.first = blockIdx.x * 8 * NT;
+        }
+        const int head = seg.head;
+        seg.seq = s, seg.t0 = max(p.q_start[s], 0), seg.count = (min(p.q_start[s + 1], p.tokens) - seg.t0) * p.group;
+        if (seg.first >= seg.count) return;
+        seg.rows.set(p, seg.first, seg.count, p.start_row[s], limit, c);
+        const int floor = seg.rows.least / STAGE * STAGE;
+        if (!p.even) {
+            stages = (seg.rows.most - floor + STAGE - 1) / STAGE;
+            const int per = (stages + p.splits - 1) / p.splits;
+            from = split * per, take = per;
+        }
+        seg.base = floor + from * STAGE, seg.end = min(seg.rows.most, seg.base + take * STAGE);
+        const bool shared = p.even && take < stages;
+        seg.part = shared ? p.parts + (size_t)(2 * me + (from == 0)) * (8 * NT) * (D + 2)
+                          : !p.even && p.splits > 1 ? p.parts + (size_t)split * p.tokens * p.heads * (D + 2) : nullptr;
+        seg.row_stride = p.even ? D + 2 : 0;
+        attend_segment<T, D, NT>(p, seg, smem);
+        if (shared && p.counters) {
+            const int first = block_of_unit(begin, units, blocks), last = block_of_unit(begin + stages - 1, units, blocks);
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                int* counter = p.counters + s * p.cache.kv_heads + head;
+                last_here = atomicAdd(counter, 1) == last - first;
+                if (last_here) *counter = 0;  // for the next launch
+                __threadfence();
+            }
+            __syncthreads();
+            if (last_here)
+                for (int r = threadIdx.x >> 5; r < seg.count; r += WARPS)
+                    join_row<T, D>(p, first, last, 8 * NT, r, seg.t0 + r / p.group, head * p.group + r % p.group, threadIdx.x & 31);
+        }
+        if (!p.even) return;
+        __syncthreads();  // shared memory is free again
+        u += take;
+    }
+    if (!p.counters && me == 0) {  // what the joining kernel needs
+        int* to = (int*)(p.parts + (size_t)2 * gridDim.x * (8 * NT) * (D + 2));
+        for (int i = threadIdx.x; i <= p.seqs; i += WARPS * 32) to[i] = before[i];
+        if (threadIdx.x == 0) to[p.seqs + 1] = blocks;
+    }
+}
+
+// Block (row, kv head, request) joins the parts of one query row: the warps take them in turn and are added in their order.
+template <typename T, int D>
+__global__ void __launch_bounds__(WARPS * 32) packed_attention_join_even_kernel(const PackedAttention p, int grid) {
+    constexpr int W = D / 32;
+    __shared__ float tops[WARPS], sums[WARPS], outs[WARPS][D];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x, head = blockIdx.y, s = blockIdx.z, rows = gridDim.x;
+    const int* before = (const int*)(p.parts + (size_t)2 * grid * rows * (D + 2));
+    const int t0 = max(p.q_start[s], 0), count = (min(p.q_start[s + 1], p.tokens) - t0) * p.group;
+    if (r >= count) return;
+    const int units = before[p.seqs], blocks = before[p.seqs + 1], stages = (before[s + 1] - before[s]) / p.cache.kv_heads;
+    const int begin = before[s] + head * stages;
+    const int first = block_of_unit(begin, units, blocks), last = block_of_unit(begin + stages - 1, units, blocks);
+    if (first == last) return;  // one block had all of it
+    const auto at = [&](int i) { return p.parts + ((size_t)(2 * i + (i == first)) * rows + r) * (D + 2); };
+    float top = -FLT_MAX;
+    for (int i = first + threadIdx.x; i <= last; i += WARPS * 32) top = fmaxf(top, at(i)[D]);
+    top = warp_max(top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, tops[w]);
+    float acc[W] = {}, sum = 0.0f;
+#pragma unroll 4
+    for (int i = first + warp; i <= last; i += WARPS) {
+        const float* part = at(i);
+        const float f = exp2_fast(part[D] - top);
+        sum += f * part[D + 1];
+#pragma unroll
+        for (int j = 0; j < W; ++j) acc[j] += f * part[32 * j + lane];
+    }
+    if (lane == 0) sums[warp] = sum;
+#pragma unroll
+    for (int j = 0; j < W; ++j) outs[warp][32 * j + lane] = acc[j];
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) sum += sums[w];
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int token = t0 + r / p.group, qh = head * p.group + r % p.group;
+    for (int d = threadIdx.x; d < D; d += WARPS * 32) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) v += outs[w][d];
+        ((T*)p.out)[(size_t)token * p.ldo + (size_t)qh * D + d] = from_float<T>(v * inv);
+    }
+    if (threadIdx.x == 0 && p.lse) p.lse[(size_t)token * p.heads + qh] = sum == 0.0f ? INFINITY : top + log2f(sum);
+}
+
+// Weights of the cached rows from the scores that the attention kernel has left: a thread a row.
+__global__ void __launch_bounds__(256) packed_attention_scored_weights_kernel(const PackedAttention p, int cols) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int head = blockIdx.y, seq = blockIdx.z, row = blockIdx.x * 256 + threadIdx.x;
+    const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
+    const int end = min(min(start + n, p.width * p.cache.page_size), p.max_rows);
+    if (row >= end || n <= 0) return;
+    int floor;
+    stages_of(p, seq, floor);
+    float total = 0.0f;
+    if (row >= floor) {
+        const float* s = p.scores + (((size_t)seq * p.cache.kv_heads + head) * p.max_stages * STAGE + row) * cols;
+        for (int i = 0; i < cols && 4 * (i / 4) < count; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(s + i);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k < count && x[k] != -INFINITY)  // (a row that is not seen, beside a sum that is not finite)
+                    total += exp2_fast(x[k] - p.lse[(size_t)(t0 + (i + k) / p.group) * p.heads + head * p.group + (i + k) % p.group]);
+        }
+    }
+    float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride + row;
+    *w = p.add && row < start ? *w + total : total;
 }
 
 // A warp joins the splits of one (token, head) in their order.
@@ -710,26 +957,60 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
         }
 }
 
+// How a step is cut: tiles of eight query rows that a block takes, whether all rows of a request fit them, and the blocks or splits.
+struct Plan {
+    int tiles, even, blocks, splits, join_kernel;
+    long long part_floats, score_floats;
+};
+
+// Tiles: two where there are more rows than eight and the registers hold them.
+Plan make_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int tokens, int max_q, int max_kv, int weights) {
+    const int sms = ferris_sm_count() > 0 ? ferris_sm_count() : 148;
+    Plan q = {};
+    const long long rows = (long long)max_q * group;
+    q.tiles = rows > 8 && (dtype == FERRIS_BF16 || head_dim <= 128) ? 2 : 1;
+    const int per_sm = head_dim * q.tiles <= 128 && dtype == FERRIS_BF16 ? 2 : 1;
+    const long long stages = max_kv / STAGE + 2, pairs = (long long)seqs * kv_heads;
+    q.even = rows <= 8 * q.tiles && seqs <= EVEN_SEQS && pairs * stages < 0x7fffffff;
+    q.splits = 1;
+    if (q.even) {
+        const long long most = pairs * stages / EVEN_STAGES;
+        q.blocks = (int)(most < 1 ? 1 : most < sms * per_sm ? most : sms * per_sm);
+        q.join_kernel = q.blocks > 16 * pairs;  // so many parts of a request that one block would be long at joining them
+        q.part_floats = 2ll * q.blocks * 8 * q.tiles * (head_dim + 2) + (q.join_kernel ? seqs + 2 : 0);
+        q.score_floats = weights ? pairs * stages * STAGE * 8 * q.tiles : 0;
+        if (q.score_floats > (1ll << 27)) q.score_floats = 0;  // (above 512 MB the scores are formed again)
+    } else {
+        const long long blocks = pairs * ((rows + 8 * q.tiles - 1) / (8 * q.tiles));
+        long long want = blocks > 0 ? (long long)sms * per_sm / blocks : 1;
+        if (want > max_kv / (WARPS * STAGE)) want = max_kv / (WARPS * STAGE);
+        if (want > 65535 / (seqs > 0 ? seqs : 1)) want = 65535 / (seqs > 0 ? seqs : 1);
+        q.splits = want < 1 ? 1 : (int)want;
+        q.part_floats = q.splits > 1 ? (long long)q.splits * tokens * kv_heads * group * (head_dim + 2) : 0;
+    }
+    return q;
+}
+
 template <typename T, int D, int NT>
-int attend_rows(const PackedAttention& p, int max_q, cudaStream_t st) {
-    const int row_tiles = (max_q * p.group + 8 * NT - 1) / (8 * NT);
+int attend_rows(const PackedAttention& p, const Plan& q, int max_q, cudaStream_t st) {
     auto kernel = packed_attention_rows_kernel<T, D, NT>;
     constexpr size_t smem = RowsPlan<D, NT>::SMEM;
     if (const int e = ferris_allow_dynamic_smem((const void*)kernel, smem)) return e;
-    return (int)ferris_launch(kernel, dim3(row_tiles, p.cache.kv_heads, p.seqs * p.splits), dim3(WARPS * 32), smem, st, p);
+    const dim3 grid = q.even ? dim3(q.blocks) : dim3((max_q * p.group + 8 * NT - 1) / (8 * NT), p.cache.kv_heads, p.seqs * p.splits);
+    return (int)ferris_launch(kernel, grid, dim3(WARPS * 32), smem, st, p);
 }
 
-// Tiles of eight query rows that a block takes: two where there are more rows than eight and the registers hold them.
 template <typename T, int D>
-int attend(const PackedAttention& p, int max_q, int max_kv, cudaStream_t st) {
-    int e;
-    if (max_q * p.group > 8 && (sizeof(T) == 2 || D <= 128))
-        e = attend_rows<T, D, (sizeof(T) == 2 || D <= 128) ? 2 : 1>(p, max_q, st);
-    else
-        e = attend_rows<T, D, 1>(p, max_q, st);
+int attend(const PackedAttention& p, const Plan& q, int max_q, int max_kv, cudaStream_t st) {
+    constexpr int MOST = sizeof(T) == 2 || D <= 128 ? 2 : 1;
+    int e = q.tiles == 2 ? attend_rows<T, D, MOST>(p, q, max_q, st) : attend_rows<T, D, 1>(p, q, max_q, st);
+    if (e == 0 && q.join_kernel)
+        e = (int)ferris_launch(packed_attention_join_even_kernel<T, D>, dim3(8 * q.tiles, p.cache.kv_heads, p.seqs), dim3(WARPS * 32), 0, st, p, q.blocks);
     if (e == 0 && p.splits > 1)
         e = (int)ferris_launch(packed_attention_join_kernel<T, D>, dim3((unsigned)(((long long)p.tokens * p.heads + 7) / 8)), dim3(256), 0, st, p);
-    if (e == 0 && p.weights) {
+    if (e == 0 && p.weights && p.scores) {
+        e = (int)ferris_launch(packed_attention_scored_weights_kernel, dim3((max_kv + 255) / 256, p.cache.kv_heads, p.seqs), dim3(256), 0, st, p, 8 * q.tiles);
+    } else if (e == 0 && p.weights) {
         auto kernel = packed_attention_weights_kernel<T, D>;
         constexpr size_t smem = (size_t)WARPS * Stage<D / 32>::BYTES;
         e = ferris_allow_dynamic_smem((const void*)kernel, smem);
@@ -740,54 +1021,63 @@ int attend(const PackedAttention& p, int max_q, int max_kv, cudaStream_t st) {
 }
 
 template <typename T>
-int attend_dim(const PackedAttention& p, int max_q, int max_kv, cudaStream_t st) {
+int attend_dim(const PackedAttention& p, const Plan& q, int max_q, int max_kv, cudaStream_t st) {
     switch (p.cache.head_dim) {
-        case 32: return attend<T, 32>(p, max_q, max_kv, st);
-        case 64: return attend<T, 64>(p, max_q, max_kv, st);
-        case 96: return attend<T, 96>(p, max_q, max_kv, st);
-        case 128: return attend<T, 128>(p, max_q, max_kv, st);
-        case 160: return attend<T, 160>(p, max_q, max_kv, st);
-        case 192: return attend<T, 192>(p, max_q, max_kv, st);
-        case 224: return attend<T, 224>(p, max_q, max_kv, st);
-        case 256: return attend<T, 256>(p, max_q, max_kv, st);
+        case 32: return attend<T, 32>(p, q, max_q, max_kv, st);
+        case 64: return attend<T, 64>(p, q, max_q, max_kv, st);
+        case 96: return attend<T, 96>(p, q, max_q, max_kv, st);
+        case 128: return attend<T, 128>(p, q, max_q, max_kv, st);
+        case 160: return attend<T, 160>(p, q, max_q, max_kv, st);
+        case 192: return attend<T, 192>(p, q, max_q, max_kv, st);
+        case 224: return attend<T, 224>(p, q, max_q, max_kv, st);
+        case 256: return attend<T, 256>(p, q, max_q, max_kv, st);
     }
     FERRIS_REFUSE("packed attention: heads of %d elements", p.cache.head_dim);
 }
 
 }  // namespace
 
-// Into how many ranges the cached rows of a step are cut: enough blocks for two to an SM, at least a stage a warp.
-FERRIS_API int ferris_packed_attention_splits(int seqs, int kv_heads, int group, int max_q, int max_kv) {
-    const int sms = ferris_sm_count() > 0 ? ferris_sm_count() : 148;
-    const long long blocks = (long long)seqs * kv_heads * ((max_q * group + 7) / 8);
-    long long want = blocks > 0 ? 2 * sms / blocks : 1, most = max_kv / (WARPS * STAGE);
-    if (want > most) want = most;
-    if (want > 65535 / (seqs > 0 ? seqs : 1)) want = 65535 / (seqs > 0 ? seqs : 1);
-    return want < 1 ? 1 : (int)want;
+// What scratch a step needs: floats of parts and of scores, counters (whole numbers that are nought, and are left so).
+FERRIS_API int ferris_packed_attention_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int tokens, int max_q, int max_kv,
+                                            int weights, long long* floats) {
+    const Plan q = make_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_q, max_kv, weights);
+    floats[0] = q.part_floats;
+    floats[1] = q.score_floats;
+    floats[2] = q.even && !q.join_kernel ? (long long)seqs * kv_heads : 0;
+    return FERRIS_OK;
 }
 
 FERRIS_API int ferris_packed_attention(const void* q, int ldq, void* out, int ldo, int dtype, void* k_codes, void* k_scales, void* v_codes,
                                        void* v_scales, int pages, int kv_heads, int page_size, int head_dim, const int* tables, int width,
                                        const int* q_start, const int* start_row, int seqs, int tokens, int heads, int max_q, int max_kv,
-                                       int window, float scale, float* lse, float* parts, int splits, float* weights, const int* seq_slot,
-                                       long long slot_stride, int head_stride, int max_rows, int add, void* stream) {
+                                       int window, float scale, float* lse, float* parts, float* scores, int* counters, float* weights,
+                                       const int* seq_slot, long long slot_stride, int head_stride, int max_rows, int add, void* stream) {
     PackedAttention p = {};
     p.cache = {(uint8_t*)k_codes, (uint32_t*)k_scales, (uint8_t*)v_codes, (uint32_t*)v_scales, pages, kv_heads, page_size, head_dim};
     if (const char* why = packed_cache_refusal(p.cache)) FERRIS_REFUSE("%s", why);
     if (heads <= 0 || heads % kv_heads) FERRIS_REFUSE("packed attention: %d heads over %d kv heads", heads, kv_heads);
-    if (window < 0 || width <= 0 || splits <= 0) FERRIS_REFUSE("packed attention: window %d, %d blocks, %d splits", window, width, splits);
-    if (splits > 1 && !parts) FERRIS_REFUSE("packed attention: %d splits without scratch", splits);
+    if (window < 0 || width <= 0) FERRIS_REFUSE("packed attention: window %d, %d blocks", window, width);
     if (weights && !lse) FERRIS_REFUSE("packed attention: weights without scratch");
     if (seqs <= 0 || tokens <= 0 || max_q <= 0) return FERRIS_OK;
-    if ((long long)seqs * splits > 65535 || kv_heads > 65535) FERRIS_REFUSE("packed attention: %d requests, %d splits", seqs, splits);
     if ((long long)width * page_size > 0x7fffffff - 16 * WARPS * STAGE) FERRIS_REFUSE("packed attention: %d blocks of %d rows", width, page_size);
+    const Plan plan = make_plan(dtype, head_dim, seqs, kv_heads, heads / kv_heads, tokens, max_q, max_kv, weights != nullptr);
+    if (plan.part_floats && !parts) FERRIS_REFUSE("packed attention: no scratch for its parts");
+    if (plan.even && !plan.join_kernel && !counters) FERRIS_REFUSE("packed attention: no counters");
+    if (kv_heads > 65535 || (!plan.even && (long long)seqs * plan.splits > 65535) || seqs > 65535)
+        FERRIS_REFUSE("packed attention: %d requests of %d kv heads", seqs, kv_heads);
     p.q = q, p.out = out, p.ldq = ldq, p.ldo = ldo;
     p.tables = tables, p.width = width, p.q_start = q_start, p.start_row = start_row;
     p.seqs = seqs, p.heads = heads, p.group = heads / kv_heads, p.window = window, p.scale = scale * LOG2E;
-    p.lse = lse, p.parts = parts, p.splits = splits, p.tokens = tokens;
+    p.lse = lse, p.parts = parts, p.splits = plan.splits, p.tokens = tokens;
+    p.even = plan.even, p.counters = plan.join_kernel ? nullptr : counters, p.scores = plan.score_floats ? scores : nullptr;
+    p.max_stages = max_kv / STAGE + 2;
+    if (page_size > 1) {
+        while ((2 << p.page_shift) < page_size) ++p.page_shift;
+        p.page_mul = (uint32_t)(((1ull << (32 + p.page_shift)) + page_size - 1) / page_size);
+    }
     p.weights = weights, p.seq_slot = seq_slot, p.slot_stride = slot_stride, p.head_stride = head_stride, p.max_rows = max_rows, p.add = add;
     p.status = ferris_status_ptr();
-    if (dtype == FERRIS_BF16) return attend_dim<bf16>(p, max_q, max_kv, (cudaStream_t)stream);
-    if (dtype == FERRIS_F32) return attend_dim<float>(p, max_q, max_kv, (cudaStream_t)stream);
+    if (dtype == FERRIS_BF16) return attend_dim<bf16>(p, plan, max_q, max_kv, (cudaStream_t)stream);
+    if (dtype == FERRIS_F32) return attend_dim<float>(p, plan, max_q, max_kv, (cudaStream_t)stream);
     FERRIS_REFUSE("packed attention: dtype %d is not known", dtype);
 }

@@ -39,5 +39,7 @@ inline const char* packed_cache_refusal(const PackedCache& c) {
     if (c.head_dim <= 0 || c.head_dim % 32 || c.head_dim > 256) return "packed heads have a multiple of 32 elements, at most 256";
     if (((uintptr_t)c.k_codes | (uintptr_t)c.v_codes | (uintptr_t)c.k_scales | (uintptr_t)c.v_scales) & 15)
         return "the packed cache must begin on 16 bytes";
+    if ((long long)c.pages * c.kv_heads > 0x7fffffff || (long long)c.pages * c.kv_heads * c.page_size > 0xffffffffll)
+        return "the packed cache has more rows than 32 bits count";
     return nullptr;
 }

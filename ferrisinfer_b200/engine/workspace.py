@@ -23,7 +23,8 @@ class Workspace:
         self._replaced: list = []  # outgrown buffers that recorded steps may still point at
         self._pinned = False
 
-    def get(self, name: str, shape, dtype: torch.dtype) -> torch.Tensor:
+    def get(self, name: str, shape, dtype: torch.dtype, zeroed: bool = False) -> torch.Tensor:
+        """``zeroed``: new storage is zero (counters that their kernels leave as they found them)."""
         count = 1
         for s in shape:
             count *= int(s)
@@ -32,7 +33,7 @@ class Workspace:
         if buf is None or buf.numel() < count:
             if buf is not None and self._pinned:
                 self._replaced.append(buf)
-            buf = torch.empty(max(count, 1), dtype=dtype, device=self.device)
+            buf = (torch.zeros if zeroed else torch.empty)(max(count, 1), dtype=dtype, device=self.device)
             self._buffers[key] = buf
         return buf[:count].view(*shape)
 

@@ -50,9 +50,9 @@ _SIGNATURES = {
     "ferris_packed_cache_read": [_VP, _VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP],
     "ferris_packed_cache_evict": [_VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _I, _VP, _I, _VP, _VP, _VP, _LL, _I, _I,
                                   _VP, _VP, _LL, _I, _I, _I, _I, _I, _VP],
-    "ferris_packed_attention_splits": [_I, _I, _I, _I, _I],
+    "ferris_packed_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
     "ferris_packed_attention": [_VP, _I, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _VP,
-                                _VP, _I, _VP, _VP, _LL, _I, _I, _I, _VP],
+                                _VP, _VP, _VP, _VP, _VP, _LL, _I, _I, _I, _VP],
 }
 _declared = False
 
@@ -2505,17 +2505,20 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
         out.zero_()
         return
     lib = _lib()
-    splits = lib.ferris_packed_attention_splits(S, pages.kv_heads, num_heads // pages.kv_heads, max_q_len,
-                                                min(max_kv_len, window + max_q_len) if window else max_kv_len)
-    if workspace is None and (splits > 1 or weights is not None):
+    plan = (_LL * 3)()
+    lib.ferris_packed_attention_plan(dt, D, S, pages.kv_heads, num_heads // pages.kv_heads, T, max_q_len, max_kv_len,
+                                     0 if weights is None else 1, plan)
+    if workspace is None:
         raise KernelError("packed attention: a workspace is needed")
-    parts = workspace.get("packed_attention_parts", (splits * T * num_heads * (D + 2),), torch.float32).data_ptr() if splits > 1 else None
-    lse = workspace.get("packed_attention_lse", (T * num_heads,), torch.float32).data_ptr() if weights is not None else None
+    parts, scores, counters = plan[0], plan[1], plan[2]
+    scratch = (workspace.get("packed_attention_lse", (T * num_heads,), torch.float32).data_ptr() if weights is not None else None,
+               workspace.get("packed_attention_parts", (parts,), torch.float32).data_ptr() if parts else None,
+               workspace.get("packed_attention_scores", (scores,), torch.float32).data_ptr() if scores else None,
+               workspace.get("packed_attention_counters", (counters,), torch.int32, zeroed=True).data_ptr() if counters else None)
     _check(lib.ferris_packed_attention(q.data_ptr(), ldq, out.data_ptr(), ldo, dt, *pages._args, pages.pages, pages.kv_heads, pages.page_size, D,
                                        block_tables.data_ptr(), block_tables.shape[1], seq_q_start.data_ptr(), seq_start_row.data_ptr(), S, T,
-                                       num_heads, max_q_len, max_kv_len, window, scale, lse, parts, splits, *w, 1 if add_weights else 0,
-                                       _stream()),
-           "packed attention", 1 + (splits > 1) + (weights is not None))
+                                       num_heads, max_q_len, max_kv_len, window, scale, *scratch, *w, 1 if add_weights else 0, _stream()),
+           "packed attention", 1 + (parts > 0 and not counters) + (weights is not None))
 
 
 def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows: torch.Tensor, weights: torch.Tensor,

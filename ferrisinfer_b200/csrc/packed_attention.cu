@@ -29,7 +29,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct PackedAttention {
     const void* q;
     void* out;
-    int ldq, ldo;
+    int ldq, ldo, q_aligned;  // rows of q on 16 bytes
     PackedCache cache;
     const int* tables;
     int width;  // blocks of a request's table
@@ -40,7 +40,8 @@ struct PackedAttention {
     float* lse;   // log2 of the softmax's sum of every (token, head), or nullptr
     float* parts;  // unnormalised outputs, maximum and sum (D + 2 floats) of every query row, by [split][token][head] or [part][row]
     int splits, tokens;
-    int even;       // the stages of all requests are dealt out evenly (steps whose rows fit one block)
+    int even;       // the stages of all requests are dealt out evenly (steps whose rows fit one block) ...
+    int most_blocks;  // ... to about so many blocks
     int* counters;  // per (request, kv head): blocks that have left their part (even), or nullptr: a kernel joins
     float* scores;  // [request][kv head][stage][32][8 NT], to the base of 2, or nullptr
     int max_stages;
@@ -190,15 +191,29 @@ struct Queries {
     uint32_t sum[(W + 3) / 4][2];  // the sum of group 4 i + c in three bf16 parts
     float factor;
 
-    __device__ __forceinline__ void load(const T* row, int c, bool valid) {
-        float x[W][8], top = 0.0f;
+    __device__ __forceinline__ void load(const T* row, int c, bool valid, bool aligned) {
+        float x[W][8] = {}, top = 0.0f;
+        if (valid && aligned) {
+            constexpr int N = 16 / sizeof(T);
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int i = 0; i < 8 / N; ++i) {
+                    const uint4 v = reinterpret_cast<const uint4*>(row + 32 * j + 8 * c)[i];
+                    const T* t = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                    for (int k = 0; k < N; ++k) x[j][N * i + k] = to_float(t[k]);
+                }
+        } else if (valid) {
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[j][i] = to_float(row[32 * j + 8 * c + i]);
+        }
 #pragma unroll
         for (int j = 0; j < W; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[j][i] = valid ? to_float(row[32 * j + 8 * c + i]) : 0.0f;
-                top = fmaxf(top, fabsf(x[j][i]));
-            }
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // 2^(13 - e) for 2^e <= top < 2^(e + 1), at most 2^126
@@ -334,7 +349,8 @@ template <int D, int NT>
 struct RowsPlan {
     static constexpr int W = D / 32, STAGE_BYTES = Stage<W>::BYTES;
     static constexpr int STAGES = D <= 64 ? 3 : 2;
-    static constexpr int RING = WARPS * STAGES * STAGE_BYTES, JOIN = WARPS * 8 * NT * (D + 2) * 4;
+    static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
+    static constexpr int ROW = D + 4, JOIN = WARPS * 8 * NT * ROW * 4;  // (a row's output, maximum, sum; lanes store 16 bytes without bank conflicts)
     static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 };
 
@@ -372,7 +388,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int r = first + 8 * n + g;
-        q[n].load((const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D, c, r < count);
+        q[n].load((const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D, c, r < count, p.q_aligned);
         const float inv = p.scale / q[n].factor;
 #pragma unroll
         for (int u = 0; u < 2; ++u) qs[n][u] = __shfl_sync(0xffffffffu, inv, 4 * (2 * c + u));
@@ -586,22 +602,21 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
                 for (int j = 0; j < W; ++j) low_o[n][j][u] += __shfl_xor_sync(0xffffffffu, low_o[n][j][u], x);
             }
         }
-        float* mine = joined + (size_t)(warp * NT + n) * 8 * (D + 2);
+        float* mine = joined + (size_t)(warp * NT + n) * 8 * Plan::ROW;
 #pragma unroll
-        for (int j = 0; j < W; ++j)
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // rows g + 8 of the product met codes x 16; the weights were 2^6 / v_top times the true ones
-                    const float v = o[n][j][t][i] * (i >> 1 ? 0.0009765625f : 0.015625f) * v_top + low_o[n][j][i & 1];
-                    mine[(2 * c + (i & 1)) * (D + 2) + 32 * j + 4 * g + 2 * t + (i >> 1)] = bad[n] >> (j + 8 * (i & 1)) & 1 ? NAN : v;
-                }
-        if (g == 0) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                mine[(2 * c + u) * (D + 2) + D] = m[n][u];
-                mine[(2 * c + u) * (D + 2) + D + 1] = l[n][u];
+            for (int j = 0; j < W; ++j) {
+                // rows g + 8 of the product met codes x 16; the weights were 2^6 / v_top times the true ones
+                const float low = low_o[n][j][u], even = 0.015625f * v_top, odd = 0.0009765625f * v_top;
+                float4 v = make_float4(fmaf(o[n][j][0][u], even, low), fmaf(o[n][j][0][u + 2], odd, low), fmaf(o[n][j][1][u], even, low),
+                                       fmaf(o[n][j][1][u + 2], odd, low));
+                if (bad[n] >> (j + 8 * u) & 1) v = make_float4(NAN, NAN, NAN, NAN);
+                *reinterpret_cast<float4*>(mine + (2 * c + u) * Plan::ROW + 32 * j + 4 * g) = v;
+            }
+            if (g == 0) {
+                mine[(2 * c + u) * Plan::ROW + D] = m[n][u];
+                mine[(2 * c + u) * Plan::ROW + D + 1] = l[n][u];
             }
         }
     }
@@ -611,8 +626,8 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
         const int r = first + 8 * n + warp;
         if (r >= count) break;
         const int token = t0 + r / p.group, qh = head * p.group + r % p.group;
-        const float* row = joined + (size_t)(n * 8 + warp) * (D + 2);
-        constexpr int NEXT = NT * 8 * (D + 2);
+        const float* row = joined + (size_t)(n * 8 + warp) * Plan::ROW;
+        constexpr int NEXT = NT * 8 * Plan::ROW;
         float top = -FLT_MAX, sum = 0.0f, f[WARPS];
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) top = fmaxf(top, row[w * NEXT + D]);
@@ -654,20 +669,36 @@ __device__ __forceinline__ int stages_of(const PackedAttention& p, int seq, int&
     return n > 0 ? max(1, (most - floor + STAGE - 1) / STAGE) : 0;
 }
 
-constexpr int EVEN_SEQS = 1024;  // most requests of a step whose stages are dealt out evenly
-constexpr int EVEN_STAGES = WARPS;  // fewest stages of a block, so that each warp has one
+constexpr int EVEN_SEQS = 1024;      // most requests of a step whose stages are dealt out evenly
+constexpr int EVEN_STAGES = WARPS;   // fewest stages of a block, so that each warp has one
+constexpr int EVEN_RUN = 4 * WARPS;  // stages of a block from which on a block may go on with the next request
 
-// Which parts hold the stages a .. b - 1 of `units` that are dealt out to `blocks` blocks: block i gets stages i units / blocks up to
-// (i + 1) units / blocks.  A block leaves the part that another block began in place 2 i, the part that it begins itself in 2 i + 1.
-__device__ __forceinline__ int block_of_unit(int u, int units, int blocks) { return (int)((((long long)u + 1) * blocks - 1) / units); }
+// How `units` stages are dealt out to about `most` blocks.  Long runs: block i gets stages i units / blocks up to (i + 1) units /
+// blocks, whosever they are, and every block the same.  Shorter ones, where a second request would cost a block its
+// start once more (8 requests of 4,096 rows: 15 us against 9): every request and kv head is cut into pieces of its own.
+struct Deal {
+    int units, blocks, chunk, runs;
 
-__device__ __forceinline__ int even_blocks(int units, int most) { return min(most, max(1, units / EVEN_STAGES)); }
+    __device__ __forceinline__ Deal(int units, int most) : units(units) {
+        blocks = min(most, max(1, units / EVEN_STAGES));
+        chunk = max(EVEN_STAGES, (units + most - 1) / most);
+        runs = chunk >= EVEN_RUN;
+    }
+    // blocks of a request's kv head (pieces)
+    __device__ __forceinline__ int pieces(int stages) const { return (stages + chunk - 1) / chunk; }
+    // the block that has unit u (runs)
+    __device__ __forceinline__ int block_of(int u) const { return (int)((((long long)u + 1) * blocks - 1) / units); }
+    __device__ __forceinline__ int begin_of(int block) const { return (int)((long long)block * units / blocks); }
+    // where block i leaves its part of a request whose first part is in block `first`: a run may have two parts, one that
+    // another block began and one that it begins itself
+    __device__ __forceinline__ int place(int i, int first) const { return runs ? 2 * i + (i == first) : i; }
+};
 
 // A warp joins the parts first .. last of one query row in their order.
 template <typename T, int D>
-__device__ __forceinline__ void join_row(const PackedAttention& p, int first, int last, int rows, int r, int token, int qh, int lane) {
+__device__ __forceinline__ void join_row(const PackedAttention& p, const Deal& deal, int first, int last, int rows, int r, int token, int qh, int lane) {
     constexpr int W = D / 32;
-    const auto at = [&](int i) { return p.parts + ((size_t)(2 * i + (i == first)) * rows + r) * (D + 2); };
+    const auto at = [&](int i) { return p.parts + ((size_t)deal.place(i, first) * rows + r) * (D + 2); };
     float top = -FLT_MAX;
     for (int i = first + lane; i <= last; i += 32) top = fmaxf(top, __ldcg(at(i) + D));
     top = warp_max(top);
@@ -692,19 +723,35 @@ __device__ __forceinline__ void join_row(const PackedAttention& p, int first, in
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 2 : 1) packed_attention_rows_kernel(const PackedAttention p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int before[EVEN_SEQS + 1];  // stages of the requests before each one
-    __shared__ int warp_total[WARPS], last_here;
+    __shared__ int before[EVEN_SEQS + 1];  // stages (or pieces) of the requests before each one
+    __shared__ int warp_total[2][WARPS], last_here;
     pdl_launch_dependents();
     pdl_wait();
-    const int c = threadIdx.x & 3, limit = p.width * p.cache.page_size;
+    const int c = threadIdx.x & 3, limit = p.width * p.cache.page_size, me = blockIdx.x;
     Segment<NT> seg;
-    if (p.even) {  // running sums: four requests a thread
+    Deal deal(WARPS, 1);
+    int u = 0, stop = 1, s = 0;
+    if (p.even) {
+        constexpr int EACH = EVEN_SEQS / (WARPS * 32);  // requests of a thread
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        int mine[EVEN_SEQS / (WARPS * 32)], sum = 0, floor;
+        int mine[EACH], sum = 0, floor;
 #pragma unroll
-        for (int i = 0; i < EVEN_SEQS / (WARPS * 32); ++i) {
-            const int s = threadIdx.x * (EVEN_SEQS / (WARPS * 32)) + i;
-            mine[i] = s < p.seqs ? stages_of(p, s, floor) * p.cache.kv_heads : 0;
+        for (int i = 0; i < EACH; ++i) {
+            const int at = threadIdx.x * EACH + i;
+            mine[i] = at < p.seqs ? stages_of(p, at, floor) : 0;
+            sum += mine[i];
+        }
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) warp_total[0][warp] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) sum += warp_total[0][w];
+        deal = Deal(sum * p.cache.kv_heads, p.most_blocks);
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            mine[i] = p.cache.kv_heads * (deal.runs ? mine[i] : deal.pieces(mine[i]));
             sum += mine[i];
         }
         int upto = sum;
@@ -713,36 +760,37 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
             const int v = __shfl_up_sync(0xffffffffu, upto, x);
             if (lane >= x) upto += v;
         }
-        if (lane == 31) warp_total[warp] = upto;
+        if (lane == 31) warp_total[1][warp] = upto;
         __syncthreads();
         upto -= sum;
-        for (int w = 0; w < warp; ++w) upto += warp_total[w];
+        for (int w = 0; w < warp; ++w) upto += warp_total[1][w];
 #pragma unroll
-        for (int i = 0; i < EVEN_SEQS / (WARPS * 32); ++i) {
-            before[threadIdx.x * (EVEN_SEQS / (WARPS * 32)) + i] = upto;
+        for (int i = 0; i < EACH; ++i) {
+            before[threadIdx.x * EACH + i] = upto;
             upto += mine[i];
         }
         if (threadIdx.x == WARPS * 32 - 1) before[EVEN_SEQS] = upto;
         __syncthreads();
-    }
-    int units = 0, blocks = 0, u = 0, stop = 1, s = 0;
-    const int me = blockIdx.x;
-    if (p.even) {
-        units = before[EVEN_SEQS], blocks = even_blocks(units, gridDim.x);
-        if (me >= blocks) return;
-        u = (int)((long long)me * units / blocks), stop = (int)((long long)(me + 1) * units / blocks);
+        if (me >= (deal.runs ? deal.blocks : before[EVEN_SEQS])) return;
+        u = deal.runs ? deal.begin_of(me) : me, stop = deal.runs ? deal.begin_of(me + 1) : me + 1;
     }
     while (u < stop) {
-        int stages = 1, begin = 0, take = 1, from = 0, split = 0;
+        int stages = 1, take = 1, from = 0, split = 0, first_part = 0, last_part = 0, done = 1;
         if (p.even) {
-            for (int step = EVEN_SEQS / 2; step; step >>= 1)  // the last request that begins at or before u (and has stages)
+            for (int step = EVEN_SEQS / 2; step; step >>= 1)  // the last request that begins at or before u (and has any)
                 if (s + step < EVEN_SEQS && before[s + step] <= u) s += step;
             int floor;
             stages = stages_of(p, s, floor);
-            const int rel = u - before[s];
-            seg.head = rel / stages, from = rel - seg.head * stages;
-            begin = u - from, take = min(stages - from, stop - u);
-            seg.first = 0;
+            const int rel = u - before[s], n = deal.runs ? stages : deal.pieces(stages);
+            seg.head = rel / n, seg.first = 0;
+            const int i = rel - seg.head * n;
+            if (deal.runs) {
+                from = i, take = done = min(stages - from, stop - u);
+                first_part = deal.block_of(u - from), last_part = deal.block_of(u - from + stages - 1);
+            } else {
+                from = (int)((long long)i * stages / n), take = (int)((long long)(i + 1) * stages / n) - from;
+                first_part = me - i, last_part = first_part + n - 1;
+            }
         } else {
             s = blockIdx.z / p.splits, split = blockIdx.z % p.splits, seg.head = blockIdx.y, seg.first = blockIdx.x * 8 * NT;
         }
@@ -758,33 +806,32 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
         }
         seg.base = floor + from * STAGE, seg.end = min(seg.rows.most, seg.base + take * STAGE);
         const bool shared = p.even && take < stages;
-        seg.part = shared ? p.parts + (size_t)(2 * me + (from == 0)) * (8 * NT) * (D + 2)
+        seg.part = shared ? p.parts + (size_t)deal.place(me, first_part) * (8 * NT) * (D + 2)
                           : !p.even && p.splits > 1 ? p.parts + (size_t)split * p.tokens * p.heads * (D + 2) : nullptr;
         seg.row_stride = p.even ? D + 2 : 0;
         attend_segment<T, D, NT>(p, seg, smem);
         if (shared && p.counters) {
-            const int first = block_of_unit(begin, units, blocks), last = block_of_unit(begin + stages - 1, units, blocks);
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
                 int* counter = p.counters + s * p.cache.kv_heads + head;
-                last_here = atomicAdd(counter, 1) == last - first;
+                last_here = atomicAdd(counter, 1) == last_part - first_part;
                 if (last_here) *counter = 0;  // for the next launch
                 __threadfence();
             }
             __syncthreads();
             if (last_here)
                 for (int r = threadIdx.x >> 5; r < seg.count; r += WARPS)
-                    join_row<T, D>(p, first, last, 8 * NT, r, seg.t0 + r / p.group, head * p.group + r % p.group, threadIdx.x & 31);
+                    join_row<T, D>(p, deal, first_part, last_part, 8 * NT, r, seg.t0 + r / p.group, head * p.group + r % p.group, threadIdx.x & 31);
         }
         if (!p.even) return;
         __syncthreads();  // shared memory is free again
-        u += take;
+        u += done;
     }
     if (!p.counters && me == 0) {  // what the joining kernel needs
         int* to = (int*)(p.parts + (size_t)2 * gridDim.x * (8 * NT) * (D + 2));
         for (int i = threadIdx.x; i <= p.seqs; i += WARPS * 32) to[i] = before[i];
-        if (threadIdx.x == 0) to[p.seqs + 1] = blocks;
+        if (threadIdx.x == 0) to[p.seqs + 1] = deal.units;
     }
 }
 
@@ -799,11 +846,11 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_join_even_kernel(
     const int* before = (const int*)(p.parts + (size_t)2 * grid * rows * (D + 2));
     const int t0 = max(p.q_start[s], 0), count = (min(p.q_start[s + 1], p.tokens) - t0) * p.group;
     if (r >= count) return;
-    const int units = before[p.seqs], blocks = before[p.seqs + 1], stages = (before[s + 1] - before[s]) / p.cache.kv_heads;
-    const int begin = before[s] + head * stages;
-    const int first = block_of_unit(begin, units, blocks), last = block_of_unit(begin + stages - 1, units, blocks);
+    const Deal deal(before[p.seqs + 1], p.most_blocks);
+    const int n = (before[s + 1] - before[s]) / p.cache.kv_heads, begin = before[s] + head * n;
+    const int first = deal.runs ? deal.block_of(begin) : begin, last = deal.runs ? deal.block_of(begin + n - 1) : begin + n - 1;
     if (first == last) return;  // one block had all of it
-    const auto at = [&](int i) { return p.parts + ((size_t)(2 * i + (i == first)) * rows + r) * (D + 2); };
+    const auto at = [&](int i) { return p.parts + ((size_t)deal.place(i, first) * rows + r) * (D + 2); };
     float top = -FLT_MAX;
     for (int i = first + threadIdx.x; i <= last; i += WARPS * 32) top = fmaxf(top, at(i)[D]);
     top = warp_max(top);
@@ -923,7 +970,7 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
         if (rows.most <= at) continue;
         Queries<T, W, NP> q[1];
         const int r = first + g;
-        q[0].load((const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D, c, r < count);
+        q[0].load((const T*)p.q + (size_t)(t0 + r / p.group) * p.ldq + (size_t)(head * p.group + r % p.group) * D, c, r < count, p.q_aligned);
         const float inv = p.scale / q[0].factor;
         float qs[2], lse[2];
 #pragma unroll
@@ -959,8 +1006,10 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
 
 // How a step is cut: tiles of eight query rows that a block takes, whether all rows of a request fit them, and the blocks or splits.
 struct Plan {
-    int tiles, even, blocks, splits, join_kernel;
-    long long part_floats, score_floats;
+    int tiles, even, most, blocks, splits, join_kernel;
+    long long lse_floats, part_floats, score_floats, counters;
+
+    long long scratch() const { return lse_floats + part_floats + score_floats; }
 };
 
 // Tiles: two where there are more rows than eight and the registers hold them.
@@ -973,11 +1022,14 @@ Plan make_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int t
     const long long stages = max_kv / STAGE + 2, pairs = (long long)seqs * kv_heads;
     q.even = rows <= 8 * q.tiles && seqs <= EVEN_SEQS && pairs * stages < 0x7fffffff;
     q.splits = 1;
+    q.lse_floats = weights ? ((long long)tokens * kv_heads * group + 3) / 4 * 4 : 0;  // (what follows begins on 16 bytes)
     if (q.even) {
         const long long most = pairs * stages / EVEN_STAGES;
-        q.blocks = (int)(most < 1 ? 1 : most < sms * per_sm ? most : sms * per_sm);
-        q.join_kernel = q.blocks > 16 * pairs;  // so many parts of a request that one block would be long at joining them
-        q.part_floats = 2ll * q.blocks * 8 * q.tiles * (head_dim + 2) + (q.join_kernel ? seqs + 2 : 0);
+        q.most = (int)(most < 1 ? 1 : most < sms * per_sm ? most : sms * per_sm);
+        q.blocks = q.most + (int)pairs;  // (pieces: each request and kv head may have one that is not full)
+        q.join_kernel = q.most > 16 * pairs;  // so many parts of a request that one block would be long at joining them
+        q.part_floats = (2ll * q.blocks * 8 * q.tiles * (head_dim + 2) + (q.join_kernel ? seqs + 2 : 0) + 3) / 4 * 4;
+        q.counters = q.join_kernel ? 0 : pairs;
         q.score_floats = weights ? pairs * stages * STAGE * 8 * q.tiles : 0;
         if (q.score_floats > (1ll << 27)) q.score_floats = 0;  // (above 512 MB the scores are formed again)
     } else {
@@ -1037,47 +1089,62 @@ int attend_dim(const PackedAttention& p, const Plan& q, int max_q, int max_kv, c
 
 }  // namespace
 
-// What scratch a step needs: floats of parts and of scores, counters (whole numbers that are nought, and are left so).
+// What a step needs: floats of scratch, counters (whole numbers that are nought, and are left so), launches.
 FERRIS_API int ferris_packed_attention_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int tokens, int max_q, int max_kv,
-                                            int weights, long long* floats) {
+                                            int weights, long long* needs) {
     const Plan q = make_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_q, max_kv, weights);
-    floats[0] = q.part_floats;
-    floats[1] = q.score_floats;
-    floats[2] = q.even && !q.join_kernel ? (long long)seqs * kv_heads : 0;
+    needs[0] = q.scratch();
+    needs[1] = q.counters;
+    needs[2] = 1 + (q.join_kernel || q.splits > 1) + (weights ? 1 : 0);
     return FERRIS_OK;
 }
 
-FERRIS_API int ferris_packed_attention(const void* q, int ldq, void* out, int ldo, int dtype, void* k_codes, void* k_scales, void* v_codes,
-                                       void* v_scales, int pages, int kv_heads, int page_size, int head_dim, const int* tables, int width,
-                                       const int* q_start, const int* start_row, int seqs, int tokens, int heads, int max_q, int max_kv,
-                                       int window, float scale, float* lse, float* parts, float* scores, int* counters, float* weights,
-                                       const int* seq_slot, long long slot_stride, int head_stride, int max_rows, int add, void* stream) {
+// The arguments of ferris_packed_attention, as its caller lays them out: a call of this many arguments would cost its host
+// more than the launch.
+struct FerrisPackedAttention {
+    const void* q;
+    void *out, *k_codes, *k_scales, *v_codes, *v_scales;
+    const int *tables, *q_start, *start_row;
+    float* scratch;  // sums of the softmax (with weights), parts, scores, in this order
+    int* counters;
+    float* weights;
+    const int* seq_slot;
+    void* stream;
+    long long slot_stride;
+    int ldq, ldo, dtype, pages, kv_heads, page_size, head_dim, width, seqs, tokens, heads, max_q, max_kv, window, head_stride, max_rows, add;
+    float scale;
+};
+
+FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
     PackedAttention p = {};
-    p.cache = {(uint8_t*)k_codes, (uint32_t*)k_scales, (uint8_t*)v_codes, (uint32_t*)v_scales, pages, kv_heads, page_size, head_dim};
+    p.cache = {(uint8_t*)a->k_codes, (uint32_t*)a->k_scales, (uint8_t*)a->v_codes, (uint32_t*)a->v_scales, a->pages, a->kv_heads, a->page_size,
+               a->head_dim};
     if (const char* why = packed_cache_refusal(p.cache)) FERRIS_REFUSE("%s", why);
-    if (heads <= 0 || heads % kv_heads) FERRIS_REFUSE("packed attention: %d heads over %d kv heads", heads, kv_heads);
-    if (window < 0 || width <= 0) FERRIS_REFUSE("packed attention: window %d, %d blocks", window, width);
-    if (weights && !lse) FERRIS_REFUSE("packed attention: weights without scratch");
-    if (seqs <= 0 || tokens <= 0 || max_q <= 0) return FERRIS_OK;
-    if ((long long)width * page_size > 0x7fffffff - 16 * WARPS * STAGE) FERRIS_REFUSE("packed attention: %d blocks of %d rows", width, page_size);
-    const Plan plan = make_plan(dtype, head_dim, seqs, kv_heads, heads / kv_heads, tokens, max_q, max_kv, weights != nullptr);
-    if (plan.part_floats && !parts) FERRIS_REFUSE("packed attention: no scratch for its parts");
-    if (plan.even && !plan.join_kernel && !counters) FERRIS_REFUSE("packed attention: no counters");
-    if (kv_heads > 65535 || (!plan.even && (long long)seqs * plan.splits > 65535) || seqs > 65535)
-        FERRIS_REFUSE("packed attention: %d requests of %d kv heads", seqs, kv_heads);
-    p.q = q, p.out = out, p.ldq = ldq, p.ldo = ldo;
-    p.tables = tables, p.width = width, p.q_start = q_start, p.start_row = start_row;
-    p.seqs = seqs, p.heads = heads, p.group = heads / kv_heads, p.window = window, p.scale = scale * LOG2E;
-    p.lse = lse, p.parts = parts, p.splits = plan.splits, p.tokens = tokens;
-    p.even = plan.even, p.counters = plan.join_kernel ? nullptr : counters, p.scores = plan.score_floats ? scores : nullptr;
-    p.max_stages = max_kv / STAGE + 2;
-    if (page_size > 1) {
-        while ((2 << p.page_shift) < page_size) ++p.page_shift;
-        p.page_mul = (uint32_t)(((1ull << (32 + p.page_shift)) + page_size - 1) / page_size);
+    if (a->heads <= 0 || a->heads % a->kv_heads) FERRIS_REFUSE("packed attention: %d heads over %d kv heads", a->heads, a->kv_heads);
+    if (a->window < 0 || a->width <= 0) FERRIS_REFUSE("packed attention: window %d, %d blocks", a->window, a->width);
+    if (a->seqs <= 0 || a->tokens <= 0 || a->max_q <= 0) return FERRIS_OK;
+    if ((long long)a->width * a->page_size > 0x7fffffff - 16 * WARPS * STAGE) FERRIS_REFUSE("packed attention: %d blocks of %d rows", a->width, a->page_size);
+    const Plan plan = make_plan(a->dtype, a->head_dim, a->seqs, a->kv_heads, a->heads / a->kv_heads, a->tokens, a->max_q, a->max_kv, a->weights != nullptr);
+    if (plan.scratch() && !a->scratch) FERRIS_REFUSE("packed attention: no scratch");
+    if (plan.counters && !a->counters) FERRIS_REFUSE("packed attention: no counters");
+    if (a->kv_heads > 65535 || (!plan.even && (long long)a->seqs * plan.splits > 65535) || a->seqs > 65535)
+        FERRIS_REFUSE("packed attention: %d requests of %d kv heads", a->seqs, a->kv_heads);
+    p.q = a->q, p.out = a->out, p.ldq = a->ldq, p.ldo = a->ldo;
+    p.q_aligned = ((uintptr_t)a->q & 15) == 0 && (long long)a->ldq * (a->dtype == FERRIS_BF16 ? 2 : 4) % 16 == 0;
+    p.tables = a->tables, p.width = a->width, p.q_start = a->q_start, p.start_row = a->start_row;
+    p.seqs = a->seqs, p.heads = a->heads, p.group = a->heads / a->kv_heads, p.window = a->window, p.scale = a->scale * LOG2E;
+    p.lse = plan.lse_floats ? a->scratch : nullptr, p.parts = a->scratch + plan.lse_floats;
+    p.scores = plan.score_floats ? a->scratch + plan.lse_floats + plan.part_floats : nullptr;
+    p.splits = plan.splits, p.tokens = a->tokens;
+    p.even = plan.even, p.most_blocks = plan.most, p.counters = plan.counters ? a->counters : nullptr;
+    p.max_stages = a->max_kv / STAGE + 2;
+    if (a->page_size > 1) {
+        while ((2 << p.page_shift) < a->page_size) ++p.page_shift;
+        p.page_mul = (uint32_t)(((1ull << (32 + p.page_shift)) + a->page_size - 1) / a->page_size);
     }
-    p.weights = weights, p.seq_slot = seq_slot, p.slot_stride = slot_stride, p.head_stride = head_stride, p.max_rows = max_rows, p.add = add;
+    p.weights = a->weights, p.seq_slot = a->seq_slot, p.slot_stride = a->slot_stride, p.head_stride = a->head_stride, p.max_rows = a->max_rows, p.add = a->add;
     p.status = ferris_status_ptr();
-    if (dtype == FERRIS_BF16) return attend_dim<bf16>(p, plan, max_q, max_kv, (cudaStream_t)stream);
-    if (dtype == FERRIS_F32) return attend_dim<float>(p, plan, max_q, max_kv, (cudaStream_t)stream);
-    FERRIS_REFUSE("packed attention: dtype %d is not known", dtype);
+    if (a->dtype == FERRIS_BF16) return attend_dim<bf16>(p, plan, a->max_q, a->max_kv, (cudaStream_t)a->stream);
+    if (a->dtype == FERRIS_F32) return attend_dim<float>(p, plan, a->max_q, a->max_kv, (cudaStream_t)a->stream);
+    FERRIS_REFUSE("packed attention: dtype %d is not known", a->dtype);
 }

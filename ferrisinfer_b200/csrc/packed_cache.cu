@@ -328,26 +328,30 @@ int read_rows(const PackedCache& cache, const int* slots, void* k, void* v, int 
 
 }  // namespace
 
-FERRIS_API int ferris_packed_cache_write(const void* k, const void* v, int dtype, int ldk, int ldv, const int* slots, void* k_codes,
-                                         void* k_scales, void* v_codes, void* v_scales, int pages, int kv_heads, int page_size,
-                                         int head_dim, int tokens, void* stream) {
-    const PackedCache cache = make_cache(k_codes, k_scales, v_codes, v_scales, pages, kv_heads, page_size, head_dim);
-    if (const char* why = packed_cache_refusal(cache)) FERRIS_REFUSE("%s", why);
-    if (tokens <= 0) return FERRIS_OK;
-    if (dtype == FERRIS_BF16) return write_rows<bf16>(k, v, ldk, ldv, slots, cache, tokens, (cudaStream_t)stream);
-    if (dtype == FERRIS_F32) return write_rows<float>(k, v, ldk, ldv, slots, cache, tokens, (cudaStream_t)stream);
-    FERRIS_REFUSE("packed cache: dtype %d is not known", dtype);
+// The arguments of the two below, as their caller lays them out.
+struct FerrisPackedRows {
+    void *k, *v;
+    const int* slots;
+    void *k_codes, *k_scales, *v_codes, *v_scales, *stream;
+    int dtype, ldk, ldv, pages, kv_heads, page_size, head_dim, tokens;
+
+    PackedCache cache() const { return make_cache(k_codes, k_scales, v_codes, v_scales, pages, kv_heads, page_size, head_dim); }
+};
+
+FERRIS_API int ferris_packed_cache_write(const FerrisPackedRows* a) {
+    if (const char* why = packed_cache_refusal(a->cache())) FERRIS_REFUSE("%s", why);
+    if (a->tokens <= 0) return FERRIS_OK;
+    if (a->dtype == FERRIS_BF16) return write_rows<bf16>(a->k, a->v, a->ldk, a->ldv, a->slots, a->cache(), a->tokens, (cudaStream_t)a->stream);
+    if (a->dtype == FERRIS_F32) return write_rows<float>(a->k, a->v, a->ldk, a->ldv, a->slots, a->cache(), a->tokens, (cudaStream_t)a->stream);
+    FERRIS_REFUSE("packed cache: dtype %d is not known", a->dtype);
 }
 
-FERRIS_API int ferris_packed_cache_read(void* k, void* v, int dtype, int ldk, int ldv, const int* slots, void* k_codes, void* k_scales,
-                                        void* v_codes, void* v_scales, int pages, int kv_heads, int page_size, int head_dim, int tokens,
-                                        void* stream) {
-    const PackedCache cache = make_cache(k_codes, k_scales, v_codes, v_scales, pages, kv_heads, page_size, head_dim);
-    if (const char* why = packed_cache_refusal(cache)) FERRIS_REFUSE("%s", why);
-    if (tokens <= 0) return FERRIS_OK;
-    if (dtype == FERRIS_BF16) return read_rows<bf16>(cache, slots, k, v, ldk, ldv, tokens, (cudaStream_t)stream);
-    if (dtype == FERRIS_F32) return read_rows<float>(cache, slots, k, v, ldk, ldv, tokens, (cudaStream_t)stream);
-    FERRIS_REFUSE("packed cache: dtype %d is not known", dtype);
+FERRIS_API int ferris_packed_cache_read(const FerrisPackedRows* a) {
+    if (const char* why = packed_cache_refusal(a->cache())) FERRIS_REFUSE("%s", why);
+    if (a->tokens <= 0) return FERRIS_OK;
+    if (a->dtype == FERRIS_BF16) return read_rows<bf16>(a->cache(), a->slots, a->k, a->v, a->ldk, a->ldv, a->tokens, (cudaStream_t)a->stream);
+    if (a->dtype == FERRIS_F32) return read_rows<float>(a->cache(), a->slots, a->k, a->v, a->ldk, a->ldv, a->tokens, (cudaStream_t)a->stream);
+    FERRIS_REFUSE("packed cache: dtype %d is not known", a->dtype);
 }
 
 FERRIS_API int ferris_packed_cache_evict(void* from_kc, void* from_ks, void* from_vc, void* from_vs, int from_pages, int from_page_size,

@@ -12,6 +12,8 @@ last error) without locks: one thread at a time may call into it, which is how t
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from typing import Optional
 
 import torch
@@ -46,13 +48,12 @@ _SIGNATURES = {
     "ferris_gemm_skinny": [_VP, _I, _VP, _VP, _F, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
     "ferris_gemm_skinny_takes": [_I, _I, _I, _I, _I],
     "ferris_embed_gather": [_VP, _I, _VP, _VP, _I, _I, _I, _VP, _VP],
-    "ferris_packed_cache_write": [_VP, _VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP],
-    "ferris_packed_cache_read": [_VP, _VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP],
+    "ferris_packed_cache_write": [_VP],
+    "ferris_packed_cache_read": [_VP],
     "ferris_packed_cache_evict": [_VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _I, _VP, _I, _VP, _VP, _VP, _LL, _I, _I,
                                   _VP, _VP, _LL, _I, _I, _I, _I, _I, _VP],
     "ferris_packed_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
-    "ferris_packed_attention": [_VP, _I, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _VP,
-                                _VP, _VP, _VP, _VP, _VP, _LL, _I, _I, _I, _VP],
+    "ferris_packed_attention": [_VP],
 }
 _declared = False
 
@@ -2376,7 +2377,7 @@ class PackedPages:
     [pages, kv heads, page size, head size / 32, 2], (scale, least) of each group.  A row takes 5 bits an element, scales
     included, against 16 of a cache in bf16."""
 
-    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "pages", "kv_heads", "page_size", "head_dim", "_args")
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "pages", "kv_heads", "page_size", "head_dim", "width", "device_index", "_args")
 
     def __init__(self, k_codes, k_scales, v_codes, v_scales):
         for t, what, dtype in ((k_codes, "packed key codes", torch.uint8), (k_scales, "packed key scales", torch.bfloat16),
@@ -2395,6 +2396,7 @@ class PackedPages:
         if any(t.device != k_codes.device for t in (k_scales, v_codes, v_scales)):
             raise KernelError("packed cache: its four tensors must be on one device")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self.width, self.device_index = self.kv_heads * self.head_dim, k_codes.get_device()
         self._args = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
 
     @classmethod
@@ -2412,18 +2414,42 @@ class PackedPages:
         return 2 * kv_heads * (head_dim // 2 + 4 * (head_dim // PACKED_GROUP))
 
 
-def _packed_rows(k, v, slot_mapping, pages: PackedPages, what: str):
-    """Checks rows of keys and values that go with ``pages``; their strides."""
-    T, n, ldk = _rows(k, f"{what}: keys")
-    T2, n2, ldv = _rows(v, f"{what}: values")
-    _need(slot_mapping, f"{what}: slot mapping", torch.int32)
-    width = pages.kv_heads * pages.head_dim
-    if T != T2 or n != width or n2 != width or k.dtype != v.dtype or slot_mapping.numel() != T:
-        raise KernelError(f"{what}: keys {tuple(k.shape)} {k.dtype}, values {tuple(v.shape)} {v.dtype}, {slot_mapping.numel()} slots for "
+# Arguments of a call laid out for the library in one go (ctypes converts them one by one, which costs more than a launch).  The
+# library is called by one thread at a time.
+_PACKED_ROWS = struct.Struct("=8Q8i")
+_PACKED_ATTENTION = struct.Struct("=14Qq17if")
+_packed_buffer = ctypes.create_string_buffer(max(_PACKED_ROWS.size, _PACKED_ATTENTION.size))
+_packed_buffer_at = ctypes.addressof(_packed_buffer)
+
+
+def _current_stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _row_stride(t, rows: int, width: int) -> int:
+    return t.stride(0) if rows > 1 else max(t.stride(0), width)
+
+
+def _packed_rows(k, v, slot_mapping, pages: PackedPages, what: str) -> int:
+    """Lays out rows of keys and values that go with ``pages``, or raises; how many."""
+    width, dev = pages.width, pages.device_index
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(slot_mapping, torch.Tensor)
+            and k.get_device() == v.get_device() == slot_mapping.get_device() == dev):
+        raise KernelError(f"{what}: keys, values and slots must be CUDA tensors on the cache's device (there is no CPU path)")
+    T, dtype = slot_mapping.numel(), k.dtype
+    if k.shape != (T, width) or v.shape != (T, width) or v.dtype != dtype:
+        raise KernelError(f"{what}: keys {tuple(k.shape)} {k.dtype}, values {tuple(v.shape)} {v.dtype}, {T} slots for "
                           f"{pages.kv_heads} heads of {pages.head_dim}")
-    if any(t.device != pages.k_codes.device for t in (k, v, slot_mapping)):
-        raise KernelError(f"{what}: keys, values, slots and cache must be on one device")
-    return T, ldk, ldv
+    if k.stride(1) != 1 or v.stride(1) != 1:
+        raise KernelError(f"{what}: keys and values need contiguous rows, found strides {k.stride()} and {v.stride()}")
+    if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous():
+        raise KernelError(f"{what}: slot mapping must be contiguous and {torch.int32}, found {slot_mapping.dtype}")
+    if dtype not in _DT:
+        raise KernelError(f"{what}: dtype {dtype} is not supported (float32 or bfloat16)")
+    _PACKED_ROWS.pack_into(_packed_buffer, 0, k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), *pages._args, _current_stream(), _DT[dtype],
+                           _row_stride(k, T, width), _row_stride(v, T, width), pages.pages, pages.kv_heads, pages.page_size,
+                           pages.head_dim, T)
+    return T
 
 
 def packed_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, pages: PackedPages):
@@ -2431,23 +2457,15 @@ def packed_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Ten
     the rows ``slot_mapping`` (int32 [T], page * page_size + offset; below 0: the token is left out) of the packed cache.  Per
     group of 32: least = its minimum rounded down to bf16, scale = bf16((maximum - least) / 15), code = (x - least) / scale
     rounded to even; a group with NaN or infinity stands as NaN.  Two tokens with one slot leave one of them."""
-    T, ldk, ldv = _packed_rows(k, v, slot_mapping, pages, "packed cache write")
-    if T == 0:
-        return
-    _check(_lib().ferris_packed_cache_write(k.data_ptr(), v.data_ptr(), _dt(k, "keys"), ldk, ldv, slot_mapping.data_ptr(), *pages._args,
-                                            pages.pages, pages.kv_heads, pages.page_size, pages.head_dim, T, _stream()),
-           "packed cache write")
+    if _packed_rows(k, v, slot_mapping, pages, "packed cache write"):
+        _check(_lib().ferris_packed_cache_write(_packed_buffer_at), "packed cache write")
 
 
 def packed_cache_read(pages: PackedPages, slot_mapping: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     """k[t], v[t] [kv heads x head size] = the values that row ``slot_mapping[t]`` of the packed cache stands for, rounded once
     to their type (zeros where the slot is below 0)."""
-    T, ldk, ldv = _packed_rows(k, v, slot_mapping, pages, "packed cache read")
-    if T == 0:
-        return
-    _check(_lib().ferris_packed_cache_read(k.data_ptr(), v.data_ptr(), _dt(k, "keys"), ldk, ldv, slot_mapping.data_ptr(), *pages._args,
-                                           pages.pages, pages.kv_heads, pages.page_size, pages.head_dim, T, _stream()),
-           "packed cache read")
+    if _packed_rows(k, v, slot_mapping, pages, "packed cache read"):
+        _check(_lib().ferris_packed_cache_read(_packed_buffer_at), "packed cache read")
 
 
 def _weight_rows(weights, kv_heads: int, what: str) -> tuple:
@@ -2474,51 +2492,61 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
     ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` for request s, row s without it): every cached row's weight
     in the softmax, summed over the request's queries and the query heads of the kv head, is added to it; the rows that
     came with this step (and with ``add_weights`` False all of them) are set instead."""
-    T, cols, ldq = _rows(q, "packed attention queries")
-    T2, width, ldo = _rows(out, "packed attention output")
-    _need(block_tables, "block tables", torch.int32)
-    _need(seq_q_start, "first query rows", torch.int32)
-    _need(seq_start_row, "rows held before the step", torch.int32)
-    S, D = seq_start_row.numel(), pages.head_dim
-    if num_heads <= 0 or num_heads % pages.kv_heads:
-        raise KernelError(f"packed attention: {num_heads} heads cannot share {pages.kv_heads} kv heads")
-    if T != T2 or cols < num_heads * D or width != num_heads * D or out.dtype != q.dtype:
+    dev, D, hkv = pages.device_index, pages.head_dim, pages.kv_heads
+    for t in (q, out, block_tables, seq_q_start, seq_start_row):
+        if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+            raise KernelError("packed attention: all tensors must be CUDA tensors on the cache's device (there is no CPU path)")
+    for t in (block_tables, seq_q_start, seq_start_row):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError("packed attention: block tables, first query rows and rows held before the step must be contiguous and "
+                              f"{torch.int32}, found {t.dtype}")
+    S, dtype = seq_start_row.numel(), q.dtype
+    if num_heads <= 0 or num_heads % hkv:
+        raise KernelError(f"packed attention: {num_heads} heads cannot share {hkv} kv heads")
+    if q.dim() != 2 or out.shape != (q.shape[0], num_heads * D) or q.shape[1] < num_heads * D or out.dtype != dtype:
         raise KernelError(f"packed attention: q {tuple(q.shape)} {q.dtype}, out {tuple(out.shape)} {out.dtype} for {num_heads} heads of {D}")
+    T = q.shape[0]
+    if dtype not in _DT:
+        raise KernelError(f"packed attention: dtype {dtype} is not supported (float32 or bfloat16)")
+    if q.stride(1) != 1 or out.stride(1) != 1:
+        raise KernelError(f"packed attention: queries and outputs need contiguous rows, found strides {q.stride()} and {out.stride()}")
     if block_tables.dim() != 2 or block_tables.shape[0] != S or seq_q_start.numel() != S + 1:
         raise KernelError(f"packed attention: tables {tuple(block_tables.shape)}, {seq_q_start.numel()} first rows for {S} requests")
     if max_q_len < 0 or max_kv_len < 0 or window < 0:
         raise KernelError(f"packed attention: at most {max_q_len} queries, {max_kv_len} rows, window {window}")
-    if any(t.device != pages.k_codes.device for t in (q, out, block_tables, seq_q_start, seq_start_row)):
-        raise KernelError("packed attention: all tensors must be on the cache's device")
-    dt = _dt(q, "packed attention queries")
-    w = (None, None, 0, 0, 0)
+    w = (0, 0, 0, 0, 0)
     if weights is not None:
-        slots, rows, slot_stride, head_stride = _weight_rows(weights, pages.kv_heads, "packed attention weights")
+        slots, rows, slot_stride, head_stride = _weight_rows(weights, hkv, "packed attention weights")
         if seq_slot is not None:
             _need(seq_slot, "slots of the weights", torch.int32)
-        if (seq_slot.numel() != S if seq_slot is not None else slots < S) or rows < max_kv_len or weights.device != q.device:
+        if (seq_slot.numel() != S if seq_slot is not None else slots < S) or rows < max_kv_len or weights.get_device() != dev:
             raise KernelError(f"packed attention: weights {tuple(weights.shape)} for {S} requests of at most {max_kv_len} rows")
-        w = (weights.data_ptr(), None if seq_slot is None else seq_slot.data_ptr(), slot_stride, head_stride, rows)
+        w = (weights.data_ptr(), 0 if seq_slot is None else seq_slot.data_ptr(), slot_stride, head_stride, rows)
     if T == 0 or S == 0 or max_q_len == 0:
         return
     if block_tables.shape[1] == 0:
         out.zero_()
         return
-    lib = _lib()
-    plan = (_LL * 3)()
-    lib.ferris_packed_attention_plan(dt, D, S, pages.kv_heads, num_heads // pages.kv_heads, T, max_q_len, max_kv_len,
-                                     0 if weights is None else 1, plan)
     if workspace is None:
         raise KernelError("packed attention: a workspace is needed")
-    parts, scores, counters = plan[0], plan[1], plan[2]
-    scratch = (workspace.get("packed_attention_lse", (T * num_heads,), torch.float32).data_ptr() if weights is not None else None,
-               workspace.get("packed_attention_parts", (parts,), torch.float32).data_ptr() if parts else None,
-               workspace.get("packed_attention_scores", (scores,), torch.float32).data_ptr() if scores else None,
-               workspace.get("packed_attention_counters", (counters,), torch.int32, zeroed=True).data_ptr() if counters else None)
-    _check(lib.ferris_packed_attention(q.data_ptr(), ldq, out.data_ptr(), ldo, dt, *pages._args, pages.pages, pages.kv_heads, pages.page_size, D,
-                                       block_tables.data_ptr(), block_tables.shape[1], seq_q_start.data_ptr(), seq_start_row.data_ptr(), S, T,
-                                       num_heads, max_q_len, max_kv_len, window, scale, *scratch, *w, 1 if add_weights else 0, _stream()),
-           "packed attention", 1 + (parts > 0 and not counters) + (weights is not None))
+    sizes = (_DT[dtype], D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, 0 if weights is None else 1)
+    scratch, counters, launches = _packed_attention_plan(sizes, dev)
+    scratch_at = workspace.get("packed_attention", (scratch,), torch.float32).data_ptr() if scratch else 0
+    counters_at = workspace.get("packed_attention_counters", (counters,), torch.int32, zeroed=True).data_ptr() if counters else 0
+    _PACKED_ATTENTION.pack_into(
+        _packed_buffer, 0, q.data_ptr(), out.data_ptr(), *pages._args, block_tables.data_ptr(), seq_q_start.data_ptr(), seq_start_row.data_ptr(),
+        scratch_at, counters_at, w[0], w[1], _current_stream(), w[2], _row_stride(q, T, num_heads * D), _row_stride(out, T, num_heads * D), _DT[dtype],
+        pages.pages, hkv, pages.page_size, D, block_tables.shape[1], S, T, num_heads, max_q_len, max_kv_len, window, w[3], w[4],
+        1 if add_weights else 0, scale)
+    _check(_lib().ferris_packed_attention(_packed_buffer_at), "packed attention", launches)
+
+
+@functools.lru_cache(maxsize=4096)
+def _packed_attention_plan(sizes: tuple, device: int) -> tuple:
+    """Floats of scratch, counters and launches of a step of these sizes on a GPU."""
+    needs = (_LL * 3)()
+    _lib().ferris_packed_attention_plan(*sizes, needs)
+    return tuple(needs)
 
 
 def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows: torch.Tensor, weights: torch.Tensor,

@@ -6,7 +6,7 @@
 //   S^T = K Q^T   per group j of 32 elements:  s[key][q] += scale_j[key] (codes_j[key] . q_j) + least_j[key] sum(q_j)
 //   O^T = V^T P^T per group j:                 o[elem][q] += codes_j[elem][key] (p[key][q] scale_j[key]), and least_j[key] p[key][q] in 32 bits
 // so that keys and values are never formed.  A word of eight codes becomes four operands of fp16 pairs with an AND / OR (1024 + code
-// or, from the upper four bits of a byte, 1024 + 16 code) and a subtraction each; values subtract 8 more and add 8 scale to their
+// or, from the upper four bits of a byte, 1024 + 16 code) and a subtraction (or a multiply-add) each; values subtract 8 more and add 8 scale to their
 // least, so that what the sums hold is of the size of the result (unsigned codes add up to something that least nearly cancels:
 // over 32,768 rows the accumulators' rounding alone came to 0.0015 of the output).  What meets the codes is scaled by powers of two into the
 // range of fp16: a query row by its greatest element (bf16 rows then lose nothing that 32 bits would keep; 32-bit rows go in
@@ -14,81 +14,19 @@
 // 32-bit ones.  (In bf16's eight bits the outputs were off by 0.0025 to 0.005 of their norm, 0.0016 of which is their own rounding;
 // codes as fp16 numbers below the normal range need no subtraction, but the tensor cores align their products as if they
 // were large: 3e-5 of a 32-bit output.)
-#include <cuda_fp16.h>
-#include <float.h>
-
-#include "packed_cache.cuh"
+#include "packed_attention.cuh"
 
 namespace {
 
 constexpr int KEYS = 16;   // cached rows of an MMA
 constexpr int STAGE = 32;  // cached rows that a warp fetches at once
 constexpr int WARPS = 8;
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct PackedAttention {
-    const void* q;
-    void* out;
-    int ldq, ldo, q_aligned;  // rows of q on 16 bytes
-    PackedCache cache;
-    const int* tables;
-    int width;  // blocks of a request's table
-    const int* q_start;
-    const int* start_row;
-    int seqs, heads, group, window;
-    float scale;  // of the scores, times log2(e)
-    float* lse;   // log2 of the softmax's sum of every (token, head), or nullptr
-    float* parts;  // unnormalised outputs, maximum and sum (D + 2 floats) of every query row, by [split][token][head] or [part][row]
-    int splits, tokens;
-    int even;       // the stages of all requests are dealt out evenly (steps whose rows fit one block) ...
-    int most_blocks;  // ... to about so many blocks
-    int* counters;  // per (request, kv head): blocks that have left their part (even), or nullptr: a kernel joins
-    float* scores;  // [request][kv head][stage][32][8 NT], to the base of 2, or nullptr
-    int max_stages;
-    uint32_t page_mul;  // division by the page size
-    int page_shift;
-    float* weights;
-    const int* seq_slot;
-    long long slot_stride;
-    int head_stride, max_rows, add;
-    int* status;
-
-    // row / page_size for rows below 2^31: page_mul = ceil(2^(32 + shift) / page_size) with 2^shift < page_size <= 2^(shift + 1)
-    __device__ __forceinline__ int block_of(int row) const { return page_mul ? (int)(__umulhi((uint32_t)row, page_mul) >> page_shift) : row; }
-    // Index of a row of the cache: below 2^32, which the C entry sees to.
-    __device__ __forceinline__ uint32_t row_of(int page, int head, int row, int block) const {
-        return (uint32_t)(page * cache.kv_heads + head) * cache.page_size + (uint32_t)(row - block * cache.page_size);
-    }
-};
-
-// The page of a request's row, -1 where it has none.
-__device__ __forceinline__ int page_of(const PackedAttention& p, const int* table, int block) {
-    const int page = block < p.width ? table[block] : -1;
-    if (page >= p.cache.pages) {
-        ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 83);
-        return -1;
-    }
-    return page;
-}
-
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// The exponential unit alone: results below the normal range become nought.
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
 }
 
 // 16 (or 8, or 4) bytes global -> shared without registers; `live` false: zeros, and nothing is read.
@@ -104,22 +42,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int LEFT>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-
-// The four pairs of a word of codes, each an operand register: places i and i + 4 (keys), or the two halves' i (values); the odd
-// ones times 16, all of them less `OFF`.
-template <int OFF>
-__device__ __forceinline__ void code_pairs(uint32_t word, uint32_t (&pair)[4]) {
-    const uint32_t up = word >> 8;
-    pair[0] = (word & 0x000f000fu) | 0x64006400u;
-    pair[1] = (word & 0x00f000f0u) | 0x64006400u;
-    pair[2] = (up & 0x000f000fu) | 0x64006400u;
-    pair[3] = (up & 0x00f000f0u) | 0x64006400u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&pair[i]), __float2half2_rn(1024.0f + (i & 1 ? 16 * OFF : OFF)));
-        pair[i] = *reinterpret_cast<const uint32_t*>(&v);
-    }
 }
 
 // W words from shared memory, in the widest loads that their alignment allows.
@@ -226,7 +148,7 @@ struct Queries {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 mine[j] += x[j][i];
-                x[j][i] *= (i & 1) ? factor * 0.0625f : factor;  // odd places meet codes x 16
+                x[j][i] *= factor;
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -607,10 +529,9 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                // rows g + 8 of the product met codes x 16; the weights were 2^6 / v_top times the true ones
-                const float low = low_o[n][j][u], even = 0.015625f * v_top, odd = 0.0009765625f * v_top;
-                float4 v = make_float4(fmaf(o[n][j][0][u], even, low), fmaf(o[n][j][0][u + 2], odd, low), fmaf(o[n][j][1][u], even, low),
-                                       fmaf(o[n][j][1][u + 2], odd, low));
+                const float low = low_o[n][j][u], unit = 0.015625f * v_top;  // the weights were 2^6 / v_top times the true ones
+                float4 v = make_float4(fmaf(o[n][j][0][u], unit, low), fmaf(o[n][j][0][u + 2], unit, low), fmaf(o[n][j][1][u], unit, low),
+                                       fmaf(o[n][j][1][u + 2], unit, low));
                 if (bad[n] >> (j + 8 * u) & 1) v = make_float4(NAN, NAN, NAN, NAN);
                 *reinterpret_cast<float4*>(mine + (2 * c + u) * Plan::ROW + 32 * j + 4 * g) = v;
             }
@@ -666,7 +587,7 @@ __device__ __forceinline__ int stages_of(const PackedAttention& p, int seq, int&
     const int most = max(0, min(start + n, p.width * p.cache.page_size));
     const int least = min(p.window > 0 ? max(0, start - p.window + 1) : 0, most);
     floor = least / STAGE * STAGE;
-    return n > 0 ? max(1, (most - floor + STAGE - 1) / STAGE) : 0;
+    return n > 0 && n * p.group <= p.few ? max(1, (most - floor + STAGE - 1) / STAGE) : 0;
 }
 
 constexpr int EVEN_SEQS = 1024;      // most requests of a step whose stages are dealt out evenly
@@ -845,7 +766,7 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_join_even_kernel(
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x, head = blockIdx.y, s = blockIdx.z, rows = gridDim.x;
     const int* before = (const int*)(p.parts + (size_t)2 * grid * rows * (D + 2));
     const int t0 = max(p.q_start[s], 0), count = (min(p.q_start[s + 1], p.tokens) - t0) * p.group;
-    if (r >= count) return;
+    if (r >= count || count > p.few) return;
     const Deal deal(before[p.seqs + 1], p.most_blocks);
     const int n = (before[s + 1] - before[s]) / p.cache.kv_heads, begin = before[s] + head * n;
     const int first = deal.runs ? deal.block_of(begin) : begin, last = deal.runs ? deal.block_of(begin + n - 1) : begin + n - 1;
@@ -892,7 +813,7 @@ __global__ void __launch_bounds__(256) packed_attention_scored_weights_kernel(co
     const int head = blockIdx.y, seq = blockIdx.z, row = blockIdx.x * 256 + threadIdx.x;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
     const int end = min(min(start + n, p.width * p.cache.page_size), p.max_rows);
-    if (row >= end || n <= 0) return;
+    if (row >= end || n <= 0 || count > p.few) return;
     int floor;
     stages_of(p, seq, floor);
     float total = 0.0f;
@@ -943,7 +864,7 @@ __global__ void __launch_bounds__(256) packed_attention_join_kernel(const Packed
 // Weights of the cached rows:  w[key] (+)= sum over the request's queries and the kv head's query heads of
 // exp2(s - lse), a warp 32 rows of the cache, the query rows in their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(const PackedAttention p) {
+__global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(const PackedAttention p, int more) {
     constexpr int W = D / 32, NP = sizeof(T) == 4 ? 2 : 1;
     extern __shared__ __align__(16) unsigned char smem[];
     pdl_launch_dependents();
@@ -952,7 +873,7 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
     const int head = blockIdx.y, seq = blockIdx.z, at = (blockIdx.x * WARPS + warp) * STAGE;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
     const int limit = p.width * p.cache.page_size, end = min(min(start + n, limit), p.max_rows);
-    if (at >= end) return;
+    if (at >= end || count <= more) return;  // (requests of at most `more` query rows have theirs from elsewhere)
     const int* table = p.tables + (size_t)seq * p.width;
     unsigned char* stage = smem + warp * Stage<W>::BYTES;
     const uint32_t there = Stage<W>::request(p, table, head, at, end, stage, lane);
@@ -1004,31 +925,45 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
         }
 }
 
-// How a step is cut: tiles of eight query rows that a block takes, whether all rows of a request fit them, and the blocks or splits.
+// How a step is cut.  bf16 portions of prompts with heads of 64 or 128 go to the 5th-generation tensor cores (packed_prefill.cu), the
+// requests beside them that bring at most `few` query rows stay here; elsewhere all do.
+// Tiles of eight query rows that a block takes: two where there are more rows than eight and the registers hold them.
 struct Plan {
-    int tiles, even, most, blocks, splits, join_kernel;
-    long long lse_floats, part_floats, score_floats, counters;
+    int tiles, even, most, blocks, splits, join_kernel, few, here, prefill;
+    PrefillPlan prompts;
+    long long lse_floats, part_floats, score_floats, prompt_floats, counters;
 
-    long long scratch() const { return lse_floats + part_floats + score_floats; }
+    long long scratch() const { return lse_floats + part_floats + score_floats + prompt_floats; }
+    long long all_counters() const { return counters + (prefill ? prompts.counters : 0); }
 };
 
-// Tiles: two where there are more rows than eight and the registers hold them.
 Plan make_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int tokens, int max_q, int max_kv, int weights) {
     const int sms = ferris_sm_count() > 0 ? ferris_sm_count() : 148;
     Plan q = {};
-    const long long rows = (long long)max_q * group;
+    const auto fours = [](long long floats) { return (floats + 3) / 4 * 4; };  // (what follows begins on 16 bytes)
+    long long rows = (long long)max_q * group;
+    q.few = 0x7fffffff, q.here = 1;
+    if (dtype == FERRIS_BF16 && (head_dim == 64 || head_dim == 128) && rows > 16 && kv_heads <= 65535) {
+        q.prefill = 1;
+        q.few = group <= 8 ? 8 : group <= 16 ? 16 : 0;
+        q.here = seqs > 1 && q.few > 0;
+        q.prompts = packed_prefill_plan(head_dim, seqs, kv_heads, group, tokens, max_q, max_kv);
+        q.prompt_floats = fours((q.prompts.bytes + 3) / 4);
+        rows = q.few;
+    }
     q.tiles = rows > 8 && (dtype == FERRIS_BF16 || head_dim <= 128) ? 2 : 1;
     const int per_sm = head_dim * q.tiles <= 128 && dtype == FERRIS_BF16 ? 2 : 1;
     const long long stages = max_kv / STAGE + 2, pairs = (long long)seqs * kv_heads;
-    q.even = rows <= 8 * q.tiles && seqs <= EVEN_SEQS && pairs * stages < 0x7fffffff;
     q.splits = 1;
-    q.lse_floats = weights ? ((long long)tokens * kv_heads * group + 3) / 4 * 4 : 0;  // (what follows begins on 16 bytes)
+    q.lse_floats = weights ? fours((long long)tokens * kv_heads * group) : 0;
+    if (!q.here) return q;
+    q.even = rows <= 8 * q.tiles && seqs <= EVEN_SEQS && pairs * stages < 0x7fffffff;
     if (q.even) {
         const long long most = pairs * stages / EVEN_STAGES;
         q.most = (int)(most < 1 ? 1 : most < sms * per_sm ? most : sms * per_sm);
         q.blocks = q.most + (int)pairs;  // (pieces: each request and kv head may have one that is not full)
         q.join_kernel = q.most > 16 * pairs;  // so many parts of a request that one block would be long at joining them
-        q.part_floats = (2ll * q.blocks * 8 * q.tiles * (head_dim + 2) + (q.join_kernel ? seqs + 2 : 0) + 3) / 4 * 4;
+        q.part_floats = fours(2ll * q.blocks * 8 * q.tiles * (head_dim + 2) + (q.join_kernel ? seqs + 2 : 0));
         q.counters = q.join_kernel ? 0 : pairs;
         q.score_floats = weights ? pairs * stages * STAGE * 8 * q.tiles : 0;
         if (q.score_floats > (1ll << 27)) q.score_floats = 0;  // (above 512 MB the scores are formed again)
@@ -1038,7 +973,7 @@ Plan make_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int t
         if (want > max_kv / (WARPS * STAGE)) want = max_kv / (WARPS * STAGE);
         if (want > 65535 / (seqs > 0 ? seqs : 1)) want = 65535 / (seqs > 0 ? seqs : 1);
         q.splits = want < 1 ? 1 : (int)want;
-        q.part_floats = q.splits > 1 ? (long long)q.splits * tokens * kv_heads * group * (head_dim + 2) : 0;
+        q.part_floats = q.splits > 1 ? fours((long long)q.splits * tokens * kv_heads * group * (head_dim + 2)) : 0;
     }
     return q;
 }
@@ -1053,36 +988,41 @@ int attend_rows(const PackedAttention& p, const Plan& q, int max_q, cudaStream_t
 }
 
 template <typename T, int D>
-int attend(const PackedAttention& p, const Plan& q, int max_q, int max_kv, cudaStream_t st) {
+int attend(const PackedAttention& p, const Plan& q, int max_q, int max_kv, void* prompt_scratch, int* prompt_counters, cudaStream_t st) {
     constexpr int MOST = sizeof(T) == 2 || D <= 128 ? 2 : 1;
-    int e = q.tiles == 2 ? attend_rows<T, D, MOST>(p, q, max_q, st) : attend_rows<T, D, 1>(p, q, max_q, st);
-    if (e == 0 && q.join_kernel)
-        e = (int)ferris_launch(packed_attention_join_even_kernel<T, D>, dim3(8 * q.tiles, p.cache.kv_heads, p.seqs), dim3(WARPS * 32), 0, st, p, q.blocks);
-    if (e == 0 && p.splits > 1)
-        e = (int)ferris_launch(packed_attention_join_kernel<T, D>, dim3((unsigned)(((long long)p.tokens * p.heads + 7) / 8)), dim3(256), 0, st, p);
-    if (e == 0 && p.weights && p.scores) {
+    int e = 0;
+    if (q.here) {
+        e = q.tiles == 2 ? attend_rows<T, D, MOST>(p, q, max_q, st) : attend_rows<T, D, 1>(p, q, max_q, st);
+        if (e == 0 && q.join_kernel)
+            e = (int)ferris_launch(packed_attention_join_even_kernel<T, D>, dim3(8 * q.tiles, p.cache.kv_heads, p.seqs), dim3(WARPS * 32), 0, st, p, q.blocks);
+        if (e == 0 && p.splits > 1)
+            e = (int)ferris_launch(packed_attention_join_kernel<T, D>, dim3((unsigned)(((long long)p.tokens * p.heads + 7) / 8)), dim3(256), 0, st, p);
+    }
+    if (e == 0 && q.prefill) e = packed_prefill(p, q.prompts, prompt_scratch, prompt_counters, st);
+    if (e == 0 && p.weights && p.scores)
         e = (int)ferris_launch(packed_attention_scored_weights_kernel, dim3((max_kv + 255) / 256, p.cache.kv_heads, p.seqs), dim3(256), 0, st, p, 8 * q.tiles);
-    } else if (e == 0 && p.weights) {
+    if (e == 0 && p.weights && (q.prefill || !p.scores)) {
         auto kernel = packed_attention_weights_kernel<T, D>;
         constexpr size_t smem = (size_t)WARPS * Stage<D / 32>::BYTES;
         e = ferris_allow_dynamic_smem((const void*)kernel, smem);
         if (e == 0)
-            e = (int)ferris_launch(kernel, dim3((max_kv + WARPS * STAGE - 1) / (WARPS * STAGE), p.cache.kv_heads, p.seqs), dim3(WARPS * 32), smem, st, p);
+            e = (int)ferris_launch(kernel, dim3((max_kv + WARPS * STAGE - 1) / (WARPS * STAGE), p.cache.kv_heads, p.seqs), dim3(WARPS * 32), smem, st, p,
+                                   p.scores ? p.few : 0);
     }
     FERRIS_LAUNCH_CHECK();
 }
 
 template <typename T>
-int attend_dim(const PackedAttention& p, const Plan& q, int max_q, int max_kv, cudaStream_t st) {
+int attend_dim(const PackedAttention& p, const Plan& q, int max_q, int max_kv, void* ps, int* pc, cudaStream_t st) {
     switch (p.cache.head_dim) {
-        case 32: return attend<T, 32>(p, q, max_q, max_kv, st);
-        case 64: return attend<T, 64>(p, q, max_q, max_kv, st);
-        case 96: return attend<T, 96>(p, q, max_q, max_kv, st);
-        case 128: return attend<T, 128>(p, q, max_q, max_kv, st);
-        case 160: return attend<T, 160>(p, q, max_q, max_kv, st);
-        case 192: return attend<T, 192>(p, q, max_q, max_kv, st);
-        case 224: return attend<T, 224>(p, q, max_q, max_kv, st);
-        case 256: return attend<T, 256>(p, q, max_q, max_kv, st);
+        case 32: return attend<T, 32>(p, q, max_q, max_kv, ps, pc, st);
+        case 64: return attend<T, 64>(p, q, max_q, max_kv, ps, pc, st);
+        case 96: return attend<T, 96>(p, q, max_q, max_kv, ps, pc, st);
+        case 128: return attend<T, 128>(p, q, max_q, max_kv, ps, pc, st);
+        case 160: return attend<T, 160>(p, q, max_q, max_kv, ps, pc, st);
+        case 192: return attend<T, 192>(p, q, max_q, max_kv, ps, pc, st);
+        case 224: return attend<T, 224>(p, q, max_q, max_kv, ps, pc, st);
+        case 256: return attend<T, 256>(p, q, max_q, max_kv, ps, pc, st);
     }
     FERRIS_REFUSE("packed attention: heads of %d elements", p.cache.head_dim);
 }
@@ -1094,8 +1034,8 @@ FERRIS_API int ferris_packed_attention_plan(int dtype, int head_dim, int seqs, i
                                             int weights, long long* needs) {
     const Plan q = make_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_q, max_kv, weights);
     needs[0] = q.scratch();
-    needs[1] = q.counters;
-    needs[2] = 1 + (q.join_kernel || q.splits > 1) + (weights ? 1 : 0);
+    needs[1] = q.all_counters();
+    needs[2] = q.here + (q.join_kernel || q.splits > 1) + 2 * q.prefill + (weights ? (q.score_floats > 0) + (q.prefill || q.score_floats == 0) : 0);
     return FERRIS_OK;
 }
 
@@ -1126,11 +1066,13 @@ FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
     if ((long long)a->width * a->page_size > 0x7fffffff - 16 * WARPS * STAGE) FERRIS_REFUSE("packed attention: %d blocks of %d rows", a->width, a->page_size);
     const Plan plan = make_plan(a->dtype, a->head_dim, a->seqs, a->kv_heads, a->heads / a->kv_heads, a->tokens, a->max_q, a->max_kv, a->weights != nullptr);
     if (plan.scratch() && !a->scratch) FERRIS_REFUSE("packed attention: no scratch");
-    if (plan.counters && !a->counters) FERRIS_REFUSE("packed attention: no counters");
-    if (a->kv_heads > 65535 || (!plan.even && (long long)a->seqs * plan.splits > 65535) || a->seqs > 65535)
+    if (plan.all_counters() && !a->counters) FERRIS_REFUSE("packed attention: no counters");
+    if (a->kv_heads > 65535 || (plan.here && !plan.even && (long long)a->seqs * plan.splits > 65535) || a->seqs > 65535)
         FERRIS_REFUSE("packed attention: %d requests of %d kv heads", a->seqs, a->kv_heads);
     p.q = a->q, p.out = a->out, p.ldq = a->ldq, p.ldo = a->ldo;
     p.q_aligned = ((uintptr_t)a->q & 15) == 0 && (long long)a->ldq * (a->dtype == FERRIS_BF16 ? 2 : 4) % 16 == 0;
+    p.out_aligned = ((uintptr_t)a->out & 15) == 0 && (long long)a->ldo * (a->dtype == FERRIS_BF16 ? 2 : 4) % 16 == 0;
+    p.few = plan.few;
     p.tables = a->tables, p.width = a->width, p.q_start = a->q_start, p.start_row = a->start_row;
     p.seqs = a->seqs, p.heads = a->heads, p.group = a->heads / a->kv_heads, p.window = a->window, p.scale = a->scale * LOG2E;
     p.lse = plan.lse_floats ? a->scratch : nullptr, p.parts = a->scratch + plan.lse_floats;
@@ -1144,7 +1086,9 @@ FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
     }
     p.weights = a->weights, p.seq_slot = a->seq_slot, p.slot_stride = a->slot_stride, p.head_stride = a->head_stride, p.max_rows = a->max_rows, p.add = a->add;
     p.status = ferris_status_ptr();
-    if (a->dtype == FERRIS_BF16) return attend_dim<bf16>(p, plan, a->max_q, a->max_kv, (cudaStream_t)a->stream);
-    if (a->dtype == FERRIS_F32) return attend_dim<float>(p, plan, a->max_q, a->max_kv, (cudaStream_t)a->stream);
+    void* ps = a->scratch + (plan.scratch() - plan.prompt_floats);
+    int* pc = a->counters + plan.counters;
+    if (a->dtype == FERRIS_BF16) return attend_dim<bf16>(p, plan, a->max_q, a->max_kv, ps, pc, (cudaStream_t)a->stream);
+    if (a->dtype == FERRIS_F32) return attend_dim<float>(p, plan, a->max_q, a->max_kv, ps, pc, (cudaStream_t)a->stream);
     FERRIS_REFUSE("packed attention: dtype %d is not known", a->dtype);
 }

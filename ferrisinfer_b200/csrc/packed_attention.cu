@@ -864,7 +864,7 @@ __global__ void __launch_bounds__(256) packed_attention_join_kernel(const Packed
 // Weights of the cached rows:  w[key] (+)= sum over the request's queries and the kv head's query heads of
 // exp2(s - lse), a warp 32 rows of the cache, the query rows in their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(const PackedAttention p, int more) {
+__global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(const PackedAttention p) {
     constexpr int W = D / 32, NP = sizeof(T) == 4 ? 2 : 1;
     extern __shared__ __align__(16) unsigned char smem[];
     pdl_launch_dependents();
@@ -873,7 +873,7 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
     const int head = blockIdx.y, seq = blockIdx.z, at = (blockIdx.x * WARPS + warp) * STAGE;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
     const int limit = p.width * p.cache.page_size, end = min(min(start + n, limit), p.max_rows);
-    if (at >= end || count <= more) return;  // (requests of at most `more` query rows have theirs from elsewhere)
+    if (at >= end || count > p.few) return;
     const int* table = p.tables + (size_t)seq * p.width;
     unsigned char* stage = smem + warp * Stage<W>::BYTES;
     const uint32_t there = Stage<W>::request(p, table, head, at, end, stage, lane);
@@ -998,16 +998,15 @@ int attend(const PackedAttention& p, const Plan& q, int max_q, int max_kv, void*
         if (e == 0 && p.splits > 1)
             e = (int)ferris_launch(packed_attention_join_kernel<T, D>, dim3((unsigned)(((long long)p.tokens * p.heads + 7) / 8)), dim3(256), 0, st, p);
     }
-    if (e == 0 && q.prefill) e = packed_prefill(p, q.prompts, prompt_scratch, prompt_counters, st);
+    if (e == 0 && q.prefill) e = packed_prefill(p, q.prompts, max_kv, prompt_scratch, prompt_counters, st);
     if (e == 0 && p.weights && p.scores)
         e = (int)ferris_launch(packed_attention_scored_weights_kernel, dim3((max_kv + 255) / 256, p.cache.kv_heads, p.seqs), dim3(256), 0, st, p, 8 * q.tiles);
-    if (e == 0 && p.weights && (q.prefill || !p.scores)) {
+    if (e == 0 && p.weights && q.here && !p.scores) {
         auto kernel = packed_attention_weights_kernel<T, D>;
         constexpr size_t smem = (size_t)WARPS * Stage<D / 32>::BYTES;
         e = ferris_allow_dynamic_smem((const void*)kernel, smem);
         if (e == 0)
-            e = (int)ferris_launch(kernel, dim3((max_kv + WARPS * STAGE - 1) / (WARPS * STAGE), p.cache.kv_heads, p.seqs), dim3(WARPS * 32), smem, st, p,
-                                   p.scores ? p.few : 0);
+            e = (int)ferris_launch(kernel, dim3((max_kv + WARPS * STAGE - 1) / (WARPS * STAGE), p.cache.kv_heads, p.seqs), dim3(WARPS * 32), smem, st, p);
     }
     FERRIS_LAUNCH_CHECK();
 }
@@ -1035,7 +1034,7 @@ FERRIS_API int ferris_packed_attention_plan(int dtype, int head_dim, int seqs, i
     const Plan q = make_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_q, max_kv, weights);
     needs[0] = q.scratch();
     needs[1] = q.all_counters();
-    needs[2] = q.here + (q.join_kernel || q.splits > 1) + 2 * q.prefill + (weights ? (q.score_floats > 0) + (q.prefill || q.score_floats == 0) : 0);
+    needs[2] = q.here + (q.join_kernel || q.splits > 1) + 2 * q.prefill + (weights ? q.here + q.prefill : 0);
     return FERRIS_OK;
 }
 

@@ -88,4 +88,4 @@ struct PrefillPlan {
     long long bytes, counters;  // scratch; whole numbers that are nought
 };
 PrefillPlan packed_prefill_plan(int head_dim, int seqs, int kv_heads, int group, int tokens, int max_q, int max_kv);
-int packed_prefill(const PackedAttention& p, const PrefillPlan& plan, void* scratch, int* counters, cudaStream_t stream);
+int packed_prefill(const PackedAttention& p, const PrefillPlan& plan, int max_kv, void* scratch, int* counters, cudaStream_t stream);

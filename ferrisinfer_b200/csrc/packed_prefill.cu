@@ -43,6 +43,8 @@ struct Pair {
 struct Layout {
     unsigned char* queries;  // [pair][kv head][2 tiles] operands
     float* scales;           // [pair][kv head][256]: what makes a product one to the base of 2
+    float* minus_lse;        // the same: minus the log2 of the row's sum (with weights; minus infinity for rows that are not there)
+    int* first_pair;         // [request]
     Pair* pairs;
     int* before;             // [pairs + 1], then the number of pairs, units
     float* parts;            // [place][D + 2][256]
@@ -50,26 +52,30 @@ struct Layout {
 };
 
 template <typename F>
-void for_scratch(int D, int pairs, int kv_heads, int grid, F&& take) {
+void for_scratch(int D, int pairs, int kv_heads, int seqs, int grid, F&& take) {
     const long long operand = (long long)(D / 64) * 16384 + EXTRA;
     take(0, (long long)pairs * kv_heads * 2 * operand);
     take(1, (long long)pairs * kv_heads * 256 * 4);
     take(2, (long long)pairs * sizeof(Pair));
     take(3, (long long)(pairs + 3) * 4);
     take(4, 2ll * grid * (D + 2) * 256 * 4);
+    take(5, (long long)pairs * kv_heads * 256 * 4);
+    take(6, (long long)seqs * 4);
 }
 
-Layout make_layout(void* base, int D, int pairs, int kv_heads, int grid) {
+Layout make_layout(void* base, int D, int pairs, int kv_heads, int seqs, int grid) {
     Layout l = {};
     unsigned char* at = (unsigned char*)base;
     long long used = 0;
-    for_scratch(D, pairs, kv_heads, grid, [&](int what, long long bytes) {
+    for_scratch(D, pairs, kv_heads, seqs, grid, [&](int what, long long bytes) {
         unsigned char* p = at + used;
         if (what == 0) l.queries = p;
         if (what == 1) l.scales = (float*)p;
         if (what == 2) l.pairs = (Pair*)p;
         if (what == 3) l.before = (int*)p;
         if (what == 4) l.parts = (float*)p;
+        if (what == 5) l.minus_lse = (float*)p;
+        if (what == 6) l.first_pair = (int*)p;
         used += (bytes + 1023) / 1024 * 1024;
     });
     l.bytes = used;
@@ -144,6 +150,7 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
             __syncthreads();
             int at = n_pairs + upto - n;
             for (int w = 0; w < warp; ++w) at += sums[w];
+            if (s0 + tid < p.seqs) l.first_pair[s0 + tid] = at;
             int all = 0;
             for (int w = 0; w < 8; ++w) all += sums[w];
             for (int i = 0; i < 32; ++i) {
@@ -256,7 +263,10 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
         const float rest = own - __low2float(*reinterpret_cast<const __half2*>(&high));
         *reinterpret_cast<uint2*>(tile + Shape<D>::ATOMS * Shape<D>::ATOM + (c >> 1) * 2048 + (r >> 3) * 128 + (r & 7) * 16 + (c & 1) * 8) =
             c < W ? make_uint2(high, pack_f16(rest, rest)) : make_uint2(0u, 0u);
-        if (c == 0) l.scales[index * 256 + rr] = p.scale / factor;
+        if (c == 0) {
+            l.scales[index * 256 + rr] = p.scale / factor;
+            l.minus_lse[index * 256 + rr] = -INFINITY;
+        }
     }
 }
 
@@ -304,6 +314,78 @@ __device__ __forceinline__ void named_barrier(int id) {
 
 // All of an SM's tensor memory for this block: the same warp gives it back (tmem_dealloc).
 __device__ __forceinline__ void tensor_memory_begin(uint32_t* base) { tmem_alloc(base, 512); }
+
+// A cached row's keys on their way to being an operand.
+template <int D>
+struct KeyRow {
+    static constexpr int W = D / 32;
+    uint32_t word[4 * W], scale[W];
+
+    __device__ __forceinline__ void fetch(const PackedCache& cache, uint32_t at, bool there) {
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+            const uint4 a = there ? reinterpret_cast<const uint4*>(cache.k_codes)[(size_t)at * W + c] : make_uint4(0, 0, 0, 0);
+            word[4 * c] = a.x, word[4 * c + 1] = a.y, word[4 * c + 2] = a.z, word[4 * c + 3] = a.w;
+            scale[c] = there ? cache.k_scales[(size_t)at * W + c] : 0u;
+        }
+    }
+    __device__ __forceinline__ float top() const {
+        float t = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) t = fmaxf(t, fmaxf(8.0f * packed_scale(scale[j]), fabsf(fmaf(8.0f, packed_scale(scale[j]), packed_least(scale[j])))));
+        return t;
+    }
+    // Row t of the operand at `to`, times f.
+    __device__ __forceinline__ void store(unsigned char* to, int t, float f) const {
+        using S = Shape<D>;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const __half2 s2 = __float2half2_rn(packed_scale(scale[j]) * f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t x[4];
+                code_pairs<8>(word[c * W + j], x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), s2);
+                    x[e] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+                const int chunk = 4 * j + c;
+                *reinterpret_cast<uint4*>(to + (chunk >> 3) * S::ATOM + swizzle128(t, chunk & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {  // middles over 1 / 64: high, low, high, low of two groups
+            uint32_t x[2] = {0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (j + e < W) {
+                    const uint32_t sc = scale[j + e < W ? j + e : 0];
+                    const float mid = fmaf(8.0f, packed_scale(sc), packed_least(sc)) * f * 64.0f;
+                    const float high = __half2float(__float2half_rn(mid));
+                    x[e] = pack_f16(high, mid - high);
+                }
+            *reinterpret_cast<uint4*>(to + S::ATOMS * S::ATOM + (j >> 1) * 2048 + (t >> 3) * 128 + (t & 7) * 16) = make_uint4(x[0], x[0], x[1], x[1]);
+        }
+    }
+};
+
+// Exponent (biased) of a block's greatest number, within what both of these have: the power of two that brings it between 2^7 and
+// 2^8, and the way back.
+__device__ __forceinline__ uint32_t top_exponent(float top) { return min(max(__float_as_uint(top) >> 23, 8u), 254u); }
+__device__ __forceinline__ float into_range(uint32_t e) { return __uint_as_float((261u - e) << 23); }
+__device__ __forceinline__ float out_of_range(uint32_t e) { return __uint_as_float((e - 7u) << 23); }
+
+// The scores of one query tile against one block of keys (A x B^T), into tensor memory; issued by one thread.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    using S = Shape<D>;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x)
+        tcgen05_mma_bf16(d, umma_desc_k_major_sw128(a + (x >> 2) * S::ATOM) + (uint64_t)(2 * (x & 3)),  // (fp16, says the descriptor)
+                         umma_desc_k_major_sw128(b + (x >> 2) * S::ATOM) + (uint64_t)(2 * (x & 3)), idesc, x > 0 ? 1u : 0u);
+    tcgen05_mma_bf16(d, desc_extra(a + S::ATOMS * S::ATOM), desc_extra(b + S::ATOMS * S::ATOM), idesc, 1u);
+}
 
 // What the converting warps say of a block.
 template <int W>
@@ -436,7 +518,9 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
             const bool valid = row < rq.rows;
             int lo = 0, hi = 0;
             if (valid) rq.sees(p, row, lo, hi);
-            const float qs = l.scales[((size_t)job.pair * p.cache.kv_heads + job.head) * 256 + t * ROWS + r];
+            const size_t place = ((size_t)job.pair * p.cache.kv_heads + job.head) * 256 + t * ROWS + r;
+            const float qs = l.scales[place];
+            float* my_lse = l.minus_lse + place;
             float m = -FLT_MAX, sum = 0.0f, v_unit = 1.0f;
             uint32_t bad = 0;
             for (int i = act.from; i < act.to; ++i) {
@@ -590,7 +674,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
             }
             tcgen05_fence_before();
             if (!part) {
-                if (valid && p.lse) p.lse[(size_t)token * p.heads + qh] = sum == 0.0f ? INFINITY : m + log2f(sum);
+                if (valid) my_lse[0] = sum == 0.0f ? -INFINITY : -(m + log2f(sum));
                 continue;
             }
             part[(size_t)D * 256] = m;
@@ -621,7 +705,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                 }
                 store(h, v);
             }
-            if (p.lse) p.lse[(size_t)token * p.heads + qh] = sum == 0.0f ? INFINITY : m + log2f(sum);
+            my_lse[0] = sum == 0.0f ? -INFINITY : -(m + log2f(sum));
         }
     } else if (warp < SOFTMAX + CONVERT) {
         // ------------------------------------------------------------------ operands: a thread a cached row of each block
@@ -633,20 +717,19 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
             const int* table = p.tables + (size_t)pair.seq * p.width;
             int lo, end;
             rq.sees(p, min((pair.index + 1) * 2 * ROWS, rq.rows) - 1, lo, end);
-            uint32_t kw[4 * W], ks[W], vw[4 * W], vs[W];
+            KeyRow<D> key;
+            uint32_t vw[4 * W], vs[W];
             bool there = false;
             const auto fetch = [&](int i) {  // this thread's row of the job's block i
                 const int row = (job.first + i) * BLOCK + t, block = p.block_of(row);
                 const int page = row < end ? page_of(p, table, block) : -1;
                 there = page >= 0;
                 const uint32_t at = there ? p.row_of(page, job.head, row, block) : 0;
+                key.fetch(p.cache, at, there);
 #pragma unroll
                 for (int c = 0; c < W; ++c) {
-                    const uint4 a = there ? reinterpret_cast<const uint4*>(p.cache.k_codes)[(size_t)at * W + c] : make_uint4(0, 0, 0, 0);
                     const uint4 b = there ? reinterpret_cast<const uint4*>(p.cache.v_codes)[(size_t)at * W + c] : make_uint4(0, 0, 0, 0);
-                    kw[4 * c] = a.x, kw[4 * c + 1] = a.y, kw[4 * c + 2] = a.z, kw[4 * c + 3] = a.w;
                     vw[4 * c] = b.x, vw[4 * c + 1] = b.y, vw[4 * c + 2] = b.z, vw[4 * c + 3] = b.w;
-                    ks[c] = there ? p.cache.k_scales[(size_t)at * W + c] : 0u;
                     vs[c] = there ? p.cache.v_scales[(size_t)at * W + c] : 0u;
                 }
             };
@@ -655,11 +738,10 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
             for (int i = 0; i < job.count; ++i, ++n) {
                 const int stage = n & 1;
                 Info<W>& info = infos[n % INFOS];
-                float kt = 0.0f, vt = 0.0f;
+                float kt = key.top(), vt = 0.0f;
                 uint32_t mine_bad = 0;
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
-                    kt = fmaxf(kt, fmaxf(8.0f * packed_scale(ks[j]), fabsf(fmaf(8.0f, packed_scale(ks[j]), packed_least(ks[j])))));
                     if (packed_not_finite(vs[j])) {
                         mine_bad |= 1u << j;
                         vs[j] = 0;
@@ -681,9 +763,8 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                     vt = fmaxf(vt, tops[n & 1][1][x]);
                 }
                 v_top = fmaxf(v_top, vt);
-                // powers of two that bring the greatest of keys and values between 2^7 and 2^8, and the way back
-                const uint32_t ke = min(max(__float_as_uint(kt) >> 23, 8u), 254u), ve = min(max(__float_as_uint(v_top) >> 23, 8u), 254u);
-                const float kf = __uint_as_float((261u - ke) << 23), vf = __uint_as_float((261u - ve) << 23);
+                const uint32_t ke = top_exponent(kt), ve = top_exponent(v_top);
+                const float vf = into_range(ve);
                 const uint32_t here = __ballot_sync(0xffffffffu, there);
                 uint32_t bad_rows = 0;
 #pragma unroll
@@ -693,42 +774,13 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                     if (lane == 0) info.bad[j][w] = b;
                 }
                 if (w == 0 && lane == 0) {
-                    info.k_unit = __uint_as_float((ke - 7u) << 23);
-                    info.v_unit = __uint_as_float((ve - 7u) << 23);
+                    info.k_unit = out_of_range(ke);
+                    info.v_unit = out_of_range(ve);
                 }
                 if (lane == 0) info.there[w] = here;
                 // (any_bad: every warp sets or clears it for its own rows, so in four places)
                 if (lane == 0) reinterpret_cast<volatile unsigned char*>(&info.any_bad)[w] = bad_rows != 0;
-                unsigned char* kd = k_smem + stage * S::OPERAND;
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    const __half2 s2 = __float2half2_rn(packed_scale(ks[j]) * kf);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t x[4];
-                        code_pairs<8>(kw[c * W + j], x);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), s2);
-                            x[e] = *reinterpret_cast<const uint32_t*>(&v);
-                        }
-                        const int chunk = 4 * j + c;
-                        *reinterpret_cast<uint4*>(kd + (chunk >> 3) * S::ATOM + swizzle128(t, chunk & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {  // middles over 1 / 64: high, low, high, low of two groups
-                    uint32_t x[2] = {0u, 0u};
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (j + e < W) {
-                            const uint32_t sc = ks[j + e < W ? j + e : 0];
-                            const float mid = fmaf(8.0f, packed_scale(sc), packed_least(sc)) * kf * 64.0f;
-                            const float high = __half2float(__float2half_rn(mid));
-                            x[e] = pack_f16(high, mid - high);
-                        }
-                    *reinterpret_cast<uint4*>(kd + S::ATOMS * S::ATOM + (j >> 1) * 2048 + (t >> 3) * 128 + (t & 7) * 16) = make_uint4(x[0], x[0], x[1], x[1]);
-                }
+                key.store(k_smem + stage * S::OPERAND, t, into_range(ke));
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[stage]);
@@ -778,11 +830,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                 ok = ok && mbar_wait(&k_full[n & 1], (n >> 1) & 1, p.status, 91);
                 if (!ok) return;
                 tcgen05_fence_after();
-#pragma unroll
-                for (int x = 0; x < D / 16; ++x)
-                    tcgen05_mma_bf16(tmem + 128 * t, umma_desc_k_major_sw128(q + (x >> 2) * S::ATOM) + (uint64_t)(2 * (x & 3)),
-                                     umma_desc_k_major_sw128(k + (x >> 2) * S::ATOM) + (uint64_t)(2 * (x & 3)), idesc_s, x > 0 ? 1u : 0u);
-                tcgen05_mma_bf16(tmem + 128 * t, desc_extra(q + S::ATOMS * S::ATOM), desc_extra(k + S::ATOMS * S::ATOM), idesc_s, 1u);
+                issue_scores<D>(tmem + 128 * t, q, k, idesc_s);
                 tcgen05_commit(&s_ready[t]);
             };
             for (int t = 0; t < 2; ++t)
@@ -821,14 +869,170 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
     }
 }
 
+// Weights of the cached rows:  w[key] (+)= sum over the request's query rows of 2^(s - lse), S^T = K Q^T so that a thread has a key
+// and adds up along its row: no sum crosses threads, and the order is that of the queries.  A CTA takes 256 keys of one
+// request and kv head (two blocks, each its own operand, formed once) and goes through the query tiles that see any of
+// them; every tile meets both blocks.
+constexpr int W_KEYS = 2, W_STAGES = 3, W_THREADS = (4 * W_KEYS + 1) * 32;
+
 template <int D>
-int prefill(const PackedAttention& p, const PrefillPlan& plan, void* scratch, int* counters, cudaStream_t st) {
-    const Layout l = make_layout(scratch, D, plan.pairs, p.cache.kv_heads, plan.grid);
+struct WeightShape {
+    static constexpr int STAGE = Shape<D>::OPERAND + 1024;  // a query tile, its scales and minus its sums
+    static constexpr int SMEM = W_KEYS * Shape<D>::OPERAND + W_STAGES * STAGE + 1024;
+};
+
+template <int D>
+__global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(const PackedAttention p, const Layout l) {
+    using S = Shape<D>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint64_t q_full[W_STAGES], s_ready[W_KEYS][2], s_free[W_KEYS][2], k_ready;
+    __shared__ uint32_t tmem_base;
+    __shared__ float tops[W_KEYS][4];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* q_smem = smem + W_KEYS * S::OPERAND;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, seq = blockIdx.z;
+    pdl_wait();
+    const Request rq(p, seq);
+    const int key0 = blockIdx.x * W_KEYS * BLOCK, end = min(max(0, min(rq.start + rq.rows / p.group, rq.limit)), p.max_rows);
+    if (rq.rows <= p.few || key0 >= end) {
+        pdl_launch_dependents();
+        return;
+    }
+    // the tiles of the query rows that see any of these keys
+    const long long first_row = (long long)max(key0 - rq.start, 0) * p.group;
+    const long long last_row = p.window > 0 ? ((long long)key0 + W_KEYS * BLOCK - 1 - rq.start + p.window) * p.group : rq.rows;
+    const int from = (int)(min(first_row, (long long)rq.rows) / ROWS), to = (int)((max(min(last_row, (long long)rq.rows), 0ll) + ROWS - 1) / ROWS);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < W_STAGES; ++i) mbar_init(&q_full[i], 1);
+        for (int k = 0; k < W_KEYS; ++k)
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&s_ready[k][i], 1);
+                mbar_init(&s_free[k][i], 4);
+            }
+        mbar_init(&k_ready, 4 * W_KEYS);
+        mbar_fence_init();
+    }
+    if (warp == 4 * W_KEYS) tensor_memory_begin(&tmem_base);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = tmem_base;  // scores of block k, every other tile, at 256 k + 128 (tile % 2)
+    const size_t first_pair = l.first_pair[seq];
+    bool ok = true;
+    if (warp < 4 * W_KEYS) {
+        const int k = warp >> 2, t = (warp & 3) * 32 + lane, row = key0 + k * BLOCK + t, block = p.block_of(row);
+        const int page = row < end ? page_of(p, p.tables + (size_t)seq * p.width, block) : -1;
+        KeyRow<D> key;
+        key.fetch(p.cache, page >= 0 ? p.row_of(page, head, row, block) : 0, page >= 0);
+        float top = warp_max(key.top());
+        if (lane == 0) tops[k][warp & 3] = top;
+        named_barrier<128>(1 + k);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top = fmaxf(top, tops[k][x]);
+        const uint32_t e = top_exponent(top);
+        key.store(smem + k * S::OPERAND, t, into_range(e));
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_ready);
+        const float unit = out_of_range(e);
+        // this key is seen by the query rows seen_from .. seen_to - 1
+        const long long reach = p.window > 0 ? ((long long)row - rq.start + p.window) * p.group : rq.rows;
+        int seen_from = (int)min((long long)max(row - rq.start, 0) * p.group, (long long)rq.rows), seen_to = (int)max(min(reach, (long long)rq.rows), 0ll);
+        if (page < 0) seen_from = seen_to = 0;
+        float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t my_s = tmem + 256 * k + ((uint32_t)((warp & 3) * 32) << 16);
+        for (int i = from, n = 0; i < to; ++i, ++n) {
+            const float4* scales = reinterpret_cast<const float4*>(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE + S::OPERAND);
+            ok = ok && mbar_wait(&s_ready[k][n & 1], (n >> 1) & 1, p.status, 96);
+            // (the copies have landed before the scores were formed from them: the wait costs nothing, and makes them visible here)
+            ok = ok && mbar_wait(&q_full[n % W_STAGES], (n / W_STAGES) & 1, p.status, 97);
+            __syncwarp();
+            tcgen05_fence_after();
+            const int r0 = i * ROWS;
+            const bool whole = __all_sync(0xffffffffu, r0 >= seen_from && r0 + ROWS <= seen_to);
+#pragma unroll 1
+            for (int h = 0; h < ROWS / 32; ++h) {
+                uint32_t sc[32];
+                tmem_load_32x32(my_s + 128 * (n & 1) + 32 * h, sc);
+                tmem_load_wait();
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    const float4 a = scales[8 * h + c / 4], b = scales[32 + 8 * h + c / 4];
+                    const float x[4] = {fmaf(__uint_as_float(sc[c]) * unit, a.x, b.x), fmaf(__uint_as_float(sc[c + 1]) * unit, a.y, b.y),
+                                        fmaf(__uint_as_float(sc[c + 2]) * unit, a.z, b.z), fmaf(__uint_as_float(sc[c + 3]) * unit, a.w, b.w)};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int r = r0 + 32 * h + c + y;
+                        total[y] += whole || (r >= seen_from && r < seen_to) ? exp2_fast(x[y]) : 0.0f;
+                    }
+                }
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[k][n & 1]);
+        }
+        if (row < end) {
+            float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride + row;
+            const float sum = (total[0] + total[1]) + (total[2] + total[3]);
+            *w = p.add && row < rq.start ? *w + sum : sum;
+        }
+    } else if (lane == 0) {
+        const uint32_t idesc = idesc_f16(BLOCK, ROWS);
+        const int tiles = to - from;
+        const auto load = [&](int n) {
+            const int i = from + n;
+            unsigned char* dst = q_smem + (n % W_STAGES) * WeightShape<D>::STAGE;
+            uint64_t* bar = &q_full[n % W_STAGES];
+            const size_t index = (first_pair + i / 2) * p.cache.kv_heads + head;
+            mbar_expect_tx(bar, S::OPERAND + 2 * ROWS * 4);
+            bulk_load(smem_u32(dst), l.queries + (index * 2 + (i & 1)) * S::OPERAND, S::OPERAND, bar);
+            bulk_load(smem_u32(dst + S::OPERAND), l.scales + index * 256 + (i & 1) * ROWS, ROWS * 4, bar);
+            bulk_load(smem_u32(dst + S::OPERAND + ROWS * 4), l.minus_lse + index * 256 + (i & 1) * ROWS, ROWS * 4, bar);
+        };
+        for (int n = 0; n < tiles && n < W_STAGES - 1; ++n) load(n);
+        if (tiles > 0) ok = ok && mbar_wait(&k_ready, 0, p.status, 98);
+        for (int n = 0; n < tiles; ++n) {
+            ok = ok && mbar_wait(&q_full[n % W_STAGES], (n / W_STAGES) & 1, p.status, 99);
+            for (int k = 0; k < W_KEYS; ++k) {
+                if (n >= 2) ok = ok && mbar_wait(&s_free[k][n & 1], ((n >> 1) - 1) & 1, p.status, 100);
+                if (!ok) break;
+                tcgen05_fence_after();
+                issue_scores<D>(tmem + 256 * k + 128 * (n & 1), smem_u32(smem + k * S::OPERAND), smem_u32(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE), idesc);
+                tcgen05_commit(&s_ready[k][n & 1]);
+            }
+            // the place of the tile before this one, once both blocks have been through with it
+            const int next = n + W_STAGES - 1;
+            if (next < tiles) {
+                if (n >= 1)
+                    for (int k = 0; k < W_KEYS; ++k) ok = ok && mbar_wait(&s_free[k][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, 101);
+                if (ok) load(next);
+            }
+        }
+        if (!ok)  // a wait ran out: no copy may land after the block has gone
+            for (int i = 0; i < W_STAGES; ++i) mbar_wait(&q_full[i], 0, p.status, 102);
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 4 * W_KEYS) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int D>
+int prefill(const PackedAttention& p, const PrefillPlan& plan, int max_kv, void* scratch, int* counters, cudaStream_t st) {
+    const Layout l = make_layout(scratch, D, plan.pairs, p.cache.kv_heads, p.seqs, plan.pairs > TABLE ? 0 : plan.grid);
     cudaError_t e = ferris_launch(packed_queries_kernel<D>, dim3(plan.pairs + 1, p.cache.kv_heads), dim3(256), 0, st, p, l, plan.sms);
     if (e != cudaSuccess) return (int)e;
     auto kernel = packed_prefill_kernel<D>;
     if (const int r = ferris_allow_dynamic_smem((const void*)kernel, Shape<D>::SMEM)) return r;
-    return (int)ferris_launch(kernel, dim3(plan.grid), dim3(THREADS), Shape<D>::SMEM, st, p, l, counters, plan.sms, plan.pairs);
+    e = ferris_launch(kernel, dim3(plan.grid), dim3(THREADS), Shape<D>::SMEM, st, p, l, counters, plan.sms, plan.pairs);
+    if (e != cudaSuccess || !p.weights) return (int)e;
+    auto weigh = packed_prefill_weights_kernel<D>;
+    if (const int r = ferris_allow_dynamic_smem((const void*)weigh, WeightShape<D>::SMEM)) return r;
+    const int keys = W_KEYS * BLOCK;
+    return (int)ferris_launch(weigh, dim3((max_kv + keys - 1) / keys, p.cache.kv_heads, p.seqs), dim3(W_THREADS), WeightShape<D>::SMEM, st, p, l);
 }
 
 }  // namespace
@@ -843,11 +1047,11 @@ PrefillPlan packed_prefill_plan(int head_dim, int seqs, int kv_heads, int group,
     q.grid = q.pairs > TABLE ? q.pairs * kv_heads : q.sms + q.pairs * kv_heads;
     const long long blocks = (long long)q.pairs * kv_heads * (max_kv / BLOCK + 2);
     if (q.pairs <= TABLE && q.grid > blocks) q.grid = (int)blocks;
-    q.bytes = make_layout(nullptr, head_dim, q.pairs, kv_heads, q.pairs > TABLE ? 0 : q.grid).bytes;
+    q.bytes = make_layout(nullptr, head_dim, q.pairs, kv_heads, seqs, q.pairs > TABLE ? 0 : q.grid).bytes;
     q.counters = q.pairs > TABLE ? 0 : (long long)q.pairs * kv_heads;
     return q;
 }
 
-int packed_prefill(const PackedAttention& p, const PrefillPlan& plan, void* scratch, int* counters, cudaStream_t stream) {
-    return p.cache.head_dim == 64 ? prefill<64>(p, plan, scratch, counters, stream) : prefill<128>(p, plan, scratch, counters, stream);
+int packed_prefill(const PackedAttention& p, const PrefillPlan& plan, int max_kv, void* scratch, int* counters, cudaStream_t stream) {
+    return p.cache.head_dim == 64 ? prefill<64>(p, plan, max_kv, scratch, counters, stream) : prefill<128>(p, plan, max_kv, scratch, counters, stream);
 }

@@ -275,12 +275,34 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 
-// A from tensor memory: row = lane, a column holds two elements of K.
-__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// MMAs and commits for a whole warp that has come here together; the lane with `leads` issues.  (The instructions take their
+// operands from the warp's uniform registers; in code that one lane runs by itself the compiler brings them there value
+// by value, and an MMA took 120 cycles to issue, however narrow.)  Descriptors by their lower halves: the upper ones are
+// the same for all operands of a kind.
+__device__ __forceinline__ void mma_from_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t accumulate, uint32_t leads) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(accumulate), "r"(leads)
+        : "memory");
+}
+
+// A from tensor memory: row = lane, a column holds two elements of K.
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t accumulate, uint32_t leads) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(accumulate), "r"(leads)
+        : "memory");
+}
+
+__device__ __forceinline__ void commit_warp(uint64_t* bar, uint32_t leads) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leads)
         : "memory");
 }
 
@@ -292,6 +314,14 @@ __device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t 
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
         "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -336,23 +366,27 @@ struct KeyRow {
         return t;
     }
     // Row t of the operand at `to`, times f.
-    __device__ __forceinline__ void store(unsigned char* to, int t, float f) const {
+    __device__ __forceinline__ void store(unsigned char* to, int t, float f) {
         using S = Shape<D>;
+        __half2 s2[W];
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const __half2 s2 = __float2half2_rn(packed_scale(scale[j]) * f);
+        for (int j = 0; j < W; ++j) s2[j] = __float2half2_rn(packed_scale(scale[j]) * f);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {  // the words of quarter c, which then make room for the next quarter's
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int j = 0; j < W; ++j) {
                 uint32_t x[4];
-                code_pairs<8>(word[c * W + j], x);
+                code_pairs<8>(word[j], x);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), s2);
+                    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), s2[j]);
                     x[e] = *reinterpret_cast<const uint32_t*>(&v);
                 }
                 const int chunk = 4 * j + c;
-                *reinterpret_cast<uint4*>(to + (chunk >> 3) * S::ATOM + swizzle128(t, chunk & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint4*>(to + (j >> 1) * S::ATOM + swizzle128(t, chunk & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
             }
+#pragma unroll
+            for (int i = 0; i < 3 * W; ++i) word[i] = word[i + W];
         }
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {  // middles over 1 / 64: high, low, high, low of two groups
@@ -376,15 +410,19 @@ __device__ __forceinline__ uint32_t top_exponent(float top) { return min(max(__f
 __device__ __forceinline__ float into_range(uint32_t e) { return __uint_as_float((261u - e) << 23); }
 __device__ __forceinline__ float out_of_range(uint32_t e) { return __uint_as_float((e - 7u) << 23); }
 
-// The scores of one query tile against one block of keys (A x B^T), into tensor memory; issued by one thread.
+// The scores of operand a's rows against operand b's from `b_row` (a multiple of 8) on, into tensor memory; for a whole warp.
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void issue_scores(uint32_t d, uint32_t a, uint32_t b, int b_row, uint32_t idesc, uint32_t leads) {
     using S = Shape<D>;
+    const uint64_t da = umma_desc_k_major_sw128(a), db = umma_desc_k_major_sw128(b + 128 * b_row);
+    const uint32_t a0 = (uint32_t)da, b0 = (uint32_t)db, high = (uint32_t)(da >> 32);
 #pragma unroll
-    for (int x = 0; x < D / 16; ++x)
-        tcgen05_mma_bf16(d, umma_desc_k_major_sw128(a + (x >> 2) * S::ATOM) + (uint64_t)(2 * (x & 3)),  // (fp16, says the descriptor)
-                         umma_desc_k_major_sw128(b + (x >> 2) * S::ATOM) + (uint64_t)(2 * (x & 3)), idesc, x > 0 ? 1u : 0u);
-    tcgen05_mma_bf16(d, desc_extra(a + S::ATOMS * S::ATOM), desc_extra(b + S::ATOMS * S::ATOM), idesc, 1u);
+    for (int x = 0; x < D / 16; ++x) {
+        const uint32_t next = (x >> 2) * (S::ATOM >> 4) + 2 * (x & 3);  // the next 64 columns, 32 bytes along the row
+        mma_from_smem(d, a0 + next, b0 + next, high, idesc, x > 0 ? 1u : 0u, leads);
+    }
+    const uint64_t ea = desc_extra(a + S::ATOMS * S::ATOM), eb = desc_extra(b + S::ATOMS * S::ATOM + 16 * b_row);
+    mma_from_smem(d, (uint32_t)ea, (uint32_t)eb, (uint32_t)(ea >> 32), idesc, 1u, leads);
 }
 
 // What the converting warps say of a block.
@@ -449,7 +487,6 @@ struct Active {
         from = min(max(from - j.first, 0), j.count);
         to = max(min(to - j.first, j.count), from);
     }
-    __device__ __forceinline__ bool has(int i) const { return i >= from && i < to; }
 };
 
 template <int D>
@@ -509,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
         // ------------------------------------------------------------------ softmax: a thread a row
         const int t = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, my_s = tmem + 128 * t + lanes, my_o = tmem + 256 + D * t + lanes;
-        int n = 0, scored = 0, done = 0;  // blocks of the CTA so far; of this tile: scores and products waited for
+        int n = 0, done = 0;  // blocks of the CTA so far; of this tile
         while (jobs.next(job)) {
             const Pair pair = l.pairs[job.pair];
             const Request rq(p, pair.seq);
@@ -523,16 +560,14 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
             float* my_lse = l.minus_lse + place;
             float m = -FLT_MAX, sum = 0.0f, v_unit = 1.0f;
             uint32_t bad = 0;
-            for (int i = act.from; i < act.to; ++i) {
+            for (int i = act.from; i < act.to; ++i, ++done) {
                 const Info<W>& info = infos[(n + i) % INFOS];
-                ok = ok && mbar_wait(&s_ready[t], scored & 1, p.status, 84);
-                ++scored;
+                ok = ok && mbar_wait(&s_ready[t], done & 1, p.status, 84);
                 __syncwarp();
                 tcgen05_fence_after();
                 const int key0 = (job.first + i) * BLOCK;
                 const float unit = qs * info.k_unit;
-                const uint32_t all = info.there[0] & info.there[1] & info.there[2] & info.there[3];
-                const bool whole = key0 >= lo && key0 + BLOCK <= hi && all == 0xffffffffu;
+                const bool whole = key0 >= lo && key0 + BLOCK <= hi && (info.there[0] & info.there[1] & info.there[2] & info.there[3]) == 0xffffffffu;
                 if (info.any_bad)  // (rare) which of this row's outputs a value that is not finite reaches
                     for (int k = 0; k < BLOCK; ++k)
                         if (key0 + k >= lo && key0 + k < hi)
@@ -540,47 +575,30 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                             for (int j = 0; j < W; ++j) bad |= (info.bad[j][k >> 5] >> (k & 31) & 1) << j;
                 const bool first = i == act.from;
                 const float v_now = info.v_unit;
-                bool moved = !first && v_now != v_unit;  // (the same for all rows)
-                uint32_t packed[64];
-                for (bool again = __any_sync(0xffffffffu, m == -FLT_MAX);;) {
-                    // once over the scores: the weights relative to m, their sum, the scores' maximum; where a row has none
-                    // yet the maximum alone comes first
-                    float top = -INFINITY, part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const float minus = -m;
+                // The scores are read twice: for their maximum, and for the weights, which go back over them.  Loops that
+                // are not unrolled: three kinds of warps share the SM's instruction cache (with the weights of a row held in
+                // registers until its maximum is known, every fourth stall was for instructions).
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t sc[32];
+                    tmem_load_32x32(my_s + 32 * h, sc);
+                    tmem_load_wait();
+                    if (!whole) {
+                        const uint32_t there = info.there[h];
 #pragma unroll
-                    for (int h = 0; h < 8; ++h) {
-                        uint32_t sc[16];
-                        tmem_load_32x16(my_s + 16 * h, sc);
-                        tmem_load_wait();
-                        if (!whole) {
-                            const uint32_t there = info.there[h >> 1] >> (16 * (h & 1));
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) {
-                                const int key = key0 + 16 * h + c;
-                                sc[c] = key >= lo && key < hi && (there >> c & 1) ? sc[c] : 0xff800000u;
-                            }
-                        }
-                        if (again) {
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) top = fmaxf(top, __uint_as_float(sc[c]) * unit);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 16; c += 2) {
-                                const float x0 = fmaf(__uint_as_float(sc[c]), unit, minus), x1 = fmaf(__uint_as_float(sc[c + 1]), unit, minus);
-                                top = fmaxf(top, fmaxf(x0, x1));
-                                const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
-                                part[(c >> 1) & 3] += e0 + e1;
-                                packed[8 * h + (c >> 1)] = pack_f16(e0, e1);
-                            }
+                        for (int c = 0; c < 32; ++c) {
+                            const int key = key0 + 32 * h + c;
+                            sc[c] = key >= lo && key < hi && (there >> c & 1) ? sc[c] : 0xff800000u;
                         }
                     }
-                    if (!again) top -= minus;
-                    const bool grew = top > m + 8.0f;
-                    if (!again && !__any_sync(0xffffffffu, grew) && !moved) {
-                        sum += (part[0] + part[1]) + (part[2] + part[3]);
-                        break;
-                    }
-                    const float now = again || grew ? fmaxf(m, top) : m;
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) top = fmaxf(top, fmaxf(__uint_as_float(sc[c]), __uint_as_float(sc[c + 1])));
+                }
+                top *= unit;  // (never below zero; 0 x infinity, of a query row of noughts, is no maximum)
+                const bool moved = !first && v_now != v_unit;  // (the same for all rows)
+                if (__any_sync(0xffffffffu, top > m + 8.0f) || moved) {
+                    const float now = top > m + 8.0f ? top : m;
                     float f = exp2_fast(m - now);
                     m = now;
                     sum *= f;
@@ -589,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                         ok = ok && mbar_wait(&pv_done[t], (done - 1) & 1, p.status, 85);
                         __syncwarp();
                         tcgen05_fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int h = 0; h < D / 32; ++h) {
                             uint32_t o[32];
                             tmem_load_32x32(my_o + 32 * h, o);
@@ -599,22 +617,36 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                             tmem_store_32x32(my_o + 32 * h, o);
                         }
                     }
-                    moved = false;
-                    again = false;
                 }
                 v_unit = v_now;
+                const float minus = -m;
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t sc[32], packed[16];
+                    tmem_load_32x32(my_s + 32 * h, sc);
+                    tmem_load_wait();
+                    if (!whole) {
+                        const uint32_t there = info.there[h];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t w[32];
+                        for (int c = 0; c < 32; ++c) {
+                            const int key = key0 + 32 * h + c;
+                            sc[c] = key >= lo && key < hi && (there >> c & 1) ? sc[c] : 0xff800000u;
+                        }
+                    }
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) w[c] = packed[32 * h + c];
-                    tmem_store_32x32(my_s + 32 * h, w);
+                    for (int c = 0; c < 32; c += 2) {
+                        const float e0 = exp2_fast(fmaf(__uint_as_float(sc[c]), unit, minus)), e1 = exp2_fast(fmaf(__uint_as_float(sc[c + 1]), unit, minus));
+                        part[(c >> 1) & 3] += e0 + e1;
+                        packed[c >> 1] = pack_f16(e0, e1);
+                    }
+                    tmem_store_32x16(my_s + 16 * h, packed);
                 }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
                 tmem_store_wait();
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[t]);
-                ++done;
             }
             n += job.count;
             // the rows' outputs, or the pair's part of them
@@ -786,23 +818,29 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                 if (lane == 0) mbar_arrive(&k_full[stage]);
                 ok = ok && (n < 2 || mbar_wait(&v_empty[stage], ((n >> 1) - 1) & 1, p.status, 88));
                 unsigned char* vd = v_smem + stage * S::V_BYTES;
+                __half2 s2[W / 2], mid[W / 2];
 #pragma unroll
                 for (int i2 = 0; i2 < W / 2; ++i2) {
                     const float s0 = packed_scale(vs[2 * i2]) * vf, s1 = packed_scale(vs[2 * i2 + 1]) * vf;
-                    const __half2 s2 = __floats2half2_rn(s0, s1);
-                    const __half2 mid = __floats2half2_rn(fmaf(8.0f, s0, packed_least(vs[2 * i2]) * vf), fmaf(8.0f, s1, packed_least(vs[2 * i2 + 1]) * vf));
+                    s2[i2] = __floats2half2_rn(s0, s1);
+                    mid[i2] = __floats2half2_rn(fmaf(8.0f, s0, packed_least(vs[2 * i2]) * vf), fmaf(8.0f, s1, packed_least(vs[2 * i2 + 1]) * vf));
+                }
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const int chunk = g * (W / 2) + i2;
+                    for (int j = 0; j < W; ++j) {  // chunk g W / 2 + i2
+                        const int chunk = c * W + j;
                         uint32_t x[4];
-                        code_pairs<8>(vw[chunk], x);
+                        code_pairs<8>(vw[j], x);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&x[e]), s2, mid);
+                            const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&x[e]), s2[j % (W / 2)], mid[j % (W / 2)]);
                             x[e] = *reinterpret_cast<const uint32_t*>(&v);
                         }
                         *reinterpret_cast<uint4*>(vd + (chunk >> 3) * S::ATOM + swizzle128(t, chunk & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
                     }
+#pragma unroll
+                    for (int x = 0; x < 3 * W; ++x) vw[x] = vw[x + W];
                 }
                 if (i + 1 < job.count) fetch(i + 1);
                 fence_proxy_async();
@@ -810,56 +848,68 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                 if (lane == 0) mbar_arrive(&v_full[stage]);
             }
         }
-    } else if (lane == 0) {
-        // ------------------------------------------------------------------ the thread that issues
-        const uint32_t idesc_s = idesc_f16(ROWS, BLOCK), idesc_o = idesc_f16(ROWS, D) | (1u << 16);  // V is MN-major (rows along K)
-        int n = 0, weighed[2] = {0, 0}, jobs_done = 0;
+    } else {
+        // ------------------------------------------------------------------ the warp that issues
+        const uint32_t leads = lane == 0, idesc_s = idesc_f16(ROWS, BLOCK), idesc_o = idesc_f16(ROWS, D) | (1u << 16);  // V is MN-major (rows along K)
+        // (What there is one of for each tile stands in two names and is chosen from: an array with an index of the loop would lie in local
+        // memory, and this warp's few instructions are the pace of the block.)
+        int n = 0, jobs_done = 0;        // blocks, jobs
+        int weighed0 = 0, weighed1 = 0;  // blocks of each tile
+        const auto weighed = [&](int t) { return t ? weighed1 : weighed0; };
         while (jobs.next(job)) {
             const Pair pair = l.pairs[job.pair];
             const Request rq(p, pair.seq);
-            const Active act[2] = {Active(p, rq, pair, job, 0), Active(p, rq, pair, job, 1)};
+            const Active act0(p, rq, pair, job, 0), act1(p, rq, pair, job, 1);
+            const auto has = [&](int t, int i) { return i >= (t ? act1.from : act0.from) && i < (t ? act1.to : act0.to); };
             // the queries of the job before are read no more when its last products are done
             for (int t = 0; t < 2; ++t)
-                if (weighed[t]) ok = ok && mbar_wait(&pv_done[t], (weighed[t] - 1) & 1, p.status, 89);
-            mbar_expect_tx(&q_full, 2 * S::OPERAND);
-            bulk_load(smem_u32(q_smem), l.queries + ((size_t)job.pair * p.cache.kv_heads + job.head) * 2 * S::OPERAND, 2 * S::OPERAND, &q_full);
+                if (weighed(t)) ok = ok && mbar_wait(&pv_done[t], (weighed(t) - 1) & 1, p.status, 89);
+            if (ok && lane == 0) {
+                mbar_expect_tx(&q_full, 2 * S::OPERAND);
+                bulk_load(smem_u32(q_smem), l.queries + ((size_t)job.pair * p.cache.kv_heads + job.head) * 2 * S::OPERAND, 2 * S::OPERAND, &q_full);
+            }
+            __syncwarp();
             ok = ok && mbar_wait(&q_full, jobs_done & 1, p.status, 90);
             ++jobs_done;
-            const auto scores = [&](int t, int n) {
-                const uint32_t q = smem_u32(q_smem + t * S::OPERAND), k = smem_u32(k_smem + (n & 1) * S::OPERAND);
-                ok = ok && mbar_wait(&k_full[n & 1], (n >> 1) & 1, p.status, 91);
-                if (!ok) return;
+            const auto scores = [&](int t, int stage) {
                 tcgen05_fence_after();
-                issue_scores<D>(tmem + 128 * t, q, k, idesc_s);
-                tcgen05_commit(&s_ready[t]);
+                issue_scores<D>(tmem + 128 * t, smem_u32(q_smem + t * S::OPERAND), smem_u32(k_smem + stage * S::OPERAND), 0, idesc_s, leads);
+                commit_warp(&s_ready[t], leads);
             };
+            ok = ok && mbar_wait(&k_full[n & 1], (n >> 1) & 1, p.status, 91);
             for (int t = 0; t < 2; ++t)
-                if (act[t].has(0)) scores(t, n);
-            tcgen05_commit(&k_empty[n & 1]);
+                if (has(t, 0) && ok) scores(t, n & 1);
+            commit_warp(&k_empty[n & 1], leads);
+#pragma unroll 1
             for (int i = 0; i < job.count; ++i, ++n) {
+                const int stage = n & 1;
+                const bool more = i + 1 < job.count;
+                ok = ok && mbar_wait(&v_full[stage], (n >> 1) & 1, p.status, 93) && (!more || mbar_wait(&k_full[stage ^ 1], ((n + 1) >> 1) & 1, p.status, 94));
+#pragma unroll 1
                 for (int t = 0; t < 2; ++t) {
-                    if (act[t].has(i)) {
-                        ok = ok && mbar_wait(&p_ready[t], weighed[t] & 1, p.status, 92) && mbar_wait(&v_full[n & 1], (n >> 1) & 1, p.status, 93);
+                    if (has(t, i)) {
+                        ok = ok && mbar_wait(&p_ready[t], weighed(t) & 1, p.status, 92);
                         if (ok) {
                             tcgen05_fence_after();
-                            const uint64_t v = umma_desc_mn_major_sw128(smem_u32(v_smem + (n & 1) * S::V_BYTES), S::ATOM);
+                            const uint64_t v = umma_desc_mn_major_sw128(smem_u32(v_smem + stage * S::V_BYTES), S::ATOM);
 #pragma unroll
                             for (int x = 0; x < BLOCK / 16; ++x)
-                                mma_from_tmem(tmem + 256 + D * t, tmem + 128 * t + 8 * x, v + (uint64_t)(x * (2048 >> 4)), idesc_o, i > act[t].from || x > 0 ? 1u : 0u);
-                            tcgen05_commit(&pv_done[t]);
+                                mma_from_tmem(tmem + 256 + D * t, tmem + 128 * t + 8 * x, (uint32_t)v + x * (2048 >> 4), (uint32_t)(v >> 32), idesc_o,
+                                              i > (t ? act1.from : act0.from) || x > 0 ? 1u : 0u, leads);
+                            commit_warp(&pv_done[t], leads);
                         }
-                        ++weighed[t];
                         // the next scores come where these weights stand
-                        if (act[t].has(i + 1)) ok = ok && mbar_wait(&pv_done[t], (weighed[t] - 1) & 1, p.status, 94);
+                        if (has(t, i + 1)) ok = ok && mbar_wait(&pv_done[t], weighed(t) & 1, p.status, 95);
+                        weighed0 += t == 0, weighed1 += t == 1;
                     }
-                    if (i + 1 < job.count && act[t].has(i + 1)) scores(t, n + 1);
+                    if (has(t, i + 1) && ok) scores(t, stage ^ 1);
                 }
-                tcgen05_commit(&v_empty[n & 1]);
-                if (i + 1 < job.count) tcgen05_commit(&k_empty[(n + 1) & 1]);
+                commit_warp(&v_empty[stage], leads);
+                if (more) commit_warp(&k_empty[stage ^ 1], leads);
             }
         }
         for (int t = 0; t < 2; ++t)  // nothing is in flight when the tensor memory goes back
-            if (weighed[t]) mbar_wait(&pv_done[t], (weighed[t] - 1) & 1, p.status, 95);
+            if (weighed(t)) mbar_wait(&pv_done[t], (weighed(t) - 1) & 1, p.status, 103);
     }
     tcgen05_fence_before();
     __syncthreads();
@@ -956,16 +1006,29 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
                 uint32_t sc[32];
                 tmem_load_32x32(my_s + 128 * (n & 1) + 32 * h, sc);
                 tmem_load_wait();
+                float4 x[8];  // powers of the weights' logarithms
 #pragma unroll
-                for (int c = 0; c < 32; c += 4) {
-                    const float4 a = scales[8 * h + c / 4], b = scales[32 + 8 * h + c / 4];
-                    const float x[4] = {fmaf(__uint_as_float(sc[c]) * unit, a.x, b.x), fmaf(__uint_as_float(sc[c + 1]) * unit, a.y, b.y),
-                                        fmaf(__uint_as_float(sc[c + 2]) * unit, a.z, b.z), fmaf(__uint_as_float(sc[c + 3]) * unit, a.w, b.w)};
+                for (int c = 0; c < 8; ++c) {
+                    const float4 a = scales[8 * h + c], b = scales[32 + 8 * h + c];
+                    x[c] = make_float4(fmaf(__uint_as_float(sc[4 * c]) * unit, a.x, b.x), fmaf(__uint_as_float(sc[4 * c + 1]) * unit, a.y, b.y),
+                                       fmaf(__uint_as_float(sc[4 * c + 2]) * unit, a.z, b.z), fmaf(__uint_as_float(sc[4 * c + 3]) * unit, a.w, b.w));
+                }
+                if (!whole) {
+                    const int first = seen_from - r0 - 32 * h, last = seen_to - r0 - 32 * h;
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const int r = r0 + 32 * h + c + y;
-                        total[y] += whole || (r >= seen_from && r < seen_to) ? exp2_fast(x[y]) : 0.0f;
+                    for (int c = 0; c < 8; ++c) {
+                        x[c].x = 4 * c >= first && 4 * c < last ? x[c].x : -INFINITY;
+                        x[c].y = 4 * c + 1 >= first && 4 * c + 1 < last ? x[c].y : -INFINITY;
+                        x[c].z = 4 * c + 2 >= first && 4 * c + 2 < last ? x[c].z : -INFINITY;
+                        x[c].w = 4 * c + 3 >= first && 4 * c + 3 < last ? x[c].w : -INFINITY;
                     }
+                }
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    total[0] += exp2_fast(x[c].x);
+                    total[1] += exp2_fast(x[c].y);
+                    total[2] += exp2_fast(x[c].z);
+                    total[3] += exp2_fast(x[c].w);
                 }
             }
             tcgen05_fence_before();
@@ -977,10 +1040,11 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
             const float sum = (total[0] + total[1]) + (total[2] + total[3]);
             *w = p.add && row < rq.start ? *w + sum : sum;
         }
-    } else if (lane == 0) {
-        const uint32_t idesc = idesc_f16(BLOCK, ROWS);
+    } else {
+        const uint32_t idesc = idesc_f16(BLOCK, ROWS), leads = lane == 0;
         const int tiles = to - from;
         const auto load = [&](int n) {
+            if (lane) return;
             const int i = from + n;
             unsigned char* dst = q_smem + (n % W_STAGES) * WeightShape<D>::STAGE;
             uint64_t* bar = &q_full[n % W_STAGES];
@@ -998,8 +1062,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
                 if (n >= 2) ok = ok && mbar_wait(&s_free[k][n & 1], ((n >> 1) - 1) & 1, p.status, 100);
                 if (!ok) break;
                 tcgen05_fence_after();
-                issue_scores<D>(tmem + 256 * k + 128 * (n & 1), smem_u32(smem + k * S::OPERAND), smem_u32(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE), idesc);
-                tcgen05_commit(&s_ready[k][n & 1]);
+                issue_scores<D>(tmem + 256 * k + 128 * (n & 1), smem_u32(smem + k * S::OPERAND), smem_u32(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE), 0, idesc, leads);
+                commit_warp(&s_ready[k][n & 1], leads);
             }
             // the place of the tile before this one, once both blocks have been through with it
             const int next = n + W_STAGES - 1;

@@ -922,7 +922,8 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
 // Weights of the cached rows:  w[key] (+)= sum over the request's query rows of 2^(s - lse), S^T = K Q^T so that a thread has a key
 // and adds up along its row: no sum crosses threads, and the order is that of the queries.  A CTA takes 256 keys of one
 // request and kv head (two blocks, each its own operand, formed once) and goes through the query tiles that see any of
-// them; every tile meets both blocks.
+// them; every tile meets both blocks.  A thread has the same key of both blocks and one half of a tile's rows, so that what it reads of a row (scale
+// and sum, from shared memory, every lane the same) serves two keys: shared memory was as busy as the exponential unit.
 constexpr int W_KEYS = 2, W_STAGES = 3, W_THREADS = (4 * W_KEYS + 1) * 32;
 
 template <int D>
@@ -935,9 +936,9 @@ template <int D>
 __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(const PackedAttention p, const Layout l) {
     using S = Shape<D>;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t q_full[W_STAGES], s_ready[W_KEYS][2], s_free[W_KEYS][2], k_ready;
+    __shared__ uint64_t q_full[W_STAGES], s_ready[2], s_free[2], k_ready;
     __shared__ uint32_t tmem_base;
-    __shared__ float tops[W_KEYS][4];
+    __shared__ float tops[W_KEYS][4], units[W_KEYS], sums[W_KEYS][BLOCK];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* q_smem = smem + W_KEYS * S::OPERAND;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, seq = blockIdx.z;
@@ -954,11 +955,10 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
     const int from = (int)(min(first_row, (long long)rq.rows) / ROWS), to = (int)((max(min(last_row, (long long)rq.rows), 0ll) + ROWS - 1) / ROWS);
     if (threadIdx.x == 0) {
         for (int i = 0; i < W_STAGES; ++i) mbar_init(&q_full[i], 1);
-        for (int k = 0; k < W_KEYS; ++k)
-            for (int i = 0; i < 2; ++i) {
-                mbar_init(&s_ready[k][i], 1);
-                mbar_init(&s_free[k][i], 4);
-            }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_ready[i], 1);
+            mbar_init(&s_free[i], 4 * W_KEYS);
+        }
         mbar_init(&k_ready, 4 * W_KEYS);
         mbar_fence_init();
     }
@@ -985,60 +985,77 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_ready);
-        const float unit = out_of_range(e);
-        // this key is seen by the query rows seen_from .. seen_to - 1
-        const long long reach = p.window > 0 ? ((long long)row - rq.start + p.window) * p.group : rq.rows;
-        int seen_from = (int)min((long long)max(row - rq.start, 0) * p.group, (long long)rq.rows), seen_to = (int)max(min(reach, (long long)rq.rows), 0ll);
-        if (page < 0) seen_from = seen_to = 0;
-        float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const uint32_t my_s = tmem + 256 * k + ((uint32_t)((warp & 3) * 32) << 16);
+        if (t == 0) units[k] = out_of_range(e);
+        named_barrier<256>(3);
+        // from here on: key t of both blocks, rows 64 k .. 64 k + 63 of the tiles; the query rows from[x] .. to[x] - 1 see the key of block x
+        float unit[W_KEYS], total[W_KEYS][2] = {};
+        int seen_from[W_KEYS], seen_to[W_KEYS];
+#pragma unroll
+        for (int x = 0; x < W_KEYS; ++x) {
+            const int row = key0 + x * BLOCK + t;
+            const long long reach = p.window > 0 ? ((long long)row - rq.start + p.window) * p.group : rq.rows;
+            unit[x] = units[x];
+            seen_from[x] = (int)min((long long)max(row - rq.start, 0) * p.group, (long long)rq.rows);
+            seen_to[x] = (int)max(min(reach, (long long)rq.rows), 0ll);
+            if (row >= end || page_of(p, p.tables + (size_t)seq * p.width, p.block_of(row)) < 0) seen_from[x] = seen_to[x] = 0;
+        }
+        const uint32_t my_s = tmem + 64 * k + ((uint32_t)((warp & 3) * 32) << 16);
         for (int i = from, n = 0; i < to; ++i, ++n) {
-            const float4* scales = reinterpret_cast<const float4*>(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE + S::OPERAND);
-            ok = ok && mbar_wait(&s_ready[k][n & 1], (n >> 1) & 1, p.status, 96);
+            const float4* scales = reinterpret_cast<const float4*>(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE + S::OPERAND) + 16 * k;
+            ok = ok && mbar_wait(&s_ready[n & 1], (n >> 1) & 1, p.status, 96);
             // (the copies have landed before the scores were formed from them: the wait costs nothing, and makes them visible here)
             ok = ok && mbar_wait(&q_full[n % W_STAGES], (n / W_STAGES) & 1, p.status, 97);
             __syncwarp();
             tcgen05_fence_after();
-            const int r0 = i * ROWS;
-            const bool whole = __all_sync(0xffffffffu, r0 >= seen_from && r0 + ROWS <= seen_to);
+            const int r0 = i * ROWS + 64 * k;
+            const bool whole = __all_sync(0xffffffffu, r0 >= max(seen_from[0], seen_from[1]) && r0 + 64 <= min(seen_to[0], seen_to[1]));
 #pragma unroll 1
-            for (int h = 0; h < ROWS / 32; ++h) {
-                uint32_t sc[32];
-                tmem_load_32x32(my_s + 128 * (n & 1) + 32 * h, sc);
+            for (int h = 0; h < 4; ++h) {
+                uint32_t sc[W_KEYS][16];
+                tmem_load_32x16(my_s + 128 * (n & 1) + 16 * h, sc[0]);
+                tmem_load_32x16(my_s + 256 + 128 * (n & 1) + 16 * h, sc[1]);
+                float4 a[4], b[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) a[c] = scales[4 * h + c], b[c] = scales[32 + 4 * h + c];
                 tmem_load_wait();
-                float4 x[8];  // powers of the weights' logarithms
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float4 a = scales[8 * h + c], b = scales[32 + 8 * h + c];
-                    x[c] = make_float4(fmaf(__uint_as_float(sc[4 * c]) * unit, a.x, b.x), fmaf(__uint_as_float(sc[4 * c + 1]) * unit, a.y, b.y),
-                                       fmaf(__uint_as_float(sc[4 * c + 2]) * unit, a.z, b.z), fmaf(__uint_as_float(sc[4 * c + 3]) * unit, a.w, b.w));
-                }
-                if (!whole) {
-                    const int first = seen_from - r0 - 32 * h, last = seen_to - r0 - 32 * h;
+                for (int x = 0; x < W_KEYS; ++x) {
+                    float w[16];  // the weights' logarithms
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        x[c].x = 4 * c >= first && 4 * c < last ? x[c].x : -INFINITY;
-                        x[c].y = 4 * c + 1 >= first && 4 * c + 1 < last ? x[c].y : -INFINITY;
-                        x[c].z = 4 * c + 2 >= first && 4 * c + 2 < last ? x[c].z : -INFINITY;
-                        x[c].w = 4 * c + 3 >= first && 4 * c + 3 < last ? x[c].w : -INFINITY;
+                    for (int c = 0; c < 4; ++c) {
+                        w[4 * c] = fmaf(__uint_as_float(sc[x][4 * c]) * unit[x], a[c].x, b[c].x);
+                        w[4 * c + 1] = fmaf(__uint_as_float(sc[x][4 * c + 1]) * unit[x], a[c].y, b[c].y);
+                        w[4 * c + 2] = fmaf(__uint_as_float(sc[x][4 * c + 2]) * unit[x], a[c].z, b[c].z);
+                        w[4 * c + 3] = fmaf(__uint_as_float(sc[x][4 * c + 3]) * unit[x], a[c].w, b[c].w);
                     }
-                }
+                    if (!whole) {
+                        const int first = seen_from[x] - r0 - 16 * h, last = seen_to[x] - r0 - 16 * h;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    total[0] += exp2_fast(x[c].x);
-                    total[1] += exp2_fast(x[c].y);
-                    total[2] += exp2_fast(x[c].z);
-                    total[3] += exp2_fast(x[c].w);
+                        for (int c = 0; c < 16; ++c) w[c] = c >= first && c < last ? w[c] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) total[x][c & 1] += exp2_fast(w[c]);
                 }
             }
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[k][n & 1]);
+            if (lane == 0) mbar_arrive(&s_free[n & 1]);
         }
-        if (row < end) {
-            float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride + row;
-            const float sum = (total[0] + total[1]) + (total[2] + total[3]);
-            *w = p.add && row < rq.start ? *w + sum : sum;
+        if (k == 1) {
+#pragma unroll
+            for (int x = 0; x < W_KEYS; ++x) sums[x][t] = total[x][0] + total[x][1];
+        }
+        named_barrier<256>(3);
+        if (k == 0) {
+#pragma unroll
+            for (int x = 0; x < W_KEYS; ++x) {
+                const int row = key0 + x * BLOCK + t;
+                if (row < end) {
+                    float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride + row;
+                    const float sum = (total[x][0] + total[x][1]) + sums[x][t];
+                    *w = p.add && row < rq.start ? *w + sum : sum;
+                }
+            }
         }
     } else {
         const uint32_t idesc = idesc_f16(BLOCK, ROWS), leads = lane == 0;
@@ -1058,18 +1075,18 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
         if (tiles > 0) ok = ok && mbar_wait(&k_ready, 0, p.status, 98);
         for (int n = 0; n < tiles; ++n) {
             ok = ok && mbar_wait(&q_full[n % W_STAGES], (n / W_STAGES) & 1, p.status, 99);
-            for (int k = 0; k < W_KEYS; ++k) {
-                if (n >= 2) ok = ok && mbar_wait(&s_free[k][n & 1], ((n >> 1) - 1) & 1, p.status, 100);
-                if (!ok) break;
+            if (n >= 2) ok = ok && mbar_wait(&s_free[n & 1], ((n >> 1) - 1) & 1, p.status, 100);
+            if (ok) {
                 tcgen05_fence_after();
-                issue_scores<D>(tmem + 256 * k + 128 * (n & 1), smem_u32(smem + k * S::OPERAND), smem_u32(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE), 0, idesc, leads);
-                commit_warp(&s_ready[k][n & 1], leads);
+#pragma unroll 1
+                for (int k = 0; k < W_KEYS; ++k)
+                    issue_scores<D>(tmem + 256 * k + 128 * (n & 1), smem_u32(smem + k * S::OPERAND), smem_u32(q_smem + (n % W_STAGES) * WeightShape<D>::STAGE), 0, idesc, leads);
+                commit_warp(&s_ready[n & 1], leads);
             }
             // the place of the tile before this one, once both blocks have been through with it
             const int next = n + W_STAGES - 1;
             if (next < tiles) {
-                if (n >= 1)
-                    for (int k = 0; k < W_KEYS; ++k) ok = ok && mbar_wait(&s_free[k][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, 101);
+                if (n >= 1) ok = ok && mbar_wait(&s_free[(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, 101);
                 if (ok) load(next);
             }
         }

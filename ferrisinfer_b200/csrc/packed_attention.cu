@@ -1079,10 +1079,7 @@ FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
     p.splits = plan.splits, p.tokens = a->tokens;
     p.even = plan.even, p.most_blocks = plan.most, p.counters = plan.counters ? a->counters : nullptr;
     p.max_stages = a->max_kv / STAGE + 2;
-    if (a->page_size > 1) {
-        while ((2 << p.page_shift) < a->page_size) ++p.page_shift;
-        p.page_mul = (uint32_t)(((1ull << (32 + p.page_shift)) + a->page_size - 1) / a->page_size);
-    }
+    p.page = DivideBy(a->page_size);
     p.weights = a->weights, p.seq_slot = a->seq_slot, p.slot_stride = a->slot_stride, p.head_stride = a->head_stride, p.max_rows = a->max_rows, p.add = a->add;
     p.status = ferris_status_ptr();
     void* ps = a->scratch + (plan.scratch() - plan.prompt_floats);

@@ -28,16 +28,14 @@ struct PackedAttention {
     float* scores;  // [request][kv head][stage][32][8 NT], to the base of 2, or nullptr
     int max_stages;
     int few;        // most query rows of a request that the kernel for few rows takes; the other takes those with more
-    uint32_t page_mul;  // division by the page size
-    int page_shift;
+    DivideBy page;  // the page size
     float* weights;
     const int* seq_slot;
     long long slot_stride;
     int head_stride, max_rows, add;
     int* status;
 
-    // row / page_size for rows below 2^31: page_mul = ceil(2^(32 + shift) / page_size) with 2^shift < page_size <= 2^(shift + 1)
-    __device__ __forceinline__ int block_of(int row) const { return page_mul ? (int)(__umulhi((uint32_t)row, page_mul) >> page_shift) : row; }
+    __device__ __forceinline__ int block_of(int row) const { return (int)page.quotient((uint32_t)row); }
     // Index of a row of the cache: below 2^32, which the C entry sees to.
     __device__ __forceinline__ uint32_t row_of(int page, int head, int row, int block) const {
         return (uint32_t)(page * cache.kv_heads + head) * cache.page_size + (uint32_t)(row - block * cache.page_size);

@@ -1,4 +1,6 @@
 // Writing, reading and evicting rows of the paged cache in 4 bits (its bytes: packed_cache.cuh).
+#include <type_traits>
+
 #include "packed_cache.cuh"
 
 namespace {
@@ -85,39 +87,56 @@ __device__ __forceinline__ uint32_t quantise8(const Eight& e, uint32_t& scales) 
     return codes;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) packed_write_kernel(const T* k, const T* v, int ldk, int ldv, const int* __restrict__ slots,
-                                                           PackedCache cache, int tokens, int* status) {
+// Where a thread of a call over rows (token, head) stands: elements 8 (4 j + c) .. + 7 of them.
+struct RowsCall {
+    const int* slots;
+    PackedCache cache;
+    int tokens, ldk, ldv;
+    DivideBy heads, page;
+    int* status;
+
+    // The row of the cache that row i of the call names: whether there is one.
+    __device__ __forceinline__ bool find(uint32_t i, int& token, int& head, size_t& row, int where) const {
+        token = (int)heads.quotient(i);
+        head = (int)i - token * cache.kv_heads;
+        const int slot = slots[token], page_at = slot >= 0 ? (int)page.quotient((uint32_t)slot) : -1;
+        if (page_at >= cache.pages) ferris_report(status, FERRIS_STATUS_BAD_INDEX, where);
+        if (page_at < 0 || page_at >= cache.pages) return false;
+        row = cache.row(page_at, head, slot - page_at * cache.page_size);
+        return true;
+    }
+};
+
+// Bound by HBM for many tokens, by its launch for a step's: 16-byte loads of a head's elements, lanes side by side; the divisions
+// by heads and page size are multiplications (as 64-bit divisions they were half of the kernel: 8,192 tokens of 4 heads of
+// 128, written and read back, 28.8 us).
+template <typename T, int W, bool VEC>
+__global__ void __launch_bounds__(256) packed_write_kernel(const T* k, const T* v, const RowsCall q) {
     pdl_launch_dependents();
     pdl_wait();
-    const int W = cache.head_dim / 32;
-    const int per_token = cache.kv_heads * W * 4;
-    const long long n = (long long)tokens * per_token, first = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    for (long long i = first; (i & ~31ll) < n; i += (long long)gridDim.x * blockDim.x) {  // whole warps: the shuffles take all lanes
-        const bool live = i < n;
-        const int t = live ? (int)(i / per_token) : 0, r = live ? (int)(i % per_token) : 0;
-        const int c = r & 3, j = (r >> 2) % W, head = (r >> 2) / W;
-        const int slot = live ? slots[t] : -1;
-        const int page = slot >= 0 ? slot / cache.page_size : -1;
-        if (page >= cache.pages) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 80);
-        const bool store = page >= 0 && page < cache.pages;
+    constexpr uint32_t LANES = 4 * W;  // of a row
+    const uint32_t all = (uint32_t)q.tokens * q.cache.kv_heads * LANES;  // (the C entry sees to 32 bits)
+    for (uint32_t at = blockIdx.x * 256 + threadIdx.x; (at & ~31u) < all; at += gridDim.x * 256) {  // whole warps: the lanes of a group meet in shuffles
+        const uint32_t i = at / LANES, r = at % LANES, c = r & 3, j = r >> 2;
+        int token, head;
+        size_t row;
+        const bool store = at < all && q.find(i, token, head, row, 80);
         Eight ek = {}, ev = {};
         if (store) {
-            const size_t at = (size_t)head * cache.head_dim + 32 * j + 8 * c;
-            ek = load8<T, VEC>(k + (size_t)t * ldk + at);
-            ev = load8<T, VEC>(v + (size_t)t * ldv + at);
+            const size_t col = (size_t)head * (32 * W) + 32 * j + 8 * c;
+            ek = load8<T, VEC>(k + (size_t)token * q.ldk + col);
+            ev = load8<T, VEC>(v + (size_t)token * q.ldv + col);
         }
         uint32_t ks, vs;
         const uint32_t kc = quantise8(ek, ks), vc = quantise8(ev, vs);
         if (store) {
-            const size_t row = cache.row(page, head, slot - page * cache.page_size);
-            reinterpret_cast<uint32_t*>(cache.k_codes)[row * (4 * W) + c * W + j] = kc;
-            uint16_t* vd = reinterpret_cast<uint16_t*>(cache.v_codes) + row * (8 * W);
+            reinterpret_cast<uint32_t*>(q.cache.k_codes)[row * (4 * W) + c * W + j] = kc;
+            uint16_t* vd = reinterpret_cast<uint16_t*>(q.cache.v_codes) + row * (8 * W);
             vd[(2 * c) * W + j] = (uint16_t)vc;
             vd[(2 * c + 1) * W + j] = (uint16_t)(vc >> 16);
             if (c == 0) {
-                cache.k_scales[row * W + j] = ks;
-                cache.v_scales[row * W + j] = vs;
+                q.cache.k_scales[row * W + j] = ks;
+                q.cache.v_scales[row * W + j] = vs;
             }
         }
     }
@@ -132,32 +151,38 @@ __device__ __forceinline__ Eight dequantise8(uint32_t codes, uint32_t scales) {
     return e;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) packed_read_kernel(PackedCache cache, const int* __restrict__ slots, T* k, T* v, int ldk, int ldv,
-                                                          int tokens, int* status) {
+template <typename T, int W, bool VEC>
+__global__ void __launch_bounds__(256) packed_read_kernel(T* k, T* v, const RowsCall q) {
     pdl_launch_dependents();
     pdl_wait();
-    const int W = cache.head_dim / 32;
-    const int per_token = cache.kv_heads * W * 4;
-    const long long n = (long long)tokens * per_token;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const int t = (int)(i / per_token), r = (int)(i % per_token);
-        const int c = r & 3, j = (r >> 2) % W, head = (r >> 2) / W;
-        const int slot = slots[t];
-        const int page = slot >= 0 ? slot / cache.page_size : -1;
-        if (page >= cache.pages) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 81);
-        Eight ek = {}, ev = {};
-        if (page >= 0 && page < cache.pages) {
-            const size_t row = cache.row(page, head, slot - page * cache.page_size);
-            const uint32_t kc = reinterpret_cast<const uint32_t*>(cache.k_codes)[row * (4 * W) + c * W + j];
-            const uint16_t* vs = reinterpret_cast<const uint16_t*>(cache.v_codes) + row * (8 * W);
-            const uint32_t vc = (uint32_t)vs[(2 * c) * W + j] | (uint32_t)vs[(2 * c + 1) * W + j] << 16;
-            ek = dequantise8(kc, cache.k_scales[row * W + j]);
-            ev = dequantise8(vc, cache.v_scales[row * W + j]);
+    constexpr uint32_t LANES = 4 * W;
+    constexpr int EACH = 4;  // rows of a thread, fetched together
+    const uint32_t rows = (uint32_t)q.tokens * q.cache.kv_heads, threads = gridDim.x * 256;
+    for (uint32_t first = blockIdx.x * 256 + threadIdx.x; first < rows * LANES; first += threads * EACH) {  // (rows x lanes: the C entry sees to 32 bits)
+        uint32_t kc[EACH], vc[EACH], ks[EACH], vs[EACH];
+        int token[EACH], head[EACH];
+#pragma unroll
+        for (int x = 0; x < EACH; ++x) {
+            const uint32_t at = first + x * threads, i = at / LANES, r = at % LANES, c = r & 3, j = r >> 2;
+            kc[x] = vc[x] = ks[x] = vs[x] = 0;
+            token[x] = -1;
+            size_t row;
+            if (at < rows * LANES && q.find(i, token[x], head[x], row, 81)) {
+                const uint16_t* src = reinterpret_cast<const uint16_t*>(q.cache.v_codes) + row * (8 * W);
+                kc[x] = reinterpret_cast<const uint32_t*>(q.cache.k_codes)[row * (4 * W) + c * W + j];
+                vc[x] = (uint32_t)src[(2 * c) * W + j] | (uint32_t)src[(2 * c + 1) * W + j] << 16;
+                ks[x] = q.cache.k_scales[row * W + j];
+                vs[x] = q.cache.v_scales[row * W + j];
+            }
         }
-        const size_t at = (size_t)head * cache.head_dim + 32 * j + 8 * c;
-        store8<T, VEC>(k + (size_t)t * ldk + at, ek);
-        store8<T, VEC>(v + (size_t)t * ldv + at, ev);
+#pragma unroll
+        for (int x = 0; x < EACH; ++x) {
+            if (token[x] < 0) continue;
+            const uint32_t r = (first + x * threads) % LANES;
+            const size_t at = (size_t)head[x] * (32 * W) + 8 * (4 * (r >> 2) + (r & 3));
+            store8<T, VEC>(k + (size_t)token[x] * q.ldk + at, dequantise8(kc[x], ks[x]));
+            store8<T, VEC>(v + (size_t)token[x] * q.ldv + at, dequantise8(vc[x], vs[x]));
+        }
     }
 }
 
@@ -174,124 +199,187 @@ __device__ __forceinline__ uint32_t weight_key(float w, int row, int n, int keep
 }
 
 constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_HELD = 48 * 1024;  // rows whose keys a block's shared memory holds
 
-// One block per (request, kv head): the budget-th greatest key by its four bytes, most significant first (a histogram
-// of 256 bins each), then the kept rows in order, every warp its own run of rows.
+// A cluster of blocks per (request, kv head), each with a run of its rows, whose keys it holds in shared memory (longer runs are
+// read again each time).  The budget-th greatest key by its four bytes, most significant first: a histogram of 256 bins
+// each, added up over the cluster; then the kept rows in order, every warp its own run of rows.  What bounds it is the
+// chain of barriers: one a byte, two for the ranks.  Lanes with the same byte count as one: rows that nothing has
+// attended all fall into one bin.
 __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(const float* weights, long long slot_stride, int head_stride,
                                                                             const int* __restrict__ seq_rows, const int* __restrict__ seq_slot,
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
                                                                             int kept_head_stride, int budget, int keep_first, int keep_last,
-                                                                            int max_rows) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t chosen[2];
-    __shared__ int greater[32], equal[32];
+                                                                            int max_rows, int held) {
+    extern __shared__ uint32_t keys[];  // [held]
+    __shared__ uint32_t hist[4][256], total[256];
+    __shared__ int greater[32], equal[32], counts[2];
     pdl_launch_dependents();
     pdl_wait();
     const int s = blockIdx.y, h = blockIdx.x, heads = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int blocks = gridDim.z, rank = blockIdx.z;
     const int n = min(max(seq_rows[s], 0), max_rows), slot = seq_slot ? seq_slot[s] : s;
     const float* w = weights + slot * slot_stride + (long long)h * head_stride;
     int* rows = kept_rows + ((size_t)s * heads + h) * budget;
     float* kw = kept_weights ? kept_weights + slot * kept_slot_stride + (long long)h * kept_head_stride : nullptr;
     const int stay = min(n, budget);
-    for (int i = stay + tid; i < budget; i += EVICT_THREADS) rows[i] = -1;
-    if (n <= budget) {
-        for (int i = tid; i < n; i += EVICT_THREADS) {
+    for (int i = stay + rank * EVICT_THREADS + tid; i < budget; i += blocks * EVICT_THREADS) rows[i] = -1;
+    if (n <= budget) {  // (the whole cluster)
+        for (int i = rank * EVICT_THREADS + tid; i < n; i += blocks * EVICT_THREADS) {
             rows[i] = i;
             if (kw) kw[i] = w[i];
         }
         return;
     }
+    // this block's rows: whole runs of 32 for each of its warps
+    const int run = (n + 32 * 32 * blocks - 1) / (32 * 32 * blocks) * 32, begin = min(rank * 32 * run, n), end = min(begin + 32 * run, n);
+    const bool hold = end - begin <= held;
+    const auto key_of = [&](int r) { return hold ? keys[r - begin] : weight_key(w[r], r, n, keep_first, keep_last); };
+    (&hist[0][0])[tid] = 0;
+    if (hold)
+        for (int r = begin + tid; r < end; r += EVICT_THREADS) keys[r - begin] = weight_key(w[r], r, n, keep_first, keep_last);
+    __syncthreads();
     uint32_t prefix = 0;
     int want = budget;  // how many of the rows that share the prefix stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += EVICT_THREADS) hist[i] = 0;
-        __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-        for (int i = tid; i < n; i += EVICT_THREADS) {
-            const uint32_t key = weight_key(w[i], i, n, keep_first, keep_last);
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
+#pragma unroll 1
+    for (int byte = 0; byte < 4; ++byte) {
+        const int shift = 24 - 8 * byte;
+        const uint32_t mask = byte == 0 ? 0u : 0xffffffffu << (shift + 8);
+        for (int r0 = begin + 32 * warp; r0 < end; r0 += EVICT_THREADS) {
+            const int r = r0 + lane;
+            const uint32_t key = r < end ? key_of(r) : 0u;
+            const uint32_t bin = r < end && (key & mask) == prefix ? (key >> shift) & 255 : 256;
+            const uint32_t same = __match_any_sync(0xffffffffu, bin);
+            if (bin < 256 && lane == __ffs(same) - 1) atomicAdd(&hist[byte][bin], __popc(same));
+        }
+        const uint32_t* bins = hist[byte];
+        if (blocks > 1) {
+            cluster_sync();
+            if (tid < 256) {
+                uint32_t sum = 0;
+                for (int b = 0; b < blocks; ++b) sum += __float_as_uint(ld_peer_shared_f32(smem_u32(&hist[byte][tid]), b));
+                total[tid] = sum;
+            }
+            bins = total;
         }
         __syncthreads();
-        if (tid == 0) {
-            int left = want, b = 255;
-            for (; b > 0 && (int)hist[b] < left; --b) left -= (int)hist[b];
-            chosen[0] = (uint32_t)b;
-            chosen[1] = (uint32_t)left;
+        // every warp finds the bin for itself: eight bins a lane, from the greatest down
+        uint32_t mine[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            mine[i] = bins[255 - 8 * lane - i];
+            sum += mine[i];
         }
-        __syncthreads();
-        prefix |= chosen[0] << shift;
-        want = (int)chosen[1];
-        __syncthreads();
+        uint32_t upto = sum;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, x);
+            if (lane >= x) upto += v;
+        }
+        const int owner = __ffs(__ballot_sync(0xffffffffu, upto >= (uint32_t)want)) - 1;
+        uint32_t before = upto - sum;
+        int bin = 0, left = want;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (!found && before + mine[i] >= (uint32_t)want) {
+                found = true;
+                bin = 255 - 8 * lane - i;
+                left = want - (int)before;
+            }
+            before += mine[i];
+        }
+        prefix |= (uint32_t)__shfl_sync(0xffffffffu, bin, owner) << shift;
+        want = __shfl_sync(0xffffffffu, left, owner);
+        __syncthreads();  // (`total` is read no more)
     }
     // rows with key > prefix all stay, of those with key == prefix the first `want`
-    const int run = (n + 1023) / 1024 * 32, begin = min(warp * run, n), end = min(begin + run, n);
+    const int from = min(begin + warp * run, end), to = min(from + run, end);
     int gt = 0, eq = 0;
-    for (int i = begin; i < end; i += 32) {
+    for (int i = from; i < to; i += 32) {
         const int r = i + lane;
-        const uint32_t key = r < end ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
-        gt += __popc(__ballot_sync(0xffffffffu, r < end && key > prefix));
-        eq += __popc(__ballot_sync(0xffffffffu, r < end && key == prefix));
+        const uint32_t key = r < to ? key_of(r) : 0u;
+        gt += __popc(__ballot_sync(0xffffffffu, r < to && key > prefix));
+        eq += __popc(__ballot_sync(0xffffffffu, r < to && key == prefix));
     }
     if (lane == 0) {
         greater[warp] = gt;
         equal[warp] = eq;
     }
     __syncthreads();
-    int before_gt = 0, before_eq = 0;
-    for (int i = 0; i < warp; ++i) {
-        before_gt += greater[i];
-        before_eq += equal[i];
+    int before_gt = lane < warp ? greater[lane] : 0, before_eq = lane < warp ? equal[lane] : 0;
+    before_gt = __reduce_add_sync(0xffffffffu, before_gt);
+    before_eq = __reduce_add_sync(0xffffffffu, before_eq);
+    if (blocks > 1) {
+        if (warp == 31 && lane == 0) {
+            counts[0] = before_gt + gt;
+            counts[1] = before_eq + eq;
+        }
+        cluster_sync();
+        for (int b = 0; b < rank; ++b) {
+            before_gt += (int)__float_as_uint(ld_peer_shared_f32(smem_u32(&counts[0]), b));
+            before_eq += (int)__float_as_uint(ld_peer_shared_f32(smem_u32(&counts[1]), b));
+        }
+        cluster_arrive_release();  // (a block's shared memory stays until all have read it)
     }
-    for (int i = begin; i < end; i += 32) {
+    for (int i = from; i < to; i += 32) {
         const int r = i + lane;
-        const float wr = r < end ? w[r] : 0.0f;
-        const uint32_t key = r < end ? weight_key(wr, r, n, keep_first, keep_last) : 0u;
-        const uint32_t above = __ballot_sync(0xffffffffu, r < end && key > prefix);
-        const uint32_t same = __ballot_sync(0xffffffffu, r < end && key == prefix);
+        const uint32_t key = r < to ? key_of(r) : 0u;
+        const uint32_t above = __ballot_sync(0xffffffffu, r < to && key > prefix);
+        const uint32_t same = __ballot_sync(0xffffffffu, r < to && key == prefix);
         const uint32_t lower = (1u << lane) - 1;
-        const int rank = before_eq + __popc(same & lower);
-        const bool stays = r < end && (key > prefix || (key == prefix && rank < want));
+        const int place = before_eq + __popc(same & lower);  // among the equal ones
+        const bool stays = r < to && (key > prefix || (key == prefix && place < want));
         if (stays) {
-            const int at = before_gt + __popc(above & lower) + min(rank, want);
+            const int at = before_gt + __popc(above & lower) + min(place, want);
             rows[at] = r;
-            if (kw) kw[at] = wr;
+            if (kw) kw[at] = w[r];
         }
         before_gt += __popc(above);
         before_eq += __popc(same);
     }
+    if (blocks > 1) cluster_wait();
 }
 
-// Kept rows from their pages into others: block (rows, head, request), a thread 16 bytes of codes or one word of scales.
+// Kept rows from their pages into others: every thread 16 bytes of codes of a row's keys and of its values, W threads a row, and the
+// rows' scales by the same threads; four rows of a thread are fetched together.
+template <int W>
 __global__ void __launch_bounds__(256) packed_evict_move_kernel(PackedCache from, PackedCache to, const int* __restrict__ from_tables,
                                                                 int from_width, const int* __restrict__ to_tables, int to_width,
-                                                                const int* kept_rows, int budget, int rows_per_block, int* status) {
+                                                                const int* kept_rows, int budget, DivideBy from_page, DivideBy to_page, int* status) {
     pdl_launch_dependents();
     pdl_wait();
-    const int s = blockIdx.z, h = blockIdx.y, heads = gridDim.y, W = from.head_dim / 32, ps = from.page_size, qs = to.page_size;
+    constexpr int EACH = 4, ROWS = 256 / W;  // rows that a block takes at once
+    const int s = blockIdx.z, h = blockIdx.y, heads = gridDim.y, part = threadIdx.x % W;
     const int* kept = kept_rows + ((size_t)s * heads + h) * budget;
-    const int first = blockIdx.x * rows_per_block, count = min(rows_per_block, budget - first);
-    const int per_row = 4 * W;  // W pieces of 16 bytes of codes and W words of scales, of keys and of values
-    for (int i = threadIdx.x; i < count * per_row; i += blockDim.x) {
-        const int at = first + i / per_row, part = i % per_row;
-        const int row = kept[at];
-        if (row < 0 || row / ps >= from_width || at / qs >= to_width) continue;
-        const int sp = from_tables[(size_t)s * from_width + row / ps], dp = to_tables[(size_t)s * to_width + at / qs];
-        if (sp < 0 || dp < 0) continue;
-        if (sp >= from.pages || dp >= to.pages) {
-            ferris_report(status, FERRIS_STATUS_BAD_INDEX, 82);
-            continue;
-        }
-        const size_t a = from.row(sp, h, row % ps), b = to.row(dp, h, at % qs);
-        const int j = part % W;
-        if (part < W) {
-            reinterpret_cast<uint4*>(to.k_codes)[b * W + j] = reinterpret_cast<const uint4*>(from.k_codes)[a * W + j];
-        } else if (part < 2 * W) {
-            reinterpret_cast<uint4*>(to.v_codes)[b * W + j] = reinterpret_cast<const uint4*>(from.v_codes)[a * W + j];
-        } else if (part < 3 * W) {
-            to.k_scales[b * W + j] = from.k_scales[a * W + j];
-        } else {
-            to.v_scales[b * W + j] = from.v_scales[a * W + j];
-        }
+    if (threadIdx.x >= ROWS * W) return;
+    uint4 kc[EACH], vc[EACH];
+    uint32_t ks[EACH], vs[EACH];
+    size_t dst[EACH];
+    bool live[EACH];
+#pragma unroll
+    for (int x = 0; x < EACH; ++x) {
+        const int at = (blockIdx.x * EACH + x) * ROWS + threadIdx.x / W, row = at < budget ? kept[at] : -1;
+        const int sb = row >= 0 ? (int)from_page.quotient(row) : 0, db = (int)to_page.quotient(at);
+        live[x] = row >= 0 && sb < from_width && db < to_width;
+        const int sp = live[x] ? from_tables[(size_t)s * from_width + sb] : -1, dp = live[x] ? to_tables[(size_t)s * to_width + db] : -1;
+        if (sp >= from.pages || dp >= to.pages) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 82);
+        live[x] = sp >= 0 && dp >= 0 && sp < from.pages && dp < to.pages;
+        if (!live[x]) continue;
+        const size_t a = from.row(sp, h, row - sb * from.page_size) * W + part;
+        dst[x] = to.row(dp, h, at - db * to.page_size) * W + part;
+        kc[x] = reinterpret_cast<const uint4*>(from.k_codes)[a];
+        vc[x] = reinterpret_cast<const uint4*>(from.v_codes)[a];
+        ks[x] = from.k_scales[a];
+        vs[x] = from.v_scales[a];
+    }
+#pragma unroll
+    for (int x = 0; x < EACH; ++x) {
+        if (!live[x]) continue;
+        reinterpret_cast<uint4*>(to.k_codes)[dst[x]] = kc[x];
+        reinterpret_cast<uint4*>(to.v_codes)[dst[x]] = vc[x];
+        to.k_scales[dst[x]] = ks[x];
+        to.v_scales[dst[x]] = vs[x];
     }
 }
 
@@ -304,26 +392,45 @@ bool eights_aligned(const void* p, int ld) {
     return ((uintptr_t)p & 15) == 0 && ld % (16 / (int)sizeof(T)) == 0;
 }
 
-int blocks_for(long long threads) {
-    const long long most = (long long)(ferris_sm_count() > 0 ? ferris_sm_count() : 148) * 8;
-    const long long blocks = (threads + 255) / 256;
-    return (int)(blocks < most ? blocks : most);
-}
+int sms() { return ferris_sm_count() > 0 ? ferris_sm_count() : 148; }
 
-template <typename T>
-int write_rows(const void* k, const void* v, int ldk, int ldv, const int* slots, const PackedCache& cache, int tokens, cudaStream_t st) {
-    const int blocks = blocks_for((long long)tokens * cache.kv_heads * (cache.head_dim / 8));
-    auto kernel = eights_aligned<T>(k, ldk) && eights_aligned<T>(v, ldv) ? packed_write_kernel<T, true> : packed_write_kernel<T, false>;
-    ferris_launch(kernel, dim3(blocks), dim3(256), 0, st, (const T*)k, (const T*)v, ldk, ldv, slots, cache, tokens, ferris_status_ptr());
+template <typename T, int W>
+int write_rows(const void* k, const void* v, const RowsCall& q, cudaStream_t st) {
+    const bool vec = eights_aligned<T>(k, q.ldk) && eights_aligned<T>(v, q.ldv);
+    const long long need = ((long long)q.tokens * q.cache.kv_heads * 4 * W + 255) / 256, most = sms() * 8;
+    const int blocks = (int)(need < most ? need : most);
+    if (vec)
+        ferris_launch(packed_write_kernel<T, W, true>, dim3(blocks), dim3(256), 0, st, (const T*)k, (const T*)v, q);
+    else
+        ferris_launch(packed_write_kernel<T, W, false>, dim3(blocks), dim3(256), 0, st, (const T*)k, (const T*)v, q);
     FERRIS_LAUNCH_CHECK();
 }
 
-template <typename T>
-int read_rows(const PackedCache& cache, const int* slots, void* k, void* v, int ldk, int ldv, int tokens, cudaStream_t st) {
-    const int blocks = blocks_for((long long)tokens * cache.kv_heads * (cache.head_dim / 8));
-    auto kernel = eights_aligned<T>(k, ldk) && eights_aligned<T>(v, ldv) ? packed_read_kernel<T, true> : packed_read_kernel<T, false>;
-    ferris_launch(kernel, dim3(blocks), dim3(256), 0, st, cache, slots, (T*)k, (T*)v, ldk, ldv, tokens, ferris_status_ptr());
+template <typename T, int W>
+int read_rows(void* k, void* v, const RowsCall& q, cudaStream_t st) {
+    const bool vec = eights_aligned<T>(k, q.ldk) && eights_aligned<T>(v, q.ldv);
+    const long long need = ((long long)q.tokens * q.cache.kv_heads * 4 * W + 255) / 256, most = sms() * 8;
+    const int blocks = (int)(need < most ? need : most);
+    if (vec)
+        ferris_launch(packed_read_kernel<T, W, true>, dim3(blocks), dim3(256), 0, st, (T*)k, (T*)v, q);
+    else
+        ferris_launch(packed_read_kernel<T, W, false>, dim3(blocks), dim3(256), 0, st, (T*)k, (T*)v, q);
     FERRIS_LAUNCH_CHECK();
+}
+
+// f<W>() for heads of 32 W elements.
+template <typename F>
+int with_groups(int head_dim, F&& f) {
+    switch (head_dim / 32) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 3: return f(std::integral_constant<int, 3>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 5: return f(std::integral_constant<int, 5>());
+        case 6: return f(std::integral_constant<int, 6>());
+        case 7: return f(std::integral_constant<int, 7>());
+        default: return f(std::integral_constant<int, 8>());
+    }
 }
 
 }  // namespace
@@ -338,21 +445,28 @@ struct FerrisPackedRows {
     PackedCache cache() const { return make_cache(k_codes, k_scales, v_codes, v_scales, pages, kv_heads, page_size, head_dim); }
 };
 
-FERRIS_API int ferris_packed_cache_write(const FerrisPackedRows* a) {
-    if (const char* why = packed_cache_refusal(a->cache())) FERRIS_REFUSE("%s", why);
+namespace {
+
+template <bool WRITE>
+int rows_call(const FerrisPackedRows* a) {
+    const PackedCache cache = a->cache();
+    if (const char* why = packed_cache_refusal(cache)) FERRIS_REFUSE("%s", why);
     if (a->tokens <= 0) return FERRIS_OK;
-    if (a->dtype == FERRIS_BF16) return write_rows<bf16>(a->k, a->v, a->ldk, a->ldv, a->slots, a->cache(), a->tokens, (cudaStream_t)a->stream);
-    if (a->dtype == FERRIS_F32) return write_rows<float>(a->k, a->v, a->ldk, a->ldv, a->slots, a->cache(), a->tokens, (cudaStream_t)a->stream);
-    FERRIS_REFUSE("packed cache: dtype %d is not known", a->dtype);
+    if ((long long)a->tokens * a->kv_heads * (a->head_dim / 8) > 0x3fffffffll) FERRIS_REFUSE("packed cache: %d tokens in one call", a->tokens);
+    if (a->dtype != FERRIS_BF16 && a->dtype != FERRIS_F32) FERRIS_REFUSE("packed cache: dtype %d is not known", a->dtype);
+    const RowsCall q = {a->slots, cache, a->tokens, a->ldk, a->ldv, DivideBy(a->kv_heads), DivideBy(a->page_size), ferris_status_ptr()};
+    cudaStream_t st = (cudaStream_t)a->stream;
+    return with_groups(a->head_dim, [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        if (WRITE) return a->dtype == FERRIS_BF16 ? write_rows<bf16, W>(a->k, a->v, q, st) : write_rows<float, W>(a->k, a->v, q, st);
+        return a->dtype == FERRIS_BF16 ? read_rows<bf16, W>(a->k, a->v, q, st) : read_rows<float, W>(a->k, a->v, q, st);
+    });
 }
 
-FERRIS_API int ferris_packed_cache_read(const FerrisPackedRows* a) {
-    if (const char* why = packed_cache_refusal(a->cache())) FERRIS_REFUSE("%s", why);
-    if (a->tokens <= 0) return FERRIS_OK;
-    if (a->dtype == FERRIS_BF16) return read_rows<bf16>(a->cache(), a->slots, a->k, a->v, a->ldk, a->ldv, a->tokens, (cudaStream_t)a->stream);
-    if (a->dtype == FERRIS_F32) return read_rows<float>(a->cache(), a->slots, a->k, a->v, a->ldk, a->ldv, a->tokens, (cudaStream_t)a->stream);
-    FERRIS_REFUSE("packed cache: dtype %d is not known", a->dtype);
-}
+}  // namespace
+
+FERRIS_API int ferris_packed_cache_write(const FerrisPackedRows* a) { return rows_call<true>(a); }
+FERRIS_API int ferris_packed_cache_read(const FerrisPackedRows* a) { return rows_call<false>(a); }
 
 FERRIS_API int ferris_packed_cache_evict(void* from_kc, void* from_ks, void* from_vc, void* from_vs, int from_pages, int from_page_size,
                                          void* to_kc, void* to_ks, void* to_vc, void* to_vs, int to_pages, int to_page_size, int kv_heads,
@@ -369,13 +483,20 @@ FERRIS_API int ferris_packed_cache_evict(void* from_kc, void* from_ks, void* fro
     if (seqs <= 0) return FERRIS_OK;
     if (seqs > 65535 || kv_heads > 65535) FERRIS_REFUSE("eviction: %d requests of %d kv heads", seqs, kv_heads);
     cudaStream_t st = (cudaStream_t)stream;
-    cudaError_t e = ferris_launch(packed_evict_select_kernel, dim3(kv_heads, seqs), dim3(EVICT_THREADS), 0, st, weights, slot_stride, head_stride,
-                                  seq_rows, seq_slot, kept_rows, kept_weights, kept_slot_stride, kept_head_stride, budget, keep_first,
-                                  keep_last, max_rows);
-    if (e == cudaSuccess) {
-        const int rows_per_block = 64;
-        ferris_launch(packed_evict_move_kernel, dim3((budget + rows_per_block - 1) / rows_per_block, kv_heads, seqs), dim3(256), 0, st, from, to,
-                      from_tables, from_width, to_tables, to_width, (const int*)kept_rows, budget, rows_per_block, ferris_status_ptr());
-    }
-    FERRIS_LAUNCH_CHECK();
+    // blocks of a cluster: about 8,192 rows each, at most eight (the most that is portable)
+    int blocks = 1;
+    while (blocks < 8 && (long long)blocks * 8192 < max_rows) blocks *= 2;
+    const int each = ((max_rows + 1024 * blocks - 1) / (1024 * blocks)) * 1024, held = each < EVICT_HELD ? each : EVICT_HELD;
+    if (const int r = ferris_allow_dynamic_smem((const void*)packed_evict_select_kernel, (size_t)held * 4)) return r;
+    cudaError_t e = ferris_launch_cluster(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,
+                                          weights, slot_stride, head_stride, seq_rows, seq_slot, kept_rows, kept_weights, kept_slot_stride,
+                                          kept_head_stride, budget, keep_first, keep_last, max_rows, held);
+    if (e != cudaSuccess) FERRIS_LAUNCH_CHECK();
+    return with_groups(head_dim, [&](auto w) {
+        constexpr int W = decltype(w)::value, ROWS = 256 / W * 4;
+        ferris_launch(packed_evict_move_kernel<W>, dim3((budget + ROWS - 1) / ROWS, kv_heads, seqs), dim3(256), 0, st, from, to, from_tables,
+                      from_width, to_tables, to_width, (const int*)kept_rows, budget, DivideBy(from_page_size), DivideBy(to_page_size),
+                      ferris_status_ptr());
+        FERRIS_LAUNCH_CHECK();
+    });
 }

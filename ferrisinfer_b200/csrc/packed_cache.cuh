@@ -13,6 +13,20 @@
 #include "common.cuh"
 #include "sm100.cuh"
 
+// n / d for n below 2^31 by a multiplication: multiplier = ceil(2^(32 + shift) / d) with 2^shift < d <= 2^(shift + 1).
+struct DivideBy {
+    uint32_t multiplier;
+    int shift;
+
+    explicit DivideBy(int d) : multiplier(0), shift(0) {
+        if (d <= 1) return;
+        while ((2ll << shift) < d) ++shift;
+        multiplier = (uint32_t)(((1ull << (32 + shift)) + d - 1) / d);
+    }
+    DivideBy() = default;
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return multiplier ? __umulhi(n, multiplier) >> shift : n; }
+};
+
 struct PackedCache {
     uint8_t* k_codes;
     uint32_t* k_scales;

@@ -204,8 +204,8 @@ constexpr int EVICT_HELD = 48 * 1024;  // rows whose keys a block's shared memor
 // A cluster of blocks per (request, kv head), each with a run of its rows, whose keys it holds in shared memory (longer runs are
 // read again each time).  The budget-th greatest key by its four bytes, most significant first: a histogram of 256 bins
 // each, added up over the cluster; then the kept rows in order, every warp its own run of rows.  What bounds it is the
-// chain of barriers: one a byte, two for the ranks.  Lanes with the same byte count as one: rows that nothing has
-// attended all fall into one bin.
+// chain of barriers: one a byte, two for the ranks.  Lanes that share a bin count as one (rows that nothing has
+// attended all fall into one) where that is quick to see: `match.any` took half of the kernel's time.
 __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(const float* weights, long long slot_stride, int head_stride,
                                                                             const int* __restrict__ seq_rows, const int* __restrict__ seq_slot,
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
@@ -249,8 +249,16 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
             const int r = r0 + lane;
             const uint32_t key = r < end ? key_of(r) : 0u;
             const uint32_t bin = r < end && (key & mask) == prefix ? (key >> shift) & 255 : 256;
-            const uint32_t same = __match_any_sync(0xffffffffu, bin);
-            if (bin < 256 && lane == __ffs(same) - 1) atomicAdd(&hist[byte][bin], __popc(same));
+            uint32_t rest = __ballot_sync(0xffffffffu, bin < 256);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // the bins of two lanes for all that share them, the others one by one
+                if (!rest) break;
+                const int lead = __ffs(rest) - 1;
+                const uint32_t same = __ballot_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, lead));
+                if (lane == lead) atomicAdd(&hist[byte][bin], __popc(same));
+                rest &= ~same;
+            }
+            if (rest >> lane & 1) atomicAdd(&hist[byte][bin], 1u);
         }
         const uint32_t* bins = hist[byte];
         if (blocks > 1) {

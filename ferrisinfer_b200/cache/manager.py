@@ -24,7 +24,8 @@ Here ONE manager serves all requests:
 * Every pool has one page more than it hands out, and every state tensor one slot more
   (``padding_page``, ``padding_slot``): rows that only fill a step up to a recorded batch size write
   their key, value and state there, where no request ever reads.
-* A need of another kind than these two brings its own builder (``register_cache_need``).
+* A ``PackedKV`` need is a ``PagedKV`` whose pages hold keys and values in 4 bits.
+* A need of another kind than these brings its own builder (``register_cache_need``).
 * With prefix sharing, full pages of prompts are found by later requests through a chain hash and
   shared, not copied.  With ``keep_finished`` the index holds a reference of its own, so the pages of
   a prompt outlive the request that computed them; they count as free, and the least recently used
@@ -40,7 +41,7 @@ from typing import Any, Optional
 import torch
 
 from ..errors import CacheError, OutOfPages
-from ..parts.base import CombinedNeed, FixedState, LayerCache, PagedKV, leaf_needs
+from ..parts.base import CombinedNeed, FixedState, LayerCache, PackedKV, PagedKV, leaf_needs
 from .pages import PagePool
 
 NO_PAGE = -1
@@ -163,6 +164,17 @@ def _build_paged(manager, index, need):
     return cache
 
 
+def _build_packed(manager, index, need):
+    from ..kernels import ops
+
+    g = manager.page_group(need)
+    g.members.append(index)
+    cache = LayerCache(need=need, group=g.gid)
+    if manager.device is not None:  # (one page beyond the pool's, as above)
+        cache.packed = ops.PackedPages.empty(g.pool.num_pages + 1, need.num_kv_heads, manager.page_size, need.head_dim, manager.device)
+    return cache
+
+
 def _build_state(manager, index, need):
     return LayerCache(need=need, state=manager.new_state(need.shape, need.dtype))
 
@@ -171,6 +183,7 @@ def _build_combined(manager, index, need):
     return LayerCache(need=need, parts=[None if n is None else manager.build_cache(index, n) for n in need.needs])
 
 
+register_cache_need(PackedKV, _build_packed)  # (before the kind that it is a case of)
 register_cache_need(PagedKV, _build_paged)
 register_cache_need(FixedState, _build_state)
 register_cache_need(CombinedNeed, _build_combined)

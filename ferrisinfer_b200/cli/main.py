@@ -18,7 +18,8 @@ Where the reference takes a text, this CLI takes token ids separated by commas o
 out is the tokenizer's business (the chat, render and tokenize commands are not part of the engine).
 Options (all optional, before or after the command): --model DIR, --dtype bfloat16|float32,
 --temperature T --top-k K --top-p P --seed S (the reference's sampler fields; default greedy),
---random CONFIG.json --random-seed S (random weights instead of a folder), --page-size, --num-pages.
+--random CONFIG.json --random-seed S (random weights instead of a folder), --page-size, --num-pages,
+--cache-bits 4 (keys and values held in 4 bits).
 """
 
 from __future__ import annotations
@@ -47,6 +48,7 @@ def _parser():
     p.add_argument("--random-seed", type=int, default=0)
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--num-pages", type=int, default=None)
+    p.add_argument("--cache-bits", type=int, default=None, choices=[4])
     p.add_argument("-h", "--help", action="store_true")
     return p
 
@@ -73,8 +75,9 @@ def _engine(ns):
 
     if ns.random:
         return Engine(config=ns.random, seed=ns.random_seed, dtype=ns.dtype, page_size=ns.page_size,
-                      num_pages=ns.num_pages)
-    return Engine(ns.model or DEFAULT_HF_PATH, dtype=ns.dtype, page_size=ns.page_size, num_pages=ns.num_pages)
+                      num_pages=ns.num_pages, cache_bits=ns.cache_bits)
+    return Engine(ns.model or DEFAULT_HF_PATH, dtype=ns.dtype, page_size=ns.page_size, num_pages=ns.num_pages,
+                  cache_bits=ns.cache_bits)
 
 
 def _rate(n, seconds):

@@ -46,6 +46,9 @@ Options beyond the reference's layer, each a parameter of its own:
                         lambda v1 as its values, v1 being the values that the layer with "source" projected for the same
                         token in this pass; the source's own number is read if the folder has it, and not used
   ``fp32_weights``      the softmax's weights and the weighted sum of values stay in 32-bit (the general kernel)
+  ``cache_bits``        4: keys (rotated) and values are held in 4 bits (``PackedKV``) and attended by the kernels of the packed
+                        cache, in either precision; for the plain layer (a window may stand with it) whose heads have a
+                        multiple of 32 elements, at most 256
   a ``scaled_rotary`` position encoding (either pair layout, part of a head, scaled frequencies) rotates in the kernel
   that also norms and writes the cache; it goes with ``qk_norm``, ``values_from_keys``, ``chunk`` and value heads of
   their own size, not with the unit norm or the temperature
@@ -62,7 +65,7 @@ from typing import Optional
 import torch
 
 from ..kernels import ops
-from .base import CombinedNeed, LayerCache, Mixer, PagedKV, PositionEncoding, TensorSpec
+from .base import CombinedNeed, LayerCache, Mixer, PackedKV, PagedKV, PositionEncoding, TensorSpec
 from .plan import PartSpec, build_part, register_part
 from .recurrent import _fused_rows
 
@@ -84,7 +87,7 @@ class GroupedQueryAttention(Mixer):
                  values_from_keys: bool = False, qk_norm: Optional[dict] = None, chunk: Optional[int] = None,
                  fp32_weights: bool = False, output_gate: Optional[dict] = None, output_scale: float = 1.0,
                  pool: Optional[int] = None, value_mix: Optional[dict] = None, keep_first: int = 0,
-                 softcap: Optional[float] = None):
+                 softcap: Optional[float] = None, cache_bits: Optional[int] = None):
         if num_heads % num_kv_heads:
             raise ValueError(f"{num_heads} heads cannot share {num_kv_heads} kv heads")
         self.hidden_size, self.num_heads = int(hidden_size), int(num_heads)
@@ -166,6 +169,13 @@ class GroupedQueryAttention(Mixer):
         if not self.plain and not hasattr(self.position, "table") and getattr(self.position, "rotary_dim", 0):
             raise ValueError("unit-norm keys, a query temperature or value heads of their own size go with a "
                              "position encoding that rotates nothing")
+        self.cache_bits = None if cache_bits is None else int(cache_bits)
+        if self.cache_bits is not None:
+            if self.cache_bits != 4 or self.head_dim % ops.PACKED_GROUP or self.head_dim > 256:
+                raise ValueError(f"a cache of {cache_bits} bits for heads of {self.head_dim} (4 bits, a multiple of {ops.PACKED_GROUP} "
+                                 "elements, at most 256)")
+            if not self.plain or type(self.position).score_slopes is not PositionEncoding.score_slopes:
+                raise ValueError("a cache of 4 bits goes with the plain attention layer: no options but a window, no penalty on the scores")
         self.tensor_names = dict(tensor_names) if tensor_names else None
         self.bias_names = dict(bias_names) if bias_names else None
         self.qkv_weight = self.qkv_bias = self.o_weight = None
@@ -244,6 +254,8 @@ class GroupedQueryAttention(Mixer):
 
     # -------------------------------------------------------------------- cache
     def cache_need(self):
+        if self.cache_bits is not None:
+            return PackedKV(self.num_kv_heads, self.head_dim, self.window)
         dv = None if self.v_head_dim == self.head_dim else self.v_head_dim
         need = PagedKV(self.num_kv_heads, self.head_dim, self.window, dv, chunk=self.chunk, run=self.pool,
                        keep_first=self.keep_first)
@@ -299,6 +311,9 @@ class GroupedQueryAttention(Mixer):
                 ops.gate_mul(out, gate, out, self.output_gate[1], self.output_scale)
             ops.gemm(out, self.o_weight, None, h, accumulate=accumulate, fixed_weight=True)
             return
+        if self.cache_bits is not None:
+            self._forward_packed(x, h, qkv, ctx, meta, cache, owns_cache, accumulate)
+            return
         table = self.position.rotary_table(qkv.device)
         inv_freq, rotary = table if table is not None else (None, 0)
         slopes = self.position.score_slopes(nh, qkv.device)
@@ -320,6 +335,30 @@ class GroupedQueryAttention(Mixer):
                                       self.window or 0, self.scale, write_kv=owns_cache, lazy_merge=True,
                                       rotated=fused, score_slopes=slopes)
         ops.gemm(attended, self.o_weight, None, h, accumulate=accumulate, fixed_weight=True)
+
+
+    def _forward_packed(self, x, h, qkv, ctx, meta, cache, owns_cache, accumulate):
+        """The plain layer over a cache in 4 bits."""
+        T, nh, nkv, d = x.shape[0], self.num_heads, self.num_kv_heads, self.head_dim
+        ops.gemm(x, self.qkv_weight, self.qkv_bias, qkv, fixed_weight=True)
+        table = self.position.rotary_table(qkv.device)
+        k, v = qkv[:, self.q_size:self.q_size + self.kv_size], qkv[:, self.q_size + self.kv_size:]
+        if table is None:
+            self.position.apply(qkv, ctx.positions, nh, nkv, d)
+        elif table[1]:
+            # the rotation leaves k and v in rows of their own: pages of one token
+            rows = ctx.workspace.get("packed_rows", (2, T, nkv, 1, d), x.dtype)
+            order = ctx.shared.get("row_order")
+            if order is None:
+                order = ctx.shared["row_order"] = torch.arange(T, dtype=torch.int32, device=qkv.device)
+            ops.rope_cache_write(qkv, ctx.positions, table[0], order, rows[0], rows[1], nh, nkv, d, table[1], 1, write_kv=owns_cache)
+            k, v = rows[0].view(T, self.kv_size), rows[1].view(T, self.kv_size)
+        if owns_cache:
+            ops.packed_cache_write(k, v, meta.slot_mapping, cache.packed)
+        out = ctx.workspace.get("attn_out", (T, self.q_size), x.dtype)
+        ops.packed_attention(qkv, out, cache.packed, meta.block_tables, ctx.seq_q_start, ctx.seq_start_pos, ctx.max_q_len, ctx.max_kv_len,
+                             nh, self.scale, window=self.window or 0, workspace=ctx.workspace)
+        ops.gemm(out, self.o_weight, None, h, accumulate=accumulate, fixed_weight=True)
 
 
 register_part("mixer", "gqa_attention", GroupedQueryAttention)

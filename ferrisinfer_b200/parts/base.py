@@ -79,6 +79,12 @@ class PagedKV:
 
 
 @dataclass(frozen=True)
+class PackedKV(PagedKV):
+    """A ``PagedKV`` whose keys and values are held in 4 bits (``ops.PackedPages``): the mixer writes and reads them with the
+    kernels of the packed cache, whatever the compute dtype.  Key and value heads of one size, a row per token, no chunks."""
+
+
+@dataclass(frozen=True)
 class FixedState:
     """The mixer keeps a tensor of ``shape`` per request, whatever the request's length.
     It is zeroed when a request is admitted."""
@@ -166,14 +172,15 @@ class LayerCache:
     """What one run of a layer's mixer owns in the cache.
 
     ``group``: id of the page group (PagedKV) whose block tables address ``k`` and ``v``
-    ([pages, kv heads, page size, head dim]); ``state``: [slots, *shape] for FixedState; ``parts``: the caches
-    of a CombinedNeed's needs.
+    ([pages, kv heads, page size, head dim]), or ``packed``, the pages of a PackedKV; ``state``: [slots, *shape] for
+    FixedState; ``parts``: the caches of a CombinedNeed's needs.
     """
 
     need: Any
     group: Optional[int] = None
     k: Optional[torch.Tensor] = None
     v: Optional[torch.Tensor] = None
+    packed: Any = None
     state: Optional[torch.Tensor] = None
     parts: Optional[list] = None
 
@@ -336,6 +343,6 @@ def role_dtype(role: str, compute_dtype: torch.dtype, stored: torch.dtype) -> to
 
 
 __all__ = [
-    "PagedKV", "FixedState", "CombinedNeed", "leaf_needs", "PagedMeta", "SeqInfo", "StepContext", "LayerCache", "Part", "Norm",
+    "PagedKV", "PackedKV", "FixedState", "CombinedNeed", "leaf_needs", "PagedMeta", "SeqInfo", "StepContext", "LayerCache", "Part", "Norm",
     "PositionEncoding", "Mixer", "FeedForward", "Block", "TensorSpec", "role_dtype",
 ]

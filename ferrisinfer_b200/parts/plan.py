@@ -15,7 +15,7 @@ the code that runs them.
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Any, Optional
 
 
@@ -99,6 +99,17 @@ class ModelPlan:
     # run as x / m <- x / m + y: the plan's embedding is divided by m, and a norm over x / m with eps / m^2 is the norm over x
     # with eps, so the factor costs nothing and no weight is rounded again.
     residual_unit: float = 1.0
+
+    def with_cache_bits(self, bits: Optional[int]) -> "ModelPlan":
+        """The same model with its attention layers' keys and values held in ``bits`` (4; None: in the compute dtype).  Every layer
+        must be a plain ``gqa_attention``."""
+        if bits is None:
+            return self
+        for layer in self.layers:
+            if layer.mixer.kind != "gqa_attention":
+                raise ValueError(f"{layer.prefix}: a cache of {bits} bits goes with plain attention layers, not with '{layer.mixer.kind}'")
+        return replace(self, layers=tuple(replace(layer, mixer=PartSpec(layer.mixer.kind, {**layer.mixer.params, "cache_bits": bits}))
+                                          for layer in self.layers))
 
     def validate(self) -> None:
         if self.residual_streams < 1:

@@ -164,14 +164,14 @@ def _to_device_pipelined(st: SafetensorsFolder, names: list, device: torch.devic
     return out
 
 
-def load_model(folder: str, dtype="bfloat16", device="cuda", strict: bool = True) -> tuple:
+def load_model(folder: str, dtype="bfloat16", device="cuda", strict: bool = True, cache_bits: Optional[int] = None) -> tuple:
     """(model, config) of ``folder`` (config.json + safetensors), bound to ``device``.
     ``strict`` False: tensors of the folder that no part asks for are left alone instead of being an error;
-    their names are in ``model.unexpected_tensors``."""
+    their names are in ``model.unexpected_tensors``.  ``cache_bits``: see ``ModelPlan.with_cache_bits``."""
     compute_dtype = parse_dtype(dtype)
     device = torch.device(device)
     arch, cfg = resolve_config(folder)
-    model = build_model(arch.plan(cfg))
+    model = build_model(arch.plan(cfg).with_cache_bits(cache_bits))
     st = SafetensorsFolder(folder)
     try:
         specs = model.tensor_specs()

@@ -29,6 +29,15 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same into nothing: c = A B.
+__device__ __forceinline__ void mma_f16_16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // 16 (or 8, or 4) bytes global -> shared without registers; `live` false: zeros, and nothing is read.
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
@@ -90,9 +99,9 @@ struct Stage {
             const int piece = i * 32 + lane, r = piece / W, part = piece % W;
             const uint32_t a = __shfl_sync(0xffffffffu, at, r);
             const bool live = there >> r & 1;
-            const size_t src = (size_t)a * (16 * W) + 16 * part;
-            copy_async<16>(dst + r * K_ROW + 16 * part, p.cache.k_codes + src, live);
-            copy_async<16>(dst + V_AT + r * V_ROW + 16 * part, p.cache.v_codes + src, live);
+            // (the piece's offset belongs to the base: a row then costs one wide multiply-add)
+            copy_async<16>(dst + r * K_ROW + 16 * part, (p.cache.k_codes + 16 * part) + (size_t)a * (16 * W), live);
+            copy_async<16>(dst + V_AT + r * V_ROW + 16 * part, (p.cache.v_codes + 16 * part) + (size_t)a * (16 * W), live);
         }
         constexpr int N = W % 4 == 0 ? 16 : W % 2 == 0 ? 8 : 4;
 #pragma unroll
@@ -218,12 +227,17 @@ struct Keys {
             const float s0 = packed_scale(scale[0][j]), s1 = packed_scale(scale[1][j]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float d[4];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const uint32_t a[4] = {a0[2 * t], a1[2 * t], a0[2 * t + 1], a1[2 * t + 1]};
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) mma_f16_16816(d, a, q[n].b[j][t][0][i], q[n].b[j][t][1][i]);
+                    for (int i = 0; i < NP; ++i) {
+                        if (t == 0 && i == 0)
+                            mma_f16_16816_first(d, a, q[n].b[j][t][0][i], q[n].b[j][t][1][i]);
+                        else
+                            mma_f16_16816(d, a, q[n].b[j][t][0][i], q[n].b[j][t][1][i]);
+                    }
                 }
                 s[n][0] = fmaf(s0, d[0], s[n][0]);
                 s[n][1] = fmaf(s0, d[1], s[n][1]);
@@ -296,7 +310,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
     const int head = seg.head, t0 = seg.t0, count = seg.count, first = seg.first, base = seg.base, end = seg.end;
     const int* table = p.tables + (size_t)seg.seq * p.width;
     const Rows<NT>& rows = seg.rows;
-    float* scores = p.scores ? p.scores + ((size_t)seg.seq * p.cache.kv_heads + head) * p.max_stages * (STAGE * 8 * NT) : nullptr;
+    float* scores = p.scores ? p.scores + ((size_t)seg.seq * p.cache.kv_heads + head) * p.max_stages * (STAGE * 8 * NT) + g * (8 * NT) + 2 * c : nullptr;
 
     unsigned char* ring = smem + warp * STAGES * Plan::STAGE_BYTES;
     uint32_t there[STAGES];
@@ -375,7 +389,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        *reinterpret_cast<float2*>(scores + ((size_t)at + KEYS * h + g + 8 * x) * (8 * NT) + 8 * n + 2 * c) = make_float2(s[h][n][2 * x], s[h][n][2 * x + 1]);
+                        *reinterpret_cast<float2*>(scores + (size_t)at * (8 * NT) + (KEYS * h + 8 * x) * (8 * NT) + 8 * n) = make_float2(s[h][n][2 * x], s[h][n][2 * x + 1]);
         }
         // The maximum is left behind by up to 2^8: only a score above that makes the warp find a new one and scale what it has.
         float high[NT][2];

@@ -23,11 +23,7 @@ class Workspace:
         self._replaced: list = []  # outgrown buffers that recorded steps may still point at
         self._pinned = False
 
-    def get(self, name: str, shape, dtype: torch.dtype, zeroed: bool = False) -> torch.Tensor:
-        """``zeroed``: new storage is zero (counters that their kernels leave as they found them)."""
-        count = 1
-        for s in shape:
-            count *= int(s)
+    def _storage(self, name: str, count: int, dtype: torch.dtype, zeroed: bool = False) -> torch.Tensor:
         key = (name, dtype)
         buf = self._buffers.get(key)
         if buf is None or buf.numel() < count:
@@ -35,7 +31,18 @@ class Workspace:
                 self._replaced.append(buf)
             buf = (torch.zeros if zeroed else torch.empty)(max(count, 1), dtype=dtype, device=self.device)
             self._buffers[key] = buf
-        return buf[:count].view(*shape)
+        return buf
+
+    def get(self, name: str, shape, dtype: torch.dtype) -> torch.Tensor:
+        count = 1
+        for s in shape:
+            count *= int(s)
+        return self._storage(name, count, dtype)[:count].view(*shape)
+
+    def address(self, name: str, count: int, dtype: torch.dtype, zeroed: bool = False) -> int:
+        """Where ``count`` elements of the buffer lie (0: none are wanted), for callers that hand it to the library at once.
+        ``zeroed``: new storage is zero (counters that their kernels leave as they found them)."""
+        return self._storage(name, count, dtype, zeroed).data_ptr() if count else 0
 
     def reserve(self, name: str, shape, dtype: torch.dtype) -> None:
         self.get(name, shape, dtype)

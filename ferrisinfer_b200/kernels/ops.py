@@ -2426,29 +2426,42 @@ def _current_stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def _row_stride(t, rows: int, width: int) -> int:
-    return t.stride(0) if rows > 1 else max(t.stride(0), width)
+_packed_library = None
+
+
+def _packed_lib():
+    """The library, once it is known to be loaded."""
+    global _packed_library
+    if _packed_library is None:
+        _packed_library = _lib()
+    return _packed_library
 
 
 def _packed_rows(k, v, slot_mapping, pages: PackedPages, what: str) -> int:
     """Lays out rows of keys and values that go with ``pages``, or raises; how many."""
     width, dev = pages.width, pages.device_index
-    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(slot_mapping, torch.Tensor)
-            and k.get_device() == v.get_device() == slot_mapping.get_device() == dev):
+    try:  # (a tensor of the host has device -1)
+        there = dev == k.get_device() == v.get_device() == slot_mapping.get_device()
+    except AttributeError:
+        there = False
+    if not there:
         raise KernelError(f"{what}: keys, values and slots must be CUDA tensors on the cache's device (there is no CPU path)")
-    T, dtype = slot_mapping.numel(), k.dtype
-    if k.shape != (T, width) or v.shape != (T, width) or v.dtype != dtype:
+    T, dtype, shape = slot_mapping.numel(), k.dtype, (slot_mapping.numel(), width)
+    if k.shape != shape or v.shape != shape or v.dtype != dtype:
         raise KernelError(f"{what}: keys {tuple(k.shape)} {k.dtype}, values {tuple(v.shape)} {v.dtype}, {T} slots for "
                           f"{pages.kv_heads} heads of {pages.head_dim}")
-    if k.stride(1) != 1 or v.stride(1) != 1:
+    ldk, k_step = k.stride()
+    ldv, v_step = v.stride()
+    if k_step != 1 or v_step != 1:
         raise KernelError(f"{what}: keys and values need contiguous rows, found strides {k.stride()} and {v.stride()}")
     if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous():
         raise KernelError(f"{what}: slot mapping must be contiguous and {torch.int32}, found {slot_mapping.dtype}")
     if dtype not in _DT:
         raise KernelError(f"{what}: dtype {dtype} is not supported (float32 or bfloat16)")
+    if T == 1:
+        ldk, ldv = max(ldk, width), max(ldv, width)
     _PACKED_ROWS.pack_into(_packed_buffer, 0, k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), *pages._args, _current_stream(), _DT[dtype],
-                           _row_stride(k, T, width), _row_stride(v, T, width), pages.pages, pages.kv_heads, pages.page_size,
-                           pages.head_dim, T)
+                           ldk, ldv, pages.pages, pages.kv_heads, pages.page_size, pages.head_dim, T)
     return T
 
 
@@ -2458,14 +2471,14 @@ def packed_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Ten
     group of 32: least = its minimum rounded down to bf16, scale = bf16((maximum - least) / 15), code = (x - least) / scale
     rounded to even; a group with NaN or infinity stands as NaN.  Two tokens with one slot leave one of them."""
     if _packed_rows(k, v, slot_mapping, pages, "packed cache write"):
-        _check(_lib().ferris_packed_cache_write(_packed_buffer_at), "packed cache write")
+        _check(_packed_lib().ferris_packed_cache_write(_packed_buffer_at), "packed cache write")
 
 
 def packed_cache_read(pages: PackedPages, slot_mapping: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     """k[t], v[t] [kv heads x head size] = the values that row ``slot_mapping[t]`` of the packed cache stands for, rounded once
     to their type (zeros where the slot is below 0)."""
     if _packed_rows(k, v, slot_mapping, pages, "packed cache read"):
-        _check(_lib().ferris_packed_cache_read(_packed_buffer_at), "packed cache read")
+        _check(_packed_lib().ferris_packed_cache_read(_packed_buffer_at), "packed cache read")
 
 
 def _weight_rows(weights, kv_heads: int, what: str) -> tuple:
@@ -2493,24 +2506,29 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
     in the softmax, summed over the request's queries and the query heads of the kv head, is added to it; the rows that
     came with this step (and with ``add_weights`` False all of them) are set instead."""
     dev, D, hkv = pages.device_index, pages.head_dim, pages.kv_heads
-    for t in (q, out, block_tables, seq_q_start, seq_start_row):
-        if not isinstance(t, torch.Tensor) or t.get_device() != dev:
-            raise KernelError("packed attention: all tensors must be CUDA tensors on the cache's device (there is no CPU path)")
-    for t in (block_tables, seq_q_start, seq_start_row):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise KernelError("packed attention: block tables, first query rows and rows held before the step must be contiguous and "
-                              f"{torch.int32}, found {t.dtype}")
-    S, dtype = seq_start_row.numel(), q.dtype
+    try:  # (a tensor of the host has device -1)
+        there = dev == q.get_device() == out.get_device() == block_tables.get_device() == seq_q_start.get_device() == seq_start_row.get_device()
+    except AttributeError:
+        there = False
+    if not there:
+        raise KernelError("packed attention: all tensors must be CUDA tensors on the cache's device (there is no CPU path)")
+    if not (block_tables.dtype == seq_q_start.dtype == seq_start_row.dtype == torch.int32
+            and block_tables.is_contiguous() and seq_q_start.is_contiguous() and seq_start_row.is_contiguous()):
+        raise KernelError("packed attention: block tables, first query rows and rows held before the step must be contiguous and "
+                          f"{torch.int32}, found {block_tables.dtype}, {seq_q_start.dtype} and {seq_start_row.dtype}")
+    S, dtype, cols, table_shape = seq_start_row.numel(), q.dtype, num_heads * D, block_tables.shape
     if num_heads <= 0 or num_heads % hkv:
         raise KernelError(f"packed attention: {num_heads} heads cannot share {hkv} kv heads")
-    if q.dim() != 2 or out.shape != (q.shape[0], num_heads * D) or q.shape[1] < num_heads * D or out.dtype != dtype:
+    T = out.shape[0] if out.dim() == 2 else -1
+    if q.dim() != 2 or q.shape[0] != T or out.shape[1] != cols or q.shape[1] < cols or out.dtype != dtype:
         raise KernelError(f"packed attention: q {tuple(q.shape)} {q.dtype}, out {tuple(out.shape)} {out.dtype} for {num_heads} heads of {D}")
-    T = q.shape[0]
     if dtype not in _DT:
         raise KernelError(f"packed attention: dtype {dtype} is not supported (float32 or bfloat16)")
-    if q.stride(1) != 1 or out.stride(1) != 1:
+    ldq, q_step = q.stride()
+    ldo, out_step = out.stride()
+    if q_step != 1 or out_step != 1:
         raise KernelError(f"packed attention: queries and outputs need contiguous rows, found strides {q.stride()} and {out.stride()}")
-    if block_tables.dim() != 2 or block_tables.shape[0] != S or seq_q_start.numel() != S + 1:
+    if len(table_shape) != 2 or table_shape[0] != S or seq_q_start.numel() != S + 1:
         raise KernelError(f"packed attention: tables {tuple(block_tables.shape)}, {seq_q_start.numel()} first rows for {S} requests")
     if max_q_len < 0 or max_kv_len < 0 or window < 0:
         raise KernelError(f"packed attention: at most {max_q_len} queries, {max_kv_len} rows, window {window}")
@@ -2524,28 +2542,28 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
         w = (weights.data_ptr(), 0 if seq_slot is None else seq_slot.data_ptr(), slot_stride, head_stride, rows)
     if T == 0 or S == 0 or max_q_len == 0:
         return
-    if block_tables.shape[1] == 0:
+    if table_shape[1] == 0:
         out.zero_()
         return
     if workspace is None:
         raise KernelError("packed attention: a workspace is needed")
-    sizes = (_DT[dtype], D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, 0 if weights is None else 1)
-    scratch, counters, launches = _packed_attention_plan(sizes, dev)
-    scratch_at = workspace.get("packed_attention", (scratch,), torch.float32).data_ptr() if scratch else 0
-    counters_at = workspace.get("packed_attention_counters", (counters,), torch.int32, zeroed=True).data_ptr() if counters else 0
+    dt = _DT[dtype]
+    scratch, counters, launches = _packed_attention_plan(dt, D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, 0 if weights is None else 1, dev)
+    if T == 1:
+        ldq, ldo = max(ldq, cols), max(ldo, cols)
     _PACKED_ATTENTION.pack_into(
         _packed_buffer, 0, q.data_ptr(), out.data_ptr(), *pages._args, block_tables.data_ptr(), seq_q_start.data_ptr(), seq_start_row.data_ptr(),
-        scratch_at, counters_at, w[0], w[1], _current_stream(), w[2], _row_stride(q, T, num_heads * D), _row_stride(out, T, num_heads * D), _DT[dtype],
-        pages.pages, hkv, pages.page_size, D, block_tables.shape[1], S, T, num_heads, max_q_len, max_kv_len, window, w[3], w[4],
-        1 if add_weights else 0, scale)
-    _check(_lib().ferris_packed_attention(_packed_buffer_at), "packed attention", launches)
+        workspace.address("packed_attention", scratch, torch.float32), workspace.address("packed_attention_counters", counters, torch.int32, True),
+        w[0], w[1], _current_stream(), w[2], ldq, ldo, dt, pages.pages, hkv, pages.page_size, D, table_shape[1], S, T, num_heads, max_q_len,
+        max_kv_len, window, w[3], w[4], 1 if add_weights else 0, scale)
+    _check(_packed_lib().ferris_packed_attention(_packed_buffer_at), "packed attention", launches)
 
 
 @functools.lru_cache(maxsize=4096)
-def _packed_attention_plan(sizes: tuple, device: int) -> tuple:
+def _packed_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_q, max_kv, weights, device: int) -> tuple:
     """Floats of scratch, counters and launches of a step of these sizes on a GPU."""
     needs = (_LL * 3)()
-    _lib().ferris_packed_attention_plan(*sizes, needs)
+    _lib().ferris_packed_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_q, max_kv, weights, needs)
     return tuple(needs)
 
 

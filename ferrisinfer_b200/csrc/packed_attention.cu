@@ -976,7 +976,7 @@ Plan make_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int t
         const long long most = pairs * stages / EVEN_STAGES;
         q.most = (int)(most < 1 ? 1 : most < sms * per_sm ? most : sms * per_sm);
         q.blocks = q.most + (int)pairs;  // (pieces: each request and kv head may have one that is not full)
-        q.join_kernel = q.most > 16 * pairs;  // so many parts of a request that one block would be long at joining them
+        q.join_kernel = q.most > 32 * pairs;  // so many parts of a request that one block would be long at joining them
         q.part_floats = fours(2ll * q.blocks * 8 * q.tiles * (head_dim + 2) + (q.join_kernel ? seqs + 2 : 0));
         q.counters = q.join_kernel ? 0 : pairs;
         q.score_floats = weights ? pairs * stages * STAGE * 8 * q.tiles : 0;

@@ -476,35 +476,45 @@ int rows_call(const FerrisPackedRows* a) {
 FERRIS_API int ferris_packed_cache_write(const FerrisPackedRows* a) { return rows_call<true>(a); }
 FERRIS_API int ferris_packed_cache_read(const FerrisPackedRows* a) { return rows_call<false>(a); }
 
-FERRIS_API int ferris_packed_cache_evict(void* from_kc, void* from_ks, void* from_vc, void* from_vs, int from_pages, int from_page_size,
-                                         void* to_kc, void* to_ks, void* to_vc, void* to_vs, int to_pages, int to_page_size, int kv_heads,
-                                         int head_dim, const int* from_tables, int from_width, const int* to_tables, int to_width,
-                                         const int* seq_rows, const int* seq_slot, const float* weights, long long slot_stride,
-                                         int head_stride, int max_rows, int* kept_rows, float* kept_weights, long long kept_slot_stride,
-                                         int kept_head_stride, int seqs, int budget, int keep_first, int keep_last, void* stream) {
-    const PackedCache from = make_cache(from_kc, from_ks, from_vc, from_vs, from_pages, kv_heads, from_page_size, head_dim);
-    const PackedCache to = make_cache(to_kc, to_ks, to_vc, to_vs, to_pages, kv_heads, to_page_size, head_dim);
+// The arguments of the one below, as its caller lays them out.
+struct FerrisPackedEvict {
+    void *from_kc, *from_ks, *from_vc, *from_vs, *to_kc, *to_ks, *to_vc, *to_vs;
+    const int *from_tables, *to_tables, *seq_rows, *seq_slot;
+    const float* weights;
+    int* kept_rows;
+    float* kept_weights;
+    void* stream;
+    long long slot_stride, kept_slot_stride;
+    int from_pages, from_page_size, to_pages, to_page_size, kv_heads, head_dim, from_width, to_width, head_stride, max_rows, kept_head_stride,
+        seqs, budget, keep_first, keep_last;
+};
+
+FERRIS_API int ferris_packed_cache_evict(const FerrisPackedEvict* a) {
+    const int kv_heads = a->kv_heads, head_dim = a->head_dim, seqs = a->seqs, budget = a->budget, keep_first = a->keep_first, keep_last = a->keep_last,
+              max_rows = a->max_rows;
+    const PackedCache from = make_cache(a->from_kc, a->from_ks, a->from_vc, a->from_vs, a->from_pages, kv_heads, a->from_page_size, head_dim);
+    const PackedCache to = make_cache(a->to_kc, a->to_ks, a->to_vc, a->to_vs, a->to_pages, kv_heads, a->to_page_size, head_dim);
     if (const char* why = packed_cache_refusal(from)) FERRIS_REFUSE("%s", why);
     if (const char* why = packed_cache_refusal(to)) FERRIS_REFUSE("%s", why);
     if (budget <= 0 || keep_first < 0 || keep_last < 0 || keep_first > budget - keep_last)
         FERRIS_REFUSE("eviction: %d first and %d last rows of a budget of %d", keep_first, keep_last, budget);
     if (seqs <= 0) return FERRIS_OK;
     if (seqs > 65535 || kv_heads > 65535) FERRIS_REFUSE("eviction: %d requests of %d kv heads", seqs, kv_heads);
-    cudaStream_t st = (cudaStream_t)stream;
+    cudaStream_t st = (cudaStream_t)a->stream;
     // blocks of a cluster: about 8,192 rows each, at most eight (the most that is portable)
     int blocks = 1;
     while (blocks < 8 && (long long)blocks * 8192 < max_rows) blocks *= 2;
     const int each = ((max_rows + 1024 * blocks - 1) / (1024 * blocks)) * 1024, held = each < EVICT_HELD ? each : EVICT_HELD;
     if (const int r = ferris_allow_dynamic_smem((const void*)packed_evict_select_kernel, (size_t)held * 4)) return r;
     cudaError_t e = ferris_launch_cluster(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,
-                                          weights, slot_stride, head_stride, seq_rows, seq_slot, kept_rows, kept_weights, kept_slot_stride,
-                                          kept_head_stride, budget, keep_first, keep_last, max_rows, held);
+                                          a->weights, a->slot_stride, a->head_stride, a->seq_rows, a->seq_slot, a->kept_rows, a->kept_weights,
+                                          a->kept_slot_stride, a->kept_head_stride, budget, keep_first, keep_last, max_rows, held);
     if (e != cudaSuccess) FERRIS_LAUNCH_CHECK();
     return with_groups(head_dim, [&](auto w) {
         constexpr int W = decltype(w)::value, ROWS = 256 / W * 4;
-        ferris_launch(packed_evict_move_kernel<W>, dim3((budget + ROWS - 1) / ROWS, kv_heads, seqs), dim3(256), 0, st, from, to, from_tables,
-                      from_width, to_tables, to_width, (const int*)kept_rows, budget, DivideBy(from_page_size), DivideBy(to_page_size),
-                      ferris_status_ptr());
+        ferris_launch(packed_evict_move_kernel<W>, dim3((budget + ROWS - 1) / ROWS, kv_heads, seqs), dim3(256), 0, st, from, to,
+                      a->from_tables, a->from_width, a->to_tables, a->to_width, (const int*)a->kept_rows, budget, DivideBy(a->from_page_size),
+                      DivideBy(a->to_page_size), ferris_status_ptr());
         FERRIS_LAUNCH_CHECK();
     });
 }

@@ -50,8 +50,7 @@ _SIGNATURES = {
     "ferris_embed_gather": [_VP, _I, _VP, _VP, _I, _I, _I, _VP, _VP],
     "ferris_packed_cache_write": [_VP],
     "ferris_packed_cache_read": [_VP],
-    "ferris_packed_cache_evict": [_VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _I, _VP, _I, _VP, _VP, _VP, _LL, _I, _I,
-                                  _VP, _VP, _LL, _I, _I, _I, _I, _I, _VP],
+    "ferris_packed_cache_evict": [_VP],
     "ferris_packed_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
     "ferris_packed_attention": [_VP],
 }
@@ -2418,7 +2417,8 @@ class PackedPages:
 # library is called by one thread at a time.
 _PACKED_ROWS = struct.Struct("=8Q8i")
 _PACKED_ATTENTION = struct.Struct("=14Qq17if")
-_packed_buffer = ctypes.create_string_buffer(max(_PACKED_ROWS.size, _PACKED_ATTENTION.size))
+_PACKED_EVICT = struct.Struct("=16Q2q15i")
+_packed_buffer = ctypes.create_string_buffer(max(_PACKED_ROWS.size, _PACKED_ATTENTION.size, _PACKED_EVICT.size))
 _packed_buffer_at = ctypes.addressof(_packed_buffer)
 
 
@@ -2483,10 +2483,12 @@ def packed_cache_read(pages: PackedPages, slot_mapping: torch.Tensor, k: torch.T
 
 def _weight_rows(weights, kv_heads: int, what: str) -> tuple:
     """(slots, rows, slot stride, head stride) of weights fp32 [slots, kv heads, rows]."""
-    _need(weights, what, torch.float32, contiguous=False)
-    if weights.dim() != 3 or weights.shape[1] != kv_heads or (weights.shape[2] > 1 and weights.stride(2) != 1):
+    if not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or weights.dim() != 3:
+        raise KernelError(f"{what} must be a {torch.float32} tensor [slots, {kv_heads}, rows]")
+    (slots, heads, rows), (slot_stride, head_stride, step) = weights.shape, weights.stride()
+    if heads != kv_heads or (rows > 1 and step != 1):
         raise KernelError(f"{what} must be [slots, {kv_heads}, rows] with contiguous rows, found {tuple(weights.shape)}")
-    return weights.shape[0], weights.shape[2], weights.stride(0), weights.stride(1)
+    return slots, rows, slot_stride, head_stride
 
 
 def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, block_tables: torch.Tensor, seq_q_start: torch.Tensor,
@@ -2580,9 +2582,19 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
     held, so other requests may share them.  Afterwards the request holds min(seq_rows[s], budget) rows.
     ``kept_rows`` (int32 [S, kv heads, budget]) gets their numbers, -1 behind them; ``kept_weights`` (fp32 [slots, kv heads, >=
     budget], not the memory of ``weights``) their weights.  ``workspace`` is for scratch that large requests need."""
-    for t, what in ((block_tables, "block tables"), (seq_rows, "rows of the requests"), (kept_tables, "block tables of the kept rows"),
-                    (kept_rows, "numbers of the kept rows")):
-        _need(t, what, torch.int32)
+    dev = pages.device_index
+    try:  # (a tensor of the host has device -1)
+        there = dev == kept_pages.device_index == block_tables.get_device() == seq_rows.get_device() == kept_tables.get_device() \
+            == kept_rows.get_device() == weights.get_device()
+        there = there and (seq_slot is None or seq_slot.get_device() == dev) and (kept_weights is None or kept_weights.get_device() == dev)
+    except AttributeError:
+        there = False
+    if not there:
+        raise KernelError("eviction: all tensors must be CUDA tensors on the cache's device (there is no CPU path)")
+    for t in (block_tables, seq_rows, kept_tables, kept_rows):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"eviction: block tables, rows of the requests and numbers of kept rows must be contiguous and {torch.int32}, "
+                              f"found {t.dtype}")
     S, hkv = seq_rows.numel(), pages.kv_heads
     if kept_pages.kv_heads != hkv or kept_pages.head_dim != pages.head_dim:
         raise KernelError(f"eviction: from {hkv} heads of {pages.head_dim} into {kept_pages.kv_heads} of {kept_pages.head_dim}")
@@ -2597,7 +2609,7 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
         _need(seq_slot, "slots of the weights", torch.int32)
     if seq_slot.numel() != S if seq_slot is not None else slots < S:
         raise KernelError(f"eviction: weights {tuple(weights.shape)} for {S} requests")
-    kept = (None, 0, 0)
+    kept = (0, 0, 0)
     if kept_weights is not None:
         kslots, krows, kslot_stride, khead_stride = _weight_rows(kept_weights, hkv, "eviction: kept weights")
         if krows < budget or kslots < (slots if seq_slot is not None else S):
@@ -2605,15 +2617,12 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
         if kept_weights.data_ptr() == weights.data_ptr():
             raise KernelError("eviction: kept weights need memory of their own")
         kept = (kept_weights.data_ptr(), kslot_stride, khead_stride)
-    tensors = [block_tables, seq_rows, weights, kept_pages.k_codes, kept_tables, kept_rows, seq_slot, kept_weights]
-    if any(t is not None and t.device != pages.k_codes.device for t in tensors):
-        raise KernelError("eviction: all tensors must be on the cache's device")
     if S == 0 or rows == 0 or block_tables.shape[1] == 0 or kept_tables.shape[1] == 0:
         kept_rows.fill_(-1)
         return
-    _check(_lib().ferris_packed_cache_evict(*pages._args, pages.pages, pages.page_size, *kept_pages._args, kept_pages.pages,
-                                            kept_pages.page_size, hkv, pages.head_dim, block_tables.data_ptr(), block_tables.shape[1],
-                                            kept_tables.data_ptr(), kept_tables.shape[1], seq_rows.data_ptr(),
-                                            None if seq_slot is None else seq_slot.data_ptr(), weights.data_ptr(), slot_stride, head_stride,
-                                            rows, kept_rows.data_ptr(), *kept, S, budget, keep_first, keep_last, _stream()),
-           "eviction", 2)
+    _PACKED_EVICT.pack_into(
+        _packed_buffer, 0, *pages._args, *kept_pages._args, block_tables.data_ptr(), kept_tables.data_ptr(), seq_rows.data_ptr(),
+        0 if seq_slot is None else seq_slot.data_ptr(), weights.data_ptr(), kept_rows.data_ptr(), kept[0], _current_stream(), slot_stride, kept[1],
+        pages.pages, pages.page_size, kept_pages.pages, kept_pages.page_size, hkv, pages.head_dim, block_tables.shape[1], kept_tables.shape[1],
+        head_stride, rows, kept[2], S, budget, keep_first, keep_last)
+    _check(_packed_lib().ferris_packed_cache_evict(_packed_buffer_at), "eviction", 2)

@@ -52,37 +52,57 @@ __device__ __forceinline__ void store8(T* p, const Eight& e) {
     }
 }
 
+// Minimum and maximum that NaN goes through.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // The codes of this lane's 8 elements (element i in bits 4 i) and the group's word of scales; all 32 lanes take part.
+//
+// code = round(d / scale) to even, d = x - least, without sixteen divisions a thread: q = d (1 / scale) is off by an ulp or two, its
+// rounding c (by adding 1.5 x 2^23, whose last bits it then is) at most by one, and that only beside a tie; the rest
+// d - c scale, exact in one multiply-add (c scale has 12 bits, the rest no more than d), says which way, and whether it IS a tie.
 __device__ __forceinline__ uint32_t quantise8(const Eight& e, uint32_t& scales) {
-    float low = e.x[0], high = e.x[0], sum = 0.0f;  // fminf and fmaxf drop NaN: the sum keeps it, and infinities
+    float low = e.x[0], high = e.x[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        low = fminf(low, e.x[i]);
-        high = fmaxf(high, e.x[i]);
-        sum += 0.0f * e.x[i];
+    for (int i = 1; i < 8; ++i) {
+        low = min_nan(low, e.x[i]);
+        high = max_nan(high, e.x[i]);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
     const bf16 least_h = __float2bfloat16_rd(low);
     const float least = __bfloat162float(least_h);
     const bf16 scale_h = __float2bfloat16_rn(__fdiv_rn(high - least, 15.0f));
     const float scale = __bfloat162float(scale_h);
-    if (!(sum == 0.0f) || !isfinite(least) || !isfinite(scale)) {
+    if (!isfinite(least) || !isfinite(scale)) {  // (NaN and infinities show in one of them)
         scales = 0x7fc07fc0u;
         return 0;
     }
     scales = (uint32_t)__bfloat16_as_ushort(scale_h) | (uint32_t)__bfloat16_as_ushort(least_h) << 16;
     uint32_t codes = 0;
-    if (scale > 0.0f) {
+    if (scale >= 0x1p-100f) {
+        const float inv = __fdiv_rn(1.0f, scale), half = 0.5f * scale;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float q = rintf(__fdiv_rn(e.x[i] - least, scale));
-            codes |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * i);
+        for (int i = 7; i >= 0; --i) {
+            const float d = e.x[i] - least, t = fmaf(d, inv, 12582912.0f), rest = fmaf(-(t - 12582912.0f), scale, d);
+            int code = __float_as_int(t) & 31;
+            if (fabsf(rest) > half || (fabsf(rest) == half && (code & 1))) code += rest > 0.0f ? 1 : -1;
+            codes = codes << 4 | (uint32_t)min(code, 15);
         }
+    } else if (scale > 0.0f) {  // (1 / scale may be no number)
+#pragma unroll 1
+        for (int i = 7; i >= 0; --i) codes = codes << 4 | (uint32_t)fminf(rintf(__fdiv_rn(e.x[i] - least, scale)), 15.0f);
     }
     return codes;
 }
@@ -198,7 +218,7 @@ __device__ __forceinline__ uint32_t weight_key(float w, int row, int n, int keep
     return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_THREADS = 512, EVICT_WARPS = EVICT_THREADS / 32;
 constexpr int EVICT_HELD = 48 * 1024;  // rows whose keys a block's shared memory holds
 
 // A cluster of blocks per (request, kv head), each with a run of its rows, whose keys it holds in shared memory (longer runs are
@@ -213,7 +233,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
                                                                             int max_rows, int held) {
     extern __shared__ uint32_t keys[];  // [held]
     __shared__ uint32_t hist[4][256], total[256];
-    __shared__ int greater[32], equal[32], counts[2];
+    __shared__ int greater[EVICT_WARPS], equal[EVICT_WARPS], counts[2];
     pdl_launch_dependents();
     pdl_wait();
     const int s = blockIdx.y, h = blockIdx.x, heads = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -232,11 +252,13 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
         return;
     }
     // this block's rows: whole runs of 32 for each of its warps
-    const int run = (n + 32 * 32 * blocks - 1) / (32 * 32 * blocks) * 32, begin = min(rank * 32 * run, n), end = min(begin + 32 * run, n);
+    const int run = (n + 32 * EVICT_WARPS * blocks - 1) / (32 * EVICT_WARPS * blocks) * 32, begin = min(rank * EVICT_WARPS * run, n),
+              end = min(begin + EVICT_WARPS * run, n);
     const bool hold = end - begin <= held;
     const auto key_of = [&](int r) { return hold ? keys[r - begin] : weight_key(w[r], r, n, keep_first, keep_last); };
-    (&hist[0][0])[tid] = 0;
+    for (int i = tid; i < 4 * 256; i += EVICT_THREADS) (&hist[0][0])[i] = 0;
     if (hold)
+#pragma unroll 8
         for (int r = begin + tid; r < end; r += EVICT_THREADS) keys[r - begin] = weight_key(w[r], r, n, keep_first, keep_last);
     __syncthreads();
     uint32_t prefix = 0;
@@ -250,6 +272,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
             const uint32_t key = r < end ? key_of(r) : 0u;
             const uint32_t bin = r < end && (key & mask) == prefix ? (key >> shift) & 255 : 256;
             uint32_t rest = __ballot_sync(0xffffffffu, bin < 256);
+            if (!rest) continue;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {  // the bins of two lanes for all that share them, the others one by one
                 if (!rest) break;
@@ -315,11 +338,11 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
         equal[warp] = eq;
     }
     __syncthreads();
-    int before_gt = lane < warp ? greater[lane] : 0, before_eq = lane < warp ? equal[lane] : 0;
+    int before_gt = lane < warp ? greater[lane] : 0, before_eq = lane < warp ? equal[lane] : 0;  // (lanes below EVICT_WARPS)
     before_gt = __reduce_add_sync(0xffffffffu, before_gt);
     before_eq = __reduce_add_sync(0xffffffffu, before_eq);
     if (blocks > 1) {
-        if (warp == 31 && lane == 0) {
+        if (warp == EVICT_WARPS - 1 && lane == 0) {
             counts[0] = before_gt + gt;
             counts[1] = before_eq + eq;
         }
@@ -501,10 +524,10 @@ FERRIS_API int ferris_packed_cache_evict(const FerrisPackedEvict* a) {
     if (seqs <= 0) return FERRIS_OK;
     if (seqs > 65535 || kv_heads > 65535) FERRIS_REFUSE("eviction: %d requests of %d kv heads", seqs, kv_heads);
     cudaStream_t st = (cudaStream_t)a->stream;
-    // blocks of a cluster: about 8,192 rows each, at most eight (the most that is portable)
+    // blocks of a cluster: about 4,096 rows each while every SM has one, else 8,192; at most eight (the most that is portable)
     int blocks = 1;
-    while (blocks < 8 && (long long)blocks * 8192 < max_rows) blocks *= 2;
-    const int each = ((max_rows + 1024 * blocks - 1) / (1024 * blocks)) * 1024, held = each < EVICT_HELD ? each : EVICT_HELD;
+    while (blocks < 8 && (long long)blocks * ((long long)seqs * kv_heads * blocks < sms() ? 4096 : 8192) < max_rows) blocks *= 2;
+    const int each = ((max_rows + EVICT_THREADS * blocks - 1) / (EVICT_THREADS * blocks)) * EVICT_THREADS, held = each < EVICT_HELD ? each : EVICT_HELD;
     if (const int r = ferris_allow_dynamic_smem((const void*)packed_evict_select_kernel, (size_t)held * 4)) return r;
     cudaError_t e = ferris_launch_cluster(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,
                                           a->weights, a->slot_stride, a->head_stride, a->seq_rows, a->seq_slot, a->kept_rows, a->kept_weights,

@@ -171,14 +171,16 @@ __device__ __forceinline__ Eight dequantise8(uint32_t codes, uint32_t scales) {
     return e;
 }
 
+constexpr int READ_EACH = 4;
+
 template <typename T, int W, bool VEC>
 __global__ void __launch_bounds__(256) packed_read_kernel(T* k, T* v, const RowsCall q) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr uint32_t LANES = 4 * W;
-    constexpr int EACH = 4;  // rows of a thread, fetched together
-    const uint32_t rows = (uint32_t)q.tokens * q.cache.kv_heads, threads = gridDim.x * 256;
-    for (uint32_t first = blockIdx.x * 256 + threadIdx.x; first < rows * LANES; first += threads * EACH) {  // (rows x lanes: the C entry sees to 32 bits)
+    constexpr int EACH = READ_EACH;  // rows of a thread, fetched together
+    const uint32_t rows = (uint32_t)q.tokens * q.cache.kv_heads, threads = gridDim.x * 256, first = blockIdx.x * 256 + threadIdx.x;
+    {
         uint32_t kc[EACH], vc[EACH], ks[EACH], vs[EACH];
         int token[EACH], head[EACH];
 #pragma unroll
@@ -220,19 +222,20 @@ __device__ __forceinline__ uint32_t weight_key(float w, int row, int n, int keep
 
 constexpr int EVICT_THREADS = 512, EVICT_WARPS = EVICT_THREADS / 32;
 constexpr int EVICT_HELD = 48 * 1024;  // rows whose keys a block's shared memory holds
+constexpr int EVICT_COPIES = 4;        // of a histogram: lanes that meet in a bin wait for one another
 
 // A cluster of blocks per (request, kv head), each with a run of its rows, whose keys it holds in shared memory (longer runs are
 // read again each time).  The budget-th greatest key by its four bytes, most significant first: a histogram of 256 bins
 // each, added up over the cluster; then the kept rows in order, every warp its own run of rows.  What bounds it is the
-// chain of barriers: one a byte, two for the ranks.  Lanes that share a bin count as one (rows that nothing has
-// attended all fall into one) where that is quick to see: `match.any` took half of the kernel's time.
+// chain of short passes and barriers, so a lane takes four rows at a time, each on its own (with lanes that share a bin
+// found by votes, or by `match.any`, a pass over 32 rows took 350 cycles).
 __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(const float* weights, long long slot_stride, int head_stride,
                                                                             const int* __restrict__ seq_rows, const int* __restrict__ seq_slot,
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
                                                                             int kept_head_stride, int budget, int keep_first, int keep_last,
                                                                             int max_rows, int held) {
     extern __shared__ uint32_t keys[];  // [held]
-    __shared__ uint32_t hist[4][256], total[256];
+    __shared__ uint32_t hist[4][EVICT_COPIES][256], total[256];
     __shared__ int greater[EVICT_WARPS], equal[EVICT_WARPS], counts[2];
     pdl_launch_dependents();
     pdl_wait();
@@ -251,15 +254,22 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
         }
         return;
     }
-    // this block's rows: whole runs of 32 for each of its warps
+    // this block's rows: runs of whole 32 rows for each of its warps
     const int run = (n + 32 * EVICT_WARPS * blocks - 1) / (32 * EVICT_WARPS * blocks) * 32, begin = min(rank * EVICT_WARPS * run, n),
               end = min(begin + EVICT_WARPS * run, n);
     const bool hold = end - begin <= held;
-    const auto key_of = [&](int r) { return hold ? keys[r - begin] : weight_key(w[r], r, n, keep_first, keep_last); };
-    for (int i = tid; i < 4 * 256; i += EVICT_THREADS) (&hist[0][0])[i] = 0;
+    // keys of four rows from r (a multiple of four) on; 0, which no weight has, behind the end
+    const auto keys_of = [&](int r) {
+        if (hold) return *reinterpret_cast<const uint4*>(keys + (r - begin));
+        uint32_t k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = r + i < end ? weight_key(w[r + i], r + i, n, keep_first, keep_last) : 0u;
+        return make_uint4(k[0], k[1], k[2], k[3]);
+    };
+    for (int i = tid; i < 4 * EVICT_COPIES * 256; i += EVICT_THREADS) (&hist[0][0][0])[i] = 0;
     if (hold)
 #pragma unroll 8
-        for (int r = begin + tid; r < end; r += EVICT_THREADS) keys[r - begin] = weight_key(w[r], r, n, keep_first, keep_last);
+        for (int r = begin + tid; r < (end + 3) / 4 * 4; r += EVICT_THREADS) keys[r - begin] = r < end ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
     __syncthreads();
     uint32_t prefix = 0;
     int want = budget;  // how many of the rows that share the prefix stay
@@ -267,38 +277,39 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     for (int byte = 0; byte < 4; ++byte) {
         const int shift = 24 - 8 * byte;
         const uint32_t mask = byte == 0 ? 0u : 0xffffffffu << (shift + 8);
-        for (int r0 = begin + 32 * warp; r0 < end; r0 += EVICT_THREADS) {
-            const int r = r0 + lane;
-            const uint32_t key = r < end ? key_of(r) : 0u;
-            const uint32_t bin = r < end && (key & mask) == prefix ? (key >> shift) & 255 : 256;
-            uint32_t rest = __ballot_sync(0xffffffffu, bin < 256);
-            if (!rest) continue;
+        uint32_t* mine_of = hist[byte][lane % EVICT_COPIES];
+#pragma unroll 2
+        for (int r = begin + 4 * tid; r < end; r += 4 * EVICT_THREADS) {
+            const uint4 k = keys_of(r);
+            const uint32_t four[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {  // the bins of two lanes for all that share them, the others one by one
-                if (!rest) break;
-                const int lead = __ffs(rest) - 1;
-                const uint32_t same = __ballot_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, lead));
-                if (lane == lead) atomicAdd(&hist[byte][bin], __popc(same));
-                rest &= ~same;
-            }
-            if (rest >> lane & 1) atomicAdd(&hist[byte][bin], 1u);
+            for (int i = 0; i < 4; ++i)
+                if (four[i] && (four[i] & mask) == prefix) atomicAdd(&mine_of[(four[i] >> shift) & 255], 1u);
         }
-        const uint32_t* bins = hist[byte];
+        __syncthreads();
+        if (tid < 256) {
+            uint32_t sum = 0;
+#pragma unroll
+            for (int x = 0; x < EVICT_COPIES; ++x) sum += hist[byte][x][tid];
+            if (blocks > 1)
+                hist[byte][0][tid] = sum;
+            else
+                total[tid] = sum;
+        }
         if (blocks > 1) {
             cluster_sync();
             if (tid < 256) {
                 uint32_t sum = 0;
-                for (int b = 0; b < blocks; ++b) sum += __float_as_uint(ld_peer_shared_f32(smem_u32(&hist[byte][tid]), b));
+                for (int b = 0; b < blocks; ++b) sum += __float_as_uint(ld_peer_shared_f32(smem_u32(&hist[byte][0][tid]), b));
                 total[tid] = sum;
             }
-            bins = total;
         }
         __syncthreads();
         // every warp finds the bin for itself: eight bins a lane, from the greatest down
         uint32_t mine[8], sum = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            mine[i] = bins[255 - 8 * lane - i];
+            mine[i] = total[255 - 8 * lane - i];
             sum += mine[i];
         }
         uint32_t upto = sum;
@@ -327,12 +338,13 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     // rows with key > prefix all stay, of those with key == prefix the first `want`
     const int from = min(begin + warp * run, end), to = min(from + run, end);
     int gt = 0, eq = 0;
-    for (int i = from; i < to; i += 32) {
-        const int r = i + lane;
-        const uint32_t key = r < to ? key_of(r) : 0u;
-        gt += __popc(__ballot_sync(0xffffffffu, r < to && key > prefix));
-        eq += __popc(__ballot_sync(0xffffffffu, r < to && key == prefix));
+    for (int r = from + 4 * lane; r < to; r += 128) {
+        const uint4 k = keys_of(r);
+        gt += (k.x > prefix) + (k.y > prefix) + (k.z > prefix) + (k.w > prefix);
+        eq += (k.x == prefix) + (k.y == prefix) + (k.z == prefix) + (k.w == prefix);
     }
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) {
         greater[warp] = gt;
         equal[warp] = eq;
@@ -353,21 +365,33 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
         }
         cluster_arrive_release();  // (a block's shared memory stays until all have read it)
     }
-    for (int i = from; i < to; i += 32) {
-        const int r = i + lane;
-        const uint32_t key = r < to ? key_of(r) : 0u;
-        const uint32_t above = __ballot_sync(0xffffffffu, r < to && key > prefix);
-        const uint32_t same = __ballot_sync(0xffffffffu, r < to && key == prefix);
-        const uint32_t lower = (1u << lane) - 1;
-        const int place = before_eq + __popc(same & lower);  // among the equal ones
-        const bool stays = r < to && (key > prefix || (key == prefix && place < want));
-        if (stays) {
-            const int at = before_gt + __popc(above & lower) + min(place, want);
-            rows[at] = r;
-            if (kw) kw[at] = w[r];
+    for (int r0 = from; r0 < to; r0 += 128) {
+        const int r = r0 + 4 * lane;
+        const uint4 k = r < to ? keys_of(r) : make_uint4(0, 0, 0, 0);
+        const uint32_t four[4] = {k.x, k.y, k.z, k.w};
+        int mine = 0;  // those above in the lower half, the equal ones in the upper
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += (four[i] > prefix) + ((four[i] == prefix) << 16);
+        int upto = mine;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, x);
+            if (lane >= x) upto += v;
         }
-        before_gt += __popc(above);
-        before_eq += __popc(same);
+        int above = before_gt + ((upto - mine) & 0xffff), same = before_eq + ((upto - mine) >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (four[i] > prefix || (four[i] == prefix && same < want)) {
+                const int at = above + min(same, want);
+                rows[at] = r + i;
+                if (kw) kw[at] = w[r + i];
+            }
+            above += four[i] > prefix;
+            same += four[i] == prefix;
+        }
+        upto = __shfl_sync(0xffffffffu, upto, 31);
+        before_gt += upto & 0xffff;
+        before_eq += upto >> 16;
     }
     if (blocks > 1) cluster_wait();
 }
@@ -440,8 +464,9 @@ int write_rows(const void* k, const void* v, const RowsCall& q, cudaStream_t st)
 template <typename T, int W>
 int read_rows(void* k, void* v, const RowsCall& q, cudaStream_t st) {
     const bool vec = eights_aligned<T>(k, q.ldk) && eights_aligned<T>(v, q.ldv);
-    const long long need = ((long long)q.tokens * q.cache.kv_heads * 4 * W + 255) / 256, most = sms() * 8;
-    const int blocks = (int)(need < most ? need : most);
+    const long long all = (long long)q.tokens * q.cache.kv_heads * 4 * W, few = (long long)sms() * 2;
+    // a row a thread where that leaves SMs without work
+    const int blocks = (int)((all + 255) / 256 <= few ? (all + 255) / 256 : (all + 256 * READ_EACH - 1) / (256 * READ_EACH) > few ? (all + 256 * READ_EACH - 1) / (256 * READ_EACH) : few);
     if (vec)
         ferris_launch(packed_read_kernel<T, W, true>, dim3(blocks), dim3(256), 0, st, (T*)k, (T*)v, q);
     else
@@ -524,9 +549,9 @@ FERRIS_API int ferris_packed_cache_evict(const FerrisPackedEvict* a) {
     if (seqs <= 0) return FERRIS_OK;
     if (seqs > 65535 || kv_heads > 65535) FERRIS_REFUSE("eviction: %d requests of %d kv heads", seqs, kv_heads);
     cudaStream_t st = (cudaStream_t)a->stream;
-    // blocks of a cluster: about 4,096 rows each while every SM has one, else 8,192; at most eight (the most that is portable)
+    // blocks of a cluster: about 8,192 rows each, at most eight (the most that is portable)
     int blocks = 1;
-    while (blocks < 8 && (long long)blocks * ((long long)seqs * kv_heads * blocks < sms() ? 4096 : 8192) < max_rows) blocks *= 2;
+    while (blocks < 8 && (long long)blocks * 8192 < max_rows) blocks *= 2;
     const int each = ((max_rows + EVICT_THREADS * blocks - 1) / (EVICT_THREADS * blocks)) * EVICT_THREADS, held = each < EVICT_HELD ? each : EVICT_HELD;
     if (const int r = ferris_allow_dynamic_smem((const void*)packed_evict_select_kernel, (size_t)held * 4)) return r;
     cudaError_t e = ferris_launch_cluster(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,

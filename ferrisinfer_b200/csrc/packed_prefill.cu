@@ -46,7 +46,7 @@ struct Layout {
     float* minus_lse;        // the same: minus the log2 of the row's sum (with weights; minus infinity for rows that are not there)
     int* first_pair;         // [request]
     Pair* pairs;
-    int* before;             // [pairs + 1], then the number of pairs, units
+    int* before;             // [pairs + 1], then the number of pairs, units, blocks of a piece
     float* parts;            // [place][D + 2][256]
     long long bytes;
 };
@@ -57,7 +57,7 @@ void for_scratch(int D, int pairs, int kv_heads, int seqs, int grid, F&& take) {
     take(0, (long long)pairs * kv_heads * 2 * operand);
     take(1, (long long)pairs * kv_heads * 256 * 4);
     take(2, (long long)pairs * sizeof(Pair));
-    take(3, (long long)(pairs + 3) * 4);
+    take(3, (long long)(pairs + 4) * 4);
     take(4, 2ll * grid * (D + 2) * 256 * 4);
     take(5, (long long)pairs * kv_heads * 256 * 4);
     take(6, (long long)seqs * 4);
@@ -86,11 +86,12 @@ Layout make_layout(void* base, int D, int pairs, int kv_heads, int seqs, int gri
 // with the next pair where they are long, pieces of each pair where they are short.
 struct Deal {
     int units, blocks, chunk, runs;
-    __device__ __forceinline__ Deal(int units, int most) : units(units) {
+    __device__ __forceinline__ Deal(int units, int most, int chunk) : units(units), chunk(chunk) {
         blocks = min(most, max(1, units / LEAST_PIECE));
-        chunk = max(LEAST_PIECE, (units + most - 1) / most);
         runs = chunk >= RUN;
     }
+    // Blocks of a piece where every CTA gets the same; pieces may have to be longer (packed_queries_kernel).
+    static __device__ __forceinline__ int even_chunk(int units, int most) { return max(LEAST_PIECE, (units + most - 1) / most); }
     __device__ __forceinline__ int pieces(int n) const { return (n + chunk - 1) / chunk; }
     __device__ __forceinline__ int block_of(int u) const { return (int)((((long long)u + 1) * blocks - 1) / units); }
     __device__ __forceinline__ int begin_of(int block) const { return (int)((long long)block * units / blocks); }
@@ -131,7 +132,7 @@ __device__ __forceinline__ int warp_inclusive(int v, int lane) {
     return v;
 }
 
-// The last block of the first row lists the pairs and how their blocks are dealt out; every other block forms the two
+// The first block lists the pairs and how their blocks are dealt out; every other block (of the second row on: of the others) forms the two
 // operand tiles of a pair: query rows in fp16, times a power of two that brings a row's greatest element to 2^13, columns in the
 // order of the keys' codes (8 elements 0 4 1 5 2 6 3 7), and the rows' group sums over 64 in two parts.
 template <int D>
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
-    if (blockIdx.x == gridDim.x - 1) {
+    if (blockIdx.x == 0) {
         if (blockIdx.y) return;
         int n_pairs = 0;
         for (int s0 = 0; s0 < p.seqs; s0 += 256) {  // the pairs of 256 requests at a time, a warp's lanes along a request's
@@ -177,7 +178,23 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
         for (int w = 0; w < 8; ++w) units += sums[w];
         __syncthreads();
         units *= p.cache.kv_heads;
-        const Deal deal(max(units, 1), sms);
+        // Pieces that leave a CTA more than there are SMs would make all of them wait for a second round (six prompts of up to 700
+        // tokens: 39 us): where the pairs are few enough, pieces are lengthened until they fit.
+        int chunk = Deal::even_chunk(max(units, 1), sms);
+        while (chunk < RUN && n_pairs * p.cache.kv_heads <= sms) {
+            int pieces = 0;
+            for (int i = tid; i < n_pairs; i += 256) pieces += (l.pairs[i].count + chunk - 1) / chunk;
+            pieces = __reduce_add_sync(0xffffffffu, pieces);
+            __syncthreads();
+            if (lane == 0) sums[warp] = pieces;
+            __syncthreads();
+            pieces = 0;
+            for (int w = 0; w < 8; ++w) pieces += sums[w];
+            if (pieces * p.cache.kv_heads <= sms) break;
+            ++chunk;
+        }
+        __syncthreads();
+        const Deal deal(max(units, 1), sms, chunk);
         int before = 0;
         for (int i0 = 0; i0 < n_pairs; i0 += 256) {
             const int c = i0 + tid < n_pairs ? l.pairs[i0 + tid].count : 0, n = p.cache.kv_heads * (deal.runs ? c : deal.pieces(c));
@@ -194,25 +211,27 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
             l.before[n_pairs] = before;
             l.before[gridDim.x] = n_pairs;  // (gridDim.x - 1 pairs at most)
             l.before[gridDim.x + 1] = units;
+            l.before[gridDim.x + 2] = chunk;
         }
         return;
     }
     // which request's pair this is: a lane a request
+    const int pair = (int)blockIdx.x - 1;
     int seq = -1, k = 0;
     for (int s0 = 0, before = 0; s0 < p.seqs && seq < 0; s0 += 32) {
         const int n = s0 + lane < p.seqs ? Request(p, s0 + lane).pairs(p) : 0, upto = warp_inclusive(n, lane);
-        const unsigned here = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + upto);
+        const unsigned here = __ballot_sync(0xffffffffu, pair < before + upto);
         if (here) {
             const int at = __ffs(here) - 1;
             seq = s0 + at;
-            k = (int)blockIdx.x - before - __shfl_sync(0xffffffffu, upto - n, at);
+            k = pair - before - __shfl_sync(0xffffffffu, upto - n, at);
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (seq < 0) return;
     const Request rq(p, seq);
     const int head = blockIdx.y, g = lane >> 2, c = lane & 3;
-    const size_t index = (size_t)blockIdx.x * gridDim.y + head;
+    const size_t index = (size_t)pair * gridDim.y + head;
     for (int rr = 8 * warp + g; rr < 2 * ROWS; rr += 64) {
         const int row = k * 2 * ROWS + rr, r = rr % ROWS;
         const bool valid = row < rq.rows;
@@ -506,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     const int n_pairs = l.before[pair_room + 1], units = l.before[pair_room + 2];
-    Jobs jobs = {0, 0, 0, pair_room > TABLE, Deal(max(units, 1), sms), before, n_pairs, p.cache.kv_heads, (int)gridDim.x, l.pairs};
+    Jobs jobs = {0, 0, 0, pair_room > TABLE, Deal(max(units, 1), sms, l.before[pair_room + 3]), before, n_pairs, p.cache.kv_heads, (int)gridDim.x, l.pairs};
     if (jobs.direct) {
         jobs.u = blockIdx.x, jobs.stop = min(jobs.u + 1, n_pairs * p.cache.kv_heads);
     } else {

@@ -34,9 +34,9 @@ struct Shape {
     static constexpr int SMEM = 4 * OPERAND + 2 * V_BYTES + 1024;
 };
 
-// A pair of tiles: request, which one of the request, first block of cached rows and how many.
-struct Pair {
-    int seq, index, first, count;
+// A pair of tiles: request, which one of the request, first block of cached rows and how many; and what a request is.
+struct __align__(16) Pair {
+    int seq, index, first, count, t0, rows, start, limit;
 };
 
 // Scratch of a step: queries as operands, their scales, the pairs, running sums of blocks (or pieces), parts.
@@ -100,6 +100,7 @@ struct Deal {
 
 struct Request {
     int t0, rows, start, limit;
+    __device__ __forceinline__ explicit Request(const Pair& pair) : t0(pair.t0), rows(pair.rows), start(pair.start), limit(pair.limit) {}
     __device__ __forceinline__ Request(const PackedAttention& p, int seq) {
         t0 = max(p.q_start[seq], 0);
         rows = (min(p.q_start[seq + 1], p.tokens) - t0) * p.group;
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
                 if (mine == 0) continue;
                 const Request rq(p, seq);
                 for (int k = lane; k < mine; k += 32) {
-                    Pair q = {seq, k, 0, 0};
+                    Pair q = {seq, k, 0, 0, rq.t0, rq.rows, rq.start, rq.limit};
                     int to;
                     rq.blocks(p, k * 2 * ROWS, min((k + 1) * 2 * ROWS, rq.rows) - 1, q.first, to);
                     q.count = max(1, to - q.first);
@@ -444,6 +445,12 @@ __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t a, uint32_t b,
     mma_from_smem(d, (uint32_t)ea, (uint32_t)eb, (uint32_t)(ea >> 32), idesc, 1u, leads);
 }
 
+// Of 32 rows from `row` on, those in [lo, hi).
+__device__ __forceinline__ uint32_t rows_within(int row, int lo, int hi) {
+    const int from = max(lo - row, 0), to = min(hi - row, 32);
+    return from >= to ? 0u : (0xffffffffu >> (32 - (to - from))) << from;
+}
+
 // What the converting warps say of a block.
 template <int W>
 struct Info {
@@ -568,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
         int n = 0, done = 0;  // blocks of the CTA so far; of this tile
         while (jobs.next(job)) {
             const Pair pair = l.pairs[job.pair];
-            const Request rq(p, pair.seq);
+            const Request rq(pair);
             const Active act(p, rq, pair, job, t);
             const int row = pair.index * 2 * ROWS + t * ROWS + r;
             const bool valid = row < rq.rows;
@@ -604,12 +611,9 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                     tmem_load_32x32(my_s + 32 * h, sc);
                     tmem_load_wait();
                     if (!whole) {
-                        const uint32_t there = info.there[h];
+                        const uint32_t seen = info.there[h] & rows_within(key0 + 32 * h, lo, hi);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const int key = key0 + 32 * h + c;
-                            sc[c] = key >= lo && key < hi && (there >> c & 1) ? sc[c] : 0xff800000u;
-                        }
+                        for (int c = 0; c < 32; ++c) sc[c] = seen & 1u << c ? sc[c] : 0xff800000u;
                     }
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) top = fmaxf(top, fmaxf(__uint_as_float(sc[c]), __uint_as_float(sc[c + 1])));
@@ -646,12 +650,9 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                     tmem_load_32x32(my_s + 32 * h, sc);
                     tmem_load_wait();
                     if (!whole) {
-                        const uint32_t there = info.there[h];
+                        const uint32_t seen = info.there[h] & rows_within(key0 + 32 * h, lo, hi);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const int key = key0 + 32 * h + c;
-                            sc[c] = key >= lo && key < hi && (there >> c & 1) ? sc[c] : 0xff800000u;
-                        }
+                        for (int c = 0; c < 32; ++c) sc[c] = seen & 1u << c ? sc[c] : 0xff800000u;
                     }
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
@@ -764,7 +765,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
         int n = 0;
         while (jobs.next(job)) {
             const Pair pair = l.pairs[job.pair];
-            const Request rq(p, pair.seq);
+            const Request rq(pair);
             const int* table = p.tables + (size_t)pair.seq * p.width;
             int lo, end;
             rq.sees(p, min((pair.index + 1) * 2 * ROWS, rq.rows) - 1, lo, end);
@@ -877,7 +878,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
         const auto weighed = [&](int t) { return t ? weighed1 : weighed0; };
         while (jobs.next(job)) {
             const Pair pair = l.pairs[job.pair];
-            const Request rq(p, pair.seq);
+            const Request rq(pair);
             const Active act0(p, rq, pair, job, 0), act1(p, rq, pair, job, 1);
             const auto has = [&](int t, int i) { return i >= (t ? act1.from : act0.from) && i < (t ? act1.to : act0.to); };
             // the queries of the job before are read no more when its last products are done

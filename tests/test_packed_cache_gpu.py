@@ -275,6 +275,33 @@ def test_scores_far_apart_and_scales_of_all_sizes(ops, workspace, dtype):
     check_step(ops, workspace, [(37, 40), (20, 40)], 4, 2, 64, 16, dtype, seed=6, spoil=spoil)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, D, queries", [(7, 1, 64, 1), (4, 1, 128, 1), (2, 1, 96, 3), (8, 1, 64, 9)])
+def test_sums_over_very_many_rows(ops, workspace, dtype, heads, kv_heads, D, queries):
+    """70,000 rows of nearly equal weight, so that the output is small beside what is added up."""
+    gen, n, ps = rng(D), 70000, 16
+    pages = -(-n // ps)
+    cache = []
+    for _ in range(2):
+        cache.append(torch.randint(0, 256, (pages, kv_heads, ps, D // 2), generator=gen, device=DEV, dtype=torch.uint8))
+        scale = 0.05 + 0.3 * torch.rand(pages, kv_heads, ps, D // 32, generator=gen, device=DEV)
+        cache.append(torch.stack([scale, -7.5 * scale], -1).to(torch.bfloat16))
+    tables = torch.randperm(pages, generator=gen, device=DEV).to(torch.int32)[None].contiguous()
+    q = torch.randn(queries, heads * D, generator=gen, device=DEV).to(dtype)
+    out, weights = torch.empty_like(q), torch.zeros(1, kv_heads, n, device=DEV)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    ops.packed_attention(q, out, packed(ops, cache), tables, i32(0, queries), i32(n - queries), queries, n, heads, 0.3 * D ** -0.5, weights=weights,
+                         workspace=workspace)
+    k, v, has = plain.request_rows(cache, tables[0], n, ps)
+    want, w, _, _ = plain.attend(q.double().view(queries, heads, D), k, v, has, n - queries, 0.3 * D ** -0.5)
+    off = (out.double().view(queries, heads, D) - want).norm() / want.norm()
+    # 32-bit rows: scores and weights within a few 2^-23, sums of 16 to 32 rows cut off at 24 bits, those added up in rounded fp32 over
+    # some thousand places in turn, errors of both signs; bf16 rows: the result's rounding (2^-9 on average, at most 2^-8 of each number)
+    # and weights in eleven bits.
+    assert off < (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -18), off
+    assert ((weights[0].double() - w).abs() / w).max() < 2.0 ** -15 and (weights[0].double() - w).norm() / w.norm() < 2.0 ** -18
+
+
 def test_same_bits_from_run_to_run(ops, workspace):
     cache, tables, q, q_start, start_row, rows = make_step(2, [(1, 900), (1, 2500)], 12, 2, 128, 16, torch.bfloat16)
     pages, seen = packed(ops, cache), []

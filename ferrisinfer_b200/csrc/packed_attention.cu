@@ -612,7 +612,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
 // Stages of 32 cached rows that a request's queries see together (at least one, so that every request has a block), from which on.
 __device__ __forceinline__ int stages_of(const PackedAttention& p, int seq, int& floor) {
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, start = p.start_row[seq];
-    const int most = max(0, min(start + n, p.width * p.cache.page_size));
+    const int most = max(0, min(start + n, p.limit));
     const int least = min(p.window > 0 ? max(0, start - p.window + 1) : 0, most);
     floor = least / STAGE * STAGE;
     return n > 0 && n * p.group <= p.few ? max(1, (most - floor + STAGE - 1) / STAGE) : 0;
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
     __shared__ int warp_total[2][WARPS], last_here;
     pdl_launch_dependents();
     pdl_wait();
-    const int c = threadIdx.x & 3, limit = p.width * p.cache.page_size, me = blockIdx.x;
+    const int c = threadIdx.x & 3, limit = p.limit, me = blockIdx.x;
     Segment<NT> seg;
     Deal deal(WARPS, 1);
     int u = 0, stop = 1, s = 0;
@@ -745,6 +745,7 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
         }
         const int head = seg.head;
         seg.seq = s, seg.t0 = max(p.q_start[s], 0), seg.count = (min(p.q_start[s + 1], p.tokens) - seg.t0) * p.group;
+        if (p.even) seg.count = min(seg.count, 8 * NT);  // (what the caller says no request exceeds)
         if (seg.first >= seg.count) return;
         seg.rows.set(p, seg.first, seg.count, p.start_row[s], limit, c);
         const int floor = seg.rows.least / STAGE * STAGE;
@@ -840,8 +841,13 @@ __global__ void __launch_bounds__(256) packed_attention_scored_weights_kernel(co
     pdl_wait();
     const int head = blockIdx.y, seq = blockIdx.z, row = blockIdx.x * 256 + threadIdx.x;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
-    const int end = min(min(start + n, p.width * p.cache.page_size), p.max_rows);
-    if (row >= end || n <= 0 || count > p.few) return;
+    const int end = min(min(start + n, p.limit), p.max_rows);
+    if (n <= 0 || count > p.few || count > cols) return;  // (the whole block)
+    __shared__ float lse[16];  // of the request's query rows
+    if (threadIdx.x < count)
+        lse[threadIdx.x] = p.lse[(size_t)(t0 + threadIdx.x / p.group) * p.heads + head * p.group + threadIdx.x % p.group];
+    __syncthreads();
+    if (row >= end) return;
     int floor;
     stages_of(p, seq, floor);
     float total = 0.0f;
@@ -853,7 +859,7 @@ __global__ void __launch_bounds__(256) packed_attention_scored_weights_kernel(co
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 if (i + k < count && x[k] != -INFINITY)  // (a row that is not seen, beside a sum that is not finite)
-                    total += exp2_fast(x[k] - p.lse[(size_t)(t0 + (i + k) / p.group) * p.heads + head * p.group + (i + k) % p.group]);
+                    total += exp2_fast(x[k] - lse[i + k]);
         }
     }
     float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride + row;
@@ -900,7 +906,7 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const int head = blockIdx.y, seq = blockIdx.z, at = (blockIdx.x * WARPS + warp) * STAGE;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
-    const int limit = p.width * p.cache.page_size, end = min(min(start + n, limit), p.max_rows);
+    const int limit = p.limit, end = min(min(start + n, limit), p.max_rows);
     if (at >= end || count > p.few) return;
     const int* table = p.tables + (size_t)seq * p.width;
     unsigned char* stage = smem + warp * Stage<W>::BYTES;
@@ -1108,6 +1114,7 @@ FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
     p.even = plan.even, p.most_blocks = plan.most, p.counters = plan.counters ? a->counters : nullptr;
     p.max_stages = a->max_kv / STAGE + 2;
     p.page = DivideBy(a->page_size);
+    p.limit = a->width * a->page_size < a->max_kv ? a->width * a->page_size : a->max_kv;
     p.weights = a->weights, p.seq_slot = a->seq_slot, p.slot_stride = a->slot_stride, p.head_stride = a->head_stride, p.max_rows = a->max_rows, p.add = a->add;
     p.status = ferris_status_ptr();
     void* ps = a->scratch + (plan.scratch() - plan.prompt_floats);

@@ -15,6 +15,7 @@ struct PackedAttention {
     PackedCache cache;
     const int* tables;
     int width;  // blocks of a request's table
+    int limit;  // rows that a request may have: those of its table, and no more than the caller says
     const int* q_start;
     const int* start_row;
     int seqs, heads, group, window;

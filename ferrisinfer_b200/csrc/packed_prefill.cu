@@ -45,6 +45,7 @@ struct Layout {
     float* scales;           // [pair][kv head][256]: what makes a product one to the base of 2
     float* minus_lse;        // the same: minus the log2 of the row's sum (with weights; minus infinity for rows that are not there)
     int* first_pair;         // [request]
+    int room;                // pairs that there is room for
     Pair* pairs;
     int* before;             // [pairs + 1], then the number of pairs, units, blocks of a piece
     float* parts;            // [place][D + 2][256]
@@ -79,6 +80,7 @@ Layout make_layout(void* base, int D, int pairs, int kv_heads, int seqs, int gri
         used += (bytes + 1023) / 1024 * 1024;
     });
     l.bytes = used;
+    l.room = pairs;
     return l;
 }
 
@@ -105,7 +107,7 @@ struct Request {
         t0 = max(p.q_start[seq], 0);
         rows = (min(p.q_start[seq + 1], p.tokens) - t0) * p.group;
         start = p.start_row[seq];
-        limit = p.width * p.cache.page_size;
+        limit = p.limit;
     }
     __device__ __forceinline__ int pairs(const PackedAttention& p) const { return rows > p.few ? (rows + 2 * ROWS - 1) / (2 * ROWS) : 0; }
     __device__ __forceinline__ void sees(const PackedAttention& p, int r, int& lo, int& hi) const {
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
                 const int mine = __shfl_sync(0xffffffffu, n, i), first = __shfl_sync(0xffffffffu, at, i), seq = s0 + 32 * warp + i;
                 if (mine == 0) continue;
                 const Request rq(p, seq);
-                for (int k = lane; k < mine; k += 32) {
+                for (int k = lane; k < mine && first + k < (int)gridDim.x - 1; k += 32) {  // (as many as there is room for)
                     Pair q = {seq, k, 0, 0, rq.t0, rq.rows, rq.start, rq.limit};
                     int to;
                     rq.blocks(p, k * 2 * ROWS, min((k + 1) * 2 * ROWS, rq.rows) - 1, q.first, to);
@@ -170,6 +172,7 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
             n_pairs += all;
             __syncthreads();
         }
+        n_pairs = min(n_pairs, (int)gridDim.x - 1);
         int units = 0;
         for (int i = tid; i < n_pairs; i += 256) units += l.pairs[i].count;
         units = __reduce_add_sync(0xffffffffu, units);
@@ -972,7 +975,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
     // the tiles of the query rows that see any of these keys
     const long long first_row = (long long)max(key0 - rq.start, 0) * p.group;
     const long long last_row = p.window > 0 ? ((long long)key0 + W_KEYS * BLOCK - 1 - rq.start + p.window) * p.group : rq.rows;
-    const int from = (int)(min(first_row, (long long)rq.rows) / ROWS), to = (int)((max(min(last_row, (long long)rq.rows), 0ll) + ROWS - 1) / ROWS);
+    const int from = (int)(min(first_row, (long long)rq.rows) / ROWS);
+    int to = (int)((max(min(last_row, (long long)rq.rows), 0ll) + ROWS - 1) / ROWS);
     if (threadIdx.x == 0) {
         for (int i = 0; i < W_STAGES; ++i) mbar_init(&q_full[i], 1);
         for (int i = 0; i < 2; ++i) {
@@ -989,6 +993,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
     pdl_launch_dependents();
     const uint32_t tmem = tmem_base;  // scores of block k, every other tile, at 256 k + 128 (tile % 2)
     const size_t first_pair = l.first_pair[seq];
+    to = min(to, max(2 * (l.room - (int)first_pair), from));
     bool ok = true;
     if (warp < 4 * W_KEYS) {
         const int k = warp >> 2, t = (warp & 3) * 32 + lane, row = key0 + k * BLOCK + t, block = p.block_of(row);

@@ -2502,7 +2502,7 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
     [S + 1]; they cover all of q) and held ``seq_start_row[s]`` rows (int32 [S]) of the cache before them; its query i sees rows
     0 .. seq_start_row[s] + i, with ``window`` > 0 the last so many of them, as far as ``block_tables`` (int32 [S, blocks]) names
     pages for them.  A query that sees nothing gives zeros.  ``max_q_len``, ``max_kv_len``: the most queries and rows (those of the
-    step included) of any request.
+    step included) of any request; rows beyond ``max_kv_len`` are not seen.
 
     ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` for request s, row s without it): every cached row's weight
     in the softmax, summed over the request's queries and the query heads of the kv head, is added to it; the rows that

@@ -312,6 +312,23 @@ def test_same_bits_from_run_to_run(ops, workspace):
     assert all(torch.equal(a, b) for one in seen[1:] for a, b in zip(seen[0], one))
 
 
+@pytest.mark.parametrize("lengths", [[(1, 500), (1, 90)], [(70, 300), (1, 100), (3, 9)]])
+def test_rows_beyond_what_the_caller_names_are_not_seen(ops, workspace, lengths):
+    cache, tables, q, q_start, start_row, rows = make_step(3, lengths, 6, 2, 64, 16, torch.bfloat16)
+    most, at = 200, 0
+    out, weights = torch.empty_like(q), torch.zeros(len(lengths), 2, most, device=DEV)
+    ops.packed_attention(q, out, packed(ops, cache), tables, q_start, start_row, max(n for n, _ in lengths), most, 6, 0.125, weights=weights, workspace=workspace)
+    for i, ((n, start), r) in enumerate(zip(lengths, rows)):
+        k, v, has = plain.request_rows(cache, tables[i], r, 16)
+        has[most:] = False
+        want, w, size, _ = plain.attend(q[at:at + n].double().view(n, 6, 64), k, v, has, start, 0.125)
+        got = out[at:at + n].double().view(n, 6, 64)
+        assert ((got - want).abs() <= (size + 4) * 2.0 ** -10 + want.abs() * 2.0 ** -8).all()
+        held = min(r, most)
+        assert ((weights[i, :, :held].double() - w[:, :held]).abs() <= w[:, :held] * 2.0 ** -14 + 1e-12).all()
+        at += n
+
+
 def test_on_another_stream(ops, workspace):
     check_step(ops, workspace, [(1, 90)], 4, 2, 64, 16, torch.bfloat16)
     stream = torch.cuda.Stream()

@@ -127,9 +127,9 @@ struct RowsCall {
     }
 };
 
-// Bound by HBM for many tokens, by its launch for a step's: 16-byte loads of a head's elements, lanes side by side; the divisions
-// by heads and page size are multiplications (as 64-bit divisions they were half of the kernel: 8,192 tokens of 4 heads of
-// 128, written and read back, 28.8 us).
+// Bound by its instructions for many tokens (8,192 tokens of 4 heads of 128: 13.5 us, 1.6 TB/s; 21 us with a division for each
+// element), by its launch for a step's (3.1 us): 16-byte loads of a head's elements, lanes side by side; the divisions by
+// heads and page size are multiplications (here and in the read, written and read back 28.8 -> 24.8 us against 64-bit divisions).
 template <typename T, int W, bool VEC>
 __global__ void __launch_bounds__(256) packed_write_kernel(const T* k, const T* v, const RowsCall q) {
     pdl_launch_dependents();
@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(256) packed_write_kernel(const T* k, const T* 
     }
 }
 
-// read: out[t] = the values that the row at slots[t] stands for, rounded once (zeros for slots below 0)
+// read: out[t] = the values that the row at slots[t] stands for, rounded once (zeros for slots below 0).  Bound by memory for many
+// tokens: 65,536 of 4 heads of 128 40 us (4.4 TB/s), 8,192 6.5 us (3.4 TB/s).
 __device__ __forceinline__ Eight dequantise8(uint32_t codes, uint32_t scales) {
     const float scale = packed_scale(scales), least = packed_least(scales);
     Eight e;
@@ -227,8 +228,9 @@ constexpr int EVICT_COPIES = 4;        // of a histogram: lanes that meet in a b
 // A cluster of blocks per (request, kv head), each with a run of its rows, whose keys it holds in shared memory (longer runs are
 // read again each time).  The budget-th greatest key by its four bytes, most significant first: a histogram of 256 bins
 // each, added up over the cluster; then the kept rows in order, every warp its own run of rows.  What bounds it is the
-// chain of short passes and barriers, so a lane takes four rows at a time, each on its own (with lanes that share a bin
-// found by votes, or by `match.any`, a pass over 32 rows took 350 cycles).
+// chain of short passes and barriers, so a lane takes four rows at a time, each on its own.  16 requests of up to 32,768 rows and
+// 4 heads: 32 us (one row at a time, lanes that share a bin found by votes, 44 to 47; all of the eviction with the read-back was
+// no faster with `match.any`); 5,000 rows of one request 16 us.
 __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(const float* weights, long long slot_stride, int head_stride,
                                                                             const int* __restrict__ seq_rows, const int* __restrict__ seq_slot,
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
@@ -397,7 +399,8 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
 }
 
 // Kept rows from their pages into others: every thread 16 bytes of codes of a row's keys and of its values, W threads a row, and the
-// rows' scales by the same threads; four rows of a thread are fetched together.
+// rows' scales by the same threads; four rows of a thread are fetched together.  16 requests of 4,096 kept rows, 4 heads of 128: 25 us
+// (84 MB read and written, 3.4 TB/s).
 template <int W>
 __global__ void __launch_bounds__(256) packed_evict_move_kernel(PackedCache from, PackedCache to, const int* __restrict__ from_tables,
                                                                 int from_width, const int* __restrict__ to_tables, int to_width,

@@ -843,8 +843,8 @@ __global__ void __launch_bounds__(256) packed_attention_scored_weights_kernel(co
     pdl_wait();
     const int head = blockIdx.y, seq = blockIdx.z, row = blockIdx.x * 256 + threadIdx.x;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
-    const int end = min(min(start + n, p.limit), p.max_rows);
-    if (n <= 0 || count > p.few || count > cols) return;  // (the whole block)
+    const int end = min(min(start + n, p.limit), p.max_rows), slot = slot_of(p, seq);
+    if (n <= 0 || count > p.few || count > cols || slot < 0) return;  // (the whole block)
     __shared__ float lse[16];  // of the request's query rows
     if (threadIdx.x < count)
         lse[threadIdx.x] = p.lse[(size_t)(t0 + threadIdx.x / p.group) * p.heads + head * p.group + threadIdx.x % p.group];
@@ -864,7 +864,7 @@ __global__ void __launch_bounds__(256) packed_attention_scored_weights_kernel(co
                     total += exp2_fast(x[k] - lse[i + k]);
         }
     }
-    float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride + row;
+    float* w = p.weights + slot * p.slot_stride + (long long)head * p.head_stride + row;
     *w = p.add && row < start ? *w + total : total;
 }
 
@@ -908,8 +908,8 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const int head = blockIdx.y, seq = blockIdx.z, at = (blockIdx.x * WARPS + warp) * STAGE;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
-    const int limit = p.limit, end = min(min(start + n, limit), p.max_rows);
-    if (at >= end || count > p.few) return;
+    const int limit = p.limit, end = min(min(start + n, limit), p.max_rows), slot = slot_of(p, seq);
+    if (at >= end || count > p.few || slot < 0) return;
     const int* table = p.tables + (size_t)seq * p.width;
     unsigned char* stage = smem + warp * Stage<W>::BYTES;
     const uint32_t there = Stage<W>::request(p, table, head, at, end, stage, lane);
@@ -948,7 +948,7 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
             }
         }
     }
-    float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride;
+    float* w = p.weights + slot * p.slot_stride + (long long)head * p.head_stride;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -1086,7 +1086,8 @@ struct FerrisPackedAttention {
     const int* seq_slot;
     void* stream;
     long long slot_stride;
-    int ldq, ldo, dtype, pages, kv_heads, page_size, head_dim, width, seqs, tokens, heads, max_q, max_kv, window, head_stride, max_rows, add;
+    int ldq, ldo, dtype, pages, kv_heads, page_size, head_dim, width, seqs, tokens, heads, max_q, max_kv, window, head_stride, max_rows, add,
+        slots;
     float scale;
 };
 
@@ -1117,7 +1118,7 @@ FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
     p.max_stages = a->max_kv / STAGE + 2;
     p.page = DivideBy(a->page_size);
     p.limit = a->width * a->page_size < a->max_kv ? a->width * a->page_size : a->max_kv;
-    p.weights = a->weights, p.seq_slot = a->seq_slot, p.slot_stride = a->slot_stride, p.head_stride = a->head_stride, p.max_rows = a->max_rows, p.add = a->add;
+    p.weights = a->weights, p.seq_slot = a->seq_slot, p.slots = a->slots, p.slot_stride = a->slot_stride, p.head_stride = a->head_stride, p.max_rows = a->max_rows, p.add = a->add;
     p.status = ferris_status_ptr();
     void* ps = a->scratch + (plan.scratch() - plan.prompt_floats);
     int* pc = a->counters + plan.counters;

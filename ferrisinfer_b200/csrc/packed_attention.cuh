@@ -32,6 +32,7 @@ struct PackedAttention {
     DivideBy page;  // the page size
     float* weights;
     const int* seq_slot;
+    int slots;  // rows of the weights that requests may have
     long long slot_stride;
     int head_stride, max_rows, add;
     int* status;
@@ -42,6 +43,16 @@ struct PackedAttention {
         return (uint32_t)(page * cache.kv_heads + head) * cache.page_size + (uint32_t)(row - block * cache.page_size);
     }
 };
+
+// The row of the weights that belongs to a request, -1 where it has none.
+__device__ __forceinline__ int slot_of(const PackedAttention& p, int seq) {
+    const int slot = p.seq_slot ? p.seq_slot[seq] : seq;
+    if (slot >= p.slots) {
+        ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 104);
+        return -1;
+    }
+    return slot;
+}
 
 // The page of a request's row, -1 where it has none.
 __device__ __forceinline__ int page_of(const PackedAttention& p, const int* table, int block) {

@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
                                                                             const int* __restrict__ seq_rows, const int* __restrict__ seq_slot,
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
                                                                             int kept_head_stride, int budget, int keep_first, int keep_last,
-                                                                            int max_rows, int held) {
+                                                                            int max_rows, int held, int slots, int* status) {
     extern __shared__ uint32_t keys[];  // [held]
     __shared__ uint32_t hist[4][EVICT_COPIES][256], total[256];
     __shared__ int greater[EVICT_WARPS], equal[EVICT_WARPS], counts[2];
@@ -243,7 +243,9 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     pdl_wait();
     const int s = blockIdx.y, h = blockIdx.x, heads = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int blocks = gridDim.z, rank = blockIdx.z;
-    const int n = min(max(seq_rows[s], 0), max_rows), slot = seq_slot ? seq_slot[s] : s;
+    const int slot = seq_slot ? seq_slot[s] : s;
+    if (slot >= slots) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 105);
+    const int n = slot < 0 || slot >= slots ? 0 : min(max(seq_rows[s], 0), max_rows);  // (without weights: no rows; nothing of w is then read)
     const float* w = weights + slot * slot_stride + (long long)h * head_stride;
     int* rows = kept_rows + ((size_t)s * heads + h) * budget;
     float* kw = kept_weights ? kept_weights + slot * kept_slot_stride + (long long)h * kept_head_stride : nullptr;
@@ -537,7 +539,7 @@ struct FerrisPackedEvict {
     void* stream;
     long long slot_stride, kept_slot_stride;
     int from_pages, from_page_size, to_pages, to_page_size, kv_heads, head_dim, from_width, to_width, head_stride, max_rows, kept_head_stride,
-        seqs, budget, keep_first, keep_last;
+        seqs, budget, keep_first, keep_last, slots;
 };
 
 FERRIS_API int ferris_packed_cache_evict(const FerrisPackedEvict* a) {
@@ -559,7 +561,8 @@ FERRIS_API int ferris_packed_cache_evict(const FerrisPackedEvict* a) {
     if (const int r = ferris_allow_dynamic_smem((const void*)packed_evict_select_kernel, (size_t)held * 4)) return r;
     cudaError_t e = ferris_launch_cluster(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,
                                           a->weights, a->slot_stride, a->head_stride, a->seq_rows, a->seq_slot, a->kept_rows, a->kept_weights,
-                                          a->kept_slot_stride, a->kept_head_stride, budget, keep_first, keep_last, max_rows, held);
+                                          a->kept_slot_stride, a->kept_head_stride, budget, keep_first, keep_last, max_rows, held, a->slots,
+                                          ferris_status_ptr());
     if (e != cudaSuccess) FERRIS_LAUNCH_CHECK();
     return with_groups(head_dim, [&](auto w) {
         constexpr int W = decltype(w)::value, ROWS = 256 / W * 4;

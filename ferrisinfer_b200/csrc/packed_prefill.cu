@@ -971,7 +971,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
     pdl_wait();
     const Request rq(p, seq);
     const int key0 = blockIdx.x * W_KEYS * BLOCK, end = min(max(0, min(rq.start + rq.rows / p.group, rq.limit)), p.max_rows);
-    if (rq.rows <= p.few || key0 >= end) {
+    const int slot = slot_of(p, seq);
+    if (rq.rows <= p.few || key0 >= end || slot < 0) {
         pdl_launch_dependents();
         return;
     }
@@ -1079,7 +1080,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
             for (int x = 0; x < W_KEYS; ++x) {
                 const int row = key0 + x * BLOCK + t;
                 if (row < end) {
-                    float* w = p.weights + (long long)(p.seq_slot ? p.seq_slot[seq] : seq) * p.slot_stride + (long long)head * p.head_stride + row;
+                    float* w = p.weights + slot * p.slot_stride + (long long)head * p.head_stride + row;
                     const float sum = (total[x][0] + total[x][1]) + sums[x][t];
                     *w = p.add && row < rq.start ? *w + sum : sum;
                 }

@@ -2416,8 +2416,8 @@ class PackedPages:
 # Arguments of a call laid out for the library in one go (ctypes converts them one by one, which costs more than a launch).  The
 # library is called by one thread at a time.
 _PACKED_ROWS = struct.Struct("=8Q8i")
-_PACKED_ATTENTION = struct.Struct("=14Qq17if")
-_PACKED_EVICT = struct.Struct("=16Q2q15i")
+_PACKED_ATTENTION = struct.Struct("=14Qq18if")
+_PACKED_EVICT = struct.Struct("=16Q2q16i")
 _packed_buffer = ctypes.create_string_buffer(max(_PACKED_ROWS.size, _PACKED_ATTENTION.size, _PACKED_EVICT.size))
 _packed_buffer_at = ctypes.addressof(_packed_buffer)
 
@@ -2504,9 +2504,9 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
     pages for them.  A query that sees nothing gives zeros.  ``max_q_len``, ``max_kv_len``: the most queries and rows (those of the
     step included) of any request; rows beyond ``max_kv_len`` are not seen.
 
-    ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` for request s, row s without it): every cached row's weight
-    in the softmax, summed over the request's queries and the query heads of the kv head, is added to it; the rows that
-    came with this step (and with ``add_weights`` False all of them) are set instead."""
+    ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` for request s, row s without it; below 0: the request has
+    none): every cached row's weight in the softmax, summed over the request's queries and the query heads of the kv head, is
+    added to it; the rows that came with this step (and with ``add_weights`` False all of them) are set instead."""
     dev, D, hkv = pages.device_index, pages.head_dim, pages.kv_heads
     try:  # (a tensor of the host has device -1)
         there = dev == q.get_device() == out.get_device() == block_tables.get_device() == seq_q_start.get_device() == seq_start_row.get_device()
@@ -2534,14 +2534,15 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
         raise KernelError(f"packed attention: tables {tuple(block_tables.shape)}, {seq_q_start.numel()} first rows for {S} requests")
     if max_q_len < 0 or max_kv_len < 0 or window < 0:
         raise KernelError(f"packed attention: at most {max_q_len} queries, {max_kv_len} rows, window {window}")
-    w = (0, 0, 0, 0, 0)
+    w = (0, 0, 0, 0, 0, 0)
     if weights is not None:
         slots, rows, slot_stride, head_stride = _weight_rows(weights, hkv, "packed attention weights")
         if seq_slot is not None:
             _need(seq_slot, "slots of the weights", torch.int32)
-        if (seq_slot.numel() != S if seq_slot is not None else slots < S) or rows < max_kv_len or weights.get_device() != dev:
+        if (seq_slot.numel() != S or seq_slot.get_device() != dev if seq_slot is not None else slots < S) or rows < max_kv_len \
+                or weights.get_device() != dev:
             raise KernelError(f"packed attention: weights {tuple(weights.shape)} for {S} requests of at most {max_kv_len} rows")
-        w = (weights.data_ptr(), 0 if seq_slot is None else seq_slot.data_ptr(), slot_stride, head_stride, rows)
+        w = (weights.data_ptr(), 0 if seq_slot is None else seq_slot.data_ptr(), slot_stride, head_stride, rows, slots)
     if T == 0 or S == 0 or max_q_len == 0:
         return
     if table_shape[1] == 0:
@@ -2557,7 +2558,7 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
         _packed_buffer, 0, q.data_ptr(), out.data_ptr(), *pages._args, block_tables.data_ptr(), seq_q_start.data_ptr(), seq_start_row.data_ptr(),
         workspace.address("packed_attention", scratch, torch.float32), workspace.address("packed_attention_counters", counters, torch.int32, True),
         w[0], w[1], _current_stream(), w[2], ldq, ldo, dt, pages.pages, hkv, pages.page_size, D, table_shape[1], S, T, num_heads, max_q_len,
-        max_kv_len, window, w[3], w[4], 1 if add_weights else 0, scale)
+        max_kv_len, window, w[3], w[4], 1 if add_weights else 0, w[5], scale)
     _check(_packed_lib().ferris_packed_attention(_packed_buffer_at), "packed attention", launches)
 
 
@@ -2577,7 +2578,7 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
 
     Of the ``seq_rows[s]`` rows (int32 [S]) of request s there stay its first ``keep_first``, its last ``keep_last`` and, of the
     others, those of the greatest ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` or s; the lower row first among
-    equals, NaN before every number).  They move, in their order, into rows 0, 1, ... of the pages that ``kept_tables`` (int32
+    equals, NaN before every number; a slot below 0: nothing of the request is kept).  They move, in their order, into rows 0, 1, ... of the pages that ``kept_tables`` (int32
     [S, blocks]) names in ``kept_pages`` (the same cache will do; none of the pages that are read).  The old pages keep what they
     held, so other requests may share them.  Afterwards the request holds min(seq_rows[s], budget) rows.
     ``kept_rows`` (int32 [S, kv heads, budget]) gets their numbers, -1 behind them; ``kept_weights`` (fp32 [slots, kv heads, >=
@@ -2624,5 +2625,5 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
         _packed_buffer, 0, *pages._args, *kept_pages._args, block_tables.data_ptr(), kept_tables.data_ptr(), seq_rows.data_ptr(),
         0 if seq_slot is None else seq_slot.data_ptr(), weights.data_ptr(), kept_rows.data_ptr(), kept[0], _current_stream(), slot_stride, kept[1],
         pages.pages, pages.page_size, kept_pages.pages, kept_pages.page_size, hkv, pages.head_dim, block_tables.shape[1], kept_tables.shape[1],
-        head_stride, rows, kept[2], S, budget, keep_first, keep_last)
+        head_stride, rows, kept[2], S, budget, keep_first, keep_last, slots)
     _check(_packed_lib().ferris_packed_cache_evict(_packed_buffer_at), "eviction", 2)

@@ -1,0 +1,129 @@
+"""The packed cache at its edges: values far apart, rows and scores that are no numbers, loose bounds, holes, slots."""
+
+import math
+
+import pytest
+import torch
+
+import plain_packed as plain
+from test_packed_cache_gpu import make_step, packed
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from ferrisinfer_b200.kernels import ops as module
+
+    module.require_device()
+    return module
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(ops):
+    yield
+    torch.cuda.synchronize()
+    ops.check_kernel_status()
+
+
+@pytest.fixture(scope="module")
+def workspace():
+    from ferrisinfer_b200.engine.workspace import Workspace
+
+    return Workspace(DEV)
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def parts_of(cache, table, rows, page_size):
+    """|middle| + 8 scale of every element of the values of a request's rows, 64 bits: what stands in its sums beside what
+    the two make together (a value is middle + scale x (code - 8))."""
+    r = torch.arange(rows, device=DEV)
+    page = table.long()[(r // page_size).clamp(max=table.numel() - 1)].clamp(min=0)
+    s = cache[3][page, :, r % page_size].double()
+    return ((s[..., 1] + 8 * s[..., 0]).abs() + 8 * s[..., 0]).repeat_interleave(32, -1)
+
+
+def attend_and_compare(ops, workspace, step, lengths, heads, kv_heads, D, page_size, scale=None, window=0, max_q=None, max_kv=None, far=()):
+    """One step with the rows' weights against the plain form; the bounds follow each number's own sums.  ``far``: (request, row) whose
+    weight is nought whatever the last bits of its score."""
+    cache, tables, q, q_start, start_row, rows = step
+    scale = D ** -0.5 if scale is None else scale
+    most = max(rows)
+    out = torch.full((q.shape[0], heads * D), 7.0, dtype=q.dtype, device=DEV)
+    weights = torch.full((len(lengths), kv_heads, most), 3.0, device=DEV)
+    ops.packed_attention(q, out, packed(ops, cache), tables, q_start, start_row, max(n for n, _ in lengths) if max_q is None else max_q,
+                         most if max_kv is None else max_kv, heads, scale, window=window,
+                         weights=weights if max_kv is None else None, add_weights=False, workspace=workspace)
+    at = 0
+    for i, ((n, start), r) in enumerate(zip(lengths, rows)):
+        k, v, has = plain.request_rows(cache, tables[i], r, page_size)
+        mine = q[at:at + n].double().view(n, heads, D)
+        want, w, _, _ = plain.attend(mine, k, v, has, start, scale, window)
+        near = has.clone()
+        near[[row for request, row in far if request == i]] = False
+        spread = plain.attend(mine, k, v, near, start, scale, window)[3]
+        size = plain.attend(mine, k, parts_of(cache, tables[i], r, page_size), has, start, scale, window)[0]
+        # Scores: a sum of D / 8 + 8 steps of 24-bit numbers (cut rather than rounded), twice: in a weight and in the sum that it is
+        # divided by; the exponential and the weights' sums beside them.  Outputs: for bf16 rows weights, and their products
+        # with scales, in eleven bits (2^-9 covers both and their sum), and the result once more; else 24-bit sums.
+        rel = (D / 8 + 8) * 2.0 ** -23 * spread * 2 + 2.0 ** -19
+        lossy = 2.0 ** -9 if q.dtype == torch.bfloat16 else 0.0
+        bound = size * (rel[..., None] + lossy) + want.abs() * (lossy + 2.0 ** -23) + 1e-30
+        got = out[at:at + n].double().view(n, heads, D)
+        nan = torch.isnan(want)
+        assert torch.equal(torch.isnan(got), nan), (i, (torch.isnan(got) != nan).nonzero()[:4])
+        assert ((got - want).abs() <= bound)[~nan].all(), (i, ((got - want).abs() / bound)[~nan].max())
+        if max_kv is None and n:
+            g, nan = weights[i, :, :r].double(), torch.isnan(w)
+            assert torch.equal(torch.isnan(g), nan)
+            e = rel.nan_to_num(0.0).max()
+            assert ((g - w).abs() <= w * (e + 2.0 ** -20) + 1e-30)[~nan].all(), (i, ((g - w).abs() / (w * e + 1e-30))[~nan].max())
+        at += n
+    return out
+
+
+def with_queries(step, change):
+    cache, tables, q, *rest = step
+    return (cache, tables, change(q.clone()), *rest)
+
+
+# --------------------------------------------------------------------------------------------- slots of the weights
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths", [[(1, 90), (1, 30), (1, 50)], [(40, 90), (1, 30), (60, 50)], [(3, 90), (40, 30), (5, 50)]])
+def test_slots_outside_the_weights_touch_nothing(ops, workspace, dtype, lengths):
+    """A request whose slot is below 0 has no weights; one at or beyond their count is reported.  Neither touches their surroundings."""
+    cache, tables, q, q_start, start_row, rows = make_step(1, lengths, 6, 2, 64, 16, dtype)
+    pages, most = packed(ops, cache), max(rows)
+    for slots, wrong in ((i32(-1, 1, 0), False), (i32(0, 3, -7), True), (i32(2 ** 31 - 1, 2, -2 ** 31), True)):
+        around, out = torch.full((9, 2, most), 3.0, device=DEV), torch.empty(q.shape[0], 384, dtype=dtype, device=DEV)
+        ops.packed_attention(q, out, pages, tables, q_start, start_row, max(n for n, _ in lengths), most, 6, 0.125, weights=around[3:6], seq_slot=slots,
+                             add_weights=False, workspace=workspace)
+        assert (ops.kernel_status() != 0) == wrong
+        named = {int(s): i for i, s in enumerate(slots.tolist()) if 0 <= s < 3}
+        for row in range(9):
+            held = rows[named[row - 3]] if row - 3 in named else 0
+            assert (around[row, :, held:] == 3).all() and (held == 0 or not (around[row, :, :held] == 3).any())
+        assert out.float().isfinite().all()
+
+
+def test_eviction_by_slots_outside_the_weights_keeps_nothing(ops, workspace):
+    cache = ops.PackedPages.empty(12, 2, 16, 64, DEV)
+    for t in (cache.k_codes, cache.v_codes):
+        t.random_(0, 256)
+    before = [t.clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)]
+    tables, to = torch.arange(8, dtype=torch.int32, device=DEV).view(4, 2), i32(8, 9, 10, 11)[:, None].contiguous()
+    around, kept_around = torch.rand(9, 2, 30, device=DEV), torch.full((9, 2, 8), 5.0, device=DEV)
+    kept = torch.full((4, 2, 8), 77, dtype=torch.int32, device=DEV)
+    ops.packed_cache_evict(cache, tables, i32(30, 30, 6, 30), around[3:6], cache, to, kept, 8, seq_slot=i32(-1, 3, 1, 2 ** 31 - 1), kept_weights=kept_around[3:6],
+                           workspace=workspace)
+    assert ops.kernel_status() != 0
+    assert (kept[[0, 1, 3]] == -1).all() and kept[2].tolist() == [[0, 1, 2, 3, 4, 5, -1, -1]] * 2
+    assert torch.equal(kept_around[4, :, :6], around[4, :, :6])
+    kept_around[4, :, :6] = 5.0
+    assert (kept_around == 5).all()
+    for a, b in zip(before, (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)):
+        assert torch.equal(a[8:10], b[8:10]) and torch.equal(a[11], b[11])

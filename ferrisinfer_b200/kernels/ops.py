@@ -2491,6 +2491,25 @@ def _weight_rows(weights, kv_heads: int, what: str) -> tuple:
     return slots, rows, slot_stride, head_stride
 
 
+def _rows_meet(a: torch.Tensor, a_rows: int, b: torch.Tensor, b_rows: int) -> bool:
+    """Whether the first ``a_rows`` and ``b_rows`` elements of the rows of two tensors [slots, heads, rows] (the same type, contiguous rows) share memory."""
+    def span(t, rows):
+        at = t.data_ptr() // t.element_size()
+        return at, at + (t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + rows
+
+    (a_from, a_to), (b_from, b_to) = span(a, a_rows), span(b, b_rows)
+    if a_from >= b_to or b_from >= a_to or 0 in a.shape or 0 in b.shape:
+        return False
+    runs = sorted((at + s * t.stride(0) + h * t.stride(1), rows, which) for which, t, at, rows in ((0, a, a_from, a_rows), (1, b, b_from, b_rows))
+                  for s in range(t.shape[0]) for h in range(t.shape[1]))
+    ends = [0, 0]  # of the runs so far
+    for at, rows, which in runs:
+        if at < ends[1 - which]:
+            return True
+        ends[which] = max(ends[which], at + rows)
+    return False
+
+
 def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, block_tables: torch.Tensor, seq_q_start: torch.Tensor,
                      seq_start_row: torch.Tensor, max_q_len: int, max_kv_len: int, num_heads: int, scale: float, window: int = 0,
                      weights: Optional[torch.Tensor] = None, seq_slot: Optional[torch.Tensor] = None, add_weights: bool = True,
@@ -2582,7 +2601,7 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
     [S, blocks]) names in ``kept_pages`` (the same cache will do; none of the pages that are read).  The old pages keep what they
     held, so other requests may share them.  Afterwards the request holds min(seq_rows[s], budget) rows.
     ``kept_rows`` (int32 [S, kv heads, budget]) gets their numbers, -1 behind them; ``kept_weights`` (fp32 [slots, kv heads, >=
-    budget], not the memory of ``weights``) their weights.  ``workspace`` is for scratch that large requests need."""
+    budget], no memory of ``weights``) their weights.  ``workspace`` is for scratch that large requests need."""
     dev = pages.device_index
     try:  # (a tensor of the host has device -1)
         there = dev == kept_pages.device_index == block_tables.get_device() == seq_rows.get_device() == kept_tables.get_device() \
@@ -2615,7 +2634,7 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
         kslots, krows, kslot_stride, khead_stride = _weight_rows(kept_weights, hkv, "eviction: kept weights")
         if krows < budget or kslots < (slots if seq_slot is not None else S):
             raise KernelError(f"eviction: kept weights {tuple(kept_weights.shape)} for {budget} rows of {S} requests")
-        if kept_weights.data_ptr() == weights.data_ptr():
+        if _rows_meet(weights, rows, kept_weights, budget):
             raise KernelError("eviction: kept weights need memory of their own")
         kept = (kept_weights.data_ptr(), kslot_stride, khead_stride)
     if S == 0 or rows == 0 or block_tables.shape[1] == 0 or kept_tables.shape[1] == 0:

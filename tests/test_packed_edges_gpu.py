@@ -127,3 +127,25 @@ def test_eviction_by_slots_outside_the_weights_keeps_nothing(ops, workspace):
     assert (kept_around == 5).all()
     for a, b in zip(before, (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)):
         assert torch.equal(a[8:10], b[8:10]) and torch.equal(a[11], b[11])
+
+
+def test_kept_weights_share_no_memory_with_the_weights(ops, workspace):
+    from ferrisinfer_b200.errors import KernelError
+
+    cache = ops.PackedPages.empty(8, 2, 16, 64, DEV)
+    memory = torch.rand(2, 2, 2, 40, device=DEV)
+    kept_rows = torch.zeros(2, 2, 8, dtype=torch.int32, device=DEV)
+    call = lambda w, kept: ops.packed_cache_evict(cache, i32(0, 1, 2, 3).view(2, 2), i32(30, 20), w, cache, i32(4, 5).view(2, 1), kept_rows, 8,
+                                                  kept_weights=kept, workspace=workspace)
+    flat = memory.view(-1)
+    for w, kept in ((memory[:, :, 0], memory[:, :, 0]), (memory[:, :, 0], memory[:, :, 0, 5:]), (memory[:, :, 0, 5:], memory[:, :, 0]),
+                    (memory[:, :, 0], memory.flatten(2)[:, :, 39:50]), (flat[:160].view(2, 2, 40), flat[159:159 + 160].view(2, 2, 40)),
+                    (flat[100:260].view(2, 2, 40), flat[:124].as_strided((2, 2, 8), (100, 10, 1)))):
+        with pytest.raises(KernelError):
+            call(w, kept)
+    # rows between one another's, and one behind the other
+    for w, kept in ((memory[:, :, 0], memory[:, :, 1]), (memory[:, :, 1], memory[:, :, 0]), (flat[:160].view(2, 2, 40), flat[160:].view(2, 2, 40)),
+                    (memory[:, :, 0, 8:], memory[:, :, 0, :8])):
+        old = w.clone()
+        call(w, kept)
+        assert torch.equal(w, old) and all(torch.equal(kept[s, h, :8], old[s, h][kept_rows[s, h].long()]) for s in range(2) for h in range(2))

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
                                                                             int kept_head_stride, int budget, int keep_first, int keep_last,
                                                                             int max_rows, int held, int slots, int* status) {
-    extern __shared__ uint32_t keys[];  // [held]
+    extern __shared__ __align__(16) uint32_t keys[];  // [held], read four at a time
     __shared__ uint32_t hist[4][EVICT_COPIES][256], total[256];
     __shared__ int greater[EVICT_WARPS], equal[EVICT_WARPS], counts[2];
     pdl_launch_dependents();

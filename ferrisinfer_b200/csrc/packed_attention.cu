@@ -1108,9 +1108,11 @@ FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
     p.q = a->q, p.out = a->out, p.ldq = a->ldq, p.ldo = a->ldo;
     p.q_aligned = ((uintptr_t)a->q & 15) == 0 && (long long)a->ldq * (a->dtype == FERRIS_BF16 ? 2 : 4) % 16 == 0;
     p.out_aligned = ((uintptr_t)a->out & 15) == 0 && (long long)a->ldo * (a->dtype == FERRIS_BF16 ? 2 : 4) % 16 == 0;
+    p.scale = a->scale * LOG2E;
+    if (!isfinite(p.scale)) FERRIS_REFUSE("packed attention: scale %g", (double)a->scale);
     p.few = plan.few;
     p.tables = a->tables, p.width = a->width, p.q_start = a->q_start, p.start_row = a->start_row;
-    p.seqs = a->seqs, p.heads = a->heads, p.group = a->heads / a->kv_heads, p.window = a->window, p.scale = a->scale * LOG2E;
+    p.seqs = a->seqs, p.heads = a->heads, p.group = a->heads / a->kv_heads, p.window = a->window;
     p.lse = plan.lse_floats ? a->scratch : nullptr, p.parts = a->scratch + plan.lse_floats;
     p.scores = plan.score_floats ? a->scratch + plan.lse_floats + plan.part_floats : nullptr;
     p.splits = plan.splits, p.tokens = a->tokens;

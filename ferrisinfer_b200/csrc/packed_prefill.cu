@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(256) packed_queries_kernel(const PackedAttenti
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = (int)(__float_as_uint(top) >> 23);
-        const float factor = top > 0.0f && e < 255 ? __uint_as_float((uint32_t)min(267 - e, 253) << 23) : 1.0f;
+        // (a negative scale goes into the queries, so that what makes a product a score is never below nought)
+        const float factor = copysignf(top > 0.0f && e < 255 ? __uint_as_float((uint32_t)min(267 - e, 253) << 23) : 1.0f, p.scale);
         unsigned char* tile = l.queries + (index * 2 + rr / ROWS) * Shape<D>::OPERAND;
         float own = 0.0f;  // the sum of group c
 #pragma unroll
@@ -597,7 +598,9 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                 __syncwarp();
                 tcgen05_fence_after();
                 const int key0 = (job.first + i) * BLOCK;
-                const float unit = qs * info.k_unit;
+                // Above nought: rows that are not seen stand as minus infinity, which times nought would be NaN.  A product below the
+                // normal range (small queries beside keys of nought, a scale of nought) makes scores of nought all the same.
+                const float unit = fmaxf(qs * info.k_unit, FLT_MIN);
                 const bool whole = key0 >= lo && key0 + BLOCK <= hi && (info.there[0] & info.there[1] & info.there[2] & info.there[3]) == 0xffffffffu;
                 if (info.any_bad)  // (rare) which of this row's outputs a value that is not finite reaches
                     for (int k = 0; k < BLOCK; ++k)
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) top = fmaxf(top, fmaxf(__uint_as_float(sc[c]), __uint_as_float(sc[c + 1])));
                 }
-                top *= unit;  // (never below zero; 0 x infinity, of a query row of noughts, is no maximum)
+                top *= unit;
                 const bool moved = !first && v_now != v_unit;  // (the same for all rows)
                 if (__any_sync(0xffffffffu, top > m + 8.0f) || moved) {
                     const float now = top > m + 8.0f ? top : m;

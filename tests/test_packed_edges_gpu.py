@@ -149,3 +149,37 @@ def test_kept_weights_share_no_memory_with_the_weights(ops, workspace):
         old = w.clone()
         call(w, kept)
         assert torch.equal(w, old) and all(torch.equal(kept[s, h, :8], old[s, h][kept_rows[s, h].long()]) for s in range(2) for h in range(2))
+
+
+# --------------------------------------------------------------------------------------------- scores of prompts
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths, empty", [([(150, 200)], (0, 128)), ([(40, 300), (150, 0)], (128, 256))])
+def test_small_queries_and_a_block_of_rows_without_keys(ops, workspace, dtype, D, lengths, empty):
+    """A block of 128 rows that has no page, or whose keys are all nought, beside queries of 1e-4 and less: numbers all the same."""
+    step = make_step(3, lengths, 6, 2, D, 16, dtype)
+    for small in (1e-4, 1e-20, 0.0):
+        less = with_queries(step, lambda q: q * small)
+        cache, tables = [t.clone() for t in less[0]], less[1].clone()
+        pages = tables[0, empty[0] // 16:empty[1] // 16].long()
+        for t in cache[:2]:
+            t[pages] = 0  # scale, least and codes of the keys
+        attend_and_compare(ops, workspace, (cache, *less[1:]), lengths, 6, 2, D, 16)
+        tables[0, empty[0] // 16:empty[1] // 16] = -1
+        attend_and_compare(ops, workspace, (less[0], tables, *less[2:]), lengths, 6, 2, D, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("lengths", [[(150, 200), (1, 90)], [(1, 40), (1, 300)]])
+def test_a_scale_that_is_nought_or_negative(ops, workspace, dtype, scale, lengths):
+    for D in (64, 128):
+        attend_and_compare(ops, workspace, make_step(4, lengths, 6, 2, D, 16, dtype), lengths, 6, 2, D, 16, scale=scale)
+
+
+def test_a_scale_that_is_no_number_is_refused(ops, workspace):
+    from ferrisinfer_b200.errors import KernelError
+
+    for scale in (math.nan, math.inf, 3e38):
+        with pytest.raises(KernelError):
+            attend_and_compare(ops, workspace, make_step(4, [(1, 40)], 6, 2, 64, 16, torch.bfloat16), [(1, 40)], 6, 2, 64, 16, scale=scale)

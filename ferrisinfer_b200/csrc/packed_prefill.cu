@@ -759,7 +759,8 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                 float v[32] = {};
                 for (int i = job.begin_part; i <= job.last_part; ++i) {
                     const float mi = __ldcg(at(i) + D * 256), f = exp2_fast(mi - m) * share;
-                    if (mi == -FLT_MAX) continue;  // nothing that the row sees: a part that was not written
+                    // nothing that the row sees: a part that was not written (scores of NaN alone leave the maximum there too, not the sum)
+                    if (mi == -FLT_MAX && __ldcg(at(i) + (D + 1) * 256) == 0.0f) continue;
 #pragma unroll
                     for (int c = 0; c < 32; ++c) v[c] += f * __ldcg(at(i) + (size_t)(32 * h + c) * 256);
                 }

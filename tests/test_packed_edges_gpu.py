@@ -183,3 +183,15 @@ def test_a_scale_that_is_no_number_is_refused(ops, workspace):
     for scale in (math.nan, math.inf, 3e38):
         with pytest.raises(KernelError):
             attend_and_compare(ops, workspace, make_step(4, [(1, 40)], 6, 2, 64, 16, torch.bfloat16), [(1, 40)], 6, 2, 64, 16, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[(300, 3000)], [(40, 0)], [(90, 700), (1, 2000)]])
+def test_queries_that_are_not_numbers(ops, workspace, dtype, D, lengths):
+    """NaN in a query is NaN in its output, however many blocks share the row's cached rows."""
+    def spoil(q):
+        q[5, 3], q[17, 4 * D + 1] = math.nan, math.nan
+        return q
+
+    attend_and_compare(ops, workspace, with_queries(make_step(5, lengths, 6, 2, D, 16, dtype), spoil), lengths, 6, 2, D, 16)

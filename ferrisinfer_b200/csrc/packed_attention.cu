@@ -983,6 +983,7 @@ Plan make_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int t
         q.prefill = 1;
         q.few = group <= 8 ? 8 : group <= 16 ? 16 : 0;
         q.here = seqs > 1 && q.few > 0;
+        if (!q.here) q.few = 0;  // (the tensor cores' kernel takes every request: max_q only bounds what they bring)
         q.prompts = packed_prefill_plan(head_dim, seqs, kv_heads, group, tokens, max_q, max_kv);
         q.prompt_floats = fours((q.prompts.bytes + 3) / 4);
         rows = q.few;

@@ -195,3 +195,12 @@ def test_queries_that_are_not_numbers(ops, workspace, dtype, D, lengths):
         return q
 
     attend_and_compare(ops, workspace, with_queries(make_step(5, lengths, 6, 2, D, 16, dtype), spoil), lengths, 6, 2, D, 16)
+
+
+# --------------------------------------------------------------------------------------------- bounds that are not tight
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, D, n", [(28, 4, 128, 1), (14, 2, 64, 1), (6, 2, 64, 2), (12, 1, 128, 1), (24, 1, 64, 1)])
+@pytest.mark.parametrize("max_q", [17, 512])
+def test_a_most_of_queries_that_no_request_reaches(ops, workspace, dtype, heads, kv_heads, D, n, max_q):
+    for lengths in ([(n, 90)], [(n, 90), (1, 300)]):
+        attend_and_compare(ops, workspace, make_step(7, lengths, heads, kv_heads, D, 16, dtype), lengths, heads, kv_heads, D, 16, max_q=max_q)

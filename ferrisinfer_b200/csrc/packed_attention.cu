@@ -1098,7 +1098,8 @@ FERRIS_API int ferris_packed_attention(const FerrisPackedAttention* a) {
                a->head_dim};
     if (const char* why = packed_cache_refusal(p.cache)) FERRIS_REFUSE("%s", why);
     if (a->heads <= 0 || a->heads % a->kv_heads) FERRIS_REFUSE("packed attention: %d heads over %d kv heads", a->heads, a->kv_heads);
-    if (a->window < 0 || a->width <= 0) FERRIS_REFUSE("packed attention: window %d, %d blocks", a->window, a->width);
+    if (a->window < 0 || a->width <= 0 || a->max_kv <= 0)
+        FERRIS_REFUSE("packed attention: window %d, %d blocks, at most %d rows", a->window, a->width, a->max_kv);
     if (a->seqs <= 0 || a->tokens <= 0 || a->max_q <= 0) return FERRIS_OK;
     if ((long long)a->width * a->page_size > 0x7fffffff - 16 * WARPS * STAGE) FERRIS_REFUSE("packed attention: %d blocks of %d rows", a->width, a->page_size);
     const Plan plan = make_plan(a->dtype, a->head_dim, a->seqs, a->kv_heads, a->heads / a->kv_heads, a->tokens, a->max_q, a->max_kv, a->weights != nullptr);

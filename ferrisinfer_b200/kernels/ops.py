@@ -2460,8 +2460,11 @@ def _packed_rows(k, v, slot_mapping, pages: PackedPages, what: str) -> int:
         raise KernelError(f"{what}: dtype {dtype} is not supported (float32 or bfloat16)")
     if T == 1:
         ldk, ldv = max(ldk, width), max(ldv, width)
-    _PACKED_ROWS.pack_into(_packed_buffer, 0, k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), *pages._args, _current_stream(), _DT[dtype],
-                           ldk, ldv, pages.pages, pages.kv_heads, pages.page_size, pages.head_dim, T)
+    try:
+        _PACKED_ROWS.pack_into(_packed_buffer, 0, k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), *pages._args, _current_stream(), _DT[dtype],
+                               ldk, ldv, pages.pages, pages.kv_heads, pages.page_size, pages.head_dim, T)
+    except struct.error as e:
+        raise KernelError(f"{what}: a stride or size beyond 32 bits ({e})") from None
     return T
 
 
@@ -2564,7 +2567,8 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
         w = (weights.data_ptr(), 0 if seq_slot is None else seq_slot.data_ptr(), slot_stride, head_stride, rows, slots)
     if T == 0 or S == 0 or max_q_len == 0:
         return
-    if table_shape[1] == 0:
+    max_q_len, max_kv_len = min(max_q_len, T), min(max_kv_len, table_shape[1] * pages.page_size)  # (launches and scratch go by them)
+    if max_kv_len == 0:  # nobody sees anything
         out.zero_()
         return
     if workspace is None:
@@ -2573,11 +2577,14 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
     scratch, counters, launches = _packed_attention_plan(dt, D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, 0 if weights is None else 1, dev)
     if T == 1:
         ldq, ldo = max(ldq, cols), max(ldo, cols)
-    _PACKED_ATTENTION.pack_into(
-        _packed_buffer, 0, q.data_ptr(), out.data_ptr(), *pages._args, block_tables.data_ptr(), seq_q_start.data_ptr(), seq_start_row.data_ptr(),
-        workspace.address("packed_attention", scratch, torch.float32), workspace.address("packed_attention_counters", counters, torch.int32, True),
-        w[0], w[1], _current_stream(), w[2], ldq, ldo, dt, pages.pages, hkv, pages.page_size, D, table_shape[1], S, T, num_heads, max_q_len,
-        max_kv_len, window, w[3], w[4], 1 if add_weights else 0, w[5], scale)
+    try:
+        _PACKED_ATTENTION.pack_into(
+            _packed_buffer, 0, q.data_ptr(), out.data_ptr(), *pages._args, block_tables.data_ptr(), seq_q_start.data_ptr(), seq_start_row.data_ptr(),
+            workspace.address("packed_attention", scratch, torch.float32), workspace.address("packed_attention_counters", counters, torch.int32, True),
+            w[0], w[1], _current_stream(), w[2], ldq, ldo, dt, pages.pages, hkv, pages.page_size, D, table_shape[1], S, T, num_heads, max_q_len,
+            max_kv_len, min(window, 0x7fffffff), w[3], w[4], 1 if add_weights else 0, w[5], scale)
+    except (struct.error, OverflowError) as e:
+        raise KernelError(f"packed attention: a stride, size or scale beyond 32 bits ({e})") from None
     _check(_packed_lib().ferris_packed_attention(_packed_buffer_at), "packed attention", launches)
 
 
@@ -2640,9 +2647,12 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
     if S == 0 or rows == 0 or block_tables.shape[1] == 0 or kept_tables.shape[1] == 0:
         kept_rows.fill_(-1)
         return
-    _PACKED_EVICT.pack_into(
-        _packed_buffer, 0, *pages._args, *kept_pages._args, block_tables.data_ptr(), kept_tables.data_ptr(), seq_rows.data_ptr(),
-        0 if seq_slot is None else seq_slot.data_ptr(), weights.data_ptr(), kept_rows.data_ptr(), kept[0], _current_stream(), slot_stride, kept[1],
-        pages.pages, pages.page_size, kept_pages.pages, kept_pages.page_size, hkv, pages.head_dim, block_tables.shape[1], kept_tables.shape[1],
-        head_stride, rows, kept[2], S, budget, keep_first, keep_last, slots)
+    try:
+        _PACKED_EVICT.pack_into(
+            _packed_buffer, 0, *pages._args, *kept_pages._args, block_tables.data_ptr(), kept_tables.data_ptr(), seq_rows.data_ptr(),
+            0 if seq_slot is None else seq_slot.data_ptr(), weights.data_ptr(), kept_rows.data_ptr(), kept[0], _current_stream(), slot_stride, kept[1],
+            pages.pages, pages.page_size, kept_pages.pages, kept_pages.page_size, hkv, pages.head_dim, block_tables.shape[1], kept_tables.shape[1],
+            head_stride, rows, kept[2], S, budget, keep_first, keep_last, slots)
+    except struct.error as e:
+        raise KernelError(f"eviction: a stride or size beyond 32 bits ({e})") from None
     _check(_packed_lib().ferris_packed_cache_evict(_packed_buffer_at), "eviction", 2)

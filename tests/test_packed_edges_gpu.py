@@ -204,3 +204,37 @@ def test_queries_that_are_not_numbers(ops, workspace, dtype, D, lengths):
 def test_a_most_of_queries_that_no_request_reaches(ops, workspace, dtype, heads, kv_heads, D, n, max_q):
     for lengths in ([(n, 90)], [(n, 90), (1, 300)]):
         attend_and_compare(ops, workspace, make_step(7, lengths, heads, kv_heads, D, 16, dtype), lengths, heads, kv_heads, D, 16, max_q=max_q)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("max_q", [2 ** 30, 2 ** 40])
+def test_a_most_of_queries_beyond_32_bits(ops, workspace, dtype, max_q):
+    for lengths in ([(1, 90)], [(70, 90), (1, 300)]):
+        attend_and_compare(ops, workspace, make_step(7, lengths, 6, 2, 64, 16, dtype), lengths, 6, 2, 64, 16, max_q=max_q)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths", [[(1, 90), (1, 300)], [(70, 30), (1, 300)]])
+def test_a_most_of_rows_that_no_request_reaches(ops, workspace, dtype, lengths):
+    for max_kv in (10 ** 6, 2 ** 31 - 1, 2 ** 40):
+        attend_and_compare(ops, workspace, make_step(8, lengths, 6, 2, 64, 16, dtype), lengths, 6, 2, 64, 16, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [1, 40])
+def test_no_rows_at_all(ops, workspace, dtype, n):
+    """A caller who says that no request has a row: outputs of nought, no weight touched."""
+    cache, tables, q, q_start, start_row, rows = make_step(9, [(n, 20)], 4, 2, 64, 16, dtype)
+    out, weights = torch.full((n, 256), 7.0, dtype=dtype, device=DEV), torch.full((1, 2, 30), 3.0, device=DEV)
+    ops.packed_attention(q, out, packed(ops, cache), tables, q_start, start_row, n, 0, 4, 0.125, weights=weights, workspace=workspace)
+    assert (out == 0).all() and (weights == 3).all()
+
+
+def test_numbers_that_the_library_cannot_take(ops, workspace):
+    from ferrisinfer_b200.errors import KernelError
+
+    lengths = [(1, 90), (1, 300)]
+    step = make_step(8, lengths, 6, 2, 64, 16, torch.bfloat16)
+    attend_and_compare(ops, workspace, step, lengths, 6, 2, 64, 16, window=2 ** 40)  # (a window that holds everything)
+    with pytest.raises(KernelError):
+        attend_and_compare(ops, workspace, step, lengths, 6, 2, 64, 16, scale=1e300)

@@ -909,7 +909,7 @@ __global__ void __launch_bounds__(WARPS * 32) packed_attention_weights_kernel(co
     const int head = blockIdx.y, seq = blockIdx.z, at = (blockIdx.x * WARPS + warp) * STAGE;
     const int t0 = max(p.q_start[seq], 0), n = min(p.q_start[seq + 1], p.tokens) - t0, count = n * p.group, start = p.start_row[seq];
     const int limit = p.limit, end = min(min(start + n, limit), p.max_rows), slot = slot_of(p, seq);
-    if (at >= end || count > p.few || slot < 0) return;
+    if (at >= end || n <= 0 || count > p.few || slot < 0) return;
     const int* table = p.tables + (size_t)seq * p.width;
     unsigned char* stage = smem + warp * Stage<W>::BYTES;
     const uint32_t there = Stage<W>::request(p, table, head, at, end, stage, lane);

@@ -2528,7 +2528,8 @@ def packed_attention(q: torch.Tensor, out: torch.Tensor, pages: PackedPages, blo
 
     ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` for request s, row s without it; below 0: the request has
     none): every cached row's weight in the softmax, summed over the request's queries and the query heads of the kv head, is
-    added to it; the rows that came with this step (and with ``add_weights`` False all of them) are set instead."""
+    added to it; the rows that came with this step (and with ``add_weights`` False all of them) are set instead.  A request
+    without queries keeps its weights."""
     dev, D, hkv = pages.device_index, pages.head_dim, pages.kv_heads
     try:  # (a tensor of the host has device -1)
         there = dev == q.get_device() == out.get_device() == block_tables.get_device() == seq_q_start.get_device() == seq_start_row.get_device()

@@ -238,3 +238,15 @@ def test_numbers_that_the_library_cannot_take(ops, workspace):
     attend_and_compare(ops, workspace, step, lengths, 6, 2, 64, 16, window=2 ** 40)  # (a window that holds everything)
     with pytest.raises(KernelError):
         attend_and_compare(ops, workspace, step, lengths, 6, 2, 64, 16, scale=1e300)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, others", [(6, [(1, 50)]), (6, [(40, 50)]), (6, [(40, 50), (1, 20)]), (40, [(40, 50)]), (40, [(1, 50)])])
+@pytest.mark.parametrize("add", [True, False])
+def test_a_request_without_queries_keeps_its_weights(ops, workspace, dtype, heads, others, add):
+    lengths = [(0, 100), *others]
+    cache, tables, q, q_start, start_row, rows = make_step(10, lengths, heads, 2, 64, 16, dtype)
+    out, weights = torch.empty(q.shape[0], heads * 64, dtype=dtype, device=DEV), torch.full((len(lengths), 2, max(rows)), 3.0, device=DEV)
+    ops.packed_attention(q, out, packed(ops, cache), tables, q_start, start_row, max(n for n, _ in lengths), max(rows), heads, 0.125,
+                         weights=weights, add_weights=add, workspace=workspace)
+    assert (weights[0] == 3).all() and (weights[1, :, :50] != 3).all()

@@ -10,7 +10,7 @@
 // word of eight codes becomes its sixteen bytes with 13 instructions; in the order in which they come out of the word, which the
 // queries' columns and the outputs' follow.
 //   S = Q K^T    tcgen05.mma 128 x 128 into tensor memory, fp32
-//   P = 2^(S - m) read by a thread a row, written back over S as fp16: the A operand of
+//   P = 2^(S - m + 7) read by a thread a row, written back over S as fp16: the A operand of
 //   O += P V     tcgen05.mma 128 x D, accumulated in tensor memory over all blocks.
 // The maximum m of a row is left behind by up to 2^8: O is scaled (read and written by its warps) only when a score exceeds
 // that, which after the first blocks of a row is rare.  While the softmax warps of one tile work, the tensor cores work for the other.
@@ -26,6 +26,9 @@ constexpr int SOFTMAX = 8, CONVERT = 4, THREADS = (SOFTMAX + CONVERT + 1) * 32;
 constexpr int EXTRA = 4096;  // sixteen further columns of an operand: 128 rows x 32 bytes
 constexpr int INFOS = 4;
 constexpr int TABLE = 1024;  // most pairs of tiles (of one kv head) whose blocks are dealt out evenly
+// Weights are formed 2^7 times too great, as are their sums: at most 2^15 then, and eleven bits in fp16 down to 2^-21 of the maximum (2^-14
+// without it: thousands of rows of a weight of e^-15 of the greatest came out off by 0.026 of what they add up to).
+constexpr float RAISE = 7.0f;
 constexpr int LEAST_PIECE = 4, RUN = 16;  // blocks: fewest of a piece; from which on a CTA may go on with the next pair
 
 template <int D>
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                     }
                 }
                 v_unit = v_now;
-                const float minus = -m;
+                const float minus = RAISE - m;
                 float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
                 for (int h = 0; h < 4; ++h) {
@@ -734,7 +737,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
             }
             tcgen05_fence_before();
             if (!part) {
-                if (valid) my_lse[0] = sum == 0.0f ? -INFINITY : -(m + log2f(sum));
+                if (valid) my_lse[0] = sum == 0.0f ? -INFINITY : -(m - RAISE + log2f(sum));
                 continue;
             }
             part[(size_t)D * 256] = m;
@@ -766,7 +769,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_prefill_kernel(const Packed
                 }
                 store(h, v);
             }
-            my_lse[0] = sum == 0.0f ? -INFINITY : -(m + log2f(sum));
+            my_lse[0] = sum == 0.0f ? -INFINITY : -(m - RAISE + log2f(sum));
         }
     } else if (warp < SOFTMAX + CONVERT) {
         // ------------------------------------------------------------------ operands: a thread a cached row of each block

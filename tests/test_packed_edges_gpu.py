@@ -250,3 +250,17 @@ def test_a_request_without_queries_keeps_its_weights(ops, workspace, dtype, head
     ops.packed_attention(q, out, packed(ops, cache), tables, q_start, start_row, max(n for n, _ in lengths), max(rows), heads, 0.125,
                          weights=weights, add_weights=add, workspace=workspace)
     assert (weights[0] == 3).all() and (weights[1, :, :50] != 3).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("queries", [1, 40])
+def test_many_small_weights_beside_a_great_one(ops, workspace, D, queries):
+    """2,000 rows of weight e^-15 and one that takes the rest with a value of nought: what the many say is all there is."""
+    n, gap = 2000, 15.0
+    k, v = torch.zeros(n + queries, 1, D, device=DEV), torch.ones(n + queries, 1, D, device=DEV)
+    k[0], v[0] = 1.0, 0.0
+    cache, table = plain.cache_of(k, v, 16), torch.arange(-(-(n + queries) // 16), dtype=torch.int32, device=DEV)[None].contiguous()
+    q = torch.full((queries, 6 * D), gap / 4, dtype=torch.bfloat16, device=DEV)
+    scale = 4.0 / D  # the first row's score is `gap`, the others' are nought
+    step = (cache, table, q, i32(0, queries), i32(n), [n + queries])
+    attend_and_compare(ops, workspace, step, [(queries, n)], 6, 1, D, 16, scale=scale)

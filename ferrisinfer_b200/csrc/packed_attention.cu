@@ -10,8 +10,11 @@
 // least, so that what the sums hold is of the size of the result (unsigned codes add up to something that least nearly cancels:
 // over 32,768 rows the accumulators' rounding alone came to 0.0015 of the output).  What meets the codes is scaled by powers of two into the
 // range of fp16: a query row by its greatest element (bf16 rows then lose nothing that 32 bits would keep; 32-bit rows go in
-// two parts, 22 bits), p scale by the greatest scale that the warp has met, in eleven bits for bf16 rows, twice eleven for
-// 32-bit ones.  (In bf16's eight bits the outputs were off by 0.0025 to 0.005 of their norm, 0.0016 of which is their own rounding;
+// two parts, 22 bits), p scale of bf16 rows by the greatest scale that the warp has met, in eleven bits (fewer from 2^-20 of
+// that scale on).  p scale of 32-bit rows goes in three parts of bf16, 24 bits whatever the scales' range, against codes in
+// bf16 (two parts of fp16, whose steps end at 2^-24, left a group of values 2^-20 the size of another no more bits than a bf16
+// row has; six requests of up to 1,534 rows, 12 / 2 heads of 128, 12.8 us with those, 12.5 with these).
+// (In bf16's eight bits the outputs were off by 0.0025 to 0.005 of their norm, 0.0016 of which is their own rounding;
 // codes as fp16 numbers below the normal range need no subtraction, but the tensor cores align their products as if they
 // were large: 3e-5 of a 32-bit output.)
 // Bound by its instructions, about 1,250 for 32 cached rows of a warp at D = 128: 64 requests of up to 4,097 rows (28 / 4 heads of 128,
@@ -38,6 +41,11 @@ __device__ __forceinline__ void mma_f16_16816_first(float (&c)[4], const uint32_
         "{%10, %10, %10, %10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void mma_bf16_16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    c[0] = c[1] = c[2] = c[3] = 0.0f;
+    mma_bf16_16816(c, a, b0, b1);
 }
 
 // 16 (or 8, or 4) bytes global -> shared without registers; `live` false: zeros, and nothing is read.
@@ -307,7 +315,8 @@ struct Segment {
 template <typename T, int D, int NT>
 __device__ __forceinline__ void attend_segment(const PackedAttention& p, const Segment<NT>& seg, unsigned char* smem) {
     using Plan = RowsPlan<D, NT>;
-    constexpr int W = D / 32, NP = sizeof(T) == 4 ? 2 : 1, STAGES = Plan::STAGES;
+    constexpr int W = D / 32, NP = sizeof(T) == 4 ? 2 : 1, STAGES = Plan::STAGES;  // NP: parts of a query row
+    constexpr bool FULL = NP > 1;                                                   // weights times scales in 24 bits
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const int head = seg.head, t0 = seg.t0, count = seg.count, first = seg.first, base = seg.base, end = seg.end;
     const int* table = p.tables + (size_t)seg.seq * p.width;
@@ -460,7 +469,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
             float top = 0.0f;
 #pragma unroll
             for (int j = 0; j < W; ++j) top = fmaxf(top, fmaxf(packed_scale(vs[0][j]), packed_scale(vs[1][j])));
-            if (__any_sync(0xffffffffu, top > v_top)) {
+            if (!FULL && __any_sync(0xffffffffu, top > v_top)) {
                 top = warp_max(top);  // the next power of two, between 2^-120 and 2^127
                 const uint32_t e = min(max((__float_as_uint(top) >> 23) + 1, 7u), 254u);
                 const float now = __uint_as_float(e << 23), f = v_top / now;
@@ -495,8 +504,14 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
                 const float l0 = fmaf(8.0f, packed_scale(vs[0][j]), packed_least(vs[0][j])), l1 = fmaf(8.0f, packed_scale(vs[1][j]), packed_least(vs[1][j]));
                 const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
                 uint32_t a0[4], a1[4];
-                code_pairs<8>(__byte_perm(word[0][j / 2], word[1][j / 2], sel), a0);
-                code_pairs<8>(__byte_perm(word[2][j / 2], word[3][j / 2], sel), a1);
+                const uint32_t w0 = __byte_perm(word[0][j / 2], word[1][j / 2], sel), w1 = __byte_perm(word[2][j / 2], word[3][j / 2], sel);
+                if constexpr (FULL) {
+                    code_pairs_bf16<8>(w0, a0);
+                    code_pairs_bf16<8>(w1, a1);
+                } else {
+                    code_pairs<8>(w0, a0);
+                    code_pairs<8>(w1, a1);
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const float(&pr)[4] = s[h][n];
@@ -505,31 +520,34 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
                     float w[4] = {pr[0] * s0, pr[1] * s0, pr[2] * s1, pr[3] * s1};
                     // 32-bit rows: the tensor cores' sums are of sixteen rows each and are added up in rounded fp32 (theirs are cut off:
                     // over 2,600 rows of a warp 5e-5 of the output)
-                    float fresh[2][4];
+                    if constexpr (FULL) {
+                        float fresh[2][4];
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) {
-                        const uint32_t x0 = pack_f16(w[0], w[1]), x1 = pack_f16(w[2], w[3]);
-                        if (i + 1 < NP) {
-                            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&x0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&x1));
-                            w[0] -= f0.x, w[1] -= f0.y, w[2] -= f1.x, w[3] -= f1.y;
-                        }
-                        const uint32_t b0 = movmatrix_trans(x0), b1 = movmatrix_trans(x1);
+                        for (int i = 0; i < 3; ++i) {
+                            const uint32_t x0 = pack_bf16(w[0], w[1]), x1 = pack_bf16(w[2], w[3]);
+                            w[0] -= __uint_as_float(x0 << 16), w[1] -= __uint_as_float(x0 & 0xffff0000u);
+                            w[2] -= __uint_as_float(x1 << 16), w[3] -= __uint_as_float(x1 & 0xffff0000u);
+                            const uint32_t b0 = movmatrix_trans(x0), b1 = movmatrix_trans(x1);
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            const uint32_t a[4] = {a0[2 * t], a0[2 * t + 1], a1[2 * t], a1[2 * t + 1]};
-                            if (NP == 1)
-                                mma_f16_16816(o[n][j][t], a, b0, b1);
-                            else if (i == 0)
-                                mma_f16_16816_first(fresh[t], a, b0, b1);
-                            else
-                                mma_f16_16816(fresh[t], a, b0, b1);
+                            for (int t = 0; t < 2; ++t) {
+                                const uint32_t a[4] = {a0[2 * t], a0[2 * t + 1], a1[2 * t], a1[2 * t + 1]};
+                                if (i == 0)
+                                    mma_bf16_16816_first(fresh[t], a, b0, b1);
+                                else
+                                    mma_bf16_16816(fresh[t], a, b0, b1);
+                            }
                         }
-                    }
-                    if (NP > 1) {
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) o[n][j][t][i] += fresh[t][i];
+                    } else {
+                        const uint32_t b0 = movmatrix_trans(pack_f16(w[0], w[1])), b1 = movmatrix_trans(pack_f16(w[2], w[3]));
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const uint32_t a[4] = {a0[2 * t], a0[2 * t + 1], a1[2 * t], a1[2 * t + 1]};
+                            mma_f16_16816(o[n][j][t], a, b0, b1);
+                        }
                     }
                 }
             }
@@ -559,7 +577,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const float low = low_o[n][j][u], unit = 0.015625f * v_top;  // the weights were 2^6 / v_top times the true ones
+                const float low = low_o[n][j][u], unit = FULL ? 1.0f : 0.015625f * v_top;  // the weights of bf16 rows were 2^6 / v_top times the true ones
                 float4 v = make_float4(fmaf(o[n][j][0][u], unit, low), fmaf(o[n][j][0][u + 2], unit, low), fmaf(o[n][j][1][u], unit, low),
                                        fmaf(o[n][j][1][u + 2], unit, low));
                 if (bad[n] >> (j + 8 * u) & 1) v = make_float4(NAN, NAN, NAN, NAN);

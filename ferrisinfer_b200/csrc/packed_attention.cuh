@@ -92,6 +92,17 @@ __device__ __forceinline__ void code_pairs(uint32_t word, uint32_t (&pair)[4]) {
     }
 }
 
+// The same in bf16, whose eight bits hold 128 + code.
+template <int OFF>
+__device__ __forceinline__ void code_pairs_bf16(uint32_t word, uint32_t (&pair)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = (word >> (4 * i) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(128.0f + OFF));
+        pair[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
 // Steps with more query rows of a request than `few`, for bf16 rows and heads of 64 and 128 (packed_prefill.cu).
 struct PrefillPlan {
     int pairs, grid, sms;

@@ -264,3 +264,21 @@ def test_many_small_weights_beside_a_great_one(ops, workspace, D, queries):
     scale = 4.0 / D  # the first row's score is `gap`, the others' are nought
     step = (cache, table, q, i32(0, queries), i32(n), [n + queries])
     attend_and_compare(ops, workspace, step, [(queries, n)], 6, 1, D, 16, scale=scale)
+
+
+# --------------------------------------------------------------------------------------------- values of all sizes
+@pytest.mark.parametrize("heads, kv_heads, D", [(4, 2, 64), (6, 1, 128), (12, 1, 64), (2, 1, 96), (2, 1, 256)])
+@pytest.mark.parametrize("small", [2.0 ** -8, 2.0 ** -16, 2.0 ** -40])
+def test_32_bit_rows_keep_their_bits_beside_greater_values(ops, workspace, heads, kv_heads, D, small):
+    """The second group of a head is `small` times the first, and one row is as many times greater than all others in every group, with
+    a key that no query looks for: its share is nothing."""
+    lengths = [(1, 700), (3, 90), (1, 40)]
+    cache, tables, *rest = make_step(6, lengths, heads, kv_heads, D, 16, torch.float32)
+    cache[3][..., 1, :] *= small
+    scale = 0.05 * D ** -0.5
+    attend_and_compare(ops, workspace, (cache, tables, *rest), lengths, heads, kv_heads, D, 16, scale=scale)
+    page = int(tables[0, 1])
+    cache[3][page, :, 7] /= small
+    rest[0].abs_()
+    cache[1][page, :, 7] = torch.tensor([0.0, -400.0], device=DEV)  # (scale, least): a score more than a hundred below the others'
+    attend_and_compare(ops, workspace, (cache, tables, *rest), lengths, heads, kv_heads, D, 16, scale=scale, far=[(0, 23)])

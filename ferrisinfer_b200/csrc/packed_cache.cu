@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(256) packed_read_kernel(T* k, T* v, const Rows
 // ---------------------------------------------------------------------------------------------
 // evict: of the n rows of a request and kv head, `budget` stay: the first `keep_first`, the last
 // `keep_last`, and of the others those of the greatest weight, the lower row first among equals.
-// The order of floats as unsigned keys; NaN counts as greater than every number, -0 as 0.
+// A row that has no page is not there and never stays.
+// The order of floats as unsigned keys; NaN counts as greater than every number, -0 as 0; no row's key is 0.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t weight_key(float w, int row, int n, int keep_first, int keep_last) {
     if (row < keep_first || row >= n - keep_last) return 0xffffffffu;
@@ -235,10 +236,11 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
                                                                             const int* __restrict__ seq_rows, const int* __restrict__ seq_slot,
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
                                                                             int kept_head_stride, int budget, int keep_first, int keep_last,
-                                                                            int max_rows, int held, int slots, int* status) {
+                                                                            int max_rows, int held, int slots, const int* __restrict__ tables,
+                                                                            int width, DivideBy page, int page_size, int pages, int* status) {
     extern __shared__ __align__(16) uint32_t keys[];  // [held], read four at a time
     __shared__ uint32_t hist[4][EVICT_COPIES][256], total[256];
-    __shared__ int greater[EVICT_WARPS], equal[EVICT_WARPS], counts[2];
+    __shared__ int greater[EVICT_WARPS], equal[EVICT_WARPS], has_page[EVICT_WARPS], counts[2];
     pdl_launch_dependents();
     pdl_wait();
     const int s = blockIdx.y, h = blockIdx.x, heads = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -249,9 +251,26 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     const float* w = weights + slot * slot_stride + (long long)h * head_stride;
     int* rows = kept_rows + ((size_t)s * heads + h) * budget;
     float* kw = kept_weights ? kept_weights + slot * kept_slot_stride + (long long)h * kept_head_stride : nullptr;
-    const int stay = min(n, budget);
+    // the rows that have a page (every block counts all of them)
+    const int* table = tables + (size_t)s * width;
+    int there = 0;
+    for (int b = tid, all = n > 0 ? (int)page.quotient(n - 1) + 1 : 0; b < all; b += EVICT_THREADS) {
+        const int at = b < width ? table[b] : -1;
+        if (at >= pages) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 106);
+        if (at >= 0 && at < pages) there += min(page_size, n - b * page_size);
+    }
+    there = __reduce_add_sync(0xffffffffu, there);
+    if (lane == 0) has_page[warp] = there;
+    __syncthreads();
+    there = __reduce_add_sync(0xffffffffu, lane < EVICT_WARPS ? has_page[lane] : 0);
+    const bool whole = there == n;
+    const auto is_there = [&](int r) {
+        const int b = (int)page.quotient(r);
+        return whole || (b < width && table[b] >= 0 && table[b] < pages);
+    };
+    const int stay = min(there, budget);
     for (int i = stay + rank * EVICT_THREADS + tid; i < budget; i += blocks * EVICT_THREADS) rows[i] = -1;
-    if (n <= budget) {  // (the whole cluster)
+    if (whole && n <= budget) {  // (the whole cluster)
         for (int i = rank * EVICT_THREADS + tid; i < n; i += blocks * EVICT_THREADS) {
             rows[i] = i;
             if (kw) kw[i] = w[i];
@@ -262,23 +281,24 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     const int run = (n + 32 * EVICT_WARPS * blocks - 1) / (32 * EVICT_WARPS * blocks) * 32, begin = min(rank * EVICT_WARPS * run, n),
               end = min(begin + EVICT_WARPS * run, n);
     const bool hold = end - begin <= held;
-    // keys of four rows from r (a multiple of four) on; 0, which no weight has, behind the end
+    // keys of four rows from r (a multiple of four) on; 0 for rows that are not there, and behind the end
     const auto keys_of = [&](int r) {
         if (hold) return *reinterpret_cast<const uint4*>(keys + (r - begin));
         uint32_t k[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = r + i < end ? weight_key(w[r + i], r + i, n, keep_first, keep_last) : 0u;
+        for (int i = 0; i < 4; ++i) k[i] = r + i < end && is_there(r + i) ? weight_key(w[r + i], r + i, n, keep_first, keep_last) : 0u;
         return make_uint4(k[0], k[1], k[2], k[3]);
     };
     for (int i = tid; i < 4 * EVICT_COPIES * 256; i += EVICT_THREADS) (&hist[0][0][0])[i] = 0;
     if (hold)
 #pragma unroll 8
-        for (int r = begin + tid; r < (end + 3) / 4 * 4; r += EVICT_THREADS) keys[r - begin] = r < end ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
+        for (int r = begin + tid; r < (end + 3) / 4 * 4; r += EVICT_THREADS) 
+            keys[r - begin] = r < end && is_there(r) ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
     __syncthreads();
     uint32_t prefix = 0;
-    int want = budget;  // how many of the rows that share the prefix stay
+    int want = there > budget ? budget : 0;  // how many of the rows that share the prefix stay (0: all that have a key do)
 #pragma unroll 1
-    for (int byte = 0; byte < 4; ++byte) {
+    for (int byte = 0; byte < 4 && there > budget; ++byte) {
         const int shift = 24 - 8 * byte;
         const uint32_t mask = byte == 0 ? 0u : 0xffffffffu << (shift + 8);
         uint32_t* mine_of = hist[byte][lane % EVICT_COPIES];
@@ -562,6 +582,7 @@ FERRIS_API int ferris_packed_cache_evict(const FerrisPackedEvict* a) {
     cudaError_t e = ferris_launch_cluster(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,
                                           a->weights, a->slot_stride, a->head_stride, a->seq_rows, a->seq_slot, a->kept_rows, a->kept_weights,
                                           a->kept_slot_stride, a->kept_head_stride, budget, keep_first, keep_last, max_rows, held, a->slots,
+                                          a->from_tables, a->from_width, DivideBy(a->from_page_size), a->from_page_size, a->from_pages,
                                           ferris_status_ptr());
     if (e != cudaSuccess) FERRIS_LAUNCH_CHECK();
     return with_groups(head_dim, [&](auto w) {

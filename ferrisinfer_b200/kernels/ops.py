@@ -2607,7 +2607,8 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
     others, those of the greatest ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` or s; the lower row first among
     equals, NaN before every number; a slot below 0: nothing of the request is kept).  They move, in their order, into rows 0, 1, ... of the pages that ``kept_tables`` (int32
     [S, blocks]) names in ``kept_pages`` (the same cache will do; none of the pages that are read).  The old pages keep what they
-    held, so other requests may share them.  Afterwards the request holds min(seq_rows[s], budget) rows.
+    held, so other requests may share them.  A row without a page is not there to be kept, first and last ones included:
+    afterwards the request holds min(its rows that have a page, budget) rows.
     ``kept_rows`` (int32 [S, kv heads, budget]) gets their numbers, -1 behind them; ``kept_weights`` (fp32 [slots, kv heads, >=
     budget], no memory of ``weights``) their weights.  ``workspace`` is for scratch that large requests need."""
     dev = pages.device_index

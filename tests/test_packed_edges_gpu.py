@@ -282,3 +282,72 @@ def test_32_bit_rows_keep_their_bits_beside_greater_values(ops, workspace, heads
     rest[0].abs_()
     cache[1][page, :, 7] = torch.tensor([0.0, -400.0], device=DEV)  # (scale, least): a score more than a hundred below the others'
     attend_and_compare(ops, workspace, (cache, tables, *rest), lengths, heads, kv_heads, D, 16, scale=scale, far=[(0, 23)])
+
+
+# --------------------------------------------------------------------------------------------- eviction
+def kept_of(weights, there, budget, keep_first, keep_last):
+    """``plain.kept`` where row r stands only if there[r]."""
+    n = len(weights)
+    rows = [r for r in range(n) if there[r]]
+    if len(rows) <= budget:
+        return rows
+
+    def rank(r):
+        if r < keep_first or r >= n - keep_last:
+            return (0, 0.0, r)
+        w = weights[r]
+        return (1, 0.0, r) if math.isnan(w) else (2, -w, r)
+
+    return sorted(sorted(rows, key=rank)[:budget])
+
+
+@pytest.mark.parametrize("rows, budget, first, last, page_size, width", [
+    ([60, 90], 64, 4, 8, 16, 6),        # all that is there stays, or what is there is no more than the budget
+    ([500, 300, 0], 64, 20, 40, 16, 32),
+    ([1500, 260], 1400, 4, 8, 7, 215),  # fewer rows there than the budget, more rows than it
+    ([20000], 700, 100, 300, 16, 1250),  # several blocks to a request
+    ([20000], 19000, 0, 0, 64, 313),
+    ([200, 100], 32, 4, 8, 16, 8),      # a table that ends before the rows do
+])
+@pytest.mark.parametrize("kind", ["spread", "ties", "special"])
+def test_rows_without_a_page_are_not_there_to_be_kept(ops, workspace, rows, budget, first, last, page_size, width, kind):
+    gen = torch.Generator(device=DEV).manual_seed(budget + len(kind))
+    S, most, hkv, D = len(rows), max(rows), 2, 64
+    to_blocks = -(-budget // page_size)
+    pages = S * (width + to_blocks)
+    cache = ops.PackedPages.empty(pages, hkv, page_size, D, DEV)
+    for name in ("k_codes", "v_codes"):
+        getattr(cache, name).random_(0, 256, generator=gen)
+    for name in ("k_scales", "v_scales"):
+        t = getattr(cache, name)
+        t.copy_(torch.randn(t.shape, generator=gen, device=DEV).abs())
+    ids = torch.randperm(pages, generator=gen, device=DEV).to(torch.int32)
+    tables, to_tables = ids[:S * width].view(S, width).clone(), ids[S * width:].view(S, to_blocks).contiguous()
+    tables[torch.rand(S, width, generator=gen, device=DEV) < 0.3] = -1
+    tables[0, 0], tables[0, 1] = -1, int(ids[1])
+    w = torch.rand(S, hkv, most, generator=gen, device=DEV)
+    if kind == "ties":
+        w = (w * 4).floor()
+    elif kind == "special":
+        w[w < 0.05] = math.nan
+        w[(w > 0.05) & (w < 0.1)] = math.inf
+        w[(w > 0.1) & (w < 0.2)] = -math.inf
+    kept_rows, kept_w = torch.full((S, hkv, budget), 77, dtype=torch.int32, device=DEV), torch.full((S, hkv, budget + 2), 5.0, device=DEV)
+    tensors = (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)
+    old = [t.clone() for t in tensors]
+    ops.packed_cache_evict(cache, tables, i32(*rows), w, cache, to_tables, kept_rows, budget, keep_first=first, keep_last=last, kept_weights=kept_w,
+                           workspace=workspace)
+    for s, n in enumerate(rows):
+        table = tables[s].tolist() + [-1] * (n // page_size + 1)
+        there = [table[r // page_size] >= 0 for r in range(n)]
+        for h in range(hkv):
+            want = kept_of(w[s, h, :n].tolist(), there, budget, first, last)
+            assert kept_rows[s, h].tolist() == want + [-1] * (budget - len(want))
+            src, at = torch.tensor(want, dtype=torch.long, device=DEV), torch.arange(len(want), device=DEV)
+            assert torch.equal(kept_w[s, h, :len(want)].nan_to_num(-3), w[s, h][src].nan_to_num(-3))
+            assert (kept_w[s, h, len(want):] == 5).all()
+            for a, b in zip(old, tensors):
+                assert torch.equal(a[tables[s].long()[src // page_size], h, src % page_size], b[to_tables[s].long()[at // page_size], h, at % page_size])
+    for a, b in zip(old, tensors):  # what was read stays as it was
+        live = tables[tables >= 0].long()
+        assert torch.equal(a[live], b[live])

@@ -251,11 +251,20 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     const float* w = weights + slot * slot_stride + (long long)h * head_stride;
     int* rows = kept_rows + ((size_t)s * heads + h) * budget;
     float* kw = kept_weights ? kept_weights + slot * kept_slot_stride + (long long)h * kept_head_stride : nullptr;
-    // the rows that have a page (every block counts all of them)
+    // this block's rows: runs of whole 32 rows for each of its warps
+    const int run = (n + 32 * EVICT_WARPS * blocks - 1) / (32 * EVICT_WARPS * blocks) * 32, begin = min(rank * EVICT_WARPS * run, n),
+              end = min(begin + EVICT_WARPS * run, n);
+    const bool hold = end - begin <= held;
+    for (int i = tid; i < 4 * EVICT_COPIES * 256; i += EVICT_THREADS) (&hist[0][0][0])[i] = 0;
     const int* table = tables + (size_t)s * width;
+    const int all = n > 0 ? (int)page.quotient(n - 1) + 1 : 0, first_page = tid < min(all, width) ? table[tid] : -1;
+    if (hold && n > budget)  // (as if all rows were there: which are is counted meanwhile)
+#pragma unroll 8
+        for (int r = begin + tid; r < (end + 3) / 4 * 4; r += EVICT_THREADS) keys[r - begin] = r < end ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
+    // the rows that have a page (every block counts all of them)
     int there = 0;
-    for (int b = tid, all = n > 0 ? (int)page.quotient(n - 1) + 1 : 0; b < all; b += EVICT_THREADS) {
-        const int at = b < width ? table[b] : -1;
+    for (int b = tid; b < all; b += EVICT_THREADS) {
+        const int at = b == tid ? first_page : b < width ? table[b] : -1;
         if (at >= pages) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 106);
         if (at >= 0 && at < pages) there += min(page_size, n - b * page_size);
     }
@@ -277,10 +286,11 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
         }
         return;
     }
-    // this block's rows: runs of whole 32 rows for each of its warps
-    const int run = (n + 32 * EVICT_WARPS * blocks - 1) / (32 * EVICT_WARPS * blocks) * 32, begin = min(rank * EVICT_WARPS * run, n),
-              end = min(begin + EVICT_WARPS * run, n);
-    const bool hold = end - begin <= held;
+    if (hold && !whole) {
+        for (int r = begin + tid; r < (end + 3) / 4 * 4; r += EVICT_THREADS)
+            keys[r - begin] = r < end && is_there(r) ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
+        __syncthreads();
+    }
     // keys of four rows from r (a multiple of four) on; 0 for rows that are not there, and behind the end
     const auto keys_of = [&](int r) {
         if (hold) return *reinterpret_cast<const uint4*>(keys + (r - begin));
@@ -289,12 +299,6 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
         for (int i = 0; i < 4; ++i) k[i] = r + i < end && is_there(r + i) ? weight_key(w[r + i], r + i, n, keep_first, keep_last) : 0u;
         return make_uint4(k[0], k[1], k[2], k[3]);
     };
-    for (int i = tid; i < 4 * EVICT_COPIES * 256; i += EVICT_THREADS) (&hist[0][0][0])[i] = 0;
-    if (hold)
-#pragma unroll 8
-        for (int r = begin + tid; r < (end + 3) / 4 * 4; r += EVICT_THREADS) 
-            keys[r - begin] = r < end && is_there(r) ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
-    __syncthreads();
     uint32_t prefix = 0;
     int want = there > budget ? budget : 0;  // how many of the rows that share the prefix stay (0: all that have a key do)
 #pragma unroll 1

@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     const int blocks = gridDim.z, rank = blockIdx.z;
     const int slot = seq_slot ? seq_slot[s] : s;
     if (slot >= slots) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 105);
+    if (slot >= 0 && seq_rows[s] > max_rows) ferris_report(status, FERRIS_STATUS_BAD_INDEX, 107);  // (rows that no weight speaks for)
     const int n = slot < 0 || slot >= slots ? 0 : min(max(seq_rows[s], 0), max_rows);  // (without weights: no rows; nothing of w is then read)
     const float* w = weights + slot * slot_stride + (long long)h * head_stride;
     int* rows = kept_rows + ((size_t)s * heads + h) * budget;

@@ -2603,7 +2603,7 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
                        workspace=None):
     """Cut every request down to ``budget`` rows of the packed cache, each kv head to its own.
 
-    Of the ``seq_rows[s]`` rows (int32 [S]) of request s there stay its first ``keep_first``, its last ``keep_last`` and, of the
+    Of the ``seq_rows[s]`` rows (int32 [S]; no more than ``weights`` has, which is reported) of request s there stay its first ``keep_first``, its last ``keep_last`` and, of the
     others, those of the greatest ``weights`` (fp32 [slots, kv heads, rows], row ``seq_slot[s]`` or s; the lower row first among
     equals, NaN before every number; a slot below 0: nothing of the request is kept).  They move, in their order, into rows 0, 1, ... of the pages that ``kept_tables`` (int32
     [S, blocks]) names in ``kept_pages`` (the same cache will do; none of the pages that are read).  The old pages keep what they

@@ -351,3 +351,11 @@ def test_rows_without_a_page_are_not_there_to_be_kept(ops, workspace, rows, budg
     for a, b in zip(old, tensors):  # what was read stays as it was
         live = tables[tables >= 0].long()
         assert torch.equal(a[live], b[live])
+
+
+def test_eviction_says_when_weights_end_before_the_rows(ops, workspace):
+    cache = ops.PackedPages.empty(8, 1, 16, 64, DEV)
+    kept_rows = torch.empty(1, 1, 10, dtype=torch.int32, device=DEV)
+    ops.packed_cache_evict(cache, i32(0, 1, 2, 3)[None].contiguous(), i32(60), torch.rand(1, 1, 50, device=DEV), cache, i32(4)[None].contiguous(),
+                           kept_rows, 10, workspace=workspace)
+    assert ops.kernel_status() != 0

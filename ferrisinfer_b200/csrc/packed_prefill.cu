@@ -16,6 +16,8 @@
 // that, which after the first blocks of a row is rare.  While the softmax warps of one tile work, the tensor cores work for the other.
 // Bound by the chain of softmax, product and scores of a tile (the weights stand where the next scores go): 512 tokens after 32,768 rows
 // (28 / 4 heads of 128) about 300 us in a sequence of calls, 800 TFLOP/s; tensor pipe 35 % busy, issue slots 49 %.
+#include <algorithm>
+
 #include "packed_attention.cuh"
 
 namespace {
@@ -57,23 +59,26 @@ struct Layout {
     long long bytes;
 };
 
+// Places for parts (Deal::place): pieces leave one a CTA, runs two, but those are dealt out to no more CTAs than there are SMs.
+int part_places(int grid, int sms) { return std::max(grid, 2 * std::min(grid, sms)); }
+
 template <typename F>
-void for_scratch(int D, int pairs, int kv_heads, int seqs, int grid, F&& take) {
+void for_scratch(int D, int pairs, int kv_heads, int seqs, int places, F&& take) {
     const long long operand = (long long)(D / 64) * 16384 + EXTRA;
     take(0, (long long)pairs * kv_heads * 2 * operand);
     take(1, (long long)pairs * kv_heads * 256 * 4);
     take(2, (long long)pairs * sizeof(Pair));
     take(3, (long long)(pairs + 4) * 4);
-    take(4, 2ll * grid * (D + 2) * 256 * 4);
+    take(4, (long long)places * (D + 2) * 256 * 4);
     take(5, (long long)pairs * kv_heads * 256 * 4);
     take(6, (long long)seqs * 4);
 }
 
-Layout make_layout(void* base, int D, int pairs, int kv_heads, int seqs, int grid) {
+Layout make_layout(void* base, int D, int pairs, int kv_heads, int seqs, int places) {
     Layout l = {};
     unsigned char* at = (unsigned char*)base;
     long long used = 0;
-    for_scratch(D, pairs, kv_heads, seqs, grid, [&](int what, long long bytes) {
+    for_scratch(D, pairs, kv_heads, seqs, places, [&](int what, long long bytes) {
         unsigned char* p = at + used;
         if (what == 0) l.queries = p;
         if (what == 1) l.scales = (float*)p;
@@ -1139,7 +1144,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) packed_prefill_weights_kernel(co
 
 template <int D>
 int prefill(const PackedAttention& p, const PrefillPlan& plan, int max_kv, void* scratch, int* counters, cudaStream_t st) {
-    const Layout l = make_layout(scratch, D, plan.pairs, p.cache.kv_heads, p.seqs, plan.pairs > TABLE ? 0 : plan.grid);
+    const Layout l = make_layout(scratch, D, plan.pairs, p.cache.kv_heads, p.seqs, plan.pairs > TABLE ? 0 : part_places(plan.grid, plan.sms));
     cudaError_t e = ferris_launch(packed_queries_kernel<D>, dim3(plan.pairs + 1, p.cache.kv_heads), dim3(256), 0, st, p, l, plan.sms);
     if (e != cudaSuccess) return (int)e;
     auto kernel = packed_prefill_kernel<D>;
@@ -1164,7 +1169,7 @@ PrefillPlan packed_prefill_plan(int head_dim, int seqs, int kv_heads, int group,
     q.grid = q.pairs > TABLE ? q.pairs * kv_heads : q.sms + q.pairs * kv_heads;
     const long long blocks = (long long)q.pairs * kv_heads * (max_kv / BLOCK + 2);
     if (q.pairs <= TABLE && q.grid > blocks) q.grid = (int)blocks;
-    q.bytes = make_layout(nullptr, head_dim, q.pairs, kv_heads, seqs, q.pairs > TABLE ? 0 : q.grid).bytes;
+    q.bytes = make_layout(nullptr, head_dim, q.pairs, kv_heads, seqs, q.pairs > TABLE ? 0 : part_places(q.grid, q.sms)).bytes;
     q.counters = q.pairs > TABLE ? 0 : (long long)q.pairs * kv_heads;
     return q;
 }

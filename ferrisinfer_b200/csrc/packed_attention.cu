@@ -766,7 +766,7 @@ __global__ void __launch_bounds__(WARPS * 32, D * NT <= 128 && sizeof(T) == 2 ? 
         const int head = seg.head;
         seg.seq = s, seg.t0 = max(p.q_start[s], 0), seg.count = (min(p.q_start[s + 1], p.tokens) - seg.t0) * p.group;
         if (p.even) seg.count = min(seg.count, 8 * NT);  // (what the caller says no request exceeds)
-        if (seg.first >= seg.count) return;
+        if (seg.first >= seg.count || (!p.even && seg.count > p.few)) return;  // (more rows than `few`: the other kernel's)
         seg.rows.set(p, seg.first, seg.count, p.start_row[s], limit, c);
         const int floor = seg.rows.least / STAGE * STAGE;
         if (!p.even) {
@@ -1038,7 +1038,8 @@ int attend_rows(const PackedAttention& p, const Plan& q, int max_q, cudaStream_t
     auto kernel = packed_attention_rows_kernel<T, D, NT>;
     constexpr size_t smem = RowsPlan<D, NT>::SMEM;
     if (const int e = ferris_allow_dynamic_smem((const void*)kernel, smem)) return e;
-    const dim3 grid = q.even ? dim3(q.blocks) : dim3((max_q * p.group + 8 * NT - 1) / (8 * NT), p.cache.kv_heads, p.seqs * p.splits);
+    const long long rows = (long long)max_q * p.group < p.few ? (long long)max_q * p.group : p.few;  // of a request that this kernel takes
+    const dim3 grid = q.even ? dim3(q.blocks) : dim3((unsigned)((rows + 8 * NT - 1) / (8 * NT)), p.cache.kv_heads, p.seqs * p.splits);
     return (int)ferris_launch(kernel, grid, dim3(WARPS * 32), smem, st, p);
 }
 

@@ -359,3 +359,68 @@ def test_eviction_says_when_weights_end_before_the_rows(ops, workspace):
     ops.packed_cache_evict(cache, i32(0, 1, 2, 3)[None].contiguous(), i32(60), torch.rand(1, 1, 50, device=DEV), cache, i32(4)[None].contiguous(),
                            kept_rows, 10, workspace=workspace)
     assert ops.kernel_status() != 0
+
+
+# --------------------------------------------------------------------------------------------- many requests, long ones
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_requests_than_are_dealt_out_evenly_and_a_prompt(ops, workspace, D):
+    lengths = [(1, i % 3) for i in range(1100)] + [(70, 30)] + [(1, 5)] * 3
+    attend_and_compare(ops, workspace, make_step(11, lengths, 4, 2, D, 16, torch.bfloat16), lengths, 4, 2, D, 16)
+
+
+def test_more_pairs_of_tiles_than_are_dealt_out_evenly(ops, workspace):
+    lengths = [(3, i % 4) for i in range(1030)]  # 18 query rows of a kv head each, a pair of tiles of their own
+    attend_and_compare(ops, workspace, make_step(12, lengths, 6, 1, 64, 16, torch.bfloat16), lengths, 6, 1, 64, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_scores_than_are_kept(ops, workspace, dtype):
+    """Tables so wide that the scores of a step would fill more than 512 MB: the weights come from scores formed again."""
+    lengths = [(1, 100 + i) for i in range(40)]
+    cache, tables, *rest = make_step(13, lengths, 8, 4, 64, 16, dtype)
+    wide = torch.full((len(lengths), 8192), -1, dtype=torch.int32, device=DEV)
+    wide[:, :tables.shape[1]] = tables
+    q, q_start, start_row, rows = rest
+    out, weights = torch.empty(40, 512, dtype=dtype, device=DEV), torch.zeros(40, 4, 131072, device=DEV)
+    ops.packed_attention(q, out, packed(ops, cache), wide, q_start, start_row, 1, 131072, 8, 0.125, weights=weights, workspace=workspace)
+    other, same = torch.empty_like(out), torch.zeros(40, 4, max(rows), device=DEV)
+    ops.packed_attention(q, other, packed(ops, cache), tables, q_start, start_row, 1, max(rows), 8, 0.125, weights=same, workspace=workspace)
+    # The same scores and sums, cut into other pieces: 24-bit sums of a few hundred weights, then the type's rounding.
+    assert (out.double() - other.double()).abs().max() <= other.double().abs().max() * (2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -18)
+    assert ((weights[:, :, :max(rows)] - same).abs() <= same * 2.0 ** -18).all() and (weights[:, :, max(rows):] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_runs_of_prompts_are_cut_and_joined(ops, workspace, D):
+    """Portions after so many rows that a CTA goes on from one pair of tiles to the next, against a call for each alone."""
+    lengths = [(130, 40000), (200, 30000), (64, 65000), (3, 9000)]
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    rows, ps = [n + s for n, s in lengths], 64
+    blocks = [-(-r // ps) for r in rows]
+    cache = []
+    for _ in range(2):
+        cache.append(torch.randint(0, 256, (sum(blocks), 1, ps, D // 2), generator=gen, device=DEV, dtype=torch.uint8))
+        scale = 0.05 + 0.2 * torch.rand(sum(blocks), 1, ps, D // 32, generator=gen, device=DEV)
+        cache.append(torch.stack([scale, -7.5 * scale], -1).to(torch.bfloat16))
+    ids = torch.randperm(sum(blocks), generator=gen, device=DEV).to(torch.int32)
+    tables = torch.full((len(lengths), max(blocks)), -1, dtype=torch.int32, device=DEV)
+    starts = [0]
+    for i, b in enumerate(blocks):
+        tables[i, :b] = ids[sum(blocks[:i]):sum(blocks[:i + 1])]
+        starts.append(starts[-1] + lengths[i][0])
+    q = torch.randn(starts[-1], 7 * D, generator=gen, device=DEV).bfloat16()
+    out, weights = torch.empty_like(q), torch.zeros(len(lengths), 1, max(rows), device=DEV)
+    pages = packed(ops, cache)
+    ops.packed_attention(q, out, pages, tables, i32(*starts), i32(*(s for _, s in lengths)), 200, max(rows), 7, D ** -0.5, weights=weights,
+                         workspace=workspace)
+    for i, (n, start) in enumerate(lengths):
+        k, v, _ = plain.request_rows(cache, tables[i], rows[i], ps)
+        mine = q[starts[i]:starts[i + 1]].double().view(n, 7, D).transpose(0, 1)
+        s = (mine @ k[:, 0].t()) * D ** -0.5
+        s.masked_fill_(torch.arange(rows[i], device=DEV) > start + torch.arange(n, device=DEV)[:, None], -math.inf)
+        p = torch.softmax(s, -1)
+        want, got = (p @ v[:, 0]).transpose(0, 1), out[starts[i]:starts[i + 1]].double().view(n, 7, D)
+        # bf16 rows: the result's rounding (2^-9 on average) and weights and values in eleven bits
+        assert (got - want).norm() <= 2.0 ** -8 * want.norm()
+        w = p.sum((0, 1))
+        assert ((weights[i, 0, :rows[i]].double() - w).abs() <= w * 2.0 ** -14).all()

@@ -78,8 +78,8 @@ inline cudaError_t ferris_launch(Kernel kernel, dim3 grid, dim3 block, size_t sm
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// The same with the CTAs of each (x, y) grouped along z into clusters of `cluster_z`.
-template <typename Kernel, typename... Args>
+// The same with the CTAs of each (x, y) grouped along z into clusters of `cluster_z`; EARLY false: not before the kernel in front has ended.
+template <bool EARLY = true, typename Kernel, typename... Args>
 inline cudaError_t ferris_launch_cluster(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                                          unsigned cluster_z, Args... args) {
     cudaLaunchConfig_t cfg = {};
@@ -95,7 +95,7 @@ inline cudaError_t ferris_launch_cluster(Kernel kernel, dim3 grid, dim3 block, s
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = ferris_pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = EARLY && ferris_pdl_enabled() ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 

@@ -230,8 +230,8 @@ constexpr int EVICT_COPIES = 4;        // of a histogram: lanes that meet in a b
 // read again each time).  The budget-th greatest key by its four bytes, most significant first: a histogram of 256 bins
 // each, added up over the cluster; then the kept rows in order, every warp its own run of rows.  What bounds it is the
 // chain of short passes and barriers, so a lane takes four rows at a time, each on its own.  16 requests of up to 32,768 rows and
-// 4 heads: 32 us (one row at a time, lanes that share a bin found by votes, 44 to 47; all of the eviction with the read-back was
-// no faster with `match.any`); 5,000 rows of one request 16 us.
+// 4 heads: 29 us (keys formed one after the other, 34; besides one row at a time, lanes that share a bin found by votes, 44 to 47;
+// all of the eviction with the read-back was no faster with `match.any`); 5,000 rows of one request 15 us.
 __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(const float* weights, long long slot_stride, int head_stride,
                                                                             const int* __restrict__ seq_rows, const int* __restrict__ seq_slot,
                                                                             int* kept_rows, float* kept_weights, long long kept_slot_stride,
@@ -241,7 +241,6 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     extern __shared__ __align__(16) uint32_t keys[];  // [held], read four at a time
     __shared__ uint32_t hist[4][EVICT_COPIES][256], total[256];
     __shared__ int greater[EVICT_WARPS], equal[EVICT_WARPS], has_page[EVICT_WARPS], counts[2];
-    pdl_wait();  // (dependents come in as blocks end: let in beside these passes, the blocks that move rows made 16 requests' eviction 112 us, not 100)
     const int s = blockIdx.y, h = blockIdx.x, heads = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int blocks = gridDim.z, rank = blockIdx.z;
     const int slot = seq_slot ? seq_slot[s] : s;
@@ -259,8 +258,16 @@ __global__ void __launch_bounds__(EVICT_THREADS) packed_evict_select_kernel(cons
     const int* table = tables + (size_t)s * width;
     const int all = n > 0 ? (int)page.quotient(n - 1) + 1 : 0, first_page = tid < min(all, width) ? table[tid] : -1;
     if (hold && n > budget)  // (as if all rows were there: which are is counted meanwhile)
-#pragma unroll 8
-        for (int r = begin + tid; r < (end + 3) / 4 * 4; r += EVICT_THREADS) keys[r - begin] = r < end ? weight_key(w[r], r, n, keep_first, keep_last) : 0u;
+        for (int r0 = begin + tid; r0 < (end + 3) / 4 * 4; r0 += 8 * EVICT_THREADS) {
+            float v[8];  // all on their way before the first is used
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = r0 + i * EVICT_THREADS < end ? w[r0 + i * EVICT_THREADS] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i * EVICT_THREADS;
+                if (r < (end + 3) / 4 * 4) keys[r - begin] = r < end ? weight_key(v[i], r, n, keep_first, keep_last) : 0u;
+            }
+        }
     // the rows that have a page (every block counts all of them)
     int there = 0;
     for (int b = tid; b < all; b += EVICT_THREADS) {
@@ -583,7 +590,9 @@ FERRIS_API int ferris_packed_cache_evict(const FerrisPackedEvict* a) {
     while (blocks < 8 && (long long)blocks * 8192 < max_rows) blocks *= 2;
     const int each = ((max_rows + EVICT_THREADS * blocks - 1) / (EVICT_THREADS * blocks)) * EVICT_THREADS, held = each < EVICT_HELD ? each : EVICT_HELD;
     if (const int r = ferris_allow_dynamic_smem((const void*)packed_evict_select_kernel, (size_t)held * 4)) return r;
-    cudaError_t e = ferris_launch_cluster(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,
+    // In its turn of the stream, and its dependents not before its blocks end: blocks of this kernel beside those of the one in front, or
+    // blocks that move rows beside these, cost more than the launch that they hide (16 requests with the read-back 108 us, not 94).
+    cudaError_t e = ferris_launch_cluster<false>(packed_evict_select_kernel, dim3(kv_heads, seqs, blocks), dim3(EVICT_THREADS), (size_t)held * 4, st, blocks,
                                           a->weights, a->slot_stride, a->head_stride, a->seq_rows, a->seq_slot, a->kept_rows, a->kept_weights,
                                           a->kept_slot_stride, a->kept_head_stride, budget, keep_first, keep_last, max_rows, held, a->slots,
                                           a->from_tables, a->from_width, DivideBy(a->from_page_size), a->from_page_size, a->from_pages,

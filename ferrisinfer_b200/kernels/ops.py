@@ -2496,15 +2496,8 @@ def _weight_rows(weights, kv_heads: int, what: str) -> tuple:
 
 def _rows_meet(a: torch.Tensor, a_rows: int, b: torch.Tensor, b_rows: int) -> bool:
     """Whether the first ``a_rows`` and ``b_rows`` elements of the rows of two tensors [slots, heads, rows] (the same type, contiguous rows) share memory."""
-    def span(t, rows):
-        at = t.data_ptr() // t.element_size()
-        return at, at + (t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + rows
-
-    (a_from, a_to), (b_from, b_to) = span(a, a_rows), span(b, b_rows)
-    if a_from >= b_to or b_from >= a_to or 0 in a.shape or 0 in b.shape:
-        return False
-    runs = sorted((at + s * t.stride(0) + h * t.stride(1), rows, which) for which, t, at, rows in ((0, a, a_from, a_rows), (1, b, b_from, b_rows))
-                  for s in range(t.shape[0]) for h in range(t.shape[1]))
+    runs = sorted((t.data_ptr() // t.element_size() + s * t.stride(0) + h * t.stride(1), rows, which)
+                  for which, t, rows in ((0, a, a_rows), (1, b, b_rows)) if rows for s in range(t.shape[0]) for h in range(t.shape[1]))
     ends = [0, 0]  # of the runs so far
     for at, rows, which in runs:
         if at < ends[1 - which]:
@@ -2643,9 +2636,11 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
         kslots, krows, kslot_stride, khead_stride = _weight_rows(kept_weights, hkv, "eviction: kept weights")
         if krows < budget or kslots < (slots if seq_slot is not None else S):
             raise KernelError(f"eviction: kept weights {tuple(kept_weights.shape)} for {budget} rows of {S} requests")
-        if _rows_meet(weights, rows, kept_weights, budget):
+        at, kept_at = weights.data_ptr(), kept_weights.data_ptr()
+        if (at < kept_at + 4 * ((kslots - 1) * kslot_stride + (hkv - 1) * khead_stride + budget)
+                and kept_at < at + 4 * ((slots - 1) * slot_stride + (hkv - 1) * head_stride + rows) and _rows_meet(weights, rows, kept_weights, budget)):
             raise KernelError("eviction: kept weights need memory of their own")
-        kept = (kept_weights.data_ptr(), kslot_stride, khead_stride)
+        kept = (kept_at, kslot_stride, khead_stride)
     if S == 0 or rows == 0 or block_tables.shape[1] == 0 or kept_tables.shape[1] == 0:
         kept_rows.fill_(-1)
         return

@@ -4,8 +4,7 @@
 
 One layer's queries, keys and values are drawn at random, some keys so that many queries look for them.  The requests bring their
 prompts in portions, then single tokens; the cache keeps the rows that attention weighs most.  Printed at the end: rows and bytes
-held against a cache that keeps everything in bf16, how many of the sought keys stayed, and how far the last outputs are
-from attention over everything.
+held against a cache that keeps everything in bf16, and how far the last outputs are from attention over everything.
 """
 
 import argparse

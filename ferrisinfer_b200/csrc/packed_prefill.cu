@@ -15,7 +15,8 @@
 // The maximum m of a row is left behind by up to 2^8: O is scaled (read and written by its warps) only when a score exceeds
 // that, which after the first blocks of a row is rare.  While the softmax warps of one tile work, the tensor cores work for the other.
 // Bound by the chain of softmax, product and scores of a tile (the weights stand where the next scores go): 512 tokens after 32,768 rows
-// (28 / 4 heads of 128) about 300 us in a sequence of calls, 800 TFLOP/s; tensor pipe 35 % busy, issue slots 49 %.
+// (28 / 4 heads of 128) about 310 us in a sequence of calls, 770 TFLOP/s (345 by itself, caches cold); tensor pipe 35 % busy, issue
+// slots 48 %.
 #include <algorithm>
 
 #include "packed_attention.cuh"

@@ -2472,7 +2472,7 @@ def packed_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Ten
     """Keys and values [T, kv heads x head size] (bf16 or fp32, rows contiguous: columns of a fused projection are fine) into
     the rows ``slot_mapping`` (int32 [T], page * page_size + offset; below 0: the token is left out) of the packed cache.  Per
     group of 32: least = its minimum rounded down to bf16, scale = bf16((maximum - least) / 15), code = (x - least) / scale
-    rounded to even; a group with NaN or infinity stands as NaN.  Two tokens with one slot leave one of them."""
+    rounded to even; a group with NaN or infinity stands as NaN.  What a slot that two tokens share holds is not said: parts of either."""
     if _packed_rows(k, v, slot_mapping, pages, "packed cache write"):
         _check(_packed_lib().ferris_packed_cache_write(_packed_buffer_at), "packed cache write")
 
@@ -2603,7 +2603,7 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
     held, so other requests may share them.  A row without a page is not there to be kept, first and last ones included:
     afterwards the request holds min(its rows that have a page, budget) rows.
     ``kept_rows`` (int32 [S, kv heads, budget]) gets their numbers, -1 behind them; ``kept_weights`` (fp32 [slots, kv heads, >=
-    budget], no memory of ``weights``) their weights.  ``workspace`` is for scratch that large requests need."""
+    budget], no memory of ``weights``) their weights.  Eviction needs no scratch: ``workspace`` is taken as elsewhere and not used."""
     dev = pages.device_index
     try:  # (a tensor of the host has device -1)
         there = dev == kept_pages.device_index == block_tables.get_device() == seq_rows.get_device() == kept_tables.get_device() \

@@ -10,8 +10,9 @@
 // least, so that what the sums hold is of the size of the result (unsigned codes add up to something that least nearly cancels:
 // over 32,768 rows the accumulators' rounding alone came to 0.0015 of the output).  What meets the codes is scaled by powers of two into the
 // range of fp16: a query row by its greatest element (bf16 rows then lose nothing that 32 bits would keep; 32-bit rows go in
-// two parts, 22 bits), p scale of bf16 rows by the greatest scale that the warp has met, in eleven bits (fewer from 2^-20 of
-// that scale on).  p scale of 32-bit rows goes in three parts of bf16, 24 bits whatever the scales' range, against codes in
+// two parts, 22 bits), p scale of bf16 rows by the greatest scale of its group that the warp has met, in eleven bits (rows whose
+// scale and weight together are below 2^-20 of that scale keep fewer; with one power for all groups, of a group of values 2^-24 the
+// size of another was off by 0.007, of 2^-30 by 0.9).  p scale of 32-bit rows goes in three parts of bf16, 24 bits whatever the scales' range, against codes in
 // bf16 (two parts of fp16, whose steps end at 2^-24, left a group of values 2^-20 the size of another no more bits than a bf16
 // row has; six requests of up to 1,534 rows, 12 / 2 heads of 128, 12.8 us with those, 12.5 with these).
 // (In bf16's eight bits the outputs were off by 0.0025 to 0.005 of their norm, 0.0016 of which is their own rounding;
@@ -342,7 +343,10 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
         for (int u = 0; u < 2; ++u) qs[n][u] = __shfl_sync(0xffffffffu, inv, 4 * (2 * c + u));
     }
     float o[NT][W][2][4] = {}, low_o[NT][W][2] = {}, m[NT][2], l[NT][2] = {};
-    float v_top = 0.0f, v_fit = 1.0f;  // a power of two no scale of values met so far is above, and what brings such scales to 2^6
+    // of each group: a power of two no scale of values met so far is above, and what brings such scales to 2^6
+    float v_top[W], v_fit[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) v_top[j] = 0.0f, v_fit[j] = 1.0f;
     uint32_t bad[NT] = {};             // groups whose output is not finite: bit j of column 2c, bit j + 8 of column 2c + 1
 #pragma unroll
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -FLT_MAX;  // (finite: differences of it are numbers)
@@ -446,6 +450,31 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
                     l[n][i & 1] += e;
                 }
 
+        if constexpr (!FULL) {  // a lane a row: whether any of the stage's scales is above what has been met
+            uint32_t mine[W];
+            load_words<W>(mine, stage + Stage<W>::VS_AT + lane * Stage<W>::S_ROW);
+            bool greater = false;
+#pragma unroll
+            for (int j = 0; j < W; ++j) greater |= packed_scale(mine[j]) > v_top[j];
+            if (__any_sync(0xffffffffu, greater)) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    const float top = warp_max(packed_scale(mine[j]));
+                    if (!(top > v_top[j])) continue;  // (NaN is not)
+                    // the next power of two, between 2^-120 and 2^127
+                    const uint32_t e = min(max((__float_as_uint(top) >> 23) + 1, 7u), 254u);
+                    const float now = __uint_as_float(e << 23), f = v_top[j] / now;
+                    v_top[j] = now;
+                    v_fit[j] = __uint_as_float((260u - e) << 23);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[n][j][t][i] *= f;
+                }
+            }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t vs[2][W];
@@ -467,24 +496,6 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
                             }
                         }
             }
-            float top = 0.0f;
-#pragma unroll
-            for (int j = 0; j < W; ++j) top = fmaxf(top, fmaxf(packed_scale(vs[0][j]), packed_scale(vs[1][j])));
-            if (!FULL && __any_sync(0xffffffffu, top > v_top)) {
-                top = warp_max(top);  // the next power of two, between 2^-120 and 2^127
-                const uint32_t e = min(max((__float_as_uint(top) >> 23) + 1, 7u), 254u);
-                const float now = __uint_as_float(e << 23), f = v_top / now;
-                v_top = now;
-                v_fit = __uint_as_float((260u - e) << 23);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < W; ++j)
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[n][j][t][i] *= f;
-            }
             uint32_t word[4][(W + 1) / 2];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -501,7 +512,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
             }
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const float s0 = packed_scale(vs[0][j]) * v_fit, s1 = packed_scale(vs[1][j]) * v_fit;
+                const float s0 = packed_scale(vs[0][j]) * v_fit[j], s1 = packed_scale(vs[1][j]) * v_fit[j];
                 const float l0 = fmaf(8.0f, packed_scale(vs[0][j]), packed_least(vs[0][j])), l1 = fmaf(8.0f, packed_scale(vs[1][j]), packed_least(vs[1][j]));
                 const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
                 uint32_t a0[4], a1[4];
@@ -578,7 +589,7 @@ __device__ __forceinline__ void attend_segment(const PackedAttention& p, const S
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const float low = low_o[n][j][u], unit = FULL ? 1.0f : 0.015625f * v_top;  // the weights of bf16 rows were 2^6 / v_top times the true ones
+                const float low = low_o[n][j][u], unit = FULL ? 1.0f : 0.015625f * v_top[j];  // the weights of bf16 rows were 2^6 / v_top times the true ones
                 float4 v = make_float4(fmaf(o[n][j][0][u], unit, low), fmaf(o[n][j][0][u + 2], unit, low), fmaf(o[n][j][1][u], unit, low),
                                        fmaf(o[n][j][1][u + 2], unit, low));
                 if (bad[n] >> (j + 8 * u) & 1) v = make_float4(NAN, NAN, NAN, NAN);

@@ -424,3 +424,13 @@ def test_long_runs_of_prompts_are_cut_and_joined(ops, workspace, D):
         assert (got - want).norm() <= 2.0 ** -8 * want.norm()
         w = p.sum((0, 1))
         assert ((weights[i, 0, :rows[i]].double() - w).abs() <= w * 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("heads, kv_heads, D, n", [(4, 2, 64, 3), (6, 1, 128, 1), (12, 1, 64, 1), (2, 1, 96, 4), (2, 1, 256, 8)])
+@pytest.mark.parametrize("small", [2.0 ** -8, 2.0 ** -24, 2.0 ** -40])
+def test_few_bf16_rows_keep_small_groups_beside_great_ones(ops, workspace, heads, kv_heads, D, n, small):
+    """The second group of a head is `small` times the others, in steps that the kernel for few rows takes."""
+    lengths = [(1, 700), (n, 90), (1, 40)]
+    cache, tables, *rest = make_step(15, lengths, heads, kv_heads, D, 16, torch.bfloat16)
+    cache[3][..., 1, :] *= small
+    attend_and_compare(ops, workspace, (cache, tables, *rest), lengths, heads, kv_heads, D, 16, scale=0.05 * D ** -0.5)

@@ -19,8 +19,8 @@
 // codes as fp16 numbers below the normal range need no subtraction, but the tensor cores align their products as if they
 // were large: 3e-5 of a 32-bit output.)
 // Bound by its instructions, about 1,400 for 32 cached rows of a warp at D = 128 with all that is before and behind them, and by their
-// latencies: 64 requests of up to 4,097 rows (28 / 4 heads of 128, scores kept) 62 us, 1.7 TB/s, issue slots 42 % used, ALU pipe 34 %,
-// tensor pipe 8 %; one of 131,072 rows (12 / 2 heads) 25 us and 9.7 for the join of its parts.
+// latencies: 64 requests of up to 4,097 rows (28 / 4 heads of 128, scores kept) 64 us, 1.7 TB/s, issue slots 42 % used, ALU pipe 34 %,
+// tensor pipe 8 %; one of 131,072 rows (12 / 2 heads) 25.5 us and 9.7 for the join of its parts.
 #include "packed_attention.cuh"
 
 namespace {

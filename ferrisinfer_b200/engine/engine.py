@@ -85,7 +85,8 @@ class Engine:
         such pages stay in the cache after the last request that held them has ended (or was preempted), for
         later requests with the same beginning, until a request needs their room.
         ``cache_bits`` 4: keys and values are held in 4 bits, with a scale and a least value for every 32 neighbours of a head (5 bits
-        an element with them: 3.2 times as many tokens as in bf16); for models of plain attention layers.
+        an element with them: 3.2 times as many tokens as in bf16); for models of plain attention layers.  Steps over short contexts take
+        longer than with the cache in bf16.
         ``run_ahead``: queue the next decode step while the GPU still runs the current one (see ``step``)."""
         ops.require_device()
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())

@@ -1,0 +1,309 @@
+// Verification of trees of drafted tokens against the target's probabilities, from given random numbers.
+//
+// At a node x the target's distribution is r / R, at first r = p_x (its row of probabilities) and R = 1.  Its children are tried in
+// their order; child c, drawn from the draft's distribution q_x, is accepted if u_c q_x(t_c) R < r(t_c), that is with the
+// probability min(1, (r(t_c) / R) / q_x(t_c)), and the walk goes on from it.  Refused, it leaves the residual: r <- max(r - R q_x, 0), R <- sum r (where
+// nothing is left, r and R stay).  A draft without probabilities has chosen its tokens for certain: q_x(t_c) = 1, r(t_c) <- 0, R <- R - r(t_c).
+// Where no child is accepted the next token is drawn from r: the first i with sum_{j <= i} r_j > u_root sum_j r_j.  So tokens
+// follow the target's distribution whatever was drafted.  All of it in 64 bits: at a border a rounding would be another token.
+//
+// A cluster of eight blocks takes a request, each an eighth of the vocabulary.  The tree, the random numbers and every node's p and q
+// are fetched at once; each block then walks by itself, all of them the same way, and the blocks meet only where a row has to be gone through: after
+// the refusal of a token that has a q, and for the last draw, whose passes leave the sums of every warp's run of elements, so that the draw goes
+// through one run again.  Sums are added up in one order whatever the timing.
+#include <math.h>
+
+#include "common.cuh"
+#include "sm100.cuh"
+
+namespace {
+
+constexpr int CLUSTER = 8, THREADS = 512, WARPS = THREADS / 32, NODES = 256;
+
+struct VerifyTree {
+    const float* probs;
+    const float* draft;  // or nullptr
+    long long ldp, ldd;
+    const int* tokens;
+    const int* parents;
+    const int* q_start;
+    const float* uniforms;
+    int* out_nodes;
+    int* out_accepted;
+    int* out_token;
+    int seqs, rows, vocab, width;
+    int* status;
+};
+
+__device__ __forceinline__ double ld_peer_shared_f64(uint32_t addr, uint32_t rank) {
+    uint32_t remote;
+    double v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Whatever is no probability counts as none.
+__device__ __forceinline__ float probability(float v) { return v > 0.0f ? v : 0.0f; }
+
+struct Shared {
+    float p[NODES], q[NODES], u[NODES];  // of each node's token in its parent's rows
+    int token[NODES];
+    short parent[NODES];
+    double refused[NODES];   // R of each refusal that left a residual
+    int gone[NODES];         // tokens that were refused without probabilities
+    double part[2][WARPS];   // sums of the warps' runs of the last pass, by the parity of its number
+    double block[2];         // the block's
+};
+
+struct Pass {
+    const float* p;
+    const float* q;
+    int lo, hi;  // the warp's run
+    bool aligned;
+};
+
+// What is left of an element after the refusals so far.
+__device__ __forceinline__ double residual(const Shared& s, int refusals, float p, float q) {
+    double r = (double)probability(p);
+    const double qq = (double)probability(q);
+    for (int k = 0; k < refusals; ++k) r = fmax(__dsub_rn(r, __dmul_rn(s.refused[k], qq)), 0.0);  // (two roundings, as written)
+    return r;
+}
+
+// f(element, what is left of it) for four neighbours from i on.
+template <bool DRAFT>
+__device__ __forceinline__ void four(const Shared& s, const Pass& w, int i, int refusals, int gone, double (&r)[4]) {
+    float p[4] = {}, q[4] = {};
+    if (w.aligned && i + 4 <= w.hi) {
+        const float4 v = *reinterpret_cast<const float4*>(w.p + i);
+        p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
+        if (DRAFT) {
+            const float4 v2 = *reinterpret_cast<const float4*>(w.q + i);
+            q[0] = v2.x, q[1] = v2.y, q[2] = v2.z, q[3] = v2.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k < w.hi) {
+                p[k] = w.p[i + k];
+                if (DRAFT) q[k] = w.q[i + k];
+            }
+    }
+    if (!DRAFT)
+        for (int g = 0; g < gone; ++g) {
+            const unsigned at = (unsigned)(s.gone[g] - i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (at == (unsigned)k) p[k] = 0.0f;
+        }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = DRAFT ? residual(s, refusals, p[k], q[k]) : (double)probability(p[k]);
+}
+
+__device__ __forceinline__ double run_sum(const Shared& s, const Pass& w, int refusals, int gone) {
+    double sum = 0.0, r[4];
+    for (int i = w.lo + 4 * (threadIdx.x & 31); i < w.hi; i += 128) {
+        if (refusals)
+            four<true>(s, w, i, refusals, gone, r);
+        else
+            four<false>(s, w, i, refusals, gone, r);
+        sum += (r[0] + r[1]) + (r[2] + r[3]);
+    }
+    return warp_sum64(sum);
+}
+
+__global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a) {
+    __shared__ Shared s;
+    __shared__ double whole[CLUSTER];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int seq = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int first = min(max(a.q_start[seq], 0), a.rows);
+    int n = min(max(a.q_start[seq + 1], first), a.rows) - first;
+    if (n > NODES) {
+        if (threadIdx.x == 0) ferris_report(a.status, FERRIS_STATUS_BAD_INDEX, 130);
+        n = NODES;
+    }
+    const bool drafted = a.draft != nullptr;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        int up = a.parents[first + i];
+        const int t = a.tokens[first + i];
+        float p = 0.0f, q = 1.0f;
+        if (i && (up >= i || up < -1)) {
+            ferris_report(a.status, FERRIS_STATUS_BAD_INDEX, 131);
+            up = -1;
+        }
+        if (i && up >= 0) {
+            if (t < 0 || t >= a.vocab) {
+                ferris_report(a.status, FERRIS_STATUS_BAD_INDEX, 132);
+                up = -1;  // nobody's child
+            } else {
+                p = probability(a.probs[(first + up) * a.ldp + t]);
+                if (drafted) q = probability(a.draft[(first + up) * a.ldd + t]);
+            }
+        }
+        s.parent[i] = (short)(i ? up : -1), s.token[i] = t, s.p[i] = p, s.q[i] = q, s.u[i] = a.uniforms[first + i];
+    }
+    __syncthreads();
+    // this warp's run of elements: runs begin on four elements, and follow one another over the blocks of the cluster
+    const int per = (((a.vocab + CLUSTER * WARPS - 1) / (CLUSTER * WARPS)) + 3) & ~3;
+    Pass w;
+    w.lo = min(a.vocab, (int)(rank * WARPS + warp) * per), w.hi = min(a.vocab, w.lo + per);
+    int passes = 0;
+    // the sum over the row of what is left, the same in all blocks; the runs' sums stay in s.part, the blocks' in `whole`
+    auto sum_up = [&](int refusals, int gone) {
+        const int b = passes++ & 1;
+        const double mine = run_sum(s, w, refusals, gone);
+        if (lane == 0) s.part[b][warp] = mine;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double t = 0.0;
+            for (int i = 0; i < WARPS; ++i) t += s.part[b][i];
+            s.block[b] = t;
+        }
+        cluster_sync();  // (nobody writes this half again before all have read it: there is a barrier more between)
+        if (threadIdx.x < CLUSTER) whole[threadIdx.x] = ld_peer_shared_f64(smem_u32(&s.block[b]), threadIdx.x);
+        __syncthreads();
+        double t = 0.0;
+        for (int i = 0; i < CLUSTER; ++i) t += whole[i];
+        __syncthreads();
+        return t;
+    };
+    int node = 0, path = 1, refusals = 0, gone = 0;
+    double left = 1.0, total = -1.0;  // total: of the last pass over what is left as it is now, below 0: none
+    if (rank == 0 && threadIdx.x == 0 && n) a.out_nodes[(size_t)seq * a.width] = 0;
+    auto look_at = [&](int x) {
+        w.p = a.probs + (first + x) * a.ldp;
+        w.q = drafted ? a.draft + (first + x) * a.ldd : w.p;
+        w.aligned = (((uintptr_t)w.p | (uintptr_t)w.q) & 15) == 0;
+    };
+    if (n) look_at(0);
+    for (int c = 1; c < n; ++c) {
+        if (s.parent[c] != node || path == a.width) continue;
+        double r;
+        if (drafted)
+            r = residual(s, refusals, s.p[c], s.q[c]);
+        else {
+            r = s.p[c];
+            for (int g = 0; g < gone; ++g)
+                if (s.gone[g] == s.token[c]) r = 0.0;
+        }
+        if ((double)s.u[c] * (drafted ? (double)s.q[c] : 1.0) * left < r) {
+            if (rank == 0 && threadIdx.x == 0) a.out_nodes[(size_t)seq * a.width + path] = c;
+            node = c, ++path, refusals = 0, gone = 0, left = 1.0, total = -1.0;
+            look_at(c);
+            continue;
+        }
+        // (the barrier keeps those who still read the list from those who add to it)
+        __syncthreads();
+        if (drafted) {
+            if (threadIdx.x == 0) s.refused[refusals] = left;
+            __syncthreads();
+            const double t = sum_up(refusals + 1, 0);
+            if (t > 0.0) ++refusals, left = t, total = t;
+            else total = -1.0;  // (the sums of the runs are no longer those of what is left)
+        } else {
+            if (threadIdx.x == 0) s.gone[gone] = s.token[c];
+            ++gone, left -= r;
+            __syncthreads();
+        }
+    }
+    if (n && total < 0.0) total = sum_up(refusals, gone);
+    int token = -1;
+    if (n && total > 0.0) {
+        const int b = (passes - 1) & 1;
+        const double u = (double)s.u[0], aim = u > 0.0 ? u * total : 0.0;
+        // the last block whose elements begin at or below the aim and hold anything; in it the last such run; in it the first element beyond the aim
+        double before = 0.0, at = 0.0;
+        int owner = -1;
+        for (int i = 0; i < CLUSTER; ++i) {
+            if (whole[i] > 0.0 && at <= aim) owner = i, before = at;
+            at += whole[i];
+        }
+        if (owner == (int)rank && warp == 0) {
+            at = before;
+            int run = -1;
+            for (int i = 0; i < WARPS; ++i) {
+                if (s.part[b][i] > 0.0 && at <= aim) run = i, before = at;
+                at += s.part[b][i];
+            }
+            w.lo = min(a.vocab, (int)(rank * WARPS + run) * per), w.hi = min(a.vocab, w.lo + per);
+            int found = -1, last = -1;
+            for (int i0 = w.lo; i0 < w.hi && found < 0; i0 += 128) {
+                const int i = i0 + 4 * lane;
+                double r[4] = {};
+                if (i < w.hi) {
+                    if (refusals)
+                        four<true>(s, w, i, refusals, gone, r);
+                    else
+                        four<false>(s, w, i, refusals, gone, r);
+                }
+                const double mine = (r[0] + r[1]) + (r[2] + r[3]);
+                double upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                double run_at = before + (upto - mine);
+                int hit = -1, any = -1;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    run_at += r[k];
+                    if (r[k] > 0.0) {
+                        any = i + k;
+                        if (hit < 0 && run_at > aim) hit = i + k;
+                    }
+                }
+                const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
+                if (some) last = __shfl_sync(0xffffffffu, any, 31 - __clz(some));
+                if (hits) found = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            if (lane == 0) a.out_token[seq] = found >= 0 ? found : last;
+        }
+    } else if (rank == 0 && threadIdx.x == 0)
+        a.out_token[seq] = token;
+    if (rank == 0) {
+        if (threadIdx.x == 0) a.out_accepted[seq] = n ? path - 1 : 0;
+        for (int i = (n ? path : 0) + threadIdx.x; i < a.width; i += THREADS) a.out_nodes[(size_t)seq * a.width + i] = -1;
+    }
+    cluster_sync();  // nobody leaves while others may read its sums
+}
+
+}  // namespace
+
+// Arguments as ops.verify_tree lays them out.
+struct VerifyTreeArgs {
+    const void *probs, *draft, *tokens, *parents, *q_start, *uniforms, *out_nodes, *out_accepted, *out_token, *stream;
+    long long ldp, ldd;
+    int seqs, rows, vocab, width;
+};
+
+FERRIS_API int ferris_verify_tree(const VerifyTreeArgs* x) {
+    if (x->seqs <= 0) return FERRIS_OK;
+    if (x->rows < 0 || x->vocab <= 0 || x->width <= 0 || x->ldp < x->vocab || (x->draft && x->ldd < x->vocab))
+        FERRIS_REFUSE("%d rows of %d probabilities, paths of %d nodes", x->rows, x->vocab, x->width);
+    VerifyTree a;
+    a.probs = (const float*)x->probs, a.draft = (const float*)x->draft, a.ldp = x->ldp, a.ldd = x->ldd;
+    a.tokens = (const int*)x->tokens, a.parents = (const int*)x->parents, a.q_start = (const int*)x->q_start;
+    a.uniforms = (const float*)x->uniforms;
+    a.out_nodes = (int*)const_cast<void*>(x->out_nodes), a.out_accepted = (int*)const_cast<void*>(x->out_accepted);
+    a.out_token = (int*)const_cast<void*>(x->out_token);
+    a.seqs = x->seqs, a.rows = x->rows, a.vocab = x->vocab, a.width = x->width;
+    a.status = ferris_status_ptr();
+    const cudaError_t e = ferris_launch_cluster(verify_tree_kernel, dim3(x->seqs, 1, CLUSTER), dim3(THREADS), 0, (cudaStream_t)x->stream, CLUSTER, a);
+    if (e != cudaSuccess) {
+        ferris_set_error("%s", cudaGetErrorString(e));
+        return (int)e;
+    }
+    FERRIS_LAUNCH_CHECK();
+}

@@ -53,6 +53,11 @@ _SIGNATURES = {
     "ferris_packed_cache_evict": [_VP],
     "ferris_packed_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
     "ferris_packed_attention": [_VP],
+    "ferris_tree_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _VP],
+    "ferris_tree_attention": [_VP],
+    "ferris_sampling_probs": [_VP, _LL, _VP, _LL, _I, _I, _VP, _VP, _VP, _VP],
+    "ferris_verify_tree": [_VP],
+    "ferris_tree_rows": [_VP],
 }
 _declared = False
 
@@ -2653,3 +2658,252 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
     except struct.error as e:
         raise KernelError(f"eviction: a stride or size beyond 32 bits ({e})") from None
     _check(_packed_lib().ferris_packed_cache_evict(_packed_buffer_at), "eviction", 2)
+
+
+# ------------------------------------------------------------------------------------------
+# steps over trees of drafted tokens
+# ------------------------------------------------------------------------------------------
+TREE_NODES = 256  # most tokens of a request's tree
+
+# Arguments of a call laid out for the library in one go, as for the packed cache.
+_TREE_ATTENTION = struct.Struct("=10Q15if")
+_TREE_ROWS = struct.Struct("=6Q9i")
+_VERIFY_TREE = struct.Struct("=10Q2q4i")
+_tree_buffer = ctypes.create_string_buffer(max(_TREE_ATTENTION.size, _TREE_ROWS.size, _VERIFY_TREE.size))
+_tree_buffer_at = ctypes.addressof(_tree_buffer)
+
+
+def _on_current_device(what: str, *tensors) -> int:
+    """The device that all the tensors are on, which has to be the current one: it is where kernels are launched."""
+    try:  # (a tensor of the host has device -1)
+        devices = {t.get_device() for t in tensors}
+    except AttributeError:
+        devices = {-1}
+    if devices == {-1} or len(devices) != 1:
+        raise KernelError(f"{what}: all tensors must be CUDA tensors on one device (there is no CPU path)")
+    dev = devices.pop()
+    if dev != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the tensors are on cuda:{dev}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return dev
+
+
+def _int32(what: str, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be contiguous and {torch.int32}, found {t.dtype}")
+
+
+def _long_rows(what: str, t: torch.Tensor) -> tuple:
+    """(rows, columns, row stride) of a matrix of fp32 with contiguous rows."""
+    if t.dim() != 2 or t.dtype != torch.float32 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise KernelError(f"{what} must be {torch.float32} and 2-D with contiguous rows, found {t.dtype}, shape {tuple(t.shape)}, strides {t.stride()}")
+    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                   seq_q_start: torch.Tensor, seq_start_row: torch.Tensor, parents: torch.Tensor, max_q_len: int, max_kv_len: int,
+                   num_heads: int, scale: float, window: int = 0, workspace=None):
+    """Attention of a step over trees of drafted tokens (a chain, or a single token, is a tree) over the paged cache, in which their own
+    keys and values already are: node i of request s in row ``seq_start_row[s]`` + i, rotated by its position, seq_start_row[s] + its depth.
+
+    ``q`` [T, >= num_heads x head size] (bf16 or fp32; its first columns, so the rows of a fused projection will do), ``out``
+    [T, num_heads x head size] of the same type; ``k_cache``, ``v_cache`` [pages, kv heads, page size, head size] of the same type, head sizes
+    that are a multiple of 8 up to 256.  Request s brings the rows ``seq_q_start[s]`` .. ``seq_q_start[s + 1] - 1`` (int32 [S + 1]); rows behind
+    the last request's are left as they are.  ``parents`` (int32 [T]): each node's parent, the number of an earlier
+    node of its request, or -1.  A node sees the ``seq_start_row[s]`` (int32 [S]) rows of its request's text, itself and its ancestors;
+    with ``window`` > 0 of these the keys whose position is above its own less the window; and only rows for which ``block_tables`` (int32 [S, blocks])
+    names a page.  What a node does not see has no effect, whatever it holds; a node that sees nothing gives zeros.
+    ``max_q_len`` (at most TREE_NODES), ``max_kv_len``: the most nodes and rows (nodes included) of any request.  Nodes beyond the one are
+    not attended, which is reported (``check_kernel_status``), rows beyond the other are not seen.  A parent that is no earlier node is reported
+    and counts as none."""
+    what = "tree attention"
+    dev = _on_current_device(what, q, out, k_cache, v_cache, block_tables, seq_q_start, seq_start_row, parents)
+    _int32(what, **{"block tables": block_tables, "first query rows": seq_q_start, "rows of the text": seq_start_row, "parents": parents})
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise KernelError(f"{what}: keys {tuple(k_cache.shape)} and values {tuple(v_cache.shape)} must be contiguous [pages, kv heads, page size, head size]")
+    pages, hkv, page_size, D = k_cache.shape
+    dtype, S, cols = q.dtype, seq_start_row.numel(), num_heads * D
+    if dtype not in _DT or not dtype == out.dtype == k_cache.dtype == v_cache.dtype:
+        raise KernelError(f"{what}: q {q.dtype}, out {out.dtype}, cache {k_cache.dtype} and {v_cache.dtype} (all float32 or all bfloat16)")
+    if num_heads <= 0 or hkv <= 0 or num_heads % hkv:
+        raise KernelError(f"{what}: {num_heads} heads cannot share {hkv} kv heads")
+    if D <= 0 or D % 8 or D > 256:
+        raise KernelError(f"{what}: heads have a multiple of 8 elements, at most 256, not {D}")
+    T = out.shape[0] if out.dim() == 2 else -1
+    if q.dim() != 2 or q.shape[0] != T or out.shape[1] != cols or q.shape[1] < cols or parents.numel() != T:
+        raise KernelError(f"{what}: q {tuple(q.shape)}, out {tuple(out.shape)}, {parents.numel()} parents for {num_heads} heads of {D}")
+    (ldq, q_step), (ldo, out_step) = q.stride(), out.stride()
+    if q_step != 1 or out_step != 1:
+        raise KernelError(f"{what}: queries and outputs need contiguous rows, found strides {q.stride()} and {out.stride()}")
+    if block_tables.dim() != 2 or block_tables.shape[0] != S or seq_q_start.numel() != S + 1:
+        raise KernelError(f"{what}: tables {tuple(block_tables.shape)}, {seq_q_start.numel()} first rows for {S} requests")
+    if max_q_len < 0 or max_kv_len < 0 or window < 0 or max_q_len > TREE_NODES:
+        raise KernelError(f"{what}: at most {max_q_len} nodes (of {TREE_NODES}), {max_kv_len} rows, window {window}")
+    if T == 0 or S == 0 or max_q_len == 0:
+        return
+    max_q_len, width = min(max_q_len, T), block_tables.shape[1]
+    max_kv_len = min(max_kv_len, width * page_size)
+    if max_kv_len == 0 or pages == 0:  # nobody sees anything
+        raise KernelError(f"{what}: no rows can be seen: at most {max_kv_len} of {pages} pages")
+    if workspace is None:
+        raise KernelError(f"{what}: a workspace is needed")
+    dt = _DT[dtype]
+    splits, scratch, launches = _tree_attention_plan(dt, D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, dev)
+    if T == 1:
+        ldq, ldo = max(ldq, cols), max(ldo, cols)
+    try:
+        _TREE_ATTENTION.pack_into(
+            _tree_buffer, 0, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_q_start.data_ptr(),
+            seq_start_row.data_ptr(), parents.data_ptr(), workspace.address("tree_attention", scratch, torch.float32), _current_stream(), ldq, ldo, dt,
+            pages, hkv, page_size, D, width, S, T, num_heads, max_q_len, max_kv_len, min(window, 0x7fffffff), splits, scale)
+    except (struct.error, OverflowError) as e:
+        raise KernelError(f"{what}: a stride, size or scale beyond 32 bits ({e})") from None
+    _check(_packed_lib().ferris_tree_attention(_tree_buffer_at), what, launches)
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, device: int) -> tuple:
+    """Parts of a request's rows, floats of scratch and launches of a step of these sizes on a GPU."""
+    needs = (_LL * 3)()
+    _lib().ferris_tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, needs)
+    return tuple(needs)
+
+
+def sampling_probs(logits: torch.Tensor, out: torch.Tensor, temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
+                   top_p: Optional[torch.Tensor] = None):
+    """out[r] = the probabilities that ``sample`` draws row r's token from: fp32 [n, V] for fp32 ``logits`` [n, V] (rows contiguous; ``out`` may be
+    ``logits``, or memory apart from it).
+
+    Per row (fp32, int32, fp32 [n]): ``temperature`` (not above 0: 1 at the greatest logit, the first among equals; so too without it, with top_k 1 and with
+    top_p not above 0), ``top_k`` (<= 0 or None: the whole vocabulary) greatest logits, the lower index first among equals, and of these the shortest
+    prefix whose mass reaches ``top_p`` (>= 1 or None: all) of theirs.  A NaN counts as minus infinity; where the greatest logit is infinite those that equal it
+    share the mass."""
+    what = "sampling probabilities"
+    options = [t for t in (temperature, top_k, top_p) if t is not None]
+    _on_current_device(what, logits, out, *options)
+    n, V, ldl = _long_rows(f"{what}: logits", logits)
+    n2, V2, ldo = _long_rows(f"{what}: output", out)
+    if (n, V) != (n2, V2):
+        raise KernelError(f"{what}: logits {tuple(logits.shape)}, output {tuple(out.shape)}")
+    for t, name, dtype in ((temperature, "temperatures", torch.float32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32)):
+        if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
+            raise KernelError(f"{what}: {name} must be {n} contiguous {dtype}, found {tuple(t.shape)} {t.dtype}")
+    if n == 0 or V == 0:
+        return
+    if n > 1 and ldo < V:
+        raise KernelError(f"{what}: the rows of the output overlap (row stride {ldo})")
+    begin, end = logits.data_ptr(), logits.data_ptr() + 4 * ((n - 1) * ldl + V)
+    if not (out.data_ptr() == begin and (ldo == ldl or n == 1)) and out.data_ptr() < end and begin < out.data_ptr() + 4 * ((n - 1) * ldo + V):
+        raise KernelError(f"{what}: the output must be the logits themselves or lie apart from them")
+    if ldl < V:  # rows that share memory, as expand makes them: only read
+        logits, ldl = logits.contiguous(), V
+    _check(_packed_lib().ferris_sampling_probs(logits.data_ptr(), ldl, out.data_ptr(), ldo, n, V, 0 if temperature is None else temperature.data_ptr(),
+                                               0 if top_k is None else top_k.data_ptr(), 0 if top_p is None else top_p.data_ptr(), _current_stream()), what)
+
+
+def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, seq_q_start: torch.Tensor, uniforms: torch.Tensor,
+                out_nodes: torch.Tensor, out_accepted: torch.Tensor, out_token: torch.Tensor, draft_probs: Optional[torch.Tensor] = None):
+    """Accept or refuse the drafted tokens of a step so that the tokens which come out follow the target's probabilities.
+
+    Request s has the rows ``seq_q_start[s]`` .. ``seq_q_start[s + 1] - 1`` (int32 [S + 1]), at most TREE_NODES: the nodes of a tree whose first is the token that
+    was known.  ``probs`` (fp32 [T, V], contiguous rows): the target's probabilities of the token after each node (``sampling_probs``);
+    ``tokens`` (int32 [T]): each node's token; ``parents`` (int32 [T]): the number of its parent among the request's nodes.  ``draft_probs`` (as ``probs``):
+    row x holds the probabilities that the children of node x were drawn from, independently of one another; None: the drafts were chosen, not drawn.
+    ``uniforms`` (fp32 [T], 0 <= u < 1): every node's random number, the first node's for the last draw.
+
+    From the first node on, a node's children are tried in their order: child c with token t is accepted if u q(t) R < r(t), where r is the
+    node's row of ``probs`` and R = 1 at first, and after every refusal r = max(r - R q, 0), R = sum r (both stay where that is nothing); without
+    ``draft_probs`` q(t) = 1 and a refusal sets R = R - r(t), r(t) = 0.  Where no child is accepted, the next token is the first whose running sum of r exceeds
+    u times the sum of r (the lowest index first).  In 64 bits.
+
+    ``out_nodes`` (int32 [S, width]) gets the first node and the accepted ones, -1 behind them (a path ends where it is full);
+    ``out_accepted`` (int32 [S]) how many were accepted; ``out_token`` (int32 [S]) the next token.  A request without nodes has no path, 0 accepted and the token -1, which is
+    also that of a row without any probability.  NaN and negative probabilities count as 0.  Tokens outside the vocabulary and parents that are no earlier node are
+    reported (``check_kernel_status``), and such nodes not tried."""
+    what = "verification"
+    given = (probs, tokens, parents, seq_q_start, uniforms, out_nodes, out_accepted, out_token)
+    _on_current_device(what, *given, *(() if draft_probs is None else (draft_probs,)))
+    T, V, ldp = _long_rows(f"{what}: probabilities", probs)
+    _int32(what, **{"tokens": tokens, "parents": parents, "first rows": seq_q_start, "paths": out_nodes, "numbers of accepted nodes": out_accepted,
+                    "next tokens": out_token})
+    S = seq_q_start.numel() - 1
+    if uniforms.dtype != torch.float32 or not uniforms.is_contiguous():
+        raise KernelError(f"{what}: random numbers must be contiguous and {torch.float32}, found {uniforms.dtype}")
+    if S < 0 or not tokens.numel() == parents.numel() == uniforms.numel() == T or V == 0:
+        raise KernelError(f"{what}: probabilities {tuple(probs.shape)}, {tokens.numel()} tokens, {parents.numel()} parents, {uniforms.numel()} random numbers, "
+                          f"{seq_q_start.numel()} first rows")
+    if out_nodes.dim() != 2 or out_nodes.shape[0] != S or out_nodes.shape[1] < 1 or out_accepted.numel() != S or out_token.numel() != S:
+        raise KernelError(f"{what}: paths {tuple(out_nodes.shape)}, {out_accepted.numel()} numbers of accepted nodes and {out_token.numel()} next tokens for {S} requests")
+    ldd = 0
+    if draft_probs is not None:
+        T2, V2, ldd = _long_rows(f"{what}: draft's probabilities", draft_probs)
+        if (T2, V2) != (T, V):
+            raise KernelError(f"{what}: probabilities {tuple(probs.shape)}, the draft's {tuple(draft_probs.shape)}")
+    if S == 0:
+        return
+    # (rows that share memory, as expand makes them, are only read; the library wants rows that do not)
+    if ldp < V:
+        probs, ldp = probs.contiguous(), V
+    if draft_probs is not None and ldd < V:
+        draft_probs, ldd = draft_probs.contiguous(), V
+    try:
+        _VERIFY_TREE.pack_into(
+            _tree_buffer, 0, probs.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
+            seq_q_start.data_ptr(), uniforms.data_ptr(), out_nodes.data_ptr(), out_accepted.data_ptr(), out_token.data_ptr(), _current_stream(),
+            ldp, ldd, S, T, V, out_nodes.shape[1])
+    except struct.error as e:
+        raise KernelError(f"{what}: a size beyond 32 bits ({e})") from None
+    _check(_packed_lib().ferris_verify_tree(_tree_buffer_at), what)
+
+
+class CacheLayers:
+    """The paged caches of a model's layers that share block tables: [(keys, values), ...], each [pages, kv heads, page size, head size], all of
+    one shape and type, on one device.  Made once; it holds the tensors and, on the device, where they lie."""
+
+    __slots__ = ("layers", "pages", "kv_heads", "page_size", "row_bytes", "device_index", "align", "table")
+
+    def __init__(self, layers):
+        self.layers = [(k, v) for k, v in layers]
+        if not self.layers:
+            raise KernelError("cache layers: none are given")
+        first = self.layers[0][0]
+        for t in (t for layer in self.layers for t in layer):
+            _need(t, "a layer's cache")
+            if t.dim() != 4 or t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
+                raise KernelError(f"cache layers: {tuple(t.shape)} {t.dtype} on {t.device} beside {tuple(first.shape)} {first.dtype} on {first.device}")
+        self.pages, self.kv_heads, self.page_size, head_dim = first.shape
+        self.row_bytes, self.device_index = head_dim * first.element_size(), first.get_device()
+        if 0 in first.shape or self.row_bytes % 2:
+            raise KernelError(f"cache layers: nothing can be moved in caches of {tuple(first.shape)} {first.dtype}")
+        at = [t.data_ptr() for layer in self.layers for t in layer]
+        self.align = 16
+        while any(a % self.align for a in at):
+            self.align //= 2
+        self.table = torch.tensor(at, dtype=torch.int64).to(first.device)
+
+
+def keep_tree_rows(layers: CacheLayers, block_tables: torch.Tensor, seq_start_row: torch.Tensor, nodes: torch.Tensor, accepted: torch.Tensor):
+    """The cached rows of the accepted nodes move together behind their request's text, in all ``layers``.
+
+    Request s has ``seq_start_row[s]`` (int32 [S]) rows of text, and node i of its tree the row behind them by i, in the pages that ``block_tables`` (int32
+    [S, blocks]) names.  ``nodes`` (int32 [S, width], width at most TREE_NODES) and ``accepted`` (int32 [S]) are what ``verify_tree`` leaves: row seq_start_row[s] + nodes[s, j] becomes
+    row seq_start_row[s] + j for j = 1 .. accepted[s] (no further than nodes has; none where it is below 1).  Rows behind those hold what is left.  Nodes that
+    do not go up are reported (``check_kernel_status``) and end their request's moves, and so are rows without a page, which do not move."""
+    what = "rows of accepted nodes"
+    if not isinstance(layers, CacheLayers):
+        raise KernelError(f"{what}: the caches are given as CacheLayers, found {type(layers).__name__}")
+    dev = _on_current_device(what, block_tables, seq_start_row, nodes, accepted)
+    if dev != layers.device_index:
+        raise KernelError(f"{what}: the caches are on cuda:{layers.device_index}, the tables on cuda:{dev}")
+    _int32(what, **{"block tables": block_tables, "rows of the text": seq_start_row, "nodes": nodes, "numbers of accepted nodes": accepted})
+    S = seq_start_row.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != S or nodes.dim() != 2 or nodes.shape[0] != S or accepted.numel() != S:
+        raise KernelError(f"{what}: tables {tuple(block_tables.shape)}, nodes {tuple(nodes.shape)}, {accepted.numel()} numbers for {S} requests")
+    if nodes.shape[1] > TREE_NODES:
+        raise KernelError(f"{what}: paths of at most {TREE_NODES} nodes, not {nodes.shape[1]}")
+    if S == 0 or nodes.shape[1] <= 1 or block_tables.shape[1] == 0:
+        return
+    _TREE_ROWS.pack_into(_tree_buffer, 0, layers.table.data_ptr(), block_tables.data_ptr(), seq_start_row.data_ptr(), nodes.data_ptr(), accepted.data_ptr(),
+                         _current_stream(), len(layers.layers), layers.pages, layers.kv_heads, layers.page_size, layers.row_bytes, layers.align,
+                         block_tables.shape[1], S, nodes.shape[1])
+    _check(_packed_lib().ferris_tree_rows(_tree_buffer_at), what)

@@ -9,7 +9,7 @@
 namespace {
 
 // ---------------------------------------------------------------------------------------------
-// Every geometry, both types, on the CUDA cores.  A block takes 32 query rows of a request and kv head, four to a warp, and goes
+// fp32, on the CUDA cores.  A block takes 32 query rows of a request and kv head, four to a warp, and goes
 // over its part in tiles of 32 cached rows, which lie in shared memory in 32 bits:
 //   scores   a lane is a cached row: its dot products with the warp's four query rows
 //   outputs  a lane is every 32nd group of four columns: a cached row's weights for the four query rows are one read
@@ -19,20 +19,7 @@ constexpr int ROWS = 32, WARP_ROWS = 4, KEYS = 32, THREADS = 256;
 
 __host__ __device__ constexpr int padded(int d) { return d + 4; }  // rows of 16 bytes more: lanes read neighbouring rows without conflicts
 
-template <typename T>
-__device__ __forceinline__ void load4(float* to, const T* from);
-template <>
-__device__ __forceinline__ void load4<float>(float* to, const float* from) {
-    *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(from);
-}
-template <>
-__device__ __forceinline__ void load4<bf16>(float* to, const bf16* from) {
-    const uint2 v = *reinterpret_cast<const uint2*>(from);
-    *reinterpret_cast<float4*>(to) = make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
-                                                 __uint_as_float(v.y & 0xffff0000u));
-}
-
-template <typename T, int COLUMNS>  // COLUMNS: groups of four columns of a lane
+template <int COLUMNS>  // COLUMNS: groups of four columns of a lane
 __global__ void __launch_bounds__(THREADS) tree_attention_kernel(const TreeAttention p) {
     extern __shared__ __align__(16) float smem[];
     __shared__ TreeLines tree;
@@ -49,10 +36,10 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(const TreeAtten
     if (row0 >= count) return;
     tree_lines(p, r, tree);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const T* q = (const T*)p.q;
+    const float* q = (const float*)p.q;
     for (int i = threadIdx.x; i < ROWS * D; i += THREADS) {
         const int row = i / D, c = i % D, at = row0 + row;
-        qs[row * LD + c] = at < count ? to_float(q[(size_t)(r.first + at / p.group) * p.ldq + (head * p.group + at % p.group) * D + c]) : 0.0f;
+        qs[row * LD + c] = at < count ? q[(size_t)(r.first + at / p.group) * p.ldq + (head * p.group + at % p.group) * D + c] : 0.0f;
     }
     int node[WARP_ROWS];
 #pragma unroll
@@ -82,8 +69,8 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(const TreeAtten
             if (!(there >> i & 1)) continue;
             const size_t at = tree_row_at(p, __shfl_sync(0xffffffffu, page, i), head, key0 + i);
             for (int c = lane * 4; c < D; c += 128) {
-                load4(ks + i * LD + c, (const T*)p.k_cache + at + c);
-                load4(vs + i * LD + c, (const T*)p.v_cache + at + c);
+                *reinterpret_cast<float4*>(ks + i * LD + c) = *reinterpret_cast<const float4*>((const float*)p.k_cache + at + c);
+                *reinterpret_cast<float4*>(vs + i * LD + c) = *reinterpret_cast<const float4*>((const float*)p.v_cache + at + c);
             }
         }
         __syncthreads();
@@ -155,14 +142,14 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(const TreeAtten
             }
             if (lane == 0) to[D] = m[i], to[D + 1] = sum;
         } else {
-            T* to = (T*)p.out + (size_t)token * p.ldo + h * D;
+            float* to = (float*)p.out + (size_t)token * p.ldo + h * D;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
             for (int c = 0; c < COLUMNS; ++c) {
                 const int col = (c * 32 + lane) * 4;
                 if (col < D) {
-                    to[col] = from_float<T>(o[i][c].x * inv), to[col + 1] = from_float<T>(o[i][c].y * inv);
-                    to[col + 2] = from_float<T>(o[i][c].z * inv), to[col + 3] = from_float<T>(o[i][c].w * inv);
+                    to[col] = o[i][c].x * inv, to[col + 1] = o[i][c].y * inv;
+                    to[col + 2] = o[i][c].z * inv, to[col + 3] = o[i][c].w * inv;
                 }
             }
         }
@@ -170,7 +157,6 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(const TreeAtten
 }
 
 // The parts of a (token, head) joined, a warp each.  A token that no request brings is left alone.
-template <typename T>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeAttention p) {
     pdl_wait();
     pdl_launch_dependents();
@@ -191,25 +177,62 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeAttention p) {
     }
     sum = warp_sum(sum);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* to = (T*)p.out + (size_t)(r.first + row / p.heads) * p.ldo + (row % p.heads) * D;
+    float* to = (float*)p.out + (size_t)(r.first + row / p.heads) * p.ldo + (row % p.heads) * D;
     for (int c = lane; c < D; c += 32) {
         float o = 0.0f;
         for (int s = 0; s < p.splits; ++s) o = fmaf(exp2f(from[s * step + D] - base), from[s * step + c], o);
-        to[c] = from_float<T>(o * inv);
+        to[c] = o * inv;
     }
 }
 
-template <typename T>
+// The parts that the blocks of tree_attention_mma.cu left: of the rows of items that lie in several blocks, a warp each.
+__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, const TreeUnits units, int grid) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int D = p.head_dim, lane = threadIdx.x & 31, seq = blockIdx.y;
+    const TreeRequest r = tree_request(p, seq);
+    const int at = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (at >= r.nodes * p.heads) return;
+    long long before = 0;
+    const long long total = tree_total_units(p, units, seq, &before);
+    const int blocks = tree_blocks(total, grid);
+    const int head = at % p.heads / p.group, row = at / p.heads * p.group + at % p.group, block = row / units.rows;  // (token-major: at % heads % group)
+    const TreeShape s = tree_shape(p, units, r);
+    const long long first = before + ((long long)head * s.blocks + block) * s.tiles;
+    const int from = tree_owner(first, total, blocks), to = tree_owner(first + s.tiles - 1, total, blocks);
+    if (from == to) return;  // written by the block that has it
+    // the first block's part is that of an item which begins in it
+    auto part = [&](int b) { return p.parts + ((size_t)(2 * b + (b == from)) * units.rows + row % units.rows) * (D + 2); };
+    float m = -INFINITY;
+    for (int b = from + lane; b <= to; b += 32) m = fmaxf(m, part(b)[D]);
+    m = warp_max(m);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o[8] = {};
+    for (int b = from; b <= to; ++b) {
+        const float* x = part(b);
+        const float f = exp2f(x[D] - base);
+        l = fmaf(f, x[D + 1], l);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c * 32 + lane < D) o[c] = fmaf(f, x[c * 32 + lane], o[c]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bf16* out = (bf16*)p.out + (size_t)(r.first + at / p.heads) * p.ldo + at % p.heads * D;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        if (c * 32 + lane < D) out[c * 32 + lane] = from_float<bf16>(o[c] * inv);
+}
+
 int launch(const TreeAttention& p, cudaStream_t stream) {
     const int blocks = (int)(((long long)p.max_nodes * p.group + ROWS - 1) / ROWS) * p.kv_heads;
     const size_t smem = (size_t)(ROWS + 2 * KEYS) * padded(p.head_dim) * sizeof(float);
     const dim3 grid(p.splits, blocks, p.seqs);
-    const auto kernel = p.head_dim <= 128 ? tree_attention_kernel<T, 1> : tree_attention_kernel<T, 2>;
+    const auto kernel = p.head_dim <= 128 ? tree_attention_kernel<1> : tree_attention_kernel<2>;
     const int rc = ferris_allow_dynamic_smem((const void*)kernel, smem);
     if (rc != FERRIS_OK) return rc;
     cudaError_t e = ferris_launch(kernel, grid, dim3(THREADS), smem, stream, p);
     if (e == cudaSuccess && p.parts)
-        e = ferris_launch(tree_join_kernel<T>, dim3((p.max_nodes * p.heads + 7) / 8, p.seqs), dim3(256), 0, stream, p);
+        e = ferris_launch(tree_join_kernel, dim3((p.max_nodes * p.heads + 7) / 8, p.seqs), dim3(256), 0, stream, p);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;
@@ -222,6 +245,13 @@ int launch(const TreeAttention& p, cudaStream_t stream) {
 // How a step is cut: parts of a request's rows, floats of scratch, launches.
 FERRIS_API int ferris_tree_attention_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int tokens, int max_nodes, int max_kv,
                                           long long* needs) {
+    if (dtype == FERRIS_BF16) {
+        const TreeMmaPlan plan = tree_mma_plan(head_dim, seqs, kv_heads, group, max_nodes, max_kv);
+        needs[0] = 1;
+        needs[1] = 2ll * plan.blocks * plan.rows * (head_dim + 2);
+        needs[2] = 2;
+        return FERRIS_OK;
+    }
     const long long blocks = ((long long)max_nodes * group + ROWS - 1) / ROWS * kv_heads * seqs;
     const int sms = ferris_sm_count();
     const long long tiles = (max_kv + KEYS - 1) / KEYS;
@@ -264,5 +294,20 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     p.splits = a->splits > 1 ? a->splits : 1;
     p.parts = p.splits > 1 ? (float*)const_cast<void*>(a->parts) : nullptr;
     p.status = ferris_status_ptr();
-    return a->dtype == FERRIS_BF16 ? launch<bf16>(p, (cudaStream_t)a->stream) : launch<float>(p, (cudaStream_t)a->stream);
+    if (a->dtype == FERRIS_BF16) {
+        const TreeMmaPlan plan = tree_mma_plan(a->head_dim, a->seqs, a->kv_heads, p.group, a->max_nodes, p.limit);
+        if (!a->parts) FERRIS_REFUSE("parts need scratch");
+        p.parts = (float*)const_cast<void*>(a->parts);
+        const int rc = tree_attention_mma(p, plan, (cudaStream_t)a->stream);
+        if (rc != FERRIS_OK) return rc;
+        const TreeUnits units = {plan.unit, plan.rows};
+        const cudaError_t e = ferris_launch(tree_parts_kernel, dim3((p.max_nodes * p.heads + 7) / 8, p.seqs), dim3(256), 0, (cudaStream_t)a->stream, p, units,
+                                            plan.blocks);
+        if (e != cudaSuccess) {
+            ferris_set_error("%s", cudaGetErrorString(e));
+            return (int)e;
+        }
+        FERRIS_LAUNCH_CHECK();
+    }
+    return launch(p, (cudaStream_t)a->stream);
 }

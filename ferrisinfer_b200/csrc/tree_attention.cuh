@@ -8,6 +8,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "packed_cache.cuh"
 
@@ -30,7 +32,7 @@ struct TreeAttention {
     int seqs, tokens, heads, kv_heads, group, head_dim, pages, page_size, max_nodes, window;
     float scale;  // of the scores, times log2(e)
     DivideBy page;  // the page size
-    float* parts;  // [part][token][head][D + 2]: unnormalised output, maximum (to the base of 2) and sum, or nullptr: one part, `out` itself
+    float* parts;  // of D + 2 numbers a query row: unnormalised output, maximum (to the base of 2) and sum
     int splits;
     int* status;
 };
@@ -116,3 +118,102 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeAttention& p, const Tree
     }
     return m & bits_between(0, r.rows - key0);
 }
+
+// ---------------------------------------------------------------------------------------------
+// The work of a step as units: an item is a block of query rows of a request and kv head, a unit `unit` cached rows of it.  Units are numbered
+// through, requests first, then kv heads, then blocks of query rows, then cached rows.
+// ---------------------------------------------------------------------------------------------
+struct TreeUnits {
+    int unit, rows;  // cached rows of a unit, query rows of a block
+};
+
+// Units in front of a request's cached rows that none of its nodes sees, units of an item, items.
+struct TreeShape {
+    int low, tiles, blocks;
+};
+
+__device__ __forceinline__ TreeShape tree_shape(const TreeAttention& p, const TreeUnits& u, const TreeRequest& r) {
+    TreeShape s;
+    s.low = p.window > 0 ? max(0, r.start - p.window + 1) / u.unit : 0;
+    s.tiles = max((r.rows + u.unit - 1) / u.unit - s.low, 1);  // (nothing that could be seen: still a unit, which says so)
+    s.blocks = (r.nodes * p.group + u.rows - 1) / u.rows;
+    return s;
+}
+
+__device__ __forceinline__ long long tree_scan(long long v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += x;
+    }
+    return v;
+}
+
+// Units of the requests 32 i + lane, by a whole warp.
+__device__ __forceinline__ long long tree_units_of(const TreeAttention& p, const TreeUnits& u, int seq, TreeRequest& r) {
+    if (seq >= p.seqs) return 0;
+    r = tree_request(p, seq);
+    const TreeShape s = tree_shape(p, u, r);
+    return (long long)s.tiles * s.blocks * p.kv_heads;
+}
+
+// All units of the step, and those of the requests before `seq`; by a whole warp.
+__device__ __forceinline__ long long tree_total_units(const TreeAttention& p, const TreeUnits& u, int seq = -1, long long* before = nullptr) {
+    long long total = 0;
+    for (int s0 = 0; s0 < p.seqs; s0 += 32) {
+        TreeRequest r;
+        const long long mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
+        if (before && seq >= s0 && seq < s0 + 32) *before = total + __shfl_sync(0xffffffffu, upto - mine, seq - s0);
+        total += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return total;
+}
+
+struct TreeItem {
+    TreeRequest request;
+    int seq, head, block, tile, tiles, low;
+};
+
+// The item that a unit belongs to, and which of its units it is; by a whole warp.
+__device__ __forceinline__ TreeItem tree_item(const TreeAttention& p, const TreeUnits& u, long long unit) {
+    TreeItem item;
+    long long before = 0;
+    for (int s0 = 0;; s0 += 32) {
+        TreeRequest r = {};
+        const long long mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
+        const unsigned here = __ballot_sync(0xffffffffu, unit < before + upto);
+        if (here) {
+            const int at = __ffs(here) - 1;
+            item.seq = s0 + at;
+            item.request.first = __shfl_sync(0xffffffffu, r.first, at);
+            item.request.nodes = __shfl_sync(0xffffffffu, r.nodes, at);
+            item.request.start = __shfl_sync(0xffffffffu, r.start, at);
+            item.request.rows = __shfl_sync(0xffffffffu, r.rows, at);
+            before += __shfl_sync(0xffffffffu, upto - mine, at);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+        if (s0 >= p.seqs) {  // (no such unit)
+            item = TreeItem();
+            return item;
+        }
+    }
+    const TreeShape s = tree_shape(p, u, item.request);
+    const long long in = unit - before;
+    item.tile = (int)(in % s.tiles), item.tiles = s.tiles, item.low = s.low;
+    item.block = (int)(in / s.tiles % s.blocks), item.head = (int)(in / s.tiles / s.blocks);
+    return item;
+}
+
+// Blocks that get units: every one of them at least one, so that each between the first and the last of an item leaves a part of it.
+__device__ __forceinline__ int tree_blocks(long long total, int grid) { return total < grid ? (int)total : grid; }
+
+// The block that has a unit when block c has those from total c / blocks on.
+__device__ __forceinline__ int tree_owner(long long unit, long long total, int blocks) { return (int)(((unit + 1) * blocks - 1) / total); }
+
+// bf16, on mma.sync (tree_attention_mma.cu).
+struct TreeMmaPlan {
+    int unit, rows, blocks;
+};
+TreeMmaPlan tree_mma_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv);
+int tree_attention_mma(const TreeAttention& p, const TreeMmaPlan& plan, cudaStream_t stream);

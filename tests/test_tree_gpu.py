@@ -95,6 +95,8 @@ class Step:
     def run(self, ops, workspace, window=0, out=None, most=None):
         out = torch.full((self.q.shape[0], self.heads * self.D), 7.0, dtype=self.q.dtype, device=DEV) if out is None else out
         most = most or self.most
+        for buffer in workspace._buffers.values():  # (what a call finds in its scratch has no effect)
+            buffer.fill_(math.nan if buffer.is_floating_point() else 0)
         self.device_tensors = [ints(self.tables), ints(self.q_start), ints(self.starts), ints(self.parents)]
         ops.tree_attention(self.q, out, self.k, self.v, *self.device_tensors, most[0], most[1], self.heads, self.D ** -0.5, window=window, workspace=workspace)
         return out

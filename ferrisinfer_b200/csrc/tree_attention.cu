@@ -193,12 +193,11 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
     const TreeRequest r = tree_request(p, seq);
     const int at = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (at >= r.nodes * p.heads) return;
-    long long before = 0;
-    const long long total = tree_total_units(p, units, seq, &before);
-    const int blocks = tree_blocks(total, grid);
+    int before = 0;
+    const int total = tree_total_units(p, units, seq, &before), blocks = tree_blocks(total, grid);
     const int head = at % p.heads / p.group, row = at / p.heads * p.group + at % p.group, block = row / units.rows;  // (token-major: at % heads % group)
     const TreeShape s = tree_shape(p, units, r);
-    const long long first = before + ((long long)head * s.blocks + block) * s.tiles;
+    const int first = before + (head * s.blocks + block) * s.tiles;
     const int from = tree_owner(first, total, blocks), to = tree_owner(first + s.tiles - 1, total, blocks);
     if (from == to) return;  // written by the block that has it
     // the first block's part is that of an item which begins in it
@@ -297,6 +296,7 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     if (a->dtype == FERRIS_BF16) {
         const TreeMmaPlan plan = tree_mma_plan(a->head_dim, a->seqs, a->kv_heads, p.group, a->max_nodes, p.limit);
         if (!a->parts) FERRIS_REFUSE("parts need scratch");
+        if (!plan.fits) FERRIS_REFUSE("%d requests of up to %d rows exceed one launch", a->seqs, p.limit);
         p.parts = (float*)const_cast<void*>(a->parts);
         const int rc = tree_attention_mma(p, plan, (cudaStream_t)a->stream);
         if (rc != FERRIS_OK) return rc;

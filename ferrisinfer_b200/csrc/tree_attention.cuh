@@ -140,29 +140,29 @@ __device__ __forceinline__ TreeShape tree_shape(const TreeAttention& p, const Tr
     return s;
 }
 
-__device__ __forceinline__ long long tree_scan(long long v) {
+__device__ __forceinline__ int tree_scan(int v) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, v, o);
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
         if ((threadIdx.x & 31) >= o) v += x;
     }
     return v;
 }
 
 // Units of the requests 32 i + lane, by a whole warp.
-__device__ __forceinline__ long long tree_units_of(const TreeAttention& p, const TreeUnits& u, int seq, TreeRequest& r) {
+__device__ __forceinline__ int tree_units_of(const TreeAttention& p, const TreeUnits& u, int seq, TreeRequest& r) {
     if (seq >= p.seqs) return 0;
     r = tree_request(p, seq);
     const TreeShape s = tree_shape(p, u, r);
-    return (long long)s.tiles * s.blocks * p.kv_heads;
+    return s.tiles * s.blocks * p.kv_heads;
 }
 
 // All units of the step, and those of the requests before `seq`; by a whole warp.
-__device__ __forceinline__ long long tree_total_units(const TreeAttention& p, const TreeUnits& u, int seq = -1, long long* before = nullptr) {
-    long long total = 0;
+__device__ __forceinline__ int tree_total_units(const TreeAttention& p, const TreeUnits& u, int seq = -1, int* before = nullptr) {
+    int total = 0;
     for (int s0 = 0; s0 < p.seqs; s0 += 32) {
         TreeRequest r;
-        const long long mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
+        const int mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
         if (before && seq >= s0 && seq < s0 + 32) *before = total + __shfl_sync(0xffffffffu, upto - mine, seq - s0);
         total += __shfl_sync(0xffffffffu, upto, 31);
     }
@@ -175,12 +175,12 @@ struct TreeItem {
 };
 
 // The item that a unit belongs to, and which of its units it is; by a whole warp.
-__device__ __forceinline__ TreeItem tree_item(const TreeAttention& p, const TreeUnits& u, long long unit) {
+__device__ __forceinline__ TreeItem tree_item(const TreeAttention& p, const TreeUnits& u, int unit) {
     TreeItem item;
-    long long before = 0;
+    int before = 0;
     for (int s0 = 0;; s0 += 32) {
         TreeRequest r = {};
-        const long long mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
+        const int mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
         const unsigned here = __ballot_sync(0xffffffffu, unit < before + upto);
         if (here) {
             const int at = __ffs(here) - 1;
@@ -199,21 +199,29 @@ __device__ __forceinline__ TreeItem tree_item(const TreeAttention& p, const Tree
         }
     }
     const TreeShape s = tree_shape(p, u, item.request);
-    const long long in = unit - before;
-    item.tile = (int)(in % s.tiles), item.tiles = s.tiles, item.low = s.low;
-    item.block = (int)(in / s.tiles % s.blocks), item.head = (int)(in / s.tiles / s.blocks);
+    const int in = unit - before, nth = in / s.tiles;
+    item.tile = in - nth * s.tiles, item.tiles = s.tiles, item.low = s.low;
+    item.head = nth / s.blocks, item.block = nth - item.head * s.blocks;
     return item;
 }
 
 // Blocks that get units: every one of them at least one, so that each between the first and the last of an item leaves a part of it.
-__device__ __forceinline__ int tree_blocks(long long total, int grid) { return total < grid ? (int)total : grid; }
-
-// The block that has a unit when block c has those from total c / blocks on.
-__device__ __forceinline__ int tree_owner(long long unit, long long total, int blocks) { return (int)(((unit + 1) * blocks - 1) / total); }
+__device__ __forceinline__ int tree_blocks(int total, int grid) { return min(total, grid); }
+// The first unit of a block: the first total % blocks of them have one more than the others.
+__device__ __forceinline__ int tree_begin(int block, int total, int blocks) {
+    const int per = total / blocks, more = total - per * blocks;
+    return block * per + min(block, more);
+}
+// The block that has a unit.
+__device__ __forceinline__ int tree_owner(int unit, int total, int blocks) {
+    const int per = total / blocks, more = total - per * blocks, at = more * (per + 1);
+    return unit < at ? unit / (per + 1) : more + (unit - at) / per;
+}
 
 // bf16, on mma.sync (tree_attention_mma.cu).
 struct TreeMmaPlan {
     int unit, rows, blocks;
+    bool fits;  // units are counted in 32 bits
 };
 TreeMmaPlan tree_mma_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv);
 int tree_attention_mma(const TreeAttention& p, const TreeMmaPlan& plan, cudaStream_t stream);

@@ -33,14 +33,16 @@ __device__ __forceinline__ float exp2_unit(float x) {
 // Sizes of a variant: heads padded to DP elements, MS slabs of 16 query rows to a warp, WR warps to a tile, NW warps.
 template <int DP, int MS, int WR, int NW, int ST>
 struct Plan {
-    static constexpr int GROUPS = NW / WR, TILE = 16 * WR, UNIT = TILE * GROUPS, ROWS = 16 * MS * WR;
+    static constexpr int FETCH = NW == 4 ? 16 : 128 / NW;  // cached rows of a stage that a warp fetches
+    static constexpr int GROUPS = NW / WR, TILE = FETCH * WR, UNIT = TILE * GROUPS, ROWS = 16 * MS * WR;
+    static_assert(TILE % 16 == 0, "tiles of whole MMAs");
     static constexpr int ROW = DP * 2 + (DP % 64 ? 16 : 0);  // bytes of a row: eight rows of one 16-byte column lie on different banks
-    static constexpr int RING = NW * 16 * 2 * ROW * ST;
+    static constexpr int RING = UNIT * 2 * ROW * ST;
     static constexpr int JOIN = NW * 16 * MS * (DP + 4) * 4;
     static constexpr int Q_AT = RING > JOIN ? RING : JOIN;
     static constexpr int SMEM = Q_AT + ROWS * ROW;
-    static constexpr bool Q_HELD = MS * DP <= 128;  // fragments of the query rows stay in registers
-    static constexpr int BLOCKS = DP <= 64 && MS == 1 ? 2 : 1;
+    static constexpr bool Q_HELD = MS * DP <= (NW == 16 ? 64 : 128);  // fragments of the query rows stay in registers
+    static constexpr int BLOCKS = DP <= 64 && NW == 8 ? 2 : 1;
 };
 
 // Byte offset of a 16-byte column of a row.
@@ -55,10 +57,10 @@ __device__ __forceinline__ uint32_t place(int row, int column) {
 template <int DP, int MS, int WR, int NW, int ST>
 __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tree_attention_mma_kernel(const TreeAttention p, const TreeUnits units) {
     using P = Plan<DP, MS, WR, NW, ST>;
-    constexpr int KS = DP / 16, SUB = P::TILE < 32 ? P::TILE : 32, NT = SUB / 8;
+    constexpr int KS = DP / 16, SUB = P::TILE < 32 ? P::TILE : 32, NT = SUB / 8, FETCH = P::FETCH;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ TreeLines tree;
-    __shared__ uint32_t there[ST][NW];  // which of the 16 cached rows that a warp fetched have a page
+    __shared__ uint32_t there[ST][NW];  // which of the cached rows that a warp fetched have a page
     __shared__ float row_m[NW][16 * MS], row_l[NW][16 * MS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = warp / WR, wr = warp % WR, D = p.head_dim;
@@ -66,15 +68,14 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
     unsigned char* q_smem = smem + P::Q_AT;
     pdl_wait();
     pdl_launch_dependents();
-    const long long total = tree_total_units(p, units);
-    const int blocks = tree_blocks(total, gridDim.x);
+    const int total = tree_total_units(p, units), blocks = tree_blocks(total, gridDim.x);
     if ((int)blockIdx.x >= blocks) return;
-    const long long begin = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
-    for (long long unit = begin; unit < end;) {
+    const int end = tree_begin(blockIdx.x + 1, total, blocks);
+    for (int unit = tree_begin(blockIdx.x, total, blocks); unit < end;) {
         const TreeItem item = tree_item(p, units, unit);
         const TreeRequest r = item.request;
         const int head = item.head, row0 = item.block * P::ROWS, count = r.nodes * p.group;
-        const int first = item.tile, last = (int)min((long long)item.tiles, first + (end - unit));  // tiles of UNIT rows
+        const int first = item.tile, last = min(item.tiles, first + (end - unit));  // tiles of UNIT rows
         const bool whole_item = first == 0 && last == item.tiles;
         const int* table = p.tables + (size_t)item.seq * p.width;
         const int low = item.low;  // tiles of the request in front of its first
@@ -82,20 +83,20 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
         auto request = [&](int i) {
             const int s = i % ST;
             if (i < last) {
-                const int row = (low + i) * P::UNIT + group * P::TILE + wr * 16 + (lane & 15);
+                const int row = (low + i) * P::UNIT + group * P::TILE + wr * FETCH + (lane & (FETCH - 1));
                 const int page = row < r.rows ? tree_page(p, table, row) : -1;
                 const size_t at = page >= 0 ? tree_row_at(p, page, head, row) : 0;
-                const uint32_t live = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+                const uint32_t live = __ballot_sync(0xffffffffu, page >= 0) & ((1u << FETCH) - 1);
                 if (lane == 0) there[s][warp] = live;
                 const uint32_t k_dst = smem_u32(ring + (size_t)(2 * s) * P::TILE * P::ROW), v_dst = k_dst + P::TILE * P::ROW;
                 constexpr int CH = DP / 8;
 #pragma unroll
-                for (int c = 0; c < (16 * CH + 31) / 32; ++c) {
+                for (int c = 0; c < (FETCH * CH + 31) / 32; ++c) {
                     const int piece = c * 32 + lane, rr = piece / CH, column = piece % CH;
-                    const size_t from = __shfl_sync(0xffffffffu, at, rr & 15) + column * 8;
+                    const size_t from = __shfl_sync(0xffffffffu, at, rr & (FETCH - 1)) + column * 8;
                     const bool ok = (live >> rr & 1) && column * 8 < D;
-                    if (16 * CH % 32 == 0 || rr < 16) {
-                        const uint32_t to = place<DP>(wr * 16 + rr, column);
+                    if (FETCH * CH % 32 == 0 || rr < FETCH) {
+                        const uint32_t to = place<DP>(wr * FETCH + rr, column);
                         copy_async(k_dst + to, (const bf16*)p.k_cache + (ok ? from : 0), ok);
                         copy_async(v_dst + to, (const bf16*)p.v_cache + (ok ? from : 0), ok);
                     }
@@ -203,8 +204,9 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
                         }
                     }
                 }
-                uint32_t pages = there[s][group * WR + sub * 2];
-                if (SUB == 32) pages |= there[s][group * WR + sub * 2 + (SUB == 32)] << 16;
+                uint32_t pages = 0;
+#pragma unroll
+                for (int k = 0; k < SUB / FETCH; ++k) pages |= there[s][group * WR + sub * (SUB / FETCH) + k] << (k * FETCH);
                 const bool whole = key0 >= sure_low && key0 + SUB <= sure_high && pages == (SUB == 32 ? 0xffffffffu : 0xffffu);
                 uint32_t sees[MS][2];
                 if (!whole) {
@@ -394,9 +396,9 @@ void with_variant(int D, int rows, F f) {
 #define TREE_ROWS_OF(DP, ST)              \
     do {                                  \
         if (rows <= 16) TREE_VARIANT(DP, 1, 1, 8, ST); \
-        if (rows <= 32) TREE_VARIANT(DP, 2, 1, 8, ST); \
-        if (rows <= 64) TREE_VARIANT(DP, 2, 2, 8, ST); \
-        TREE_VARIANT(DP, 2, 4, 8, 2);     \
+        if (rows <= 32) TREE_VARIANT(DP, 1, 2, 16, ST); \
+        if (rows <= 64) TREE_VARIANT(DP, 1, 4, 16, ST); \
+        TREE_VARIANT(DP, 1, 8, 16, 2);     \
     } while (0)
     if (D <= 32) TREE_ROWS_OF(32, 3);
     if (D <= 64) TREE_ROWS_OF(64, 3);
@@ -424,6 +426,7 @@ TreeMmaPlan tree_mma_plan(int head_dim, int seqs, int kv_heads, int group, int m
         const int sms = ferris_sm_count();
         const long long want = (long long)(sms > 0 ? sms : 148) * P::BLOCKS;
         plan.blocks = (int)(want < most ? want : most);
+        plan.fits = most <= 0x7fffffff;
     });
     return plan;
 }

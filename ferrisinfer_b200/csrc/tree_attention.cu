@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(const TreeAtten
     const TreeRequest r = tree_request(p, seq);
     const int count = r.nodes * p.group;
     if (row0 >= count) return;
-    tree_lines(p, r, tree);
+    tree_lines<THREADS>(p, r, tree, [] { __syncthreads(); });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float* q = (const float*)p.q;
     for (int i = threadIdx.x; i < ROWS * D; i += THREADS) {
@@ -185,41 +185,46 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeAttention p) {
     }
 }
 
-// The parts that the blocks of tree_attention_mma.cu left: of the rows of items that lie in several blocks, a warp each.
-__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, const TreeUnits units, int grid) {
+// The parts that the groups of a bf16 step's blocks left of items that lie in several, a warp a (token, head).
+template <int COLUMNS>  // pairs of columns of a lane
+__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes) {
     pdl_wait();
     pdl_launch_dependents();
     const int D = p.head_dim, lane = threadIdx.x & 31, seq = blockIdx.y;
     const TreeRequest r = tree_request(p, seq);
     const int at = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (at >= r.nodes * p.heads) return;
-    int before = 0;
-    const int total = tree_total_units(p, units, seq, &before), blocks = tree_blocks(total, grid);
-    const int head = at % p.heads / p.group, row = at / p.heads * p.group + at % p.group, block = row / units.rows;  // (token-major: at % heads % group)
-    const TreeShape s = tree_shape(p, units, r);
-    const int first = before + (head * s.blocks + block) * s.tiles;
-    const int from = tree_owner(first, total, blocks), to = tree_owner(first + s.tiles - 1, total, blocks);
-    if (from == to) return;  // written by the block that has it
-    // the first block's part is that of an item which begins in it
-    auto part = [&](int b) { return p.parts + ((size_t)(2 * b + (b == from)) * units.rows + row % units.rows) * (D + 2); };
+    const int node = at / p.heads, q_head = at - node * p.heads, head = q_head / p.group, row = node * p.group + q_head - head * p.group;
+    const int2 span = p.spans[seq * p.kv_heads + head];
+    if (span.x == span.y) return;  // written by the block that has it
+    const int block = row / rows, in = row - block * rows;
+    auto part = [&](int g) { return tree_part(p, g * lanes + block, g == span.x, rows, in); };
     float m = -INFINITY;
-    for (int b = from + lane; b <= to; b += 32) m = fmaxf(m, part(b)[D]);
+    for (int g = span.x + lane; g <= span.y; g += 32) m = fmaxf(m, part(g)[D]);
     m = warp_max(m);
     const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[8] = {};
-    for (int b = from; b <= to; ++b) {
-        const float* x = part(b);
-        const float f = exp2f(x[D] - base);
-        l = fmaf(f, x[D + 1], l);
+    float l = 0.0f;
+    float2 o[COLUMNS];
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-            if (c * 32 + lane < D) o[c] = fmaf(f, x[c * 32 + lane], o[c]);
+    for (int c = 0; c < COLUMNS; ++c) o[c] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (int g = span.x; g <= span.y; ++g) {
+        const float* x = part(g);
+        const float2 ml = *reinterpret_cast<const float2*>(x + D);
+        const float f = exp2f(ml.x - base);
+        l = fmaf(f, ml.y, l);
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+            if (c * 64 + 2 * lane < D) {
+                const float2 v = *reinterpret_cast<const float2*>(x + c * 64 + 2 * lane);
+                o[c].x = fmaf(f, v.x, o[c].x), o[c].y = fmaf(f, v.y, o[c].y);
+            }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    bf16* out = (bf16*)p.out + (size_t)(r.first + at / p.heads) * p.ldo + at % p.heads * D;
+    bf16* out = (bf16*)p.out + (size_t)(r.first + node) * p.ldo + q_head * D;
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-        if (c * 32 + lane < D) out[c * 32 + lane] = from_float<bf16>(o[c] * inv);
+    for (int c = 0; c < COLUMNS; ++c)
+        if (c * 64 + 2 * lane < D) out[c * 64 + 2 * lane] = from_float<bf16>(o[c].x * inv), out[c * 64 + 2 * lane + 1] = from_float<bf16>(o[c].y * inv);
 }
 
 int launch(const TreeAttention& p, cudaStream_t stream) {
@@ -241,13 +246,12 @@ int launch(const TreeAttention& p, cudaStream_t stream) {
 
 }  // namespace
 
-// How a step is cut: parts of a request's rows, floats of scratch, launches.
-FERRIS_API int ferris_tree_attention_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int tokens, int max_nodes, int max_kv,
-                                          long long* needs) {
+// How a step is cut: parts of a request's rows (32 bits), floats of scratch, launches.
+FERRIS_API int ferris_tree_attention_plan(int dtype, int head_dim, int seqs, int kv_heads, int group, int tokens, int max_nodes, int max_kv, int page_size,
+                                          long long cache_rows, float scale, int window, long long* needs) {
     if (dtype == FERRIS_BF16) {
-        const TreeMmaPlan plan = tree_mma_plan(head_dim, seqs, kv_heads, group, max_nodes, max_kv);
         needs[0] = 1;
-        needs[1] = 2ll * plan.blocks * plan.rows * (head_dim + 2);
+        needs[1] = tree_plan(head_dim, seqs, kv_heads, group, max_nodes, max_kv, page_size, cache_rows, scale, window).floats(seqs, kv_heads, head_dim);
         needs[2] = 2;
         return FERRIS_OK;
     }
@@ -292,17 +296,20 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     p.page = DivideBy(a->page_size);
     p.splits = a->splits > 1 ? a->splits : 1;
     p.parts = p.splits > 1 ? (float*)const_cast<void*>(a->parts) : nullptr;
+    p.spans = nullptr;
     p.status = ferris_status_ptr();
     if (a->dtype == FERRIS_BF16) {
-        const TreeMmaPlan plan = tree_mma_plan(a->head_dim, a->seqs, a->kv_heads, p.group, a->max_nodes, p.limit);
         if (!a->parts) FERRIS_REFUSE("parts need scratch");
+        const TreePlan plan = tree_plan(a->head_dim, a->seqs, a->kv_heads, p.group, a->max_nodes, p.limit, a->page_size,
+                                        (long long)a->pages * a->kv_heads * a->page_size, a->scale, a->window);
         if (!plan.fits) FERRIS_REFUSE("%d requests of up to %d rows exceed one launch", a->seqs, p.limit);
         p.parts = (float*)const_cast<void*>(a->parts);
-        const int rc = tree_attention_mma(p, plan, (cudaStream_t)a->stream);
+        p.spans = (int2*)(p.parts + 2ll * plan.groups * plan.lanes * plan.rows * (p.head_dim + 2));
+        const int rc = plan.tensor ? tree_attention_tc(p, plan, (cudaStream_t)a->stream) : tree_attention_mma(p, plan, (cudaStream_t)a->stream);
         if (rc != FERRIS_OK) return rc;
-        const TreeUnits units = {plan.unit, plan.rows};
-        const cudaError_t e = ferris_launch(tree_parts_kernel, dim3((p.max_nodes * p.heads + 7) / 8, p.seqs), dim3(256), 0, (cudaStream_t)a->stream, p, units,
-                                            plan.blocks);
+        const dim3 grid((p.max_nodes * p.heads + 7) / 8, p.seqs);
+        const auto kernel = p.head_dim <= 64 ? tree_parts_kernel<1> : p.head_dim <= 128 ? tree_parts_kernel<2> : tree_parts_kernel<4>;
+        const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, (cudaStream_t)a->stream, p, plan.rows, plan.lanes);
         if (e != cudaSuccess) {
             ferris_set_error("%s", cudaGetErrorString(e));
             return (int)e;

@@ -34,6 +34,7 @@ struct TreeAttention {
     DivideBy page;  // the page size
     float* parts;  // of D + 2 numbers a query row: unnormalised output, maximum (to the base of 2) and sum
     int splits;
+    int2* spans;  // first and last group of every request and kv head
     int* status;
 };
 
@@ -77,10 +78,11 @@ struct TreeLines {
     short depth[TREE_NODES];
 };
 
-// By all threads of the block, which are synchronised when it returns.  A parent that is not an earlier node of the request
-// counts as none.
-__device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeRequest& r, TreeLines& t) {
-    for (int i = threadIdx.x; i < r.nodes; i += blockDim.x) {
+// By the first `threads` of a block, for whom `barrier` is one; they are synchronised when it returns.  A parent that is not an earlier node of the
+// request counts as none.
+template <int THREADS, typename Barrier>
+__device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeRequest& r, TreeLines& t, Barrier barrier) {
+    for (int i = threadIdx.x; i < r.nodes; i += THREADS) {
         int up = p.parents[r.first + i];
         if (up >= i || up < -1) {
             ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 112);
@@ -88,8 +90,8 @@ __device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeReq
         }
         t.parent[i] = (short)up;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < r.nodes; i += blockDim.x) {
+    barrier();
+    for (int i = threadIdx.x; i < r.nodes; i += THREADS) {
 #pragma unroll
         for (int w = 0; w < TREE_WORDS; ++w) t.line[i][w] = 0u;
         int depth = 0;
@@ -97,7 +99,7 @@ __device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeReq
             if (p.window <= 0 || depth < p.window) t.line[i][at >> 5] |= 1u << (at & 31);
         t.depth[i] = (short)(depth - 1);
     }
-    __syncthreads();
+    barrier();
 }
 
 // Bits lo .. hi - 1 of 32, for bounds anywhere.
@@ -120,25 +122,24 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeAttention& p, const Tree
 }
 
 // ---------------------------------------------------------------------------------------------
-// The work of a step as units: an item is a block of query rows of a request and kv head, a unit `unit` cached rows of it.  Units are numbered
-// through, requests first, then kv heads, then blocks of query rows, then cached rows.
+// The work of a bf16 step as units: a unit is UNIT cached rows of a request and kv head, an item all units of one.  Units are numbered through,
+// requests first, then kv heads, then cached rows, and dealt out evenly, whatever the requests' lengths, to groups of `lanes` blocks: the blocks of a group take
+// the same cached rows at the same time, each its own block of query rows (a request with fewer query rows leaves some without work).
+// An item that lies in one group is written by it; of others every group leaves its part (at most two of a group), which tree_parts_kernel joins
+// in the order of the units, so that results do not depend on timing.
 // ---------------------------------------------------------------------------------------------
-struct TreeUnits {
-    int unit, rows;  // cached rows of a unit, query rows of a block
+struct TreePlan {
+    int unit, rows;   // cached rows of a unit, query rows of a block
+    int groups, lanes;  // groups of blocks, blocks of a group
+    bool tensor;      // on tcgen05 (tree_attention_tc.cu), otherwise on mma.sync (tree_attention_mma.cu)
+    bool fits;        // units are counted in 32 bits
+    long long floats(int seqs, int kv_heads, int head_dim) const {  // of scratch: parts, and behind them the items' groups
+        return 2ll * groups * lanes * rows * (head_dim + 2) + 2ll * seqs * kv_heads;
+    }
 };
-
-// Units in front of a request's cached rows that none of its nodes sees, units of an item, items.
-struct TreeShape {
-    int low, tiles, blocks;
-};
-
-__device__ __forceinline__ TreeShape tree_shape(const TreeAttention& p, const TreeUnits& u, const TreeRequest& r) {
-    TreeShape s;
-    s.low = p.window > 0 ? max(0, r.start - p.window + 1) / u.unit : 0;
-    s.tiles = max((r.rows + u.unit - 1) / u.unit - s.low, 1);  // (nothing that could be seen: still a unit, which says so)
-    s.blocks = (r.nodes * p.group + u.rows - 1) / u.rows;
-    return s;
-}
+TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window);
+int tree_attention_mma(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
+int tree_attention_tc(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
 
 __device__ __forceinline__ int tree_scan(int v) {
 #pragma unroll
@@ -149,79 +150,83 @@ __device__ __forceinline__ int tree_scan(int v) {
     return v;
 }
 
-// Units of the requests 32 i + lane, by a whole warp.
-__device__ __forceinline__ int tree_units_of(const TreeAttention& p, const TreeUnits& u, int seq, TreeRequest& r) {
-    if (seq >= p.seqs) return 0;
-    r = tree_request(p, seq);
-    const TreeShape s = tree_shape(p, u, r);
-    return s.tiles * s.blocks * p.kv_heads;
+// First and last unit of an item: units of cached rows that none of the nodes sees are left out in front.
+template <int UNIT>
+__device__ __forceinline__ int tree_low(const TreeAttention& p, const TreeRequest& r) {
+    return p.window > 0 ? max(0, r.start - p.window + 1) / UNIT : 0;
 }
-
-// All units of the step, and those of the requests before `seq`; by a whole warp.
-__device__ __forceinline__ int tree_total_units(const TreeAttention& p, const TreeUnits& u, int seq = -1, int* before = nullptr) {
-    int total = 0;
-    for (int s0 = 0; s0 < p.seqs; s0 += 32) {
-        TreeRequest r;
-        const int mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
-        if (before && seq >= s0 && seq < s0 + 32) *before = total + __shfl_sync(0xffffffffu, upto - mine, seq - s0);
-        total += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return total;
+template <int UNIT>
+__device__ __forceinline__ int tree_tiles(const TreeAttention& p, const TreeRequest& r) {
+    // (nodes that can see nothing: still a unit, which says so)
+    return r.nodes > 0 ? max((r.rows + UNIT - 1) / UNIT - tree_low<UNIT>(p, r), 1) : 0;
 }
 
 struct TreeItem {
     TreeRequest request;
-    int seq, head, block, tile, tiles, low;
+    int seq, head;
+    int first, last, tiles, low;  // its units that are this group's, of all its units; units in front of them
 };
 
-// The item that a unit belongs to, and which of its units it is; by a whole warp.
-__device__ __forceinline__ TreeItem tree_item(const TreeAttention& p, const TreeUnits& u, int unit) {
-    TreeItem item;
-    int before = 0;
-    for (int s0 = 0;; s0 += 32) {
-        TreeRequest r = {};
-        const int mine = tree_units_of(p, u, s0 + (threadIdx.x & 31), r), upto = tree_scan(mine);
-        const unsigned here = __ballot_sync(0xffffffffu, unit < before + upto);
-        if (here) {
-            const int at = __ffs(here) - 1;
-            item.seq = s0 + at;
-            item.request.first = __shfl_sync(0xffffffffu, r.first, at);
-            item.request.nodes = __shfl_sync(0xffffffffu, r.nodes, at);
-            item.request.start = __shfl_sync(0xffffffffu, r.start, at);
-            item.request.rows = __shfl_sync(0xffffffffu, r.rows, at);
-            before += __shfl_sync(0xffffffffu, upto - mine, at);
-            break;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-        if (s0 >= p.seqs) {  // (no such unit)
-            item = TreeItem();
-            return item;
-        }
+// Goes through a group's units, item by item; by whole warps, each for itself.
+template <int UNIT>
+struct TreeWalk {
+    int total, groups, unit, end;  // units of the step; groups that have some; where this one is, where it ends
+    TreeRequest mine;              // of request 32 s0 + lane
+    int s0, before, upto;          // units before these requests, and up to and with this lane's
+
+    __device__ __forceinline__ void look_at(const TreeAttention& p, int chunk) {
+        s0 = chunk;
+        const int seq = 32 * chunk + (threadIdx.x & 31);
+        mine.nodes = 0;
+        if (seq < p.seqs) mine = tree_request(p, seq);
+        upto = tree_scan(mine.nodes > 0 ? tree_tiles<UNIT>(p, mine) * p.kv_heads : 0);
     }
-    const TreeShape s = tree_shape(p, u, item.request);
-    const int in = unit - before, nth = in / s.tiles;
-    item.tile = in - nth * s.tiles, item.tiles = s.tiles, item.low = s.low;
-    item.head = nth / s.blocks, item.block = nth - item.head * s.blocks;
-    return item;
-}
-
-// Blocks that get units: every one of them at least one, so that each between the first and the last of an item leaves a part of it.
-__device__ __forceinline__ int tree_blocks(int total, int grid) { return min(total, grid); }
-// The first unit of a block: the first total % blocks of them have one more than the others.
-__device__ __forceinline__ int tree_begin(int block, int total, int blocks) {
-    const int per = total / blocks, more = total - per * blocks;
-    return block * per + min(block, more);
-}
-// The block that has a unit.
-__device__ __forceinline__ int tree_owner(int unit, int total, int blocks) {
-    const int per = total / blocks, more = total - per * blocks, at = more * (per + 1);
-    return unit < at ? unit / (per + 1) : more + (unit - at) / per;
-}
-
-// bf16, on mma.sync (tree_attention_mma.cu).
-struct TreeMmaPlan {
-    int unit, rows, blocks;
-    bool fits;  // units are counted in 32 bits
+    // Group `group` of as many as the grid has.
+    __device__ __forceinline__ void begin(const TreeAttention& p, int group, int grid) {
+        total = 0;
+        const int chunks = (p.seqs + 31) / 32;
+        for (int c = 0; c < chunks; ++c) {
+            look_at(p, c);
+            before = total;
+            total += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        groups = min(total, grid);  // (each at least one unit, so that every group between the first and the last of an item leaves a part of it)
+        if (group >= groups) {
+            unit = end = 0;
+            return;
+        }
+        const int per = total / groups, more = total - per * groups;
+        unit = group * per + min(group, more), end = unit + per + (group < more);
+        if (chunks > 1) look_at(p, 0), before = 0;
+    }
+    __device__ __forceinline__ int owner(int u) const {
+        const int per = total / groups, more = total - per * groups, at = more * (per + 1);
+        return u < at ? u / (per + 1) : more + (u - at) / per;
+    }
+    __device__ __forceinline__ bool next(const TreeAttention& p, TreeItem& item, int& first_unit) {
+        if (unit >= end) return false;
+        unsigned here;
+        while (!(here = __ballot_sync(0xffffffffu, unit < before + upto))) {
+            before += __shfl_sync(0xffffffffu, upto, 31);
+            look_at(p, s0 + 1);
+        }
+        const int at = __ffs(here) - 1;
+        item.seq = 32 * s0 + at;
+        item.request.first = __shfl_sync(0xffffffffu, mine.first, at);
+        item.request.nodes = __shfl_sync(0xffffffffu, mine.nodes, at);
+        item.request.start = __shfl_sync(0xffffffffu, mine.start, at);
+        item.request.rows = __shfl_sync(0xffffffffu, mine.rows, at);
+        item.low = tree_low<UNIT>(p, item.request), item.tiles = tree_tiles<UNIT>(p, item.request);
+        const int from = before + (at ? __shfl_sync(0xffffffffu, upto, at - 1) : 0);
+        item.head = (unit - from) / item.tiles;
+        first_unit = from + item.head * item.tiles;
+        item.first = unit - first_unit, item.last = min(item.tiles, end - first_unit);
+        unit = first_unit + item.last;
+        return true;
+    }
 };
-TreeMmaPlan tree_mma_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv);
-int tree_attention_mma(const TreeAttention& p, const TreeMmaPlan& plan, cudaStream_t stream);
+
+// Where a row of a block's part lies: of an item that begins in the group, or of one that began in front of it.
+__device__ __forceinline__ float* tree_part(const TreeAttention& p, int block, bool begins, int rows, int row) {
+    return p.parts + ((size_t)(2 * block + begins) * rows + row) * (p.head_dim + 2);
+}

@@ -3,10 +3,7 @@
 // Query rows are the rows of the MMAs, cached rows their columns, scores and outputs in registers:
 //   S = Q K^T (K read as it lies, columns of the operand), P = 2^(S scale - m) rounded to bf16 (eight bits, as the output has; the sums
 //   take them unrounded), O = O 2^(m_before - m) + P V (V transposed on its way out of shared memory).
-// An item is a block of query rows of a request and kv head; its cached rows are cut into units of UNIT rows.  The units of all items, one
-// behind the other, are dealt out evenly to the blocks of the grid, whatever the requests' lengths: a block works off a run of units, which are segments of
-// one item after the other.  An item that lies in one block is written by it; of others every block leaves its part (at most two of a block), which
-// tree_parts_kernel joins in the order of the units, so that results do not depend on timing.
+// How the work is dealt out: tree_attention.cuh.
 // In a block, WR warps share a tile of 16 WR cached rows, each with 16 MS query rows; NW / WR such groups take the tiles of a unit and have
 // a ring of cp.async copies each.  Few query rows: every warp has its own tiles (WR = 1) and no barrier but at the end; many: the
 // warps share tiles, so that shared memory is read less often.
@@ -55,7 +52,7 @@ __device__ __forceinline__ uint32_t place(int row, int column) {
 }
 
 template <int DP, int MS, int WR, int NW, int ST>
-__global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tree_attention_mma_kernel(const TreeAttention p, const TreeUnits units) {
+__global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tree_attention_mma_kernel(const TreeAttention p, int lanes) {
     using P = Plan<DP, MS, WR, NW, ST>;
     constexpr int KS = DP / 16, SUB = P::TILE < 32 ? P::TILE : 32, NT = SUB / 8, FETCH = P::FETCH;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -68,17 +65,19 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
     unsigned char* q_smem = smem + P::Q_AT;
     pdl_wait();
     pdl_launch_dependents();
-    const int total = tree_total_units(p, units), blocks = tree_blocks(total, gridDim.x);
-    if ((int)blockIdx.x >= blocks) return;
-    const int end = tree_begin(blockIdx.x + 1, total, blocks);
-    for (int unit = tree_begin(blockIdx.x, total, blocks); unit < end;) {
-        const TreeItem item = tree_item(p, units, unit);
+    const int turn = blockIdx.x / lanes, row0 = (blockIdx.x - turn * lanes) * P::ROWS;
+    TreeWalk<P::UNIT> walk;
+    walk.begin(p, turn, gridDim.x / lanes);
+    TreeItem item;
+    for (int unit0; walk.next(p, item, unit0);) {
         const TreeRequest r = item.request;
-        const int head = item.head, row0 = item.block * P::ROWS, count = r.nodes * p.group;
-        const int first = item.tile, last = min(item.tiles, first + (end - unit));  // tiles of UNIT rows
+        const int head = item.head, count = r.nodes * p.group;
+        const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
+        if (first == 0 && row0 == 0 && threadIdx.x == 0)
+            p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
+        if (row0 >= count) continue;
         const int* table = p.tables + (size_t)item.seq * p.width;
-        const int low = item.low;  // tiles of the request in front of its first
         // ---- cached rows on their way
         auto request = [&](int i) {
             const int s = i % ST;
@@ -130,7 +129,7 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
         }
         // (the lines are only looked at where tiles are not seen whole: those of the tree, and with a window)
         if (p.window > 0 || (low + last) * P::UNIT > min(r.start, r.rows))
-            tree_lines(p, r, tree);  // (ends with a barrier)
+            tree_lines<NW * 32>(p, r, tree, [] { __syncthreads(); });  // (ends with a barrier)
         else
             __syncthreads();
         int node[MS][2];
@@ -363,24 +362,23 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
                 } else
                     to[0] = from_float<bf16>(v.x * inv), to[1] = from_float<bf16>(v.y * inv), to[2] = from_float<bf16>(v.z * inv), to[3] = from_float<bf16>(v.w * inv);
             } else {
-                float* to = p.parts + ((size_t)(2 * blockIdx.x + (first == 0)) * P::ROWS + row) * (D + 2);
+                float* to = tree_part(p, blockIdx.x, first == 0, P::ROWS, row);
                 reinterpret_cast<float2*>(to + c)[0] = make_float2(v.x, v.y);
                 reinterpret_cast<float2*>(to + c)[1] = make_float2(v.z, v.w);
                 if (c == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m, l);
             }
         }
         __syncthreads();  // the rings and the query rows may be written again
-        unit += last - first;
     }
 }
 
 template <int DP, int MS, int WR, int NW, int ST>
-int launch(const TreeAttention& p, const TreeUnits& units, int blocks, cudaStream_t stream) {
+int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
     using P = Plan<DP, MS, WR, NW, ST>;
     const auto kernel = tree_attention_mma_kernel<DP, MS, WR, NW, ST>;
     const int rc = ferris_allow_dynamic_smem((const void*)kernel, P::SMEM);
     if (rc != FERRIS_OK) return rc;
-    const cudaError_t e = ferris_launch(kernel, dim3(blocks), dim3(NW * 32), (size_t)P::SMEM, stream, p, units);
+    const cudaError_t e = ferris_launch(kernel, dim3(plan.groups * plan.lanes), dim3(NW * 32), (size_t)P::SMEM, stream, p, plan.lanes);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;
@@ -416,26 +414,29 @@ void with_variant(int D, int rows, F f) {
 
 }  // namespace
 
-TreeMmaPlan tree_mma_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv) {
-    TreeMmaPlan plan = {};
+TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window) {
+    TreePlan plan = {};
+    int blocks = 1;  // of an SM
     with_variant(head_dim, max_nodes * group, [&](auto dp, auto ms, auto wr, auto nw, auto st) {
         using P = Plan<dp.value, ms.value, wr.value, nw.value, st.value>;
-        plan.unit = P::UNIT, plan.rows = P::ROWS;
-        const long long items = (long long)seqs * kv_heads * ((max_nodes * group + P::ROWS - 1) / P::ROWS);
-        const long long most = items * ((max_kv + P::UNIT - 1) / P::UNIT + 1);
-        const int sms = ferris_sm_count();
-        const long long want = (long long)(sms > 0 ? sms : 148) * P::BLOCKS;
-        plan.blocks = (int)(want < most ? want : most);
-        plan.fits = most <= 0x7fffffff;
+        plan.unit = P::UNIT, plan.rows = P::ROWS, blocks = P::BLOCKS;
     });
+    // (the row of a box that lies nowhere is a number too; a scale below nought would turn maxima into minima)
+    plan.tensor = (head_dim == 64 || head_dim == 128) && max_nodes * group > 64 && page_size % 16 == 0 && cache_rows < 0x7fffffff && scale > 0.0f && scale < 1e30f;
+    if (plan.tensor) plan.unit = 128, plan.rows = 128, blocks = 1;
+    const int sms = ferris_sm_count();
+    const long long most = (long long)seqs * kv_heads * ((max_kv + plan.unit - 1) / plan.unit + 1);
+    plan.lanes = (max_nodes * group + plan.rows - 1) / plan.rows;
+    const int want = (sms > 0 ? sms : 148) * blocks / plan.lanes;
+    plan.groups = (int)(want < 1 ? 1 : want < most ? want : most);
+    plan.fits = most <= 0x7fffffff;
     return plan;
 }
 
-int tree_attention_mma(const TreeAttention& p, const TreeMmaPlan& plan, cudaStream_t stream) {
-    const TreeUnits units = {plan.unit, plan.rows};
+int tree_attention_mma(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
     int rc = FERRIS_OK;
     with_variant(p.head_dim, p.max_nodes * p.group, [&](auto dp, auto ms, auto wr, auto nw, auto st) {
-        rc = launch<dp.value, ms.value, wr.value, nw.value, st.value>(p, units, plan.blocks, stream);
+        rc = launch<dp.value, ms.value, wr.value, nw.value, st.value>(p, plan, stream);
     });
     return rc;
 }

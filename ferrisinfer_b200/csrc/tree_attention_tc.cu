@@ -1,0 +1,448 @@
+// Attention for trees of drafted tokens over the paged cache, bf16, on tcgen05: heads of 64 and 128, many query rows (who sees what, and how the work is
+// dealt out: tree_attention.cuh).
+//
+// A block of 128 query rows goes over blocks of 128 cached rows (units):
+//   S = Q K^T   128 x 128 x D, operands in shared memory (Q written once, K by TMA), sums in tensor memory
+//   P = 2^(S scale - m), rounded to bf16 (eight bits, as the output has; sums take it unrounded), into tensor memory over the scores it came from
+//   O = O + P V   P from tensor memory, V as TMA wrote it, sums in tensor memory over all units
+// Two groups of four softmax warps take the units in turn, each with scores, maxima, sums and outputs of its own, so that the tensor core works for one while
+// the other exponentiates; a thread has a row, so that nothing is exchanged.
+// m is the greatest score so far only up to 2^8: outputs are brought to a new m (read, multiplied, written back) where a score exceeds it by
+// more than eight, which after the first units is rare; what is divided by in the end has the same m, so that nothing but the range of the weights changes.
+// A TMA warp streams K and V through a ring of stages, ahead of the segment that is worked on; an MMA warp issues, in the order of the units,
+// P V of a unit and then the scores of the group's next one (the tensor core keeps the order, so that these do not overwrite weights that are still read).
+//
+// Units that every node sees whole are worked off as they are.  In others scores that are not seen become nought weights; as nought times NaN is NaN, the softmax
+// warps then look through the unit's values, set what is not finite to nought and add it, element by element, to the outputs of those who see it.
+#include "tree_attention.cuh"
+
+namespace {
+
+constexpr int ROWS = 128, UNIT = 128, PAGE_ROWS = 16;  // (a TMA box: 16 rows of 64 columns)
+constexpr int SOFTMAX_WARPS = 8, THREADS = (SOFTMAX_WARPS + 2) * 32;
+constexpr int BOX = PAGE_ROWS * 128, ATOM = UNIT * 128;  // bytes of a box; of 64 columns of a unit
+constexpr int SCORES = 0, OUTPUTS = 256, COLUMNS = 512;  // of tensor memory: two groups' scores (128 each), their outputs (D each)
+
+template <int D>
+struct Sizes {
+    static constexpr int ATOMS = D / 64, BLOCK = ATOMS * ATOM, STAGES = D == 128 ? 5 : 8;
+    static constexpr int SMEM = BLOCK * (1 + STAGES) + 1024;
+};
+
+__device__ __forceinline__ float exp2_unit(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ void tensor_memory_take(uint32_t* to, uint32_t columns) { tmem_alloc(to, columns); }
+
+// D[tensor memory] += A[tensor memory] B[shared memory]: A is 128 rows (lanes) of 16 bf16, two to a column.
+__device__ __forceinline__ void tcgen05_mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b_desc), "r"(idesc)
+        : "memory");
+}
+
+// 32 lanes x 32 columns: thread i of the warp writes lane (base lane + i).
+__device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// All softmax warps; those of one group.
+__device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void group_barrier(int g) { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); }
+
+// Stages in the order of their use by the tensor core: K 0, K 1, V 0, K 2, V 1, K 3, ..
+__device__ __forceinline__ int k_place(int i) { return i < 2 ? i : 2 * i - 1; }
+__device__ __forceinline__ int v_place(int i, int n) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; }
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1)
+    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeAttention p, int lanes, int no_row) {
+    using Z = Sizes<D>;
+    constexpr int ST = Z::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ TreeLines tree;
+    __shared__ uint64_t full[ST], empty[ST], q_ready, s_ready[2], p_ready[2], o_done[2];
+    __shared__ uint32_t tensor_base;
+    __shared__ float other_m[ROWS], other_l[ROWS];
+    __shared__ int odd[2];  // how many elements of a unit's values are not finite
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* q_smem = smem;                // [64 columns][128 rows][64] bf16, 128-byte swizzle; at a segment's end, half of a group's outputs
+    uint8_t* kv_smem = smem + Z::BLOCK;    // stages of [64 columns][128 cached rows][64]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        tma_prefetch_descriptor(&map_k);
+        tma_prefetch_descriptor(&map_v);
+        for (int s = 0; s < ST; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        mbar_init(&q_ready, SOFTMAX_WARPS);
+        for (int g = 0; g < 2; ++g) mbar_init(&s_ready[g], 1), mbar_init(&p_ready[g], 4), mbar_init(&o_done[g], 1);
+        mbar_fence_init();
+    }
+    if (warp == SOFTMAX_WARPS + 1) tensor_memory_take(&tensor_base, COLUMNS);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    // (only now: a dependent launch must not take tensor memory that this one waits for)
+    pdl_wait();
+    pdl_launch_dependents();
+    bool dead = false;  // a wait has run out: from then on nobody waits, and the kernel runs on to its end
+    auto wait = [&](uint64_t* bar, int parity, int where) {
+        if (!dead) dead = !mbar_wait(bar, parity, p.status, where);
+    };
+    const int turn = blockIdx.x / lanes, row0 = (blockIdx.x - turn * lanes) * ROWS;
+    TreeWalk<UNIT> walk;
+    walk.begin(p, turn, gridDim.x / lanes);
+    TreeItem item;
+    int unit0;
+    if (warp == SOFTMAX_WARPS) {
+        // ---- K and V on their way: eight lanes, a box of 16 rows each
+        int place0 = 0;
+        while (walk.next(p, item, unit0)) {
+            const TreeRequest r = item.request;
+            if (row0 >= r.nodes * p.group) continue;
+            const int* table = p.tables + (size_t)item.seq * p.width;
+            const int n = item.last - item.first;
+            auto row_of = [&](int i) {  // of a lane's box of unit i; outside the cache where there is none: nought
+                const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS;
+                const int page = lane < UNIT / PAGE_ROWS && i < n && row < r.rows ? tree_page(p, table, row) : -1;
+                if (page < 0) return no_row;
+                const int block = (int)p.page.quotient((uint32_t)row);
+                return (page * p.kv_heads + item.head) * p.page_size + (row - block * p.page_size);
+            };
+            auto load = [&](int place, const CUtensorMap* map, int row) {
+                const int at = place0 + place, s = at % ST;
+                if (at >= ST) wait(&empty[s], (at / ST - 1) & 1, 140);
+                if (lane == 0) mbar_expect_tx(&full[s], Z::BLOCK);
+                __syncwarp();
+                if (lane < UNIT / PAGE_ROWS) {
+#pragma unroll
+                    for (int a = 0; a < Z::ATOMS; ++a) tma_load_2d(kv_smem + (size_t)s * Z::BLOCK + a * ATOM + lane * BOX, map, 64 * a, row, &full[s]);
+                }
+            };
+            int now = row_of(0), then = row_of(1);
+            load(0, &map_k, now);
+            if (n > 1) load(1, &map_k, then);
+            for (int i = 0; i < n; ++i) {
+                const int after = row_of(i + 2);
+                load(v_place(i, n), &map_v, now);
+                if (i + 2 < n) load(k_place(i + 2), &map_k, after);
+                now = then, then = after;
+            }
+            place0 += 2 * n;
+        }
+        // (after a wait that ran out: nothing may still be on its way when the block ends)
+        if (dead)
+            for (int at = max(0, place0 - ST); at < place0; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);
+    } else if (warp == SOFTMAX_WARPS + 1) {
+        // ---- products
+        const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
+        int place0 = 0, segments = 0, done[2] = {0, 0};  // done: units of each group
+        while (walk.next(p, item, unit0)) {
+            if (row0 >= item.request.nodes * p.group) continue;
+            const int n = item.last - item.first;
+            if (lane == 0) {
+                wait(&q_ready, segments & 1, 141);
+                auto scores = [&](int i) {
+                    const int at = place0 + k_place(i), s = at % ST, g = i & 1;
+                    wait(&full[s], (at / ST) & 1, 142);
+                    tcgen05_fence_after();
+                    const uint32_t k_addr = smem_u32(kv_smem + (size_t)s * Z::BLOCK);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint64_t qd = umma_desc_k_major_sw128(smem_u32(q_smem) + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
+                        const uint64_t kd = umma_desc_k_major_sw128(k_addr + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
+                        tcgen05_mma_bf16(tensor_base + SCORES + 128 * g, qd, kd, idesc_qk, k > 0 ? 1u : 0u);
+                    }
+                    tcgen05_commit(&s_ready[g]);
+                    tcgen05_commit(&empty[s]);
+                };
+                for (int i = 0; i < 2 && i < n; ++i) scores(i);
+                for (int i = 0; i < n; ++i) {
+                    const int at = place0 + v_place(i, n), s = at % ST, g = i & 1;
+                    wait(&full[s], (at / ST) & 1, 143);
+                    wait(&p_ready[g], done[g] & 1, 144);
+                    ++done[g];
+                    tcgen05_fence_after();
+                    const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK), ATOM);
+#pragma unroll
+                    for (int k = 0; k < UNIT / 16; ++k)
+                        tcgen05_mma_bf16_ts(tensor_base + OUTPUTS + D * g, tensor_base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
+                    tcgen05_commit(&empty[s]);
+                    if (i + 2 < n)
+                        scores(i + 2);
+                    else
+                        tcgen05_commit(&o_done[g]);
+                }
+            }
+            __syncwarp();
+            place0 += 2 * n, ++segments;
+        }
+    } else {
+        // ---- softmax: group g = warp / 4, a row a thread
+        const int g = warp >> 2, t = threadIdx.x & 127;
+        const uint32_t lanes_at = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t my_scores = tensor_base + SCORES + 128 * g + lanes_at, my_out = tensor_base + OUTPUTS + D * g + lanes_at;
+        const float scale = p.scale;
+        int place0 = 0, done = 0, segments = 0;
+        while (walk.next(p, item, unit0)) {
+            const TreeRequest r = item.request;
+            const int head = item.head, count = r.nodes * p.group, n = item.last - item.first;
+            const bool whole_item = item.first == 0 && item.last == item.tiles;
+            if (item.first == 0 && row0 == 0 && threadIdx.x == 0)
+                p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
+            if (row0 >= count) continue;
+            const int at = row0 + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
+            const int* table = p.tables + (size_t)item.seq * p.width;
+            {
+                // the block's query rows, half of the columns by each group
+                const bf16* src = (const bf16*)p.q + (size_t)(r.first + max(node, 0)) * p.ldq + q_head * D;
+                const bool wide = ((uintptr_t)p.q & 15) == 0 && p.ldq % 8 == 0;
+#pragma unroll
+                for (int c = g * D / 16; c < (g + 1) * D / 16; ++c) {
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (node >= 0) {
+                        if (wide)
+                            v = *reinterpret_cast<const uint4*>(src + 8 * c);
+                        else {
+                            const unsigned short* x = reinterpret_cast<const unsigned short*>(src + 8 * c);
+                            v = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(q_smem + (c >> 3) * ATOM + swizzle128(t, c & 7)) = v;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_ready);
+            }
+            const int sure_low = p.window > 0 ? max(0, r.start + r.nodes - p.window) : 0, sure_high = min(r.start, r.rows);
+            if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<SOFTMAX_WARPS * 32>(p, r, tree, softmax_barrier);
+            {
+                uint32_t nought[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) nought[c] = 0u;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) tmem_store_32x32(my_out + 32 * c, nought);
+                tmem_store_wait();
+            }
+            float m = -INFINITY, l = 0.0f;
+            auto boxes_of = [&](int i) {  // which of the unit's eight boxes have a page
+                const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS;
+                return i < n && lane < UNIT / PAGE_ROWS && row < r.rows && tree_page(p, table, row) >= 0;
+            };
+            bool box = boxes_of(g);
+            for (int i = g; i < n; i += 2) {
+                const uint32_t boxes = __ballot_sync(0xffffffffu, box);
+                box = boxes_of(i + 2);
+                const int key0 = (item.low + item.first + i) * UNIT;
+                const bool whole = key0 >= sure_low && key0 + UNIT <= sure_high && boxes == 0xffu;
+                wait(&s_ready[g], done & 1, 145);
+                ++done;
+                tcgen05_fence_after();
+                // The scores are read twice, 32 at a time, the next ones on their way (128 in registers do not fit beside the rest).
+                uint32_t sees[UNIT / 32];
+                if (!whole) {
+#pragma unroll
+                    for (int c = 0; c < UNIT / 32; ++c) {
+                        sees[c] = node >= 0 ? tree_sees(p, r, tree, node, key0 + 32 * c) : 0u;
+                        if (!(boxes >> (2 * c) & 1)) sees[c] &= 0xffff0000u;
+                        if (!(boxes >> (2 * c + 1) & 1)) sees[c] &= 0xffffu;
+                    }
+                }
+                uint32_t x[2][32];
+                auto scores_of = [&](int c) {  // those of chunk c, as far as they are seen; those of c + 1 requested
+                    tmem_load_wait();
+                    if (c + 1 < UNIT / 32) tmem_load_32x32(my_scores + 32 * (c + 1), x[(c + 1) & 1]);
+                    if (!whole) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(sees[c] >> j & 1)) x[c & 1][j] = 0xff800000u;
+                    }
+                };
+                tmem_load_32x32(my_scores, x[0]);
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < UNIT / 32; ++c) {
+                    scores_of(c);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(x[c & 1][j]));
+                }
+                tmem_load_32x32(my_scores, x[0]);
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;  // (the scale is above nought)
+                const bool up = most > m + 8.0f || (m == -INFINITY && most > m);
+                if (__any_sync(0xffffffffu, up)) {
+                    const float now = up ? most : m, corr = now == -INFINITY ? 1.0f : exp2_unit(m - now);
+                    l *= corr, m = now;
+                    if (i > g) {
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_load_32x32(my_out + 32 * c, o);
+                            tmem_load_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                            tmem_store_32x32(my_out + 32 * c, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t w[UNIT / 2];  // (the weights go where scores of other chunks still stand: only when all have been read)
+#pragma unroll
+                for (int c = 0; c < UNIT / 32; ++c) {
+                    scores_of(c);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float a = exp2_unit(fmaf(__uint_as_float(x[c & 1][2 * j]), scale, -base));
+                        const float b = exp2_unit(fmaf(__uint_as_float(x[c & 1][2 * j + 1]), scale, -base));
+                        sum[j & 3] += a + b;
+                        w[16 * c + j] = pack_bf16(a, b);
+                    }
+                }
+                tmem_store_32x32(my_scores, w);
+                tmem_store_32x32(my_scores + 32, w + 32);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_store_wait();
+                if (!whole) {
+                    // the unit's values: what is not finite becomes nought, and goes to those who see it by itself
+                    const int place = place0 + v_place(i, n), stage = place % ST;
+                    wait(&full[stage], (place / ST) & 1, 146);
+                    uint8_t* v = kv_smem + (size_t)stage * Z::BLOCK;
+                    if (t == 0) odd[g] = 0;
+                    group_barrier(g);
+                    // (a thread: a cached row)
+                    uint32_t any = 0;
+#pragma unroll 4
+                    for (int c = 0; c < D / 8; ++c) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(v + (c >> 3) * ATOM + swizzle128(t, c & 7));
+                        const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) any |= __vcmpeq2(word[k] & 0x7f807f80u, 0x7f807f80u);
+                    }
+                    if (any) atomicAdd(&odd[g], 1);
+                    group_barrier(g);
+                    if (odd[g]) {
+                        // every thread for its query row: what it sees that is not finite (its weight is above nought, whatever it is)
+                        for (int j = 0; j < UNIT; ++j) {
+                            const bool sees = node >= 0 && (boxes >> (j >> 4) & 1) && (tree_sees(p, r, tree, node, key0 + (j & ~31)) >> (j & 31) & 1);
+                            for (int c = 0; c < D; ++c) {
+                                const bf16 x = *reinterpret_cast<const bf16*>(v + (c >> 6) * ATOM + swizzle128(j, (c >> 3) & 7) + 2 * (c & 7));
+                                const float f = __bfloat162float(x);
+                                if (isfinite(f)) continue;  // (the same for all threads)
+                                uint32_t o;
+                                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(my_out + c) : "memory");
+                                tmem_load_wait();
+                                if (sees) o = __float_as_uint(__uint_as_float(o) + f);
+                                asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(my_out + c), "r"(o) : "memory");
+                            }
+                        }
+                        tmem_store_wait();
+                        group_barrier(g);
+                        for (int c = 0; c < D; ++c) {
+                            bf16* x = reinterpret_cast<bf16*>(v + (c >> 6) * ATOM + swizzle128(t, (c >> 3) & 7) + 2 * (c & 7));
+                            if (!isfinite(__bfloat162float(*x))) *x = __float2bfloat16_rn(0.0f);
+                        }
+                        fence_proxy_async();
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[g]);
+            }
+            // ---- the groups joined: the second's outputs through the query rows' memory, half of the columns at a time
+            if (n > g) wait(&o_done[g], segments & 1, 147);
+            tcgen05_fence_after();
+            if (g == 1) other_m[t] = m, other_l[t] = l;
+            softmax_barrier();  // (both groups' products are done: nobody reads the query rows any more)
+            const float m1 = other_m[t], both = fmaxf(m, m1), base = both == -INFINITY ? 0.0f : both;
+            const float f0 = exp2_unit(m - base), f1 = exp2_unit(m1 - base), total = l * f0 + other_l[t] * f1;
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            float* join = reinterpret_cast<float*>(q_smem);  // [column][row]
+            float* part = tree_part(p, blockIdx.x, item.first == 0, ROWS, t);
+            bf16* out = (bf16*)p.out + (size_t)(r.first + max(node, 0)) * p.ldo + q_head * D;
+            const bool wide = ((uintptr_t)p.out & 15) == 0 && p.ldo % 8 == 0;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+                for (int c = 0; c < D / 64 && g == 1; ++c) {
+                    uint32_t o[32];
+                    tmem_load_32x32(my_out + h * D / 2 + 32 * c, o);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) join[(32 * c + j) * ROWS + t] = __uint_as_float(o[j]);
+                }
+                softmax_barrier();
+#pragma unroll 1
+                for (int c = 0; c < D / 64 && g == 0; ++c) {
+                    uint32_t o[32];
+                    tmem_load_32x32(my_out + h * D / 2 + 32 * c, o);
+                    tmem_load_wait();
+                    const int col = h * D / 2 + 32 * c;
+                    if (node < 0) continue;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[j + k]) * f0 + join[(32 * c + j + k) * ROWS + t] * f1;
+                        if (!whole_item) {
+#pragma unroll
+                            for (int k = 0; k < 8; k += 2) *reinterpret_cast<float2*>(part + col + j + k) = make_float2(v[k], v[k + 1]);
+                        } else if (wide) {
+                            *reinterpret_cast<uint4*>(out + col + j) = make_uint4(pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv),
+                                                                                   pack_bf16(v[4] * inv, v[5] * inv), pack_bf16(v[6] * inv, v[7] * inv));
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) out[col + j + k] = from_float<bf16>(v[k] * inv);
+                        }
+                    }
+                }
+                softmax_barrier();
+            }
+            if (!whole_item && g == 0 && node >= 0) *reinterpret_cast<float2*>(part + D) = make_float2(both, total);
+            place0 += 2 * n;
+            // (a phase of o_done passes in every segment in which the group has units, q_ready's in every segment)
+            if (n > g) ++segments;
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == SOFTMAX_WARPS + 1) {
+        tcgen05_fence_after();
+        tmem_dealloc(tensor_base, COLUMNS);
+    }
+}
+
+template <int D>
+int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
+    const uint64_t rows = (uint64_t)p.pages * p.kv_heads * p.page_size;
+    CUtensorMap map_k, map_v;
+    int rc = ferris_make_tensor_map_2d(&map_k, p.k_cache, rows, D, D, PAGE_ROWS, 64);
+    if (rc == FERRIS_OK) rc = ferris_make_tensor_map_2d(&map_v, p.v_cache, rows, D, D, PAGE_ROWS, 64);
+    if (rc == FERRIS_OK) rc = ferris_allow_dynamic_smem((const void*)tree_attention_tc_kernel<D>, Sizes<D>::SMEM);
+    if (rc != FERRIS_OK) return rc;
+    const cudaError_t e = ferris_launch(tree_attention_tc_kernel<D>, dim3(plan.groups * plan.lanes), dim3(THREADS), (size_t)Sizes<D>::SMEM, stream, map_k, map_v, p,
+                                        plan.lanes, (int)rows);
+    if (e != cudaSuccess) {
+        ferris_set_error("%s", cudaGetErrorString(e));
+        return (int)e;
+    }
+    return FERRIS_OK;
+}
+
+}  // namespace
+
+int tree_attention_tc(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
+    return p.head_dim == 64 ? launch<64>(p, plan, stream) : launch<128>(p, plan, stream);
+}

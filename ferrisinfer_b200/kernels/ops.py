@@ -53,7 +53,7 @@ _SIGNATURES = {
     "ferris_packed_cache_evict": [_VP],
     "ferris_packed_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
     "ferris_packed_attention": [_VP],
-    "ferris_tree_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _VP],
+    "ferris_tree_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _VP],
     "ferris_tree_attention": [_VP],
     "ferris_sampling_probs": [_VP, _LL, _VP, _LL, _I, _I, _VP, _VP, _VP, _VP],
     "ferris_verify_tree": [_VP],
@@ -2748,7 +2748,8 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     if workspace is None:
         raise KernelError(f"{what}: a workspace is needed")
     dt = _DT[dtype]
-    splits, scratch, launches = _tree_attention_plan(dt, D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, dev)
+    splits, scratch, launches = _tree_attention_plan(dt, D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, page_size, pages * hkv * page_size, scale,
+                                                     min(window, 0x7fffffff), dev)
     if T == 1:
         ldq, ldo = max(ldq, cols), max(ldo, cols)
     try:
@@ -2762,10 +2763,10 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
 
 
 @functools.lru_cache(maxsize=4096)
-def _tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, device: int) -> tuple:
+def _tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, page_size, cache_rows, scale, window, device: int) -> tuple:
     """Parts of a request's rows, floats of scratch and launches of a step of these sizes on a GPU."""
     needs = (_LL * 3)()
-    _lib().ferris_tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, needs)
+    _lib().ferris_tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, page_size, cache_rows, scale, window, needs)
     return tuple(needs)
 
 

@@ -185,46 +185,63 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeAttention p) {
     }
 }
 
-// The parts that the groups of a bf16 step's blocks left of items that lie in several, a warp a (token, head).
-template <int COLUMNS>  // pairs of columns of a lane
-__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes) {
+// The parts that the groups of a bf16 step's blocks left of items that lie in several: a block joins 32 query rows of an item, and as many columns.  A lane
+// is a row, as the parts lie; the warps have four columns each, and eight parts of them on their way at once.
+constexpr int JOIN_GROUPS = 256;  // parts whose factors are held at once
+
+__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes, int row_blocks) {
+    __shared__ float top[8][32], total[8][32], tile[32][33], factor[JOIN_GROUPS][32];
     pdl_wait();
     pdl_launch_dependents();
-    const int D = p.head_dim, lane = threadIdx.x & 31, seq = blockIdx.y;
-    const TreeRequest r = tree_request(p, seq);
-    const int at = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (at >= r.nodes * p.heads) return;
-    const int node = at / p.heads, q_head = at - node * p.heads, head = q_head / p.group, row = node * p.group + q_head - head * p.group;
-    const int2 span = p.spans[seq * p.kv_heads + head];
-    if (span.x == span.y) return;  // written by the block that has it
-    const int block = row / rows, in = row - block * rows;
-    auto part = [&](int g) { return tree_part(p, g * lanes + block, g == span.x, rows, in); };
+    const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.y / row_blocks, row0 = (blockIdx.y - head * row_blocks) * min(rows, 32), col0 = blockIdx.x * 32, seq = blockIdx.z;
+    const int4 span = p.spans[seq * p.kv_heads + head];
+    const int count = span.z * p.group, parts = span.y - span.x + 1;
+    if (row0 >= count || parts <= 1) return;  // (one part: written by the block that has it)
+    const int block = row0 / rows, in = row0 - block * rows + lane;  // (blocks have 16 rows or a multiple of 32)
+    const bool live = row0 + lane < count && in < rows;
+    auto part = [&](int k) { return tree_part(p, (span.x + k) * lanes + block, k == 0, rows) + in; };
     float m = -INFINITY;
-    for (int g = span.x + lane; g <= span.y; g += 32) m = fmaxf(m, part(g)[D]);
-    m = warp_max(m);
+    if (live)
+        for (int k = warp; k < parts; k += 8) m = fmaxf(m, part(k)[D * rows]);
+    top[warp][lane] = m;
+    __syncthreads();
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, top[w][lane]);
     const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    float2 o[COLUMNS];
+    float l = 0.0f, o[4] = {};
+    for (int k0 = 0; k0 < parts; k0 += JOIN_GROUPS) {
+        const int n = min(parts - k0, JOIN_GROUPS);
+        if (k0) __syncthreads();
+        for (int k = warp; k < n; k += 8) {
+            const float f = live ? exp2f(part(k0 + k)[D * rows] - base) : 0.0f;
+            factor[k][lane] = f;
+            if (live) l = fmaf(f, part(k0 + k)[(D + 1) * rows], l);
+        }
+        __syncthreads();
+        if (live)
+#pragma unroll 8
+            for (int k = 0; k < n; ++k) {
+                const float f = factor[k][lane];
+                const float* x = part(k0 + k);
 #pragma unroll
-    for (int c = 0; c < COLUMNS; ++c) o[c] = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-    for (int g = span.x; g <= span.y; ++g) {
-        const float* x = part(g);
-        const float2 ml = *reinterpret_cast<const float2*>(x + D);
-        const float f = exp2f(ml.x - base);
-        l = fmaf(f, ml.y, l);
-#pragma unroll
-        for (int c = 0; c < COLUMNS; ++c)
-            if (c * 64 + 2 * lane < D) {
-                const float2 v = *reinterpret_cast<const float2*>(x + c * 64 + 2 * lane);
-                o[c].x = fmaf(f, v.x, o[c].x), o[c].y = fmaf(f, v.y, o[c].y);
+                for (int c = 0; c < 4; ++c)
+                    if (col0 + warp * 4 + c < D) o[c] = fmaf(f, x[(col0 + warp * 4 + c) * rows], o[c]);
             }
     }
+    total[warp][lane] = l;
+    __syncthreads();
+    l = 0.0f;
+    for (int w = 0; w < 8; ++w) l += total[w][lane];
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    bf16* out = (bf16*)p.out + (size_t)(r.first + node) * p.ldo + q_head * D;
 #pragma unroll
-    for (int c = 0; c < COLUMNS; ++c)
-        if (c * 64 + 2 * lane < D) out[c * 64 + 2 * lane] = from_float<bf16>(o[c].x * inv), out[c * 64 + 2 * lane + 1] = from_float<bf16>(o[c].y * inv);
+    for (int c = 0; c < 4; ++c) tile[warp * 4 + c][lane] = o[c] * inv;
+    __syncthreads();
+    // a warp: a row's columns
+    for (int row = warp; row < 32 && row0 + row < count && in - lane + row < rows; row += 8) {
+        const int at = row0 + row;
+        if (col0 + lane < D)
+            ((bf16*)p.out)[(size_t)(span.w + at / p.group) * p.ldo + (head * p.group + at % p.group) * D + col0 + lane] = from_float<bf16>(tile[lane][row]);
+    }
 }
 
 int launch(const TreeAttention& p, cudaStream_t stream) {
@@ -304,12 +321,14 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
                                         (long long)a->pages * a->kv_heads * a->page_size, a->scale, a->window);
         if (!plan.fits) FERRIS_REFUSE("%d requests of up to %d rows exceed one launch", a->seqs, p.limit);
         p.parts = (float*)const_cast<void*>(a->parts);
-        p.spans = (int2*)(p.parts + 2ll * plan.groups * plan.lanes * plan.rows * (p.head_dim + 2));
+        // (the parts are a multiple of four floats: 2 x rows, which is a multiple of 16)
+        p.spans = (int4*)(p.parts + 2ll * plan.groups * plan.lanes * plan.rows * (p.head_dim + 2));
         const int rc = plan.tensor ? tree_attention_tc(p, plan, (cudaStream_t)a->stream) : tree_attention_mma(p, plan, (cudaStream_t)a->stream);
         if (rc != FERRIS_OK) return rc;
-        const dim3 grid((p.max_nodes * p.heads + 7) / 8, p.seqs);
-        const auto kernel = p.head_dim <= 64 ? tree_parts_kernel<1> : p.head_dim <= 128 ? tree_parts_kernel<2> : tree_parts_kernel<4>;
-        const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, (cudaStream_t)a->stream, p, plan.rows, plan.lanes);
+        const int at_once = plan.rows < 32 ? plan.rows : 32;  // rows of a block of query rows that a block joins
+        const int row_blocks = (p.max_nodes * p.group + at_once - 1) / at_once;
+        const dim3 grid((p.head_dim + 31) / 32, row_blocks * p.kv_heads, p.seqs);
+        const cudaError_t e = ferris_launch(tree_parts_kernel, grid, dim3(256), 0, (cudaStream_t)a->stream, p, plan.rows, plan.lanes, row_blocks);
         if (e != cudaSuccess) {
             ferris_set_error("%s", cudaGetErrorString(e));
             return (int)e;

@@ -32,9 +32,9 @@ struct TreeAttention {
     int seqs, tokens, heads, kv_heads, group, head_dim, pages, page_size, max_nodes, window;
     float scale;  // of the scores, times log2(e)
     DivideBy page;  // the page size
-    float* parts;  // of D + 2 numbers a query row: unnormalised output, maximum (to the base of 2) and sum
+    float* parts;
     int splits;
-    int2* spans;  // first and last group of every request and kv head
+    int4* spans;  // of every request and kv head: first and last group, nodes, their first row in q and out
     int* status;
 };
 
@@ -134,7 +134,7 @@ struct TreePlan {
     bool tensor;      // on tcgen05 (tree_attention_tc.cu), otherwise on mma.sync (tree_attention_mma.cu)
     bool fits;        // units are counted in 32 bits
     long long floats(int seqs, int kv_heads, int head_dim) const {  // of scratch: parts, and behind them the items' groups
-        return 2ll * groups * lanes * rows * (head_dim + 2) + 2ll * seqs * kv_heads;
+        return 2ll * groups * lanes * rows * (head_dim + 2) + 4ll * seqs * kv_heads;
     }
 };
 TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window);
@@ -226,7 +226,8 @@ struct TreeWalk {
     }
 };
 
-// Where a row of a block's part lies: of an item that begins in the group, or of one that began in front of it.
-__device__ __forceinline__ float* tree_part(const TreeAttention& p, int block, bool begins, int rows, int row) {
-    return p.parts + ((size_t)(2 * block + begins) * rows + row) * (p.head_dim + 2);
+// Where a block's part lies: of an item that begins in the group, or of one that began in front of it.  Column c of row r at [c][r]: D columns of the
+// unnormalised output, the maximum (to the base of 2), the sum.
+__device__ __forceinline__ float* tree_part(const TreeAttention& p, int block, bool begins, int rows) {
+    return p.parts + (size_t)(2 * block + begins) * rows * (p.head_dim + 2);
 }

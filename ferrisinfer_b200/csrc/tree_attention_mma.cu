@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
         const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
         if (first == 0 && row0 == 0 && threadIdx.x == 0)
-            p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
+            p.spans[item.seq * p.kv_heads + head] = make_int4(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1), r.nodes, r.first);
         if (row0 >= count) continue;
         const int* table = p.tables + (size_t)item.seq * p.width;
         // ---- cached rows on their way
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
         constexpr int QUADS = DP / 4;
         const bool pairs = ((uintptr_t)p.out & 3) == 0 && p.ldo % 2 == 0;
         for (int i = threadIdx.x; i < P::ROWS * QUADS; i += NW * 32) {
-            const int row = i / QUADS, c = i % QUADS * 4, at = row0 + row;
+            const int row = i % P::ROWS, c = i / P::ROWS * 4, at = row0 + row;
             if (at >= count || c >= D) continue;
             const int w = row / (16 * MS), in = row % (16 * MS);  // the warps group * WR + w have it
             float m = -INFINITY, l = 0.0f;
@@ -362,10 +362,9 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
                 } else
                     to[0] = from_float<bf16>(v.x * inv), to[1] = from_float<bf16>(v.y * inv), to[2] = from_float<bf16>(v.z * inv), to[3] = from_float<bf16>(v.w * inv);
             } else {
-                float* to = tree_part(p, blockIdx.x, first == 0, P::ROWS, row);
-                reinterpret_cast<float2*>(to + c)[0] = make_float2(v.x, v.y);
-                reinterpret_cast<float2*>(to + c)[1] = make_float2(v.z, v.w);
-                if (c == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m, l);
+                float* to = tree_part(p, blockIdx.x, first == 0, P::ROWS) + row;
+                to[c * P::ROWS] = v.x, to[(c + 1) * P::ROWS] = v.y, to[(c + 2) * P::ROWS] = v.z, to[(c + 3) * P::ROWS] = v.w;
+                if (c == 0) to[D * P::ROWS] = m, to[(D + 1) * P::ROWS] = l;
             }
         }
         __syncthreads();  // the rings and the query rows may be written again

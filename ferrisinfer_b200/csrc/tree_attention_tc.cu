@@ -19,7 +19,11 @@
 namespace {
 
 constexpr int ROWS = 128, UNIT = 128, PAGE_ROWS = 16;  // (a TMA box: 16 rows of 64 columns)
-constexpr int SOFTMAX_WARPS = 8, THREADS = (SOFTMAX_WARPS + 2) * 32;
+constexpr int SOFTMAX_WARPS = 8, THREADS = (SOFTMAX_WARPS + 4) * 32;  // + a TMA warp, an MMA warp and two without work: whole warpgroups share out registers
+// Registers of a thread: the block is launched with LAUNCH_REGISTERS for each (what 384 threads of an SM can have), of which the third warpgroup gives some to
+// the softmax's two; what these take must not be more than that, or they would wait for ever.
+constexpr int LAUNCH_REGISTERS = 168, SOFTMAX_REGISTERS = 208, OTHER_REGISTERS = 80;
+static_assert(2 * SOFTMAX_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "registers");
 constexpr int BOX = PAGE_ROWS * 128, ATOM = UNIT * 128;  // bytes of a box; of 64 columns of a unit
 constexpr int SCORES = 0, OUTPUTS = 256, COLUMNS = 512;  // of tensor memory: two groups' scores (128 each), their outputs (D each)
 
@@ -58,7 +62,38 @@ __device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t*
         "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_store_32x16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+// 128 columns of a lane.
+__device__ __forceinline__ void tmem_load_row(uint32_t taddr, uint32_t (&r)[128]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_load_32x32(taddr + 32 * c, reinterpret_cast<uint32_t(&)[32]>(r[32 * c]));
+}
+// Two fp32 at once.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) { return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int W>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[W]) {
+    if constexpr (W == 32)
+        tmem_load_32x32(taddr, r);
+    else
+        tmem_load_32x16(taddr, r);
+}
 
 // All softmax warps; those of one group.
 __device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -77,7 +112,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __shared__ TreeLines tree;
     __shared__ uint64_t full[ST], empty[ST], q_ready, s_ready[2], p_ready[2], o_done[2];
     __shared__ uint32_t tensor_base;
-    __shared__ float other_m[ROWS], other_l[ROWS];
+    __shared__ float row_m[2][ROWS], row_l[2][ROWS];
     __shared__ int odd[2];  // how many elements of a unit's values are not finite
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* q_smem = smem;                // [64 columns][128 rows][64] bf16, 128-byte swizzle; at a segment's end, half of a group's outputs
@@ -107,90 +142,94 @@ __global__ void __launch_bounds__(THREADS, 1)
     walk.begin(p, turn, gridDim.x / lanes);
     TreeItem item;
     int unit0;
-    if (warp == SOFTMAX_WARPS) {
-        // ---- K and V on their way: eight lanes, a box of 16 rows each
-        int place0 = 0;
-        while (walk.next(p, item, unit0)) {
-            const TreeRequest r = item.request;
-            if (row0 >= r.nodes * p.group) continue;
-            const int* table = p.tables + (size_t)item.seq * p.width;
-            const int n = item.last - item.first;
-            auto row_of = [&](int i) {  // of a lane's box of unit i; outside the cache where there is none: nought
-                const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS;
-                const int page = lane < UNIT / PAGE_ROWS && i < n && row < r.rows ? tree_page(p, table, row) : -1;
-                if (page < 0) return no_row;
-                const int block = (int)p.page.quotient((uint32_t)row);
-                return (page * p.kv_heads + item.head) * p.page_size + (row - block * p.page_size);
-            };
-            auto load = [&](int place, const CUtensorMap* map, int row) {
-                const int at = place0 + place, s = at % ST;
-                if (at >= ST) wait(&empty[s], (at / ST - 1) & 1, 140);
-                if (lane == 0) mbar_expect_tx(&full[s], Z::BLOCK);
-                __syncwarp();
-                if (lane < UNIT / PAGE_ROWS) {
-#pragma unroll
-                    for (int a = 0; a < Z::ATOMS; ++a) tma_load_2d(kv_smem + (size_t)s * Z::BLOCK + a * ATOM + lane * BOX, map, 64 * a, row, &full[s]);
-                }
-            };
-            int now = row_of(0), then = row_of(1);
-            load(0, &map_k, now);
-            if (n > 1) load(1, &map_k, then);
-            for (int i = 0; i < n; ++i) {
-                const int after = row_of(i + 2);
-                load(v_place(i, n), &map_v, now);
-                if (i + 2 < n) load(k_place(i + 2), &map_k, after);
-                now = then, then = after;
-            }
-            place0 += 2 * n;
-        }
-        // (after a wait that ran out: nothing may still be on its way when the block ends)
-        if (dead)
-            for (int at = max(0, place0 - ST); at < place0; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);
-    } else if (warp == SOFTMAX_WARPS + 1) {
-        // ---- products
-        const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
-        int place0 = 0, segments = 0, done[2] = {0, 0};  // done: units of each group
-        while (walk.next(p, item, unit0)) {
-            if (row0 >= item.request.nodes * p.group) continue;
-            const int n = item.last - item.first;
-            if (lane == 0) {
-                wait(&q_ready, segments & 1, 141);
-                auto scores = [&](int i) {
-                    const int at = place0 + k_place(i), s = at % ST, g = i & 1;
-                    wait(&full[s], (at / ST) & 1, 142);
-                    tcgen05_fence_after();
-                    const uint32_t k_addr = smem_u32(kv_smem + (size_t)s * Z::BLOCK);
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t qd = umma_desc_k_major_sw128(smem_u32(q_smem) + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
-                        const uint64_t kd = umma_desc_k_major_sw128(k_addr + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
-                        tcgen05_mma_bf16(tensor_base + SCORES + 128 * g, qd, kd, idesc_qk, k > 0 ? 1u : 0u);
-                    }
-                    tcgen05_commit(&s_ready[g]);
-                    tcgen05_commit(&empty[s]);
+    if (warp >= SOFTMAX_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
+        if (warp == SOFTMAX_WARPS) {
+            // ---- K and V on their way: eight lanes, a box of 16 rows each
+            int place0 = 0;
+            while (walk.next(p, item, unit0)) {
+                const TreeRequest r = item.request;
+                if (row0 >= r.nodes * p.group) continue;
+                const int* table = p.tables + (size_t)item.seq * p.width;
+                const int n = item.last - item.first;
+                auto row_of = [&](int i) {  // of a lane's box of unit i; outside the cache where there is none: nought
+                    const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS;
+                    const int page = lane < UNIT / PAGE_ROWS && i < n && row < r.rows ? tree_page(p, table, row) : -1;
+                    if (page < 0) return no_row;
+                    const int block = (int)p.page.quotient((uint32_t)row);
+                    return (page * p.kv_heads + item.head) * p.page_size + (row - block * p.page_size);
                 };
-                for (int i = 0; i < 2 && i < n; ++i) scores(i);
+                auto load = [&](int place, const CUtensorMap* map, int row) {
+                    const int at = place0 + place, s = at % ST;
+                    if (at >= ST) wait(&empty[s], (at / ST - 1) & 1, 140);
+                    if (lane == 0) mbar_expect_tx(&full[s], Z::BLOCK);
+                    __syncwarp();
+                    if (lane < UNIT / PAGE_ROWS) {
+    #pragma unroll
+                        for (int a = 0; a < Z::ATOMS; ++a) tma_load_2d(kv_smem + (size_t)s * Z::BLOCK + a * ATOM + lane * BOX, map, 64 * a, row, &full[s]);
+                    }
+                };
+                int now = row_of(0), then = row_of(1);
+                load(0, &map_k, now);
+                if (n > 1) load(1, &map_k, then);
                 for (int i = 0; i < n; ++i) {
-                    const int at = place0 + v_place(i, n), s = at % ST, g = i & 1;
-                    wait(&full[s], (at / ST) & 1, 143);
-                    wait(&p_ready[g], done[g] & 1, 144);
-                    ++done[g];
-                    tcgen05_fence_after();
-                    const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK), ATOM);
-#pragma unroll
-                    for (int k = 0; k < UNIT / 16; ++k)
-                        tcgen05_mma_bf16_ts(tensor_base + OUTPUTS + D * g, tensor_base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
-                    tcgen05_commit(&empty[s]);
-                    if (i + 2 < n)
-                        scores(i + 2);
-                    else
-                        tcgen05_commit(&o_done[g]);
+                    const int after = row_of(i + 2);
+                    load(v_place(i, n), &map_v, now);
+                    if (i + 2 < n) load(k_place(i + 2), &map_k, after);
+                    now = then, then = after;
                 }
+                place0 += 2 * n;
             }
-            __syncwarp();
-            place0 += 2 * n, ++segments;
+            // (after a wait that ran out: nothing may still be on its way when the block ends)
+            if (dead)
+                for (int at = max(0, place0 - ST); at < place0; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);
+        } else if (warp == SOFTMAX_WARPS + 1) {
+            // ---- products
+            const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
+            int place0 = 0, segments = 0, done[2] = {0, 0};  // done: units of each group
+            while (walk.next(p, item, unit0)) {
+                if (row0 >= item.request.nodes * p.group) continue;
+                const int n = item.last - item.first;
+                if (lane == 0) {
+                    wait(&q_ready, segments & 1, 141);
+                    auto scores = [&](int i) {
+                        const int at = place0 + k_place(i), s = at % ST, g = i & 1;
+                        wait(&full[s], (at / ST) & 1, 142);
+                        tcgen05_fence_after();
+                        const uint32_t k_addr = smem_u32(kv_smem + (size_t)s * Z::BLOCK);
+    #pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint64_t qd = umma_desc_k_major_sw128(smem_u32(q_smem) + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
+                            const uint64_t kd = umma_desc_k_major_sw128(k_addr + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
+                            tcgen05_mma_bf16(tensor_base + SCORES + 128 * g, qd, kd, idesc_qk, k > 0 ? 1u : 0u);
+                        }
+                        tcgen05_commit(&s_ready[g]);
+                        tcgen05_commit(&empty[s]);
+                    };
+                    for (int i = 0; i < 2 && i < n; ++i) scores(i);
+                    for (int i = 0; i < n; ++i) {
+                        const int at = place0 + v_place(i, n), s = at % ST, g = i & 1;
+                        wait(&full[s], (at / ST) & 1, 143);
+                        wait(&p_ready[g], done[g] & 1, 144);
+                        ++done[g];
+                        tcgen05_fence_after();
+                        const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK), ATOM);
+    #pragma unroll
+                        for (int k = 0; k < UNIT / 16; ++k)
+                            tcgen05_mma_bf16_ts(tensor_base + OUTPUTS + D * g, tensor_base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
+                        tcgen05_commit(&empty[s]);
+                        if (i + 2 < n)
+                            scores(i + 2);
+                        else
+                            tcgen05_commit(&o_done[g]);
+                    }
+                }
+                __syncwarp();
+                place0 += 2 * n, ++segments;
+            }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGISTERS));
         // ---- softmax: group g = warp / 4, a row a thread
         const int g = warp >> 2, t = threadIdx.x & 127;
         const uint32_t lanes_at = (uint32_t)((warp & 3) * 32) << 16;
@@ -201,8 +240,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             const TreeRequest r = item.request;
             const int head = item.head, count = r.nodes * p.group, n = item.last - item.first;
             const bool whole_item = item.first == 0 && item.last == item.tiles;
-            if (item.first == 0 && row0 == 0 && threadIdx.x == 0)
-                p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
             if (row0 >= count) continue;
             const int at = row0 + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
             const int* table = p.tables + (size_t)item.seq * p.width;
@@ -227,6 +264,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_ready);
             }
+            if (item.first == 0 && row0 == 0 && threadIdx.x == 0)
+                p.spans[item.seq * p.kv_heads + head] = make_int4(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1), r.nodes, r.first);
             const int sure_low = p.window > 0 ? max(0, r.start + r.nodes - p.window) : 0, sure_high = min(r.start, r.rows);
             if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<SOFTMAX_WARPS * 32>(p, r, tree, softmax_barrier);
             {
@@ -251,35 +290,23 @@ __global__ void __launch_bounds__(THREADS, 1)
                 wait(&s_ready[g], done & 1, 145);
                 ++done;
                 tcgen05_fence_after();
-                // The scores are read twice, 32 at a time, the next ones on their way (128 in registers do not fit beside the rest).
-                uint32_t sees[UNIT / 32];
+                uint32_t s[UNIT];
+                tmem_load_row(my_scores, s);
+                tmem_load_wait();
                 if (!whole) {
 #pragma unroll
                     for (int c = 0; c < UNIT / 32; ++c) {
-                        sees[c] = node >= 0 ? tree_sees(p, r, tree, node, key0 + 32 * c) : 0u;
-                        if (!(boxes >> (2 * c) & 1)) sees[c] &= 0xffff0000u;
-                        if (!(boxes >> (2 * c + 1) & 1)) sees[c] &= 0xffffu;
-                    }
-                }
-                uint32_t x[2][32];
-                auto scores_of = [&](int c) {  // those of chunk c, as far as they are seen; those of c + 1 requested
-                    tmem_load_wait();
-                    if (c + 1 < UNIT / 32) tmem_load_32x32(my_scores + 32 * (c + 1), x[(c + 1) & 1]);
-                    if (!whole) {
+                        uint32_t sees = node >= 0 ? tree_sees(p, r, tree, node, key0 + 32 * c) : 0u;
+                        if (!(boxes >> (2 * c) & 1)) sees &= 0xffff0000u;
+                        if (!(boxes >> (2 * c + 1) & 1)) sees &= 0xffffu;
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (!(sees[c] >> j & 1)) x[c & 1][j] = 0xff800000u;
+                            if (!(sees >> j & 1)) s[32 * c + j] = 0xff800000u;
                     }
-                };
-                tmem_load_32x32(my_scores, x[0]);
+                }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < UNIT / 32; ++c) {
-                    scores_of(c);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(x[c & 1][j]));
-                }
-                tmem_load_32x32(my_scores, x[0]);
+                for (int j = 0; j < UNIT; j += 2) top[j >> 1 & 3] = fmaxf(fmaxf(top[j >> 1 & 3], __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
                 const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;  // (the scale is above nought)
                 const bool up = most > m + 8.0f || (m == -INFINITY && most > m);
                 if (__any_sync(0xffffffffu, up)) {
@@ -287,33 +314,34 @@ __global__ void __launch_bounds__(THREADS, 1)
                     l *= corr, m = now;
                     if (i > g) {
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_load_32x32(my_out + 32 * c, o);
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_load_32x16(my_out + 16 * c, o);
                             tmem_load_wait();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                            tmem_store_32x32(my_out + 32 * c, o);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                            tmem_store_32x16(my_out + 16 * c, o);
                         }
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t w[UNIT / 2];  // (the weights go where scores of other chunks still stand: only when all have been read)
+                const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < UNIT / 32; ++c) {
-                    scores_of(c);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const float a = exp2_unit(fmaf(__uint_as_float(x[c & 1][2 * j]), scale, -base));
-                        const float b = exp2_unit(fmaf(__uint_as_float(x[c & 1][2 * j + 1]), scale, -base));
-                        sum[j & 3] += a + b;
-                        w[16 * c + j] = pack_bf16(a, b);
+                        const uint64_t x = fma_pair((uint64_t)s[32 * c + 2 * j + 1] << 32 | s[32 * c + 2 * j], scale2, base2);
+                        const float a = exp2_unit(__uint_as_float((uint32_t)x)), b = exp2_unit(__uint_as_float((uint32_t)(x >> 32)));
+                        sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
+                        s[16 * c + j] = pack_bf16(a, b);
                     }
+                    tmem_store_32x16(my_scores + 16 * c, s + 16 * c);
                 }
-                tmem_store_32x32(my_scores, w);
-                tmem_store_32x32(my_scores + 32, w + 32);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                {
+                    const uint64_t both = add_pair(sum[0], sum[1]);
+                    l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
+                }
                 tmem_store_wait();
                 if (!whole) {
                     // the unit's values: what is not finite becomes nought, and goes to those who see it by itself
@@ -361,56 +389,54 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[g]);
             }
-            // ---- the groups joined: the second's outputs through the query rows' memory, half of the columns at a time
+            // ---- the groups joined through the query rows' memory, each for half of the columns, in two rounds
             if (n > g) wait(&o_done[g], segments & 1, 147);
             tcgen05_fence_after();
-            if (g == 1) other_m[t] = m, other_l[t] = l;
+            row_m[g][t] = m, row_l[g][t] = l;
             softmax_barrier();  // (both groups' products are done: nobody reads the query rows any more)
-            const float m1 = other_m[t], both = fmaxf(m, m1), base = both == -INFINITY ? 0.0f : both;
-            const float f0 = exp2_unit(m - base), f1 = exp2_unit(m1 - base), total = l * f0 + other_l[t] * f1;
+            const float m1 = row_m[g ^ 1][t], both = fmaxf(m, m1), base = both == -INFINITY ? 0.0f : both;
+            const float f0 = exp2_unit(m - base), f1 = exp2_unit(m1 - base), total = l * f0 + row_l[g ^ 1][t] * f1;
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            float* join = reinterpret_cast<float*>(q_smem);  // [column][row]
-            float* part = tree_part(p, blockIdx.x, item.first == 0, ROWS, t);
+            constexpr int W = D / 4;  // columns of a round
+            float* mine = reinterpret_cast<float*>(q_smem) + g * W * ROWS + t;            // [column][row]: what the other group needs
+            const float* others = reinterpret_cast<const float*>(q_smem) + (g ^ 1) * W * ROWS + t;
+            float* part = tree_part(p, blockIdx.x, item.first == 0, ROWS) + t;
             bf16* out = (bf16*)p.out + (size_t)(r.first + max(node, 0)) * p.ldo + q_head * D;
             const bool wide = ((uintptr_t)p.out & 15) == 0 && p.ldo % 8 == 0;
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
-#pragma unroll 1
-                for (int c = 0; c < D / 64 && g == 1; ++c) {
-                    uint32_t o[32];
-                    tmem_load_32x32(my_out + h * D / 2 + 32 * c, o);
-                    tmem_load_wait();
+                uint32_t o[W];
+                tmem_load<W>(my_out + (g ^ 1) * 2 * W + h * W, o);
+                tmem_load_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) join[(32 * c + j) * ROWS + t] = __uint_as_float(o[j]);
-                }
+                for (int j = 0; j < W; ++j) mine[j * ROWS] = __uint_as_float(o[j]);
+                const int col = g * 2 * W + h * W;
+                tmem_load<W>(my_out + col, o);
                 softmax_barrier();
-#pragma unroll 1
-                for (int c = 0; c < D / 64 && g == 0; ++c) {
-                    uint32_t o[32];
-                    tmem_load_32x32(my_out + h * D / 2 + 32 * c, o);
-                    tmem_load_wait();
-                    const int col = h * D / 2 + 32 * c;
-                    if (node < 0) continue;
+                tmem_load_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        float v[8];
+                for (int j = 0; j < W; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f0 + others[j * ROWS] * f1);
+                if (node >= 0) {
+                    if (!whole_item) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[j + k]) * f0 + join[(32 * c + j + k) * ROWS + t] * f1;
-                        if (!whole_item) {
+                        for (int j = 0; j < W; ++j) part[(col + j) * ROWS] = __uint_as_float(o[j]);
+                    } else {
 #pragma unroll
-                            for (int k = 0; k < 8; k += 2) *reinterpret_cast<float2*>(part + col + j + k) = make_float2(v[k], v[k + 1]);
-                        } else if (wide) {
-                            *reinterpret_cast<uint4*>(out + col + j) = make_uint4(pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv),
-                                                                                   pack_bf16(v[4] * inv, v[5] * inv), pack_bf16(v[6] * inv, v[7] * inv));
-                        } else {
+                        for (int j = 0; j < W; j += 8) {
+                            float v[8];
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) out[col + j + k] = from_float<bf16>(v[k] * inv);
+                            for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[j + k]) * inv;
+                            if (wide)
+                                *reinterpret_cast<uint4*>(out + col + j) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+                            else
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) out[col + j + k] = from_float<bf16>(v[k]);
                         }
                     }
                 }
                 softmax_barrier();
             }
-            if (!whole_item && g == 0 && node >= 0) *reinterpret_cast<float2*>(part + D) = make_float2(both, total);
+            if (!whole_item && g == 0 && node >= 0) part[D * ROWS] = both, part[(D + 1) * ROWS] = total;
             place0 += 2 * n;
             // (a phase of o_done passes in every segment in which the group has units, q_ready's in every segment)
             if (n > g) ++segments;
@@ -432,6 +458,11 @@ int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
     if (rc == FERRIS_OK) rc = ferris_make_tensor_map_2d(&map_v, p.v_cache, rows, D, D, PAGE_ROWS, 64);
     if (rc == FERRIS_OK) rc = ferris_allow_dynamic_smem((const void*)tree_attention_tc_kernel<D>, Sizes<D>::SMEM);
     if (rc != FERRIS_OK) return rc;
+    static const int registers = [] {
+        cudaFuncAttributes f = {};
+        return cudaFuncGetAttributes(&f, tree_attention_tc_kernel<D>) == cudaSuccess ? f.numRegs : 0;
+    }();
+    if (registers < LAUNCH_REGISTERS) FERRIS_REFUSE("a kernel of %d registers a thread, %d are needed", registers, LAUNCH_REGISTERS);
     const cudaError_t e = ferris_launch(tree_attention_tc_kernel<D>, dim3(plan.groups * plan.lanes), dim3(THREADS), (size_t)Sizes<D>::SMEM, stream, map_k, map_v, p,
                                         plan.lanes, (int)rows);
     if (e != cudaSuccess) {

@@ -203,7 +203,12 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
     auto part = [&](int k) { return tree_part(p, (span.x + k) * lanes + block, k == 0, rows) + in; };
     float m = -INFINITY;
     if (live)
-        for (int k = warp; k < parts; k += 8) m = fmaxf(m, part(k)[D * rows]);
+        for (int k = warp; k < parts; k += 32) {  // (four at a time on their way)
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = k + 8 * u < parts ? part(k + 8 * u)[D * rows] : -INFINITY;
+            m = fmaxf(fmaxf(m, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+        }
     top[warp][lane] = m;
     __syncthreads();
     for (int w = 0; w < 8; ++w) m = fmaxf(m, top[w][lane]);
@@ -212,20 +217,38 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
     for (int k0 = 0; k0 < parts; k0 += JOIN_GROUPS) {
         const int n = min(parts - k0, JOIN_GROUPS);
         if (k0) __syncthreads();
-        for (int k = warp; k < n; k += 8) {
-            const float f = live ? exp2f(part(k0 + k)[D * rows] - base) : 0.0f;
-            factor[k][lane] = f;
-            if (live) l = fmaf(f, part(k0 + k)[(D + 1) * rows], l);
+        for (int k = warp; k < n; k += 32) {
+            float x[4] = {}, y[4] = {};
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (live && k + 8 * u < n) x[u] = part(k0 + k + 8 * u)[D * rows], y[u] = part(k0 + k + 8 * u)[(D + 1) * rows];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k + 8 * u < n) {
+                    const float f = exp2f(x[u] - base);
+                    factor[k + 8 * u][lane] = f;
+                    l = fmaf(f, y[u], l);
+                }
         }
         __syncthreads();
-        if (live)
-#pragma unroll 8
-            for (int k = 0; k < n; ++k) {
-                const float f = factor[k][lane];
-                const float* x = part(k0 + k);
+        const int col = col0 + warp * 4;
+        if (live && col < D)  // (heads have a multiple of eight columns)
+            for (int k = 0; k < n; k += 8) {
+                float x[8][4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (col0 + warp * 4 + c < D) o[c] = fmaf(f, x[(col0 + warp * 4 + c) * rows], o[c]);
+                for (int u = 0; u < 8; ++u)
+                    if (k + u < n) {
+                        const float* from = part(k0 + k + u) + col * rows;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) x[u][c] = from[c * rows];
+                    }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (k + u < n) {
+                        const float f = factor[k + u][lane];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[c] = fmaf(f, x[u][c], o[c]);
+                    }
             }
     }
     total[warp][lane] = l;

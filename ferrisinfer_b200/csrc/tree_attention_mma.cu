@@ -109,22 +109,24 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
         {
             const bf16* q = (const bf16*)p.q;
             const bool wide = ((uintptr_t)q & 15) == 0 && p.ldq % 8 == 0;
-            constexpr int CH = DP / 8;
-            for (int i = threadIdx.x; i < P::ROWS * CH; i += NW * 32) {
-                const int row = i / CH, column = i % CH, at = row0 + row;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (at < count && column * 8 < D) {
-                    const bf16* src = q + (size_t)(r.first + at / p.group) * p.ldq + (head * p.group + at % p.group) * D + column * 8;
-                    if (wide)
-                        v = *reinterpret_cast<const uint4*>(src);
-                    else {
-                        bf16 x[8];
+            constexpr int CH = DP / 8, EACH = (P::ROWS * CH + NW * 32 - 1) / (NW * 32);
+            uint4 v[EACH];  // (all on their way at once)
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) x[k] = src[k];
-                        v = *reinterpret_cast<const uint4*>(x);
-                    }
+            for (int k = 0; k < EACH; ++k) {
+                const int i = threadIdx.x + k * NW * 32, row = i / CH, column = i % CH, at = row0 + row;
+                v[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (at < count && column * 8 < D && i < P::ROWS * CH) {
+                    const unsigned short* src = (const unsigned short*)(q + (size_t)(r.first + at / p.group) * p.ldq + (head * p.group + at % p.group) * D + column * 8);
+                    if (wide)
+                        v[k] = *reinterpret_cast<const uint4*>(src);
+                    else
+                        v[k] = make_uint4(src[0] | (uint32_t)src[1] << 16, src[2] | (uint32_t)src[3] << 16, src[4] | (uint32_t)src[5] << 16, src[6] | (uint32_t)src[7] << 16);
                 }
-                *reinterpret_cast<uint4*>(q_smem + place<DP>(row, column)) = v;
+            }
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                const int i = threadIdx.x + k * NW * 32;
+                if (i < P::ROWS * CH) *reinterpret_cast<uint4*>(q_smem + place<DP>(i / CH, i % CH)) = v[k];
             }
         }
         // (the lines are only looked at where tiles are not seen whole: those of the tree, and with a window)

@@ -247,18 +247,23 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // the block's query rows, half of the columns by each group
                 const bf16* src = (const bf16*)p.q + (size_t)(r.first + max(node, 0)) * p.ldq + q_head * D;
                 const bool wide = ((uintptr_t)p.q & 15) == 0 && p.ldq % 8 == 0;
+                uint4 v[D / 16];  // (all on their way at once)
 #pragma unroll
-                for (int c = g * D / 16; c < (g + 1) * D / 16; ++c) {
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (node >= 0) {
-                        if (wide)
-                            v = *reinterpret_cast<const uint4*>(src + 8 * c);
-                        else {
-                            const unsigned short* x = reinterpret_cast<const unsigned short*>(src + 8 * c);
-                            v = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
-                        }
+                for (int c = 0; c < D / 16; ++c) v[c] = make_uint4(0u, 0u, 0u, 0u);
+                if (node >= 0 && wide) {
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * (g * D / 16 + c));
+                } else if (node >= 0) {
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        const unsigned short* x = reinterpret_cast<const unsigned short*>(src + 8 * (g * D / 16 + c));
+                        v[c] = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
                     }
-                    *reinterpret_cast<uint4*>(q_smem + (c >> 3) * ATOM + swizzle128(t, c & 7)) = v;
+                }
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    const int column = g * D / 16 + c;
+                    *reinterpret_cast<uint4*>(q_smem + (column >> 3) * ATOM + swizzle128(t, column & 7)) = v[c];
                 }
                 fence_proxy_async();
                 __syncwarp();

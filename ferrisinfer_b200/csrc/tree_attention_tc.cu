@@ -41,13 +41,32 @@ __device__ __forceinline__ float exp2_unit(float x) {
 
 __device__ __forceinline__ void tensor_memory_take(uint32_t* to, uint32_t columns) { tmem_alloc(to, columns); }
 
-// D[tensor memory] += A[tensor memory] B[shared memory]: A is 128 rows (lanes) of 16 bf16, two to a column.
-__device__ __forceinline__ void tcgen05_mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc) {
+// MMAs and commits for a whole warp that has come here together; the lane with `leads` issues.  (In code that one lane runs by itself the compiler brings
+// every operand into the uniform registers by itself: 120 cycles an MMA, whatever its size; a unit of 128 x 128 rows 3,030 cycles, so 1,870.)  Descriptors
+// by their lower halves: the upper ones are the same for all operands of a kind.
+// D[tensor memory] (+)= A[shared memory] B[shared memory]^T
+__device__ __forceinline__ void mma_from_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t accumulate, uint32_t leads) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.eq.b32 p, 0, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b_desc), "r"(idesc)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(accumulate), "r"(leads)
+        : "memory");
+}
+// D[tensor memory] += A[tensor memory] B[shared memory]: A is 128 rows (lanes) of 16 bf16, two to a column.
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t leads) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(leads)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leads) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leads)
         : "memory");
 }
 
@@ -165,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (lane == 0) mbar_expect_tx(&full[s], Z::BLOCK);
                     __syncwarp();
                     if (lane < UNIT / PAGE_ROWS) {
-    #pragma unroll
+#pragma unroll
                         for (int a = 0; a < Z::ATOMS; ++a) tma_load_2d(kv_smem + (size_t)s * Z::BLOCK + a * ATOM + lane * BOX, map, 64 * a, row, &full[s]);
                     }
                 };
@@ -186,43 +205,46 @@ __global__ void __launch_bounds__(THREADS, 1)
         } else if (warp == SOFTMAX_WARPS + 1) {
             // ---- products
             const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
-            int place0 = 0, segments = 0, done[2] = {0, 0};  // done: units of each group
+            const uint32_t leads = lane == 0, base = __shfl_sync(0xffffffffu, tensor_base, 0);
+            int place0 = 0, segments = 0, done0 = 0, done1 = 0;  // done: units of each group
             while (walk.next(p, item, unit0)) {
                 if (row0 >= item.request.nodes * p.group) continue;
                 const int n = item.last - item.first;
-                if (lane == 0) {
-                    wait(&q_ready, segments & 1, 141);
-                    auto scores = [&](int i) {
-                        const int at = place0 + k_place(i), s = at % ST, g = i & 1;
-                        wait(&full[s], (at / ST) & 1, 142);
-                        tcgen05_fence_after();
-                        const uint32_t k_addr = smem_u32(kv_smem + (size_t)s * Z::BLOCK);
-    #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const uint64_t qd = umma_desc_k_major_sw128(smem_u32(q_smem) + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
-                            const uint64_t kd = umma_desc_k_major_sw128(k_addr + (k >> 2) * ATOM) + (uint64_t)(2 * (k & 3));
-                            tcgen05_mma_bf16(tensor_base + SCORES + 128 * g, qd, kd, idesc_qk, k > 0 ? 1u : 0u);
-                        }
-                        tcgen05_commit(&s_ready[g]);
-                        tcgen05_commit(&empty[s]);
-                    };
-                    for (int i = 0; i < 2 && i < n; ++i) scores(i);
-                    for (int i = 0; i < n; ++i) {
-                        const int at = place0 + v_place(i, n), s = at % ST, g = i & 1;
-                        wait(&full[s], (at / ST) & 1, 143);
-                        wait(&p_ready[g], done[g] & 1, 144);
-                        ++done[g];
-                        tcgen05_fence_after();
-                        const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK), ATOM);
-    #pragma unroll
-                        for (int k = 0; k < UNIT / 16; ++k)
-                            tcgen05_mma_bf16_ts(tensor_base + OUTPUTS + D * g, tensor_base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
-                        tcgen05_commit(&empty[s]);
-                        if (i + 2 < n)
-                            scores(i + 2);
-                        else
-                            tcgen05_commit(&o_done[g]);
+                wait(&q_ready, segments & 1, 141);
+                auto scores = [&](int i) {
+                    const int at = place0 + k_place(i), s = at % ST, g = i & 1;
+                    wait(&full[s], (at / ST) & 1, 142);
+                    __syncwarp();
+                    tcgen05_fence_after();
+                    const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem)), k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK));
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t next = (k >> 2) * (ATOM >> 4) + 2 * (k & 3);  // the next 64 columns, 32 bytes along the row
+                        mma_from_smem(base + SCORES + 128 * g, (uint32_t)q_desc + next, (uint32_t)k_desc + next, (uint32_t)(q_desc >> 32), idesc_qk, k > 0, leads);
                     }
+                    commit(&s_ready[g], leads);
+                    commit(&empty[s], leads);
+                };
+                for (int i = 0; i < 2 && i < n; ++i) scores(i);
+                for (int i = 0; i < n; ++i) {
+                    const int at = place0 + v_place(i, n), s = at % ST, g = i & 1;
+                    wait(&full[s], (at / ST) & 1, 143);
+                    wait(&p_ready[g], (g ? done1 : done0) & 1, 144);
+                    if (g)
+                        ++done1;
+                    else
+                        ++done0;
+                    __syncwarp();
+                    tcgen05_fence_after();
+                    const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK), ATOM);
+#pragma unroll
+                    for (int k = 0; k < UNIT / 16; ++k)
+                        mma_from_tmem(base + OUTPUTS + D * g, base + SCORES + 128 * g + 8 * k, (uint32_t)v_desc + k * (BOX >> 4), (uint32_t)(v_desc >> 32), idesc_pv, leads);
+                    commit(&empty[s], leads);
+                    if (i + 2 < n)
+                        scores(i + 2);
+                    else
+                        commit(&o_done[g], leads);
                 }
                 __syncwarp();
                 place0 += 2 * n, ++segments;
@@ -242,6 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool whole_item = item.first == 0 && item.last == item.tiles;
             if (row0 >= count) continue;
             const int at = row0 + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
+            const bool live = row0 + (warp & 3) * 32 < count;  // any of the warp's rows
             const int* table = p.tables + (size_t)item.seq * p.width;
             {
                 // the block's query rows, half of the columns by each group
@@ -295,59 +318,61 @@ __global__ void __launch_bounds__(THREADS, 1)
                 wait(&s_ready[g], done & 1, 145);
                 ++done;
                 tcgen05_fence_after();
-                uint32_t s[UNIT];
-                tmem_load_row(my_scores, s);
-                tmem_load_wait();
-                if (!whole) {
+                if (live) {  // (rows that are not there have nobody's weights)
+                    uint32_t s[UNIT];
+                    tmem_load_row(my_scores, s);
+                    tmem_load_wait();
+                    if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < UNIT / 32; ++c) {
-                        uint32_t sees = node >= 0 ? tree_sees(p, r, tree, node, key0 + 32 * c) : 0u;
-                        if (!(boxes >> (2 * c) & 1)) sees &= 0xffff0000u;
-                        if (!(boxes >> (2 * c + 1) & 1)) sees &= 0xffffu;
+                        for (int c = 0; c < UNIT / 32; ++c) {
+                            uint32_t sees = node >= 0 ? tree_sees(p, r, tree, node, key0 + 32 * c) : 0u;
+                            if (!(boxes >> (2 * c) & 1)) sees &= 0xffff0000u;
+                            if (!(boxes >> (2 * c + 1) & 1)) sees &= 0xffffu;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!(sees >> j & 1)) s[32 * c + j] = 0xff800000u;
-                    }
-                }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < UNIT; j += 2) top[j >> 1 & 3] = fmaxf(fmaxf(top[j >> 1 & 3], __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
-                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;  // (the scale is above nought)
-                const bool up = most > m + 8.0f || (m == -INFINITY && most > m);
-                if (__any_sync(0xffffffffu, up)) {
-                    const float now = up ? most : m, corr = now == -INFINITY ? 1.0f : exp2_unit(m - now);
-                    l *= corr, m = now;
-                    if (i > g) {
-#pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t o[16];
-                            tmem_load_32x16(my_out + 16 * c, o);
-                            tmem_load_wait();
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                            tmem_store_32x16(my_out + 16 * c, o);
+                            for (int j = 0; j < 32; ++j)
+                                if (!(sees >> j & 1)) s[32 * c + j] = 0xff800000u;
                         }
                     }
-                }
-                const float base = m == -INFINITY ? 0.0f : m;
-                const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
-                uint64_t sum[2] = {0, 0};
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < UNIT / 32; ++c) {
+                    for (int j = 0; j < UNIT; j += 2) top[j >> 1 & 3] = fmaxf(fmaxf(top[j >> 1 & 3], __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;  // (the scale is above nought)
+                    const bool up = most > m + 8.0f || (m == -INFINITY && most > m);
+                    if (__any_sync(0xffffffffu, up)) {
+                        const float now = up ? most : m, corr = now == -INFINITY ? 1.0f : exp2_unit(m - now);
+                        l *= corr, m = now;
+                        if (i > g) {
+#pragma unroll 1
+                            for (int c = 0; c < D / 16; ++c) {
+                                uint32_t o[16];
+                                tmem_load_32x16(my_out + 16 * c, o);
+                                tmem_load_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const uint64_t x = fma_pair((uint64_t)s[32 * c + 2 * j + 1] << 32 | s[32 * c + 2 * j], scale2, base2);
-                        const float a = exp2_unit(__uint_as_float((uint32_t)x)), b = exp2_unit(__uint_as_float((uint32_t)(x >> 32)));
-                        sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
-                        s[16 * c + j] = pack_bf16(a, b);
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                                tmem_store_32x16(my_out + 16 * c, o);
+                            }
+                        }
                     }
-                    tmem_store_32x16(my_scores + 16 * c, s + 16 * c);
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+                    uint64_t sum[2] = {0, 0};
+#pragma unroll
+                    for (int c = 0; c < UNIT / 32; ++c) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const uint64_t x = fma_pair((uint64_t)s[32 * c + 2 * j + 1] << 32 | s[32 * c + 2 * j], scale2, base2);
+                            const float a = exp2_unit(__uint_as_float((uint32_t)x)), b = exp2_unit(__uint_as_float((uint32_t)(x >> 32)));
+                            sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
+                            s[16 * c + j] = pack_bf16(a, b);
+                        }
+                        tmem_store_32x16(my_scores + 16 * c, s + 16 * c);
+                    }
+                    {
+                        const uint64_t both = add_pair(sum[0], sum[1]);
+                        l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
+                    }
+                    tmem_store_wait();
                 }
-                {
-                    const uint64_t both = add_pair(sum[0], sum[1]);
-                    l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
-                }
-                tmem_store_wait();
                 if (!whole) {
                     // the unit's values: what is not finite becomes nought, and goes to those who see it by itself
                     const int place = place0 + v_place(i, n), stage = place % ST;

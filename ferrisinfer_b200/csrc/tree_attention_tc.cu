@@ -41,34 +41,23 @@ __device__ __forceinline__ float exp2_unit(float x) {
 
 __device__ __forceinline__ void tensor_memory_take(uint32_t* to, uint32_t columns) { tmem_alloc(to, columns); }
 
-// MMAs and commits for a whole warp that has come here together; the lane with `leads` issues.  (In code that one lane runs by itself the compiler brings
-// every operand into the uniform registers by itself: 120 cycles an MMA, whatever its size; a unit of 128 x 128 rows 3,030 cycles, so 1,870.)  Descriptors
-// by their lower halves: the upper ones are the same for all operands of a kind.
-// D[tensor memory] (+)= A[shared memory] B[shared memory]^T
-__device__ __forceinline__ void mma_from_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t accumulate, uint32_t leads) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
-        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
-        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(accumulate), "r"(leads)
-        : "memory");
-}
 // D[tensor memory] += A[tensor memory] B[shared memory]: A is 128 rows (lanes) of 16 bf16, two to a column.
-__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t leads) {
+__device__ __forceinline__ void tcgen05_mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
-        "setp.eq.b32 p, 0, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "mov.b64 b, {%2, %3};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(leads)
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b_desc), "r"(idesc)
         : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leads) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "setp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leads)
-        : "memory");
+// One lane of a whole warp.  MMAs take their operands from the warp's uniform registers: what they are formed from has to be known to be the same in all
+// lanes (a shuffle from one lane says so), or the compiler brings every operand there by itself.
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
 }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // 32 lanes x 32 columns: thread i of the warp writes lane (base lane + i).
 __device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t* r) {
@@ -205,25 +194,27 @@ __global__ void __launch_bounds__(THREADS, 1)
         } else if (warp == SOFTMAX_WARPS + 1) {
             // ---- products
             const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
-            const uint32_t leads = lane == 0, base = __shfl_sync(0xffffffffu, tensor_base, 0);
+            const uint32_t base = uniform(tensor_base);
             int place0 = 0, segments = 0, done0 = 0, done1 = 0;  // done: units of each group
             while (walk.next(p, item, unit0)) {
                 if (row0 >= item.request.nodes * p.group) continue;
-                const int n = item.last - item.first;
+                const int n = uniform(item.last - item.first);
                 wait(&q_ready, segments & 1, 141);
                 auto scores = [&](int i) {
                     const int at = place0 + k_place(i), s = at % ST, g = i & 1;
                     wait(&full[s], (at / ST) & 1, 142);
-                    __syncwarp();
                     tcgen05_fence_after();
-                    const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem)), k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK));
+                    if (elected()) {
+                        const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem)), k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + s * Z::BLOCK));
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t next = (k >> 2) * (ATOM >> 4) + 2 * (k & 3);  // the next 64 columns, 32 bytes along the row
-                        mma_from_smem(base + SCORES + 128 * g, (uint32_t)q_desc + next, (uint32_t)k_desc + next, (uint32_t)(q_desc >> 32), idesc_qk, k > 0, leads);
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint64_t next = (k >> 2) * (ATOM >> 4) + 2 * (k & 3);  // the next 64 columns, 32 bytes along the row
+                            tcgen05_mma_bf16(base + SCORES + 128 * g, q_desc + next, k_desc + next, idesc_qk, k > 0 ? 1u : 0u);
+                        }
+                        tcgen05_commit(&s_ready[g]);
+                        tcgen05_commit(&empty[s]);
                     }
-                    commit(&s_ready[g], leads);
-                    commit(&empty[s], leads);
+                    __syncwarp();
                 };
                 for (int i = 0; i < 2 && i < n; ++i) scores(i);
                 for (int i = 0; i < n; ++i) {
@@ -234,17 +225,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                         ++done1;
                     else
                         ++done0;
-                    __syncwarp();
                     tcgen05_fence_after();
-                    const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + (size_t)s * Z::BLOCK), ATOM);
+                    if (elected()) {
+                        const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + s * Z::BLOCK), ATOM);
 #pragma unroll
-                    for (int k = 0; k < UNIT / 16; ++k)
-                        mma_from_tmem(base + OUTPUTS + D * g, base + SCORES + 128 * g + 8 * k, (uint32_t)v_desc + k * (BOX >> 4), (uint32_t)(v_desc >> 32), idesc_pv, leads);
-                    commit(&empty[s], leads);
-                    if (i + 2 < n)
-                        scores(i + 2);
-                    else
-                        commit(&o_done[g], leads);
+                        for (int k = 0; k < UNIT / 16; ++k)
+                            tcgen05_mma_bf16_ts(base + OUTPUTS + D * g, base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
+                        tcgen05_commit(&empty[s]);
+                        if (i + 2 >= n) tcgen05_commit(&o_done[g]);
+                    }
+                    __syncwarp();
+                    if (i + 2 < n) scores(i + 2);
                 }
                 __syncwarp();
                 place0 += 2 * n, ++segments;

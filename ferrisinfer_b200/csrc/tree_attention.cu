@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeAttention p) {
 
 // The parts that the groups of a bf16 step's blocks left of items that lie in several: a block joins 32 query rows of an item, and as many columns.  A lane
 // is a row, as the parts lie; the warps have four columns each, and eight parts of them on their way at once.
-constexpr int JOIN_GROUPS = 256;  // parts whose factors are held at once
+constexpr int JOIN_GROUPS = 64;  // parts whose factors are held at once
 
 __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes, int row_blocks) {
     __shared__ float top[8][32], total[8][32], tile[32][33], factor[JOIN_GROUPS][32];

@@ -424,7 +424,7 @@ TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_node
     });
     // (the row of a box that lies nowhere is a number too; a scale below nought would turn maxima into minima)
     plan.tensor = (head_dim == 64 || head_dim == 128) && max_nodes * group > 16 && page_size % 16 == 0 && cache_rows < 0x7fffffff && scale > 0.0f && scale < 1e30f;
-    if (plan.tensor) plan.unit = 128, plan.rows = 128, blocks = 1;
+    if (plan.tensor) plan.unit = 128, plan.rows = max_nodes * group > 128 ? 256 : 128, blocks = 1;
     const int sms = ferris_sm_count();
     const long long most = (long long)seqs * kv_heads * ((max_kv + plan.unit - 1) / plan.unit + 1);
     plan.lanes = (max_nodes * group + plan.rows - 1) / plan.rows;

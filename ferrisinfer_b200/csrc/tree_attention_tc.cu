@@ -5,8 +5,9 @@
 //   S = Q K^T   128 x 128 x D, operands in shared memory (Q written once, K by TMA), sums in tensor memory
 //   P = 2^(S scale - m), rounded to bf16 (eight bits, as the output has; sums take it unrounded), into tensor memory over the scores it came from
 //   O = O + P V   P from tensor memory, V as TMA wrote it, sums in tensor memory over all units
-// Two groups of four softmax warps take the units in turn, each with scores, maxima, sums and outputs of its own, so that the tensor core works for one while
-// the other exponentiates; a thread has a row, so that nothing is exchanged.
+// Two groups of four softmax warps, each with scores, maxima, sums and outputs of its own, so that the tensor core works for one while
+// the other exponentiates: of up to 128 query rows they take the units in turn and are joined at the end, of more (WIDE) each has 128 rows of its own, and K and V are
+// fetched once for both; a thread has a row, so that nothing is exchanged.
 // m is the greatest score so far only up to 2^8: outputs are brought to a new m (read, multiplied, written back) where a score exceeds it by
 // more than eight, which after the first units is rare; what is divided by in the end has the same m, so that nothing but the range of the weights changes.
 // A TMA warp streams K and V through a ring of stages, ahead of the segment that is worked on; an MMA warp issues, in the order of the units,
@@ -27,10 +28,10 @@ static_assert(2 * SOFTMAX_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "
 constexpr int BOX = PAGE_ROWS * 128, ATOM = UNIT * 128;  // bytes of a box; of 64 columns of a unit
 constexpr int SCORES = 0, OUTPUTS = 256, COLUMNS = 512;  // of tensor memory: two groups' scores (128 each), their outputs (D each)
 
-template <int D>
+template <int D, bool WIDE>
 struct Sizes {
-    static constexpr int ATOMS = D / 64, BLOCK = ATOMS * ATOM, STAGES = D == 128 ? 5 : 8;
-    static constexpr int SMEM = BLOCK * (1 + STAGES) + 1024;
+    static constexpr int ATOMS = D / 64, BLOCK = ATOMS * ATOM, TILES = WIDE ? 2 : 1, STAGES = D == 64 ? 8 : WIDE ? 4 : 5;
+    static constexpr int SMEM = BLOCK * (TILES + STAGES) + 1024;
 };
 
 __device__ __forceinline__ float exp2_unit(float x) {
@@ -107,24 +108,26 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[W]) {
 __device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void group_barrier(int g) { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); }
 
-// Stages in the order of their use by the tensor core: K 0, K 1, V 0, K 2, V 1, K 3, ..
-__device__ __forceinline__ int k_place(int i) { return i < 2 ? i : 2 * i - 1; }
-__device__ __forceinline__ int v_place(int i, int n) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; }
+// Stages in the order of their use by the tensor core: K 0, K 1, V 0, K 2, V 1, K 3, ..; where both groups use them, K 0, V 0, K 1, ..
+template <bool WIDE>
+__device__ __forceinline__ int k_place(int i) { return WIDE ? 2 * i : i < 2 ? i : 2 * i - 1; }
+template <bool WIDE>
+__device__ __forceinline__ int v_place(int i, int n) { return WIDE || i + 1 == n ? 2 * i + 1 : 2 * i + 2; }
 
-template <int D>
+template <int D, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 1)
     tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeAttention p, int lanes, int no_row) {
-    using Z = Sizes<D>;
+    using Z = Sizes<D, WIDE>;
     constexpr int ST = Z::STAGES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ TreeLines tree;
     __shared__ uint64_t full[ST], empty[ST], q_ready, s_ready[2], p_ready[2], o_done[2];
     __shared__ uint32_t tensor_base;
-    __shared__ float row_m[2][ROWS], row_l[2][ROWS];
+    __shared__ float row_m[2][ROWS], row_l[2][ROWS];  // (not WIDE)
     __shared__ int odd[2];  // how many elements of a unit's values are not finite
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* q_smem = smem;                // [64 columns][128 rows][64] bf16, 128-byte swizzle; at a segment's end, half of a group's outputs
-    uint8_t* kv_smem = smem + Z::BLOCK;    // stages of [64 columns][128 cached rows][64]
+    uint8_t* kv_smem = smem + Z::TILES * Z::BLOCK;  // stages of [64 columns][128 cached rows][64]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         tma_prefetch_descriptor(&map_k);
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto wait = [&](uint64_t* bar, int parity, int where) {
         if (!dead) dead = !mbar_wait(bar, parity, p.status, where);
     };
-    const int turn = blockIdx.x / lanes, row0 = (blockIdx.x - turn * lanes) * ROWS;
+    const int turn = blockIdx.x / lanes, row0 = (blockIdx.x - turn * lanes) * ROWS * Z::TILES;
     TreeWalk<UNIT> walk;
     walk.begin(p, turn, gridDim.x / lanes);
     TreeItem item;
@@ -160,11 +163,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (row0 >= r.nodes * p.group) continue;
                 const int* table = p.tables + (size_t)item.seq * p.width;
                 const int n = item.last - item.first;
-                auto row_of = [&](int i) {  // of a lane's box of unit i; outside the cache where there is none: nought
-                    const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS;
-                    const int page = lane < UNIT / PAGE_ROWS && i < n && row < r.rows ? tree_page(p, table, row) : -1;
-                    if (page < 0) return no_row;
-                    const int block = (int)p.page.quotient((uint32_t)row);
+                // the page of a lane's box of unit i, on its way; its row of the cache; outside the cache where there is none: nought
+                auto page_of = [&](int i) {
+                    const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS, block = (int)p.page.quotient((uint32_t)row);
+                    return lane < UNIT / PAGE_ROWS && i < n && row < r.rows && block < p.width ? table[block] : -1;
+                };
+                auto row_of = [&](int i, int page) {
+                    if (page >= p.pages) ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 111);
+                    if (page < 0 || page >= p.pages) return no_row;
+                    const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS, block = (int)p.page.quotient((uint32_t)row);
                     return (page * p.kv_heads + item.head) * p.page_size + (row - block * p.page_size);
                 };
                 auto load = [&](int place, const CUtensorMap* map, int row) {
@@ -177,14 +184,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                         for (int a = 0; a < Z::ATOMS; ++a) tma_load_2d(kv_smem + (size_t)s * Z::BLOCK + a * ATOM + lane * BOX, map, 64 * a, row, &full[s]);
                     }
                 };
-                int now = row_of(0), then = row_of(1);
+                int page = page_of(0), next = page_of(1), after = page_of(2);
+                int now = row_of(0, page), then = row_of(1, next);
                 load(0, &map_k, now);
-                if (n > 1) load(1, &map_k, then);
+                if (!WIDE && n > 1) load(1, &map_k, then);
                 for (int i = 0; i < n; ++i) {
-                    const int after = row_of(i + 2);
-                    load(v_place(i, n), &map_v, now);
-                    if (i + 2 < n) load(k_place(i + 2), &map_k, after);
-                    now = then, then = after;
+                    const int last = row_of(i + 2, after);
+                    after = page_of(i + 3);
+                    load(v_place<WIDE>(i, n), &map_v, now);
+                    if (WIDE && i + 1 < n) load(k_place<WIDE>(i + 1), &map_k, then);
+                    if (!WIDE && i + 2 < n) load(k_place<WIDE>(i + 2), &map_k, last);
+                    now = then, then = last;
                 }
                 place0 += 2 * n;
             }
@@ -199,27 +209,28 @@ __global__ void __launch_bounds__(THREADS, 1)
             while (walk.next(p, item, unit0)) {
                 if (row0 >= item.request.nodes * p.group) continue;
                 const int n = uniform(item.last - item.first);
+                const bool two = WIDE && uniform(row0 + ROWS < item.request.nodes * p.group);  // (WIDE: the second group has rows)
                 wait(&q_ready, segments & 1, 141);
-                auto scores = [&](int i) {
-                    const int at = place0 + k_place(i), s = at % ST, g = i & 1;
-                    wait(&full[s], (at / ST) & 1, 142);
+                auto scores = [&](int i, int g) {
+                    const int at = place0 + k_place<WIDE>(i), s = at % ST;
+                    if (!WIDE || g == 0) wait(&full[s], (at / ST) & 1, 142);
                     tcgen05_fence_after();
                     if (elected()) {
-                        const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem)), k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + s * Z::BLOCK));
+                        const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem + (WIDE ? g * Z::BLOCK : 0)));
+                        const uint64_t k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + s * Z::BLOCK));
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k) {
                             const uint64_t next = (k >> 2) * (ATOM >> 4) + 2 * (k & 3);  // the next 64 columns, 32 bytes along the row
                             tcgen05_mma_bf16(base + SCORES + 128 * g, q_desc + next, k_desc + next, idesc_qk, k > 0 ? 1u : 0u);
                         }
                         tcgen05_commit(&s_ready[g]);
-                        tcgen05_commit(&empty[s]);
+                        if (!two || g) tcgen05_commit(&empty[s]);
                     }
                     __syncwarp();
                 };
-                for (int i = 0; i < 2 && i < n; ++i) scores(i);
-                for (int i = 0; i < n; ++i) {
-                    const int at = place0 + v_place(i, n), s = at % ST, g = i & 1;
-                    wait(&full[s], (at / ST) & 1, 143);
+                auto outputs = [&](int i, int g, bool last) {
+                    const int at = place0 + v_place<WIDE>(i, n), s = at % ST;
+                    if (!WIDE || g == 0) wait(&full[s], (at / ST) & 1, 143);
                     wait(&p_ready[g], (g ? done1 : done0) & 1, 144);
                     if (g)
                         ++done1;
@@ -231,11 +242,25 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int k = 0; k < UNIT / 16; ++k)
                             tcgen05_mma_bf16_ts(base + OUTPUTS + D * g, base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
-                        tcgen05_commit(&empty[s]);
-                        if (i + 2 >= n) tcgen05_commit(&o_done[g]);
+                        if (!two || g) tcgen05_commit(&empty[s]);
+                        if (last) tcgen05_commit(&o_done[g]);
                     }
                     __syncwarp();
-                    if (i + 2 < n) scores(i + 2);
+                };
+                if constexpr (WIDE) {
+                    scores(0, 0);
+                    if (two) scores(0, 1);
+                    for (int i = 0; i < n; ++i)
+                        for (int g = 0; g <= two; ++g) {
+                            outputs(i, g, i + 1 == n);
+                            if (i + 1 < n) scores(i + 1, g);
+                        }
+                } else {
+                    for (int i = 0; i < 2 && i < n; ++i) scores(i, i);
+                    for (int i = 0; i < n; ++i) {
+                        outputs(i, i & 1, i + 2 >= n);
+                        if (i + 2 < n) scores(i + 2, i & 1);
+                    }
                 }
                 __syncwarp();
                 place0 += 2 * n, ++segments;
@@ -254,30 +279,36 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int head = item.head, count = r.nodes * p.group, n = item.last - item.first;
             const bool whole_item = item.first == 0 && item.last == item.tiles;
             if (row0 >= count) continue;
-            const int at = row0 + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
-            const bool live = row0 + (warp & 3) * 32 < count;  // any of the warp's rows
+            const int at = row0 + (WIDE ? g * ROWS : 0) + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
+            const bool live = at - lane < count;                                    // any of the warp's rows
+            const int from = WIDE ? 0 : g, step = WIDE ? 1 : 2;                     // the group's units
+            const bool both = !WIDE || row0 + ROWS < count, here = both || g == 0;  // both groups have rows; this one has
+            const int units = here ? n : 0;
             const int* table = p.tables + (size_t)item.seq * p.width;
             {
                 // the block's query rows, half of the columns by each group
                 const bf16* src = (const bf16*)p.q + (size_t)(r.first + max(node, 0)) * p.ldq + q_head * D;
                 const bool wide = ((uintptr_t)p.q & 15) == 0 && p.ldq % 8 == 0;
-                uint4 v[D / 16];  // (all on their way at once)
+                constexpr int EACH = WIDE ? D / 8 : D / 16;  // 16 bytes at a time: a row, or half of one
+                const int first = WIDE ? 0 : g * EACH;
+                uint8_t* to = q_smem + (WIDE ? g * Z::BLOCK : 0);
+                uint4 v[EACH];  // (all on their way at once)
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) v[c] = make_uint4(0u, 0u, 0u, 0u);
+                for (int c = 0; c < EACH; ++c) v[c] = make_uint4(0u, 0u, 0u, 0u);
                 if (node >= 0 && wide) {
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * (g * D / 16 + c));
+                    for (int c = 0; c < EACH; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * (first + c));
                 } else if (node >= 0) {
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        const unsigned short* x = reinterpret_cast<const unsigned short*>(src + 8 * (g * D / 16 + c));
+                    for (int c = 0; c < EACH; ++c) {
+                        const unsigned short* x = reinterpret_cast<const unsigned short*>(src + 8 * (first + c));
                         v[c] = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
                     }
                 }
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    const int column = g * D / 16 + c;
-                    *reinterpret_cast<uint4*>(q_smem + (column >> 3) * ATOM + swizzle128(t, column & 7)) = v[c];
+                for (int c = 0; c < EACH; ++c) {
+                    const int column = first + c;
+                    *reinterpret_cast<uint4*>(to + (column >> 3) * ATOM + swizzle128(t, column & 7)) = v[c];
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -296,14 +327,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tmem_store_wait();
             }
             float m = -INFINITY, l = 0.0f;
-            auto boxes_of = [&](int i) {  // which of the unit's eight boxes have a page
-                const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS;
-                return i < n && lane < UNIT / PAGE_ROWS && row < r.rows && tree_page(p, table, row) >= 0;
+            // the page of a lane's box of a unit's eight, on its way while the unit before is worked on; -1: none
+            auto page_of = [&](int i) {
+                const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS, block = (int)p.page.quotient((uint32_t)row);
+                return i < units && lane < UNIT / PAGE_ROWS && row < r.rows && block < p.width ? table[block] : -1;
             };
-            bool box = boxes_of(g);
-            for (int i = g; i < n; i += 2) {
-                const uint32_t boxes = __ballot_sync(0xffffffffu, box);
-                box = boxes_of(i + 2);
+            int page = page_of(from);
+            for (int i = from; i < units; i += step) {
+                const uint32_t boxes = __ballot_sync(0xffffffffu, page >= 0 && page < p.pages);  // (the TMA warp reports pages that are not there)
+                page = page_of(i + step);
                 const int key0 = (item.low + item.first + i) * UNIT;
                 const bool whole = key0 >= sure_low && key0 + UNIT <= sure_high && boxes == 0xffu;
                 wait(&s_ready[g], done & 1, 145);
@@ -332,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (__any_sync(0xffffffffu, up)) {
                         const float now = up ? most : m, corr = now == -INFINITY ? 1.0f : exp2_unit(m - now);
                         l *= corr, m = now;
-                        if (i > g) {
+                        if (i > from) {
 #pragma unroll 1
                             for (int c = 0; c < D / 16; ++c) {
                                 uint32_t o[16];
@@ -366,23 +398,32 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 if (!whole) {
                     // the unit's values: what is not finite becomes nought, and goes to those who see it by itself
-                    const int place = place0 + v_place(i, n), stage = place % ST;
+                    const int place = place0 + v_place<WIDE>(i, n), stage = place % ST;
                     wait(&full[stage], (place / ST) & 1, 146);
                     uint8_t* v = kv_smem + (size_t)stage * Z::BLOCK;
-                    if (t == 0) odd[g] = 0;
-                    group_barrier(g);
+                    // (units that both groups work on are looked through and changed by the first, with the second beside it)
+                    const bool shared = WIDE && both, mine = !shared || g == 0;
+                    int& found = odd[shared ? 0 : g];
+                    auto barrier = [&] {
+                        if (shared)
+                            softmax_barrier();
+                        else
+                            group_barrier(g);
+                    };
+                    if (t == 0 && mine) found = 0;
+                    barrier();
                     // (a thread: a cached row)
                     uint32_t any = 0;
 #pragma unroll 4
-                    for (int c = 0; c < D / 8; ++c) {
+                    for (int c = 0; c < D / 8 && mine; ++c) {
                         const uint4 x = *reinterpret_cast<const uint4*>(v + (c >> 3) * ATOM + swizzle128(t, c & 7));
                         const uint32_t word[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) any |= __vcmpeq2(word[k] & 0x7f807f80u, 0x7f807f80u);
                     }
-                    if (any) atomicAdd(&odd[g], 1);
-                    group_barrier(g);
-                    if (odd[g]) {
+                    if (any) atomicAdd(&found, 1);
+                    barrier();
+                    if (found) {
                         // every thread for its query row: what it sees that is not finite (its weight is above nought, whatever it is)
                         for (int j = 0; j < UNIT; ++j) {
                             const bool sees = node >= 0 && (boxes >> (j >> 4) & 1) && (tree_sees(p, r, tree, node, key0 + (j & ~31)) >> (j & 31) & 1);
@@ -398,69 +439,97 @@ __global__ void __launch_bounds__(THREADS, 1)
                             }
                         }
                         tmem_store_wait();
-                        group_barrier(g);
-                        for (int c = 0; c < D; ++c) {
+                        barrier();
+                        for (int c = 0; c < D && mine; ++c) {
                             bf16* x = reinterpret_cast<bf16*>(v + (c >> 6) * ATOM + swizzle128(t, (c >> 3) & 7) + 2 * (c & 7));
                             if (!isfinite(__bfloat162float(*x))) *x = __float2bfloat16_rn(0.0f);
                         }
                         fence_proxy_async();
+                        if (shared) barrier();
                     }
                 }
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[g]);
             }
-            // ---- the groups joined through the query rows' memory, each for half of the columns, in two rounds
-            if (n > g) wait(&o_done[g], segments & 1, 147);
+            if (units > from) wait(&o_done[g], segments & 1, 147);
             tcgen05_fence_after();
-            row_m[g][t] = m, row_l[g][t] = l;
-            softmax_barrier();  // (both groups' products are done: nobody reads the query rows any more)
-            const float m1 = row_m[g ^ 1][t], both = fmaxf(m, m1), base = both == -INFINITY ? 0.0f : both;
-            const float f0 = exp2_unit(m - base), f1 = exp2_unit(m1 - base), total = l * f0 + row_l[g ^ 1][t] * f1;
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            constexpr int W = D / 4;  // columns of a round
-            float* mine = reinterpret_cast<float*>(q_smem) + g * W * ROWS + t;            // [column][row]: what the other group needs
-            const float* others = reinterpret_cast<const float*>(q_smem) + (g ^ 1) * W * ROWS + t;
-            float* part = tree_part(p, blockIdx.x, item.first == 0, ROWS) + t;
+            float* part = tree_part(p, blockIdx.x, item.first == 0, ROWS * Z::TILES) + (WIDE ? g * ROWS : 0) + t;
             bf16* out = (bf16*)p.out + (size_t)(r.first + max(node, 0)) * p.ldo + q_head * D;
             const bool wide = ((uintptr_t)p.out & 15) == 0 && p.ldo % 8 == 0;
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                uint32_t o[W];
-                tmem_load<W>(my_out + (g ^ 1) * 2 * W + h * W, o);
-                tmem_load_wait();
+            // columns of this thread's row, to the output (times `inv`) or to the block's part
+            auto leave = [&](auto& o, int col, float inv) {
+                if (node < 0) return;
+                constexpr int W = sizeof(o) / 4;
+                if (!whole_item) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) mine[j * ROWS] = __uint_as_float(o[j]);
-                const int col = g * 2 * W + h * W;
-                tmem_load<W>(my_out + col, o);
-                softmax_barrier();
-                tmem_load_wait();
+                    for (int j = 0; j < W; ++j) part[(col + j) * (ROWS * Z::TILES)] = __uint_as_float(o[j]);
+                } else {
 #pragma unroll
-                for (int j = 0; j < W; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f0 + others[j * ROWS] * f1);
-                if (node >= 0) {
-                    if (!whole_item) {
+                    for (int j = 0; j < W; j += 8) {
+                        float v[8];
 #pragma unroll
-                        for (int j = 0; j < W; ++j) part[(col + j) * ROWS] = __uint_as_float(o[j]);
-                    } else {
+                        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[j + k]) * inv;
+                        if (wide)
+                            *reinterpret_cast<uint4*>(out + col + j) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+                        else
 #pragma unroll
-                        for (int j = 0; j < W; j += 8) {
-                            float v[8];
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[j + k]) * inv;
-                            if (wide)
-                                *reinterpret_cast<uint4*>(out + col + j) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-                            else
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) out[col + j + k] = from_float<bf16>(v[k]);
-                        }
+                            for (int k = 0; k < 8; ++k) out[col + j + k] = from_float<bf16>(v[k]);
                     }
                 }
-                softmax_barrier();
+            };
+            auto leave_sums = [&](float most, float total) {
+                if (!whole_item && node >= 0) part[D * (ROWS * Z::TILES)] = most, part[(D + 1) * (ROWS * Z::TILES)] = total;
+            };
+            if constexpr (WIDE) {
+                // ---- every group its rows
+                if (live && here) {
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_load_32x32(my_out + 32 * c, o);
+                        tmem_load_wait();
+                        leave(o, 32 * c, inv);
+                    }
+                    leave_sums(m, l);
+                }
+                softmax_barrier();  // (the lines of ancestors may be written again)
+            } else {
+                // ---- the groups joined through the query rows' memory, each for half of the columns, in two rounds
+                row_m[g][t] = m, row_l[g][t] = l;
+                softmax_barrier();  // (both groups' products are done: nobody reads the query rows any more)
+                const float m1 = row_m[g ^ 1][t], most = fmaxf(m, m1), base = most == -INFINITY ? 0.0f : most;
+                const float f0 = exp2_unit(m - base), f1 = exp2_unit(m1 - base), total = l * f0 + row_l[g ^ 1][t] * f1;
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                constexpr int W = D / 4;  // columns of a round
+                float* mine = reinterpret_cast<float*>(q_smem) + g * W * ROWS + t;  // [column][row]: what the other group needs
+                const float* others = reinterpret_cast<const float*>(q_smem) + (g ^ 1) * W * ROWS + t;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t o[W];
+                    const int col = g * 2 * W + h * W;
+                    if (live) {
+                        tmem_load<W>(my_out + (g ^ 1) * 2 * W + h * W, o);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int j = 0; j < W; ++j) mine[j * ROWS] = __uint_as_float(o[j]);
+                        tmem_load<W>(my_out + col, o);
+                    }
+                    softmax_barrier();
+                    if (live) {
+                        tmem_load_wait();
+#pragma unroll
+                        for (int j = 0; j < W; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f0 + others[j * ROWS] * f1);
+                        leave(o, col, inv);
+                    }
+                    softmax_barrier();
+                }
+                if (g == 0) leave_sums(most, total);
             }
-            if (!whole_item && g == 0 && node >= 0) part[D * ROWS] = both, part[(D + 1) * ROWS] = total;
             place0 += 2 * n;
             // (a phase of o_done passes in every segment in which the group has units, q_ready's in every segment)
-            if (n > g) ++segments;
+            if (units > from) ++segments;
         }
     }
     tcgen05_fence_before();
@@ -471,20 +540,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
 }
 
-template <int D>
+template <int D, bool WIDE>
 int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
     const uint64_t rows = (uint64_t)p.pages * p.kv_heads * p.page_size;
     CUtensorMap map_k, map_v;
     int rc = ferris_make_tensor_map_2d(&map_k, p.k_cache, rows, D, D, PAGE_ROWS, 64);
     if (rc == FERRIS_OK) rc = ferris_make_tensor_map_2d(&map_v, p.v_cache, rows, D, D, PAGE_ROWS, 64);
-    if (rc == FERRIS_OK) rc = ferris_allow_dynamic_smem((const void*)tree_attention_tc_kernel<D>, Sizes<D>::SMEM);
+    if (rc == FERRIS_OK) rc = ferris_allow_dynamic_smem((const void*)tree_attention_tc_kernel<D, WIDE>, Sizes<D, WIDE>::SMEM);
     if (rc != FERRIS_OK) return rc;
     static const int registers = [] {
         cudaFuncAttributes f = {};
-        return cudaFuncGetAttributes(&f, tree_attention_tc_kernel<D>) == cudaSuccess ? f.numRegs : 0;
+        return cudaFuncGetAttributes(&f, tree_attention_tc_kernel<D, WIDE>) == cudaSuccess ? f.numRegs : 0;
     }();
     if (registers < LAUNCH_REGISTERS) FERRIS_REFUSE("a kernel of %d registers a thread, %d are needed", registers, LAUNCH_REGISTERS);
-    const cudaError_t e = ferris_launch(tree_attention_tc_kernel<D>, dim3(plan.groups * plan.lanes), dim3(THREADS), (size_t)Sizes<D>::SMEM, stream, map_k, map_v, p,
+    const cudaError_t e = ferris_launch(tree_attention_tc_kernel<D, WIDE>, dim3(plan.groups * plan.lanes), dim3(THREADS), (size_t)Sizes<D, WIDE>::SMEM, stream, map_k, map_v, p,
                                         plan.lanes, (int)rows);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
@@ -496,5 +565,6 @@ int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
 }  // namespace
 
 int tree_attention_tc(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
-    return p.head_dim == 64 ? launch<64>(p, plan, stream) : launch<128>(p, plan, stream);
+    if (p.head_dim == 64) return plan.rows > ROWS ? launch<64, true>(p, plan, stream) : launch<64, false>(p, plan, stream);
+    return plan.rows > ROWS ? launch<128, true>(p, plan, stream) : launch<128, false>(p, plan, stream);
 }

@@ -8,10 +8,14 @@
 // Which tokens stay is decided on masses in 64 bits: w is computed in 64 bits and held as a whole number of 2^-45, so that sums are exact
 // and do not depend on the order of additions, and borders fall as they do in exact arithmetic up to 2^-45 of the greatest weight.
 //
-// A cluster of eight blocks takes a row; each keeps its eighth in shared memory where it fits.  Rows without top-k and top-p are a softmax: the maximum, the sum, the quotients.  Otherwise
-// a histogram of 1,024 bins, linear in the logit, finds the bin in which the top_k-th token, or the mass, falls (each block adds up an
-// eighth of the bins of all blocks); the elements of that bin (with top_k <= 512 all from it upward) are gathered, at most 512, and ordered by counting for
-// each what lies before it.  A bin of more elements is cut up by the digits of its elements' keys until one has no more than that.
+// A cluster of up to eight blocks takes a row; each keeps its share in shared memory where it fits (two blocks to an SM), so that a row is read once and written once.
+//   neither top-k nor top-p   a softmax in 32 bits: the maximum, the exponentials and their sum, the quotients
+//   top_k <= 512              the top_k-th of the threads' own maxima bounds the top_k-th logit from below, and few logits lie above it: a histogram of the maxima
+//                             (one a thread), the logits from the bin of the top_k-th on gathered, ordered by counting for each what lies before it
+//   top-p alone               masses above seven bounds (each thread's in registers) say between which two the border lies; a histogram of what lies there,
+//                             linear in the logit, in which bin; the bin's elements are gathered and ordered in the same way
+//   otherwise                 a histogram of the whole row
+// A bin of more than 512 elements is cut up by the digits of its elements' keys until one has no more.
 #include <float.h>
 #include <math.h>
 
@@ -23,11 +27,14 @@ namespace {
 typedef unsigned long long u64;
 typedef unsigned int u32;
 
-constexpr int CLUSTER = 8, THREADS = 512, WARPS = THREADS / 32;
-constexpr int BINS = 1024, OWN_BINS = BINS / CLUSTER;
+constexpr int MOST_BLOCKS = 8, THREADS = 512, WARPS = THREADS / 32;
+constexpr int BINS = 1024, OWN_BINS = 256;  // a block adds up BINS / blocks of the row's bins: at most a quarter
+constexpr int LEAST_BLOCKS = BINS / OWN_BINS;
 constexpr int LIST = 512;    // elements that are ordered by counting
 constexpr int DIGIT = 10;    // bits of a digit of the keys: a histogram's bins
+constexpr int BOUNDS = 7;
 constexpr double UNIT = 35184372088832.0;  // 2^45
+constexpr double LOG2E = 1.4426950408889634;
 
 __device__ __forceinline__ u64 ld_peer_shared_u64(const void* at, u32 rank) {
     u32 remote;
@@ -41,6 +48,11 @@ __device__ __forceinline__ u32 ld_peer_shared_u32(const void* at, u32 rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(at)), "r"(rank));
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
     return v;
+}
+__device__ __forceinline__ u32 cluster_blocks() {
+    u32 n;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
 }
 
 struct SamplingProbs {
@@ -64,50 +76,84 @@ struct Entry {
 };
 
 struct Shared {
-    u32 count[BINS];   // this block's histogram
-    u64 mass[BINS];
-    u32 own_count[OWN_BINS];  // the row's, of this block's eighth of the bins
+    union {
+        struct {
+            u32 count[BINS];  // this block's histogram
+            u64 mass[BINS];
+        };
+        Entry list[LIST];  // this block's elements of a bin, when the histograms have been added up
+    };
+    Entry all[LIST];  // the row's
+    u32 own_count[OWN_BINS];  // the row's, of this block's bins
     u64 own_mass[OWN_BINS];
     u64 total_count, total_mass;  // of these
     Found found;
-    u64 best;          // the block's greatest key
-    float least, sum;  // its least finite logit, its part of the softmax's sum
-    u64 kept_mass;
+    float value[4];    // what blocks tell each other, each place once
+    u64 above[BOUNDS + 1];  // masses above the bounds, and of all
+    u32 index;
     u32 listed;
-    Entry list[LIST];  // this block's
-    Entry all[LIST];   // the row's
-    u64 threshold, retained;
+    u64 threshold, retained, kept_mass;
     u64 red[WARPS];
     float fred[33];
 };
 
 // Ordered as the logits are, the lower index first among equals.
-__device__ __forceinline__ u64 key_of(float l, int i) {
-    const u32 u = __float_as_uint(l == 0.0f ? 0.0f : l);  // (both noughts are one)
-    return (u64)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (u32)~(u32)i;
+__device__ __forceinline__ u32 order_of(float l) {
+    const u32 u = __float_as_uint(l + 0.0f);  // (both noughts are one)
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float number(float l) { return l != l ? -INFINITY : l; }
+__device__ __forceinline__ float logit_of(u32 order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
+__device__ __forceinline__ u64 key_of(float l, int i) { return (u64)order_of(l) << 32 | (u32)~(u32)i; }
+// Of a NaN minus infinity.
+__device__ __forceinline__ float number(float l) { return fmaxf(l, -INFINITY); }
+
+// 2^y for y <= 0 up to 2^-46 of itself (nought below 2^-60): the nearest whole number apart, and the Taylor polynomial of 2^f for |f| <= 1/2, whose
+// twelfth term is 6e-15.
+__device__ __forceinline__ double exp2_64(double y) {
+    const double magic = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to a whole number
+    const double t = fmax(y, -1000.0) + magic, f = fmax(y, -1000.0) - (t - magic);
+    double r = 4.44553827187081e-10;  // ln(2)^k / k! for k = 11 .. 0
+    r = fma(r, f, 7.054911620801121e-09);
+    r = fma(r, f, 1.0178086009239696e-07);
+    r = fma(r, f, 1.3215486790144305e-06);
+    r = fma(r, f, 1.5252733804059838e-05);
+    r = fma(r, f, 0.00015403530393381606);
+    r = fma(r, f, 0.0013333558146428441);
+    r = fma(r, f, 0.009618129107628477);
+    r = fma(r, f, 0.055504108664821576);
+    r = fma(r, f, 0.2402265069591007);
+    r = fma(r, f, 0.6931471805599453);
+    r = fma(r, f, 1.0);
+    const int n = __double2loint(t);
+    return n < -60 ? 0.0 : __hiloint2double(__double2hiint(r) + n * (1 << 20), __double2loint(r));
+}
 
 struct Row {
     const float* at;  // this block's elements: shared memory, or the row itself
     int lo, n;        // the first one's index, their number
-    float top, T, bins_per;
+    float top, high, bins_per;  // the greatest logit; where the linear histogram begins
+    double rate;      // log2(e) / T
 
     __device__ __forceinline__ float logit(int i) const { return number(at[i]); }
-    __device__ __forceinline__ double weight(float l) const {
-        return l == top ? 1.0 : exp(((double)l - (double)top) / (double)T);
-    }
-    __device__ __forceinline__ u64 mass(float l) const { return (u64)__double2ull_rn(weight(l) * UNIT); }
+    __device__ __forceinline__ double weight(float l) const { return l == top ? 1.0 : exp2_64(((double)l - (double)top) * rate); }
+    // (adding 2^52 rounds to a whole number, which is then the lower bits)
+    __device__ __forceinline__ u64 mass(float l) const { return (u64)__double_as_longlong(fma(weight(l), UNIT, 4503599627370496.0)) & 0xfffffffffffffull; }
     // The greatest logits in the highest bin; what lies below the histogram's range in bin 0.
     __device__ __forceinline__ int bin(float l) const {
-        const float x = l == top ? 0.0f : (top - l) * bins_per;
+        const float x = l >= high ? 0.0f : (high - l) * bins_per;
         return BINS - 1 - (int)fminf(x, (float)(BINS - 1));
     }
 };
 
-__device__ __forceinline__ u64 block_sum_u64(Shared& s, u64 v) {
+// Sums over the block and over the row's blocks, for all threads; the one ends behind a barrier of the block, the others want the values
+// to be there (a barrier of the cluster in between).
+__device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ u64 block_sum_u64(Shared& s, u64 v) {
+    v = warp_sum_u64(v);
     if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = v;
     __syncthreads();
     u64 t = 0;
@@ -115,9 +161,27 @@ __device__ __forceinline__ u64 block_sum_u64(Shared& s, u64 v) {
     __syncthreads();
     return t;
 }
+__device__ __forceinline__ u64 row_sum_u64(const u64* at) {
+    const u32 lane = threadIdx.x & 31;
+    return warp_sum_u64(lane < cluster_blocks() ? ld_peer_shared_u64(at, lane) : 0);
+}
+__device__ __forceinline__ float row_value(const float* at, float none) {
+    const u32 lane = threadIdx.x & 31;
+    return lane < cluster_blocks() ? __uint_as_float(ld_peer_shared_u32(at, lane)) : none;
+}
+__device__ __forceinline__ float block_max(Shared& s, float v) {
+    v = warp_max(v);
+    if ((threadIdx.x & 31) == 0) s.fred[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = s.fred[0];
+    for (int w = 1; w < WARPS; ++w) v = fmaxf(v, s.fred[w]);
+    __syncthreads();
+    return v;
+}
 
-// Which elements a search goes through: those of a bin of the linear histogram whose keys begin with some digits.
+// Which elements a search goes through: those between two logits, of a bin of the linear histogram, whose keys begin with some digits.
 struct Subset {
+    float low = -INFINITY, high = INFINITY;  // low < l <= high (or all that is at least minus infinity)
     int bin = -1;  // -1: all
     u64 prefix = 0;
     int digits = 0;  // of the prefix
@@ -126,83 +190,91 @@ struct Subset {
         const int s = shift(digit);
         return (int)((s >= 0 ? key >> s : key << -s) & (BINS - 1));
     }
-    __device__ __forceinline__ bool holds(const Row& r, float l, u64 key) const {
-        if (bin >= 0 && r.bin(l) != bin) return false;
-        return digits == 0 || (key >> shift(digits - 1)) == (prefix >> shift(digits - 1));
+    __device__ __forceinline__ bool between(float l) const { return l <= high && (l > low || low == -INFINITY); }
+    __device__ __forceinline__ bool holds(const Row& r, float l, int i) const {
+        if (!between(l) || (bin >= 0 && r.bin(l) != bin)) return false;
+        return digits == 0 || (key_of(l, i) >> shift(digits - 1)) == (prefix >> shift(digits - 1));
     }
 };
 
-// The histogram of a subset (linear for all elements, by the next digit of their keys for others) over the whole row: every block is
-// left with its eighth of the bins, and with its sums.  Ends behind a barrier of the cluster.
+// The histogram of a block adds up to the row's: every block is left with its share of the bins, and with its sums.  Ends behind a barrier of the cluster.
 template <bool MASS>
-__device__ void histogram(Shared& s, const Row& r, const Subset& in) {
-    for (int b = threadIdx.x; b < BINS; b += THREADS) {
-        s.count[b] = 0;
-        if (MASS) s.mass[b] = 0;
-    }
-    __syncthreads();
-    u32 low = 0;  // what falls into bin 0 of the linear histogram, mostly far below all others: added up first
-    u64 low_mass = 0;
-    for (int i = threadIdx.x; i < r.n; i += THREADS) {
-        const float l = r.logit(i);
-        int b;
-        if (in.bin < 0)
-            b = r.bin(l);
-        else {
-            const u64 key = key_of(l, r.lo + i);
-            if (!in.holds(r, l, key)) continue;
-            b = Subset::value(key, in.digits);
-        }
-        const u64 m = MASS ? r.mass(l) : 0;
-        if (in.bin < 0 && b == 0)
-            ++low, low_mass += m;
-        else {
-            atomicAdd(&s.count[b], 1u);
-            if (MASS) atomicAdd(&s.mass[b], m);
-        }
-    }
-    if (low) {
-        atomicAdd(&s.count[0], low);
-        if (MASS) atomicAdd(&s.mass[0], low_mass);
-    }
+__device__ void add_up(Shared& s) {
     cluster_sync();
-    const u32 rank = cluster_ctarank();
+    const u32 rank = cluster_ctarank(), blocks = cluster_blocks();
+    const int first = rank * BINS / blocks, own = (rank + 1) * BINS / blocks - first;
     u64 c = 0, m = 0;
-    if (threadIdx.x < OWN_BINS) {
-        const int b = rank * OWN_BINS + threadIdx.x;
-        for (int k = 0; k < CLUSTER; ++k) {
-            c += ld_peer_shared_u32(&s.count[b], k);
-            if (MASS) m += ld_peer_shared_u64(&s.mass[b], k);
+    if ((int)threadIdx.x < own) {
+        const int b = first + threadIdx.x;
+        u32 cc[MOST_BLOCKS];
+        u64 mm[MOST_BLOCKS];
+#pragma unroll
+        for (int k = 0; k < MOST_BLOCKS; ++k) {
+            cc[k] = k < (int)blocks ? ld_peer_shared_u32(&s.count[b], k) : 0;
+            mm[k] = MASS && k < (int)blocks ? ld_peer_shared_u64(&s.mass[b], k) : 0;
         }
-        s.own_count[threadIdx.x] = (u32)c;
-        s.own_mass[threadIdx.x] = m;
+#pragma unroll
+        for (int k = 0; k < MOST_BLOCKS; ++k) c += cc[k], m += mm[k];
     }
+    if (threadIdx.x < OWN_BINS) s.own_count[threadIdx.x] = (u32)c, s.own_mass[threadIdx.x] = m;  // (nought behind its bins)
     c = block_sum_u64(s, c);
     if (MASS) m = block_sum_u64(s, m);
     if (threadIdx.x == 0) s.total_count = c, s.total_mass = m;
     cluster_sync();  // the sums are there; nobody reads the blocks' histograms any more
 }
 
+__device__ __forceinline__ void clear(Shared& s) {
+    for (int b = threadIdx.x; b < BINS; b += THREADS) s.count[b] = 0, s.mass[b] = 0;
+    __syncthreads();
+}
+
+// The histogram of a subset over the whole row: linear, or of elements of one bin by the next digit of their keys.
+__device__ void histogram(Shared& s, const Row& r, const Subset& in) {
+    clear(s);
+    u32 low = 0;  // what falls into bin 0 of the linear histogram, mostly far below all others: added up first
+    u64 low_mass = 0;
+    for (int i = threadIdx.x; i < r.n; i += THREADS) {
+        const float l = r.logit(i);
+        if (!in.holds(r, l, r.lo + i)) continue;
+        const int b = in.bin < 0 ? r.bin(l) : Subset::value(key_of(l, r.lo + i), in.digits);
+        const u64 m = r.mass(l);
+        if (in.bin < 0 && b == 0)
+            ++low, low_mass += m;
+        else {
+            atomicAdd(&s.count[b], 1u);
+            atomicAdd(&s.mass[b], m);
+        }
+    }
+    if (low) {
+        atomicAdd(&s.count[0], low);
+        atomicAdd(&s.mass[0], low_mass);
+    }
+    add_up<true>(s);
+}
+
 // The bin in which the running total of a histogram, from the highest bin down, first reaches `aim` (of counts, or of
 // masses); the lowest that holds anything where it does not.  All blocks get the same.  Ends behind a barrier of the cluster.
 __device__ Found find_bin(Shared& s, bool by_count, u64 aim) {
-    u64 count[CLUSTER], mass[CLUSTER];
+    const int lane = threadIdx.x & 31, blocks = cluster_blocks();
+    // the blocks' sums, the last block (which has the highest bins) first
+    const u64 count = lane < blocks ? ld_peer_shared_u64(&s.total_count, blocks - 1 - lane) : 0, mass = lane < blocks ? ld_peer_shared_u64(&s.total_mass, blocks - 1 - lane) : 0;
+    u64 upto_c = count, upto_m = mass;
 #pragma unroll
-    for (int k = 0; k < CLUSTER; ++k) count[k] = ld_peer_shared_u64(&s.total_count, k), mass[k] = ld_peer_shared_u64(&s.total_mass, k);
-    u64 c = 0, m = 0, before_c = 0, before_m = 0;
-    int owner = -1;
-#pragma unroll
-    for (int k = CLUSTER - 1; k >= 0; --k) {
-        // (the last block with anything in it that begins below the aim)
-        if (count[k] && (owner < 0 || (by_count ? c : m) < aim)) owner = k, before_c = c, before_m = m;
-        c += count[k], m += mass[k];
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 tc = __shfl_up_sync(0xffffffffu, upto_c, o), tm = __shfl_up_sync(0xffffffffu, upto_m, o);
+        if (lane >= o) upto_c += tc, upto_m += tm;
     }
+    // the last block with anything in it that begins below the aim
+    const unsigned some = __ballot_sync(0xffffffffu, count != 0 && (by_count ? upto_c - count : upto_m - mass) < aim);
+    const int at = some ? 31 - __clz(some) : 0, owner = blocks - 1 - at;
+    const u64 before_c = __shfl_sync(0xffffffffu, upto_c - count, at), before_m = __shfl_sync(0xffffffffu, upto_m - mass, at);
     if (owner == (int)cluster_ctarank() && threadIdx.x < 32) {
-        // four bins a lane, the highest first
-        const int lane = threadIdx.x, top = OWN_BINS - 1 - 4 * lane;
+        // eight bins a lane, the highest first
+        constexpr int EACH = OWN_BINS / 32;
+        const int top = OWN_BINS - 1 - EACH * lane;
         u64 pc = 0, pm = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) pc += s.own_count[top - k], pm += s.own_mass[top - k];
+        for (int k = 0; k < EACH; ++k) pc += s.own_count[top - k], pm += s.own_mass[top - k];
         u64 uc = pc, um = pm;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -213,16 +285,15 @@ __device__ Found find_bin(Shared& s, bool by_count, u64 aim) {
         int bin = -1;
         u64 bc = 0, bm = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < EACH; ++k) {
             const u32 n = s.own_count[top - k];
             if (n && (by_count ? ac : am) < aim) bin = top - k, bc = ac, bm = am;
             ac += n, am += s.own_mass[top - k];
         }
-        const unsigned some = __ballot_sync(0xffffffffu, bin >= 0);
-        const int last = 31 - __clz(some);
-        if (lane == last) {
-            s.found.bin = cluster_ctarank() * OWN_BINS + bin;
-            s.found.count = s.own_count[bin];
+        const unsigned any = __ballot_sync(0xffffffffu, bin >= 0);
+        if (any ? lane == 31 - __clz(any) : lane == 0) {
+            s.found.bin = owner * BINS / blocks + max(bin, 0);
+            s.found.count = s.own_count[max(bin, 0)];
             s.found.before_count = bc, s.found.before_mass = bm;
         }
     }
@@ -235,28 +306,39 @@ __device__ Found find_bin(Shared& s, bool by_count, u64 aim) {
     return f;
 }
 
-// The elements that `in` holds (with `upward` those of higher bins too), `n` <= LIST of them in the row, into s.all of every block.
-__device__ void gather(Shared& s, const Row& r, const Subset& in, bool upward, bool mass) {
+// The elements for which take(l, i) holds into s.all of every block: how many of them there are in the row (if more than LIST, some are missing).
+template <typename Take>
+__device__ u32 gather(Shared& s, const Row& r, Take take) {
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < r.n; i += THREADS) {
         const float l = r.logit(i);
-        const u64 key = key_of(l, r.lo + i);
-        if (upward ? r.bin(l) < in.bin : !in.holds(r, l, key)) continue;
+        if (!take(l, r.lo + i)) continue;
         const u32 at = atomicAdd(&s.listed, 1u);
-        if (at < LIST) s.list[at].key = key, s.list[at].mass = mass ? r.mass(l) : 0;
+        if (at < LIST) s.list[at].key = key_of(l, r.lo + i), s.list[at].mass = r.mass(l);
     }
     cluster_sync();
+    const u32 lane = threadIdx.x & 31, blocks = cluster_blocks();
+    const u32 mine = lane < blocks ? ld_peer_shared_u32(&s.listed, lane) : 0;
     u32 offset = 0;
-    for (int k = 0; k < CLUSTER; ++k) {
-        const u32 n = min(ld_peer_shared_u32(&s.listed, k), (u32)LIST);
-        for (u32 i = threadIdx.x; i < n && offset + i < LIST; i += THREADS) {
+    for (u32 k = 0; k < blocks; ++k) {
+        const u32 n = __shfl_sync(0xffffffffu, mine, k);
+        for (u32 i = threadIdx.x; i < n && i < LIST && offset + i < LIST; i += THREADS) {
             s.all[offset + i].key = ld_peer_shared_u64(&s.list[i].key, k);
             s.all[offset + i].mass = ld_peer_shared_u64(&s.list[i].mass, k);
         }
         offset += n;
     }
     cluster_sync();  // the lists are complete, and nobody's own is read any more
+    return offset;
+}
+
+// Of this thread's element of the n in s.all: how many lie before it, and their mass.
+__device__ __forceinline__ void ranks(const Shared& s, int n, const Entry& mine, u64& count, u64& mass) {
+    count = 0, mass = 0;
+    if ((int)threadIdx.x < n)
+        for (int i = 0; i < n; ++i)
+            if (s.all[i].key > mine.key) ++count, mass += s.all[i].mass;
 }
 
 // ceil(p m), exactly, for 0 < p < 1: what a mass has to reach.
@@ -283,15 +365,14 @@ struct Quantile {
     u64 key, mass;
 };
 
-// From the row's linear histogram, which stands in the blocks' eighths (masses too where they are wanted).
-__device__ Quantile quantile(Shared& s, const Row& r, bool by_count, u64 aim) {
+// From the linear histogram of `in`, which stands in the blocks' shares.
+__device__ Quantile quantile(Shared& s, const Row& r, Subset in, bool by_count, u64 aim) {
     Found f = find_bin(s, by_count, aim);
-    Subset in;
     in.bin = f.bin;
     u64 before_mass = f.before_mass;
     aim -= min(aim, by_count ? f.before_count : f.before_mass);
     while (f.count > LIST) {
-        histogram<true>(s, r, in);
+        histogram(s, r, in);
         f = find_bin(s, by_count, aim);
         const int shift = Subset::shift(in.digits);
         in.prefix |= shift >= 0 ? (u64)f.bin << shift : (u64)f.bin >> -shift;
@@ -299,16 +380,14 @@ __device__ Quantile quantile(Shared& s, const Row& r, bool by_count, u64 aim) {
         before_mass += f.before_mass;
         aim -= min(aim, by_count ? f.before_count : f.before_mass);
     }
-    gather(s, r, in, false, true);
-    const int n = (int)f.count;
+    const int n = (int)gather(s, r, [&](float l, int i) { return in.holds(r, l, i); });
     if (threadIdx.x == 0) s.threshold = 0, s.retained = 0;
     __syncthreads();
+    const Entry mine = s.all[threadIdx.x];
+    u64 count, mass;
+    ranks(s, n, mine, count, mass);
     if ((int)threadIdx.x < n) {
-        const Entry mine = s.all[threadIdx.x];
-        u64 count = 0, mass = 0;
-        for (int i = 0; i < n; ++i)
-            if (s.all[i].key > mine.key) ++count, mass += s.all[i].mass;
-        // the last one that begins below the aim: its predecessor's end lies below, and its own does not or nothing follows
+        // the last one that begins below the aim: its own end does not lie below, or nothing follows
         const u64 begins = by_count ? count : mass, ends = by_count ? count + 1 : mass + mine.mass;
         if ((begins < aim && ends >= aim) || (count == (u64)n - 1 && ends < aim)) s.threshold = mine.key, s.retained = mass + mine.mass;
     }
@@ -318,8 +397,17 @@ __device__ Quantile quantile(Shared& s, const Row& r, bool by_count, u64 aim) {
     return q;
 }
 
+// f(i, four neighbours from i on) over this block's elements, and one by one(i) over those at the end; with loads and stores of 16 bytes where `wide`.
+template <typename Four, typename One>
+__device__ __forceinline__ void for_elements(int n, bool wide, Four four, One one) {
+    const int whole = wide ? n & ~3 : 0;
+#pragma unroll 5
+    for (int i = 4 * threadIdx.x; i < whole; i += 4 * THREADS) four(i);
+    for (int i = whole + threadIdx.x; i < n; i += THREADS) one(i);
+}
+
 template <bool KEEP>  // the block's elements fit shared memory
-__global__ void __launch_bounds__(THREADS) sampling_probs_kernel(const SamplingProbs a) {
+__global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const SamplingProbs a) {
     __shared__ Shared s;
     extern __shared__ __align__(16) float kept[];
     pdl_wait();
@@ -328,153 +416,207 @@ __global__ void __launch_bounds__(THREADS) sampling_probs_kernel(const SamplingP
     const u32 rank = cluster_ctarank();
     const float* logits = a.logits + (long long)row * a.ldl;
     float* out = a.out + (long long)row * a.ldo;
-    const float T = a.temperature ? a.temperature[row] : 0.0f, p = a.top_p ? a.top_p[row] : 1.0f;
+    const float given = a.temperature ? a.temperature[row] : 0.0f, p = a.top_p ? a.top_p[row] : 1.0f;
     const int k = a.top_k ? a.top_k[row] : 0;
-    const bool greedy = !(T > 0.0f) || k == 1 || !(p > 0.0f);
+    const bool greedy = !(given > 0.0f) || k == 1 || !(p > 0.0f);
+    const float T = fminf(fmaxf(given, FLT_EPSILON), FLT_MAX);
     Row r;
     r.lo = min(a.vocab, (int)rank * a.per), r.n = min(a.vocab, r.lo + a.per) - r.lo;
     r.at = KEEP ? kept : logits + r.lo;
-    r.T = fmaxf(T, FLT_EPSILON);
-    // fetch, greatest key, least finite logit
-    u64 best = 0;
-    float least = INFINITY;
-    auto take = [&](float l, int i) {
-        if (KEEP) kept[i] = l;
-        l = number(l);
-        const u64 key = key_of(l, r.lo + i);
-        best = key > best ? key : best;
-        if (l > -INFINITY) least = fminf(least, l);
-    };
-    if ((((uintptr_t)(logits + r.lo)) & 15) == 0) {
-        const int whole = r.n & ~3;
-        for (int i = 4 * threadIdx.x; i < whole; i += 4 * THREADS) {
+    r.rate = LOG2E / (double)T;
+    const bool wide_in = (((uintptr_t)(logits + r.lo)) & 15) == 0, wide_out = (((uintptr_t)(out + r.lo)) & 15) == 0;
+    // the greatest logit: the thread's, the block's, the row's
+    float mine = -INFINITY;
+    for_elements(
+        r.n, wide_in,
+        [&](int i) {
             const float4 v = *reinterpret_cast<const float4*>(logits + r.lo + i);
-            take(v.x, i), take(v.y, i + 1), take(v.z, i + 2), take(v.w, i + 3);
-        }
-        for (int i = whole + threadIdx.x; i < r.n; i += THREADS) take(logits[r.lo + i], i);
-    } else
-        for (int i = threadIdx.x; i < r.n; i += THREADS) take(logits[r.lo + i], i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 x = __shfl_xor_sync(0xffffffffu, best, o);
-        best = x > best ? x : best;
-    }
-    least = -warp_max(-least);
-    if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = best, s.fred[threadIdx.x >> 5] = least;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < WARPS; ++w) {
-            best = s.red[w] > best ? s.red[w] : best;
-            least = fminf(least, s.fred[w]);
-        }
-        s.best = best, s.least = least;
-    }
+            if (KEEP) *reinterpret_cast<float4*>(kept + i) = v;
+            mine = fmaxf(fmaxf(mine, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+        },
+        [&](int i) {
+            const float l = logits[r.lo + i];
+            if (KEEP) kept[i] = l;
+            mine = fmaxf(mine, l);
+        });
+    const float block_top = block_max(s, mine);
+    // the least finite maximum of a thread
+    const int quads = wide_in ? r.n & ~3 : 0;
+    const bool has = 4 * (int)threadIdx.x < quads || quads + (int)threadIdx.x < r.n;
+    const float block_least = -block_max(s, mine > -INFINITY ? -mine : -INFINITY);
+    if (threadIdx.x == 0) s.value[0] = block_top, s.value[1] = block_least;
     cluster_sync();
-    best = 0, least = INFINITY;
-#pragma unroll
-    for (int c = 0; c < CLUSTER; ++c) {
-        const u64 x = ld_peer_shared_u64(&s.best, c);
-        best = x > best ? x : best;
-        least = fminf(least, __uint_as_float(ld_peer_shared_u32(&s.least, c)));
-    }
-    const u32 ordered = (u32)(best >> 32);
-    r.top = __uint_as_float(ordered & 0x80000000u ? ordered & 0x7fffffffu : ~ordered);
-    u64 threshold = 0;    // the least key that stays
-    float inv = 1.0f;     // of the softmax's sum (rows without top-k and top-p)
-    double retained = 1.0;
+    r.top = r.high = warp_max(row_value(&s.value[0], -INFINITY));
+    const float least = -warp_max(-row_value(&s.value[1], INFINITY));
+    out += r.lo;
     const bool by_k = !greedy && k > 0 && k < a.vocab, by_p = !greedy && p < 1.0f;
-    if (greedy)
-        threshold = best;
-    else if (!by_k && !by_p) {
-        float sum = 0.0f;
-        for (int i = threadIdx.x; i < r.n; i += THREADS) {
-            const float l = r.logit(i);
-            sum += l == r.top ? 1.0f : expf((l - r.top) / r.T);
-        }
-        sum = block_sum(sum, s.fred);
-        if (threadIdx.x == 0) s.sum = sum;
+    if (greedy) {
+        // the first index among those of the greatest logit
+        u32 first = 0xffffffffu;
+        for (int i = threadIdx.x; i < r.n; i += THREADS)
+            if (r.logit(i) == r.top) first = min(first, (u32)(r.lo + i));
+        first = __reduce_min_sync(0xffffffffu, first);
+        if (threadIdx.x == 0) s.index = 0xffffffffu;
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) atomicMin(&s.index, first);
         cluster_sync();
-        float total = 0.0f;
-#pragma unroll
-        for (int c = 0; c < CLUSTER; ++c) total += __uint_as_float(ld_peer_shared_u32(&s.sum, c));
-        inv = 1.0f / total;
+        const u32 lane = threadIdx.x & 31;
+        first = __reduce_min_sync(0xffffffffu, lane < cluster_blocks() ? ld_peer_shared_u32(&s.index, lane) : 0xffffffffu) - (u32)r.lo;
+        auto of = [&](int i) { return (u32)i == first ? 1.0f : 0.0f; };
+        for_elements(
+            r.n, wide_out, [&](int i) { *reinterpret_cast<float4*>(out + i) = make_float4(of(i), of(i + 1), of(i + 2), of(i + 3)); },
+            [&](int i) { out[i] = of(i); });
+    } else if (!by_k && !by_p) {
+        const float rate = (float)r.rate;
+        const bool infinite = isinf(r.top);
+        // (the difference is rounded once, its product with log2(e) / T twice: an exponent is off by 2^-23 of itself, as if it were divided by T)
+        auto weight = [&](float l) { return infinite ? (number(l) == r.top ? 1.0f : 0.0f) : exp2f((number(l) - r.top) * rate); };
+        float sum = 0.0f;
+        for_elements(
+            r.n, KEEP,
+            [&](int i) {
+                float4 v = *reinterpret_cast<const float4*>(r.at + i);
+                v = make_float4(weight(v.x), weight(v.y), weight(v.z), weight(v.w));
+                if (KEEP) *reinterpret_cast<float4*>(kept + i) = v;
+                sum += (v.x + v.y) + (v.z + v.w);
+            },
+            [&](int i) {
+                const float w = weight(r.at[i]);
+                if (KEEP) kept[i] = w;
+                sum += w;
+            });
+        sum = block_sum(sum, s.fred);  // (ends with a barrier: the weights are there for all)
+        if (threadIdx.x == 0) s.value[2] = sum;
+        cluster_sync();
+        const float inv = 1.0f / warp_sum(row_value(&s.value[2], 0.0f));
+        auto of = [&](int i) { return (KEEP ? kept[i] : weight(r.at[i])) * inv; };
+        for_elements(
+            r.n, wide_out,
+            [&](int i) {
+                if (KEEP) {
+                    const float4 v = *reinterpret_cast<const float4*>(kept + i);
+                    *reinterpret_cast<float4*>(out + i) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                } else
+                    *reinterpret_cast<float4*>(out + i) = make_float4(of(i), of(i + 1), of(i + 2), of(i + 3));
+            },
+            [&](int i) { out[i] = of(i); });
     } else {
-        float range = r.top - least;
-        if (!(range > 0.0f) || range == INFINITY) range = range == INFINITY ? FLT_MAX : 1.0f;
-        // what weighs less than 2^-46 of the greatest has no mass: where only masses count, bin 0 takes all of it
-        if (!by_k) range = fminf(range, 32.0f * r.T);
-        r.bins_per = (float)(BINS - 1) / range;
-        u64 mass = 0;
-        const Subset all;
-        bool listed = false;
-        if (by_k) {
-            if (k > LIST)
-                histogram<true>(s, r, all);
-            else {
-                histogram<false>(s, r, all);
+        u64 threshold = 0, mass = 0;  // the least key that stays; the mass of those that do
+        bool done = false;
+        auto set_range = [&](float range) {
+            if (!(range > 0.0f)) range = 1.0f;
+            r.bins_per = (float)(BINS - 1) / fminf(range, FLT_MAX);
+        };
+        Subset all;
+        if (by_k && k <= LIST) {
+            // the k-th of the threads' maxima: no fewer than k logits lie in its bin and above
+            set_range(r.top - least);
+            clear(s);
+            if (has) atomicAdd(&s.count[r.bin(number(mine))], 1u);
+            add_up<false>(s);
+            const u64 threads = row_sum_u64(&s.total_count);
+            if (threads >= (u64)k) {
                 const Found f = find_bin(s, true, (u64)k);
-                if (f.before_count + f.count <= LIST) {  // they and all above them, ordered at once
-                    Subset in;
-                    in.bin = f.bin;
-                    gather(s, r, in, true, true);
-                    const int n = (int)(f.before_count + f.count);
+                const int n = (int)gather(s, r, [&](float l, int) { return r.bin(l) >= f.bin; });
+                if (n <= LIST) {
                     if (threadIdx.x == 0) s.threshold = ~0ull, s.retained = 0, s.kept_mass = 0;
                     __syncthreads();
-                    Entry mine = {0, 0};
-                    u64 count = 0, before = 0;
-                    const bool here = (int)threadIdx.x < n;
-                    if (here) {
-                        mine = s.all[threadIdx.x];
-                        for (int i = 0; i < n; ++i)
-                            if (s.all[i].key > mine.key) ++count, before += s.all[i].mass;
-                        if (count == (u64)k - 1) s.kept_mass = before + mine.mass;
-                    }
+                    const Entry here = s.all[threadIdx.x];
+                    u64 count, before;
+                    ranks(s, n, here, count, before);
+                    const bool in = (int)threadIdx.x < n;
+                    if (in && count == (u64)k - 1) s.kept_mass = before + here.mass;
                     __syncthreads();
                     const u64 aim = by_p ? share_of(s.kept_mass, p) : ~0ull;
-                    if (here && count < (u64)k && (count == 0 || before < aim)) {
-                        atomicMin(&s.threshold, mine.key);
-                        atomicMax(&s.retained, before + mine.mass);
+                    if (in && count < (u64)k && (count == 0 || before < aim)) {
+                        atomicMin(&s.threshold, here.key);
+                        atomicMax(&s.retained, before + here.mass);
                     }
                     __syncthreads();
                     threshold = s.threshold, mass = s.retained;
-                    listed = true;
+                    done = true;
                 }
             }
-            if (!listed) {
-                if (k <= LIST) histogram<true>(s, r, all);
-                const Quantile q = quantile(s, r, true, (u64)k);
-                threshold = q.key, mass = q.mass;
-                if (by_p) histogram<true>(s, r, all);  // (the search may have cut a bin up in its place)
-            }
-        } else
-            histogram<true>(s, r, all);
-        if (by_p && !listed) {
-            if (!by_k) {
-                mass = 0;
-#pragma unroll
-                for (int c = 0; c < CLUSTER; ++c) mass += ld_peer_shared_u64(&s.total_mass, c);
-            }
-            u64 aim = share_of(mass, p);
-            const Quantile q = quantile(s, r, false, aim ? aim : 1);
-            threshold = q.key, mass = q.mass;
         }
-        retained = (double)mass / UNIT;
+        if (!done && by_k) {
+            // the whole row's histogram, from the greatest logit to the least finite one
+            float low = INFINITY;
+            for (int i = threadIdx.x; i < r.n; i += THREADS) {
+                const float l = r.logit(i);
+                if (l > -INFINITY) low = fminf(low, l);
+            }
+            low = -block_max(s, -low);
+            if (threadIdx.x == 0) s.value[3] = low;
+            cluster_sync();
+            set_range(r.top - -warp_max(-row_value(&s.value[3], INFINITY)));
+            histogram(s, r, all);
+            const Quantile q = quantile(s, r, all, true, (u64)k);
+            threshold = q.key, mass = q.mass;
+            if (by_p) {
+                histogram(s, r, all);  // (the search may have cut a bin up in its place)
+                const u64 aim = share_of(mass, p);
+                const Quantile qp = quantile(s, r, all, false, aim ? aim : 1);
+                threshold = qp.key, mass = qp.mass;
+            }
+        } else if (!done) {
+            // masses above bounds that lie so many units of temperature below the greatest logit
+            float bound[BOUNDS];
+            {
+                const float depth[BOUNDS] = {1.0f, 2.0f, 4.0f, 6.0f, 8.0f, 11.0f, 16.0f};
+#pragma unroll
+                for (int b = 0; b < BOUNDS; ++b) bound[b] = r.top - depth[b] * T;
+            }
+            u64 above[BOUNDS + 1] = {};
+            for (int i = threadIdx.x; i < r.n; i += THREADS) {
+                const float l = r.logit(i);
+                const u64 m = r.mass(l);
+                above[BOUNDS] += m;
+#pragma unroll
+                for (int b = 0; b < BOUNDS; ++b)
+                    if (l > bound[b]) above[b] += m;
+            }
+#pragma unroll
+            for (int b = 0; b <= BOUNDS; ++b) {
+                const u64 t = block_sum_u64(s, above[b]);
+                if (threadIdx.x == 0) s.above[b] = t;
+            }
+            cluster_sync();
+#pragma unroll
+            for (int b = 0; b <= BOUNDS; ++b) above[b] = row_sum_u64(&s.above[b]);
+            const u64 share = share_of(above[BOUNDS], p), aim = share ? share : 1;
+            // between which two the border lies: the first bound above which there is enough
+            Subset in;
+            u64 before = 0;
+            in.high = r.top;
+            float depth = 32.0f * T;  // what weighs less than 2^-46 of the greatest has no mass
+#pragma unroll
+            for (int b = BOUNDS - 1; b >= 0; --b)
+                if (above[b] >= aim) in.low = bound[b];
+#pragma unroll
+            for (int b = 0; b < BOUNDS; ++b)
+                if (above[b] < aim) in.high = bound[b], before = above[b];
+            if (in.low > -INFINITY) depth = in.high - in.low;
+            r.high = in.high;
+            set_range(depth);
+            histogram(s, r, in);
+            const Quantile q = quantile(s, r, in, false, aim - before);
+            threshold = q.key, mass = before + q.mass;
+        }
+        const double inv = UNIT / (double)mass;
+        const float floor_logit = logit_of((u32)(threshold >> 32));
+        auto of = [&](float l, int i) -> float {
+            l = number(l);
+            if (l < floor_logit) return 0.0f;
+            return key_of(l, r.lo + i) >= threshold ? (float)(r.weight(l) * inv) : 0.0f;
+        };
+        for_elements(
+            r.n, wide_out && KEEP,
+            [&](int i) {
+                const float4 v = *reinterpret_cast<const float4*>(r.at + i);
+                *reinterpret_cast<float4*>(out + i) = make_float4(of(v.x, i), of(v.y, i + 1), of(v.z, i + 2), of(v.w, i + 3));
+            },
+            [&](int i) { out[i] = of(r.at[i], i); });
     }
-    // the probabilities
-    auto of = [&](int i) -> float {
-        const float l = r.logit(i);
-        if (greedy) return key_of(l, r.lo + i) == threshold ? 1.0f : 0.0f;
-        if (!by_k && !by_p) return l == r.top ? inv : expf((l - r.top) / r.T) * inv;
-        return key_of(l, r.lo + i) >= threshold ? (float)(r.weight(l) / retained) : 0.0f;
-    };
-    out += r.lo;
-    if (((uintptr_t)out & 15) == 0) {
-        const int whole = r.n & ~3;
-        for (int i = 4 * threadIdx.x; i < whole; i += 4 * THREADS)
-            *reinterpret_cast<float4*>(out + i) = make_float4(of(i), of(i + 1), of(i + 2), of(i + 3));
-        for (int i = whole + threadIdx.x; i < r.n; i += THREADS) out[i] = of(i);
-    } else
-        for (int i = threadIdx.x; i < r.n; i += THREADS) out[i] = of(i);
     cluster_sync();  // nobody leaves while others may read its shared memory
 }
 
@@ -485,15 +627,28 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
                                      const int* top_k, const float* top_p, void* stream) {
     if (rows <= 0) return FERRIS_OK;
     if (vocab <= 0 || ldl < vocab || ldo < vocab || vocab > 0x7fffffff - 64) FERRIS_REFUSE("vocabulary %d, row strides %lld and %lld", vocab, ldl, ldo);
-    SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, ((vocab + 4 * CLUSTER - 1) / (4 * CLUSTER)) * 4};
-    const size_t bytes = (size_t)a.per * 4, most = 227 * 1024 - sizeof(Shared) - 1024;
+    // Blocks of a row: of as many as give the least time if blocks run in waves, each as long as its share of the row (40 rows of 151,936: seven, 280 blocks at once,
+    // where eight would leave 24 of them for a second wave).
+    const int sms = ferris_sm_count();
+    int blocks = MOST_BLOCKS;
+    double least = 0.0;
+    auto per_block = [&](int b) { return (int)(((long long)vocab + 4 * b - 1) / (4 * b)) * 4; };
+    const size_t fixed = sizeof(Shared) + 1024, most = 227 * 1024;  // (an SM keeps a KB of every block's for itself)
+    for (int b = MOST_BLOCKS; b >= LEAST_BLOCKS; --b) {
+        const size_t bytes = (size_t)per_block(b) * 4 + fixed;
+        const long long at_once = (bytes <= most / 2 || bytes > most ? 2ll : 1ll) * (sms > 0 ? sms : 148);
+        const double time = (double)(((long long)rows * b + at_once - 1) / at_once) / b;
+        if (b == MOST_BLOCKS || time < least) least = time, blocks = b;
+    }
+    SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks)};
+    const size_t bytes = (size_t)a.per * 4;
     cudaError_t e;
-    if (bytes <= most) {
+    if (bytes + fixed <= most) {
         const int rc = ferris_allow_dynamic_smem((const void*)sampling_probs_kernel<true>, bytes);
         if (rc != FERRIS_OK) return rc;
-        e = ferris_launch_cluster(sampling_probs_kernel<true>, dim3(rows, 1, CLUSTER), dim3(THREADS), bytes, (cudaStream_t)stream, CLUSTER, a);
+        e = ferris_launch_cluster(sampling_probs_kernel<true>, dim3(rows, 1, blocks), dim3(THREADS), bytes, (cudaStream_t)stream, blocks, a);
     } else
-        e = ferris_launch_cluster(sampling_probs_kernel<false>, dim3(rows, 1, CLUSTER), dim3(THREADS), 0, (cudaStream_t)stream, CLUSTER, a);
+        e = ferris_launch_cluster(sampling_probs_kernel<false>, dim3(rows, 1, blocks), dim3(THREADS), 0, (cudaStream_t)stream, blocks, a);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;

@@ -186,84 +186,84 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeAttention p) {
 }
 
 // The parts that the groups of a bf16 step's blocks left of items that lie in several: a block joins 32 query rows of an item, and as many columns.  A lane
-// is a row, as the parts lie; the warps have four columns each, and eight parts of them on their way at once.
-constexpr int JOIN_GROUPS = 64;  // parts whose factors are held at once
+// is a row, as the parts lie; a warp has four columns, and sixteen parts of them on their way at once.  Bound by latency: the item's groups, the parts'
+// maxima and sums, the parts.
+constexpr int JOIN_PARTS = 64;  // parts that are joined at once
 
 __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes, int row_blocks) {
-    __shared__ float top[8][32], total[8][32], tile[32][33], factor[JOIN_GROUPS][32];
+    __shared__ float top[8][32], tile[32][33], factor[JOIN_PARTS][32];
     pdl_wait();
     pdl_launch_dependents();
     const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.y / row_blocks, row0 = (blockIdx.y - head * row_blocks) * min(rows, 32), col0 = blockIdx.x * 32, seq = blockIdx.z;
+    const int head = blockIdx.y / row_blocks, row0 = (blockIdx.y - head * row_blocks) * min(rows, 32), col = blockIdx.x * 32 + warp * 4, seq = blockIdx.z;
     const int4 span = p.spans[seq * p.kv_heads + head];
     const int count = span.z * p.group, parts = span.y - span.x + 1;
     if (row0 >= count || parts <= 1) return;  // (one part: written by the block that has it)
     const int block = row0 / rows, in = row0 - block * rows + lane;  // (blocks have 16 rows or a multiple of 32)
     const bool live = row0 + lane < count && in < rows;
     auto part = [&](int k) { return tree_part(p, (span.x + k) * lanes + block, k == 0, rows) + in; };
-    float m = -INFINITY;
-    if (live)
-        for (int k = warp; k < parts; k += 32) {  // (four at a time on their way)
-            float x[4];
+    float m = -INFINITY, l = 0.0f, o[4] = {};  // l: of the warp's own parts
+    for (int k0 = 0; k0 < parts; k0 += JOIN_PARTS) {
+        const int n = min(parts - k0, JOIN_PARTS);
+        float x[JOIN_PARTS / 8], y[JOIN_PARTS / 8], most = m;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = k + 8 * u < parts ? part(k + 8 * u)[D * rows] : -INFINITY;
-            m = fmaxf(fmaxf(m, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+        for (int u = 0; u < JOIN_PARTS / 8; ++u) {
+            const bool there = live && warp + 8 * u < n;
+            x[u] = there ? part(k0 + warp + 8 * u)[D * rows] : -INFINITY;
+            y[u] = there ? part(k0 + warp + 8 * u)[(D + 1) * rows] : 0.0f;
         }
-    top[warp][lane] = m;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, top[w][lane]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[4] = {};
-    for (int k0 = 0; k0 < parts; k0 += JOIN_GROUPS) {
-        const int n = min(parts - k0, JOIN_GROUPS);
-        if (k0) __syncthreads();
-        for (int k = warp; k < n; k += 32) {
-            float x[4] = {}, y[4] = {};
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (live && k + 8 * u < n) x[u] = part(k0 + k + 8 * u)[D * rows], y[u] = part(k0 + k + 8 * u)[(D + 1) * rows];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (k + 8 * u < n) {
-                    const float f = exp2f(x[u] - base);
-                    factor[k + 8 * u][lane] = f;
-                    l = fmaf(f, y[u], l);
-                }
-        }
+        for (int u = 0; u < JOIN_PARTS / 8; ++u) most = fmaxf(most, x[u]);
+        if (k0) __syncthreads();  // (the factors before are done with)
+        top[warp][lane] = most;
         __syncthreads();
-        const int col = col0 + warp * 4;
-        if (live && col < D)  // (heads have a multiple of eight columns)
-            for (int k = 0; k < n; k += 8) {
-                float x[8][4];
+        for (int w = 0; w < 8; ++w) most = fmaxf(most, top[w][lane]);
+        const float base = most == -INFINITY ? 0.0f : most, corr = exp2f(m - base);
+        m = most, l *= corr;
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+        for (int c = 0; c < 4; ++c) o[c] *= corr;
+#pragma unroll
+        for (int u = 0; u < JOIN_PARTS / 8; ++u)
+            if (warp + 8 * u < n) {
+                const float f = exp2f(x[u] - base);
+                factor[warp + 8 * u][lane] = f;
+                l = fmaf(f, y[u], l);
+            }
+        __syncthreads();
+        if (live && col < D)  // (heads have a multiple of eight columns)
+            for (int k = 0; k < n; k += 16) {
+                float v[16][4];
+#pragma unroll
+                for (int u = 0; u < 16; ++u)
                     if (k + u < n) {
                         const float* from = part(k0 + k + u) + col * rows;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) x[u][c] = from[c * rows];
+                        for (int c = 0; c < 4; ++c) v[u][c] = from[c * rows];
                     }
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                for (int u = 0; u < 16; ++u)
                     if (k + u < n) {
                         const float f = factor[k + u][lane];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) o[c] = fmaf(f, x[u][c], o[c]);
+                        for (int c = 0; c < 4; ++c) o[c] = fmaf(f, v[u][c], o[c]);
                     }
             }
     }
-    total[warp][lane] = l;
+    __syncthreads();
+    top[warp][lane] = l;
     __syncthreads();
     l = 0.0f;
-    for (int w = 0; w < 8; ++w) l += total[w][lane];
+    for (int w = 0; w < 8; ++w) l += top[w][lane];
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int c = 0; c < 4; ++c) tile[warp * 4 + c][lane] = o[c] * inv;
     __syncthreads();
     // a warp: a row's columns
+    const int out_col = blockIdx.x * 32 + lane;
     for (int row = warp; row < 32 && row0 + row < count && in - lane + row < rows; row += 8) {
         const int at = row0 + row;
-        if (col0 + lane < D)
-            ((bf16*)p.out)[(size_t)(span.w + at / p.group) * p.ldo + (head * p.group + at % p.group) * D + col0 + lane] = from_float<bf16>(tile[lane][row]);
+        if (out_col < D)
+            ((bf16*)p.out)[(size_t)(span.w + at / p.group) * p.ldo + (head * p.group + at % p.group) * D + out_col] = from_float<bf16>(tile[lane][row]);
     }
 }
 

@@ -33,6 +33,7 @@ constexpr int LEAST_BLOCKS = BINS / OWN_BINS;
 constexpr int LIST = 512;    // elements that are ordered by counting
 constexpr int DIGIT = 10;    // bits of a digit of the keys: a histogram's bins
 constexpr int BOUNDS = 7;
+constexpr int MASS_BITS = 45;
 constexpr double UNIT = 35184372088832.0;  // 2^45
 constexpr double LOG2E = 1.4426950408889634;
 
@@ -89,7 +90,8 @@ struct Shared {
     u64 total_count, total_mass;  // of these
     Found found;
     float value[4];    // what blocks tell each other, each place once
-    u64 above[BOUNDS + 1];  // masses above the bounds, and of all
+    float above[BOUNDS + 1], parts[WARPS][BOUNDS + 1];  // masses above the bounds, and of all
+    u64 over, sum;
     u32 index;
     u32 listed;
     u64 threshold, retained, kept_mass;
@@ -104,14 +106,18 @@ __device__ __forceinline__ u32 order_of(float l) {
 }
 __device__ __forceinline__ float logit_of(u32 order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
 __device__ __forceinline__ u64 key_of(float l, int i) { return (u64)order_of(l) << 32 | (u32)~(u32)i; }
-// Of a NaN minus infinity.
-__device__ __forceinline__ float number(float l) { return fmaxf(l, -INFINITY); }
 
-// 2^y for y <= 0 up to 2^-46 of itself (nought below 2^-60): the nearest whole number apart, and the Taylor polynomial of 2^f for |f| <= 1/2, whose
+__device__ __forceinline__ float exp2_unit(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 2^(y + up) for -100 <= y <= 0, up to 2^-46 of itself: the nearest whole number apart, and the Taylor polynomial of 2^f for |f| <= 1/2, whose
 // twelfth term is 6e-15.
-__device__ __forceinline__ double exp2_64(double y) {
+__device__ __forceinline__ double exp2_64(double y, int up) {
     const double magic = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to a whole number
-    const double t = fmax(y, -1000.0) + magic, f = fmax(y, -1000.0) - (t - magic);
+    const double t = y + magic, f = y - (t - magic);
     double r = 4.44553827187081e-10;  // ln(2)^k / k! for k = 11 .. 0
     r = fma(r, f, 7.054911620801121e-09);
     r = fma(r, f, 1.0178086009239696e-07);
@@ -124,20 +130,32 @@ __device__ __forceinline__ double exp2_64(double y) {
     r = fma(r, f, 0.2402265069591007);
     r = fma(r, f, 0.6931471805599453);
     r = fma(r, f, 1.0);
-    const int n = __double2loint(t);
-    return n < -60 ? 0.0 : __hiloint2double(__double2hiint(r) + n * (1 << 20), __double2loint(r));
+    return __hiloint2double(__double2hiint(r) + (__double2loint(t) + up) * (1 << 20), __double2loint(r));
 }
 
 struct Row {
     const float* at;  // this block's elements: shared memory, or the row itself
     int lo, n;        // the first one's index, their number
-    float top, high, bins_per;  // the greatest logit; where the linear histogram begins
+    bool infinite;    // the greatest logit is infinite: those that equal it stand for 0, the others for minus infinity
+    float given_top;  // the greatest logit as it is,
+    float top;        // and as it stands
+    float high, bins_per;  // where the linear histogram begins, bins per unit of logit
+    float least;      // what lies below has no mass: 2^-86 of the greatest weight
     double rate;      // log2(e) / T
 
+    __device__ __forceinline__ float number(float l) const {
+        l = fmaxf(l, -INFINITY);  // (of a NaN minus infinity)
+        return !infinite ? l : l == given_top ? 0.0f : -INFINITY;
+    }
     __device__ __forceinline__ float logit(int i) const { return number(at[i]); }
-    __device__ __forceinline__ double weight(float l) const { return l == top ? 1.0 : exp2_64(((double)l - (double)top) * rate); }
+    __device__ __forceinline__ bool nothing(float l) const { return l < least || l == -INFINITY; }
+    __device__ __forceinline__ double exponent(float l) const { return ((double)fmaxf(l, fmaxf(least, -FLT_MAX)) - (double)top) * rate; }
+    __device__ __forceinline__ double weight(float l) const { return nothing(l) ? 0.0 : exp2_64(exponent(l), 0); }
     // (adding 2^52 rounds to a whole number, which is then the lower bits)
-    __device__ __forceinline__ u64 mass(float l) const { return (u64)__double_as_longlong(fma(weight(l), UNIT, 4503599627370496.0)) & 0xfffffffffffffull; }
+    __device__ __forceinline__ u64 mass(float l) const {
+        const u64 m = (u64)__double_as_longlong(exp2_64(exponent(l), MASS_BITS) + 4503599627370496.0) & 0xfffffffffffffull;
+        return nothing(l) ? 0 : m;
+    }
     // The greatest logits in the highest bin; what lies below the histogram's range in bin 0.
     __device__ __forceinline__ int bin(float l) const {
         const float x = l >= high ? 0.0f : (high - l) * bins_per;
@@ -419,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
     const float given = a.temperature ? a.temperature[row] : 0.0f, p = a.top_p ? a.top_p[row] : 1.0f;
     const int k = a.top_k ? a.top_k[row] : 0;
     const bool greedy = !(given > 0.0f) || k == 1 || !(p > 0.0f);
-    const float T = fminf(fmaxf(given, FLT_EPSILON), FLT_MAX);
+    const float T = fminf(fmaxf(given, FLT_EPSILON), 1e30f);
     Row r;
     r.lo = min(a.vocab, (int)rank * a.per), r.n = min(a.vocab, r.lo + a.per) - r.lo;
     r.at = KEEP ? kept : logits + r.lo;
@@ -446,7 +464,10 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
     const float block_least = -block_max(s, mine > -INFINITY ? -mine : -INFINITY);
     if (threadIdx.x == 0) s.value[0] = block_top, s.value[1] = block_least;
     cluster_sync();
-    r.top = r.high = warp_max(row_value(&s.value[0], -INFINITY));
+    r.given_top = warp_max(row_value(&s.value[0], -INFINITY));
+    r.infinite = isinf(r.given_top);
+    r.top = r.high = r.infinite ? 0.0f : r.given_top;
+    r.least = r.top - 60.0f * T;
     const float least = -warp_max(-row_value(&s.value[1], INFINITY));
     out += r.lo;
     const bool by_k = !greedy && k > 0 && k < a.vocab, by_p = !greedy && p < 1.0f;
@@ -468,9 +489,8 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
             [&](int i) { out[i] = of(i); });
     } else if (!by_k && !by_p) {
         const float rate = (float)r.rate;
-        const bool infinite = isinf(r.top);
         // (the difference is rounded once, its product with log2(e) / T twice: an exponent is off by 2^-23 of itself, as if it were divided by T)
-        auto weight = [&](float l) { return infinite ? (number(l) == r.top ? 1.0f : 0.0f) : exp2f((number(l) - r.top) * rate); };
+        auto weight = [&](float l) { return exp2_unit((r.number(l) - r.top) * rate); };
         float sum = 0.0f;
         for_elements(
             r.n, KEEP,
@@ -512,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
             // the k-th of the threads' maxima: no fewer than k logits lie in its bin and above
             set_range(r.top - least);
             clear(s);
-            if (has) atomicAdd(&s.count[r.bin(number(mine))], 1u);
+            if (has) atomicAdd(&s.count[r.bin(r.number(mine))], 1u);
             add_up<false>(s);
             const u64 threads = row_sum_u64(&s.total_count);
             if (threads >= (u64)k) {
@@ -559,53 +579,79 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
                 threshold = qp.key, mass = qp.mass;
             }
         } else if (!done) {
-            // masses above bounds that lie so many units of temperature below the greatest logit
-            float bound[BOUNDS];
-            {
-                const float depth[BOUNDS] = {1.0f, 2.0f, 4.0f, 6.0f, 8.0f, 11.0f, 16.0f};
+            // Masses above bounds that lie so many units of temperature below the greatest logit, in 32 bits: between which two the border lies, with 2^-10
+            // for what they are off by.
+            const float depth[BOUNDS] = {1.0f, 2.0f, 4.0f, 6.0f, 8.0f, 11.0f, 16.0f};
+            float bound[BOUNDS], above[BOUNDS] = {}, all_mass = 0.0f;
 #pragma unroll
-                for (int b = 0; b < BOUNDS; ++b) bound[b] = r.top - depth[b] * T;
-            }
-            u64 above[BOUNDS + 1] = {};
+            for (int b = 0; b < BOUNDS; ++b) bound[b] = r.top - depth[b] * T;
+            const float rate = (float)r.rate;
             for (int i = threadIdx.x; i < r.n; i += THREADS) {
-                const float l = r.logit(i);
-                const u64 m = r.mass(l);
-                above[BOUNDS] += m;
+                const float l = r.logit(i), w = exp2_unit((l - r.top) * rate);
+                all_mass += w;
 #pragma unroll
                 for (int b = 0; b < BOUNDS; ++b)
-                    if (l > bound[b]) above[b] += m;
+                    if (l > bound[b]) above[b] += w;
             }
 #pragma unroll
             for (int b = 0; b <= BOUNDS; ++b) {
-                const u64 t = block_sum_u64(s, above[b]);
-                if (threadIdx.x == 0) s.above[b] = t;
+                const float t = warp_sum(b < BOUNDS ? above[b] : all_mass);
+                if ((threadIdx.x & 31) == 0) s.parts[threadIdx.x >> 5][b] = t;
+            }
+            __syncthreads();
+            if (threadIdx.x <= BOUNDS) {
+                float t = 0.0f;
+                for (int w = 0; w < WARPS; ++w) t += s.parts[w][threadIdx.x];
+                s.above[threadIdx.x] = t;
             }
             cluster_sync();
 #pragma unroll
-            for (int b = 0; b <= BOUNDS; ++b) above[b] = row_sum_u64(&s.above[b]);
-            const u64 share = share_of(above[BOUNDS], p), aim = share ? share : 1;
-            // between which two the border lies: the first bound above which there is enough
+            for (int b = 0; b < BOUNDS; ++b) above[b] = warp_sum(row_value(&s.above[b], 0.0f));
+            all_mass = warp_sum(row_value(&s.above[BOUNDS], 0.0f));
             Subset in;
-            u64 before = 0;
             in.high = r.top;
-            float depth = 32.0f * T;  // what weighs less than 2^-46 of the greatest has no mass
 #pragma unroll
             for (int b = BOUNDS - 1; b >= 0; --b)
-                if (above[b] >= aim) in.low = bound[b];
+                if (above[b] > p * all_mass * (1.0f + 1.0f / 1024)) in.low = bound[b];
 #pragma unroll
             for (int b = 0; b < BOUNDS; ++b)
-                if (above[b] < aim) in.high = bound[b], before = above[b];
-            if (in.low > -INFINITY) depth = in.high - in.low;
+                if (above[b] < p * all_mass * (1.0f - 1.0f / 1024)) in.high = bound[b];
+            // the histogram of what lies between them, and the masses of what lies above and of all
             r.high = in.high;
-            set_range(depth);
-            histogram(s, r, in);
-            const Quantile q = quantile(s, r, in, false, aim - before);
-            threshold = q.key, mass = before + q.mass;
+            set_range(in.low > -INFINITY ? in.high - in.low : 32.0f * T);  // (what weighs less than 2^-46 of the greatest has no mass)
+            clear(s);
+            u64 over = 0, sum = 0, low_mass = 0;
+            u32 low = 0;
+            for (int i = threadIdx.x; i < r.n; i += THREADS) {
+                const float l = r.logit(i);
+                const u64 m = r.mass(l);
+                sum += m;
+                if (l > in.high) over += m;
+                if (!in.between(l)) continue;
+                const int b = r.bin(l);
+                if (b == 0)
+                    ++low, low_mass += m;
+                else {
+                    atomicAdd(&s.count[b], 1u);
+                    atomicAdd(&s.mass[b], m);
+                }
+            }
+            if (low) {
+                atomicAdd(&s.count[0], low);
+                atomicAdd(&s.mass[0], low_mass);
+            }
+            over = block_sum_u64(s, over), sum = block_sum_u64(s, sum);
+            if (threadIdx.x == 0) s.over = over, s.sum = sum;
+            add_up<true>(s);
+            over = row_sum_u64(&s.over), sum = row_sum_u64(&s.sum);
+            const u64 aim = share_of(sum, p);
+            const Quantile q = quantile(s, r, in, false, (aim ? aim : 1) - over);
+            threshold = q.key, mass = over + q.mass;
         }
         const double inv = UNIT / (double)mass;
         const float floor_logit = logit_of((u32)(threshold >> 32));
         auto of = [&](float l, int i) -> float {
-            l = number(l);
+            l = r.number(l);
             if (l < floor_logit) return 0.0f;
             return key_of(l, r.lo + i) >= threshold ? (float)(r.weight(l) * inv) : 0.0f;
         };

@@ -28,11 +28,12 @@ typedef unsigned long long u64;
 typedef unsigned int u32;
 
 constexpr int MOST_BLOCKS = 8, THREADS = 512, WARPS = THREADS / 32;
-constexpr int BINS = 1024, OWN_BINS = 256;  // a block adds up BINS / blocks of the row's bins: at most a quarter
+constexpr int BINS = 512, OWN_BINS = 128;  // a block adds up BINS / blocks of the row's bins: at most a quarter
 constexpr int LEAST_BLOCKS = BINS / OWN_BINS;
-constexpr int LIST = 512;    // elements that are ordered by counting
-constexpr int DIGIT = 10;    // bits of a digit of the keys: a histogram's bins
+constexpr int LIST = THREADS;  // elements that are ordered by counting, one a thread
+constexpr int DIGIT = 9;    // bits of a digit of the keys: a histogram's bins
 constexpr int BOUNDS = 7;
+constexpr int MOST_ELEMENTS = 65536;  // of a block
 constexpr int MASS_BITS = 45;
 constexpr double UNIT = 35184372088832.0;  // 2^45
 constexpr double LOG2E = 1.4426950408889634;
@@ -79,8 +80,8 @@ struct Entry {
 struct Shared {
     union {
         struct {
-            u32 count[BINS];  // this block's histogram
-            u64 mass[BINS];
+            u32 count[BINS];  // this block's histogram; masses by their lower, middle and upper sixteen bits (additions of 32 bits are native, of 64 are not)
+            u32 mass[3][BINS];
         };
         Entry list[LIST];  // this block's elements of a bin, when the histograms have been added up
     };
@@ -95,8 +96,8 @@ struct Shared {
     u32 index;
     u32 listed;
     u64 threshold, retained, kept_mass;
-    u64 red[WARPS];
-    float fred[33];
+    u64 red[2][WARPS];
+    float fred[4][WARPS], scratch[33];
 };
 
 // Ordered as the logits are, the lower index first among equals.
@@ -150,7 +151,6 @@ struct Row {
     __device__ __forceinline__ float logit(int i) const { return number(at[i]); }
     __device__ __forceinline__ bool nothing(float l) const { return l < least || l == -INFINITY; }
     __device__ __forceinline__ double exponent(float l) const { return ((double)fmaxf(l, fmaxf(least, -FLT_MAX)) - (double)top) * rate; }
-    __device__ __forceinline__ double weight(float l) const { return nothing(l) ? 0.0 : exp2_64(exponent(l), 0); }
     // (adding 2^52 rounds to a whole number, which is then the lower bits)
     __device__ __forceinline__ u64 mass(float l) const {
         const u64 m = (u64)__double_as_longlong(exp2_64(exponent(l), MASS_BITS) + 4503599627370496.0) & 0xfffffffffffffull;
@@ -170,14 +170,14 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ u64 block_sum_u64(Shared& s, u64 v) {
-    v = warp_sum_u64(v);
-    if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = v;
+// (of two numbers at once)
+__device__ __forceinline__ void block_sum_u64(Shared& s, u64& v, u64& w) {
+    const int lane = threadIdx.x & 31;
+    v = warp_sum_u64(v), w = warp_sum_u64(w);
+    if (lane == 0) s.red[0][threadIdx.x >> 5] = v, s.red[1][threadIdx.x >> 5] = w;
     __syncthreads();
-    u64 t = 0;
-    for (int w = 0; w < WARPS; ++w) t += s.red[w];
+    v = warp_sum_u64(lane < WARPS ? s.red[0][lane] : 0), w = warp_sum_u64(lane < WARPS ? s.red[1][lane] : 0);
     __syncthreads();
-    return t;
 }
 __device__ __forceinline__ u64 row_sum_u64(const u64* at) {
     const u32 lane = threadIdx.x & 31;
@@ -187,14 +187,12 @@ __device__ __forceinline__ float row_value(const float* at, float none) {
     const u32 lane = threadIdx.x & 31;
     return lane < cluster_blocks() ? __uint_as_float(ld_peer_shared_u32(at, lane)) : none;
 }
-__device__ __forceinline__ float block_max(Shared& s, float v) {
+// (`place`: every call its own)
+__device__ __forceinline__ float block_max(Shared& s, int place, float v) {
     v = warp_max(v);
-    if ((threadIdx.x & 31) == 0) s.fred[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) s.fred[place][threadIdx.x >> 5] = v;
     __syncthreads();
-    v = s.fred[0];
-    for (int w = 1; w < WARPS; ++w) v = fmaxf(v, s.fred[w]);
-    __syncthreads();
-    return v;
+    return warp_max(s.fred[place][threadIdx.x & (WARPS - 1)]);
 }
 
 // Which elements a search goes through: those between two logits, of a bin of the linear histogram, whose keys begin with some digits.
@@ -203,7 +201,7 @@ struct Subset {
     int bin = -1;  // -1: all
     u64 prefix = 0;
     int digits = 0;  // of the prefix
-    static __device__ __forceinline__ int shift(int digit) { return 64 - DIGIT * (digit + 1); }  // (the last digit has four bits: below nought)
+    static __device__ __forceinline__ int shift(int digit) { return 64 - DIGIT * (digit + 1); }  // (the last digit has one bit: below nought)
     static __device__ __forceinline__ int value(u64 key, int digit) {
         const int s = shift(digit);
         return (int)((s >= 0 ? key >> s : key << -s) & (BINS - 1));
@@ -229,27 +227,48 @@ __device__ void add_up(Shared& s) {
 #pragma unroll
         for (int k = 0; k < MOST_BLOCKS; ++k) {
             cc[k] = k < (int)blocks ? ld_peer_shared_u32(&s.count[b], k) : 0;
-            mm[k] = MASS && k < (int)blocks ? ld_peer_shared_u64(&s.mass[b], k) : 0;
+            mm[k] = 0;
+            if (MASS && k < (int)blocks)
+                mm[k] = ld_peer_shared_u32(&s.mass[0][b], k) + ((u64)ld_peer_shared_u32(&s.mass[1][b], k) << 16) + ((u64)ld_peer_shared_u32(&s.mass[2][b], k) << 32);
         }
 #pragma unroll
         for (int k = 0; k < MOST_BLOCKS; ++k) c += cc[k], m += mm[k];
     }
     if (threadIdx.x < OWN_BINS) s.own_count[threadIdx.x] = (u32)c, s.own_mass[threadIdx.x] = m;  // (nought behind its bins)
-    c = block_sum_u64(s, c);
-    if (MASS) m = block_sum_u64(s, m);
+    block_sum_u64(s, c, m);
     if (threadIdx.x == 0) s.total_count = c, s.total_mass = m;
     cluster_sync();  // the sums are there; nobody reads the blocks' histograms any more
 }
 
 __device__ __forceinline__ void clear(Shared& s) {
-    for (int b = threadIdx.x; b < BINS; b += THREADS) s.count[b] = 0, s.mass[b] = 0;
+    for (int b = threadIdx.x; b < BINS; b += THREADS) s.count[b] = 0, s.mass[0][b] = 0, s.mass[1][b] = 0, s.mass[2][b] = 0;
     __syncthreads();
+}
+
+// An element into its bin: sums of sixteen bits of no more than MOST_ELEMENTS of them fit 32.
+__device__ __forceinline__ void put(Shared& s, int b, u64 mass) {
+    atomicAdd(&s.count[b], 1u);
+    atomicAdd(&s.mass[0][b], (u32)mass & 0xffffu);
+    atomicAdd(&s.mass[1][b], (u32)(mass >> 16) & 0xffffu);
+    atomicAdd(&s.mass[2][b], (u32)(mass >> 32));
+}
+
+// A thread's elements of bin 0, which nobody else puts there.
+__device__ __forceinline__ void put_low(Shared& s, u32 count, u64 mass) {
+    count = __reduce_add_sync(0xffffffffu, count), mass = warp_sum_u64(mass);
+    if ((threadIdx.x & 31) == 0 && count) {
+        atomicAdd(&s.count[0], count);
+        // (what lies above 2^48 stays in the upper part: all masses of a row together are below 2^63)
+        atomicAdd(&s.mass[0][0], (u32)mass & 0xffffu);
+        atomicAdd(&s.mass[1][0], (u32)(mass >> 16) & 0xffffu);
+        atomicAdd(&s.mass[2][0], (u32)(mass >> 32));
+    }
 }
 
 // The histogram of a subset over the whole row: linear, or of elements of one bin by the next digit of their keys.
 __device__ void histogram(Shared& s, const Row& r, const Subset& in) {
     clear(s);
-    u32 low = 0;  // what falls into bin 0 of the linear histogram, mostly far below all others: added up first
+    u32 low = 0;  // what falls into bin 0 of the linear histogram, mostly far below all others, is counted first
     u64 low_mass = 0;
     for (int i = threadIdx.x; i < r.n; i += THREADS) {
         const float l = r.logit(i);
@@ -258,15 +277,10 @@ __device__ void histogram(Shared& s, const Row& r, const Subset& in) {
         const u64 m = r.mass(l);
         if (in.bin < 0 && b == 0)
             ++low, low_mass += m;
-        else {
-            atomicAdd(&s.count[b], 1u);
-            atomicAdd(&s.mass[b], m);
-        }
+        else
+            put(s, b, m);
     }
-    if (low) {
-        atomicAdd(&s.count[0], low);
-        atomicAdd(&s.mass[0], low_mass);
-    }
+    put_low(s, low, low_mass);
     add_up<true>(s);
 }
 
@@ -336,19 +350,27 @@ __device__ u32 gather(Shared& s, const Row& r, Take take) {
         if (at < LIST) s.list[at].key = key_of(l, r.lo + i), s.list[at].mass = r.mass(l);
     }
     cluster_sync();
+    // thread t takes the row's element t, wherever it lies
     const u32 lane = threadIdx.x & 31, blocks = cluster_blocks();
-    const u32 mine = lane < blocks ? ld_peer_shared_u32(&s.listed, lane) : 0;
-    u32 offset = 0;
-    for (u32 k = 0; k < blocks; ++k) {
-        const u32 n = __shfl_sync(0xffffffffu, mine, k);
-        for (u32 i = threadIdx.x; i < n && i < LIST && offset + i < LIST; i += THREADS) {
-            s.all[offset + i].key = ld_peer_shared_u64(&s.list[i].key, k);
-            s.all[offset + i].mass = ld_peer_shared_u64(&s.list[i].mass, k);
-        }
-        offset += n;
+    u32 upto = lane < blocks ? ld_peer_shared_u32(&s.listed, lane) : 0;
+#pragma unroll
+    for (int o = 1; o < MOST_BLOCKS; o <<= 1) {
+        const u32 x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= (u32)o) upto += x;
+    }
+    const u32 total = __shfl_sync(0xffffffffu, upto, MOST_BLOCKS - 1);
+    u32 from = 0, before = 0;
+#pragma unroll
+    for (int k = 0; k < MOST_BLOCKS - 1; ++k) {
+        const u32 x = __shfl_sync(0xffffffffu, upto, k);
+        if (threadIdx.x >= x) from = k + 1, before = x;
+    }
+    if (threadIdx.x < total && threadIdx.x - before < LIST) {
+        s.all[threadIdx.x].key = ld_peer_shared_u64(&s.list[threadIdx.x - before].key, from);
+        s.all[threadIdx.x].mass = ld_peer_shared_u64(&s.list[threadIdx.x - before].mass, from);
     }
     cluster_sync();  // the lists are complete, and nobody's own is read any more
-    return offset;
+    return total;
 }
 
 // Of this thread's element of the n in s.all: how many lie before it, and their mass.
@@ -443,34 +465,38 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
     r.at = KEEP ? kept : logits + r.lo;
     r.rate = LOG2E / (double)T;
     const bool wide_in = (((uintptr_t)(logits + r.lo)) & 15) == 0, wide_out = (((uintptr_t)(out + r.lo)) & 15) == 0;
-    // the greatest logit: the thread's, the block's, the row's
+    const bool by_k = !greedy && k > 0 && k < a.vocab, by_p = !greedy && p < 1.0f;
+    // the row's share on its way, all of it at once
+    if (KEEP) {
+        const uint32_t to = smem_u32(kept);
+        const int whole = wide_in ? r.n & ~3 : 0;
+        for (int i = 4 * threadIdx.x; i < whole; i += 4 * THREADS)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * i), "l"(logits + r.lo + i) : "memory");
+        for (int i = whole + threadIdx.x; i < r.n; i += THREADS)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * i), "l"(logits + r.lo + i) : "memory");
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    // the greatest logit: the thread's (of those that it has fetched itself), the block's, the row's
     float mine = -INFINITY;
     for_elements(
         r.n, wide_in,
         [&](int i) {
-            const float4 v = *reinterpret_cast<const float4*>(logits + r.lo + i);
-            if (KEEP) *reinterpret_cast<float4*>(kept + i) = v;
+            const float4 v = *reinterpret_cast<const float4*>(r.at + i);
             mine = fmaxf(fmaxf(mine, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
         },
-        [&](int i) {
-            const float l = logits[r.lo + i];
-            if (KEEP) kept[i] = l;
-            mine = fmaxf(mine, l);
-        });
-    const float block_top = block_max(s, mine);
-    // the least finite maximum of a thread
+        [&](int i) { mine = fmaxf(mine, r.at[i]); });
+    const float block_top = block_max(s, 0, mine);
+    // (for top-k) the least finite maximum of a thread
     const int quads = wide_in ? r.n & ~3 : 0;
     const bool has = 4 * (int)threadIdx.x < quads || quads + (int)threadIdx.x < r.n;
-    const float block_least = -block_max(s, mine > -INFINITY ? -mine : -INFINITY);
+    const float block_least = by_k ? -block_max(s, 1, mine > -INFINITY ? -mine : -INFINITY) : 0.0f;
     if (threadIdx.x == 0) s.value[0] = block_top, s.value[1] = block_least;
     cluster_sync();
     r.given_top = warp_max(row_value(&s.value[0], -INFINITY));
     r.infinite = isinf(r.given_top);
     r.top = r.high = r.infinite ? 0.0f : r.given_top;
     r.least = r.top - 60.0f * T;
-    const float least = -warp_max(-row_value(&s.value[1], INFINITY));
     out += r.lo;
-    const bool by_k = !greedy && k > 0 && k < a.vocab, by_p = !greedy && p < 1.0f;
     if (greedy) {
         // the first index among those of the greatest logit
         u32 first = 0xffffffffu;
@@ -505,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
                 if (KEEP) kept[i] = w;
                 sum += w;
             });
-        sum = block_sum(sum, s.fred);  // (ends with a barrier: the weights are there for all)
+        sum = block_sum(sum, s.scratch);  // (ends with a barrier: the weights are there for all)
         if (threadIdx.x == 0) s.value[2] = sum;
         cluster_sync();
         const float inv = 1.0f / warp_sum(row_value(&s.value[2], 0.0f));
@@ -530,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
         Subset all;
         if (by_k && k <= LIST) {
             // the k-th of the threads' maxima: no fewer than k logits lie in its bin and above
-            set_range(r.top - least);
+            set_range(r.top - -warp_max(-row_value(&s.value[1], INFINITY)));
             clear(s);
             if (has) atomicAdd(&s.count[r.bin(r.number(mine))], 1u);
             add_up<false>(s);
@@ -565,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
                 const float l = r.logit(i);
                 if (l > -INFINITY) low = fminf(low, l);
             }
-            low = -block_max(s, -low);
+            low = -block_max(s, 2, -low);
             if (threadIdx.x == 0) s.value[3] = low;
             cluster_sync();
             set_range(r.top - -warp_max(-row_value(&s.value[3], INFINITY)));
@@ -631,16 +657,11 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
                 const int b = r.bin(l);
                 if (b == 0)
                     ++low, low_mass += m;
-                else {
-                    atomicAdd(&s.count[b], 1u);
-                    atomicAdd(&s.mass[b], m);
-                }
+                else
+                    put(s, b, m);
             }
-            if (low) {
-                atomicAdd(&s.count[0], low);
-                atomicAdd(&s.mass[0], low_mass);
-            }
-            over = block_sum_u64(s, over), sum = block_sum_u64(s, sum);
+            put_low(s, low, low_mass);
+            block_sum_u64(s, over, sum);
             if (threadIdx.x == 0) s.over = over, s.sum = sum;
             add_up<true>(s);
             over = row_sum_u64(&s.over), sum = row_sum_u64(&s.sum);
@@ -648,12 +669,12 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
             const Quantile q = quantile(s, r, in, false, (aim ? aim : 1) - over);
             threshold = q.key, mass = over + q.mass;
         }
-        const double inv = UNIT / (double)mass;
-        const float floor_logit = logit_of((u32)(threshold >> 32));
+        // (which tokens stay is decided; their probabilities in 32 bits, as without top-k and top-p)
+        const float inv = (float)(UNIT / (double)mass), rate = (float)r.rate, border = logit_of((u32)(threshold >> 32));
         auto of = [&](float l, int i) -> float {
             l = r.number(l);
-            if (l < floor_logit) return 0.0f;
-            return key_of(l, r.lo + i) >= threshold ? (float)(r.weight(l) * inv) : 0.0f;
+            const float w = exp2_unit((l - r.top) * rate) * inv;
+            return l > border || (l == border && key_of(l, r.lo + i) >= threshold) ? w : 0.0f;
         };
         for_elements(
             r.n, wide_out && KEEP,
@@ -672,7 +693,8 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
 FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* out, long long ldo, int rows, int vocab, const float* temperature,
                                      const int* top_k, const float* top_p, void* stream) {
     if (rows <= 0) return FERRIS_OK;
-    if (vocab <= 0 || ldl < vocab || ldo < vocab || vocab > 0x7fffffff - 64) FERRIS_REFUSE("vocabulary %d, row strides %lld and %lld", vocab, ldl, ldo);
+    if (vocab <= 0 || ldl < vocab || ldo < vocab) FERRIS_REFUSE("vocabulary %d, row strides %lld and %lld", vocab, ldl, ldo);
+    if (vocab > MOST_BLOCKS * MOST_ELEMENTS) FERRIS_REFUSE("a vocabulary of %d, at most %d", vocab, MOST_BLOCKS * MOST_ELEMENTS);
     // Blocks of a row: of as many as give the least time if blocks run in waves, each as long as its share of the row (40 rows of 151,936: seven, 280 blocks at once,
     // where eight would leave 24 of them for a second wave).
     const int sms = ferris_sm_count();
@@ -684,7 +706,7 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
         const size_t bytes = (size_t)per_block(b) * 4 + fixed;
         const long long at_once = (bytes <= most / 2 || bytes > most ? 2ll : 1ll) * (sms > 0 ? sms : 148);
         const double time = (double)(((long long)rows * b + at_once - 1) / at_once) / b;
-        if (b == MOST_BLOCKS || time < least) least = time, blocks = b;
+        if (b == MOST_BLOCKS || (time < least && per_block(b) <= MOST_ELEMENTS)) least = time, blocks = b;
     }
     SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks)};
     const size_t bytes = (size_t)a.per * 4;

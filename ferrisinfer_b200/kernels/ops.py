@@ -2772,7 +2772,7 @@ def _tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nod
 
 def sampling_probs(logits: torch.Tensor, out: torch.Tensor, temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
                    top_p: Optional[torch.Tensor] = None):
-    """out[r] = the probabilities that ``sample`` draws row r's token from: fp32 [n, V] for fp32 ``logits`` [n, V] (rows contiguous; ``out`` may be
+    """out[r] = the probabilities that ``sample`` draws row r's token from: fp32 [n, V] for fp32 ``logits`` [n, V] (V at most 524,288; rows contiguous; ``out`` may be
     ``logits``, or memory apart from it).
 
     Per row (fp32, int32, fp32 [n]): ``temperature`` (not above 0: 1 at the greatest logit, the first among equals; so too without it, with top_k 1 and with

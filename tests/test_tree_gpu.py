@@ -669,6 +669,8 @@ def test_refusals(ops, workspace):
         ops.sampling_probs(flat[:400].view(4, 100), flat[10:410].view(4, 100))
     with pytest.raises(KernelError, match="overlap"):
         ops.sampling_probs(logits, flat[:100].expand(4, 100))
+    with pytest.raises(KernelError, match="524288"):
+        ops.sampling_probs(torch.zeros(1, 524289, device=DEV), torch.zeros(1, 524289, device=DEV))
     with pytest.raises(KernelError, match="top_k"):
         ops.sampling_probs(logits, torch.zeros_like(logits), torch.ones(4, device=DEV), torch.ones(4, device=DEV))
     with pytest.raises(KernelError, match="one device"):

@@ -65,6 +65,7 @@ struct SamplingProbs {
     const int* top_k;
     const float* top_p;
     int vocab, per;  // elements of a block
+    int skip;        // rows without top-k and top-p are another kernel's
 };
 
 struct Found {
@@ -446,6 +447,13 @@ __device__ __forceinline__ void for_elements(int n, bool wide, Four four, One on
     for (int i = whole + threadIdx.x; i < n; i += THREADS) one(i);
 }
 
+// Whether a row is sampled from as it is, without top-k and top-p.
+__device__ __forceinline__ bool plain_row(const SamplingProbs& a, int row) {
+    const int k = a.top_k ? a.top_k[row] : 0;  // (all three on their way together)
+    const float T = a.temperature ? a.temperature[row] : 0.0f, p = a.top_p ? a.top_p[row] : 1.0f;
+    return (T > 0.0f) & (k <= 0 || (k >= a.vocab && k != 1)) & (p >= 1.0f);
+}
+
 template <bool KEEP>  // the block's elements fit shared memory
 __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const SamplingProbs a) {
     __shared__ Shared s;
@@ -453,6 +461,7 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
     pdl_wait();
     pdl_launch_dependents();
     const int row = blockIdx.x;
+    if (a.skip && plain_row(a, row)) return;
     const u32 rank = cluster_ctarank();
     const float* logits = a.logits + (long long)row * a.ldl;
     float* out = a.out + (long long)row * a.ldo;
@@ -687,6 +696,83 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
     cluster_sync();  // nobody leaves while others may read its shared memory
 }
 
+// ---------------------------------------------------------------------------------------------
+// Many rows without top-k and top-p: a cluster of up to sixteen blocks a row, of which five or six share an SM, so that some wait for their shares while others
+// exponentiate and write.  A block exponentiates against its own greatest logit; blocks meet once, for their greatest logits and sums.
+// ---------------------------------------------------------------------------------------------
+constexpr int PLAIN_THREADS = 256, PLAIN_WARPS = PLAIN_THREADS / 32, PLAIN_SHARE = 10240;  // threads; elements of a block, if sixteen blocks will do
+
+__global__ void __launch_bounds__(PLAIN_THREADS) sampling_softmax_kernel(const SamplingProbs a) {
+    extern __shared__ __align__(16) float x[];
+    __shared__ float value[2], part[2][PLAIN_WARPS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int row = blockIdx.x, lane = threadIdx.x & 31;
+    const float* logits = a.logits + row * a.ldl;
+    const int lo = min(a.vocab, (int)cluster_ctarank() * a.per), n = min(a.vocab, lo + a.per) - lo;
+    if (!plain_row(a, row)) return;
+    logits += lo;
+    const uint32_t at = smem_u32(x);
+    const int wide = ((uintptr_t)logits & 15) == 0 ? n & ~3 : 0;
+    for (int i = 4 * threadIdx.x; i < wide; i += 4 * PLAIN_THREADS)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + 4 * i), "l"(logits + i) : "memory");
+    for (int i = wide + threadIdx.x; i < n; i += PLAIN_THREADS)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 4 * i), "l"(logits + i) : "memory");
+    const float rate = (float)(LOG2E / (double)fminf(fmaxf(a.temperature[row], FLT_EPSILON), 1e30f));
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    const int whole = n & ~3;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int i = 4 * threadIdx.x; i < whole; i += 4 * PLAIN_THREADS) {
+        const float4 v = *reinterpret_cast<const float4*>(x + i);
+        top = fmaxf(fmaxf(top, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+    }
+    for (int i = whole + threadIdx.x; i < n; i += PLAIN_THREADS) top = fmaxf(top, x[i]);
+    top = warp_max(top);
+    if (lane == 0) part[0][threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = warp_max(part[0][lane & (PLAIN_WARPS - 1)]);
+    // (of an infinite maximum: those that equal it, all alike; a NaN counts as minus infinity)
+    const bool infinite = isinf(top);
+    auto weight = [&](float l) { return infinite ? (fmaxf(l, -INFINITY) == top ? 1.0f : 0.0f) : exp2_unit((fmaxf(l, -INFINITY) - top) * rate); };
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = 4 * threadIdx.x; i < whole; i += 4 * PLAIN_THREADS) {
+        float4 v = *reinterpret_cast<const float4*>(x + i);
+        v = make_float4(weight(v.x), weight(v.y), weight(v.z), weight(v.w));
+        *reinterpret_cast<float4*>(x + i) = v;
+        sum += (v.x + v.y) + (v.z + v.w);
+    }
+    for (int i = whole + threadIdx.x; i < n; i += PLAIN_THREADS) {
+        x[i] = weight(x[i]);
+        sum += x[i];
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) part[1][threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        sum = warp_sum(lane < PLAIN_WARPS ? part[1][lane] : 0.0f);
+        if (lane == 0) value[0] = top, value[1] = sum;
+    }
+    cluster_sync();
+    const float tops = row_value(&value[0], -INFINITY), sums = row_value(&value[1], 0.0f), most = warp_max(tops);
+    cluster_arrive_release();  // (its own values are read: who waits for that may leave)
+    auto factor = [&](float t) { return t == most ? 1.0f : exp2_unit((t - most) * rate); };
+    const float scale = factor(top) / warp_sum(sums * factor(tops));
+    float* out = a.out + row * a.ldo + lo;
+    if (((uintptr_t)out & 15) == 0) {
+#pragma unroll 4
+        for (int i = 4 * threadIdx.x; i < whole; i += 4 * PLAIN_THREADS) {
+            const float4 v = *reinterpret_cast<const float4*>(x + i);
+            *reinterpret_cast<float4*>(out + i) = make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+        }
+        for (int i = whole + threadIdx.x; i < n; i += PLAIN_THREADS) out[i] = x[i] * scale;
+    } else
+        for (int i = threadIdx.x; i < n; i += PLAIN_THREADS) out[i] = x[i] * scale;
+    cluster_wait();
+}
+
 }  // namespace
 
 // logits, out fp32 [rows, vocab] with row strides ldl, ldo: the same memory, or apart.  temperature, top_k, top_p: per row, or null for greedy rows.
@@ -708,9 +794,32 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
         const double time = (double)(((long long)rows * b + at_once - 1) / at_once) / b;
         if (b == MOST_BLOCKS || (time < least && per_block(b) <= MOST_ELEMENTS)) least = time, blocks = b;
     }
-    SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks)};
-    const size_t bytes = (size_t)a.per * 4;
+    SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks), 0};
     cudaError_t e;
+    // More rows than run at once: those without top-k and top-p by the kernel of smaller blocks (of fewer rows the launch would cost more than it saves).
+    int parts = (vocab + PLAIN_SHARE - 1) / PLAIN_SHARE;
+    parts = parts <= 4 ? 4 : parts <= 8 ? 8 : 16;
+    const size_t share = (size_t)per_block(parts) * 4;
+    if ((long long)rows * MOST_BLOCKS > 2ll * sms && share + 2048 <= most && temperature) {
+        const int rc = ferris_allow_dynamic_smem((const void*)sampling_softmax_kernel, share);
+        if (rc != FERRIS_OK) return rc;
+        if (parts > 8) {
+            e = cudaFuncSetAttribute(sampling_softmax_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) {
+                ferris_set_error("%s", cudaGetErrorString(e));
+                return (int)e;
+            }
+        }
+        SamplingProbs b = a;
+        b.per = per_block(parts);
+        e = ferris_launch_cluster(sampling_softmax_kernel, dim3(rows, 1, parts), dim3(PLAIN_THREADS), share, (cudaStream_t)stream, parts, b);
+        if (e != cudaSuccess) {
+            ferris_set_error("%s", cudaGetErrorString(e));
+            return (int)e;
+        }
+        a.skip = 1;
+    }
+    const size_t bytes = (size_t)a.per * 4;
     if (bytes + fixed <= most) {
         const int rc = ferris_allow_dynamic_smem((const void*)sampling_probs_kernel<true>, bytes);
         if (rc != FERRIS_OK) return rc;

@@ -331,6 +331,27 @@ def test_probabilities_of_rows_with_options_of_their_own(ops):
     check_probs(ops, logits_of(7, 5003), [0.0, 1.0, 0.7, 0.5, 1e-9, 3.0, 0.01], [1, 0, 20, 900, 4, 2, 0], [1.0, 1.0, 0.9, 0.8, 1.0, 1.0, 0.5])
 
 
+@pytest.mark.parametrize("V", [7, 1030, 4099])
+def test_probabilities_of_many_rows(ops, V):
+    """(more than run at once, plain ones among others)"""
+    n = 150
+    logits = logits_of(n, V)
+    logits[3], logits[4], logits[5, ::2], logits[6], logits[7] = -math.inf, math.nan, math.nan, 2.5, -math.inf
+    logits[7, V // 2], logits[8, 5], logits[9, V - 1] = 1.0, math.inf, -math.inf
+    options = [(1.0, 0, 1.0), (0.7, 5, 0.9), (0.5, 0, 1.0), (0.0, 0, 1.0), (1.0, 0, 0.8), (2.0, V, 1.0), (1.0, 1, 1.0)]
+    for first in ([(1.0, 0, 1.0)] * n, [options[i % 7] for i in range(n)], [options[1]] * n):
+        check_probs(ops, logits, *zip(*first))
+    wide = torch.zeros(n, V + 9, device=DEV)
+    wide[:, 3:3 + V] = logits
+    want, out = torch.empty_like(logits), torch.full((n, V + 6), 9.0, device=DEV)
+    ops.sampling_probs(logits, want, torch.ones(n, device=DEV))
+    ops.sampling_probs(wide[:, 3:3 + V], out[:, 1:1 + V], torch.ones(n, device=DEV))
+    assert torch.allclose(out[:, 1:1 + V], want, rtol=1e-5, atol=1e-37) and (out[:, 0] == 9).all() and (out[:, 1 + V:] == 9).all()
+    same = logits.clone()
+    ops.sampling_probs(same, same, torch.ones(n, device=DEV))
+    assert torch.equal(same, want)
+
+
 @pytest.mark.parametrize("V", [11, 2048, 20001])
 @pytest.mark.parametrize("top_k, top_p", [(0, 0.5), (5, 1.0), (700, 1.0), (700, 0.25), (0, 1.0), (10, 0.5), (0, 0.125)])
 def test_equal_logits_stay_by_their_index(ops, V, top_k, top_p):

@@ -697,80 +697,83 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows without top-k and top-p: a cluster of up to sixteen blocks a row, of which five or six share an SM, so that some wait for their shares while others
-// exponentiate and write.  A block exponentiates against its own greatest logit; blocks meet once, for their greatest logits and sums.
+// Many rows without top-k and top-p: a cluster of up to sixteen blocks a row, of which four share an SM, so that some wait for their shares while others
+// exponentiate and write.  A thread holds its forty elements in registers and exponentiates against the greatest of them; warps, blocks and the cluster bring their
+// sums to a common maximum, once each.  Blocks hand each other maximum and sum by stores (reading them from the others took 5,000 cycles of 26,000).
 // ---------------------------------------------------------------------------------------------
-constexpr int PLAIN_THREADS = 256, PLAIN_WARPS = PLAIN_THREADS / 32, PLAIN_SHARE = 10240;  // threads; elements of a block, if sixteen blocks will do
+constexpr int PLAIN_THREADS = 256, PLAIN_WARPS = PLAIN_THREADS / 32, PLAIN_QUADS = 10, PLAIN_SHARE = 4 * PLAIN_QUADS * PLAIN_THREADS, PLAIN_BLOCKS = 16;
 
-__global__ void __launch_bounds__(PLAIN_THREADS) sampling_softmax_kernel(const SamplingProbs a) {
-    extern __shared__ __align__(16) float x[];
-    __shared__ float value[2], part[2][PLAIN_WARPS];
+__global__ void __launch_bounds__(PLAIN_THREADS, 4) sampling_softmax_kernel(const SamplingProbs a) {
+    __shared__ float part[2][PLAIN_WARPS], row_part[2][PLAIN_BLOCKS];
+    cluster_arrive_relaxed();
     pdl_wait();
     pdl_launch_dependents();
-    const int row = blockIdx.x, lane = threadIdx.x & 31;
-    const float* logits = a.logits + row * a.ldl;
+    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = cluster_blocks();
     const int lo = min(a.vocab, (int)cluster_ctarank() * a.per), n = min(a.vocab, lo + a.per) - lo;
-    if (!plain_row(a, row)) return;
-    logits += lo;
-    const uint32_t at = smem_u32(x);
-    const int wide = ((uintptr_t)logits & 15) == 0 ? n & ~3 : 0;
-    for (int i = 4 * threadIdx.x; i < wide; i += 4 * PLAIN_THREADS)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + 4 * i), "l"(logits + i) : "memory");
-    for (int i = wide + threadIdx.x; i < n; i += PLAIN_THREADS)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 4 * i), "l"(logits + i) : "memory");
-    const float rate = (float)(LOG2E / (double)fminf(fmaxf(a.temperature[row], FLT_EPSILON), 1e30f));
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-    const int whole = n & ~3;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int i = 4 * threadIdx.x; i < whole; i += 4 * PLAIN_THREADS) {
-        const float4 v = *reinterpret_cast<const float4*>(x + i);
-        top = fmaxf(fmaxf(top, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+    const float* logits = a.logits + row * a.ldl + lo;
+    if (!plain_row(a, row)) {
+        cluster_wait();
+        return;
     }
-    for (int i = whole + threadIdx.x; i < n; i += PLAIN_THREADS) top = fmaxf(top, x[i]);
-    top = warp_max(top);
-    if (lane == 0) part[0][threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = warp_max(part[0][lane & (PLAIN_WARPS - 1)]);
+    const bool wide = ((uintptr_t)logits & 15) == 0;
+    float4 v[PLAIN_QUADS];
+#pragma unroll
+    for (int q = 0; q < PLAIN_QUADS; ++q) {
+        const int i = 4 * (threadIdx.x + q * PLAIN_THREADS);
+        if (wide && i + 4 <= n)
+            v[q] = *reinterpret_cast<const float4*>(logits + i);
+        else
+            v[q] = make_float4(i < n ? logits[i] : -INFINITY, i + 1 < n ? logits[i + 1] : -INFINITY, i + 2 < n ? logits[i + 2] : -INFINITY, i + 3 < n ? logits[i + 3] : -INFINITY);
+    }
+    const float rate = (float)LOG2E / fminf(fmaxf(a.temperature[row], FLT_EPSILON), 1e30f);
+    float top = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < PLAIN_QUADS; ++q) top = fmaxf(fmaxf(top, fmaxf(v[q].x, v[q].y)), fmaxf(v[q].z, v[q].w));
     // (of an infinite maximum: those that equal it, all alike; a NaN counts as minus infinity)
     const bool infinite = isinf(top);
-    auto weight = [&](float l) { return infinite ? (fmaxf(l, -INFINITY) == top ? 1.0f : 0.0f) : exp2_unit((fmaxf(l, -INFINITY) - top) * rate); };
+    auto weight = [&](float l, int i) { return infinite ? (fmaxf(l, -INFINITY) == top && i < n ? 1.0f : 0.0f) : exp2_unit((fmaxf(l, -INFINITY) - top) * rate); };
     float sum = 0.0f;
-#pragma unroll 4
-    for (int i = 4 * threadIdx.x; i < whole; i += 4 * PLAIN_THREADS) {
-        float4 v = *reinterpret_cast<const float4*>(x + i);
-        v = make_float4(weight(v.x), weight(v.y), weight(v.z), weight(v.w));
-        *reinterpret_cast<float4*>(x + i) = v;
-        sum += (v.x + v.y) + (v.z + v.w);
+#pragma unroll
+    for (int q = 0; q < PLAIN_QUADS; ++q) {
+        const int i = 4 * (threadIdx.x + q * PLAIN_THREADS);
+        v[q] = make_float4(weight(v[q].x, i), weight(v[q].y, i + 1), weight(v[q].z, i + 2), weight(v[q].w, i + 3));
+        sum += (v[q].x + v[q].y) + (v[q].z + v[q].w);
     }
-    for (int i = whole + threadIdx.x; i < n; i += PLAIN_THREADS) {
-        x[i] = weight(x[i]);
-        sum += x[i];
-    }
-    sum = warp_sum(sum);
-    if (lane == 0) part[1][threadIdx.x >> 5] = sum;
+    // what a sum against `t` is against `most`
+    auto factor = [&](float t, float most) { return t == most ? 1.0f : exp2_unit((t - most) * rate); };
+    float most = warp_max(top), total = warp_sum(sum * factor(top, most));
+    if (lane == 0) part[0][warp] = most, part[1][warp] = total;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        sum = warp_sum(lane < PLAIN_WARPS ? part[1][lane] : 0.0f);
-        if (lane == 0) value[0] = top, value[1] = sum;
+    cluster_wait();  // (all blocks have begun)
+    if (warp == 0) {
+        const float t = lane < PLAIN_WARPS ? part[0][lane] : -INFINITY, x = lane < PLAIN_WARPS ? part[1][lane] : 0.0f;
+        most = warp_max(t), total = warp_sum(x * factor(t, most));
+        if (lane < blocks) {
+            st_peer_shared_f32(smem_u32(&row_part[0][cluster_ctarank()]), lane, most);
+            st_peer_shared_f32(smem_u32(&row_part[1][cluster_ctarank()]), lane, total);
+        }
     }
     cluster_sync();
-    const float tops = row_value(&value[0], -INFINITY), sums = row_value(&value[1], 0.0f), most = warp_max(tops);
-    cluster_arrive_release();  // (its own values are read: who waits for that may leave)
-    auto factor = [&](float t) { return t == most ? 1.0f : exp2_unit((t - most) * rate); };
-    const float scale = factor(top) / warp_sum(sums * factor(tops));
+    {
+        const float t = lane < blocks ? row_part[0][lane] : -INFINITY, x = lane < blocks ? row_part[1][lane] : 0.0f;
+        most = warp_max(t), total = warp_sum(x * factor(t, most));
+    }
+    const float scale = factor(top, most) / total;
     float* out = a.out + row * a.ldo + lo;
-    if (((uintptr_t)out & 15) == 0) {
-#pragma unroll 4
-        for (int i = 4 * threadIdx.x; i < whole; i += 4 * PLAIN_THREADS) {
-            const float4 v = *reinterpret_cast<const float4*>(x + i);
-            *reinterpret_cast<float4*>(out + i) = make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+    const bool wide_out = ((uintptr_t)out & 15) == 0;
+#pragma unroll
+    for (int q = 0; q < PLAIN_QUADS; ++q) {
+        const int i = 4 * (threadIdx.x + q * PLAIN_THREADS);
+        const float4 w = make_float4(v[q].x * scale, v[q].y * scale, v[q].z * scale, v[q].w * scale);
+        if (wide_out && i + 4 <= n)
+            *reinterpret_cast<float4*>(out + i) = w;
+        else {
+            if (i < n) out[i] = w.x;
+            if (i + 1 < n) out[i + 1] = w.y;
+            if (i + 2 < n) out[i + 2] = w.z;
+            if (i + 3 < n) out[i + 3] = w.w;
         }
-        for (int i = whole + threadIdx.x; i < n; i += PLAIN_THREADS) out[i] = x[i] * scale;
-    } else
-        for (int i = threadIdx.x; i < n; i += PLAIN_THREADS) out[i] = x[i] * scale;
-    cluster_wait();
+    }
 }
 
 }  // namespace
@@ -798,11 +801,8 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
     cudaError_t e;
     // More rows than run at once: those without top-k and top-p by the kernel of smaller blocks (of fewer rows the launch would cost more than it saves).
     int parts = (vocab + PLAIN_SHARE - 1) / PLAIN_SHARE;
-    parts = parts <= 4 ? 4 : parts <= 8 ? 8 : 16;
-    const size_t share = (size_t)per_block(parts) * 4;
-    if ((long long)rows * MOST_BLOCKS > 2ll * sms && share + 2048 <= most && temperature) {
-        const int rc = ferris_allow_dynamic_smem((const void*)sampling_softmax_kernel, share);
-        if (rc != FERRIS_OK) return rc;
+    if ((long long)rows * MOST_BLOCKS > 2ll * sms && per_block(PLAIN_BLOCKS) <= PLAIN_SHARE && temperature) {
+        while (per_block(parts) > PLAIN_SHARE) ++parts;
         if (parts > 8) {
             e = cudaFuncSetAttribute(sampling_softmax_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) {
@@ -812,7 +812,7 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
         }
         SamplingProbs b = a;
         b.per = per_block(parts);
-        e = ferris_launch_cluster(sampling_softmax_kernel, dim3(rows, 1, parts), dim3(PLAIN_THREADS), share, (cudaStream_t)stream, parts, b);
+        e = ferris_launch_cluster(sampling_softmax_kernel, dim3(rows, 1, parts), dim3(PLAIN_THREADS), 0, (cudaStream_t)stream, parts, b);
         if (e != cudaSuccess) {
             ferris_set_error("%s", cudaGetErrorString(e));
             return (int)e;

@@ -65,7 +65,7 @@ struct SamplingProbs {
     const int* top_k;
     const float* top_p;
     int vocab, per;  // elements of a block
-    int skip;        // rows without top-k and top-p are another kernel's
+    int rows, skip;  // skip: rows without top-k and top-p are another kernel's
 };
 
 struct Found {
@@ -454,14 +454,8 @@ __device__ __forceinline__ bool plain_row(const SamplingProbs& a, int row) {
     return (T > 0.0f) & (k <= 0 || (k >= a.vocab && k != 1)) & (p >= 1.0f);
 }
 
-template <bool KEEP>  // the block's elements fit shared memory
-__global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const SamplingProbs a) {
-    __shared__ Shared s;
-    extern __shared__ __align__(16) float kept[];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int row = blockIdx.x;
-    if (a.skip && plain_row(a, row)) return;
+template <bool KEEP>  // the block's elements fit shared memory: `kept`
+__device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, Shared& s, float* kept) {
     const u32 rank = cluster_ctarank();
     const float* logits = a.logits + (long long)row * a.ldl;
     float* out = a.out + (long long)row * a.ldo;
@@ -693,7 +687,21 @@ __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const Sampli
             },
             [&](int i) { out[i] = of(r.at[i], i); });
     }
-    cluster_sync();  // nobody leaves while others may read its shared memory
+    cluster_sync();  // nobody goes on, or leaves, while others may read its shared memory
+}
+
+// A cluster a row, or (`skip`) clusters that go over the rows which are left.
+template <bool KEEP>
+__global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const SamplingProbs a) {
+    __shared__ Shared s;
+    extern __shared__ __align__(16) float kept[];
+    pdl_wait();
+    pdl_launch_dependents();
+    for (int first = blockIdx.x; first < a.rows; first += 32 * gridDim.x) {
+        const int mine = first + (threadIdx.x & 31) * gridDim.x;
+        unsigned here = __ballot_sync(0xffffffffu, mine < a.rows && !(a.skip && plain_row(a, mine)));
+        for (; here; here &= here - 1) probabilities<KEEP>(a, first + (__ffs(here) - 1) * gridDim.x, s, kept);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -797,7 +805,7 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
         const double time = (double)(((long long)rows * b + at_once - 1) / at_once) / b;
         if (b == MOST_BLOCKS || (time < least && per_block(b) <= MOST_ELEMENTS)) least = time, blocks = b;
     }
-    SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks), 0};
+    SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks), rows, 0};
     cudaError_t e;
     // More rows than run at once: those without top-k and top-p by the kernel of smaller blocks (of fewer rows the launch would cost more than it saves).
     int parts = (vocab + PLAIN_SHARE - 1) / PLAIN_SHARE;
@@ -820,12 +828,13 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
         a.skip = 1;
     }
     const size_t bytes = (size_t)a.per * 4;
+    const int at_once = 2 * sms / blocks, clusters = a.skip && at_once < rows ? at_once : rows;
     if (bytes + fixed <= most) {
         const int rc = ferris_allow_dynamic_smem((const void*)sampling_probs_kernel<true>, bytes);
         if (rc != FERRIS_OK) return rc;
-        e = ferris_launch_cluster(sampling_probs_kernel<true>, dim3(rows, 1, blocks), dim3(THREADS), bytes, (cudaStream_t)stream, blocks, a);
+        e = ferris_launch_cluster(sampling_probs_kernel<true>, dim3(clusters, 1, blocks), dim3(THREADS), bytes, (cudaStream_t)stream, blocks, a);
     } else
-        e = ferris_launch_cluster(sampling_probs_kernel<false>, dim3(rows, 1, blocks), dim3(THREADS), 0, (cudaStream_t)stream, blocks, a);
+        e = ferris_launch_cluster(sampling_probs_kernel<false>, dim3(clusters, 1, blocks), dim3(THREADS), 0, (cudaStream_t)stream, blocks, a);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;

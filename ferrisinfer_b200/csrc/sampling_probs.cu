@@ -51,6 +51,16 @@ __device__ __forceinline__ u32 ld_peer_shared_u32(const void* at, u32 rank) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
     return v;
 }
+__device__ __forceinline__ void st_peer_shared_u32(const void* at, u32 rank, u32 v) {
+    u32 remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(at)), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_peer_shared_u64(const void* at, u32 rank, u64 v) {
+    u32 remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(at)), "r"(rank));
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote), "l"(v) : "memory");
+}
 __device__ __forceinline__ u32 cluster_blocks() {
     u32 n;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
@@ -89,13 +99,15 @@ struct Shared {
     Entry all[LIST];  // the row's
     u32 own_count[OWN_BINS];  // the row's, of this block's bins
     u64 own_mass[OWN_BINS];
-    u64 total_count, total_mass;  // of these
+    // what blocks tell each other, by the teller's rank (stores into the others' memory; reading it from there takes thousands of cycles)
+    u64 total_count[MOST_BLOCKS], total_mass[MOST_BLOCKS];  // of its bins
     Found found;
-    float value[4];    // what blocks tell each other, each place once
-    float above[BOUNDS + 1], parts[WARPS][BOUNDS + 1];  // masses above the bounds, and of all
-    u64 over, sum;
-    u32 index;
-    u32 listed;
+    float value[4][MOST_BLOCKS];
+    float above[MOST_BLOCKS][BOUNDS + 1];  // masses above the bounds, and of all
+    u64 over[MOST_BLOCKS], sum[MOST_BLOCKS];
+    u32 index[MOST_BLOCKS], listed[MOST_BLOCKS];
+    float parts[WARPS][BOUNDS + 1];
+    u32 count_listed;
     u64 threshold, retained, kept_mass;
     u64 red[2][WARPS];
     float fred[4][WARPS], scratch[33];
@@ -164,8 +176,8 @@ struct Row {
     }
 };
 
-// Sums over the block and over the row's blocks, for all threads; the one ends behind a barrier of the block, the others want the values
-// to be there (a barrier of the cluster in between).
+// Sums over the block and over the row's blocks, for all threads; the one ends behind a barrier of the block, the others are of what the blocks have told (a
+// barrier of the cluster in between).
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -182,11 +194,24 @@ __device__ __forceinline__ void block_sum_u64(Shared& s, u64& v, u64& w) {
 }
 __device__ __forceinline__ u64 row_sum_u64(const u64* at) {
     const u32 lane = threadIdx.x & 31;
-    return warp_sum_u64(lane < cluster_blocks() ? ld_peer_shared_u64(at, lane) : 0);
+    return warp_sum_u64(lane < cluster_blocks() ? at[lane] : 0);
 }
 __device__ __forceinline__ float row_value(const float* at, float none) {
     const u32 lane = threadIdx.x & 31;
-    return lane < cluster_blocks() ? __uint_as_float(ld_peer_shared_u32(at, lane)) : none;
+    return lane < cluster_blocks() ? at[lane] : none;
+}
+// By all threads of the first warp: a number of this block's to all of the row's.
+__device__ __forceinline__ void tell(float* at, float v) {
+    const u32 lane = threadIdx.x & 31;
+    if (lane < cluster_blocks()) st_peer_shared_u32(at + cluster_ctarank(), lane, __float_as_uint(v));
+}
+__device__ __forceinline__ void tell(u32* at, u32 v) {
+    const u32 lane = threadIdx.x & 31;
+    if (lane < cluster_blocks()) st_peer_shared_u32(at + cluster_ctarank(), lane, v);
+}
+__device__ __forceinline__ void tell(u64* at, u64 v) {
+    const u32 lane = threadIdx.x & 31;
+    if (lane < cluster_blocks()) st_peer_shared_u64(at + cluster_ctarank(), lane, v);
 }
 // (`place`: every call its own)
 __device__ __forceinline__ float block_max(Shared& s, int place, float v) {
@@ -237,7 +262,7 @@ __device__ void add_up(Shared& s) {
     }
     if (threadIdx.x < OWN_BINS) s.own_count[threadIdx.x] = (u32)c, s.own_mass[threadIdx.x] = m;  // (nought behind its bins)
     block_sum_u64(s, c, m);
-    if (threadIdx.x == 0) s.total_count = c, s.total_mass = m;
+    if (threadIdx.x < 32) tell(s.total_count, c), tell(s.total_mass, m);
     cluster_sync();  // the sums are there; nobody reads the blocks' histograms any more
 }
 
@@ -290,7 +315,7 @@ __device__ void histogram(Shared& s, const Row& r, const Subset& in) {
 __device__ Found find_bin(Shared& s, bool by_count, u64 aim) {
     const int lane = threadIdx.x & 31, blocks = cluster_blocks();
     // the blocks' sums, the last block (which has the highest bins) first
-    const u64 count = lane < blocks ? ld_peer_shared_u64(&s.total_count, blocks - 1 - lane) : 0, mass = lane < blocks ? ld_peer_shared_u64(&s.total_mass, blocks - 1 - lane) : 0;
+    const u64 count = lane < blocks ? s.total_count[blocks - 1 - lane] : 0, mass = lane < blocks ? s.total_mass[blocks - 1 - lane] : 0;
     u64 upto_c = count, upto_m = mass;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -324,36 +349,36 @@ __device__ Found find_bin(Shared& s, bool by_count, u64 aim) {
             ac += n, am += s.own_mass[top - k];
         }
         const unsigned any = __ballot_sync(0xffffffffu, bin >= 0);
-        if (any ? lane == 31 - __clz(any) : lane == 0) {
-            s.found.bin = owner * BINS / blocks + max(bin, 0);
-            s.found.count = s.own_count[max(bin, 0)];
-            s.found.before_count = bc, s.found.before_mass = bm;
+        const int from = any ? 31 - __clz(any) : 0;
+        bin = max(__shfl_sync(0xffffffffu, bin, from), 0), bc = __shfl_sync(0xffffffffu, bc, from), bm = __shfl_sync(0xffffffffu, bm, from);
+        if (lane < blocks) {
+            st_peer_shared_u32(&s.found.bin, lane, owner * BINS / blocks + bin);
+            st_peer_shared_u32(&s.found.count, lane, s.own_count[bin]);
+            st_peer_shared_u64(&s.found.before_count, lane, bc);
+            st_peer_shared_u64(&s.found.before_mass, lane, bm);
         }
     }
     cluster_sync();
-    Found f;
-    f.bin = (int)ld_peer_shared_u32(&s.found.bin, owner);
-    f.count = ld_peer_shared_u32(&s.found.count, owner);
-    f.before_count = ld_peer_shared_u64(&s.found.before_count, owner);
-    f.before_mass = ld_peer_shared_u64(&s.found.before_mass, owner);
-    return f;
+    return s.found;
 }
 
 // The elements for which take(l, i) holds into s.all of every block: how many of them there are in the row (if more than LIST, some are missing).
 template <typename Take>
 __device__ u32 gather(Shared& s, const Row& r, Take take) {
-    if (threadIdx.x == 0) s.listed = 0;
+    if (threadIdx.x == 0) s.count_listed = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < r.n; i += THREADS) {
         const float l = r.logit(i);
         if (!take(l, r.lo + i)) continue;
-        const u32 at = atomicAdd(&s.listed, 1u);
+        const u32 at = atomicAdd(&s.count_listed, 1u);
         if (at < LIST) s.list[at].key = key_of(l, r.lo + i), s.list[at].mass = r.mass(l);
     }
+    __syncthreads();
+    if (threadIdx.x < 32) tell(s.listed, s.count_listed);
     cluster_sync();
     // thread t takes the row's element t, wherever it lies
     const u32 lane = threadIdx.x & 31, blocks = cluster_blocks();
-    u32 upto = lane < blocks ? ld_peer_shared_u32(&s.listed, lane) : 0;
+    u32 upto = lane < blocks ? s.listed[lane] : 0;
 #pragma unroll
     for (int o = 1; o < MOST_BLOCKS; o <<= 1) {
         const u32 x = __shfl_up_sync(0xffffffffu, upto, o);
@@ -493,9 +518,9 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
     const int quads = wide_in ? r.n & ~3 : 0;
     const bool has = 4 * (int)threadIdx.x < quads || quads + (int)threadIdx.x < r.n;
     const float block_least = by_k ? -block_max(s, 1, mine > -INFINITY ? -mine : -INFINITY) : 0.0f;
-    if (threadIdx.x == 0) s.value[0] = block_top, s.value[1] = block_least;
+    if (threadIdx.x < 32) tell(s.value[0], block_top), tell(s.value[1], block_least);
     cluster_sync();
-    r.given_top = warp_max(row_value(&s.value[0], -INFINITY));
+    r.given_top = warp_max(row_value(s.value[0], -INFINITY));
     r.infinite = isinf(r.given_top);
     r.top = r.high = r.infinite ? 0.0f : r.given_top;
     r.least = r.top - 60.0f * T;
@@ -506,12 +531,14 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
         for (int i = threadIdx.x; i < r.n; i += THREADS)
             if (r.logit(i) == r.top) first = min(first, (u32)(r.lo + i));
         first = __reduce_min_sync(0xffffffffu, first);
-        if (threadIdx.x == 0) s.index = 0xffffffffu;
+        if (threadIdx.x == 0) s.count_listed = 0xffffffffu;
         __syncthreads();
-        if ((threadIdx.x & 31) == 0) atomicMin(&s.index, first);
+        if ((threadIdx.x & 31) == 0) atomicMin(&s.count_listed, first);
+        __syncthreads();
+        if (threadIdx.x < 32) tell(s.index, s.count_listed);
         cluster_sync();
         const u32 lane = threadIdx.x & 31;
-        first = __reduce_min_sync(0xffffffffu, lane < cluster_blocks() ? ld_peer_shared_u32(&s.index, lane) : 0xffffffffu) - (u32)r.lo;
+        first = __reduce_min_sync(0xffffffffu, lane < cluster_blocks() ? s.index[lane] : 0xffffffffu) - (u32)r.lo;
         auto of = [&](int i) { return (u32)i == first ? 1.0f : 0.0f; };
         for_elements(
             r.n, wide_out, [&](int i) { *reinterpret_cast<float4*>(out + i) = make_float4(of(i), of(i + 1), of(i + 2), of(i + 3)); },
@@ -535,9 +562,9 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
                 sum += w;
             });
         sum = block_sum(sum, s.scratch);  // (ends with a barrier: the weights are there for all)
-        if (threadIdx.x == 0) s.value[2] = sum;
+        if (threadIdx.x < 32) tell(s.value[2], sum);
         cluster_sync();
-        const float inv = 1.0f / warp_sum(row_value(&s.value[2], 0.0f));
+        const float inv = 1.0f / warp_sum(row_value(s.value[2], 0.0f));
         auto of = [&](int i) { return (KEEP ? kept[i] : weight(r.at[i])) * inv; };
         for_elements(
             r.n, wide_out,
@@ -559,11 +586,11 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
         Subset all;
         if (by_k && k <= LIST) {
             // the k-th of the threads' maxima: no fewer than k logits lie in its bin and above
-            set_range(r.top - -warp_max(-row_value(&s.value[1], INFINITY)));
+            set_range(r.top - -warp_max(-row_value(s.value[1], INFINITY)));
             clear(s);
             if (has) atomicAdd(&s.count[r.bin(r.number(mine))], 1u);
             add_up<false>(s);
-            const u64 threads = row_sum_u64(&s.total_count);
+            const u64 threads = row_sum_u64(s.total_count);
             if (threads >= (u64)k) {
                 const Found f = find_bin(s, true, (u64)k);
                 const int n = (int)gather(s, r, [&](float l, int) { return r.bin(l) >= f.bin; });
@@ -595,9 +622,9 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
                 if (l > -INFINITY) low = fminf(low, l);
             }
             low = -block_max(s, 2, -low);
-            if (threadIdx.x == 0) s.value[3] = low;
+            if (threadIdx.x < 32) tell(s.value[3], low);
             cluster_sync();
-            set_range(r.top - -warp_max(-row_value(&s.value[3], INFINITY)));
+            set_range(r.top - -warp_max(-row_value(s.value[3], INFINITY)));
             histogram(s, r, all);
             const Quantile q = quantile(s, r, all, true, (u64)k);
             threshold = q.key, mass = q.mass;
@@ -628,15 +655,21 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
                 if ((threadIdx.x & 31) == 0) s.parts[threadIdx.x >> 5][b] = t;
             }
             __syncthreads();
-            if (threadIdx.x <= BOUNDS) {
+            if (threadIdx.x < MOST_BLOCKS * (BOUNDS + 1)) {
+                const u32 b = threadIdx.x % (BOUNDS + 1), to = threadIdx.x / (BOUNDS + 1);
                 float t = 0.0f;
-                for (int w = 0; w < WARPS; ++w) t += s.parts[w][threadIdx.x];
-                s.above[threadIdx.x] = t;
+                for (int w = 0; w < WARPS; ++w) t += s.parts[w][b];
+                if (to < cluster_blocks()) st_peer_shared_u32(&s.above[cluster_ctarank()][b], to, __float_as_uint(t));
             }
             cluster_sync();
+            {
+                const int b = threadIdx.x % (BOUNDS + 1);
+                float t = 0.0f;
+                for (u32 k = 0; k < cluster_blocks(); ++k) t += s.above[k][b];
 #pragma unroll
-            for (int b = 0; b < BOUNDS; ++b) above[b] = warp_sum(row_value(&s.above[b], 0.0f));
-            all_mass = warp_sum(row_value(&s.above[BOUNDS], 0.0f));
+                for (int c = 0; c < BOUNDS; ++c) above[c] = __shfl_sync(0xffffffffu, t, c);
+                all_mass = __shfl_sync(0xffffffffu, t, BOUNDS);
+            }
             Subset in;
             in.high = r.top;
 #pragma unroll
@@ -665,9 +698,9 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             }
             put_low(s, low, low_mass);
             block_sum_u64(s, over, sum);
-            if (threadIdx.x == 0) s.over = over, s.sum = sum;
+            if (threadIdx.x < 32) tell(s.over, over), tell(s.sum, sum);
             add_up<true>(s);
-            over = row_sum_u64(&s.over), sum = row_sum_u64(&s.sum);
+            over = row_sum_u64(s.over), sum = row_sum_u64(s.sum);
             const u64 aim = share_of(sum, p);
             const Quantile q = quantile(s, r, in, false, (aim ? aim : 1) - over);
             threshold = q.key, mass = over + q.mass;
@@ -695,6 +728,7 @@ template <bool KEEP>
 __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const SamplingProbs a) {
     __shared__ Shared s;
     extern __shared__ __align__(16) float kept[];
+    cluster_sync();  // (all blocks have begun: their memory may be written)
     pdl_wait();
     pdl_launch_dependents();
     for (int first = blockIdx.x; first < a.rows; first += 32 * gridDim.x) {

@@ -108,6 +108,7 @@ struct Shared {
     u32 index[MOST_BLOCKS], listed[MOST_BLOCKS];
     float parts[WARPS][BOUNDS + 1];
     u32 count_listed;
+    double powers[32];
     u64 threshold, retained, kept_mass;
     u64 red[2][WARPS];
     float fred[4][WARPS], scratch[33];
@@ -127,54 +128,70 @@ __device__ __forceinline__ float exp2_unit(float x) {
     return r;
 }
 
-// 2^(y + up) for -100 <= y <= 0, up to 2^-46 of itself: the nearest whole number apart, and the Taylor polynomial of 2^f for |f| <= 1/2, whose
-// twelfth term is 6e-15.
-__device__ __forceinline__ double exp2_64(double y, int up) {
+__device__ const double powers_of_two[32] = {  // 2^(j / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+
+// 2^(z / 32 + up) for -3200 <= z <= 0, up to 2^-46 of itself: the nearest whole number apart, of which five bits choose one of 2^(0/32) .. 2^(31/32) (`powers`) and the
+// others are the exponent, and the Taylor polynomial of 2^(f / 32) for |f| <= 1/2, whose sixth term is 2e-15.
+__device__ __forceinline__ double exp2_64(double z, int up, const double* powers) {
     const double magic = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to a whole number
-    const double t = y + magic, f = y - (t - magic);
-    double r = 4.44553827187081e-10;  // ln(2)^k / k! for k = 11 .. 0
-    r = fma(r, f, 7.054911620801121e-09);
-    r = fma(r, f, 1.0178086009239696e-07);
-    r = fma(r, f, 1.3215486790144305e-06);
-    r = fma(r, f, 1.5252733804059838e-05);
-    r = fma(r, f, 0.00015403530393381606);
-    r = fma(r, f, 0.0013333558146428441);
-    r = fma(r, f, 0.009618129107628477);
-    r = fma(r, f, 0.055504108664821576);
-    r = fma(r, f, 0.2402265069591007);
-    r = fma(r, f, 0.6931471805599453);
+    const double t = z + magic, f = z - (t - magic);
+    double r = 3.9737099845494154e-11;  // (ln(2) / 32)^k / k! for k = 5 .. 0
+    r = fma(r, f, 9.172562701824643e-09);
+    r = fma(r, f, 1.6938509724371819e-06);
+    r = fma(r, f, 0.00023459619820224677);
+    r = fma(r, f, 0.02166084939249829);
     r = fma(r, f, 1.0);
-    return __hiloint2double(__double2hiint(r) + (__double2loint(t) + up) * (1 << 20), __double2loint(r));
+    const int n = __double2loint(t);
+    const double power = powers[n & 31];
+    return r * __hiloint2double(__double2hiint(power) + ((n >> 5) + up) * (1 << 20), __double2loint(power));
 }
 
 struct Row {
     const float* at;  // this block's elements: shared memory, or the row itself
     int lo, n;        // the first one's index, their number
-    bool infinite;    // the greatest logit is infinite: those that equal it stand for 0, the others for minus infinity
+    bool odd;         // a NaN counts as minus infinity; where the greatest logit is infinite or near that, the others stand as their distance from it (at 0)
     float given_top;  // the greatest logit as it is,
     float top;        // and as it stands
     float high, bins_per;  // where the linear histogram begins, bins per unit of logit
     float least;      // what lies below has no mass: 2^-86 of the greatest weight
-    double rate;      // log2(e) / T
+    double rate;      // 32 log2(e) / T
+    const double* powers;
 
     __device__ __forceinline__ float number(float l) const {
-        l = fmaxf(l, -INFINITY);  // (of a NaN minus infinity)
-        return !infinite ? l : l == given_top ? 0.0f : -INFINITY;
+        if (!odd) return l;
+        l = fmaxf(l, -INFINITY);
+        return fabsf(given_top) < 1e37f ? l : l == given_top ? 0.0f : l - given_top;
     }
     __device__ __forceinline__ float logit(int i) const { return number(at[i]); }
-    __device__ __forceinline__ bool nothing(float l) const { return l < least || l == -INFINITY; }
-    __device__ __forceinline__ double exponent(float l) const { return ((double)fmaxf(l, fmaxf(least, -FLT_MAX)) - (double)top) * rate; }
-    // (adding 2^52 rounds to a whole number, which is then the lower bits)
+    // (adding 2^52 rounds to a whole number, which is then the lower bits; the least may be the greatest, where a temperature is nothing beside the logits)
     __device__ __forceinline__ u64 mass(float l) const {
-        const u64 m = (u64)__double_as_longlong(exp2_64(exponent(l), MASS_BITS) + 4503599627370496.0) & 0xfffffffffffffull;
-        return nothing(l) ? 0 : m;
+        const u64 m = (u64)__double_as_longlong(exp2_64(((double)fmaxf(l, least) - (double)top) * rate, MASS_BITS, powers) + 4503599627370496.0) & 0xfffffffffffffull;
+        return l < least ? 0 : m;
     }
     // The greatest logits in the highest bin; what lies below the histogram's range in bin 0.
-    __device__ __forceinline__ int bin(float l) const {
-        const float x = l >= high ? 0.0f : (high - l) * bins_per;
-        return BINS - 1 - (int)fminf(x, (float)(BINS - 1));
-    }
+    __device__ __forceinline__ float depth(float l) const { return l >= high ? 0.0f : (high - l) * bins_per; }
+    __device__ __forceinline__ int bin(float l) const { return BINS - 1 - (int)fminf(depth(l), (float)(BINS - 1)); }
+    // (the same comparisons without a bin's number)
+    __device__ __forceinline__ bool from_bin_on(float l, int b) const { return b == 0 || depth(l) < (float)(BINS - b); }
+    __device__ __forceinline__ bool in_bin(float l, int b) const { return from_bin_on(l, b) && (b == BINS - 1 || depth(l) >= (float)(BINS - 1 - b)); }
 };
+
+// f(logit, index) for all elements of the block.  (One by one: what a row goes through once is fetched once, and four elements at a time, four times the
+// instructions, took longer: 40 rows by mass 97 us for 85.)
+template <typename F>
+__device__ __forceinline__ void each(const Row& r, F f) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < r.n; i += THREADS) f(r.logit(i), r.lo + i);
+}
 
 // Sums over the block and over the row's blocks, for all threads; the one ends behind a barrier of the block, the others are of what the blocks have told (a
 // barrier of the cluster in between).
@@ -234,7 +251,7 @@ struct Subset {
     }
     __device__ __forceinline__ bool between(float l) const { return l <= high && (l > low || low == -INFINITY); }
     __device__ __forceinline__ bool holds(const Row& r, float l, int i) const {
-        if (!between(l) || (bin >= 0 && r.bin(l) != bin)) return false;
+        if (!between(l) || (bin >= 0 && !r.in_bin(l, bin))) return false;
         return digits == 0 || (key_of(l, i) >> shift(digits - 1)) == (prefix >> shift(digits - 1));
     }
 };
@@ -296,16 +313,15 @@ __device__ void histogram(Shared& s, const Row& r, const Subset& in) {
     clear(s);
     u32 low = 0;  // what falls into bin 0 of the linear histogram, mostly far below all others, is counted first
     u64 low_mass = 0;
-    for (int i = threadIdx.x; i < r.n; i += THREADS) {
-        const float l = r.logit(i);
-        if (!in.holds(r, l, r.lo + i)) continue;
-        const int b = in.bin < 0 ? r.bin(l) : Subset::value(key_of(l, r.lo + i), in.digits);
+    each(r, [&](float l, int i) {
+        if (!in.holds(r, l, i)) return;
+        const int b = in.bin < 0 ? r.bin(l) : Subset::value(key_of(l, i), in.digits);
         const u64 m = r.mass(l);
         if (in.bin < 0 && b == 0)
             ++low, low_mass += m;
         else
             put(s, b, m);
-    }
+    });
     put_low(s, low, low_mass);
     add_up<true>(s);
 }
@@ -367,12 +383,13 @@ template <typename Take>
 __device__ u32 gather(Shared& s, const Row& r, Take take) {
     if (threadIdx.x == 0) s.count_listed = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < r.n; i += THREADS) {
-        const float l = r.logit(i);
-        if (!take(l, r.lo + i)) continue;
+    each(r, [&](float l, int i) {
+        if (!take(l, i)) return;
         const u32 at = atomicAdd(&s.count_listed, 1u);
-        if (at < LIST) s.list[at].key = key_of(l, r.lo + i), s.list[at].mass = r.mass(l);
-    }
+        if (at < LIST) s.list[at].key = key_of(l, i);
+    });
+    __syncthreads();
+    if (threadIdx.x < s.count_listed && threadIdx.x < LIST) s.list[threadIdx.x].mass = r.mass(logit_of((u32)(s.list[threadIdx.x].key >> 32)));
     __syncthreads();
     if (threadIdx.x < 32) tell(s.listed, s.count_listed);
     cluster_sync();
@@ -467,7 +484,7 @@ __device__ Quantile quantile(Shared& s, const Row& r, Subset in, bool by_count, 
 template <typename Four, typename One>
 __device__ __forceinline__ void for_elements(int n, bool wide, Four four, One one) {
     const int whole = wide ? n & ~3 : 0;
-#pragma unroll 5
+#pragma unroll 2
     for (int i = 4 * threadIdx.x; i < whole; i += 4 * THREADS) four(i);
     for (int i = whole + threadIdx.x; i < n; i += THREADS) one(i);
 }
@@ -491,7 +508,9 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
     Row r;
     r.lo = min(a.vocab, (int)rank * a.per), r.n = min(a.vocab, r.lo + a.per) - r.lo;
     r.at = KEEP ? kept : logits + r.lo;
-    r.rate = LOG2E / (double)T;
+    r.rate = 32.0 * LOG2E / (double)T;
+    r.powers = s.powers;
+    const float rate = (float)(LOG2E / (double)T);
     const bool wide_in = (((uintptr_t)(logits + r.lo)) & 15) == 0, wide_out = (((uintptr_t)(out + r.lo)) & 15) == 0;
     const bool by_k = !greedy && k > 0 && k < a.vocab, by_p = !greedy && p < 1.0f;
     // the row's share on its way, all of it at once
@@ -506,14 +525,22 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
     }
     // the greatest logit: the thread's (of those that it has fetched itself), the block's, the row's
     float mine = -INFINITY;
+    bool nan = false;
     for_elements(
         r.n, wide_in,
         [&](int i) {
             const float4 v = *reinterpret_cast<const float4*>(r.at + i);
             mine = fmaxf(fmaxf(mine, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+            nan |= isnan(v.x) | isnan(v.y) | isnan(v.z) | isnan(v.w);
         },
-        [&](int i) { mine = fmaxf(mine, r.at[i]); });
+        [&](int i) {
+            mine = fmaxf(mine, r.at[i]);
+            nan |= isnan(r.at[i]);
+        });
+    nan = __any_sync(0xffffffffu, nan);
+    if ((threadIdx.x & 31) == 0) s.fred[3][threadIdx.x >> 5] = nan ? 1.0f : 0.0f;
     const float block_top = block_max(s, 0, mine);
+    nan = __any_sync(0xffffffffu, s.fred[3][threadIdx.x & (WARPS - 1)] != 0.0f);
     // (for top-k) the least finite maximum of a thread
     const int quads = wide_in ? r.n & ~3 : 0;
     const bool has = 4 * (int)threadIdx.x < quads || quads + (int)threadIdx.x < r.n;
@@ -521,8 +548,8 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
     if (threadIdx.x < 32) tell(s.value[0], block_top), tell(s.value[1], block_least);
     cluster_sync();
     r.given_top = warp_max(row_value(s.value[0], -INFINITY));
-    r.infinite = isinf(r.given_top);
-    r.top = r.high = r.infinite ? 0.0f : r.given_top;
+    r.odd = nan || !(fabsf(r.given_top) < 1e37f);
+    r.top = r.high = fabsf(r.given_top) < 1e37f ? r.given_top : 0.0f;
     r.least = r.top - 60.0f * T;
     out += r.lo;
     if (greedy) {
@@ -544,7 +571,6 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             r.n, wide_out, [&](int i) { *reinterpret_cast<float4*>(out + i) = make_float4(of(i), of(i + 1), of(i + 2), of(i + 3)); },
             [&](int i) { out[i] = of(i); });
     } else if (!by_k && !by_p) {
-        const float rate = (float)r.rate;
         // (the difference is rounded once, its product with log2(e) / T twice: an exponent is off by 2^-23 of itself, as if it were divided by T)
         auto weight = [&](float l) { return exp2_unit((r.number(l) - r.top) * rate); };
         float sum = 0.0f;
@@ -593,7 +619,7 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             const u64 threads = row_sum_u64(s.total_count);
             if (threads >= (u64)k) {
                 const Found f = find_bin(s, true, (u64)k);
-                const int n = (int)gather(s, r, [&](float l, int) { return r.bin(l) >= f.bin; });
+                const int n = (int)gather(s, r, [&](float l, int) { return r.from_bin_on(l, f.bin); });
                 if (n <= LIST) {
                     if (threadIdx.x == 0) s.threshold = ~0ull, s.retained = 0, s.kept_mass = 0;
                     __syncthreads();
@@ -617,10 +643,9 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
         if (!done && by_k) {
             // the whole row's histogram, from the greatest logit to the least finite one
             float low = INFINITY;
-            for (int i = threadIdx.x; i < r.n; i += THREADS) {
-                const float l = r.logit(i);
+            each(r, [&](float l, int) {
                 if (l > -INFINITY) low = fminf(low, l);
-            }
+            });
             low = -block_max(s, 2, -low);
             if (threadIdx.x < 32) tell(s.value[3], low);
             cluster_sync();
@@ -641,14 +666,13 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             float bound[BOUNDS], above[BOUNDS] = {}, all_mass = 0.0f;
 #pragma unroll
             for (int b = 0; b < BOUNDS; ++b) bound[b] = r.top - depth[b] * T;
-            const float rate = (float)r.rate;
-            for (int i = threadIdx.x; i < r.n; i += THREADS) {
-                const float l = r.logit(i), w = exp2_unit((l - r.top) * rate);
+            each(r, [&](float l, int) {
+                const float w = exp2_unit((l - r.top) * rate);
                 all_mass += w;
 #pragma unroll
                 for (int b = 0; b < BOUNDS; ++b)
                     if (l > bound[b]) above[b] += w;
-            }
+            });
 #pragma unroll
             for (int b = 0; b <= BOUNDS; ++b) {
                 const float t = warp_sum(b < BOUNDS ? above[b] : all_mass);
@@ -684,18 +708,17 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             clear(s);
             u64 over = 0, sum = 0, low_mass = 0;
             u32 low = 0;
-            for (int i = threadIdx.x; i < r.n; i += THREADS) {
-                const float l = r.logit(i);
+            each(r, [&](float l, int) {
                 const u64 m = r.mass(l);
                 sum += m;
                 if (l > in.high) over += m;
-                if (!in.between(l)) continue;
+                if (!in.between(l)) return;
                 const int b = r.bin(l);
                 if (b == 0)
                     ++low, low_mass += m;
                 else
                     put(s, b, m);
-            }
+            });
             put_low(s, low, low_mass);
             block_sum_u64(s, over, sum);
             if (threadIdx.x < 32) tell(s.over, over), tell(s.sum, sum);
@@ -706,7 +729,7 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             threshold = q.key, mass = over + q.mass;
         }
         // (which tokens stay is decided; their probabilities in 32 bits, as without top-k and top-p)
-        const float inv = (float)(UNIT / (double)mass), rate = (float)r.rate, border = logit_of((u32)(threshold >> 32));
+        const float inv = (float)(UNIT / (double)mass), border = logit_of((u32)(threshold >> 32));
         auto of = [&](float l, int i) -> float {
             l = r.number(l);
             const float w = exp2_unit((l - r.top) * rate) * inv;
@@ -728,6 +751,7 @@ template <bool KEEP>
 __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const SamplingProbs a) {
     __shared__ Shared s;
     extern __shared__ __align__(16) float kept[];
+    if (threadIdx.x < 32) s.powers[threadIdx.x] = powers_of_two[threadIdx.x];
     cluster_sync();  // (all blocks have begun: their memory may be written)
     pdl_wait();
     pdl_launch_dependents();

@@ -180,6 +180,9 @@ struct Row {
     // The greatest logits in the highest bin; what lies below the histogram's range in bin 0.
     __device__ __forceinline__ float depth(float l) const { return l >= high ? 0.0f : (high - l) * bins_per; }
     __device__ __forceinline__ int bin(float l) const { return BINS - 1 - (int)fminf(depth(l), (float)(BINS - 1)); }
+    // Logits between which all of a bin's lie, a bin more to each side: most elements are told apart by them alone.
+    __device__ __forceinline__ float below_bin(int b) const { return b == 0 ? -INFINITY : high - (float)(BINS + 1 - b) / bins_per; }
+    __device__ __forceinline__ float above_bin(int b) const { return b >= BINS - 2 ? INFINITY : high - (float)(BINS - 3 - b) / bins_per; }
     // (the same comparisons without a bin's number)
     __device__ __forceinline__ bool from_bin_on(float l, int b) const { return b == 0 || depth(l) < (float)(BINS - b); }
     __device__ __forceinline__ bool in_bin(float l, int b) const { return from_bin_on(l, b) && (b == BINS - 1 || depth(l) >= (float)(BINS - 1 - b)); }
@@ -378,13 +381,13 @@ __device__ Found find_bin(Shared& s, bool by_count, u64 aim) {
     return s.found;
 }
 
-// The elements for which take(l, i) holds into s.all of every block: how many of them there are in the row (if more than LIST, some are missing).
+// The elements for which take(l, i) holds, none of which lies outside low .. high, into s.all of every block: how many of them there are in the row (if more than LIST, some are missing).
 template <typename Take>
-__device__ u32 gather(Shared& s, const Row& r, Take take) {
+__device__ u32 gather(Shared& s, const Row& r, float low, float high, Take take) {
     if (threadIdx.x == 0) s.count_listed = 0;
     __syncthreads();
     each(r, [&](float l, int i) {
-        if (!take(l, i)) return;
+        if (!(l >= low && l <= high) || !take(l, i)) return;
         const u32 at = atomicAdd(&s.count_listed, 1u);
         if (at < LIST) s.list[at].key = key_of(l, i);
     });
@@ -463,7 +466,7 @@ __device__ Quantile quantile(Shared& s, const Row& r, Subset in, bool by_count, 
         before_mass += f.before_mass;
         aim -= min(aim, by_count ? f.before_count : f.before_mass);
     }
-    const int n = (int)gather(s, r, [&](float l, int i) { return in.holds(r, l, i); });
+    const int n = (int)gather(s, r, r.below_bin(in.bin), r.above_bin(in.bin), [&](float l, int i) { return in.holds(r, l, i); });
     if (threadIdx.x == 0) s.threshold = 0, s.retained = 0;
     __syncthreads();
     const Entry mine = s.all[threadIdx.x];
@@ -619,7 +622,7 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             const u64 threads = row_sum_u64(s.total_count);
             if (threads >= (u64)k) {
                 const Found f = find_bin(s, true, (u64)k);
-                const int n = (int)gather(s, r, [&](float l, int) { return r.from_bin_on(l, f.bin); });
+                const int n = (int)gather(s, r, r.below_bin(f.bin), INFINITY, [&](float l, int) { return r.from_bin_on(l, f.bin); });
                 if (n <= LIST) {
                     if (threadIdx.x == 0) s.threshold = ~0ull, s.retained = 0, s.kept_mass = 0;
                     __syncthreads();
@@ -732,8 +735,8 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
         const float inv = (float)(UNIT / (double)mass), border = logit_of((u32)(threshold >> 32));
         auto of = [&](float l, int i) -> float {
             l = r.number(l);
-            const float w = exp2_unit((l - r.top) * rate) * inv;
-            return l > border || (l == border && key_of(l, r.lo + i) >= threshold) ? w : 0.0f;
+            if (!(l >= border) || (l == border && key_of(l, r.lo + i) < threshold)) return 0.0f;
+            return exp2_unit((l - r.top) * rate) * inv;
         };
         for_elements(
             r.n, wide_out && KEEP,

@@ -35,12 +35,10 @@ struct VerifyTree {
     int* status;
 };
 
-__device__ __forceinline__ double ld_peer_shared_f64(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ void st_peer_shared_f64(uint32_t addr, uint32_t rank, double v) {
     uint32_t remote;
-    double v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote) : "memory");
-    return v;
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"(v) : "memory");
 }
 
 __device__ __forceinline__ double warp_sum64(double v) {
@@ -59,7 +57,7 @@ struct Shared {
     double refused[NODES];   // R of each refusal that left a residual
     int gone[NODES];         // tokens that were refused without probabilities
     double part[2][WARPS];   // sums of the warps' runs of the last pass, by the parity of its number
-    double block[2];         // the block's
+    double block[2][CLUSTER];  // those of the row's blocks
 };
 
 struct Pass {
@@ -77,51 +75,59 @@ __device__ __forceinline__ double residual(const Shared& s, int refusals, float 
     return r;
 }
 
-// f(element, what is left of it) for four neighbours from i on.
+// Four neighbours from i on, of both rows; nought behind the run's end.
 template <bool DRAFT>
-__device__ __forceinline__ void four(const Shared& s, const Pass& w, int i, int refusals, int gone, double (&r)[4]) {
-    float p[4] = {}, q[4] = {};
+__device__ __forceinline__ void fetch(const Pass& w, int i, float4& p, float4& q) {
+    p = q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (w.aligned && i + 4 <= w.hi) {
-        const float4 v = *reinterpret_cast<const float4*>(w.p + i);
-        p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
-        if (DRAFT) {
-            const float4 v2 = *reinterpret_cast<const float4*>(w.q + i);
-            q[0] = v2.x, q[1] = v2.y, q[2] = v2.z, q[3] = v2.w;
-        }
+        p = *reinterpret_cast<const float4*>(w.p + i);
+        if (DRAFT) q = *reinterpret_cast<const float4*>(w.q + i);
     } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i + k < w.hi) {
-                p[k] = w.p[i + k];
-                if (DRAFT) q[k] = w.q[i + k];
-            }
+        if (i < w.hi) p.x = w.p[i], q.x = DRAFT ? w.q[i] : 0.0f;
+        if (i + 1 < w.hi) p.y = w.p[i + 1], q.y = DRAFT ? w.q[i + 1] : 0.0f;
+        if (i + 2 < w.hi) p.z = w.p[i + 2], q.z = DRAFT ? w.q[i + 2] : 0.0f;
+        if (i + 3 < w.hi) p.w = w.p[i + 3], q.w = DRAFT ? w.q[i + 3] : 0.0f;
     }
+}
+
+// What is left of them.
+template <bool DRAFT>
+__device__ __forceinline__ void left_of(const Shared& s, int i, float4 p, float4 q, int refusals, int gone, double (&r)[4]) {
     if (!DRAFT)
         for (int g = 0; g < gone; ++g) {
             const unsigned at = (unsigned)(s.gone[g] - i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (at == (unsigned)k) p[k] = 0.0f;
+            if (at == 0) p.x = 0.0f;
+            if (at == 1) p.y = 0.0f;
+            if (at == 2) p.z = 0.0f;
+            if (at == 3) p.w = 0.0f;
         }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) r[k] = DRAFT ? residual(s, refusals, p[k], q[k]) : (double)probability(p[k]);
+    r[0] = DRAFT ? residual(s, refusals, p.x, q.x) : (double)probability(p.x);
+    r[1] = DRAFT ? residual(s, refusals, p.y, q.y) : (double)probability(p.y);
+    r[2] = DRAFT ? residual(s, refusals, p.z, q.z) : (double)probability(p.z);
+    r[3] = DRAFT ? residual(s, refusals, p.w, q.w) : (double)probability(p.w);
 }
 
+// The sum of what is left of a warp's run, five groups of 128 elements on their way at once (one at a time, a pass over 151,936 elements waited ten times for memory).
+template <bool DRAFT>
 __device__ __forceinline__ double run_sum(const Shared& s, const Pass& w, int refusals, int gone) {
+    constexpr int AHEAD = 5;
     double sum = 0.0, r[4];
-    for (int i = w.lo + 4 * (threadIdx.x & 31); i < w.hi; i += 128) {
-        if (refusals)
-            four<true>(s, w, i, refusals, gone, r);
-        else
-            four<false>(s, w, i, refusals, gone, r);
-        sum += (r[0] + r[1]) + (r[2] + r[3]);
+    for (int i0 = w.lo + 4 * (threadIdx.x & 31); i0 < w.hi; i0 += 128 * AHEAD) {
+        float4 p[AHEAD], q[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) fetch<DRAFT>(w, i0 + 128 * k, p[k], q[k]);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            left_of<DRAFT>(s, i0 + 128 * k, p[k], q[k], refusals, gone, r);
+            sum += (r[0] + r[1]) + (r[2] + r[3]);
+        }
     }
     return warp_sum64(sum);
 }
 
 __global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a) {
     __shared__ Shared s;
-    __shared__ double whole[CLUSTER];
+    cluster_arrive_relaxed();
     pdl_wait();
     pdl_launch_dependents();
     const int seq = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,28 +159,27 @@ __global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a
         s.parent[i] = (short)(i ? up : -1), s.token[i] = t, s.p[i] = p, s.q[i] = q, s.u[i] = a.uniforms[first + i];
     }
     __syncthreads();
+    cluster_wait();  // (all blocks have begun: their memory may be written)
     // this warp's run of elements: runs begin on four elements, and follow one another over the blocks of the cluster
     const int per = (((a.vocab + CLUSTER * WARPS - 1) / (CLUSTER * WARPS)) + 3) & ~3;
     Pass w;
     w.lo = min(a.vocab, (int)(rank * WARPS + warp) * per), w.hi = min(a.vocab, w.lo + per);
     int passes = 0;
-    // the sum over the row of what is left, the same in all blocks; the runs' sums stay in s.part, the blocks' in `whole`
+    // the sum over the row of what is left, the same in all blocks; the runs' sums stay in s.part, the blocks' in s.block
     auto sum_up = [&](int refusals, int gone) {
         const int b = passes++ & 1;
-        const double mine = run_sum(s, w, refusals, gone);
+        const double mine = refusals ? run_sum<true>(s, w, refusals, gone) : run_sum<false>(s, w, refusals, gone);
         if (lane == 0) s.part[b][warp] = mine;
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x < CLUSTER) {
+            // (every block's sum into every block's memory; nobody writes a half again before all have read it: there is a barrier of the cluster more between)
             double t = 0.0;
             for (int i = 0; i < WARPS; ++i) t += s.part[b][i];
-            s.block[b] = t;
+            st_peer_shared_f64(smem_u32(&s.block[b][rank]), threadIdx.x, t);
         }
-        cluster_sync();  // (nobody writes this half again before all have read it: there is a barrier more between)
-        if (threadIdx.x < CLUSTER) whole[threadIdx.x] = ld_peer_shared_f64(smem_u32(&s.block[b]), threadIdx.x);
-        __syncthreads();
+        cluster_sync();
         double t = 0.0;
-        for (int i = 0; i < CLUSTER; ++i) t += whole[i];
-        __syncthreads();
+        for (int i = 0; i < CLUSTER; ++i) t += s.block[b][i];
         return t;
     };
     int node = 0, path = 1, refusals = 0, gone = 0;
@@ -225,8 +230,8 @@ __global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a
         double before = 0.0, at = 0.0;
         int owner = -1;
         for (int i = 0; i < CLUSTER; ++i) {
-            if (whole[i] > 0.0 && at <= aim) owner = i, before = at;
-            at += whole[i];
+            if (s.block[b][i] > 0.0 && at <= aim) owner = i, before = at;
+            at += s.block[b][i];
         }
         if (owner == (int)rank && warp == 0) {
             at = before;
@@ -241,10 +246,14 @@ __global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a
                 const int i = i0 + 4 * lane;
                 double r[4] = {};
                 if (i < w.hi) {
-                    if (refusals)
-                        four<true>(s, w, i, refusals, gone, r);
-                    else
-                        four<false>(s, w, i, refusals, gone, r);
+                    float4 p, q;
+                    if (refusals) {
+                        fetch<true>(w, i, p, q);
+                        left_of<true>(s, i, p, q, refusals, gone, r);
+                    } else {
+                        fetch<false>(w, i, p, q);
+                        left_of<false>(s, i, p, q, refusals, gone, r);
+                    }
                 }
                 const double mine = (r[0] + r[1]) + (r[2] + r[3]);
                 double upto = mine;
@@ -276,7 +285,6 @@ __global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a
         if (threadIdx.x == 0) a.out_accepted[seq] = n ? path - 1 : 0;
         for (int i = (n ? path : 0) + threadIdx.x; i < a.width; i += THREADS) a.out_nodes[(size_t)seq * a.width + i] = -1;
     }
-    cluster_sync();  // nobody leaves while others may read its sums
 }
 
 }  // namespace

@@ -33,8 +33,7 @@ struct TreeAttention {
     float scale;  // of the scores, times log2(e)
     DivideBy page;  // the page size
     float* parts;
-    int splits;
-    int4* spans;  // of every request and kv head: first and last group, nodes, their first row in q and out
+    int2* spans;  // first and last group of every request (that has nodes) and kv head
     int* status;
 };
 
@@ -122,7 +121,7 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeAttention& p, const Tree
 }
 
 // ---------------------------------------------------------------------------------------------
-// The work of a bf16 step as units: a unit is UNIT cached rows of a request and kv head, an item all units of one.  Units are numbered through,
+// The work of a step as units: a unit is UNIT cached rows of a request and kv head, an item all units of one.  Units are numbered through,
 // requests first, then kv heads, then cached rows, and dealt out evenly, whatever the requests' lengths, to groups of `lanes` blocks: the blocks of a group take
 // the same cached rows at the same time, each its own block of query rows (a request with fewer query rows leaves some without work).
 // An item that lies in one group is written by it; of others every group leaves its part (at most two of a group), which tree_parts_kernel joins
@@ -134,12 +133,23 @@ struct TreePlan {
     bool tensor;      // on tcgen05 (tree_attention_tc.cu), otherwise on mma.sync (tree_attention_mma.cu)
     bool fits;        // units are counted in 32 bits
     long long floats(int seqs, int kv_heads, int head_dim) const {  // of scratch: parts, and behind them the items' groups
-        return 2ll * groups * lanes * rows * (head_dim + 2) + 4ll * seqs * kv_heads;
+        return 2ll * groups * lanes * rows * (head_dim + 2) + 2ll * seqs * kv_heads;
+    }
+    // As many groups as the SMs have room for (`blocks` of the kernel's blocks on each), and there can be units for.
+    void deal(int seqs, int kv_heads, int group, int max_nodes, int max_kv, int blocks) {
+        const int sms = ferris_sm_count();
+        const long long most = (long long)seqs * kv_heads * ((max_kv + unit - 1) / unit + 1);
+        lanes = (max_nodes * group + rows - 1) / rows;
+        const int want = (sms > 0 ? sms : 148) * blocks / lanes;
+        groups = (int)(want < 1 ? 1 : want < most ? want : most);
+        fits = most <= 0x7fffffff;
     }
 };
 TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window);
 int tree_attention_mma(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
 int tree_attention_tc(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
+TreePlan tree_plan_f32(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv);
+int tree_attention_f32(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
 
 __device__ __forceinline__ int tree_scan(int v) {
 #pragma unroll

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
         const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
         if (first == 0 && row0 == 0 && threadIdx.x == 0)
-            p.spans[item.seq * p.kv_heads + head] = make_int4(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1), r.nodes, r.first);
+            p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
         if (row0 >= count) continue;
         const int* table = p.tables + (size_t)item.seq * p.width;
         // ---- cached rows on their way
@@ -425,12 +425,7 @@ TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_node
     // (the row of a box that lies nowhere is a number too; a scale below nought would turn maxima into minima)
     plan.tensor = (head_dim == 64 || head_dim == 128) && max_nodes * group > 16 && page_size % 16 == 0 && cache_rows < 0x7fffffff && scale > 0.0f && scale < 1e30f;
     if (plan.tensor) plan.unit = 128, plan.rows = max_nodes * group > 128 ? 256 : 128, blocks = 1;
-    const int sms = ferris_sm_count();
-    const long long most = (long long)seqs * kv_heads * ((max_kv + plan.unit - 1) / plan.unit + 1);
-    plan.lanes = (max_nodes * group + plan.rows - 1) / plan.rows;
-    const int want = (sms > 0 ? sms : 148) * blocks / plan.lanes;
-    plan.groups = (int)(want < 1 ? 1 : want < most ? want : most);
-    plan.fits = most <= 0x7fffffff;
+    plan.deal(seqs, kv_heads, group, max_nodes, max_kv, blocks);
     return plan;
 }
 

@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (lane == 0) mbar_arrive(&q_ready);
             }
             if (item.first == 0 && row0 == 0 && threadIdx.x == 0)
-                p.spans[item.seq * p.kv_heads + head] = make_int4(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1), r.nodes, r.first);
+                p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
             const int sure_low = p.window > 0 ? max(0, r.start + r.nodes - p.window) : 0, sure_high = min(r.start, r.rows);
             if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<SOFTMAX_WARPS * 32>(p, r, tree, softmax_barrier);
             {

@@ -53,7 +53,7 @@ _SIGNATURES = {
     "ferris_packed_cache_evict": [_VP],
     "ferris_packed_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
     "ferris_packed_attention": [_VP],
-    "ferris_tree_attention_plan": [_I, _I, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _VP],
+    "ferris_tree_attention_scratch": [_I, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _I],
     "ferris_tree_attention": [_VP],
     "ferris_sampling_probs": [_VP, _LL, _VP, _LL, _I, _I, _VP, _VP, _VP, _VP],
     "ferris_verify_tree": [_VP],
@@ -2666,7 +2666,7 @@ def packed_cache_evict(pages: PackedPages, block_tables: torch.Tensor, seq_rows:
 TREE_NODES = 256  # most tokens of a request's tree
 
 # Arguments of a call laid out for the library in one go, as for the packed cache.
-_TREE_ATTENTION = struct.Struct("=10Q15if")
+_TREE_ATTENTION = struct.Struct("=10Q14if")
 _TREE_ROWS = struct.Struct("=6Q9i")
 _VERIFY_TREE = struct.Struct("=10Q2q4i")
 _tree_buffer = ctypes.create_string_buffer(max(_TREE_ATTENTION.size, _TREE_ROWS.size, _VERIFY_TREE.size))
@@ -2748,26 +2748,25 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     if workspace is None:
         raise KernelError(f"{what}: a workspace is needed")
     dt = _DT[dtype]
-    splits, scratch, launches = _tree_attention_plan(dt, D, S, hkv, num_heads // hkv, T, max_q_len, max_kv_len, page_size, pages * hkv * page_size, scale,
-                                                     min(window, 0x7fffffff), dev)
+    scratch = _tree_attention_scratch(dt, D, S, hkv, num_heads // hkv, max_q_len, max_kv_len, page_size, pages * hkv * page_size, scale, min(window, 0x7fffffff), dev)
     if T == 1:
         ldq, ldo = max(ldq, cols), max(ldo, cols)
     try:
         _TREE_ATTENTION.pack_into(
             _tree_buffer, 0, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_q_start.data_ptr(),
             seq_start_row.data_ptr(), parents.data_ptr(), workspace.address("tree_attention", scratch, torch.float32), _current_stream(), ldq, ldo, dt,
-            pages, hkv, page_size, D, width, S, T, num_heads, max_q_len, max_kv_len, min(window, 0x7fffffff), splits, scale)
+            pages, hkv, page_size, D, width, S, T, num_heads, max_q_len, max_kv_len, min(window, 0x7fffffff), scale)
     except (struct.error, OverflowError) as e:
         raise KernelError(f"{what}: a stride, size or scale beyond 32 bits ({e})") from None
-    _check(_packed_lib().ferris_tree_attention(_tree_buffer_at), what, launches)
+    _check(_packed_lib().ferris_tree_attention(_tree_buffer_at), what, 2)
 
 
 @functools.lru_cache(maxsize=4096)
-def _tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, page_size, cache_rows, scale, window, device: int) -> tuple:
-    """Parts of a request's rows, floats of scratch and launches of a step of these sizes on a GPU."""
-    needs = (_LL * 3)()
-    _lib().ferris_tree_attention_plan(dtype, head_dim, seqs, kv_heads, group, tokens, max_nodes, max_kv, page_size, cache_rows, scale, window, needs)
-    return tuple(needs)
+def _tree_attention_scratch(dtype, head_dim, seqs, kv_heads, group, max_nodes, max_kv, page_size, cache_rows, scale, window, device: int) -> int:
+    """Floats of scratch of a step of these sizes on a GPU."""
+    fn = _lib().ferris_tree_attention_scratch
+    fn.restype = _LL
+    return fn(dtype, head_dim, seqs, kv_heads, group, max_nodes, max_kv, page_size, cache_rows, scale, window)
 
 
 def sampling_probs(logits: torch.Tensor, out: torch.Tensor, temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,

@@ -132,6 +132,22 @@ def test_attention_over_geometries(ops, workspace, dtype, heads, kv_heads, D, pa
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("heads, kv_heads, D, page_size", GEOMETRIES)
+def test_requests_without_nodes_take_nothing_from_the_scratch(ops, dtype, heads, kv_heads, D, page_size):
+    """Whatever the scratch holds where a request without nodes would have its place: here, small numbers that could be blocks' and rows'."""
+    from ferrisinfer_b200.engine.workspace import Workspace
+
+    step = Step(dtype, heads, kv_heads, D, page_size, [0, 5, 0, 0, 17, 0], [7, 99, 3, 300, 200, 0])
+    for numbers in ([0, 3], [2, 9], [0, 1, 0, 0], [1, 0]):
+        workspace = Workspace(DEV)
+        workspace.get("tree_attention", (1 << 24,), torch.float32).view(torch.int32).copy_(ints(numbers).repeat((1 << 24) // len(numbers)))
+        out = torch.full((22, heads * D), 7.0, dtype=dtype, device=DEV)
+        ops.tree_attention(step.q, out, step.k, step.v, ints(step.tables), ints(step.q_start), ints(step.starts), ints(step.parents), *step.most, heads,
+                           D ** -0.5, workspace=workspace)
+        step.check(out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("kind", ["tree", "chain", "star", "roots"])
 @pytest.mark.parametrize("nodes, starts", [([1], [0]), ([1], [1]), ([2], [15]), ([8, 8, 8], [16, 17, 31]), ([33, 64], [128, 127]), ([256, 3], [5, 700]),
                                            ([65], [0]), ([31, 32], [32, 33])])

@@ -14,19 +14,19 @@ namespace {
 constexpr int JOIN_PARTS = 64;  // parts that are joined at once
 
 template <typename T>
-__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes, int row_blocks) {
+__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes, int slices) {
     __shared__ float top[8][32], tile[32][33], factor[JOIN_PARTS][32];
     pdl_wait();
     pdl_launch_dependents();
     const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.y / row_blocks, row0 = (blockIdx.y - head * row_blocks) * min(rows, 32), col = blockIdx.x * 32 + warp * 4, seq = blockIdx.z;
-    const int2 span = p.spans[seq * p.kv_heads + head];  // (of a request without nodes whatever was there)
+    const int head = blockIdx.y / slices, row0 = (blockIdx.y - head * slices) * min(rows, 32), block = row0 / rows, col = blockIdx.x * 32 + warp * 4, seq = blockIdx.z;
+    const int2 span = tree_span(p, seq, head, block);  // (of query rows that are not there whatever was there)
     const TreeRequest r = tree_request(p, seq);
     const int count = r.nodes * p.group, parts = span.y - span.x + 1;
     if (row0 >= count || parts <= 1) return;  // (one part: written by the block that has it)
-    const int block = row0 / rows, in = row0 - block * rows + lane;  // (blocks have 16 rows or a multiple of 32)
+    const int in = row0 - block * rows + lane, lane_block = lanes > 1 ? block : 0;  // (blocks have 16 rows or a multiple of 32)
     const bool live = row0 + lane < count && in < rows;
-    auto part = [&](int k) { return tree_part(p, (span.x + k) * lanes + block, k == 0, rows) + in; };
+    auto part = [&](int k) { return tree_part(p, (span.x + k) * lanes + lane_block, k == 0, rows) + in; };
     float m = -INFINITY, l = 0.0f, o[4] = {};  // l: of the warp's own parts
     for (int k0 = 0; k0 < parts; k0 += JOIN_PARTS) {
         const int n = min(parts - k0, JOIN_PARTS);
@@ -138,15 +138,16 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
                                   (long long)a->pages * a->kv_heads * a->page_size, a->scale, a->window);
     if (!plan.fits) FERRIS_REFUSE("%d requests of up to %d rows exceed one launch", a->seqs, p.limit);
     p.parts = (float*)const_cast<void*>(a->parts);
-    p.spans = (int2*)(p.parts + 2ll * plan.groups * plan.lanes * plan.rows * (p.head_dim + 2));
+    p.spans = (int2*)(p.parts + plan.part_floats(p.head_dim));
+    p.row_blocks = plan.row_blocks;
     const cudaStream_t stream = (cudaStream_t)a->stream;
     const int rc = a->dtype != FERRIS_BF16 ? tree_attention_f32(p, plan, stream) : plan.tensor ? tree_attention_tc(p, plan, stream) : tree_attention_mma(p, plan, stream);
     if (rc != FERRIS_OK) return rc;
     const int at_once = plan.rows < 32 ? plan.rows : 32;  // rows of a block of query rows that a block joins
-    const int row_blocks = (p.max_nodes * p.group + at_once - 1) / at_once;
-    const dim3 grid((p.head_dim + 31) / 32, row_blocks * p.kv_heads, p.seqs);
+    const int slices = (p.max_nodes * p.group + at_once - 1) / at_once;
+    const dim3 grid((p.head_dim + 31) / 32, slices * p.kv_heads, p.seqs);
     const auto kernel = a->dtype == FERRIS_BF16 ? tree_parts_kernel<bf16> : tree_parts_kernel<float>;
-    const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, stream, p, plan.rows, plan.lanes, row_blocks);
+    const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, stream, p, plan.rows, plan.lanes, slices);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;

@@ -33,7 +33,8 @@ struct TreeAttention {
     float scale;  // of the scores, times log2(e)
     DivideBy page;  // the page size
     float* parts;
-    int2* spans;  // first and last group of every request (that has nodes) and kv head
+    int2* spans;  // first and last group of every item: request (that has nodes), kv head, block of query rows
+    int row_blocks;
     int* status;
 };
 
@@ -121,27 +122,31 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeAttention& p, const Tree
 }
 
 // ---------------------------------------------------------------------------------------------
-// The work of a step as units: a unit is UNIT cached rows of a request and kv head, an item all units of one.  Units are numbered through,
-// requests first, then kv heads, then cached rows, and dealt out evenly, whatever the requests' lengths, to groups of `lanes` blocks: the blocks of a group take
-// the same cached rows at the same time, each its own block of query rows (a request with fewer query rows leaves some without work).
-// An item that lies in one group is written by it; of others every group leaves its part (at most two of a group), which tree_parts_kernel joins
-// in the order of the units, so that results do not depend on timing.
+// The work of a step.  An item is a block of query rows of a request and kv head, a tile UNIT cached rows of it; the tiles are numbered through and
+// dealt out evenly to the blocks of the grid, whatever the requests' lengths.  Two ways:
+// FLAT   requests first, then kv heads, blocks of query rows, cached rows: all blocks have the same number of tiles.
+// lanes  groups of `lanes` blocks, one for every block of query rows that the largest request has; requests, kv heads, cached rows are dealt out to the groups.
+//        The blocks of a group go over the same cached rows side by side, so that those are read from memory once, however long the cache.
+// An item that lies in one block is written by it; of others every block leaves its part (at most two of a block), which tree_parts_kernel joins
+// in the order of the tiles, so that results do not depend on timing.
 // ---------------------------------------------------------------------------------------------
 struct TreePlan {
-    int unit, rows;   // cached rows of a unit, query rows of a block
-    int groups, lanes;  // groups of blocks, blocks of a group
-    bool tensor;      // on tcgen05 (tree_attention_tc.cu), otherwise on mma.sync (tree_attention_mma.cu)
-    bool fits;        // units are counted in 32 bits
-    long long floats(int seqs, int kv_heads, int head_dim) const {  // of scratch: parts, and behind them the items' groups
-        return 2ll * groups * lanes * rows * (head_dim + 2) + 2ll * seqs * kv_heads;
+    int unit, rows;          // cached rows of a tile, query rows of a block
+    int groups, lanes;       // groups of blocks, blocks of a group
+    int row_blocks;          // of a request at most
+    bool tensor;             // on tcgen05 (tree_attention_tc.cu), otherwise on mma.sync (tree_attention_mma.cu)
+    bool fits;               // tiles are counted in 32 bits
+    long long part_floats(int head_dim) const { return 2ll * groups * lanes * rows * (head_dim + 2); }
+    long long floats(int seqs, int kv_heads, int head_dim) const {  // of scratch: parts, and behind them who has the items
+        return part_floats(head_dim) + 2ll * seqs * kv_heads * row_blocks;
     }
-    // As many groups as the SMs have room for (`blocks` of the kernel's blocks on each), and there can be units for.
-    void deal(int seqs, int kv_heads, int group, int max_nodes, int max_kv, int blocks) {
+    // As many blocks as the SMs have room for (`blocks` on each), and there can be tiles for.
+    void deal(int seqs, int kv_heads, int group, int max_nodes, int max_kv, int blocks, bool flat) {
         const int sms = ferris_sm_count();
-        const long long most = (long long)seqs * kv_heads * ((max_kv + unit - 1) / unit + 1);
-        lanes = (max_nodes * group + rows - 1) / rows;
-        const int want = (sms > 0 ? sms : 148) * blocks / lanes;
-        groups = (int)(want < 1 ? 1 : want < most ? want : most);
+        row_blocks = (max_nodes * group + rows - 1) / rows, lanes = flat ? 1 : row_blocks;
+        const long long most = (long long)seqs * kv_heads * (flat ? row_blocks : 1) * ((max_kv + unit - 1) / unit + 1);
+        const long long room = (long long)(sms > 0 ? sms : 148) * blocks / lanes;
+        groups = (int)(room < 1 ? 1 : room < most ? room : most);
         fits = most <= 0x7fffffff;
     }
 };
@@ -160,83 +165,90 @@ __device__ __forceinline__ int tree_scan(int v) {
     return v;
 }
 
-// First and last unit of an item: units of cached rows that none of the nodes sees are left out in front.
-template <int UNIT>
-__device__ __forceinline__ int tree_low(const TreeAttention& p, const TreeRequest& r) {
-    return p.window > 0 ? max(0, r.start - p.window + 1) / UNIT : 0;
-}
-template <int UNIT>
-__device__ __forceinline__ int tree_tiles(const TreeAttention& p, const TreeRequest& r) {
-    // (nodes that can see nothing: still a unit, which says so)
-    return r.nodes > 0 ? max((r.rows + UNIT - 1) / UNIT - tree_low<UNIT>(p, r), 1) : 0;
-}
-
 struct TreeItem {
     TreeRequest request;
-    int seq, head;
-    int first, last, tiles, low;  // its units that are this group's, of all its units; units in front of them
+    int seq, head, block;
+    int first, last, tiles, low;  // its tiles that are this group's, of all its tiles; tiles of the request in front of them, which none of its nodes sees
+    int start;                    // number of its first tile
 };
 
-// Goes through a group's units, item by item; by whole warps, each for itself.
-template <int UNIT>
+// Goes through a group's share, item by item; by whole warps, each for itself.
+template <int UNIT, int ROWS, bool FLAT>
 struct TreeWalk {
-    int total, groups, unit, end;  // units of the step; groups that have some; where this one is, where it ends
-    TreeRequest mine;              // of request 32 s0 + lane
-    int s0, before, upto;          // units before these requests, and up to and with this lane's
+    int at, end, lane_block;  // where this group is and where it ends; block of query rows of this lane
+    int per, more;            // tiles of a group, and groups that have one more
+    TreeRequest mine;         // of request 32 s0 + lane
+    int s0, before, upto;     // tiles before these requests, and up to and with this lane's
+
+    static __device__ __forceinline__ int low(const TreeAttention& p, const TreeRequest& r) { return p.window > 0 ? max(0, r.start - p.window + 1) / UNIT : 0; }
+    static __device__ __forceinline__ int tiles(const TreeAttention& p, const TreeRequest& r) {
+        return max((r.rows + UNIT - 1) / UNIT - low(p, r), 1);  // (nodes that can see nothing: still a tile, which says so)
+    }
+    static __device__ __forceinline__ int blocks(const TreeAttention& p, const TreeRequest& r) { return FLAT ? (r.nodes * p.group + ROWS - 1) / ROWS : 1; }
 
     __device__ __forceinline__ void look_at(const TreeAttention& p, int chunk) {
         s0 = chunk;
         const int seq = 32 * chunk + (threadIdx.x & 31);
         mine.nodes = 0;
         if (seq < p.seqs) mine = tree_request(p, seq);
-        upto = tree_scan(mine.nodes > 0 ? tree_tiles<UNIT>(p, mine) * p.kv_heads : 0);
+        upto = tree_scan(mine.nodes > 0 ? tiles(p, mine) * blocks(p, mine) * p.kv_heads : 0);
     }
-    // Group `group` of as many as the grid has.
-    __device__ __forceinline__ void begin(const TreeAttention& p, int group, int grid) {
-        total = 0;
-        const int chunks = (p.seqs + 31) / 32;
+    __device__ __forceinline__ void begin(const TreeAttention& p, int lanes) {
+        const int group = blockIdx.x / lanes, chunks = (p.seqs + 31) / 32;
+        lane_block = blockIdx.x - group * lanes;
+        int total = 0;
         for (int c = 0; c < chunks; ++c) {
             look_at(p, c);
             before = total;
             total += __shfl_sync(0xffffffffu, upto, 31);
         }
-        groups = min(total, grid);  // (each at least one unit, so that every group between the first and the last of an item leaves a part of it)
-        if (group >= groups) {
-            unit = end = 0;
-            return;
-        }
-        const int per = total / groups, more = total - per * groups;
-        unit = group * per + min(group, more), end = unit + per + (group < more);
+        const int groups = gridDim.x / lanes;  // (those that have no tiles leave no part either)
+        per = total / groups, more = total - per * groups;
+        at = group * per + min(group, more), end = at + per + (group < more);
         if (chunks > 1) look_at(p, 0), before = 0;
     }
-    __device__ __forceinline__ int owner(int u) const {
-        const int per = total / groups, more = total - per * groups, at = more * (per + 1);
-        return u < at ? u / (per + 1) : more + (u - at) / per;
+    // The group that has a tile.
+    __device__ __forceinline__ int owner(int tile) const {
+        const int longer = more * (per + 1);
+        return tile < longer ? tile / (per + 1) : more + (tile - longer) / per;
     }
-    __device__ __forceinline__ bool next(const TreeAttention& p, TreeItem& item, int& first_unit) {
-        if (unit >= end) return false;
-        unsigned here;
-        while (!(here = __ballot_sync(0xffffffffu, unit < before + upto))) {
-            before += __shfl_sync(0xffffffffu, upto, 31);
-            look_at(p, s0 + 1);
+    // First and last group of an item.
+    __device__ __forceinline__ int2 span(const TreeItem& i) const { return make_int2(owner(i.start), owner(i.start + i.tiles - 1)); }
+
+    __device__ __forceinline__ bool next(const TreeAttention& p, TreeItem& item) {
+        while (at < end) {
+            unsigned here;
+            while (!(here = __ballot_sync(0xffffffffu, at < before + upto))) {
+                before += __shfl_sync(0xffffffffu, upto, 31);
+                look_at(p, s0 + 1);
+            }
+            const int lane = __ffs(here) - 1;
+            item.seq = 32 * s0 + lane;
+            item.request.first = __shfl_sync(0xffffffffu, mine.first, lane);
+            item.request.nodes = __shfl_sync(0xffffffffu, mine.nodes, lane);
+            item.request.start = __shfl_sync(0xffffffffu, mine.start, lane);
+            item.request.rows = __shfl_sync(0xffffffffu, mine.rows, lane);
+            const TreeRequest& r = item.request;
+            item.low = low(p, r), item.tiles = tiles(p, r);
+            const int from = before + (lane ? __shfl_sync(0xffffffffu, upto, lane - 1) : 0);
+            const int n = (at - from) / item.tiles, blocks_each = blocks(p, r);
+            item.head = n / blocks_each;
+            item.block = FLAT ? n - item.head * blocks_each : lane_block;
+            item.start = from + n * item.tiles;
+            item.first = at - item.start, item.last = min(item.tiles, end - item.start);
+            at = item.start + item.last;
+            if (FLAT || item.block * ROWS < r.nodes * p.group) return true;
         }
-        const int at = __ffs(here) - 1;
-        item.seq = 32 * s0 + at;
-        item.request.first = __shfl_sync(0xffffffffu, mine.first, at);
-        item.request.nodes = __shfl_sync(0xffffffffu, mine.nodes, at);
-        item.request.start = __shfl_sync(0xffffffffu, mine.start, at);
-        item.request.rows = __shfl_sync(0xffffffffu, mine.rows, at);
-        item.low = tree_low<UNIT>(p, item.request), item.tiles = tree_tiles<UNIT>(p, item.request);
-        const int from = before + (at ? __shfl_sync(0xffffffffu, upto, at - 1) : 0);
-        item.head = (unit - from) / item.tiles;
-        first_unit = from + item.head * item.tiles;
-        item.first = unit - first_unit, item.last = min(item.tiles, end - first_unit);
-        unit = first_unit + item.last;
-        return true;
+        return false;
     }
 };
 
-// Where a block's part lies: of an item that begins in the group, or of one that began in front of it.  Column c of row r at [c][r]: D columns of the
+// Who has an item, said by the block that has its beginning.
+__device__ __forceinline__ int2& tree_span(const TreeAttention& p, int seq, int head, int block) {
+    return p.spans[(seq * p.kv_heads + head) * p.row_blocks + block];
+}
+
+// Where a block's part lies: of an item that begins in it, or of one that began in front of it.  Column c of row r at [c][r]: D columns of the
 // unnormalised output, the maximum (to the base of 2), the sum.
 __device__ __forceinline__ float* tree_part(const TreeAttention& p, int block, bool begins, int rows) {
     return p.parts + (size_t)(2 * block + begins) * rows * (p.head_dim + 2);

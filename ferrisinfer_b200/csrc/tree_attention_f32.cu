@@ -31,7 +31,7 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool l
 }
 
 template <int DP, int G>
-__global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const TreeAttention p, int lanes) {
+__global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const TreeAttention p) {
     using Z = Sizes<DP, G>;
     constexpr int LD = Z::LD, EACH = Z::EACH;
     extern __shared__ __align__(16) float smem[];
@@ -44,18 +44,15 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
     float* weights = qs + Z::QUERIES + warp * Z::KEYS * WARP_ROWS;  // [cached row][query row]
     pdl_wait();
     pdl_launch_dependents();
-    const int turn = blockIdx.x / lanes, row0 = (blockIdx.x - turn * lanes) * Z::ROWS;
-    TreeWalk<Z::TILE> walk;
-    walk.begin(p, turn, gridDim.x / lanes);
+    TreeWalk<Z::TILE, Z::ROWS, true> walk;
+    walk.begin(p, 1);
     TreeItem item;
-    for (int unit0; walk.next(p, item, unit0);) {
+    while (walk.next(p, item)) {
         const TreeRequest r = item.request;
-        const int head = item.head, count = r.nodes * p.group;
+        const int head = item.head, count = r.nodes * p.group, row0 = item.block * Z::ROWS;
         const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
-        if (first == 0 && row0 == 0 && threadIdx.x == 0)
-            p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
-        if (row0 >= count) continue;
+        if (first == 0 && threadIdx.x == 0) tree_span(p, item.seq, head, item.block) = walk.span(item);
         const int* table = p.tables + (size_t)item.seq * p.width;
         // ---- cached rows on their way: a warp takes every eighth of the tile
         auto request = [&](int i) {
@@ -264,7 +261,7 @@ int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
     const auto kernel = tree_attention_f32_kernel<DP, G>;
     const int rc = ferris_allow_dynamic_smem((const void*)kernel, Sizes<DP, G>::BYTES);
     if (rc != FERRIS_OK) return rc;
-    const cudaError_t e = ferris_launch(kernel, dim3(plan.groups * plan.lanes), dim3(THREADS), (size_t)Sizes<DP, G>::BYTES, stream, p, plan.lanes);
+    const cudaError_t e = ferris_launch(kernel, dim3(plan.groups), dim3(THREADS), (size_t)Sizes<DP, G>::BYTES, stream, p);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;
@@ -289,7 +286,7 @@ TreePlan tree_plan_f32(int head_dim, int seqs, int kv_heads, int group, int max_
         using Z = Sizes<dp.value, g.value>;
         plan.unit = Z::TILE, plan.rows = Z::ROWS;
     });
-    plan.deal(seqs, kv_heads, group, max_nodes, max_kv, 1);
+    plan.deal(seqs, kv_heads, group, max_nodes, max_kv, 1, true);
     return plan;
 }
 

@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t place(int row, int column) {
 }
 
 template <int DP, int MS, int WR, int NW, int ST>
-__global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tree_attention_mma_kernel(const TreeAttention p, int lanes) {
+__global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tree_attention_mma_kernel(const TreeAttention p) {
     using P = Plan<DP, MS, WR, NW, ST>;
     constexpr int KS = DP / 16, SUB = P::TILE < 32 ? P::TILE : 32, NT = SUB / 8, FETCH = P::FETCH;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -65,18 +65,15 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
     unsigned char* q_smem = smem + P::Q_AT;
     pdl_wait();
     pdl_launch_dependents();
-    const int turn = blockIdx.x / lanes, row0 = (blockIdx.x - turn * lanes) * P::ROWS;
-    TreeWalk<P::UNIT> walk;
-    walk.begin(p, turn, gridDim.x / lanes);
+    TreeWalk<P::UNIT, P::ROWS, true> walk;
+    walk.begin(p, 1);
     TreeItem item;
-    for (int unit0; walk.next(p, item, unit0);) {
+    while (walk.next(p, item)) {
         const TreeRequest r = item.request;
-        const int head = item.head, count = r.nodes * p.group;
+        const int head = item.head, count = r.nodes * p.group, row0 = item.block * P::ROWS;
         const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
-        if (first == 0 && row0 == 0 && threadIdx.x == 0)
-            p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
-        if (row0 >= count) continue;
+        if (first == 0 && threadIdx.x == 0) tree_span(p, item.seq, head, item.block) = walk.span(item);
         const int* table = p.tables + (size_t)item.seq * p.width;
         // ---- cached rows on their way
         auto request = [&](int i) {
@@ -379,7 +376,7 @@ int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
     const auto kernel = tree_attention_mma_kernel<DP, MS, WR, NW, ST>;
     const int rc = ferris_allow_dynamic_smem((const void*)kernel, P::SMEM);
     if (rc != FERRIS_OK) return rc;
-    const cudaError_t e = ferris_launch(kernel, dim3(plan.groups * plan.lanes), dim3(NW * 32), (size_t)P::SMEM, stream, p, plan.lanes);
+    const cudaError_t e = ferris_launch(kernel, dim3(plan.groups), dim3(NW * 32), (size_t)P::SMEM, stream, p);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;
@@ -425,7 +422,7 @@ TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_node
     // (the row of a box that lies nowhere is a number too; a scale below nought would turn maxima into minima)
     plan.tensor = (head_dim == 64 || head_dim == 128) && max_nodes * group > 16 && page_size % 16 == 0 && cache_rows < 0x7fffffff && scale > 0.0f && scale < 1e30f;
     if (plan.tensor) plan.unit = 128, plan.rows = max_nodes * group > 128 ? 256 : 128, blocks = 1;
-    plan.deal(seqs, kv_heads, group, max_nodes, max_kv, blocks);
+    plan.deal(seqs, kv_heads, group, max_nodes, max_kv, blocks, !plan.tensor);
     return plan;
 }
 

@@ -148,19 +148,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto wait = [&](uint64_t* bar, int parity, int where) {
         if (!dead) dead = !mbar_wait(bar, parity, p.status, where);
     };
-    const int turn = blockIdx.x / lanes, row0 = (blockIdx.x - turn * lanes) * ROWS * Z::TILES;
-    TreeWalk<UNIT> walk;
-    walk.begin(p, turn, gridDim.x / lanes);
+    TreeWalk<UNIT, ROWS * Z::TILES, false> walk;
+    walk.begin(p, lanes);
     TreeItem item;
-    int unit0;
     if (warp >= SOFTMAX_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
         if (warp == SOFTMAX_WARPS) {
             // ---- K and V on their way: eight lanes, a box of 16 rows each
             int place0 = 0;
-            while (walk.next(p, item, unit0)) {
+            while (walk.next(p, item)) {
                 const TreeRequest r = item.request;
-                if (row0 >= r.nodes * p.group) continue;
+                if (item.first == 0 && lane == 0) tree_span(p, item.seq, item.head, item.block) = walk.span(item);
                 const int* table = p.tables + (size_t)item.seq * p.width;
                 const int n = item.last - item.first;
                 // the page of a lane's box of unit i, on its way; its row of the cache; outside the cache where there is none: nought
@@ -206,10 +204,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
             const uint32_t base = uniform(tensor_base);
             int place0 = 0, segments = 0, done0 = 0, done1 = 0;  // done: units of each group
-            while (walk.next(p, item, unit0)) {
-                if (row0 >= item.request.nodes * p.group) continue;
+            while (walk.next(p, item)) {
                 const int n = uniform(item.last - item.first);
-                const bool two = WIDE && uniform(row0 + ROWS < item.request.nodes * p.group);  // (WIDE: the second group has rows)
+                const bool two = WIDE && uniform((item.block * Z::TILES + 1) * ROWS < item.request.nodes * p.group);  // (WIDE: the second group has rows)
                 wait(&q_ready, segments & 1, 141);
                 auto scores = [&](int i, int g) {
                     const int at = place0 + k_place<WIDE>(i), s = at % ST;
@@ -274,11 +271,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t my_scores = tensor_base + SCORES + 128 * g + lanes_at, my_out = tensor_base + OUTPUTS + D * g + lanes_at;
         const float scale = p.scale;
         int place0 = 0, done = 0, segments = 0;
-        while (walk.next(p, item, unit0)) {
+        while (walk.next(p, item)) {
             const TreeRequest r = item.request;
             const int head = item.head, count = r.nodes * p.group, n = item.last - item.first;
             const bool whole_item = item.first == 0 && item.last == item.tiles;
-            if (row0 >= count) continue;
+            const int row0 = item.block * ROWS * Z::TILES;
             const int at = row0 + (WIDE ? g * ROWS : 0) + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
             const bool live = at - lane < count;                                    // any of the warp's rows
             const int from = WIDE ? 0 : g, step = WIDE ? 1 : 2;                     // the group's units
@@ -314,8 +311,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_ready);
             }
-            if (item.first == 0 && row0 == 0 && threadIdx.x == 0)
-                p.spans[item.seq * p.kv_heads + head] = make_int2(turn, whole_item ? turn : walk.owner(unit0 + item.tiles - 1));
             const int sure_low = p.window > 0 ? max(0, r.start + r.nodes - p.window) : 0, sure_high = min(r.start, r.rows);
             if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<SOFTMAX_WARPS * 32>(p, r, tree, softmax_barrier);
             {

@@ -2,17 +2,16 @@
 // dealt out: tree_attention.cuh).
 //
 // A block of 128 query rows goes over blocks of 128 cached rows (units):
-//   S = Q K^T   operands in shared memory (Q written once, K by TMA), sums in tensor memory
+//   S = Q K^T   128 x 128 x D, operands in shared memory (Q written once, K by TMA), sums in tensor memory
 //   P = 2^(S scale - m), rounded to bf16 (eight bits, as the output has; sums take it unrounded), into tensor memory over the scores it came from
 //   O = O + P V   P from tensor memory, V as TMA wrote it, sums in tensor memory over all units
-// Two groups of four softmax warps, each with maxima, sums and outputs of its own, so that the tensor core works for one while
-// the other exponentiates; a thread has a row, so that nothing is exchanged.  Of up to 128 query rows each group takes half of a unit's cached rows, and they are
-// joined at the end; of more (WIDE) each has 128 rows of its own and a unit in two halves, and K and V are fetched once for both.  Either way a group goes over pieces of
-// 128 x 64 scores in two places by turns: the scores of the next piece are there before the weights of this one are.
+// Two groups of four softmax warps, each with scores, maxima, sums and outputs of its own, so that the tensor core works for one while
+// the other exponentiates: of up to 128 query rows they take the units in turn and are joined at the end, of more (WIDE) each has 128 rows of its own, and K and V are
+// fetched once for both; a thread has a row, so that nothing is exchanged.
 // m is the greatest score so far only up to 2^8: outputs are brought to a new m (read, multiplied, written back) where a score exceeds it by
 // more than eight, which after the first units is rare; what is divided by in the end has the same m, so that nothing but the range of the weights changes.
-// A TMA warp streams K and V through a ring of stages, ahead of the segment that is worked on; an MMA warp issues
-// P V of a piece and then the scores that take its place (the tensor core keeps the order, so that these do not overwrite weights that are still read).
+// A TMA warp streams K and V through a ring of stages, ahead of the segment that is worked on; an MMA warp issues, in the order of the units,
+// P V of a unit and then the scores of the group's next one (the tensor core keeps the order, so that these do not overwrite weights that are still read).
 //
 // Units that every node sees whole are worked off as they are.  In others scores that are not seen become nought weights; as nought times NaN is NaN, the softmax
 // warps then look through the unit's values, set what is not finite to nought and add it, element by element, to the outputs of those who see it.
@@ -20,14 +19,14 @@
 
 namespace {
 
-constexpr int ROWS = 128, UNIT = 128, PIECE = 64, PAGE_ROWS = 16;  // (a TMA box: 16 rows of 64 columns)
+constexpr int ROWS = 128, UNIT = 128, PAGE_ROWS = 16;  // (a TMA box: 16 rows of 64 columns)
 constexpr int SOFTMAX_WARPS = 8, THREADS = (SOFTMAX_WARPS + 4) * 32;  // + a TMA warp, an MMA warp and two without work: whole warpgroups share out registers
 // Registers of a thread: the block is launched with LAUNCH_REGISTERS for each (what 384 threads of an SM can have), of which the third warpgroup gives some to
 // the softmax's two; what these take must not be more than that, or they would wait for ever.
 constexpr int LAUNCH_REGISTERS = 168, SOFTMAX_REGISTERS = 208, OTHER_REGISTERS = 80;
 static_assert(2 * SOFTMAX_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "registers");
 constexpr int BOX = PAGE_ROWS * 128, ATOM = UNIT * 128;  // bytes of a box; of 64 columns of a unit
-constexpr int SCORES = 0, OUTPUTS = 256, COLUMNS = 512;  // of tensor memory: scores of two pieces of two groups, their outputs (D each)
+constexpr int SCORES = 0, OUTPUTS = 256, COLUMNS = 512;  // of tensor memory: two groups' scores (128 each), their outputs (D each)
 
 template <int D, bool WIDE>
 struct Sizes {
@@ -78,10 +77,10 @@ __device__ __forceinline__ void tmem_store_32x16(uint32_t taddr, const uint32_t*
                  "r"(r[14]), "r"(r[15])
                  : "memory");
 }
-// A piece's columns of a lane.
-__device__ __forceinline__ void tmem_load_row(uint32_t taddr, uint32_t (&r)[PIECE]) {
+// 128 columns of a lane.
+__device__ __forceinline__ void tmem_load_row(uint32_t taddr, uint32_t (&r)[128]) {
 #pragma unroll
-    for (int c = 0; c < PIECE / 32; ++c) tmem_load_32x32(taddr + 32 * c, reinterpret_cast<uint32_t(&)[32]>(r[32 * c]));
+    for (int c = 0; c < 4; ++c) tmem_load_32x32(taddr + 32 * c, reinterpret_cast<uint32_t(&)[32]>(r[32 * c]));
 }
 // Two fp32 at once.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) { return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo); }
@@ -109,10 +108,7 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[W]) {
 __device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void group_barrier(int g) { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); }
 
-// Where in tensor memory a group's piece is.
-template <bool WIDE>
-__device__ __forceinline__ int piece_at(int g, int place) { return SCORES + (WIDE ? 128 * g + PIECE * place : PIECE * g + 128 * place); }
-// Stages in the order of their use by the tensor core: K 0, K 1, V 0, K 2, V 1, K 3, ..; WIDE, with both places for one unit, K 0, V 0, K 1, ..
+// Stages in the order of their use by the tensor core: K 0, K 1, V 0, K 2, V 1, K 3, ..; where both groups use them, K 0, V 0, K 1, ..
 template <bool WIDE>
 __device__ __forceinline__ int k_place(int i) { return WIDE ? 2 * i : i < 2 ? i : 2 * i - 1; }
 template <bool WIDE>
@@ -125,10 +121,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int ST = Z::STAGES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ TreeLines tree;
-    __shared__ uint64_t full[ST], empty[ST], q_ready, s_ready[2][2], p_ready[2][2], o_done[2][2];  // (group and place; without WIDE the scores of both groups come at once)
+    __shared__ uint64_t full[ST], empty[ST], q_ready, s_ready[2], p_ready[2], o_done[2];
     __shared__ uint32_t tensor_base;
     __shared__ float row_m[2][ROWS], row_l[2][ROWS];  // (not WIDE)
-    __shared__ int odd[2];  // threads that have found values of a unit that are not finite; by turns
+    __shared__ int odd[2];  // how many elements of a unit's values are not finite
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* q_smem = smem;                // [64 columns][128 rows][64] bf16, 128-byte swizzle; at a segment's end, half of a group's outputs
     uint8_t* kv_smem = smem + Z::TILES * Z::BLOCK;  // stages of [64 columns][128 cached rows][64]
@@ -138,9 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tma_prefetch_descriptor(&map_v);
         for (int s = 0; s < ST; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
         mbar_init(&q_ready, SOFTMAX_WARPS);
-        for (int g = 0; g < 2; ++g) {
-            for (int k = 0; k < 2; ++k) mbar_init(&s_ready[g][k], 1), mbar_init(&p_ready[g][k], 4), mbar_init(&o_done[g][k], 1);
-        }
+        for (int g = 0; g < 2; ++g) mbar_init(&s_ready[g], 1), mbar_init(&p_ready[g], 4), mbar_init(&o_done[g], 1);
         mbar_fence_init();
     }
     if (warp == SOFTMAX_WARPS + 1) tensor_memory_take(&tensor_base, COLUMNS);
@@ -207,66 +201,63 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int at = max(0, place0 - ST); at < place0; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);
         } else if (warp == SOFTMAX_WARPS + 1) {
             // ---- products
-            const uint32_t idesc_qk = umma_idesc_bf16(ROWS, WIDE ? PIECE : UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
+            const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
             const uint32_t base = uniform(tensor_base);
-            int place0 = 0, segments = 0, done0 = 0, done1 = 0;  // done: pieces of each group
+            int place0 = 0, segments = 0, done0 = 0, done1 = 0;  // done: units of each group
             while (walk.next(p, item)) {
                 const int n = uniform(item.last - item.first);
-                const bool two = !WIDE || uniform((item.block * Z::TILES + 1) * ROWS < item.request.nodes * p.group);  // (the second group has rows)
+                const bool two = WIDE && uniform((item.block * Z::TILES + 1) * ROWS < item.request.nodes * p.group);  // (WIDE: the second group has rows)
                 wait(&q_ready, segments & 1, 141);
-                // WIDE: of half h of unit i for group g; otherwise of unit i for both groups
-                auto scores = [&](int i, int h, int g) {
-                    const int at = place0 + k_place<WIDE>(i), s = at % ST, place = WIDE ? h : (done0 + i) & 1;
-                    if (h == 0 && g == 0) wait(&full[s], (at / ST) & 1, 142);
+                auto scores = [&](int i, int g) {
+                    const int at = place0 + k_place<WIDE>(i), s = at % ST;
+                    if (!WIDE || g == 0) wait(&full[s], (at / ST) & 1, 142);
                     tcgen05_fence_after();
                     if (elected()) {
                         const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem + (WIDE ? g * Z::BLOCK : 0)));
-                        const uint64_t k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + s * Z::BLOCK + h * PIECE * 128));
+                        const uint64_t k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + s * Z::BLOCK));
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k) {
                             const uint64_t next = (k >> 2) * (ATOM >> 4) + 2 * (k & 3);  // the next 64 columns, 32 bytes along the row
-                            tcgen05_mma_bf16(base + piece_at<WIDE>(g, place), q_desc + next, k_desc + next, idesc_qk, k > 0 ? 1u : 0u);
+                            tcgen05_mma_bf16(base + SCORES + 128 * g, q_desc + next, k_desc + next, idesc_qk, k > 0 ? 1u : 0u);
                         }
-                        tcgen05_commit(&s_ready[g][place]);
-                        if (!WIDE || (h == 1 && g == two)) tcgen05_commit(&empty[s]);
+                        tcgen05_commit(&s_ready[g]);
+                        if (!two || g) tcgen05_commit(&empty[s]);
                     }
                     __syncwarp();
                 };
-                // of half h of unit i for group g
-                auto outputs = [&](int i, int h, int g) {
-                    const int at = place0 + v_place<WIDE>(i, n), s = at % ST, piece = (g ? done1 : done0) + (WIDE ? 2 * i + h : i), place = piece & 1;
-                    if (g == 0 && (!WIDE || h == 0)) wait(&full[s], (at / ST) & 1, 143);
-                    wait(&p_ready[g][place], (piece >> 1) & 1, 144);
+                auto outputs = [&](int i, int g, bool last) {
+                    const int at = place0 + v_place<WIDE>(i, n), s = at % ST;
+                    if (!WIDE || g == 0) wait(&full[s], (at / ST) & 1, 143);
+                    wait(&p_ready[g], (g ? done1 : done0) & 1, 144);
+                    if (g)
+                        ++done1;
+                    else
+                        ++done0;
                     tcgen05_fence_after();
                     if (elected()) {
-                        const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + s * Z::BLOCK + h * PIECE * 128), ATOM);
+                        const uint64_t v_desc = umma_desc_mn_major_sw128(smem_u32(kv_smem + s * Z::BLOCK), ATOM);
 #pragma unroll
-                        for (int k = 0; k < PIECE / 16; ++k)
-                            tcgen05_mma_bf16_ts(base + OUTPUTS + D * g, base + piece_at<WIDE>(g, place) + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
-                        tcgen05_commit(&o_done[g][place]);
-                        if (h == 1 && g == two) tcgen05_commit(&empty[s]);
+                        for (int k = 0; k < UNIT / 16; ++k)
+                            tcgen05_mma_bf16_ts(base + OUTPUTS + D * g, base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
+                        if (!two || g) tcgen05_commit(&empty[s]);
+                        if (last) tcgen05_commit(&o_done[g]);
                     }
                     __syncwarp();
                 };
                 if constexpr (WIDE) {
-                    for (int h = 0; h < 2; ++h)
-                        for (int g = 0; g <= two; ++g) scores(0, h, g);
+                    scores(0, 0);
+                    if (two) scores(0, 1);
                     for (int i = 0; i < n; ++i)
-                        for (int h = 0; h < 2; ++h)
-                            for (int g = 0; g <= two; ++g) {
-                                outputs(i, h, g);
-                                if (i + 1 < n) scores(i + 1, h, g);
-                            }
-                    done0 += 2 * n, done1 += two ? 2 * n : 0;
+                        for (int g = 0; g <= two; ++g) {
+                            outputs(i, g, i + 1 == n);
+                            if (i + 1 < n) scores(i + 1, g);
+                        }
                 } else {
-                    scores(0, 0, 0);
-                    if (n > 1) scores(1, 0, 0);
+                    for (int i = 0; i < 2 && i < n; ++i) scores(i, i);
                     for (int i = 0; i < n; ++i) {
-                        outputs(i, 0, 0);
-                        outputs(i, 1, 1);
-                        if (i + 2 < n) scores(i + 2, 0, 0);
+                        outputs(i, i & 1, i + 2 >= n);
+                        if (i + 2 < n) scores(i + 2, i & 1);
                     }
-                    done0 += n, done1 += n;
                 }
                 __syncwarp();
                 place0 += 2 * n, ++segments;
@@ -277,14 +268,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         // ---- softmax: group g = warp / 4, a row a thread
         const int g = warp >> 2, t = threadIdx.x & 127;
         const uint32_t lanes_at = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t my_out = tensor_base + OUTPUTS + D * g + lanes_at;
+        const uint32_t my_scores = tensor_base + SCORES + 128 * g + lanes_at, my_out = tensor_base + OUTPUTS + D * g + lanes_at;
         const float scale = p.scale;
-        int place0 = 0, done = 0;  // done: pieces of the group
-        // Until a piece is in the outputs.  (A wait tells a phase from the one before it only.  When the scores of a piece are there, all outputs but those of the piece
-        // before it are done: the last two pieces have a barrier each, and at a segment's end both are waited for.)
-        auto outputs_of = [&](int piece) {
-            if (piece >= 0) wait(&o_done[g][piece & 1], (piece >> 1) & 1, 147);
-        };
+        int place0 = 0, done = 0, segments = 0;
         while (walk.next(p, item)) {
             const TreeRequest r = item.request;
             const int head = item.head, count = r.nodes * p.group, n = item.last - item.first;
@@ -292,6 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int row0 = item.block * ROWS * Z::TILES;
             const int at = row0 + (WIDE ? g * ROWS : 0) + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
             const bool live = at - lane < count;                                    // any of the warp's rows
+            const int from = WIDE ? 0 : g, step = WIDE ? 1 : 2;                     // the group's units
             const bool both = !WIDE || row0 + ROWS < count, here = both || g == 0;  // both groups have rows; this one has
             const int units = here ? n : 0;
             const int* table = p.tables + (size_t)item.seq * p.width;
@@ -335,28 +322,85 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tmem_store_wait();
             }
             float m = -INFINITY, l = 0.0f;
-            int looked = 0;
             // the page of a lane's box of a unit's eight, on its way while the unit before is worked on; -1: none
             auto page_of = [&](int i) {
                 const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS, block = (int)p.page.quotient((uint32_t)row);
                 return i < units && lane < UNIT / PAGE_ROWS && row < r.rows && block < p.width ? table[block] : -1;
             };
-            int page = page_of(0);
-            for (int i = 0; i < units; ++i) {
+            int page = page_of(from);
+            for (int i = from; i < units; i += step) {
                 const uint32_t boxes = __ballot_sync(0xffffffffu, page >= 0 && page < p.pages);  // (the TMA warp reports pages that are not there)
-                page = page_of(i + 1);
+                page = page_of(i + step);
                 const int key0 = (item.low + item.first + i) * UNIT;
                 const bool whole = key0 >= sure_low && key0 + UNIT <= sure_high && boxes == 0xffu;
+                wait(&s_ready[g], done & 1, 145);
+                ++done;
+                tcgen05_fence_after();
+                if (live) {  // (rows that are not there have nobody's weights)
+                    uint32_t s[UNIT];
+                    tmem_load_row(my_scores, s);
+                    tmem_load_wait();
+                    if (!whole) {
+#pragma unroll
+                        for (int c = 0; c < UNIT / 32; ++c) {
+                            uint32_t sees = node >= 0 ? tree_sees(p, r, tree, node, key0 + 32 * c) : 0u;
+                            if (!(boxes >> (2 * c) & 1)) sees &= 0xffff0000u;
+                            if (!(boxes >> (2 * c + 1) & 1)) sees &= 0xffffu;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!(sees >> j & 1)) s[32 * c + j] = 0xff800000u;
+                        }
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < UNIT; j += 2) top[j >> 1 & 3] = fmaxf(fmaxf(top[j >> 1 & 3], __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;  // (the scale is above nought)
+                    const bool up = most > m + 8.0f || (m == -INFINITY && most > m);
+                    if (__any_sync(0xffffffffu, up)) {
+                        const float now = up ? most : m, corr = now == -INFINITY ? 1.0f : exp2_unit(m - now);
+                        l *= corr, m = now;
+                        if (i > from) {
+#pragma unroll 1
+                            for (int c = 0; c < D / 16; ++c) {
+                                uint32_t o[16];
+                                tmem_load_32x16(my_out + 16 * c, o);
+                                tmem_load_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                                tmem_store_32x16(my_out + 16 * c, o);
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+                    uint64_t sum[2] = {0, 0};
+#pragma unroll
+                    for (int c = 0; c < UNIT / 32; ++c) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const uint64_t x = fma_pair((uint64_t)s[32 * c + 2 * j + 1] << 32 | s[32 * c + 2 * j], scale2, base2);
+                            const float a = exp2_unit(__uint_as_float((uint32_t)x)), b = exp2_unit(__uint_as_float((uint32_t)(x >> 32)));
+                            sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
+                            s[16 * c + j] = pack_bf16(a, b);
+                        }
+                        tmem_store_32x16(my_scores + 16 * c, s + 16 * c);
+                    }
+                    {
+                        const uint64_t both = add_pair(sum[0], sum[1]);
+                        l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
+                    }
+                    tmem_store_wait();
+                }
                 if (!whole) {
                     // the unit's values: what is not finite becomes nought, and goes to those who see it by itself
                     const int place = place0 + v_place<WIDE>(i, n), stage = place % ST;
                     wait(&full[stage], (place / ST) & 1, 146);
                     uint8_t* v = kv_smem + (size_t)stage * Z::BLOCK;
                     // (units that both groups work on are looked through and changed by the first, with the second beside it)
-                    const bool mine = !both || g == 0;
-                    int& found = odd[looked++ & 1];  // (the next unit's while this one's is still read)
+                    const bool shared = WIDE && both, mine = !shared || g == 0;
+                    int& found = odd[shared ? 0 : g];
                     auto barrier = [&] {
-                        if (both)
+                        if (shared)
                             softmax_barrier();
                         else
                             group_barrier(g);
@@ -376,9 +420,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     barrier();
                     if (found) {
                         // every thread for its query row: what it sees that is not finite (its weight is above nought, whatever it is)
-                        if (done > 0) outputs_of(done - 1);
-                        tcgen05_fence_after();
-                        for (int j = WIDE ? 0 : g * PIECE; j < (WIDE ? UNIT : (g + 1) * PIECE); ++j) {
+                        for (int j = 0; j < UNIT; ++j) {
                             const bool sees = node >= 0 && (boxes >> (j >> 4) & 1) && (tree_sees(p, r, tree, node, key0 + (j & ~31)) >> (j & 31) & 1);
                             for (int c = 0; c < D; ++c) {
                                 const bf16 x = *reinterpret_cast<const bf16*>(v + (c >> 6) * ATOM + swizzle128(j, (c >> 3) & 7) + 2 * (c & 7));
@@ -398,80 +440,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                             if (!isfinite(__bfloat162float(*x))) *x = __float2bfloat16_rn(0.0f);
                         }
                         fence_proxy_async();
-                        if (both) barrier();
+                        if (shared) barrier();
                     }
                 }
-                // the group's pieces
-#pragma unroll 1
-                for (int h = 0; h < (WIDE ? 2 : 1); ++h, ++done) {
-                    const int place = done & 1, half = (WIDE ? h : g) * PIECE;
-                    const uint32_t my_scores = tensor_base + lanes_at + piece_at<WIDE>(g, place);
-                    wait(&s_ready[WIDE ? g : 0][place], (done >> 1) & 1, 145);
-                    tcgen05_fence_after();
-                    if (live) {  // (rows that are not there have nobody's weights)
-                        uint32_t s[PIECE];
-                        tmem_load_row(my_scores, s);
-                        tmem_load_wait();
-                        if (!whole) {
-    #pragma unroll
-                            for (int c = 0; c < PIECE / 32; ++c) {
-                                uint32_t sees = node >= 0 ? tree_sees(p, r, tree, node, key0 + half + 32 * c) : 0u;
-                                if (!(boxes >> (half / 16 + 2 * c) & 1)) sees &= 0xffff0000u;
-                                if (!(boxes >> (half / 16 + 2 * c + 1) & 1)) sees &= 0xffffu;
-    #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (!(sees >> j & 1)) s[32 * c + j] = 0xff800000u;
-                            }
-                        }
-                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    #pragma unroll
-                        for (int j = 0; j < PIECE; j += 2) top[j >> 1 & 3] = fmaxf(fmaxf(top[j >> 1 & 3], __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
-                        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;  // (the scale is above nought)
-                        const bool up = most > m + 8.0f || (m == -INFINITY && most > m);
-                        if (__any_sync(0xffffffffu, up)) {
-                            const float now = up ? most : m, corr = now == -INFINITY ? 1.0f : exp2_unit(m - now);
-                            l *= corr, m = now;
-                            if (i > 0 || h > 0) {
-                                outputs_of(done - 1);
-                                tcgen05_fence_after();
-    #pragma unroll 1
-                                for (int c = 0; c < D / 16; ++c) {
-                                    uint32_t o[16];
-                                    tmem_load_32x16(my_out + 16 * c, o);
-                                    tmem_load_wait();
-    #pragma unroll
-                                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                                    tmem_store_32x16(my_out + 16 * c, o);
-                                }
-                            }
-                        }
-                        const float base = m == -INFINITY ? 0.0f : m;
-                        const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
-                        uint64_t sum[2] = {0, 0};
-    #pragma unroll
-                        for (int c = 0; c < PIECE / 32; ++c) {
-    #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const uint64_t x = fma_pair((uint64_t)s[32 * c + 2 * j + 1] << 32 | s[32 * c + 2 * j], scale2, base2);
-                                const float a = exp2_unit(__uint_as_float((uint32_t)x)), b = exp2_unit(__uint_as_float((uint32_t)(x >> 32)));
-                                sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
-                                s[16 * c + j] = pack_bf16(a, b);
-                            }
-                            tmem_store_32x16(my_scores + 16 * c, s + 16 * c);
-                        }
-                        {
-                            const uint64_t both = add_pair(sum[0], sum[1]);
-                            l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
-                        }
-                        tmem_store_wait();
-                    }
-                    tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_ready[g][place]);
-                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[g]);
             }
-            if (units > 0) outputs_of(done - 2);
-            if (units > 0) outputs_of(done - 1);
+            if (units > from) wait(&o_done[g], segments & 1, 147);
             tcgen05_fence_after();
             float* part = tree_part(p, blockIdx.x, item.first == 0, ROWS * Z::TILES) + (WIDE ? g * ROWS : 0) + t;
             bf16* out = (bf16*)p.out + (size_t)(r.first + max(node, 0)) * p.ldo + q_head * D;
@@ -547,6 +523,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (g == 0) leave_sums(most, total);
             }
             place0 += 2 * n;
+            // (a phase of o_done passes in every segment in which the group has units, q_ready's in every segment)
+            if (units > from) ++segments;
         }
     }
     tcgen05_fence_before();

@@ -19,14 +19,16 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
     pdl_wait();
     pdl_launch_dependents();
     const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.y / slices, row0 = (blockIdx.y - head * slices) * min(rows, 32), block = row0 / rows, col = blockIdx.x * 32 + warp * 4, seq = blockIdx.z;
-    const int2 span = tree_span(p, seq, head, block);  // (of query rows that are not there whatever was there)
+    // group z's item, if it goes on in others; with lanes, the blocks of query rows one after the other
+    const int4 begun = p.begun[blockIdx.z];
+    if (begun.x < 0) return;  // (items that lie in one group are written by it)
+    const int seq = begun.x, head = begun.y, lane_block = blockIdx.y / slices, block = lanes > 1 ? lane_block : begun.z, parts = begun.w - blockIdx.z + 1;
+    const int from_row = (blockIdx.y - lane_block * slices) * 32, row0 = block * rows + from_row, col = blockIdx.x * 32 + warp * 4;
     const TreeRequest r = tree_request(p, seq);
-    const int count = r.nodes * p.group, parts = span.y - span.x + 1;
-    if (row0 >= count || parts <= 1) return;  // (one part: written by the block that has it)
-    const int in = row0 - block * rows + lane, lane_block = lanes > 1 ? block : 0;  // (blocks have 16 rows or a multiple of 32)
+    const int count = r.nodes * p.group, in = from_row + lane;
+    if (row0 >= count) return;
     const bool live = row0 + lane < count && in < rows;
-    auto part = [&](int k) { return tree_part(p, (span.x + k) * lanes + lane_block, k == 0, rows) + in; };
+    auto part = [&](int k) { return tree_part(p, (blockIdx.z + k) * lanes + lane_block, k == 0, rows) + in; };
     float m = -INFINITY, l = 0.0f, o[4] = {};  // l: of the warp's own parts
     for (int k0 = 0; k0 < parts; k0 += JOIN_PARTS) {
         const int n = min(parts - k0, JOIN_PARTS);
@@ -102,7 +104,7 @@ TreePlan plan_of(int dtype, int head_dim, int seqs, int kv_heads, int group, int
 // Floats of scratch of a step of these sizes.
 FERRIS_API long long ferris_tree_attention_scratch(int dtype, int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size,
                                                    long long cache_rows, float scale, int window) {
-    return plan_of(dtype, head_dim, seqs, kv_heads, group, max_nodes, max_kv, page_size, cache_rows, scale, window).floats(seqs, kv_heads, head_dim);
+    return plan_of(dtype, head_dim, seqs, kv_heads, group, max_nodes, max_kv, page_size, cache_rows, scale, window).floats(head_dim);
 }
 
 // Arguments as ops.tree_attention lays them out.
@@ -120,7 +122,6 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     if (a->pages <= 0 || a->page_size <= 0 || a->width <= 0 || a->max_kv <= 0)
         FERRIS_REFUSE("%d pages of %d rows, tables of %d blocks, %d rows at most", a->pages, a->page_size, a->width, a->max_kv);
     if (((uintptr_t)a->k_cache | (uintptr_t)a->v_cache) & 15) FERRIS_REFUSE("the cache must begin on 16 bytes");
-    if (a->seqs > 65535 || (long long)a->max_nodes * a->heads > 65535 * 8ll) FERRIS_REFUSE("%d requests of %d tokens exceed one launch", a->seqs, a->max_nodes);
     if (!a->parts || ((uintptr_t)a->parts & 15)) FERRIS_REFUSE("parts need scratch that begins on 16 bytes");
     TreeAttention p;
     p.q = a->q, p.out = const_cast<void*>(a->out), p.k_cache = a->k_cache, p.v_cache = a->v_cache;
@@ -136,16 +137,14 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     p.status = ferris_status_ptr();
     const TreePlan plan = plan_of(a->dtype, a->head_dim, a->seqs, a->kv_heads, p.group, a->max_nodes, p.limit, a->page_size,
                                   (long long)a->pages * a->kv_heads * a->page_size, a->scale, a->window);
-    if (!plan.fits) FERRIS_REFUSE("%d requests of up to %d rows exceed one launch", a->seqs, p.limit);
+    if (!plan.fits) FERRIS_REFUSE("%d requests of up to %d tokens and %d rows exceed one launch", a->seqs, a->max_nodes, p.limit);
     p.parts = (float*)const_cast<void*>(a->parts);
-    p.spans = (int2*)(p.parts + plan.part_floats(p.head_dim));
-    p.row_blocks = plan.row_blocks;
+    p.begun = (int4*)(p.parts + plan.part_floats(p.head_dim));
     const cudaStream_t stream = (cudaStream_t)a->stream;
     const int rc = a->dtype != FERRIS_BF16 ? tree_attention_f32(p, plan, stream) : plan.tensor ? tree_attention_tc(p, plan, stream) : tree_attention_mma(p, plan, stream);
     if (rc != FERRIS_OK) return rc;
-    const int at_once = plan.rows < 32 ? plan.rows : 32;  // rows of a block of query rows that a block joins
-    const int slices = (p.max_nodes * p.group + at_once - 1) / at_once;
-    const dim3 grid((p.head_dim + 31) / 32, slices * p.kv_heads, p.seqs);
+    const int slices = (plan.rows + 31) / 32;
+    const dim3 grid((p.head_dim + 31) / 32, slices * plan.lanes, plan.groups);
     const auto kernel = a->dtype == FERRIS_BF16 ? tree_parts_kernel<bf16> : tree_parts_kernel<float>;
     const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, stream, p, plan.rows, plan.lanes, slices);
     if (e != cudaSuccess) {

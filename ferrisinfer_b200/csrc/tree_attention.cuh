@@ -33,8 +33,7 @@ struct TreeAttention {
     float scale;  // of the scores, times log2(e)
     DivideBy page;  // the page size
     float* parts;
-    int2* spans;  // first and last group of every item: request (that has nodes), kv head, block of query rows
-    int row_blocks;
+    int4* begun;  // of every group: the item that begins in it and goes on in others
     int* status;
 };
 
@@ -133,21 +132,19 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeAttention& p, const Tree
 struct TreePlan {
     int unit, rows;          // cached rows of a tile, query rows of a block
     int groups, lanes;       // groups of blocks, blocks of a group
-    int row_blocks;          // of a request at most
     bool tensor;             // on tcgen05 (tree_attention_tc.cu), otherwise on mma.sync (tree_attention_mma.cu)
-    bool fits;               // tiles are counted in 32 bits
+    bool fits;               // tiles are counted in 32 bits, and lanes are a launch's second dimension
     long long part_floats(int head_dim) const { return 2ll * groups * lanes * rows * (head_dim + 2); }
-    long long floats(int seqs, int kv_heads, int head_dim) const {  // of scratch: parts, and behind them who has the items
-        return part_floats(head_dim) + 2ll * seqs * kv_heads * row_blocks;
-    }
+    long long floats(int head_dim) const { return part_floats(head_dim) + 4ll * groups; }  // of scratch: parts, and behind them the items that groups have begun
     // As many blocks as the SMs have room for (`blocks` on each), and there can be tiles for.
     void deal(int seqs, int kv_heads, int group, int max_nodes, int max_kv, int blocks, bool flat) {
         const int sms = ferris_sm_count();
-        row_blocks = (max_nodes * group + rows - 1) / rows, lanes = flat ? 1 : row_blocks;
+        const int row_blocks = (max_nodes * group + rows - 1) / rows;
+        lanes = flat ? 1 : row_blocks;
         const long long most = (long long)seqs * kv_heads * (flat ? row_blocks : 1) * ((max_kv + unit - 1) / unit + 1);
         const long long room = (long long)(sms > 0 ? sms : 148) * blocks / lanes;
         groups = (int)(room < 1 ? 1 : room < most ? room : most);
-        fits = most <= 0x7fffffff;
+        fits = most <= 0x7fffffff && lanes <= 4096;
     }
 };
 TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window);
@@ -212,8 +209,11 @@ struct TreeWalk {
         const int longer = more * (per + 1);
         return tile < longer ? tile / (per + 1) : more + (tile - longer) / per;
     }
-    // First and last group of an item.
-    __device__ __forceinline__ int2 span(const TreeItem& i) const { return make_int2(owner(i.start), owner(i.start + i.tiles - 1)); }
+    // What is written into TreeAttention::begun when an item goes on in the groups behind this one: request (-1: no such item), kv head, block of query rows, last group.
+    static __device__ __forceinline__ int4 none() { return make_int4(-1, 0, 0, 0); }
+    __device__ __forceinline__ void note(const TreeItem& i, int4& begun) const {
+        if (i.first == 0 && i.last < i.tiles) begun = make_int4(i.seq, i.head, i.block, owner(i.start + i.tiles - 1));
+    }
 
     __device__ __forceinline__ bool next(const TreeAttention& p, TreeItem& item) {
         while (at < end) {
@@ -242,11 +242,6 @@ struct TreeWalk {
         return false;
     }
 };
-
-// Who has an item, said by the block that has its beginning.
-__device__ __forceinline__ int2& tree_span(const TreeAttention& p, int seq, int head, int block) {
-    return p.spans[(seq * p.kv_heads + head) * p.row_blocks + block];
-}
 
 // Where a block's part lies: of an item that begins in it, or of one that began in front of it.  Column c of row r at [c][r]: D columns of the
 // unnormalised output, the maximum (to the base of 2), the sum.

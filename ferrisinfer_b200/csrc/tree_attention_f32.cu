@@ -47,12 +47,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
     TreeWalk<Z::TILE, Z::ROWS, true> walk;
     walk.begin(p, 1);
     TreeItem item;
+    int4 begun = walk.none();
     while (walk.next(p, item)) {
         const TreeRequest r = item.request;
         const int head = item.head, count = r.nodes * p.group, row0 = item.block * Z::ROWS;
         const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
-        if (first == 0 && threadIdx.x == 0) tree_span(p, item.seq, head, item.block) = walk.span(item);
+        walk.note(item, begun);
         const int* table = p.tables + (size_t)item.seq * p.width;
         // ---- cached rows on their way: a warp takes every eighth of the tile
         auto request = [&](int i) {
@@ -254,6 +255,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
         }
         __syncthreads();  // the tiles and the query rows may be written again
     }
+    if (threadIdx.x == 0) p.begun[blockIdx.x] = begun;
 }
 
 template <int DP, int G>

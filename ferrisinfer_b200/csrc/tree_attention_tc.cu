@@ -156,9 +156,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (warp == SOFTMAX_WARPS) {
             // ---- K and V on their way: eight lanes, a box of 16 rows each
             int place0 = 0;
+            int4 begun = walk.none();
             while (walk.next(p, item)) {
                 const TreeRequest r = item.request;
-                if (item.first == 0 && lane == 0) tree_span(p, item.seq, item.head, item.block) = walk.span(item);
+                walk.note(item, begun);
                 const int* table = p.tables + (size_t)item.seq * p.width;
                 const int n = item.last - item.first;
                 // the page of a lane's box of unit i, on its way; its row of the cache; outside the cache where there is none: nought
@@ -196,6 +197,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 place0 += 2 * n;
             }
+            if (lane == 0 && blockIdx.x % lanes == 0) p.begun[blockIdx.x / lanes] = begun;  // (the first block of a group has query rows of every item)
             // (after a wait that ran out: nothing may still be on its way when the block ends)
             if (dead)
                 for (int at = max(0, place0 - ST); at < place0; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);

@@ -67,12 +67,20 @@ struct Pass {
     bool aligned;
 };
 
-// What is left of an element after the refusals so far.
-__device__ __forceinline__ double residual(const Shared& s, int refusals, float p, float q) {
-    double r = (double)probability(p);
-    const double qq = (double)probability(q);
-    for (int k = 0; k < refusals; ++k) r = fmax(__dsub_rn(r, __dmul_rn(s.refused[k], qq)), 0.0);  // (two roundings, as written)
-    return r;
+// What is left of elements after the refusals so far.
+template <int N>
+__device__ __forceinline__ void residuals(const Shared& s, int refusals, const float (&p)[N], const float (&q)[N], double (&r)[N]) {
+    double qq[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) r[j] = (double)probability(p[j]), qq[j] = (double)probability(q[j]);
+    for (int k = 0; k < refusals; ++k) {
+        const double left = s.refused[k];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const double x = __dsub_rn(r[j], __dmul_rn(left, qq[j]));  // (two roundings, as written)
+            r[j] = x > 0.0 ? x : 0.0;
+        }
+    }
 }
 
 // Four neighbours from i on, of both rows; nought behind the run's end.
@@ -101,16 +109,15 @@ __device__ __forceinline__ void left_of(const Shared& s, int i, float4 p, float4
             if (at == 2) p.z = 0.0f;
             if (at == 3) p.w = 0.0f;
         }
-    r[0] = DRAFT ? residual(s, refusals, p.x, q.x) : (double)probability(p.x);
-    r[1] = DRAFT ? residual(s, refusals, p.y, q.y) : (double)probability(p.y);
-    r[2] = DRAFT ? residual(s, refusals, p.z, q.z) : (double)probability(p.z);
-    r[3] = DRAFT ? residual(s, refusals, p.w, q.w) : (double)probability(p.w);
+    const float ps[4] = {p.x, p.y, p.z, p.w}, qs[4] = {q.x, q.y, q.z, q.w};
+    residuals(s, DRAFT ? refusals : 0, ps, qs, r);
 }
 
-// The sum of what is left of a warp's run, five groups of 128 elements on their way at once (one at a time, a pass over 151,936 elements waited ten times for memory).
+// The sum of what is left of a warp's run, AHEAD groups of 128 elements on their way at once: two (five are more than registers have room for beside the doubles
+// of two blocks an SM: 64 requests took 66 us, with three 51, with two 48).
 template <bool DRAFT>
 __device__ __forceinline__ double run_sum(const Shared& s, const Pass& w, int refusals, int gone) {
-    constexpr int AHEAD = 5;
+    constexpr int AHEAD = 2;
     double sum = 0.0, r[4];
     for (int i0 = w.lo + 4 * (threadIdx.x & 31); i0 < w.hi; i0 += 128 * AHEAD) {
         float4 p[AHEAD], q[AHEAD];
@@ -125,7 +132,7 @@ __device__ __forceinline__ double run_sum(const Shared& s, const Pass& w, int re
     return warp_sum64(sum);
 }
 
-__global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a) {
+__global__ void __launch_bounds__(THREADS, 2) verify_tree_kernel(const VerifyTree a) {
     __shared__ Shared s;
     cluster_arrive_relaxed();
     pdl_wait();
@@ -194,9 +201,12 @@ __global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyTree a
     for (int c = 1; c < n; ++c) {
         if (s.parent[c] != node || path == a.width) continue;
         double r;
-        if (drafted)
-            r = residual(s, refusals, s.p[c], s.q[c]);
-        else {
+        if (drafted) {
+            const float ps[1] = {s.p[c]}, qs[1] = {s.q[c]};
+            double rs[1];
+            residuals(s, refusals, ps, qs, rs);
+            r = rs[0];
+        } else {
             r = s.p[c];
             for (int g = 0; g < gone; ++g)
                 if (s.gone[g] == s.token[c]) r = 0.0;

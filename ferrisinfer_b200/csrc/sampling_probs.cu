@@ -95,8 +95,8 @@ struct Shared {
             u32 mass[3][BINS];
         };
         Entry list[LIST];  // this block's elements of a bin, when the histograms have been added up
+        Entry all[LIST];   // and then the row's, when nobody reads the others' any more
     };
-    Entry all[LIST];  // the row's
     u32 own_count[OWN_BINS];  // the row's, of this block's bins
     u64 own_mass[OWN_BINS];
     // what blocks tell each other, by the teller's rank (stores into the others' memory; reading it from there takes thousands of cycles)
@@ -411,11 +411,12 @@ __device__ u32 gather(Shared& s, const Row& r, float low, float high, Take take)
         const u32 x = __shfl_sync(0xffffffffu, upto, k);
         if (threadIdx.x >= x) from = k + 1, before = x;
     }
-    if (threadIdx.x < total && threadIdx.x - before < LIST) {
-        s.all[threadIdx.x].key = ld_peer_shared_u64(&s.list[threadIdx.x - before].key, from);
-        s.all[threadIdx.x].mass = ld_peer_shared_u64(&s.list[threadIdx.x - before].mass, from);
-    }
-    cluster_sync();  // the lists are complete, and nobody's own is read any more
+    const bool in = threadIdx.x < total && threadIdx.x - before < LIST;
+    Entry mine;
+    if (in) mine.key = ld_peer_shared_u64(&s.list[threadIdx.x - before].key, from), mine.mass = ld_peer_shared_u64(&s.list[threadIdx.x - before].mass, from);
+    cluster_sync();  // (nobody's own is read any more)
+    if (in) s.all[threadIdx.x] = mine;
+    __syncthreads();
     return total;
 }
 
@@ -848,23 +849,47 @@ __global__ void __launch_bounds__(PLAIN_THREADS, 4) sampling_softmax_kernel(cons
 }  // namespace
 
 // logits, out fp32 [rows, vocab] with row strides ldl, ldo: the same memory, or apart.  temperature, top_k, top_p: per row, or null for greedy rows.
+// How many clusters of `blocks` run at once: clusters lie in parts of the GPU that have different numbers of SMs, so that these are fewer than the SMs have room
+// for (of seven blocks, two on an SM, 37 for 42).
+static int clusters_at_once(int blocks, bool keep, size_t bytes) {
+    static thread_local struct { size_t bytes; int clusters; } asked[MOST_BLOCKS + 1] = {};
+    auto& known = asked[blocks];
+    if (known.clusters && known.bytes == bytes) return known.clusters;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, 1, blocks), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = bytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = blocks;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    int n = 0;
+    if (keep && ferris_allow_dynamic_smem((const void*)sampling_probs_kernel<true>, (int)bytes) != FERRIS_OK) return 1;
+    const cudaError_t e = keep ? cudaOccupancyMaxActiveClusters(&n, sampling_probs_kernel<true>, &cfg) : cudaOccupancyMaxActiveClusters(&n, sampling_probs_kernel<false>, &cfg);
+    if (e != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        return 1;
+    }
+    known.bytes = bytes, known.clusters = n;
+    return n;
+}
+
 FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* out, long long ldo, int rows, int vocab, const float* temperature,
                                      const int* top_k, const float* top_p, void* stream) {
     if (rows <= 0) return FERRIS_OK;
     if (vocab <= 0 || ldl < vocab || ldo < vocab) FERRIS_REFUSE("vocabulary %d, row strides %lld and %lld", vocab, ldl, ldo);
     if (vocab > MOST_BLOCKS * MOST_ELEMENTS) FERRIS_REFUSE("a vocabulary of %d, at most %d", vocab, MOST_BLOCKS * MOST_ELEMENTS);
-    // Blocks of a row: of as many as give the least time if blocks run in waves, each as long as its share of the row (40 rows of 151,936: seven, 280 blocks at once,
-    // where eight would leave 24 of them for a second wave).
+    // Blocks of a row: of as many as give the least time if clusters run in waves, each as long as a block's share of the row (40 rows of 151,936: six, all at once,
+    // 60 us; seven, of which 37 run at once, 84).
     const int sms = ferris_sm_count();
-    int blocks = MOST_BLOCKS;
+    int blocks = MOST_BLOCKS, at_once = 1;
     double least = 0.0;
     auto per_block = [&](int b) { return (int)(((long long)vocab + 4 * b - 1) / (4 * b)) * 4; };
     const size_t fixed = sizeof(Shared) + 1024, most = 227 * 1024;  // (an SM keeps a KB of every block's for itself)
     for (int b = MOST_BLOCKS; b >= LEAST_BLOCKS; --b) {
-        const size_t bytes = (size_t)per_block(b) * 4 + fixed;
-        const long long at_once = (bytes <= most / 2 || bytes > most ? 2ll : 1ll) * (sms > 0 ? sms : 148);
-        const double time = (double)(((long long)rows * b + at_once - 1) / at_once) / b;
-        if (b == MOST_BLOCKS || (time < least && per_block(b) <= MOST_ELEMENTS)) least = time, blocks = b;
+        const size_t bytes = (size_t)per_block(b) * 4;
+        const bool keep = bytes + fixed <= most;
+        const int clusters = clusters_at_once(b, keep, keep ? bytes : 0);
+        const double time = (double)((rows + clusters - 1) / clusters) / b;
+        if (b == MOST_BLOCKS || (time < least && per_block(b) <= MOST_ELEMENTS)) least = time, blocks = b, at_once = clusters;
     }
     SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks), rows, 0};
     cudaError_t e;
@@ -889,7 +914,7 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
         a.skip = 1;
     }
     const size_t bytes = (size_t)a.per * 4;
-    const int at_once = 2 * sms / blocks, clusters = a.skip && at_once < rows ? at_once : rows;
+    const int clusters = a.skip && at_once < rows ? at_once : rows;
     if (bytes + fixed <= most) {
         const int rc = ferris_allow_dynamic_smem((const void*)sampling_probs_kernel<true>, bytes);
         if (rc != FERRIS_OK) return rc;

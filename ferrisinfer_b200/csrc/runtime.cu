@@ -3,6 +3,8 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include <mutex>
+
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -76,14 +78,21 @@ FERRIS_API int ferris_sm_count() {
 // The status word that kernels with bounded waits write when a wait runs out.
 // ---------------------------------------------------------------------------------------------
 static __device__ int g_status_word = 0;
-static int* g_status_ptr = nullptr;
+constexpr int STATUS_DEVICES = 64;
+static int* g_status_ptr[STATUS_DEVICES] = {};
 
+// The current device's: every device has a word of its own.
 int* ferris_status_ptr() {
-    if (!g_status_ptr) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return nullptr;
+    int* known = dev < STATUS_DEVICES ? g_status_ptr[dev] : nullptr;
+    if (!known) {
         void* p = nullptr;
-        if (cudaGetSymbolAddress(&p, g_status_word) == cudaSuccess) g_status_ptr = (int*)p;
+        if (cudaGetSymbolAddress(&p, g_status_word) != cudaSuccess) return nullptr;
+        known = (int*)p;
+        if (dev < STATUS_DEVICES) g_status_ptr[dev] = known;
     }
-    return g_status_ptr;
+    return known;
 }
 
 // Reads and clears the status word (synchronises the device).  0 = no kernel reported a fault.
@@ -135,7 +144,7 @@ struct MapSlot {
     bool used;
 };
 constexpr int MAP_SLOTS = 256;
-MapSlot g_map_slots[MAP_SLOTS];
+thread_local MapSlot g_map_slots[MAP_SLOTS];  // (every thread's own: Python calls the library without its lock)
 inline bool same(const MapKey& a, const MapKey& b) {
     return a.base == b.base && a.rows == b.rows && a.cols == b.cols && a.row_stride == b.row_stride &&
            a.box_rows == b.box_rows && a.box_cols == b.box_cols && a.kind == b.kind;
@@ -271,6 +280,7 @@ struct SmemAllowance {
 constexpr int ALLOWANCES = 256;
 SmemAllowance g_allowances[ALLOWANCES];
 int g_allowance_count = 0;
+std::mutex g_allowance_lock;  // (a smaller allowance, set behind a greater one's back, would take that away)
 }  // namespace
 
 int ferris_allow_dynamic_smem(const void* fn, size_t bytes) {
@@ -280,6 +290,7 @@ int ferris_allow_dynamic_smem(const void* fn, size_t bytes) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;
     }
+    const std::lock_guard<std::mutex> lock(g_allowance_lock);
     SmemAllowance* hit = nullptr;
     for (int i = 0; i < g_allowance_count; ++i)
         if (g_allowances[i].fn == fn && g_allowances[i].device == dev) {

@@ -2669,8 +2669,6 @@ TREE_NODES = 256  # most tokens of a request's tree
 _TREE_ATTENTION = struct.Struct("=10Q14if")
 _TREE_ROWS = struct.Struct("=6Q9i")
 _VERIFY_TREE = struct.Struct("=10Q2q4i")
-_tree_buffer = ctypes.create_string_buffer(max(_TREE_ATTENTION.size, _TREE_ROWS.size, _VERIFY_TREE.size))
-_tree_buffer_at = ctypes.addressof(_tree_buffer)
 
 
 def _on_current_device(what: str, *tensors) -> int:
@@ -2752,13 +2750,13 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     if T == 1:
         ldq, ldo = max(ldq, cols), max(ldo, cols)
     try:
-        _TREE_ATTENTION.pack_into(
-            _tree_buffer, 0, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_q_start.data_ptr(),
+        arguments = _TREE_ATTENTION.pack(
+            q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_q_start.data_ptr(),
             seq_start_row.data_ptr(), parents.data_ptr(), workspace.address("tree_attention", scratch, torch.float32), _current_stream(), ldq, ldo, dt,
             pages, hkv, page_size, D, width, S, T, num_heads, max_q_len, max_kv_len, min(window, 0x7fffffff), scale)
     except (struct.error, OverflowError) as e:
         raise KernelError(f"{what}: a stride, size or scale beyond 32 bits ({e})") from None
-    _check(_packed_lib().ferris_tree_attention(_tree_buffer_at), what, 2)
+    _check(_packed_lib().ferris_tree_attention(arguments), what, 2)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2847,13 +2845,13 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     if draft_probs is not None and ldd < V:
         draft_probs, ldd = draft_probs.contiguous(), V
     try:
-        _VERIFY_TREE.pack_into(
-            _tree_buffer, 0, probs.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
+        arguments = _VERIFY_TREE.pack(
+            probs.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
             seq_q_start.data_ptr(), uniforms.data_ptr(), out_nodes.data_ptr(), out_accepted.data_ptr(), out_token.data_ptr(), _current_stream(),
             ldp, ldd, S, T, V, out_nodes.shape[1])
     except struct.error as e:
         raise KernelError(f"{what}: a size beyond 32 bits ({e})") from None
-    _check(_packed_lib().ferris_verify_tree(_tree_buffer_at), what)
+    _check(_packed_lib().ferris_verify_tree(arguments), what)
 
 
 class CacheLayers:
@@ -2903,7 +2901,7 @@ def keep_tree_rows(layers: CacheLayers, block_tables: torch.Tensor, seq_start_ro
         raise KernelError(f"{what}: paths of at most {TREE_NODES} nodes, not {nodes.shape[1]}")
     if S == 0 or nodes.shape[1] <= 1 or block_tables.shape[1] == 0:
         return
-    _TREE_ROWS.pack_into(_tree_buffer, 0, layers.table.data_ptr(), block_tables.data_ptr(), seq_start_row.data_ptr(), nodes.data_ptr(), accepted.data_ptr(),
-                         _current_stream(), len(layers.layers), layers.pages, layers.kv_heads, layers.page_size, layers.row_bytes, layers.align,
-                         block_tables.shape[1], S, nodes.shape[1])
-    _check(_packed_lib().ferris_tree_rows(_tree_buffer_at), what)
+    arguments = _TREE_ROWS.pack(layers.table.data_ptr(), block_tables.data_ptr(), seq_start_row.data_ptr(), nodes.data_ptr(), accepted.data_ptr(),
+                                _current_stream(), len(layers.layers), layers.pages, layers.kv_heads, layers.page_size, layers.row_bytes, layers.align,
+                                block_tables.shape[1], S, nodes.shape[1])
+    _check(_packed_lib().ferris_tree_rows(arguments), what)

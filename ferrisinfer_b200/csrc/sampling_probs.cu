@@ -910,7 +910,7 @@ FERRIS_API int ferris_sampling_probs(const float* logits, long long ldl, float* 
     }
     SamplingProbs a = {logits, out, ldl, ldo, temperature, top_k, top_p, vocab, per_block(blocks), rows, 0};
     cudaError_t e;
-    // More rows than run at once: those without top-k and top-p by the kernel of smaller blocks (37 rows without it 14.7 us, 38 with it 13.0, 512 rows 231 without and
+    // More rows than run at once: those without top-k and top-p by the kernel of smaller blocks (37 rows without it 14.7 us, 38 with it 13.0, 512 rows 190 without and
     // 120 with; of fewer rows the launch would cost more than it saves: 16 rows 10.8).
     int parts = (vocab + PLAIN_SHARE - 1) / PLAIN_SHARE;
     if ((long long)rows * MOST_BLOCKS > 2ll * sms && per_block(PLAIN_BLOCKS) <= PLAIN_SHARE && temperature) {

@@ -77,11 +77,11 @@ struct TreeLines {
     short depth[TREE_NODES];
 };
 
-// By the first `threads` of a block, for whom `barrier` is one; they are synchronised when it returns.  A parent that is not an earlier node of the
+// By THREADS of a block, for whom `barrier` is one; they are synchronised when it returns.  A parent that is not an earlier node of the
 // request counts as none.
 template <int THREADS, typename Barrier>
 __device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeRequest& r, TreeLines& t, Barrier barrier) {
-    for (int i = threadIdx.x; i < r.nodes; i += THREADS) {
+    for (int i = threadIdx.x % THREADS; i < r.nodes; i += THREADS) {
         int up = p.parents[r.first + i];
         if (up >= i || up < -1) {
             ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 112);
@@ -90,7 +90,7 @@ __device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeReq
         t.parent[i] = (short)up;
     }
     barrier();
-    for (int i = threadIdx.x; i < r.nodes; i += THREADS) {
+    for (int i = threadIdx.x % THREADS; i < r.nodes; i += THREADS) {
 #pragma unroll
         for (int w = 0; w < TREE_WORDS; ++w) t.line[i][w] = 0u;
         int depth = 0;
@@ -190,18 +190,18 @@ struct TreeWalk {
         if (seq < p.seqs) mine = tree_request(p, seq);
         upto = tree_scan(mine.nodes > 0 ? tiles(p, mine) * blocks(p, mine) * p.kv_heads : 0);
     }
-    __device__ __forceinline__ void begin(const TreeAttention& p, int lanes) {
-        const int group = blockIdx.x / lanes, chunks = (p.seqs + 31) / 32;
-        lane_block = blockIdx.x - group * lanes;
+    // Group `group` of `groups` (one beyond them has nothing).
+    __device__ __forceinline__ void begin(const TreeAttention& p, int group, int groups, int lane) {
+        const int chunks = (p.seqs + 31) / 32;
+        lane_block = lane;
         int total = 0;
         for (int c = 0; c < chunks; ++c) {
             look_at(p, c);
             before = total;
             total += __shfl_sync(0xffffffffu, upto, 31);
         }
-        const int groups = gridDim.x / lanes;  // (those that have no tiles leave no part either)
         per = total / groups, more = total - per * groups;
-        at = group * per + min(group, more), end = at + per + (group < more);
+        at = group * per + min(group, more), end = group < groups ? at + per + (group < more) : at;  // (groups that have no tiles leave no part either)
         if (chunks > 1) look_at(p, 0), before = 0;
     }
     // The group that has a tile.

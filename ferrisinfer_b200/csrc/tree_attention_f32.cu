@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
     pdl_wait();
     pdl_launch_dependents();
     TreeWalk<Z::TILE, Z::ROWS, true> walk;
-    walk.begin(p, 1);
+    walk.begin(p, blockIdx.x, gridDim.x, 0);
     TreeItem item;
     int4 begun = walk.none();
     while (walk.next(p, item)) {

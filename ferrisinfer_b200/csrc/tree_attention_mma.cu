@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
     pdl_wait();
     pdl_launch_dependents();
     TreeWalk<P::UNIT, P::ROWS, true> walk;
-    walk.begin(p, 1);
+    walk.begin(p, blockIdx.x, gridDim.x, 0);
     TreeItem item;
     int4 begun = walk.none();
     while (walk.next(p, item)) {
@@ -431,7 +431,7 @@ TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_node
     const int rows = max_nodes * group, sms = ferris_sm_count();
     const bool many = rows > 64 || (rows > 32 && (long long)seqs * kv_heads * ((max_kv + 127) / 128) > 4ll * (sms > 0 ? sms : 148));
     plan.tensor = many && (head_dim == 64 || head_dim == 128) && page_size % 16 == 0 && cache_rows < 0x7fffffff && scale > 0.0f && scale < 1e30f;
-    if (plan.tensor) plan.unit = 128, plan.rows = max_nodes * group > 128 ? 256 : 128, blocks = 1;
+    if (plan.tensor) plan.unit = 128, plan.rows = rows > 128 ? 256 : 128, blocks = rows > 128 ? 1 : 2;  // (two groups to a block)
     plan.deal(seqs, kv_heads, group, max_nodes, max_kv, blocks, !plan.tensor);
     return plan;
 }

@@ -6,12 +6,13 @@
 //   P = 2^(S scale - m), rounded to bf16 (eight bits, as the output has; sums take it unrounded), into tensor memory over the scores it came from
 //   O = O + P V   P from tensor memory, V as TMA wrote it, sums in tensor memory over all units
 // Two groups of four softmax warps, each with scores, maxima, sums and outputs of its own, so that the tensor core works for one while
-// the other exponentiates: of up to 128 query rows they take the units in turn and are joined at the end, of more (WIDE) each has 128 rows of its own, and K and V are
-// fetched once for both; a thread has a row, so that nothing is exchanged.
+// the other exponentiates; a thread has a row, so that nothing is exchanged.  Of up to 128 query rows each group goes over a share of its own, with a ring of
+// stages, a TMA warp and an MMA warp of its own: one begins or ends an item while the other goes on.  Of more (WIDE) each has 128 rows of one item, and K and V are
+// fetched once for both.
 // m is the greatest score so far only up to 2^8: outputs are brought to a new m (read, multiplied, written back) where a score exceeds it by
 // more than eight, which after the first units is rare; what is divided by in the end has the same m, so that nothing but the range of the weights changes.
 // A TMA warp streams K and V through a ring of stages, ahead of the segment that is worked on; an MMA warp issues, in the order of the units,
-// P V of a unit and then the scores of the group's next one (the tensor core keeps the order, so that these do not overwrite weights that are still read).
+// P V of a unit and then the scores of the next one (the tensor core keeps the order, so that these do not overwrite weights that are still read).
 //
 // Units that every node sees whole are worked off as they are.  In others scores that are not seen become nought weights; as nought times NaN is NaN, the softmax
 // warps then look through the unit's values, set what is not finite to nought and add it, element by element, to the outputs of those who see it.
@@ -26,7 +27,7 @@
 namespace {
 
 constexpr int ROWS = 128, UNIT = 128, PAGE_ROWS = 16;  // (a TMA box: 16 rows of 64 columns)
-constexpr int SOFTMAX_WARPS = 8, THREADS = (SOFTMAX_WARPS + 4) * 32;  // + a TMA warp, an MMA warp and two without work: whole warpgroups share out registers
+constexpr int SOFTMAX_WARPS = 8, THREADS = (SOFTMAX_WARPS + 4) * 32;  // + two TMA warps and two MMA warps, of which WIDE has work for one each: whole warpgroups share out registers
 // Registers of a thread: the block is launched with LAUNCH_REGISTERS for each (what 384 threads of an SM can have), of which the third warpgroup gives some to
 // the softmax's two; what these take must not be more than that, or they would wait for ever.
 constexpr int LAUNCH_REGISTERS = 168, SOFTMAX_REGISTERS = 208, OTHER_REGISTERS = 80;
@@ -36,8 +37,10 @@ constexpr int SCORES = 0, OUTPUTS = 256, COLUMNS = 512;  // of tensor memory: tw
 
 template <int D, bool WIDE>
 struct Sizes {
-    static constexpr int ATOMS = D / 64, BLOCK = ATOMS * ATOM, TILES = WIDE ? 2 : 1, STAGES = D == 64 ? 8 : WIDE ? 4 : 5;
-    static constexpr int SMEM = BLOCK * (TILES + STAGES) + 1024;
+    static constexpr int ATOMS = D / 64, BLOCK = ATOMS * ATOM, STAGES = D == 64 ? 8 : 4;
+    static constexpr int RING = WIDE ? STAGES : STAGES / 2;  // stages of a ring: both groups' or each one's
+    static constexpr int GROUP_ROWS = WIDE ? 2 * ROWS : ROWS;  // query rows of an item
+    static constexpr int SMEM = BLOCK * (2 + STAGES) + 1024;
 };
 
 __device__ __forceinline__ float exp2_unit(float x) {
@@ -102,48 +105,34 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int W>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[W]) {
-    if constexpr (W == 32)
-        tmem_load_32x32(taddr, r);
-    else
-        tmem_load_32x16(taddr, r);
-}
-
 // All softmax warps; those of one group.
 __device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void group_barrier(int g) { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); }
 
-// Stages in the order of their use by the tensor core: K 0, K 1, V 0, K 2, V 1, K 3, ..; where both groups use them, K 0, V 0, K 1, ..
-template <bool WIDE>
-__device__ __forceinline__ int k_place(int i) { return WIDE ? 2 * i : i < 2 ? i : 2 * i - 1; }
-template <bool WIDE>
-__device__ __forceinline__ int v_place(int i, int n) { return WIDE || i + 1 == n ? 2 * i + 1 : 2 * i + 2; }
-
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 1)
-    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeAttention p, int lanes, int no_row) {
+    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeAttention p, int groups, int lanes, int no_row) {
     using Z = Sizes<D, WIDE>;
-    constexpr int ST = Z::STAGES;
+    constexpr int ST = Z::RING;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ TreeLines tree;
-    __shared__ uint64_t full[ST], empty[ST], q_ready, s_ready[2], p_ready[2], o_done[2];
+    __shared__ TreeLines trees[WIDE ? 1 : 2];
+    __shared__ uint64_t fulls[Z::STAGES], empties[Z::STAGES], q_ready[2], s_ready[2], p_ready[2], o_done[2];
     __shared__ uint32_t tensor_base;
-    __shared__ float row_m[2][ROWS], row_l[2][ROWS];  // (not WIDE)
-    __shared__ int odd[2];  // how many elements of a unit's values are not finite
+    __shared__ int odd[4];  // threads that have found a value of a unit that is not finite: of units of both groups by turns, of each one's
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t* q_smem = smem;                // [64 columns][128 rows][64] bf16, 128-byte swizzle; at a segment's end, half of a group's outputs
-    uint8_t* kv_smem = smem + Z::TILES * Z::BLOCK;  // stages of [64 columns][128 cached rows][64]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* q_smem = smem;                // of each group [64 columns][128 rows][64] bf16, 128-byte swizzle
+    // what this warp works for: softmax warps a group each, TMA and MMA warps with WIDE both
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = warp < SOFTMAX_WARPS ? warp >> 2 : warp & 1, ring = WIDE ? 0 : g * ST;
+    uint8_t* kv_smem = smem + (2 + ring) * Z::BLOCK;  // stages of [64 columns][128 cached rows][64]
+    uint64_t *full = fulls + ring, *empty = empties + ring;
     if (threadIdx.x == 0) {
         tma_prefetch_descriptor(&map_k);
         tma_prefetch_descriptor(&map_v);
-        for (int s = 0; s < ST; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-        mbar_init(&q_ready, SOFTMAX_WARPS);
-        for (int g = 0; g < 2; ++g) mbar_init(&s_ready[g], 1), mbar_init(&p_ready[g], 4), mbar_init(&o_done[g], 1);
+        for (int s = 0; s < Z::STAGES; ++s) mbar_init(&fulls[s], 1), mbar_init(&empties[s], 1);
+        for (int k = 0; k < 2; ++k) mbar_init(&q_ready[k], 4), mbar_init(&s_ready[k], 1), mbar_init(&p_ready[k], 4), mbar_init(&o_done[k], 1);
         mbar_fence_init();
     }
-    if (warp == SOFTMAX_WARPS + 1) tensor_memory_take(&tensor_base, COLUMNS);
+    if (warp == SOFTMAX_WARPS + 2) tensor_memory_take(&tensor_base, COLUMNS);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -154,12 +143,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto wait = [&](uint64_t* bar, int parity, int where) {
         if (!dead) dead = !mbar_wait(bar, parity, p.status, where);
     };
-    TreeWalk<UNIT, ROWS * Z::TILES, false> walk;
-    walk.begin(p, lanes);
+    // which group of the step's this one is (of few, one on every SM)
+    const int share = WIDE ? blockIdx.x / lanes : blockIdx.x + g * gridDim.x;
+    TreeWalk<UNIT, Z::GROUP_ROWS, false> walk;
+    walk.begin(p, share, groups, WIDE ? blockIdx.x - share * lanes : 0);
     TreeItem item;
     if (warp >= SOFTMAX_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
-        if (warp == SOFTMAX_WARPS) {
+        if (WIDE && g) {
+            // (nothing to do)
+        } else if (warp < SOFTMAX_WARPS + 2) {
             // ---- K and V on their way: eight lanes, a box of 16 rows each
             int place0 = 0;
             int4 begun = walk.none();
@@ -192,36 +185,35 @@ __global__ void __launch_bounds__(THREADS, 1)
                 int page = page_of(0), next = page_of(1), after = page_of(2);
                 int now = row_of(0, page), then = row_of(1, next);
                 load(0, &map_k, now);
-                if (!WIDE && n > 1) load(1, &map_k, then);
                 for (int i = 0; i < n; ++i) {
                     const int last = row_of(i + 2, after);
                     after = page_of(i + 3);
-                    load(v_place<WIDE>(i, n), &map_v, now);
-                    if (WIDE && i + 1 < n) load(k_place<WIDE>(i + 1), &map_k, then);
-                    if (!WIDE && i + 2 < n) load(k_place<WIDE>(i + 2), &map_k, last);
+                    load(2 * i + 1, &map_v, now);
+                    if (i + 1 < n) load(2 * i + 2, &map_k, then);
                     now = then, then = last;
                 }
                 place0 += 2 * n;
             }
-            if (lane == 0 && blockIdx.x % lanes == 0) p.begun[blockIdx.x / lanes] = begun;  // (the first block of a group has query rows of every item)
+            if (lane == 0 && share < groups && (!WIDE || share * lanes == blockIdx.x)) p.begun[share] = begun;  // (the first lane has query rows of every item)
             // (after a wait that ran out: nothing may still be on its way when the block ends)
             if (dead)
                 for (int at = max(0, place0 - ST); at < place0; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);
-        } else if (warp == SOFTMAX_WARPS + 1) {
+        } else {
             // ---- products
             const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
             const uint32_t base = uniform(tensor_base);
             int place0 = 0, segments = 0, done0 = 0, done1 = 0;  // done: units of each group
             while (walk.next(p, item)) {
                 const int n = uniform(item.last - item.first);
-                const bool two = WIDE && uniform((item.block * Z::TILES + 1) * ROWS < item.request.nodes * p.group);  // (WIDE: the second group has rows)
-                wait(&q_ready, segments & 1, 141);
+                // the groups that share a unit (WIDE: the second, if it has rows)
+                const int first = WIDE ? 0 : uniform(g), last = WIDE ? uniform((2 * item.block + 1) * ROWS < item.request.nodes * p.group) : first;
+                for (int k = WIDE ? 0 : first; k <= (WIDE ? 1 : first); ++k) wait(&q_ready[k], segments & 1, 141);
                 auto scores = [&](int i, int g) {
-                    const int at = place0 + k_place<WIDE>(i), s = at % ST;
-                    if (!WIDE || g == 0) wait(&full[s], (at / ST) & 1, 142);
+                    const int at = place0 + 2 * i, s = at % ST;
+                    if (g == first) wait(&full[s], (at / ST) & 1, 142);
                     tcgen05_fence_after();
                     if (elected()) {
-                        const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem + (WIDE ? g * Z::BLOCK : 0)));
+                        const uint64_t q_desc = umma_desc_k_major_sw128(smem_u32(q_smem + g * Z::BLOCK));
                         const uint64_t k_desc = umma_desc_k_major_sw128(smem_u32(kv_smem + s * Z::BLOCK));
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k) {
@@ -229,13 +221,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                             tcgen05_mma_bf16(base + SCORES + 128 * g, q_desc + next, k_desc + next, idesc_qk, k > 0 ? 1u : 0u);
                         }
                         tcgen05_commit(&s_ready[g]);
-                        if (!two || g) tcgen05_commit(&empty[s]);
+                        if (g == last) tcgen05_commit(&empty[s]);
                     }
                     __syncwarp();
                 };
-                auto outputs = [&](int i, int g, bool last) {
-                    const int at = place0 + v_place<WIDE>(i, n), s = at % ST;
-                    if (!WIDE || g == 0) wait(&full[s], (at / ST) & 1, 143);
+                auto outputs = [&](int i, int g, bool end) {
+                    const int at = place0 + 2 * i + 1, s = at % ST;
+                    if (g == first) wait(&full[s], (at / ST) & 1, 143);
                     wait(&p_ready[g], (g ? done1 : done0) & 1, 144);
                     if (g)
                         ++done1;
@@ -247,26 +239,17 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int k = 0; k < UNIT / 16; ++k)
                             tcgen05_mma_bf16_ts(base + OUTPUTS + D * g, base + SCORES + 128 * g + 8 * k, v_desc + (uint64_t)(k * (BOX >> 4)), idesc_pv);
-                        if (!two || g) tcgen05_commit(&empty[s]);
-                        if (last) tcgen05_commit(&o_done[g]);
+                        if (g == last) tcgen05_commit(&empty[s]);
+                        if (end) tcgen05_commit(&o_done[g]);
                     }
                     __syncwarp();
                 };
-                if constexpr (WIDE) {
-                    scores(0, 0);
-                    if (two) scores(0, 1);
-                    for (int i = 0; i < n; ++i)
-                        for (int g = 0; g <= two; ++g) {
-                            outputs(i, g, i + 1 == n);
-                            if (i + 1 < n) scores(i + 1, g);
-                        }
-                } else {
-                    for (int i = 0; i < 2 && i < n; ++i) scores(i, i);
-                    for (int i = 0; i < n; ++i) {
-                        outputs(i, i & 1, i + 2 >= n);
-                        if (i + 2 < n) scores(i + 2, i & 1);
+                for (int k = first; k <= last; ++k) scores(0, k);
+                for (int i = 0; i < n; ++i)
+                    for (int k = first; k <= last; ++k) {
+                        outputs(i, k, i + 1 == n);
+                        if (i + 1 < n) scores(i + 1, k);
                     }
-                }
                 __syncwarp();
                 place0 += 2 * n, ++segments;
             }
@@ -274,7 +257,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGISTERS));
         // ---- softmax: group g = warp / 4, a row a thread
-        const int g = warp >> 2, t = threadIdx.x & 127;
+        const int t = threadIdx.x & 127;
+        TreeLines& tree = trees[WIDE ? 0 : g];
+        auto barrier_of_all = [&] {  // of those who work on an item
+            if (WIDE)
+                softmax_barrier();
+            else
+                group_barrier(g);
+        };
         const uint32_t lanes_at = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t my_scores = tensor_base + SCORES + 128 * g + lanes_at, my_out = tensor_base + OUTPUTS + D * g + lanes_at;
         const float scale = p.scale;
@@ -283,44 +273,41 @@ __global__ void __launch_bounds__(THREADS, 1)
             const TreeRequest r = item.request;
             const int head = item.head, count = r.nodes * p.group, n = item.last - item.first;
             const bool whole_item = item.first == 0 && item.last == item.tiles;
-            const int row0 = item.block * ROWS * Z::TILES;
+            const int row0 = item.block * Z::GROUP_ROWS;
             const int at = row0 + (WIDE ? g * ROWS : 0) + t, node = at < count ? at / p.group : -1, q_head = head * p.group + at % p.group;
             const bool live = at - lane < count;                                    // any of the warp's rows
-            const int from = WIDE ? 0 : g, step = WIDE ? 1 : 2;                     // the group's units
-            const bool both = !WIDE || row0 + ROWS < count, here = both || g == 0;  // both groups have rows; this one has
+            const bool both = WIDE && row0 + ROWS < count, here = !WIDE || both || g == 0;  // both groups have rows; this one has
             const int units = here ? n : 0;
             const int* table = p.tables + (size_t)item.seq * p.width;
             {
-                // the block's query rows, half of the columns by each group
+                // the group's query rows
                 const bf16* src = (const bf16*)p.q + (size_t)(r.first + max(node, 0)) * p.ldq + q_head * D;
                 const bool wide = ((uintptr_t)p.q & 15) == 0 && p.ldq % 8 == 0;
-                constexpr int EACH = WIDE ? D / 8 : D / 16;  // 16 bytes at a time: a row, or half of one
-                const int first = WIDE ? 0 : g * EACH;
-                uint8_t* to = q_smem + (WIDE ? g * Z::BLOCK : 0);
+                constexpr int EACH = D / 8;  // 16 bytes at a time
+                uint8_t* to = q_smem + g * Z::BLOCK;
                 uint4 v[EACH];  // (all on their way at once)
 #pragma unroll
                 for (int c = 0; c < EACH; ++c) v[c] = make_uint4(0u, 0u, 0u, 0u);
                 if (node >= 0 && wide) {
 #pragma unroll
-                    for (int c = 0; c < EACH; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * (first + c));
+                    for (int c = 0; c < EACH; ++c) v[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
                 } else if (node >= 0) {
 #pragma unroll
                     for (int c = 0; c < EACH; ++c) {
-                        const unsigned short* x = reinterpret_cast<const unsigned short*>(src + 8 * (first + c));
+                        const unsigned short* x = reinterpret_cast<const unsigned short*>(src + 8 * c);
                         v[c] = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
                     }
                 }
 #pragma unroll
                 for (int c = 0; c < EACH; ++c) {
-                    const int column = first + c;
-                    *reinterpret_cast<uint4*>(to + (column >> 3) * ATOM + swizzle128(t, column & 7)) = v[c];
+                    *reinterpret_cast<uint4*>(to + (c >> 3) * ATOM + swizzle128(t, c & 7)) = v[c];
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&q_ready);
+                if (lane == 0) mbar_arrive(&q_ready[g]);
             }
             const int sure_low = p.window > 0 ? max(0, r.start + r.nodes - p.window) : 0, sure_high = min(r.start, r.rows);
-            if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<SOFTMAX_WARPS * 32>(p, r, tree, softmax_barrier);
+            if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<WIDE ? 256 : 128>(p, r, tree, barrier_of_all);
             {
                 uint32_t nought[32];
 #pragma unroll
@@ -330,15 +317,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tmem_store_wait();
             }
             float m = -INFINITY, l = 0.0f;
+            int looked = 0;
             // the page of a lane's box of a unit's eight, on its way while the unit before is worked on; -1: none
             auto page_of = [&](int i) {
                 const int row = (item.low + item.first + i) * UNIT + lane * PAGE_ROWS, block = (int)p.page.quotient((uint32_t)row);
                 return i < units && lane < UNIT / PAGE_ROWS && row < r.rows && block < p.width ? table[block] : -1;
             };
-            int page = page_of(from);
-            for (int i = from; i < units; i += step) {
+            int page = page_of(0);
+            for (int i = 0; i < units; ++i) {
                 const uint32_t boxes = __ballot_sync(0xffffffffu, page >= 0 && page < p.pages);  // (the TMA warp reports pages that are not there)
-                page = page_of(i + step);
+                page = page_of(i + 1);
                 const int key0 = (item.low + item.first + i) * UNIT;
                 const bool whole = key0 >= sure_low && key0 + UNIT <= sure_high && boxes == 0xffu;
                 wait(&s_ready[g], done & 1, 145);
@@ -367,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (__any_sync(0xffffffffu, up)) {
                         const float now = up ? most : m, corr = now == -INFINITY ? 1.0f : exp2_unit(m - now);
                         l *= corr, m = now;
-                        if (i > from) {
+                        if (i > 0) {
 #pragma unroll 1
                             for (int c = 0; c < D / 16; ++c) {
                                 uint32_t o[16];
@@ -401,14 +389,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 if (!whole) {
                     // the unit's values: what is not finite becomes nought, and goes to those who see it by itself
-                    const int place = place0 + v_place<WIDE>(i, n), stage = place % ST;
+                    const int place = place0 + 2 * i + 1, stage = place % ST;
                     wait(&full[stage], (place / ST) & 1, 146);
                     uint8_t* v = kv_smem + (size_t)stage * Z::BLOCK;
                     // (units that both groups work on are looked through and changed by the first, with the second beside it)
-                    const bool shared = WIDE && both, mine = !shared || g == 0;
-                    int& found = odd[shared ? 0 : g];
+                    const bool mine = !both || g == 0;
+                    int& found = odd[both ? looked & 1 : 2 + g];  // (while the other group may still read the unit's before)
+                    ++looked;
                     auto barrier = [&] {
-                        if (shared)
+                        if (both)
                             softmax_barrier();
                         else
                             group_barrier(g);
@@ -448,16 +437,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                             if (!isfinite(__bfloat162float(*x))) *x = __float2bfloat16_rn(0.0f);
                         }
                         fence_proxy_async();
-                        if (shared) barrier();
+                        if (both) barrier();
                     }
                 }
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[g]);
             }
-            if (units > from) wait(&o_done[g], segments & 1, 147);
+            if (units > 0) wait(&o_done[g], segments & 1, 147);
             tcgen05_fence_after();
-            float* part = tree_part(p, blockIdx.x, item.first == 0, ROWS * Z::TILES) + (WIDE ? g * ROWS : 0) + t;
+            float* part = tree_part(p, WIDE ? blockIdx.x : share, item.first == 0, Z::GROUP_ROWS) + (WIDE ? g * ROWS : 0) + t;
             bf16* out = (bf16*)p.out + (size_t)(r.first + max(node, 0)) * p.ldo + q_head * D;
             const bool wide = ((uintptr_t)p.out & 15) == 0 && p.ldo % 8 == 0;
             // columns of this thread's row, to the output (times `inv`) or to the block's part
@@ -466,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 constexpr int W = sizeof(o) / 4;
                 if (!whole_item) {
 #pragma unroll
-                    for (int j = 0; j < W; ++j) part[(col + j) * (ROWS * Z::TILES)] = __uint_as_float(o[j]);
+                    for (int j = 0; j < W; ++j) part[(col + j) * Z::GROUP_ROWS] = __uint_as_float(o[j]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < W; j += 8) {
@@ -482,62 +471,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             };
             auto leave_sums = [&](float most, float total) {
-                if (!whole_item && node >= 0) part[D * (ROWS * Z::TILES)] = most, part[(D + 1) * (ROWS * Z::TILES)] = total;
+                if (!whole_item && node >= 0) part[D * Z::GROUP_ROWS] = most, part[(D + 1) * Z::GROUP_ROWS] = total;
             };
-            if constexpr (WIDE) {
-                // ---- every group its rows
-                if (live && here) {
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (live && here) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_load_32x32(my_out + 32 * c, o);
-                        tmem_load_wait();
-                        leave(o, 32 * c, inv);
-                    }
-                    leave_sums(m, l);
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_load_32x32(my_out + 32 * c, o);
+                    tmem_load_wait();
+                    leave(o, 32 * c, inv);
                 }
-                softmax_barrier();  // (the lines of ancestors may be written again)
-            } else {
-                // ---- the groups joined through the query rows' memory, each for half of the columns, in two rounds
-                row_m[g][t] = m, row_l[g][t] = l;
-                softmax_barrier();  // (both groups' products are done: nobody reads the query rows any more)
-                const float m1 = row_m[g ^ 1][t], most = fmaxf(m, m1), base = most == -INFINITY ? 0.0f : most;
-                const float f0 = exp2_unit(m - base), f1 = exp2_unit(m1 - base), total = l * f0 + row_l[g ^ 1][t] * f1;
-                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                constexpr int W = D / 4;  // columns of a round
-                float* mine = reinterpret_cast<float*>(q_smem) + g * W * ROWS + t;  // [column][row]: what the other group needs
-                const float* others = reinterpret_cast<const float*>(q_smem) + (g ^ 1) * W * ROWS + t;
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t o[W];
-                    const int col = g * 2 * W + h * W;
-                    if (live) {
-                        tmem_load<W>(my_out + (g ^ 1) * 2 * W + h * W, o);
-                        tmem_load_wait();
-#pragma unroll
-                        for (int j = 0; j < W; ++j) mine[j * ROWS] = __uint_as_float(o[j]);
-                        tmem_load<W>(my_out + col, o);
-                    }
-                    softmax_barrier();
-                    if (live) {
-                        tmem_load_wait();
-#pragma unroll
-                        for (int j = 0; j < W; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f0 + others[j * ROWS] * f1);
-                        leave(o, col, inv);
-                    }
-                    softmax_barrier();
-                }
-                if (g == 0) leave_sums(most, total);
+                leave_sums(m, l);
             }
+            barrier_of_all();  // (the lines of ancestors may be written again)
             place0 += 2 * n;
             // (a phase of o_done passes in every segment in which the group has units, q_ready's in every segment)
-            if (units > from) ++segments;
+            if (units > 0) ++segments;
         }
     }
     tcgen05_fence_before();
     __syncthreads();
-    if (warp == SOFTMAX_WARPS + 1) {
+    if (warp == SOFTMAX_WARPS + 2) {
         tcgen05_fence_after();
         tmem_dealloc(tensor_base, COLUMNS);
     }
@@ -556,8 +511,9 @@ int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
         return cudaFuncGetAttributes(&f, tree_attention_tc_kernel<D, WIDE>) == cudaSuccess ? f.numRegs : 0;
     }();
     if (registers < LAUNCH_REGISTERS) FERRIS_REFUSE("a kernel of %d registers a thread, %d are needed", registers, LAUNCH_REGISTERS);
-    const cudaError_t e = ferris_launch(tree_attention_tc_kernel<D, WIDE>, dim3(plan.groups * plan.lanes), dim3(THREADS), (size_t)Sizes<D, WIDE>::SMEM, stream, map_k, map_v, p,
-                                        plan.lanes, (int)rows);
+    const int sms = ferris_sm_count(), grid = WIDE ? plan.groups * plan.lanes : plan.groups < sms ? plan.groups : sms;
+    const cudaError_t e = ferris_launch(tree_attention_tc_kernel<D, WIDE>, dim3(grid), dim3(THREADS), (size_t)Sizes<D, WIDE>::SMEM, stream, map_k, map_v, p,
+                                        plan.groups, plan.lanes, (int)rows);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;

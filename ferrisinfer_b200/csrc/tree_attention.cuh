@@ -79,10 +79,12 @@ struct TreeLines {
 
 // By THREADS of a block, for whom `barrier` is one; they are synchronised when it returns.  A parent that is not an earlier node of the
 // request counts as none.
+// (`parent`: what tree_parent says of the thread's first node, which may have been on its way for long)
+__device__ __forceinline__ int tree_parent(const TreeAttention& p, const TreeRequest& r, int i) { return i < r.nodes ? p.parents[r.first + i] : -1; }
 template <int THREADS, typename Barrier>
-__device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeRequest& r, TreeLines& t, Barrier barrier) {
+__device__ __forceinline__ void tree_lines(const TreeAttention& p, const TreeRequest& r, TreeLines& t, int parent, Barrier barrier) {
     for (int i = threadIdx.x % THREADS; i < r.nodes; i += THREADS) {
-        int up = p.parents[r.first + i];
+        int up = i < THREADS ? parent : p.parents[r.first + i];
         if (up >= i || up < -1) {
             ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 112);
             up = -1;
@@ -169,6 +171,12 @@ struct TreeItem {
     int start;                    // number of its first tile
 };
 
+// The requests of a step, if they are no more than these, as one block's warps fetch them once for all.
+struct TreeRequests {
+    static constexpr int MOST = 128;
+    int first[MOST], nodes[MOST], start[MOST], rows[MOST], upto[MOST];
+};
+
 // Goes through a group's share, item by item; by whole warps, each for itself.
 template <int UNIT, int ROWS, bool FLAT>
 struct TreeWalk {
@@ -183,26 +191,40 @@ struct TreeWalk {
     }
     static __device__ __forceinline__ int blocks(const TreeAttention& p, const TreeRequest& r) { return FLAT ? (r.nodes * p.group + ROWS - 1) / ROWS : 1; }
 
-    __device__ __forceinline__ void look_at(const TreeAttention& p, int chunk) {
+    __device__ __forceinline__ void look_at(const TreeAttention& p, const TreeRequests& known, int chunk) {
         s0 = chunk;
         const int seq = 32 * chunk + (threadIdx.x & 31);
-        mine.nodes = 0;
+        if (p.seqs <= TreeRequests::MOST) {
+            mine.first = known.first[seq], mine.nodes = known.nodes[seq], mine.start = known.start[seq], mine.rows = known.rows[seq], upto = known.upto[seq];
+            return;
+        }
+        fetch(p, seq);
+    }
+    __device__ __forceinline__ void fetch(const TreeAttention& p, int seq) {
+        mine.first = mine.nodes = mine.start = mine.rows = 0;
         if (seq < p.seqs) mine = tree_request(p, seq);
         upto = tree_scan(mine.nodes > 0 ? tiles(p, mine) * blocks(p, mine) * p.kv_heads : 0);
     }
+    // By all threads of a block (at least TreeRequests::MOST), who have to meet before they begin.
+    __device__ __forceinline__ void know(const TreeAttention& p, TreeRequests& known) {
+        const int seq = threadIdx.x;
+        if (p.seqs > TreeRequests::MOST || (seq & ~31) >= p.seqs) return;
+        fetch(p, seq);
+        known.first[seq] = mine.first, known.nodes[seq] = mine.nodes, known.start[seq] = mine.start, known.rows[seq] = mine.rows, known.upto[seq] = upto;
+    }
     // Group `group` of `groups` (one beyond them has nothing).
-    __device__ __forceinline__ void begin(const TreeAttention& p, int group, int groups, int lane) {
+    __device__ __forceinline__ void begin(const TreeAttention& p, const TreeRequests& known, int group, int groups, int lane) {
         const int chunks = (p.seqs + 31) / 32;
         lane_block = lane;
         int total = 0;
         for (int c = 0; c < chunks; ++c) {
-            look_at(p, c);
+            look_at(p, known, c);
             before = total;
             total += __shfl_sync(0xffffffffu, upto, 31);
         }
         per = total / groups, more = total - per * groups;
         at = group * per + min(group, more), end = group < groups ? at + per + (group < more) : at;  // (groups that have no tiles leave no part either)
-        if (chunks > 1) look_at(p, 0), before = 0;
+        if (chunks > 1) look_at(p, known, 0), before = 0;
     }
     // The group that has a tile.
     __device__ __forceinline__ int owner(int tile) const {
@@ -215,12 +237,12 @@ struct TreeWalk {
         if (i.first == 0 && i.last < i.tiles) begun = make_int4(i.seq, i.head, i.block, owner(i.start + i.tiles - 1));
     }
 
-    __device__ __forceinline__ bool next(const TreeAttention& p, TreeItem& item) {
+    __device__ __forceinline__ bool next(const TreeAttention& p, const TreeRequests& known, TreeItem& item) {
         while (at < end) {
             unsigned here;
             while (!(here = __ballot_sync(0xffffffffu, at < before + upto))) {
                 before += __shfl_sync(0xffffffffu, upto, 31);
-                look_at(p, s0 + 1);
+                look_at(p, known, s0 + 1);
             }
             const int lane = __ffs(here) - 1;
             item.seq = 32 * s0 + lane;

@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
     constexpr int LD = Z::LD, EACH = Z::EACH;
     extern __shared__ __align__(16) float smem[];
     __shared__ TreeLines tree;
+    __shared__ TreeRequests requests;
     __shared__ unsigned long long there[2];  // which of a stage's cached rows have a page
     __shared__ float row_m[WARPS][WARP_ROWS], row_l[WARPS][WARP_ROWS];
     float* qs = smem + 2 * Z::STAGE;
@@ -49,15 +50,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
     pdl_wait();
     pdl_launch_dependents();
     TreeWalk<Z::TILE, Z::ROWS, true> walk;
-    walk.begin(p, blockIdx.x, gridDim.x, 0);
+    walk.know(p, requests);
+    __syncthreads();
+    walk.begin(p, requests, blockIdx.x, gridDim.x, 0);
     TreeItem item;
     int4 begun = walk.none();
-    while (walk.next(p, item)) {
+    while (walk.next(p, requests, item)) {
         const TreeRequest r = item.request;
         const int head = item.head, count = r.nodes * p.group, row0 = item.block * Z::ROWS;
         const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
         walk.note(item, begun);
+        const int parent = tree_parent(p, r, threadIdx.x);
         const int* table = p.tables + (size_t)item.seq * p.width;
         // ---- cached rows on their way: a warp takes every eighth of the tile
         auto request = [&](int i) {
@@ -107,7 +111,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
             *reinterpret_cast<float4*>(qs + row * LD + c) = v;
         }
         // (the lines are only looked at where tiles are not seen whole: those of the tree, and with a window)
-        if (p.window > 0 || (low + last) * Z::TILE > min(r.start, r.rows)) tree_lines<THREADS>(p, r, tree, [] { __syncthreads(); });
+        if (p.window > 0 || (low + last) * Z::TILE > min(r.start, r.rows)) tree_lines<THREADS>(p, r, tree, parent, [] { __syncthreads(); });
         const int slab0 = row0 + slab * WARP_ROWS;
         const bool live = slab0 < count;
         float m[WARP_ROWS], l[WARP_ROWS];

@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
     constexpr int KS = DP / 16, SUB = P::TILE < 32 ? P::TILE : 32, NT = SUB / 8, FETCH = P::FETCH;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ TreeLines tree;
+    __shared__ TreeRequests requests;
     __shared__ uint32_t there[ST][NW];  // which of the cached rows that a warp fetched have a page
     __shared__ float row_m[NW][16 * MS], row_l[NW][16 * MS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -69,15 +70,18 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
     pdl_wait();
     pdl_launch_dependents();
     TreeWalk<P::UNIT, P::ROWS, true> walk;
-    walk.begin(p, blockIdx.x, gridDim.x, 0);
+    walk.know(p, requests);
+    __syncthreads();
+    walk.begin(p, requests, blockIdx.x, gridDim.x, 0);
     TreeItem item;
     int4 begun = walk.none();
-    while (walk.next(p, item)) {
+    while (walk.next(p, requests, item)) {
         const TreeRequest r = item.request;
         const int head = item.head, count = r.nodes * p.group, row0 = item.block * P::ROWS;
         const int first = item.first, last = item.last, low = item.low;
         const bool whole_item = first == 0 && last == item.tiles;
         walk.note(item, begun);
+        const int parent = tree_parent(p, r, threadIdx.x);
         const int* table = p.tables + (size_t)item.seq * p.width;
         // ---- cached rows on their way
         auto request = [&](int i) {
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(NW * 32, Plan<DP, MS, WR, NW, ST>::BLOCKS) tre
         }
         // (the lines are only looked at where tiles are not seen whole: those of the tree, and with a window)
         if (p.window > 0 || (low + last) * P::UNIT > min(r.start, r.rows))
-            tree_lines<NW * 32>(p, r, tree, [] { __syncthreads(); });  // (ends with a barrier)
+            tree_lines<NW * 32>(p, r, tree, parent, [] { __syncthreads(); });  // (ends with a barrier)
         else
             __syncthreads();
         int node[MS][2];

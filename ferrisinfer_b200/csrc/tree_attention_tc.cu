@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int ST = Z::RING;
     extern __shared__ uint8_t smem_raw[];
     __shared__ TreeLines trees[WIDE ? 1 : 2];
+    __shared__ TreeRequests requests;
     __shared__ uint64_t fulls[Z::STAGES], empties[Z::STAGES], q_ready[2], s_ready[2], p_ready[2], o_done[2];
     __shared__ uint32_t tensor_base;
     __shared__ int odd[4];  // threads that have found a value of a unit that is not finite: of units of both groups by turns, of each one's
@@ -146,7 +147,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     // which group of the step's this one is (of few, one on every SM)
     const int share = WIDE ? blockIdx.x / lanes : blockIdx.x + g * gridDim.x;
     TreeWalk<UNIT, Z::GROUP_ROWS, false> walk;
-    walk.begin(p, share, groups, WIDE ? blockIdx.x - share * lanes : 0);
+    walk.know(p, requests);
+    __syncthreads();
+    walk.begin(p, requests, share, groups, WIDE ? blockIdx.x - share * lanes : 0);
     TreeItem item;
     if (warp >= SOFTMAX_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
@@ -156,7 +159,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             // ---- K and V on their way: eight lanes, a box of 16 rows each
             int place0 = 0;
             int4 begun = walk.none();
-            while (walk.next(p, item)) {
+            while (walk.next(p, requests, item)) {
                 const TreeRequest r = item.request;
                 walk.note(item, begun);
                 const int* table = p.tables + (size_t)item.seq * p.width;
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
             const uint32_t base = uniform(tensor_base);
             int place0 = 0, segments = 0, done0 = 0, done1 = 0;  // done: units of each group
-            while (walk.next(p, item)) {
+            while (walk.next(p, requests, item)) {
                 const int n = uniform(item.last - item.first);
                 // the groups that share a unit (WIDE: the second, if it has rows)
                 const int first = WIDE ? 0 : uniform(g), last = WIDE ? uniform((2 * item.block + 1) * ROWS < item.request.nodes * p.group) : first;
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t my_scores = tensor_base + SCORES + 128 * g + lanes_at, my_out = tensor_base + OUTPUTS + D * g + lanes_at;
         const float scale = p.scale;
         int place0 = 0, done = 0, segments = 0;
-        while (walk.next(p, item)) {
+        while (walk.next(p, requests, item)) {
             const TreeRequest r = item.request;
             const int head = item.head, count = r.nodes * p.group, n = item.last - item.first;
             const bool whole_item = item.first == 0 && item.last == item.tiles;
@@ -279,6 +282,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool both = WIDE && row0 + ROWS < count, here = !WIDE || both || g == 0;  // both groups have rows; this one has
             const int units = here ? n : 0;
             const int* table = p.tables + (size_t)item.seq * p.width;
+            const int sure_low = p.window > 0 ? max(0, r.start + r.nodes - p.window) : 0, sure_high = min(r.start, r.rows);
+            const int parent = tree_parent(p, r, WIDE ? threadIdx.x : t);
             {
                 // the group's query rows
                 const bf16* src = (const bf16*)p.q + (size_t)(r.first + max(node, 0)) * p.ldq + q_head * D;
@@ -298,6 +303,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                         v[c] = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
                     }
                 }
+                uint32_t nought[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) nought[c] = 0u;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) tmem_store_32x32(my_out + 32 * c, nought);
+                tmem_store_wait();
 #pragma unroll
                 for (int c = 0; c < EACH; ++c) {
                     *reinterpret_cast<uint4*>(to + (c >> 3) * ATOM + swizzle128(t, c & 7)) = v[c];
@@ -306,16 +317,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_ready[g]);
             }
-            const int sure_low = p.window > 0 ? max(0, r.start + r.nodes - p.window) : 0, sure_high = min(r.start, r.rows);
-            if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<WIDE ? 256 : 128>(p, r, tree, barrier_of_all);
-            {
-                uint32_t nought[32];
-#pragma unroll
-                for (int c = 0; c < 32; ++c) nought[c] = 0u;
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) tmem_store_32x32(my_out + 32 * c, nought);
-                tmem_store_wait();
-            }
+            if (p.window > 0 || (item.low + item.last) * UNIT > sure_high) tree_lines<WIDE ? 256 : 128>(p, r, tree, parent, barrier_of_all);
             float m = -INFINITY, l = 0.0f;
             int looked = 0;
             // the page of a lane's box of a unit's eight, on its way while the unit before is worked on; -1: none

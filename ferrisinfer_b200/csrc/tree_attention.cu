@@ -13,9 +13,10 @@ namespace {
 // maxima and sums, the parts: 9 us by itself for 8 requests of 16 nodes, 9 to 14 for 64.
 constexpr int JOIN_PARTS = 64;  // parts that are joined at once
 
-template <typename T>
+template <typename T, int COLS>
 __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes, int slices) {
-    __shared__ float top[8][32], tile[32][33], factor[JOIN_PARTS][32];
+    constexpr int AHEAD = 64 / COLS;
+    __shared__ float top[8][32], tile[8 * COLS][33], factor[JOIN_PARTS][32];
     pdl_wait();
     pdl_launch_dependents();
     const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -23,13 +24,13 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
     const int4 begun = p.begun[blockIdx.z];
     if (begun.x < 0) return;  // (items that lie in one group are written by it)
     const int seq = begun.x, head = begun.y, lane_block = blockIdx.y / slices, block = lanes > 1 ? lane_block : begun.z, parts = begun.w - blockIdx.z + 1;
-    const int from_row = (blockIdx.y - lane_block * slices) * 32, row0 = block * rows + from_row, col = blockIdx.x * 32 + warp * 4;
+    const int from_row = (blockIdx.y - lane_block * slices) * 32, row0 = block * rows + from_row, col = (blockIdx.x * 8 + warp) * COLS;
     const TreeRequest r = tree_request(p, seq);
     const int count = r.nodes * p.group, in = from_row + lane;
     if (row0 >= count) return;
     const bool live = row0 + lane < count && in < rows;
     auto part = [&](int k) { return tree_part(p, (blockIdx.z + k) * lanes + lane_block, k == 0, rows) + in; };
-    float m = -INFINITY, l = 0.0f, o[4] = {};  // l: of the warp's own parts
+    float m = -INFINITY, l = 0.0f, o[COLS] = {};  // l: of the warp's own parts
     for (int k0 = 0; k0 < parts; k0 += JOIN_PARTS) {
         const int n = min(parts - k0, JOIN_PARTS);
         float x[JOIN_PARTS / 8], y[JOIN_PARTS / 8], most = m;
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
         const float base = most == -INFINITY ? 0.0f : most, corr = exp2f(m - base);
         m = most, l *= corr;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] *= corr;
+        for (int c = 0; c < COLS; ++c) o[c] *= corr;
 #pragma unroll
         for (int u = 0; u < JOIN_PARTS / 8; ++u)
             if (warp + 8 * u < n) {
@@ -57,22 +58,22 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
                 l = fmaf(f, y[u], l);
             }
         __syncthreads();
-        if (live && col < D)  // (heads have a multiple of eight columns)
-            for (int k = 0; k < n; k += 16) {
-                float v[16][4];
+        if (live && col < D)
+            for (int k = 0; k < n; k += AHEAD) {
+                float v[AHEAD][COLS];
 #pragma unroll
-                for (int u = 0; u < 16; ++u)
+                for (int u = 0; u < AHEAD; ++u)
                     if (k + u < n) {
                         const float* from = part(k0 + k + u) + col * rows;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) v[u][c] = from[c * rows];
+                        for (int c = 0; c < COLS; ++c) v[u][c] = col + c < D ? from[c * rows] : 0.0f;
                     }
 #pragma unroll
-                for (int u = 0; u < 16; ++u)
+                for (int u = 0; u < AHEAD; ++u)
                     if (k + u < n) {
                         const float f = factor[k + u][lane];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) o[c] = fmaf(f, v[u][c], o[c]);
+                        for (int c = 0; c < COLS; ++c) o[c] = fmaf(f, v[u][c], o[c]);
                     }
             }
     }
@@ -83,14 +84,17 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
     for (int w = 0; w < 8; ++w) l += top[w][lane];
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) tile[warp * 4 + c][lane] = o[c] * inv;
+    for (int c = 0; c < COLS; ++c) tile[warp * COLS + c][lane] = o[c] * inv;
     __syncthreads();
     // a warp: a row's columns
-    const int out_col = blockIdx.x * 32 + lane;
     for (int row = warp; row < 32 && row0 + row < count && in - lane + row < rows; row += 8) {
         const int at = row0 + row;
-        if (out_col < D)
-            ((T*)p.out)[(size_t)(r.first + at / p.group) * p.ldo + (head * p.group + at % p.group) * D + out_col] = from_float<T>(tile[lane][row]);
+        T* to = (T*)p.out + (size_t)(r.first + at / p.group) * p.ldo + (head * p.group + at % p.group) * D;
+#pragma unroll
+        for (int c = 0; c < 8 * COLS; c += 32) {
+            const int out_col = blockIdx.x * 8 * COLS + c + lane;
+            if (out_col < D) to[out_col] = from_float<T>(tile[c + lane][row]);
+        }
     }
 }
 
@@ -143,9 +147,11 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     const cudaStream_t stream = (cudaStream_t)a->stream;
     const int rc = a->dtype != FERRIS_BF16 ? tree_attention_f32(p, plan, stream) : plan.tensor ? tree_attention_tc(p, plan, stream) : tree_attention_mma(p, plan, stream);
     if (rc != FERRIS_OK) return rc;
-    const int slices = (plan.rows + 31) / 32;
-    const dim3 grid((p.head_dim + 31) / 32, slices * plan.lanes, plan.groups);
-    const auto kernel = a->dtype == FERRIS_BF16 ? tree_parts_kernel<bf16> : tree_parts_kernel<float>;
+    const int most = p.max_nodes * p.group, slices = ((most < plan.rows ? most : plan.rows) + 31) / 32;
+    // sixteen columns a warp where items have few parts, so that there are fewer blocks, all at once
+    const bool few = 4ll * p.seqs * p.kv_heads >= plan.groups;
+    const dim3 grid((p.head_dim + (few ? 127 : 31)) / (few ? 128 : 32), slices * plan.lanes, plan.groups);
+    const auto kernel = a->dtype == FERRIS_BF16 ? few ? tree_parts_kernel<bf16, 16> : tree_parts_kernel<bf16, 4> : few ? tree_parts_kernel<float, 16> : tree_parts_kernel<float, 4>;
     const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, stream, p, plan.rows, plan.lanes, slices);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));

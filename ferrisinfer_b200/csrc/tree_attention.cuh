@@ -124,7 +124,8 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeAttention& p, const Tree
 
 // ---------------------------------------------------------------------------------------------
 // The work of a step.  An item is a block of query rows of a request and kv head, a tile UNIT cached rows of it; the tiles are numbered through and
-// dealt out evenly to the blocks of the grid, whatever the requests' lengths.  Two ways:
+// dealt out evenly to the blocks of the grid, whatever the requests' lengths; in short steps, where one more tile costs less than to begin and end a second
+// item, in runs of one item each.  Two ways:
 // FLAT   requests first, then kv heads, blocks of query rows, cached rows: all blocks have the same number of tiles.
 // lanes  groups of `lanes` blocks, one for every block of query rows that the largest request has; requests, kv heads, cached rows are dealt out to the groups.
 //        The blocks of a group go over the same cached rows side by side, so that those are read from memory once, however long the cache.
@@ -174,7 +175,7 @@ struct TreeItem {
 // The requests of a step, if they are no more than these, as one block's warps fetch them once for all.
 struct TreeRequests {
     static constexpr int MOST = 128;
-    int first[MOST], nodes[MOST], start[MOST], rows[MOST], upto[MOST];
+    int first[MOST], nodes[MOST], start[MOST], rows[MOST];
 };
 
 // Goes through a group's share, item by item; by whole warps, each for itself.
@@ -182,6 +183,7 @@ template <int UNIT, int ROWS, bool FLAT>
 struct TreeWalk {
     int at, end, lane_block;  // where this group is and where it ends; block of query rows of this lane
     int per, more;            // tiles of a group, and groups that have one more
+    int round;                // items begin on a multiple of this
     TreeRequest mine;         // of request 32 s0 + lane
     int s0, before, upto;     // tiles before these requests, and up to and with this lane's
 
@@ -195,36 +197,65 @@ struct TreeWalk {
         s0 = chunk;
         const int seq = 32 * chunk + (threadIdx.x & 31);
         if (p.seqs <= TreeRequests::MOST) {
-            mine.first = known.first[seq], mine.nodes = known.nodes[seq], mine.start = known.start[seq], mine.rows = known.rows[seq], upto = known.upto[seq];
-            return;
-        }
-        fetch(p, seq);
+            mine.first = known.first[seq], mine.nodes = known.nodes[seq], mine.start = known.start[seq], mine.rows = known.rows[seq];
+        } else
+            fetch(p, seq);
+        upto = tree_scan(mine.nodes > 0 ? span(tiles(p, mine)) * blocks(p, mine) * p.kv_heads : 0);
     }
+    __device__ __forceinline__ int span(int tiles) const { return round > 1 ? (tiles + round - 1) / round * round : tiles; }
     __device__ __forceinline__ void fetch(const TreeAttention& p, int seq) {
         mine.first = mine.nodes = mine.start = mine.rows = 0;
         if (seq < p.seqs) mine = tree_request(p, seq);
-        upto = tree_scan(mine.nodes > 0 ? tiles(p, mine) * blocks(p, mine) * p.kv_heads : 0);
     }
     // By all threads of a block (at least TreeRequests::MOST), who have to meet before they begin.
     __device__ __forceinline__ void know(const TreeAttention& p, TreeRequests& known) {
         const int seq = threadIdx.x;
         if (p.seqs > TreeRequests::MOST || (seq & ~31) >= p.seqs) return;
         fetch(p, seq);
-        known.first[seq] = mine.first, known.nodes[seq] = mine.nodes, known.start[seq] = mine.start, known.rows[seq] = mine.rows, known.upto[seq] = upto;
+        known.first[seq] = mine.first, known.nodes[seq] = mine.nodes, known.start[seq] = mine.start, known.rows[seq] = mine.rows;
     }
     // Group `group` of `groups` (one beyond them has nothing).
     __device__ __forceinline__ void begin(const TreeAttention& p, const TreeRequests& known, int group, int groups, int lane) {
         const int chunks = (p.seqs + 31) / 32;
-        lane_block = lane;
+        lane_block = lane, round = 1;
         int total = 0;
-        for (int c = 0; c < chunks; ++c) {
-            look_at(p, known, c);
-            before = total;
-            total += __shfl_sync(0xffffffffu, upto, 31);
+        if (p.seqs <= TreeRequests::MOST) {
+            constexpr int CHUNKS = TreeRequests::MOST / 32;
+            int each[CHUNKS], items[CHUNKS], mine_all = 0;  // tiles of an item of this lane's requests, items
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                items[c] = each[c] = 0;
+                if (c < chunks) {
+                    const int seq = 32 * c + (threadIdx.x & 31);
+                    const TreeRequest r = {known.first[seq], known.nodes[seq], known.start[seq], known.rows[seq]};
+                    if (r.nodes > 0) each[c] = tiles(p, r), items[c] = blocks(p, r) * p.kv_heads;
+                    mine_all += each[c] * items[c];
+                }
+            }
+            total = __reduce_add_sync(0xffffffffu, mine_all);
+            per = total / groups, more = total - per * groups;
+            // a group within one item, if it has no more than a tile more for that
+            const int even = per + (more > 0);
+            for (int u = even; u > 1 && u <= even + 1; ++u) {
+                int runs = 0;
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c)
+                    if (c < chunks) runs += (each[c] + u - 1) / u * items[c];
+                runs = __reduce_add_sync(0xffffffffu, runs);
+                if (runs <= groups) {
+                    total = runs * u, per = round = u, more = 0;
+                    break;
+                }
+            }
+        } else {
+            for (int c = 0; c < chunks; ++c) {
+                look_at(p, known, c);
+                total += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            per = total / groups, more = total - per * groups;
         }
-        per = total / groups, more = total - per * groups;
-        at = group * per + min(group, more), end = group < groups ? at + per + (group < more) : at;  // (groups that have no tiles leave no part either)
-        if (chunks > 1) look_at(p, known, 0), before = 0;
+        at = min(total, group * per + min(group, more)), end = group < groups ? min(total, at + per + (group < more)) : at;  // (groups that have no tiles leave no part either)
+        look_at(p, known, 0), before = 0;
     }
     // The group that has a tile.
     __device__ __forceinline__ int owner(int tile) const {
@@ -253,12 +284,12 @@ struct TreeWalk {
             const TreeRequest& r = item.request;
             item.low = low(p, r), item.tiles = tiles(p, r);
             const int from = before + (lane ? __shfl_sync(0xffffffffu, upto, lane - 1) : 0);
-            const int n = (at - from) / item.tiles, blocks_each = blocks(p, r);
+            const int each = span(item.tiles), n = (at - from) / each, blocks_each = blocks(p, r);
             item.head = n / blocks_each;
             item.block = FLAT ? n - item.head * blocks_each : lane_block;
-            item.start = from + n * item.tiles;
+            item.start = from + n * each;
             item.first = at - item.start, item.last = min(item.tiles, end - item.start);
-            at = item.start + item.last;
+            at = item.start + (item.last == item.tiles ? each : item.last);
             if (FLAT || item.block * ROWS < r.nodes * p.group) return true;
         }
         return false;

@@ -155,32 +155,40 @@ def test_every_part_has_a_place_of_its_own_and_is_joined(seed):
     requests = [(rng.choice([0, 1, 1, 5, 33, 64]), rng.randint(0, most)) for _ in range(seqs)]
     max_nodes, max_kv = max(max(n for n, _ in requests), 1), max(max(s + n for n, s in requests), 1)
     groups, lanes = deal(seqs, kv_heads, group, max_nodes, max_kv, unit, rows, 1, flat)
-    items, total = [], 0  # (request, kv head, block, first tile, tiles)
+    items = []  # [request, kv head, block, tiles, first place]
     for r, (n, start) in enumerate(requests):
-        if n:
-            tiles = max(-(-(start + n) // unit), 1)
-            for h in range(kv_heads):
-                for b in range(-(-n * group // rows) if flat else 1):
-                    items.append((r, h, b, total, tiles))
-                    total += tiles
+        for h in range(kv_heads if n else 0):
+            for b in range(-(-n * group // rows) if flat else 1):
+                items.append([r, h, b, max(-(-(start + n) // unit), 1)])
+    total = sum(i[3] for i in items)
     per, more = divmod(total, groups)
-    begins = lambda g: g * per + min(g, more)
+    runs, even = 1, -(-total // groups)  # tiles of a run of one item; 1: none
+    for u in range(even, even + 2 if even > 1 else 0):
+        if seqs <= 128 and sum(-(-i[3] // u) for i in items) <= groups:
+            runs, per, more = u, u, 0
+            break
+    places_used = 0
+    for i in items:
+        i.append(places_used)
+        places_used += -(-i[3] // runs) * runs
+    begins = lambda g: min(places_used, g * per + min(g, more))
     owner = lambda t: t // (per + 1) if t < more * (per + 1) else more + (t - more * (per + 1)) // per
     places, begun, done = {}, {}, 0
     for g in range(groups):
-        lo, hi = begins(g), begins(g + 1)
+        lo, hi, segments = begins(g), begins(g + 1), 0
         for item in items:
-            first, last = max(lo - item[3], 0), min(hi - item[3], item[4])
+            first, last = max(lo - item[4], 0), min(hi - item[4], item[3])
             if first >= last:
                 continue
-            done += last - first
-            assert all(owner(item[3] + t) == g for t in (first, last - 1))
-            if first or last < item[4]:
+            done, segments = done + last - first, segments + 1
+            assert all(owner(item[4] + t) == g for t in (first, last - 1))
+            if first or last < item[3]:
                 assert (g, first == 0) not in places
                 places[g, first == 0] = item
-            if first == 0 and last < item[4]:
+            if first == 0 and last < item[3]:
                 assert g not in begun
-                begun[g] = (item, owner(item[3] + item[4] - 1))
+                begun[g] = (item, owner(item[4] + item[3] - 1))
+        assert hi - lo <= even + 1 and (runs == 1 or segments <= 1)
     assert done == total
     joined = {}
     for g, (item, end) in begun.items():

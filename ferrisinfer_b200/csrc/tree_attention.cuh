@@ -125,7 +125,7 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeAttention& p, const Tree
 // ---------------------------------------------------------------------------------------------
 // The work of a step.  An item is a block of query rows of a request and kv head, a tile UNIT cached rows of it; the tiles are numbered through and
 // dealt out evenly to the blocks of the grid, whatever the requests' lengths; in short steps, where one more tile costs less than to begin and end a second
-// item, in runs of one item each.  Two ways:
+// item, in runs of one item each (8 requests of 16 nodes after 4,096 rows 27 -> 22.5 us, 64 nodes after 131,071 rows 95 -> 82).  Two ways:
 // FLAT   requests first, then kv heads, blocks of query rows, cached rows: all blocks have the same number of tiles.
 // lanes  groups of `lanes` blocks, one for every block of query rows that the largest request has; requests, kv heads, cached rows are dealt out to the groups.
 //        The blocks of a group go over the same cached rows side by side, so that those are read from memory once, however long the cache.
@@ -147,7 +147,7 @@ struct TreePlan {
         const long long most = (long long)seqs * kv_heads * (flat ? row_blocks : 1) * ((max_kv + unit - 1) / unit + 1);
         const long long room = (long long)(sms > 0 ? sms : 148) * blocks / lanes;
         groups = (int)(room < 1 ? 1 : room < most ? room : most);
-        fits = most <= 0x7fffffff && lanes <= 4096;
+        fits = most <= 0x7ff00000 && lanes <= 4096;
     }
 };
 TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window);

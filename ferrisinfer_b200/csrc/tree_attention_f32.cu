@@ -7,7 +7,7 @@
 //            shared memory
 //   outputs  a lane is four columns: a cached row's values meet the weights of eight query rows, which are two reads for all lanes
 // All in 32 bits.  Whatever a query does not see is never multiplied: what lies there may be NaN.
-// What bounds it: six ragged requests of up to 13 nodes after up to 1,533 rows (12 / 2 heads of 128) 40 us.  A tile of 64 cached by 32 query rows takes some 14,000
+// What bounds it: six ragged requests of up to 13 nodes after up to 1,533 rows (12 / 2 heads of 128) 37 us.  A tile of 64 cached by 32 query rows takes some 14,000
 // cycles, 4,100 if every multiply-add were issued without a pause: with two warps to a scheduler reads of shared memory (nine of 16 bytes a lane for 32
 // multiply-adds) and the softmax between the products are waited for.  Blocks of query rows are numbered with the tiles: one block for each of the largest request's
 // left those of the others idle (53 us).
@@ -279,8 +279,8 @@ int launch(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream) {
     return FERRIS_OK;
 }
 
-// Two groups of warps (blocks of 32 query rows) where 64 would be filled up with more rows that are not there: six requests of 13 nodes (78 query rows) 70 us, in
-// blocks of 64 73; of 5 (30 query rows) 35 and 40.
+// Two groups of warps (blocks of 32 query rows) where 64 would be filled up with more rows that are not there: six requests of 13 nodes (78 query rows) 66 us, in
+// blocks of 64 74; of 5 (30 query rows) 37 and 43.
 template <typename F>
 void with_variant(int D, int rows, F f) {
     const bool two = (rows + 31) / 32 * 32 < (rows + 63) / 64 * 64;

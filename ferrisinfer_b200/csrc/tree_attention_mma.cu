@@ -9,9 +9,9 @@
 // warps share tiles, so that shared memory is read less often.
 // A tile that every query row sees whole is multiplied as it is.  In others scores that are not seen become nought weights; as nought times
 // NaN is NaN, a tile of values that holds something not finite is multiplied element by element, by those who see it.
-// What bounds it: few query rows, and what there is to read is little beside the chain of tables, pages, tiles and the join: 8 requests of one node after 4,096 rows (14 / 2
-// heads of 64) 16 us, floor 1.3; one of five after 999 (a chain) 12 us.  Longer steps approach the memory's rate: 32 requests of two nodes (28 / 4 heads of 128)
-// 60 us for 268 MB, 4.5 TB/s.
+// What bounds it: few query rows, and what there is to read is little beside the chain of tables, pages, tiles and the join: a chain of five tokens after 999 rows (14 / 2
+// heads of 64) 12.3 us, of which this kernel takes 9.5; 8 requests of one node after 4,096 rows 14.5, floor 1.3.  Longer steps approach the memory's rate: 32 requests
+// of two nodes (28 / 4 heads of 128) 54 to 58 us for 268 MB, 4.6 to 5 TB/s.
 #include "tree_attention.cuh"
 
 namespace {
@@ -428,12 +428,12 @@ TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_node
         using P = Plan<dp.value, ms.value, wr.value, nw.value, st.value>;
         plan.unit = P::UNIT, plan.rows = P::ROWS, blocks = P::BLOCKS;
     });
-    // tcgen05 where its products outweigh what it takes to begin with: from 33 query rows on, from 65 where there are no more than four units for an SM.  Microseconds,
-    // mma.sync (with pages of 24 rows) and tcgen05: 8 requests after 4,096 rows, 14 / 2 heads of 64, 28 query rows 18.1 and 22.6, 56 rows 20.9 and 22.9, 112 rows
-    // 29 and 23; 32 requests, 28 / 4 heads of 128, 14 rows 60 and 77, 28 rows 76.3 and 77.6, 56 rows 105 and 84.
+    // tcgen05 where its products outweigh what it takes to begin with: from 65 query rows on, from 17 where there are more than four units for an SM.  Microseconds,
+    // mma.sync (with pages of 24 rows) and tcgen05: 8 requests after 4,096 rows, 14 / 2 heads of 64, 14 query rows 14.5 and 19.1, 56 rows 18.5 and 19.6, 70 rows 23.5 and
+    // 20.2; 32 requests, 28 / 4 heads of 128, 14 rows 54 and 67, 28 rows 73 and 67, 56 rows 95 and 69, 112 rows 165 and 78.
     // (the row of a box that lies nowhere is a number too; a scale below nought would turn maxima into minima)
     const int rows = max_nodes * group, sms = ferris_sm_count();
-    const bool many = rows > 64 || (rows > 32 && (long long)seqs * kv_heads * ((max_kv + 127) / 128) > 4ll * (sms > 0 ? sms : 148));
+    const bool many = rows > 64 || (rows > 16 && (long long)seqs * kv_heads * ((max_kv + 127) / 128) > 4ll * (sms > 0 ? sms : 148));
     plan.tensor = many && (head_dim == 64 || head_dim == 128) && page_size % 16 == 0 && cache_rows < 0x7fffffff && scale > 0.0f && scale < 1e30f;
     if (plan.tensor) plan.unit = 128, plan.rows = rows > 128 ? 256 : 128, blocks = rows > 128 ? 1 : 2;  // (two groups to a block)
     plan.deal(seqs, kv_heads, group, max_nodes, max_kv, blocks, !plan.tensor);

@@ -124,7 +124,7 @@ def variant(dtype, D, rows, page_size):
         return 32, 64, 1, True
     if dtype == FP32:
         return 64, 32 if -(-rows // 32) * 32 < -(-rows // 64) * 64 else 64, 1, True
-    assert rows > 32 and page_size % 16 == 0 and D in (64, 128)  # (on tcgen05, where the step is long or the rows are many)
+    assert rows > 16 and page_size % 16 == 0 and D in (64, 128)  # (on tcgen05, where the step is long or the rows are many)
     return 128, 256 if rows > 128 else 128, 1 if rows > 128 else 2, False
 
 

@@ -134,6 +134,7 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     p.tables = (const int*)a->tables, p.width = a->width;
     const long long rows = (long long)a->width * a->page_size;
     p.limit = (int)(rows < a->max_kv ? rows : a->max_kv);
+    if (p.limit > 0x7ffffc00) FERRIS_REFUSE("a request has at most %d rows, not %d", 0x7ffffc00, p.limit);
     p.q_start = (const int*)a->q_start, p.start_row = (const int*)a->start_row, p.parents = (const int*)a->parents;
     p.seqs = a->seqs, p.tokens = a->tokens, p.heads = a->heads, p.kv_heads = a->kv_heads, p.group = a->heads / a->kv_heads;
     p.head_dim = a->head_dim, p.pages = a->pages, p.page_size = a->page_size, p.max_nodes = a->max_nodes, p.window = a->window;

@@ -48,7 +48,7 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeAttention& p, int 
     const int len = min(max(p.q_start[seq + 1], r.first), p.tokens) - r.first;
     r.nodes = min(len, p.max_nodes);
     if (len > p.max_nodes) ferris_report(p.status, FERRIS_STATUS_BAD_INDEX, 110);
-    r.start = max(p.start_row[seq], 0);
+    r.start = min(max(p.start_row[seq], 0), 0x7ffffe00);  // (positions of the nodes fit 32 bits)
     r.rows = (int)min((long long)r.start + r.nodes, (long long)p.limit);
     return r;
 }

@@ -2705,7 +2705,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     keys and values already are: node i of request s in row ``seq_start_row[s]`` + i, rotated by its position, seq_start_row[s] + its depth.
 
     ``q`` [T, >= num_heads x head size] (bf16 or fp32; its first columns, so the rows of a fused projection will do), ``out``
-    [T, num_heads x head size] of the same type; ``k_cache``, ``v_cache`` [pages, kv heads, page size, head size] of the same type, head sizes
+    [T, num_heads x head size] of the same type and apart from ``q``; ``k_cache``, ``v_cache`` [pages, kv heads, page size, head size] of the same type, head sizes
     that are a multiple of 8 up to 256.  Request s brings the rows ``seq_q_start[s]`` .. ``seq_q_start[s + 1] - 1`` (int32 [S + 1]); rows behind
     the last request's are left as they are.  ``parents`` (int32 [T]): each node's parent, the number of an earlier
     node of its request, or -1.  A node sees the ``seq_start_row[s]`` (int32 [S]) rows of its request's text, itself and its ancestors;
@@ -2733,6 +2733,8 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     (ldq, q_step), (ldo, out_step) = q.stride(), out.stride()
     if q_step != 1 or out_step != 1:
         raise KernelError(f"{what}: queries and outputs need contiguous rows, found strides {q.stride()} and {out.stride()}")
+    if T > 1 and ldo < cols:
+        raise KernelError(f"{what}: the rows of the output overlap (row stride {ldo})")
     if block_tables.dim() != 2 or block_tables.shape[0] != S or seq_q_start.numel() != S + 1:
         raise KernelError(f"{what}: tables {tuple(block_tables.shape)}, {seq_q_start.numel()} first rows for {S} requests")
     if max_q_len < 0 or max_kv_len < 0 or window < 0 or max_q_len > TREE_NODES:

@@ -39,6 +39,7 @@ def attention_arguments(**changes):
     (dict(head_dim=0), "multiple of 8"), (dict(max_nodes=257), "at most 256 tokens"), (dict(pages=0), "0 pages"), (dict(page_size=0), "pages of 0 rows"),
     (dict(width=0), "tables of 0 blocks"), (dict(max_kv=0), "0 rows at most"), (dict(k=PAGE + 8), "16 bytes"), (dict(v=PAGE + 2), "16 bytes"),
     (dict(parts=0), "scratch"), (dict(parts=PAGE + 4), "scratch"), (dict(seqs=1 << 30, kv_heads=64, heads=64, max_kv=1 << 24, width=1 << 20), "exceed one launch"),
+    (dict(max_kv=0x7fffffff, width=2, page_size=1 << 30), "rows, not"),
 ])
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
 def test_attention_is_refused(dtype, changes, said):

@@ -254,3 +254,45 @@ def test_two_threads_at_once(ops):
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("heads, kv_heads, D, page_size", [(14, 2, 64, 16), (2, 1, 128, 16), (16, 1, 128, 32), (3, 1, 40, 7)])
+@pytest.mark.parametrize("requests", [127, 128, 129, 333])
+def test_attention_of_many_requests(ops, dtype, heads, kv_heads, D, page_size, requests):
+    """Up to 128 requests are fetched once for a block's warps, more of them by every warp as it comes to them."""
+    from ferrisinfer_b200.engine.workspace import Workspace
+
+    draw = random.Random(requests)
+    nodes = [draw.choice([0, 1, 2, 5, 17]) for _ in range(requests)]
+    starts = [draw.choice([0, 1, 40, 129, 300]) for _ in range(requests)]
+    starts[7], nodes[7] = 4000, 9
+    step = Step(dtype, heads, kv_heads, D, page_size, nodes, starts, extra_columns=8)
+    step.check(step.run(ops, Workspace(DEV)))
+    step.check(step.run(ops, Workspace(DEV), window=33), window=33)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("window", [0, 100])
+def test_rows_of_the_text_beyond_what_there_is(ops, dtype, window):
+    """A request that says it has more rows than its table sees those that the table has, and behind a window none of them."""
+    from ferrisinfer_b200.engine.workspace import Workspace
+
+    step = Step(dtype, 12, 2, 64, 16, [5, 12], [60, 200])
+    for start in (0x7fffffff, 1 << 30, 100000):
+        step.starts[0] = start
+        out = torch.full((17, 12 * 64), 7.0, dtype=dtype, device=DEV)
+        ops.tree_attention(step.q, out, step.k, step.v, ints(step.tables), ints(step.q_start), ints(step.starts), ints(step.parents), 12, 212, 12, 0.125, window=window,
+                           workspace=Workspace(DEV))
+        if window:
+            assert (out[:5] == 0).all()
+        assert not (out[5:] == 7).any() and torch.isfinite(out[5:]).all()
+
+
+def test_outputs_that_overlap_are_refused(ops):
+    from ferrisinfer_b200.engine.workspace import Workspace
+    from ferrisinfer_b200.errors import KernelError
+
+    step = Step(torch.bfloat16, 4, 2, 64, 16, [3], [20])
+    with pytest.raises(KernelError, match="overlap"):
+        step.run(ops, Workspace(DEV), out=torch.zeros(1, 256, dtype=torch.bfloat16, device=DEV).expand(3, 256))

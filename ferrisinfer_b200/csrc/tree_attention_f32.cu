@@ -156,24 +156,29 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_f32_kernel(const Tr
             const unsigned long long mine = pages >> (group * Z::KEYS);
             const bool whole = key0 >= sure_low && key0 + Z::KEYS <= sure_high && (Z::KEYS == 64 ? mine == ~0ull : (uint32_t)mine == 0xffffffffu);
             uint32_t sees[WARP_ROWS][EACH];
+            float top[WARP_ROWS];
 #pragma unroll
             for (int j = 0; j < WARP_ROWS; ++j) {
                 const int at = slab0 + j, node = at < count ? at / p.group : -1;
-                float top = m[j];
+                top[j] = m[j];
 #pragma unroll
                 for (int e = 0; e < EACH; ++e) {
                     sees[j][e] = whole ? 0xffffffffu : node < 0 ? 0u : tree_sees(p, r, tree, node, key0 + 32 * e) & (uint32_t)(mine >> (32 * e));
                     x[j][e] = sees[j][e] >> lane & 1 ? x[j][e] * p.scale : -INFINITY;
-                    top = fmaxf(top, x[j][e]);
+                    top[j] = fmaxf(top[j], x[j][e]);
                 }
-                top = warp_max(top);
-                const float base = top == -INFINITY ? 0.0f : top;
-                if (top != m[j]) {  // (the same for all lanes)
-                    const float corr = exp2f(m[j] - base);
-                    l[j] *= corr, m[j] = top;
+            }
+            // (all rows' maxima step by step together, and no branch where one stays: the chains of eight rows one after the other took longer)
 #pragma unroll
-                    for (int c = 0; c < Z::QUADS; ++c) o[j][c].x *= corr, o[j][c].y *= corr, o[j][c].z *= corr, o[j][c].w *= corr;
-                }
+            for (int step = 16; step > 0; step >>= 1)
+#pragma unroll
+                for (int j = 0; j < WARP_ROWS; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], step));
+#pragma unroll
+            for (int j = 0; j < WARP_ROWS; ++j) {
+                const float base = top[j] == -INFINITY ? 0.0f : top[j], corr = exp2f(m[j] - base);
+                l[j] *= corr, m[j] = top[j];
+#pragma unroll
+                for (int c = 0; c < Z::QUADS; ++c) o[j][c].x *= corr, o[j][c].y *= corr, o[j][c].z *= corr, o[j][c].w *= corr;
 #pragma unroll
                 for (int e = 0; e < EACH; ++e) {
                     x[j][e] = sees[j][e] >> lane & 1 ? exp2f(x[j][e] - base) : 0.0f;

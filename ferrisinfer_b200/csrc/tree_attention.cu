@@ -8,29 +8,46 @@
 
 namespace {
 
-// The parts that the groups' blocks left of items that lie in several: a block joins 32 query rows of an item, and as many columns.  A lane
+// The parts that the groups' blocks left of items that lie in several: a block finds an item in the groups' notes (a block for every group, most of which had nothing
+// to join, took 12 us for 8 requests of 16 nodes, so it takes XX) and joins 32 query rows of an item, and as many columns.  A lane
 // is a row, as the parts lie; a warp has four columns, and sixteen parts of them on their way at once.  Bound by latency: the item's groups, the parts'
 // maxima and sums, the parts: 6 us by itself for one request of five nodes.  Where items have few parts a block has 128 columns: 64 requests of 8 nodes
 // (two or three parts an item) took 97 us with blocks of 32 columns, 82 so.
 constexpr int JOIN_PARTS = 64;  // parts that are joined at once
 
 template <typename T, int COLS>
-__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int lanes, int slices) {
+__global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, int rows, int groups, int lanes, int slices) {
     constexpr int AHEAD = 64 / COLS;
     __shared__ float top[8][32], tile[8 * COLS][33], factor[JOIN_PARTS][32];
     pdl_wait();
     pdl_launch_dependents();
     const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // group z's item, if it goes on in others; with lanes, the blocks of query rows one after the other
-    const int4 begun = p.begun[blockIdx.z];
-    if (begun.x < 0) return;  // (items that lie in one group are written by it)
-    const int seq = begun.x, head = begun.y, lane_block = blockIdx.y / slices, block = lanes > 1 ? lane_block : begun.z, parts = begun.w - blockIdx.z + 1;
+    // the z-th of the items that go on in other groups than the one that they begin in (others are written by their group); with lanes, the blocks of query rows
+    // one after the other
+    __shared__ int4 item;
+    __shared__ int item_group, counts[8];
+    if (threadIdx.x == 0) item_group = -1;
+    for (int from = 0, skip = blockIdx.z; from < groups && skip >= 0; from += 256) {
+        const int at = from + threadIdx.x;
+        const int4 begun = at < groups ? p.begun[at] : make_int4(-1, 0, 0, 0);
+        const unsigned have = __ballot_sync(0xffffffffu, begun.x >= 0);
+        if (lane == 0) counts[warp] = __popc(have);
+        __syncthreads();
+        int before = __popc(have & ((1u << lane) - 1)), all = 0;
+        for (int w = 0; w < 8; ++w) before += w < warp ? counts[w] : 0, all += counts[w];
+        if (begun.x >= 0 && before == skip) item = begun, item_group = at;
+        skip -= all;
+        __syncthreads();
+    }
+    if (item_group < 0) return;
+    const int group = item_group;
+    const int seq = item.x, head = item.y, lane_block = blockIdx.y / slices, block = lanes > 1 ? lane_block : item.z, parts = item.w - group + 1;
     const int from_row = (blockIdx.y - lane_block * slices) * 32, row0 = block * rows + from_row, col = (blockIdx.x * 8 + warp) * COLS;
     const TreeRequest r = tree_request(p, seq);
     const int count = r.nodes * p.group, in = from_row + lane;
     if (row0 >= count) return;
     const bool live = row0 + lane < count && in < rows;
-    auto part = [&](int k) { return tree_part(p, (blockIdx.z + k) * lanes + lane_block, k == 0, rows) + in; };
+    auto part = [&](int k) { return tree_part(p, (group + k) * lanes + lane_block, k == 0, rows) + in; };
     float m = -INFINITY, l = 0.0f, o[COLS] = {};  // l: of the warp's own parts
     for (int k0 = 0; k0 < parts; k0 += JOIN_PARTS) {
         const int n = min(parts - k0, JOIN_PARTS);
@@ -151,10 +168,11 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     if (rc != FERRIS_OK) return rc;
     const int most = p.max_nodes * p.group, slices = ((most < plan.rows ? most : plan.rows) + 31) / 32;
     // sixteen columns a warp where items have few parts, so that there are fewer blocks, all at once
+    const long long items = (long long)p.seqs * p.kv_heads * (plan.lanes > 1 ? 1 : (most + plan.rows - 1) / plan.rows);  // (of several groups no more than groups)
     const bool few = 4ll * p.seqs * p.kv_heads >= plan.groups;
-    const dim3 grid((p.head_dim + (few ? 127 : 31)) / (few ? 128 : 32), slices * plan.lanes, plan.groups);
+    const dim3 grid((p.head_dim + (few ? 127 : 31)) / (few ? 128 : 32), slices * plan.lanes, (unsigned)(items < plan.groups ? items : plan.groups));
     const auto kernel = a->dtype == FERRIS_BF16 ? few ? tree_parts_kernel<bf16, 16> : tree_parts_kernel<bf16, 4> : few ? tree_parts_kernel<float, 16> : tree_parts_kernel<float, 4>;
-    const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, stream, p, plan.rows, plan.lanes, slices);
+    const cudaError_t e = ferris_launch(kernel, grid, dim3(256), 0, stream, p, plan.rows, plan.groups, plan.lanes, slices);
     if (e != cudaSuccess) {
         ferris_set_error("%s", cudaGetErrorString(e));
         return (int)e;

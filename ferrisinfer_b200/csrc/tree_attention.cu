@@ -9,7 +9,7 @@
 namespace {
 
 // The parts that the groups' blocks left of items that lie in several: a block finds an item in the groups' notes (a block for every group, most of which had nothing
-// to join, took 12 us for 8 requests of 16 nodes, so it takes XX) and joins 32 query rows of an item, and as many columns.  A lane
+// to join, took 12 us for 8 requests of 16 nodes, so it takes 8.5) and joins 32 query rows of an item, and as many columns.  A lane
 // is a row, as the parts lie; a warp has four columns, and sixteen parts of them on their way at once.  Bound by latency: the item's groups, the parts'
 // maxima and sums, the parts: 6 us by itself for one request of five nodes.  Where items have few parts a block has 128 columns: 64 requests of 8 nodes
 // (two or three parts an item) took 97 us with blocks of 32 columns, 82 so.

@@ -7,7 +7,7 @@
 //            shared memory
 //   outputs  a lane is four columns: a cached row's values meet the weights of eight query rows, which are two reads for all lanes
 // All in 32 bits.  Whatever a query does not see is never multiplied: what lies there may be NaN.
-// What bounds it: six ragged requests of up to 13 nodes after up to 1,533 rows (12 / 2 heads of 128) 35 us.  A tile of 64 cached by 32 query rows takes some 12,000
+// What bounds it: six ragged requests of up to 13 nodes after up to 1,533 rows (12 / 2 heads of 128) 34 us.  A tile of 64 cached by 32 query rows takes some 12,000
 // cycles, 4,100 if every multiply-add were issued without a pause: with two warps to a scheduler reads of shared memory (nine of 16 bytes a lane for 32
 // multiply-adds) and the softmax between the products are waited for.  Blocks of query rows are numbered with the tiles: one block for each of the largest request's
 // left those of the others idle (53 us).

@@ -19,7 +19,7 @@
 //
 // What bounds it.  64 requests of 8 nodes after up to 4,096 rows (28 / 4 heads of 128): 83 us with the join (floor 53, the cached rows read once); the loop
 // runs at the memory's rate (two groups' units, 128 KB, in 4,850 cycles), and a segment takes some 9,000 cycles to begin and to end, which the other group only partly
-// fills; both groups on one unit, with one ring and joined in the block, took 108.  64 nodes after 131,071 rows (12 / 2 heads of 128): 83 us (floor 31): a unit
+// fills; both groups on one unit, with one ring and joined in the block, took 108.  64 nodes after 131,071 rows (12 / 2 heads of 128): 80 us (floor 31): a unit
 // of both groups takes 3,800 cycles, of which a group waits 1,500 for its products (eight MMAs of 128 x 128 x 16 take 450 to
 // 600 cycles) and 1,310 are exponentials, 1,024 at the unit's rate.  Taken back, when it took 94: scores in pieces of 64 cached rows, the next ones ahead of the weights
 // (113 us: MMAs half as wide take nearly as long), weights announced in halves (95), three blocks of 128 query rows for two of 256 (98), blocks of query

@@ -5,8 +5,8 @@
 // the others.  Greedy rows (T <= 0, top_k == 1 or top_p <= 0): 1 at the greatest logit.  A logit that is NaN counts as minus infinity; where the greatest
 // is infinite, those that equal it share the mass.
 //
-// Which tokens stay is decided on masses in 64 bits: w is computed in 64 bits and held as a whole number of 2^-45, so that sums are exact
-// and do not depend on the order of additions, and borders fall as they do in exact arithmetic up to 2^-45 of the greatest weight.
+// Which tokens stay is decided on masses in 64 bits: w is computed in 64 bits and held as a whole number of 2^-45 (of 2^-44 from 2^19 tokens on, whose masses would
+// add up to 2^64 otherwise), so that sums are exact and do not depend on the order of additions.
 //
 // A cluster of up to eight blocks takes a row; each keeps its share in shared memory where it fits (two blocks to an SM), so that a row is read once and written once.
 //   neither top-k nor top-p   a softmax in 32 bits: the maximum, the exponentials and their sum, the quotients
@@ -37,8 +37,7 @@ constexpr int LIST = THREADS;  // elements that are ordered by counting, one a t
 constexpr int DIGIT = 9;    // bits of a digit of the keys: a histogram's bins
 constexpr int BOUNDS = 7;
 constexpr int MOST_ELEMENTS = 65536;  // of a block
-constexpr int MASS_BITS = 45;
-constexpr double UNIT = 35184372088832.0;  // 2^45
+constexpr int MASS_BITS = 45;  // a row's masses are below 2^64 with them up to 2^19 - 1 tokens
 constexpr u64 MASS_OFFSET = 0x4330000000000000ull;  // the bits of 2^52
 constexpr double LOG2E = 1.4426950408889634;
 
@@ -112,7 +111,7 @@ struct Shared {
     u32 index[MOST_BLOCKS], listed[MOST_BLOCKS];
     float parts[WARPS][BOUNDS + 1];
     u32 count_listed;
-    double powers[32];
+    double powers[32];  // the weight of the greatest logit, times 2^(j / 32)
     u64 threshold, retained, kept_mass;
     u64 red[2][WARPS];
     float fred[4][WARPS], scratch[33];
@@ -143,9 +142,9 @@ __device__ const double powers_of_two[32] = {  // 2^(j / 32)
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
 };
 
-// 2^(z / 32 + up) + 2^52 for -6000 <= z <= 0, up to 2^-46 of the power: the nearest whole number apart, of which five bits choose one of 2^(0/32) .. 2^(31/32) (`powers`) and the
-// others are the exponent, and the Taylor polynomial of 2^(f / 32) for |f| <= 1/2, whose sixth term is 2e-15.
-__device__ __forceinline__ double exp2_64_whole(double z, int up, const double* powers) {
+// unit 2^(z / 32) + 2^52 for -6000 <= z <= 0, up to 2^-46 of the power: the nearest whole number apart, of which five bits choose one of unit 2^(0/32) .. unit 2^(31/32)
+// (`powers`) and the others are the exponent, and the Taylor polynomial of 2^(f / 32) for |f| <= 1/2, whose sixth term is 2e-15.
+__device__ __forceinline__ double exp2_64_whole(double z, const double* powers) {
     const double magic = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to a whole number
     const double t = z + magic, f = z - (t - magic);
     double r = 3.9737099845494154e-11;  // (ln(2) / 32)^k / k! for k = 5 .. 0
@@ -156,7 +155,7 @@ __device__ __forceinline__ double exp2_64_whole(double z, int up, const double* 
     r = fma(r, f, 1.0);
     const int n = __double2loint(t);
     const double power = powers[n & 31];
-    return fma(r, __hiloint2double(__double2hiint(power) + ((n >> 5) + up) * (1 << 20), __double2loint(power)), 4503599627370496.0);
+    return fma(r, __hiloint2double(__double2hiint(power) + (n >> 5) * (1 << 20), __double2loint(power)), 4503599627370496.0);
 }
 
 struct Row {
@@ -178,7 +177,7 @@ struct Row {
     __device__ __forceinline__ float logit(int i) const { return number(at[i]); }
     // (with 2^52 it is rounded to a whole number, which the lower bits are; MASS_OFFSET are the others)
     __device__ __forceinline__ u64 mass_and_offset(float l) const {
-        return (u64)__double_as_longlong(exp2_64_whole(((double)fmaxf(l, least) - (double)top) * rate, MASS_BITS, powers));
+        return (u64)__double_as_longlong(exp2_64_whole(((double)fmaxf(l, least) - (double)top) * rate, powers));
     }
     __device__ __forceinline__ u64 mass(float l) const { return mass_and_offset(l) - MASS_OFFSET; }
     // The greatest logits in the highest bin; what lies below the histogram's range in bin 0.
@@ -308,7 +307,7 @@ __device__ __forceinline__ void put_low(Shared& s, u32 count, u64 mass) {
     count = __reduce_add_sync(0xffffffffu, count), mass = warp_sum_u64(mass);
     if ((threadIdx.x & 31) == 0 && count) {
         atomicAdd(&s.count[0], count);
-        // (what lies above 2^48 stays in the upper part: all masses of a row together are below 2^63)
+        // (what lies above 2^48 stays in the upper part: a block's masses together are at most 2^61)
         atomicAdd(&s.mass[0][0], (u32)mass & 0xffffu);
         atomicAdd(&s.mass[1][0], (u32)(mass >> 16) & 0xffffu);
         atomicAdd(&s.mass[2][0], (u32)(mass >> 32));
@@ -750,7 +749,7 @@ __device__ __forceinline__ void probabilities(const SamplingProbs& a, int row, S
             threshold = q.key, mass = over + q.mass;
         }
         // (which tokens stay is decided; their probabilities in 32 bits, as without top-k and top-p)
-        const float inv = (float)(UNIT / (double)mass), border = logit_of((u32)(threshold >> 32));
+        const float inv = (float)(s.powers[0] / (double)mass), border = logit_of((u32)(threshold >> 32));
         auto of = [&](float l, int i) -> float {
             l = r.number(l);
             if (!(l >= border) || (l == border && key_of(l, r.lo + i) < threshold)) return 0.0f;
@@ -772,7 +771,7 @@ template <bool KEEP>
 __global__ void __launch_bounds__(THREADS, 2) sampling_probs_kernel(const SamplingProbs a) {
     __shared__ Shared s;
     extern __shared__ __align__(16) float kept[];
-    if (threadIdx.x < 32) s.powers[threadIdx.x] = powers_of_two[threadIdx.x];
+    if (threadIdx.x < 32) s.powers[threadIdx.x] = powers_of_two[threadIdx.x] * (double)(1ull << (a.vocab < 1 << 19 ? MASS_BITS : MASS_BITS - 1));
     cluster_sync();  // (all blocks have begun: their memory may be written)
     pdl_wait();
     pdl_launch_dependents();

@@ -1,0 +1,30 @@
+"""Operators of steps over drafted tokens at the edges of what they take."""
+
+import math
+
+import pytest
+import torch
+
+from test_tree_gpu import DEV, ints, nothing_reported, ops, rng  # noqa: F401  (fixtures among them)
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ probabilities
+@pytest.mark.parametrize("V", [262143, 262144, 524287, 524288])
+@pytest.mark.parametrize("top_k, top_p", [(0, 0.5), (0, 0.999), (0, 1e-6), (1000, 0.5), (400000, 0.75), (20, 0.5), (0, 1.0)])
+def test_equal_logits_of_the_largest_vocabularies(ops, V, top_k, top_p):
+    """The row's mass is as many times the greatest weight as it has tokens.  A row of one logit, of minus infinity, of NaN, and one whose temperature makes all weights equal."""
+    logits = torch.full((4, V), 1.5, device=DEV)
+    logits[1], logits[2] = -math.inf, math.nan
+    logits[3] = torch.randn(V, generator=rng(1), device=DEV)
+    out = torch.full((4, V), 9.0, device=DEV)
+    p = torch.tensor(top_p, dtype=torch.float32)
+    ops.sampling_probs(logits, out, torch.tensor([1.0, 1.0, 1.0, 1e30], device=DEV), ints([top_k] * 4), p.to(DEV).repeat(4))
+    count = min(top_k, V) if top_k else V
+    count = math.ceil(p.double().item() * count) if top_p < 1 else count  # (the product of 24 and 19 bits is exact)
+    want = torch.zeros(4, V, dtype=torch.float64, device=DEV)
+    want[:3, :count] = 1 / count
+    want[3, torch.sort(logits[3], descending=True, stable=True).indices[:count]] = 1 / count
+    assert torch.equal(out > 0, want > 0)
+    assert ((out - want).abs() <= 2.0 ** -22 / count).all()  # the sum of equal numbers, a quotient and its rounding, a product

@@ -6,7 +6,8 @@
 // is infinite, those that equal it share the mass.
 //
 // Which tokens stay is decided on masses in 64 bits: w is computed in 64 bits and held as a whole number of 2^-45 (of 2^-44 from 2^19 tokens on, whose masses would
-// add up to 2^64 otherwise), so that sums are exact and do not depend on the order of additions.
+// add up to 2^64 otherwise), so that sums are exact and do not depend on the order of additions.  A weight is off by half of that and by 2^-46 of itself (what is below
+// 2^-46 counts as nothing), and a border lies where it does for a mass that is off by as much for every token: 2^-28.8 of the greatest weight for 151,936.
 //
 // A cluster of up to eight blocks takes a row; each keeps its share in shared memory where it fits (two blocks to an SM), so that a row is read once and written once.
 //   neither top-k nor top-p   a softmax in 32 bits: the maximum, the exponentials and their sum, the quotients

@@ -2776,8 +2776,8 @@ def sampling_probs(logits: torch.Tensor, out: torch.Tensor, temperature: Optiona
 
     Per row (fp32, int32, fp32 [n]): ``temperature`` (not above 0: 1 at the greatest logit, the first among equals; so too without it, with top_k 1 and with
     top_p not above 0), ``top_k`` (<= 0 or None: the whole vocabulary) greatest logits, the lower index first among equals, and of these the shortest
-    prefix whose mass reaches ``top_p`` (>= 1 or None: all) of theirs.  A NaN counts as minus infinity; where the greatest logit is infinite those that equal it
-    share the mass."""
+    prefix whose mass reaches ``top_p`` (>= 1 or None: all) of theirs; masses are added up in 64 bits, each off by 2^-46 of the greatest at most (2^-45 from 2^19 tokens
+    on).  A NaN counts as minus infinity; where the greatest logit is infinite those that equal it share the mass."""
     what = "sampling probabilities"
     options = [t for t in (temperature, top_k, top_p) if t is not None]
     _on_current_device(what, logits, out, *options)

@@ -28,3 +28,27 @@ def test_equal_logits_of_the_largest_vocabularies(ops, V, top_k, top_p):
     want[3, torch.sort(logits[3], descending=True, stable=True).indices[:count]] = 1 / count
     assert torch.equal(out > 0, want > 0)
     assert ((out - want).abs() <= 2.0 ** -22 / count).all()  # the sum of equal numbers, a quotient and its rounding, a product
+
+
+@pytest.mark.parametrize("V", [151936, 524288])
+@pytest.mark.parametrize("depth", [30.0, 32.0, 40.0])
+def test_masses_that_are_nothing_one_by_one(ops, V, depth):
+    """Two great logits and a long flat tail below them: a weight is a whole number of 2^-45 of the greatest (2^-44 from 2^19 tokens on), so that n tokens' mass
+    is off by n times half of that at most, and each weight by 2^-46 of itself.  Who stays is right for some mass within that bound."""
+    logits = torch.full((2, V), -depth, device=DEV)
+    logits[:, V // 3], logits[:, V // 2] = 0.0, 0.0
+    logits[1, ::2] -= 0.25
+    logits[1, V // 3] = logits[1, V // 2] = 0.0
+    for top_p in (0.5, 0.49999997, 0.50000006, 0.99999994):
+        out = torch.full((2, V), 9.0, device=DEV)
+        p = torch.tensor([top_p] * 2, dtype=torch.float32, device=DEV)
+        ops.sampling_probs(logits, out, torch.ones(2, device=DEV), None, p)
+        order = torch.sort(logits, dim=1, descending=True, stable=True).indices
+        w = torch.exp(logits.double()).gather(1, order)
+        kept = out.gather(1, order) > 0
+        count = kept.sum(1, keepdim=True)
+        assert torch.equal(kept, torch.arange(V, device=DEV) < count)  # the first ones
+        upto = torch.cumsum(w, 1)
+        aim, bound = p.double()[:, None] * upto[:, -1:], V * 2.0 ** (-46 if V < 1 << 19 else -45) + upto[:, -1:] * 2.0 ** -45
+        assert (upto.gather(1, count - 1) >= aim - bound).all()
+        assert ((count == 1) | (upto.gather(1, (count - 2).clamp(min=0)) < aim + bound)).all()

@@ -4,7 +4,8 @@
 // their order; child c, drawn from the draft's distribution q_x, is accepted if u_c q_x(t_c) R < r(t_c), that is with the
 // probability min(1, (r(t_c) / R) / q_x(t_c)), and the walk goes on from it.  Refused, it leaves the residual: r <- max(r - R q_x, 0), R <- sum r (where
 // nothing is left, r and R stay).  A draft without probabilities has chosen its tokens for certain: q_x(t_c) = 1, r(t_c) <- 0, R <- R - r(t_c).
-// Where no child is accepted the next token is drawn from r: the first i with sum_{j <= i} r_j > u_root sum_j r_j.  So tokens
+// Where no child is accepted the next token is drawn from r: the first i with sum_{j <= i} r_j > u_root sum_j r_j.  Chosen tokens may have been all that p_x had, and
+// then, as R is a little more than what is left (32-bit probabilities do not quite add up to 1), even the last of them can be refused: it is the one that follows.  So tokens
 // follow the target's distribution whatever was drafted.  All of it in 64 bits: at a border a rounding would be another token.
 //
 // A cluster of eight blocks takes a request, each an eighth of the vocabulary.  The tree, the random numbers and every node's p and q
@@ -194,6 +195,7 @@ __global__ void __launch_bounds__(THREADS, 2) verify_tree_kernel(const VerifyTre
         return t;
     };
     int node = 0, path = 1, refusals = 0, gone = 0;
+    int token = -1;  // the last of the refused ones that had a probability (drafts without probabilities)
     double left = 1.0, total = -1.0;  // total: of the last pass over what is left as it is now, below 0: none
     if (rank == 0 && threadIdx.x == 0 && n) a.out_nodes[(size_t)seq * a.width] = 0;
     auto look_at = [&](int x) {
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, 2) verify_tree_kernel(const VerifyTre
         }
         if ((double)s.u[c] * (drafted ? (double)s.q[c] : 1.0) * left < r) {
             if (rank == 0 && threadIdx.x == 0) a.out_nodes[(size_t)seq * a.width + path] = c;
-            node = c, ++path, refusals = 0, gone = 0, left = 1.0, total = -1.0;
+            node = c, ++path, refusals = 0, gone = 0, token = -1, left = 1.0, total = -1.0;
             look_at(c);
             continue;
         }
@@ -232,11 +234,11 @@ __global__ void __launch_bounds__(THREADS, 2) verify_tree_kernel(const VerifyTre
         } else {
             if (threadIdx.x == 0) s.gone[gone] = s.token[c];
             ++gone, left -= r;
+            if (r > 0.0) token = s.token[c];
             __syncthreads();
         }
     }
     if (n && total < 0.0) total = sum_up(refusals, gone);
-    int token = -1;
     if (n && total > 0.0) {
         const int b = (passes - 1) & 1;
         const double u = (double)s.u[0], aim = u > 0.0 ? u * total : 0.0;

@@ -2814,7 +2814,7 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     From the first node on, a node's children are tried in their order: child c with token t is accepted if u q(t) R < r(t), where r is the
     node's row of ``probs`` and R = 1 at first, and after every refusal r = max(r - R q, 0), R = sum r (both stay where that is nothing); without
     ``draft_probs`` q(t) = 1 and a refusal sets R = R - r(t), r(t) = 0.  Where no child is accepted, the next token is the first whose running sum of r exceeds
-    u times the sum of r (the lowest index first).  In 64 bits.
+    u times the sum of r (the lowest index first); where refusals without ``draft_probs`` have left nothing of r, the last refused token that had a probability.  In 64 bits.
 
     ``out_nodes`` (int32 [S, width]) gets the first node and the accepted ones, -1 behind them (a path ends where it is full);
     ``out_accepted`` (int32 [S]) how many were accepted; ``out_token`` (int32 [S]) the next token.  A request without nodes has no path, 0 accepted and the token -1, which is

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_tree_gpu import DEV, ints, nothing_reported, ops, rng  # noqa: F401  (fixtures among them)
+from test_tree_gpu import DEV, ints, nothing_reported, ops, rng, run_verify  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,33 @@ def test_masses_that_are_nothing_one_by_one(ops, V, depth):
         aim, bound = p.double()[:, None] * upto[:, -1:], V * 2.0 ** (-46 if V < 1 << 19 else -45) + upto[:, -1:] * 2.0 ** -45
         assert (upto.gather(1, count - 1) >= aim - bound).all()
         assert ((count == 1) | (upto.gather(1, (count - 2).clamp(min=0)) < aim + bound)).all()
+
+
+# ------------------------------------------------------------------------------------------------ verification
+TOP = 1 - 2.0 ** -24  # the greatest random number
+
+
+@pytest.mark.parametrize("rows, tokens, parents, u, path, token", [
+    # two tokens are all that the row has, of which the last random number refuses both: 1 - 0.6 is a little more than the second's
+    ([[0.6, 0.39999995, 0.0]], [0, 0, 1], [-1, 0, 0], [0.5, TOP, TOP], [0], 1),
+    # (the other way round the second one is accepted: (1 - 2^-24) (1 - 0.39999994636) = 0.60000001788 < 0.60000002384, and its row has nothing)
+    ([[0.6, 0.39999995, 0.0]], [0, 1, 0], [-1, 0, 0], [0.5, TOP, TOP], [0, 2], -1),
+    # a row whose probabilities do not add up to one
+    ([[0.0, 0.25, 0.0]], [0, 1, 2], [-1, 0, 0], [0.0, 0.5, 0.5], [0], 1),
+    ([[0.0, 0.25, 0.0]], [0, 1, 1], [-1, 0, 0], [0.0, 0.5, 0.0], [0], 1),
+    # on the second node of a path
+    ([[0.0, 1.0, 0.0], [0.0, 0.0, 0.75]], [0, 1, 2], [-1, 0, 1], [0.3, 0.5, 0.875], [0, 1], 2),
+    # what was refused before the path went on is forgotten
+    ([[0.5, 0.5, 0.0], [0.0] * 3, [0.0] * 3], [0, 0, 1], [-1, 0, 0], [0.3, 0.875, 0.25], [0, 2], -1),
+    # nothing that could be refused
+    ([[0.0, 0.0, 0.0]], [0, 1, 2], [-1, 0, 0], [0.3, 0.5, 0.5], [0], -1),
+])
+def test_chosen_drafts_that_are_all_refused(ops, rows, tokens, parents, u, path, token):
+    """Where refusals have left nothing of a row, the token refused last of those that had a probability follows, as it would if the row added up to one."""
+    n = len(tokens)
+    for V in (3, 700):
+        probs = torch.zeros(n, V, device=DEV)
+        for i, row in enumerate(rows):
+            probs[i, :3] = torch.tensor(row, device=DEV)
+        got = run_verify(ops, probs, tokens, parents, [0, n], u, 3)
+        assert got == ([path + [-1] * (3 - len(path))], [len(path) - 1], [token])

@@ -2705,7 +2705,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     keys and values already are: node i of request s in row ``seq_start_row[s]`` + i, rotated by its position, seq_start_row[s] + its depth.
 
     ``q`` [T, >= num_heads x head size] (bf16 or fp32; its first columns, so the rows of a fused projection will do), ``out``
-    [T, num_heads x head size] of the same type and apart from ``q``; ``k_cache``, ``v_cache`` [pages, kv heads, page size, head size] of the same type, head sizes
+    [T, num_heads x head size] of the same type and apart from ``q`` and the cache; ``k_cache``, ``v_cache`` [pages, kv heads, page size, head size] of the same type, head sizes
     that are a multiple of 8 up to 256.  Request s brings the rows ``seq_q_start[s]`` .. ``seq_q_start[s + 1] - 1`` (int32 [S + 1]); rows behind
     the last request's are left as they are.  ``parents`` (int32 [T]): each node's parent, the number of an earlier
     node of its request, or -1.  A node sees the ``seq_start_row[s]`` (int32 [S]) rows of its request's text, itself and its ancestors;
@@ -2751,9 +2751,16 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     scratch = _tree_attention_scratch(dt, D, S, hkv, num_heads // hkv, max_q_len, max_kv_len, page_size, pages * hkv * page_size, scale, min(window, 0x7fffffff), dev)
     if T == 1:
         ldq, ldo = max(ldq, cols), max(ldo, cols)
+    item, q_at, out_at, k_at, v_at = 2 if dtype == torch.bfloat16 else 4, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    out_end, cache_bytes = out_at + item * ((T - 1) * ldo + cols), item * pages * hkv * page_size * D
+    if out_at < q_at + item * ((T - 1) * ldq + cols) and q_at < out_end:  # (columns beside the queries', in the same rows, are apart from them)
+        if ldq != ldo or not item * cols <= (out_at - q_at) % (item * ldq) <= item * (ldq - cols):
+            raise KernelError(f"{what}: the output must lie apart from the queries")
+    if (out_at < k_at + cache_bytes and k_at < out_end) or (out_at < v_at + cache_bytes and v_at < out_end):
+        raise KernelError(f"{what}: the output must lie apart from the cache")
     try:
         arguments = _TREE_ATTENTION.pack(
-            q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_q_start.data_ptr(),
+            q_at, out_at, k_at, v_at, block_tables.data_ptr(), seq_q_start.data_ptr(),
             seq_start_row.data_ptr(), parents.data_ptr(), workspace.address("tree_attention", scratch, torch.float32), _current_stream(), ldq, ldo, dt,
             pages, hkv, page_size, D, width, S, T, num_heads, max_q_len, max_kv_len, min(window, 0x7fffffff), scale)
     except (struct.error, OverflowError) as e:

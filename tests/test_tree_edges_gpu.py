@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_tree_gpu import DEV, ints, nothing_reported, ops, rng, run_verify  # noqa: F401  (fixtures among them)
+from test_tree_gpu import DEV, Step, ints, nothing_reported, ops, rng, run_verify, workspace  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,25 @@ def test_chosen_drafts_that_are_all_refused(ops, rows, tokens, parents, u, path,
             probs[i, :3] = torch.tensor(row, device=DEV)
         got = run_verify(ops, probs, tokens, parents, [0, n], u, 3)
         assert got == ([path + [-1] * (3 - len(path))], [len(path) - 1], [token])
+
+
+# ------------------------------------------------------------------------------------------------ memory that is shared
+def test_attention_into_memory_that_it_reads_is_refused(ops, workspace):
+    from ferrisinfer_b200.errors import KernelError
+
+    step = Step(torch.bfloat16, 4, 2, 64, 16, [3, 2], [20, 30], extra_columns=512)
+    want = step.run(ops, workspace).clone()
+    call = lambda q, out: ops.tree_attention(q, out, step.k, step.v, *step.device_tensors, *step.most, 4, 0.125, workspace=workspace)
+    flat = torch.zeros(6 * 768, dtype=torch.bfloat16, device=DEV)
+    rows = flat[:5 * 768].view(5, 768)
+    rows.copy_(step.q)
+    for q, out in ((rows, rows[:, :256]), (rows, rows[:, 255:511]), (rows[:, 200:456], rows[:, :256]),
+                   (rows, flat[64:64 + 5 * 256].view(5, 256)),                   # rows of another length
+                   (rows, flat.as_strided((5, 256), (768, 1), 700)),             # from the end of a row to the beginning of the next one
+                   (step.q, step.k.view(-1)[:5 * 256].view(5, 256)), (step.q, step.v.view(-1)[-5 * 256:].view(5, 256))):
+        with pytest.raises(KernelError, match="apart"):
+            call(q, out)
+    call(rows, rows[:, 256:512])  # columns beside the queries', in the same rows, are apart from them
+    assert torch.equal(rows[:, 256:512], want) and torch.equal(rows[:, :256], step.q[:, :256])
+    call(rows[:, :256], rows[:, 512:])
+    assert torch.equal(rows[:, 512:], want)

@@ -2691,6 +2691,19 @@ def _int32(what: str, **tensors) -> None:
             raise KernelError(f"{what}: {name} must be contiguous and {torch.int32}, found {t.dtype}")
 
 
+def _outputs_apart(what: str, outputs, inputs) -> None:
+    """Contiguous outputs share no memory with one another or with inputs (of matrices: from their first row to the last)."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in outputs]
+    held = sorted(spans)
+    if any(end > begin for (_, end), (begin, _) in zip(held, held[1:])):
+        raise KernelError(f"{what}: the outputs must lie apart from one another")
+    for t in inputs:
+        begin = t.data_ptr()
+        end = begin + t.element_size() * (t.numel() if t.is_contiguous() else (t.shape[0] - 1) * t.stride(0) + t.shape[1])
+        if t.numel() and any(a < end and begin < b for a, b in spans):
+            raise KernelError(f"{what}: the outputs must lie apart from what is read")
+
+
 def _long_rows(what: str, t: torch.Tensor) -> tuple:
     """(rows, columns, row stride) of a matrix of fp32 with contiguous rows."""
     if t.dim() != 2 or t.dtype != torch.float32 or (t.shape[1] > 1 and t.stride(1) != 1):
@@ -2823,7 +2836,7 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     ``draft_probs`` q(t) = 1 and a refusal sets R = R - r(t), r(t) = 0.  Where no child is accepted, the next token is the first whose running sum of r exceeds
     u times the sum of r (the lowest index first); where refusals without ``draft_probs`` have left nothing of r, the last refused token that had a probability.  In 64 bits.
 
-    ``out_nodes`` (int32 [S, width]) gets the first node and the accepted ones, -1 behind them (a path ends where it is full);
+    The outputs, apart from one another and from what is read: ``out_nodes`` (int32 [S, width]) gets the first node and the accepted ones, -1 behind them (a path ends where it is full);
     ``out_accepted`` (int32 [S]) how many were accepted; ``out_token`` (int32 [S]) the next token.  A request without nodes has no path, 0 accepted and the token -1, which is
     also that of a row without any probability.  NaN and negative probabilities count as 0.  Tokens outside the vocabulary and parents that are no earlier node are
     reported (``check_kernel_status``), and such nodes not tried."""
@@ -2848,6 +2861,7 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
             raise KernelError(f"{what}: probabilities {tuple(probs.shape)}, the draft's {tuple(draft_probs.shape)}")
     if S == 0:
         return
+    _outputs_apart(what, (out_nodes, out_accepted, out_token), (probs, tokens, parents, seq_q_start, uniforms) + (() if draft_probs is None else (draft_probs,)))
     # (rows that share memory, as expand makes them, are only read; the library wants rows that do not)
     if ldp < V:
         probs, ldp = probs.contiguous(), V

@@ -104,3 +104,19 @@ def test_attention_into_memory_that_it_reads_is_refused(ops, workspace):
     assert torch.equal(rows[:, 256:512], want) and torch.equal(rows[:, :256], step.q[:, :256])
     call(rows[:, :256], rows[:, 512:])
     assert torch.equal(rows[:, 512:], want)
+
+
+def test_verification_into_memory_that_it_reads_or_twice_is_refused(ops):
+    from ferrisinfer_b200.errors import KernelError
+
+    i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=DEV)
+    probs, one = torch.full((5, 30), 1 / 30, device=DEV), ints([0, 2, 5])
+    both = i32(4)
+    good = dict(probs=probs, tokens=i32(5), parents=i32(5) - 1, seq_q_start=one, uniforms=torch.zeros(5, device=DEV), out_nodes=i32(2, 2), out_accepted=i32(2), out_token=i32(2))
+    ops.verify_tree(**good)
+    for change in (dict(out_accepted=both[:2], out_token=both[1:3]), dict(out_nodes=both.view(2, 2), out_token=both[2:]), dict(out_token=good["tokens"][3:]),
+                   dict(out_accepted=good["parents"][:2]), dict(out_nodes=probs.view(torch.int32)[0, :4].view(2, 2)), dict(out_token=one[1:]),
+                   dict(out_token=good["uniforms"].view(torch.int32)[:2])):
+        with pytest.raises(KernelError, match="apart"):
+            ops.verify_tree(**{**good, **change})
+    ops.verify_tree(**{**good, "out_accepted": both[:2], "out_token": both[2:]})

@@ -2879,7 +2879,7 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
 
 class CacheLayers:
     """The paged caches of a model's layers that share block tables: [(keys, values), ...], each [pages, kv heads, page size, head size], all of
-    one shape and type, on one device.  Made once; it holds the tensors and, on the device, where they lie."""
+    one shape and type, on one device, no two in the same memory (a row would move twice).  Made once; it holds the tensors and, on the device, where they lie."""
 
     __slots__ = ("layers", "pages", "kv_heads", "page_size", "row_bytes", "device_index", "align", "table")
 
@@ -2897,6 +2897,8 @@ class CacheLayers:
         if 0 in first.shape or self.row_bytes % 2:
             raise KernelError(f"cache layers: nothing can be moved in caches of {tuple(first.shape)} {first.dtype}")
         at = [t.data_ptr() for layer in self.layers for t in layer]
+        if any(b - a < self.row_bytes * self.pages * self.kv_heads * self.page_size for a, b in zip(sorted(at), sorted(at)[1:])):
+            raise KernelError("cache layers: two of the caches share memory")
         self.align = 16
         while any(a % self.align for a in at):
             self.align //= 2

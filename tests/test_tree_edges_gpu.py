@@ -120,3 +120,16 @@ def test_verification_into_memory_that_it_reads_or_twice_is_refused(ops):
         with pytest.raises(KernelError, match="apart"):
             ops.verify_tree(**{**good, **change})
     ops.verify_tree(**{**good, "out_accepted": both[:2], "out_token": both[2:]})
+
+
+def test_cache_layers_that_share_memory_are_refused(ops):
+    from ferrisinfer_b200.errors import KernelError
+
+    cache = torch.zeros(2, 4, 2, 16, 8, device=DEV)
+    flat = torch.zeros(2 * 4 * 2 * 16 * 8, device=DEV)
+    k, v = cache
+    ops.CacheLayers([(k, v)])
+    for layers in ([(k, k)], [(k, v), (v, k.clone())], [(k, v), (k, v)], [(flat[:1024].view(4, 2, 16, 8), flat[8:1032].view(4, 2, 16, 8))]):
+        with pytest.raises(KernelError, match="share memory"):
+            ops.CacheLayers(layers)
+    ops.CacheLayers([(flat[:1024].view(4, 2, 16, 8), flat[1024:].view(4, 2, 16, 8))])

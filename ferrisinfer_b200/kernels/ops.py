@@ -2726,7 +2726,8 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     names a page.  What a node does not see has no effect, whatever it holds; a node that sees nothing gives zeros.
     ``max_q_len`` (at most TREE_NODES), ``max_kv_len``: the most nodes and rows (nodes included) of any request.  Nodes beyond the one are
     not attended, which is reported (``check_kernel_status``), rows beyond the other are not seen.  A parent that is no earlier node is reported
-    and counts as none."""
+    and counts as none.  Where there are nodes there have to be rows: a ``max_kv_len`` of 0, a cache without pages and tables without blocks are refused.
+    ``workspace`` holds the parts of rows between the call's two kernels: calls that can run at the same time need workspaces of their own."""
     what = "tree attention"
     dev = _on_current_device(what, q, out, k_cache, v_cache, block_tables, seq_q_start, seq_start_row, parents)
     _int32(what, **{"block tables": block_tables, "first query rows": seq_q_start, "rows of the text": seq_start_row, "parents": parents})
@@ -2756,7 +2757,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         return
     max_q_len, width = min(max_q_len, T), block_tables.shape[1]
     max_kv_len = min(max_kv_len, width * page_size)
-    if max_kv_len == 0 or pages == 0:  # nobody sees anything
+    if max_kv_len == 0 or pages == 0:  # (a node is a row itself: its own key and value are in the cache)
         raise KernelError(f"{what}: no rows can be seen: at most {max_kv_len} of {pages} pages")
     if workspace is None:
         raise KernelError(f"{what}: a workspace is needed")

@@ -133,3 +133,19 @@ def test_cache_layers_that_share_memory_are_refused(ops):
         with pytest.raises(KernelError, match="share memory"):
             ops.CacheLayers(layers)
     ops.CacheLayers([(flat[:1024].view(4, 2, 16, 8), flat[1024:].view(4, 2, 16, 8))])
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def test_attention_without_any_cached_row_is_refused(ops, workspace):
+    from ferrisinfer_b200.errors import KernelError
+
+    step = Step(torch.bfloat16, 4, 2, 64, 16, [3, 2], [20, 30])
+    step.run(ops, workspace)
+    tables, *others = step.device_tensors
+    out = torch.full((5, 256), 7.0, dtype=torch.bfloat16, device=DEV)
+    call = lambda k, tables, most, S=2: ops.tree_attention(step.q, out, k, k, tables, *others, *most, 4, 0.125, workspace=workspace)
+    for k, t, most in ((step.k, tables, (3, 0)), (step.k[:0], tables, (3, 40)), (step.k, tables[:, :0].contiguous(), (3, 40))):
+        with pytest.raises(KernelError, match="no rows"):
+            call(k, t, most)
+    call(step.k, tables, (0, 0))  # (no nodes either)
+    assert (out == 7).all()

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ TreeLines trees[WIDE ? 1 : 2];
     __shared__ TreeRequests requests;
-    __shared__ uint64_t fulls[Z::STAGES], empties[Z::STAGES], q_ready[2], s_ready[2], p_ready[2], o_done[2];
+    __shared__ uint64_t fulls[Z::STAGES], empties[Z::STAGES], q_ready[2], s_ready[2], p_ready[2], o_done[2], ended[2];
     __shared__ uint32_t tensor_base;
     __shared__ int odd[4];  // threads that have found a value of a unit that is not finite: of units of both groups by turns, of each one's
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tma_prefetch_descriptor(&map_k);
         tma_prefetch_descriptor(&map_v);
         for (int s = 0; s < Z::STAGES; ++s) mbar_init(&fulls[s], 1), mbar_init(&empties[s], 1);
-        for (int k = 0; k < 2; ++k) mbar_init(&q_ready[k], 4), mbar_init(&s_ready[k], 1), mbar_init(&p_ready[k], 4), mbar_init(&o_done[k], 1);
+        for (int k = 0; k < 2; ++k) mbar_init(&q_ready[k], 4), mbar_init(&s_ready[k], 1), mbar_init(&p_ready[k], 4), mbar_init(&o_done[k], 1), mbar_init(&ended[k], 1);
         mbar_fence_init();
     }
     if (warp == SOFTMAX_WARPS + 2) tensor_memory_take(&tensor_base, COLUMNS);
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             // (nothing to do)
         } else if (warp < SOFTMAX_WARPS + 2) {
             // ---- K and V on their way: eight lanes, a box of 16 rows each
-            int place0 = 0;
+            int place0 = 0, issued = 0;
             int4 begun = walk.none();
             while (walk.next(p, requests, item)) {
                 const TreeRequest r = item.request;
@@ -180,9 +180,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 auto load = [&](int place, const CUtensorMap* map, int row) {
                     const int at = place0 + place, s = at % ST;
                     if (at >= ST) wait(&empty[s], (at / ST - 1) & 1, 140);
-                    if (lane == 0) mbar_expect_tx(&full[s], Z::BLOCK);
+                    dead = __any_sync(0xffffffffu, dead);
+                    if (!dead) issued = at + 1;  // (a stage that may be in use is not written)
+                    if (!dead && lane == 0) mbar_expect_tx(&full[s], Z::BLOCK);
                     __syncwarp();
-                    if (lane < UNIT / PAGE_ROWS) {
+                    if (!dead && lane < UNIT / PAGE_ROWS) {
 #pragma unroll
                         for (int a = 0; a < Z::ATOMS; ++a) tma_load_2d(kv_smem + (size_t)s * Z::BLOCK + a * ATOM + lane * BOX, map, 64 * a, row, &full[s]);
                     }
@@ -200,9 +202,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 place0 += 2 * n;
             }
             if (lane == 0 && share < groups && (!WIDE || share * lanes == blockIdx.x)) p.begun[share] = begun;  // (the first lane has query rows of every item)
-            // (after a wait that ran out: nothing may still be on its way when the block ends)
-            if (dead)
-                for (int at = max(0, place0 - ST); at < place0; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);
+            // (nothing may still be on its way when the block ends, whosever wait has run out)
+            for (int at = max(0, issued - ST); at < issued; ++at) mbar_wait(&full[at % ST], (at / ST) & 1, p.status, 148);
         } else {
             // ---- products
             const uint32_t idesc_qk = umma_idesc_bf16(ROWS, UNIT), idesc_pv = umma_idesc_bf16(ROWS, D) | (1u << 16);  // (V: cached rows x columns)
@@ -257,6 +258,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                 __syncwarp();
                 place0 += 2 * n, ++segments;
+            }
+            // (nor may a product still read or write when the block gives its memory back)
+            if (segments > 0) {
+                if (elected()) tcgen05_commit(&ended[g]);
+                __syncwarp();
+                mbar_wait(&ended[g], 0, p.status, 149);
             }
         }
     } else {

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256) tree_parts_kernel(const TreeAttention p, 
 }
 
 TreePlan plan_of(int dtype, int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window) {
-    if (dtype != FERRIS_BF16) return tree_plan_f32(head_dim, seqs, kv_heads, group, max_nodes, max_kv);
+    if (dtype != FERRIS_BF16) return tree_plan_f32(head_dim, seqs, kv_heads, group, max_nodes, max_kv, window);
     return tree_plan(head_dim, seqs, kv_heads, group, max_nodes, max_kv, page_size, cache_rows, scale, window);
 }
 

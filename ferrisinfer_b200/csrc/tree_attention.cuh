@@ -139,7 +139,12 @@ struct TreePlan {
     bool fits;               // tiles are counted in 32 bits, and lanes are a launch's second dimension
     long long part_floats(int head_dim) const { return 2ll * groups * lanes * rows * (head_dim + 2); }
     long long floats(int head_dim) const { return part_floats(head_dim) + 4ll * groups; }  // of scratch: parts, and behind them the items that groups have begun
-    // As many blocks as the SMs have room for (`blocks` on each), and there can be tiles for.
+    // The most rows that a request's tiles hold: behind a window those of the window, of the nodes and of the tile in which it begins.
+    static int most_rows(int max_kv, int max_nodes, int window, int unit) {
+        const long long seen = (long long)window + max_nodes + unit;
+        return window > 0 && seen < max_kv ? (int)seen : max_kv;
+    }
+    // As many blocks as the SMs have room for (`blocks` on each), and there can be tiles for (max_kv: most_rows).
     void deal(int seqs, int kv_heads, int group, int max_nodes, int max_kv, int blocks, bool flat) {
         const int sms = ferris_sm_count();
         const int row_blocks = (max_nodes * group + rows - 1) / rows;
@@ -153,7 +158,7 @@ struct TreePlan {
 TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int page_size, long long cache_rows, float scale, int window);
 int tree_attention_mma(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
 int tree_attention_tc(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
-TreePlan tree_plan_f32(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv);
+TreePlan tree_plan_f32(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int window);
 int tree_attention_f32(const TreeAttention& p, const TreePlan& plan, cudaStream_t stream);
 
 __device__ __forceinline__ int tree_scan(int v) {

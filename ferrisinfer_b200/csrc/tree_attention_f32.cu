@@ -296,13 +296,13 @@ void with_variant(int D, int rows, F f) {
 
 }  // namespace
 
-TreePlan tree_plan_f32(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv) {
+TreePlan tree_plan_f32(int head_dim, int seqs, int kv_heads, int group, int max_nodes, int max_kv, int window) {
     TreePlan plan = {};
     with_variant(head_dim, max_nodes * group, [&](auto dp, auto g) {
         using Z = Sizes<dp.value, g.value>;
         plan.unit = Z::TILE, plan.rows = Z::ROWS;
     });
-    plan.deal(seqs, kv_heads, group, max_nodes, max_kv, 1, true);
+    plan.deal(seqs, kv_heads, group, max_nodes, plan.most_rows(max_kv, max_nodes, window, plan.unit), 1, true);
     return plan;
 }
 

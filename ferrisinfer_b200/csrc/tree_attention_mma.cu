@@ -430,13 +430,14 @@ TreePlan tree_plan(int head_dim, int seqs, int kv_heads, int group, int max_node
     });
     // tcgen05 where its products outweigh what it takes to begin with: from 65 query rows on, from 17 where there are more than four units for an SM.  Microseconds,
     // mma.sync (with pages of 24 rows) and tcgen05: 8 requests after 4,096 rows, 14 / 2 heads of 64, 14 query rows 14.5 and 19.1, 56 rows 18.5 and 19.6, 70 rows 23.5 and
-    // 20.2; 32 requests, 28 / 4 heads of 128, 14 rows 54 and 67, 28 rows 73 and 67, 56 rows 95 and 69, 112 rows 165 and 78.
+    // 20.2; 32 requests, 28 / 4 heads of 128, 14 rows 54 and 67, 28 rows 73 and 67, 56 rows 95 and 69, 112 rows 165 and 78.  With a window it is the units in it that count:
+    // 32 requests after 16,384 rows, 14 / 2 heads of 64, 56 rows, window 128 12.5 and 18.2; 28 / 4 heads of 128, window 1,024 35.9 and 33.8; 64 requests, 300, 47 and 28.
     // (the row of a box that lies nowhere is a number too; a scale below nought would turn maxima into minima)
     const int rows = max_nodes * group, sms = ferris_sm_count();
-    const bool many = rows > 64 || (rows > 16 && (long long)seqs * kv_heads * ((max_kv + 127) / 128) > 4ll * (sms > 0 ? sms : 148));
+    const bool many = rows > 64 || (rows > 16 && (long long)seqs * kv_heads * ((TreePlan::most_rows(max_kv, max_nodes, window, 128) + 127) / 128) > 4ll * (sms > 0 ? sms : 148));
     plan.tensor = many && (head_dim == 64 || head_dim == 128) && page_size % 16 == 0 && cache_rows < 0x7fffffff && scale > 0.0f && scale < 1e30f;
     if (plan.tensor) plan.unit = 128, plan.rows = rows > 128 ? 256 : 128, blocks = rows > 128 ? 1 : 2;  // (two groups to a block)
-    plan.deal(seqs, kv_heads, group, max_nodes, max_kv, blocks, !plan.tensor);
+    plan.deal(seqs, kv_heads, group, max_nodes, plan.most_rows(max_kv, max_nodes, window, plan.unit), blocks, !plan.tensor);
     return plan;
 }
 

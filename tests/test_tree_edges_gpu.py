@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+import plain_tree as plain
 from test_tree_gpu import DEV, Step, ints, nothing_reported, ops, rng, run_verify, workspace  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +150,21 @@ def test_attention_without_any_cached_row_is_refused(ops, workspace):
             call(k, t, most)
     call(step.k, tables, (0, 0))  # (no nodes either)
     assert (out == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("nodes", [[5, 12], [5, 70]])
+def test_texts_beyond_their_tables(ops, workspace, dtype, window, nodes):
+    """A request that says it has more rows than its table sees those that the table has, behind a window none; the other request is none the wiser."""
+    step = Step(dtype, 12, 2, 64, 16, nodes, [60, 200])
+    for t, seed in ((step.k, 5), (step.v, 6)):  # (what lies on the tables' last rows is seen now)
+        t.copy_(torch.where(torch.isnan(t), torch.randn(t.shape, generator=rng(seed), device=DEV).to(dtype), t))
+    most = max(nodes), 200 + nodes[1]
+    for start in (0x7fffffff, 1 << 30, 100000):
+        step.starts[0] = start
+        out = step.run(ops, workspace, window=window, most=most)
+        ref, mag, size = plain.tree_attention(step.q, step.k, step.v, step.tables, step.q_start, step.starts, step.parents, 12, 0.125, window, max_rows=most[1])
+        step.compare(out, ref, plain.attention_tolerance(dtype, ref, mag, size, most[1], 64))
+        assert not window or (out[:5] == 0).all()
+        assert window or (out[:5] != 0).any(1).all()

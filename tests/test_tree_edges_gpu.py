@@ -12,6 +12,18 @@ pytestmark = pytest.mark.gpu
 
 
 # ------------------------------------------------------------------------------------------------ probabilities
+def in_64_bits(logits, temperature, top_k, top_p, rows=32):
+    """(first row, probabilities) of some rows at a time; logits without NaN."""
+    place = torch.arange(logits.shape[1], device=DEV)
+    for first in range(0, len(logits), rows):
+        x = logits[first:first + rows].double()
+        T, k, p = (torch.tensor(o[first:first + rows], dtype=torch.float32, device=DEV).double()[:, None] for o in (temperature, top_k, top_p))
+        x, order = torch.sort(x, dim=1, descending=True, stable=True)
+        w = torch.where((k <= 0) | (place < k), torch.exp((x - x[:, :1]) / T), 0.0)
+        w = torch.where((p >= 1) | (place == 0) | (torch.cumsum(w, 1) - w < p * w.sum(1, keepdim=True)), w, 0.0)
+        yield first, torch.zeros_like(x).scatter_(1, order, w / w.sum(1, keepdim=True))
+
+
 @pytest.mark.parametrize("V", [262143, 262144, 524287, 524288])
 @pytest.mark.parametrize("top_k, top_p", [(0, 0.5), (0, 0.999), (0, 1e-6), (1000, 0.5), (400000, 0.75), (20, 0.5), (0, 1.0)])
 def test_equal_logits_of_the_largest_vocabularies(ops, V, top_k, top_p):
@@ -53,6 +65,31 @@ def test_masses_that_are_nothing_one_by_one(ops, V, depth):
         aim, bound = p.double()[:, None] * upto[:, -1:], V * 2.0 ** (-46 if V < 1 << 19 else -45) + upto[:, -1:] * 2.0 ** -45
         assert (upto.gather(1, count - 1) >= aim - bound).all()
         assert ((count == 1) | (upto.gather(1, (count - 2).clamp(min=0)) < aim + bound)).all()
+
+
+BATCHES = {
+    "plain": [(1.0, 0, 1.0)], "chat": [(0.7, 20, 0.9)], "mass": [(0.8, 0, 0.9)],
+    "mixed": [(1.0, 0, 1.0), (0.7, 20, 0.9), (0.8, 0, 0.9), (1.0, 3001, 0.95), (0.6, 50, 1.0), (1.3, 0, 0.5)],
+}
+
+
+@pytest.mark.parametrize("options", BATCHES.values(), ids=BATCHES.keys())
+def test_probabilities_of_a_busy_server(ops, options):
+    """512 rows of 151,936, a few likely tokens in each, against 64 bits on the same logits."""
+    n, V = 512, 151936
+    gen = rng(41)
+    logits = torch.randn(n, V, generator=gen, device=DEV) * 2
+    likely = torch.arange(20, device=DEV) * (V // 20) + torch.randint(V // 20, (n, 20), generator=gen, device=DEV)  # (no place twice)
+    logits.scatter_(1, likely, 6 + 2 * torch.randn(n, 20, generator=gen, device=DEV))
+    temperature, top_k, top_p = ([options[i % len(options)][j] for i in range(n)] for j in range(3))
+    out = torch.full((n, V), 9.0, device=DEV)
+    ops.sampling_probs(logits, out, torch.tensor(temperature, device=DEV), ints(top_k), torch.tensor(top_p, device=DEV))
+    for first, ref in in_64_bits(logits, temperature, top_k, top_p):
+        got, x = out[first:first + len(ref)].double(), logits[first:first + len(ref)].double()
+        assert torch.equal(got > 0, ref > 0)
+        # an exponent of 32 bits is off by 2^-23 of itself, the exponential, the sum and the quotient by a few 2^-24
+        exponent = (x.amax(1, keepdim=True) - x) / torch.tensor(temperature[first:first + len(ref)], device=DEV).double()[:, None]
+        assert ((got - ref).abs() <= ref * (exponent * 2.0 ** -22 + 2.0 ** -19) + 1e-37).all()
 
 
 # ------------------------------------------------------------------------------------------------ verification

@@ -13,9 +13,10 @@
 // the refusal of a token that has a q, and for the last draw, whose passes leave the sums of every warp's run of elements, so that the draw goes
 // through one run again.  Sums are added up in one order whatever the timing.
 //
-// What bounds it (151,936 tokens): one request 9.6 us, a chain of tables, one pass and the draw; 64 requests of 8 nodes with drafts' probabilities 47 us (floor 12, every
-// request's rows once): four to five passes a request with instructions in 64 bits and barriers of the cluster between.  Taken back: the rows kept in shared
-// memory between passes by clusters of sixteen (57 us), blocks of 256 threads (54).
+// What bounds it (151,936 tokens): one request 9.6 us, a chain of tables, one pass and the draw; 64 requests of 8 nodes with drafts' probabilities 45 to 56 us, as the random
+// numbers have it (floor 12, every request's rows once): four to five passes a request with instructions in 64 bits and barriers of the cluster between, by 512 blocks of
+// which 296 run at once.  A pass goes through all refusals of its node so far, so that the work grows with their square: it is small trees that are meant.  Taken back: the
+// rows kept in shared memory between passes by clusters of sixteen (57 us where it took 47), blocks of 256 threads (54).
 #include <math.h>
 
 #include "common.cuh"

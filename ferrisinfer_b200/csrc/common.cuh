@@ -30,6 +30,12 @@ int ferris_allow_dynamic_smem(const void* fn, size_t bytes);
         return FERRIS_BAD_ARGUMENT;   \
     } while (0)
 
+// Whether two pieces of memory have a byte in common (null or nothing: no).
+inline bool ferris_share_memory(const void* a, long long a_bytes, const void* b, long long b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && a_bytes > 0 && b_bytes > 0 && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
 #define FERRIS_LAUNCH_CHECK()                          \
     do {                                               \
         cudaError_t e_ = cudaGetLastError();           \

@@ -161,6 +161,15 @@ FERRIS_API int ferris_tree_attention(const TreeAttentionArgs* a) {
     const TreePlan plan = plan_of(a->dtype, a->head_dim, a->seqs, a->kv_heads, p.group, a->max_nodes, p.limit, a->page_size,
                                   (long long)a->pages * a->kv_heads * a->page_size, a->scale, a->window);
     if (!plan.fits) FERRIS_REFUSE("%d requests of up to %d tokens and %d rows exceed one launch", a->seqs, a->max_nodes, p.limit);
+    // (blocks write their outputs while others still read; columns beside the queries', in rows of one length, are apart from them)
+    const long long item = a->dtype == FERRIS_BF16 ? 2 : 4, columns = item * a->heads * a->head_dim, cache = item * a->pages * a->kv_heads * a->page_size * a->head_dim;
+    const long long q_bytes = item * (a->tokens - 1) * a->ldq + columns, out_bytes = item * (a->tokens - 1) * a->ldo + columns, line = item * a->ldq;
+    if (ferris_share_memory(a->q, q_bytes, a->out, out_bytes)) {
+        const long long behind = a->ldq == a->ldo && line > 0 ? (((long long)((uintptr_t)a->out - (uintptr_t)a->q)) % line + line) % line : 0;
+        if (behind < columns || behind > line - columns) FERRIS_REFUSE("the output must lie apart from the queries");
+    }
+    if (ferris_share_memory(a->k_cache, cache, a->out, out_bytes) || ferris_share_memory(a->v_cache, cache, a->out, out_bytes))
+        FERRIS_REFUSE("the output must lie apart from the cache");
     p.parts = (float*)const_cast<void*>(a->parts);
     p.begun = (int4*)(p.parts + plan.part_floats(p.head_dim));
     const cudaStream_t stream = (cudaStream_t)a->stream;

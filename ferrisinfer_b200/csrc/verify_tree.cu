@@ -317,6 +317,17 @@ FERRIS_API int ferris_verify_tree(const VerifyTreeArgs* x) {
     if (x->seqs <= 0) return FERRIS_OK;
     if (x->rows < 0 || x->vocab <= 0 || x->width <= 0 || x->ldp < x->vocab || (x->draft && x->ldd < x->vocab))
         FERRIS_REFUSE("%d rows of %d probabilities, paths of %d nodes", x->rows, x->vocab, x->width);
+    // (a request's blocks write while another's may not have begun to read)
+    const long long ints = 4, paths = ints * x->seqs * x->width, each = ints * x->seqs, nodes = ints * x->rows;
+    const struct { const void* at; long long bytes; } out[3] = {{x->out_nodes, paths}, {x->out_accepted, each}, {x->out_token, each}},
+        in[6] = {{x->probs, x->rows ? 4 * ((x->rows - 1) * x->ldp + x->vocab) : 0}, {x->draft, x->draft && x->rows ? 4 * ((x->rows - 1) * x->ldd + x->vocab) : 0},
+                 {x->tokens, nodes}, {x->parents, nodes}, {x->uniforms, nodes}, {x->q_start, each + 4}};
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (ferris_share_memory(out[i].at, out[i].bytes, out[j].at, out[j].bytes)) FERRIS_REFUSE("the outputs must lie apart from one another");
+        for (const auto& read : in)
+            if (ferris_share_memory(out[i].at, out[i].bytes, read.at, read.bytes)) FERRIS_REFUSE("the outputs must lie apart from what is read");
+    }
     VerifyTree a;
     a.probs = (const float*)x->probs, a.draft = (const float*)x->draft, a.ldp = x->ldp, a.ldd = x->ldd;
     a.tokens = (const int*)x->tokens, a.parents = (const int*)x->parents, a.q_start = (const int*)x->q_start;

@@ -2691,19 +2691,6 @@ def _int32(what: str, **tensors) -> None:
             raise KernelError(f"{what}: {name} must be contiguous and {torch.int32}, found {t.dtype}")
 
 
-def _outputs_apart(what: str, outputs, inputs) -> None:
-    """Contiguous outputs share no memory with one another or with inputs (of matrices: from their first row to the last)."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in outputs]
-    held = sorted(spans)
-    if any(end > begin for (_, end), (begin, _) in zip(held, held[1:])):
-        raise KernelError(f"{what}: the outputs must lie apart from one another")
-    for t in inputs:
-        begin = t.data_ptr()
-        end = begin + t.element_size() * (t.numel() if t.is_contiguous() else (t.shape[0] - 1) * t.stride(0) + t.shape[1])
-        if t.numel() and any(a < end and begin < b for a, b in spans):
-            raise KernelError(f"{what}: the outputs must lie apart from what is read")
-
-
 def _long_rows(what: str, t: torch.Tensor) -> tuple:
     """(rows, columns, row stride) of a matrix of fp32 with contiguous rows."""
     if t.dim() != 2 or t.dtype != torch.float32 or (t.shape[1] > 1 and t.stride(1) != 1):
@@ -2765,16 +2752,9 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     scratch = _tree_attention_scratch(dt, D, S, hkv, num_heads // hkv, max_q_len, max_kv_len, page_size, pages * hkv * page_size, scale, min(window, 0x7fffffff), dev)
     if T == 1:
         ldq, ldo = max(ldq, cols), max(ldo, cols)
-    item, q_at, out_at, k_at, v_at = 2 if dtype == torch.bfloat16 else 4, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    out_end, cache_bytes = out_at + item * ((T - 1) * ldo + cols), item * pages * hkv * page_size * D
-    if out_at < q_at + item * ((T - 1) * ldq + cols) and q_at < out_end:  # (columns beside the queries', in the same rows, are apart from them)
-        if ldq != ldo or not item * cols <= (out_at - q_at) % (item * ldq) <= item * (ldq - cols):
-            raise KernelError(f"{what}: the output must lie apart from the queries")
-    if (out_at < k_at + cache_bytes and k_at < out_end) or (out_at < v_at + cache_bytes and v_at < out_end):
-        raise KernelError(f"{what}: the output must lie apart from the cache")
     try:
         arguments = _TREE_ATTENTION.pack(
-            q_at, out_at, k_at, v_at, block_tables.data_ptr(), seq_q_start.data_ptr(),
+            q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_q_start.data_ptr(),
             seq_start_row.data_ptr(), parents.data_ptr(), workspace.address("tree_attention", scratch, torch.float32), _current_stream(), ldq, ldo, dt,
             pages, hkv, page_size, D, width, S, T, num_heads, max_q_len, max_kv_len, min(window, 0x7fffffff), scale)
     except (struct.error, OverflowError) as e:
@@ -2862,7 +2842,6 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
             raise KernelError(f"{what}: probabilities {tuple(probs.shape)}, the draft's {tuple(draft_probs.shape)}")
     if S == 0:
         return
-    _outputs_apart(what, (out_nodes, out_accepted, out_token), (probs, tokens, parents, seq_q_start, uniforms) + (() if draft_probs is None else (draft_probs,)))
     # (rows that share memory, as expand makes them, are only read; the library wants rows that do not)
     if ldp < V:
         probs, ldp = probs.contiguous(), V

@@ -2888,7 +2888,7 @@ class CacheLayers:
 def keep_tree_rows(layers: CacheLayers, block_tables: torch.Tensor, seq_start_row: torch.Tensor, nodes: torch.Tensor, accepted: torch.Tensor):
     """The cached rows of the accepted nodes move together behind their request's text, in all ``layers``.
 
-    Request s has ``seq_start_row[s]`` (int32 [S]) rows of text, and node i of its tree the row behind them by i, in the pages that ``block_tables`` (int32
+    Request s (of at most 65,535) has ``seq_start_row[s]`` (int32 [S]) rows of text, and node i of its tree the row behind them by i, in the pages that ``block_tables`` (int32
     [S, blocks]) names.  ``nodes`` (int32 [S, width], width at most TREE_NODES) and ``accepted`` (int32 [S]) are what ``verify_tree`` leaves: row seq_start_row[s] + nodes[s, j] becomes
     row seq_start_row[s] + j for j = 1 .. accepted[s] (no further than nodes has; none where it is below 1).  Rows behind those hold what is left.  Nodes that
     do not go up are reported (``check_kernel_status``) and end their request's moves, and so are rows without a page, which do not move."""

@@ -205,3 +205,45 @@ def test_texts_beyond_their_tables(ops, workspace, dtype, window, nodes):
         step.compare(out, ref, plain.attention_tolerance(dtype, ref, mag, size, most[1], 64))
         assert not window or (out[:5] == 0).all()
         assert window or (out[:5] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("heads, kv_heads, D, most_nodes", [(14, 2, 64, 5), (8, 2, 128, 20), (14, 2, 64, 40)])
+def test_a_recorded_step_of_a_padded_batch(ops, dtype, heads, kv_heads, D, most_nodes):
+    """Recorded once for the most requests, nodes and rows, and replayed with fewer: requests without nodes, query rows that nobody brings.  (5 nodes are 35 query rows
+    of a kv head, 20 are 80, 40 are 280.)"""
+    from ferrisinfer_b200.engine.workspace import Workspace
+
+    S, ps, most_rows = 6, 16, 640
+    T, width, pages = S * most_nodes, most_rows // ps, S * most_rows // ps + 1
+    there = {"q": torch.zeros(T, heads * D, dtype=dtype, device=DEV), "out": torch.zeros(T, heads * D, dtype=dtype, device=DEV),
+             "k": torch.zeros(pages, kv_heads, ps, D, dtype=dtype, device=DEV), "v": torch.zeros(pages, kv_heads, ps, D, dtype=dtype, device=DEV)}
+    indices = [torch.full((S, width), -1, dtype=torch.int32, device=DEV), ints([0] * (S + 1)), ints([0] * S), ints([-1] * T)]
+    workspace = Workspace(DEV)
+    call = lambda: ops.tree_attention(there["q"], there["out"], there["k"], there["v"], *indices, most_nodes, most_rows, heads, D ** -0.5, workspace=workspace)
+    call()
+    workspace.pin()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    batches = [([0] * 6, [0] * 6), ([most_nodes] * 6, [600] * 6), ([0, 1, 0, most_nodes, 2, 0], [9, 0, 600, 17, 599, 600]), ([1] * 6, [600, 0, 1, 128, 127, 300]),
+               ([0, 0, 0, 0, 0, most_nodes], [600] * 6), ([3, most_nodes, 0, 0, 0, 0], [1, 400, 0, 0, 0, 0])]
+    for nodes, starts in batches:
+        n = sum(nodes)
+        if n:
+            step = Step(dtype, heads, kv_heads, D, ps, nodes, starts)
+            for t, values in ((there["k"], step.k), (there["v"], step.v)):
+                t.fill_(math.nan)
+                t[:len(values)] = values
+            there["q"].fill_(math.nan)
+            there["q"][:n] = step.q
+            indices[0].fill_(-1)
+            indices[0][:, :len(step.tables[0])] = ints(step.tables)
+            indices[2].copy_(ints(starts)), indices[3][:n].copy_(ints(step.parents))
+        indices[1].copy_(ints([sum(nodes[:i]) for i in range(S + 1)]))
+        there["out"].fill_(7.0)
+        graph.replay()
+        if n:
+            step.check(there["out"][:n])
+        assert (there["out"][n:] == 7).all()

@@ -181,7 +181,7 @@ def test_attention_without_any_cached_row_is_refused(ops, workspace):
     step.run(ops, workspace)
     tables, *others = step.device_tensors
     out = torch.full((5, 256), 7.0, dtype=torch.bfloat16, device=DEV)
-    call = lambda k, tables, most, S=2: ops.tree_attention(step.q, out, k, k, tables, *others, *most, 4, 0.125, workspace=workspace)
+    call = lambda k, tables, most: ops.tree_attention(step.q, out, k, k, tables, *others, *most, 4, 0.125, workspace=workspace)
     for k, t, most in ((step.k, tables, (3, 0)), (step.k[:0], tables, (3, 40)), (step.k, tables[:, :0].contiguous(), (3, 40))):
         with pytest.raises(KernelError, match="no rows"):
             call(k, t, most)

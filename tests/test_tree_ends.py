@@ -1,18 +1,8 @@
 """Rules that the CUDA sources keep about what is still on its way when a block ends, read from their text, without a GPU."""
 
-import os
 import re
 
-import pytest
-
-from test_kernel_sources import CSRC, block_after, kernels_with
-
-
-def sources():
-    for name in sorted(os.listdir(CSRC)):
-        if name.endswith((".cu", ".cuh")):
-            with open(os.path.join(CSRC, name)) as f:
-                yield name, re.sub(r"//[^\n]*|/\*.*?\*/", "", f.read(), flags=re.S)
+from test_kernel_sources import block_after, kernels_with
 
 
 def tree_kernel():
